@@ -1,0 +1,49 @@
+/*
+ * policy_common.h - what the kernels of include/b3_policy.h share: element
+ * types, loads of vectors with the alignment of their elements, and
+ * reductions over a wave and a workgroup in a fixed order.
+ */
+#ifndef PUFFYSICS_AMD_POLICY_COMMON_H
+#define PUFFYSICS_AMD_POLICY_COMMON_H
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "b3_policy.h"
+
+namespace b3p {
+
+constexpr int kWave = 64;
+
+template <int TYPE>
+struct Element;
+template <>
+struct Element<B3_F32> {
+    using type = float;
+};
+template <>
+struct Element<B3_F16> {
+    using type = _Float16;
+};
+template <>
+struct Element<B3_BF16> {
+    using type = __bf16;
+};
+
+/* N elements that lie anywhere their type may: the hardware takes wide
+ * global loads and stores at any such address. */
+template <typename T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) Pack {
+    T v[N];
+};
+
+inline __device__ float to_float(float x) { return x; }
+inline __device__ float to_float(_Float16 x) { return (float)x; }
+inline __device__ float to_float(__bf16 x) { return (float)x; }
+
+inline bool is_float_type(int type) { return type == B3_F32 || type == B3_F16 || type == B3_BF16; }
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+}  // namespace b3p
+#endif

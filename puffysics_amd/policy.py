@@ -1,0 +1,396 @@
+"""What a policy's update needs next to the environments' step
+(include/b3_policy.h): `advantages` of a rollout, `log_probs` of the taken
+actions with entropies, best alternatives and the gradient, and `AdamW`.
+
+The arrays are torch CUDA tensors; the work is enqueued on the current torch
+stream and runs in libb3policy.so.  Arguments that do not fit raise
+ValueError before anything is launched; an error of a call raises B3Error.
+The reference leaves these to the trainer (docs/RL_LIBRARY.md).
+"""
+import collections
+import ctypes as C
+import os
+
+import torch
+
+from . import _native
+from .engine import B3Error
+
+POLICY_PATH = os.path.join(_native.HERE, "libb3policy.so")
+MAX_TOP = 32
+SEGMENT = 256
+
+_F32, _F16, _BF16, _U8 = 0, 1, 2, 3
+_TYPE = {torch.float32: _F32, torch.float16: _F16, torch.bfloat16: _BF16}
+_vp, _i, _ll, _d, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_double, C.c_size_t
+
+
+class B3Logits(C.Structure):
+    _fields_ = [("data", _vp), ("type", _i), ("rows", _ll), ("actions", _ll), ("row_stride", _ll), ("mask", _vp),
+                ("mask_row_stride", _ll)]
+
+
+class B3Rollout(C.Structure):
+    _fields_ = [("steps", _ll), ("envs", _ll), ("rewards", _vp), ("rewards_stride", _ll * 2), ("values", _vp),
+                ("values_type", _i), ("values_stride", _ll * 2), ("last_values", _vp), ("last_values_stride", _ll),
+                ("terminals", _vp), ("terminals_type", _i), ("terminals_stride", _ll * 2), ("advantages", _vp),
+                ("returns", _vp), ("out_stride", _ll * 2)]
+
+
+class B3AdamWTensor(C.Structure):
+    _fields_ = [("param", _vp), ("type", _i), ("numel", _ll), ("weight_decay", _d)]
+
+
+class B3AdamWState(C.Structure):
+    _fields_ = [("bits", _i), ("exp_avg", _vp), ("exp_avg_sq", _vp), ("exp_avg_scale", _vp),
+                ("exp_avg_sq_scale", _vp), ("master", _vp)]
+
+
+class B3AdamWConfig(C.Structure):
+    _fields_ = [("beta1", _d), ("beta2", _d), ("eps", _d), ("seed", C.c_uint32)]
+
+
+POLICY_SYMBOLS = [
+    ("b3_log_probs_workspace", _sz, [_ll, _ll, _i]),
+    ("b3_log_probs_gpu", _i, [B3Logits, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _sz, _vp]),
+    ("b3_log_probs_backward_gpu", _i, [B3Logits, _vp, _vp, _vp, _vp, _ll, _vp, _ll, _vp, _ll, _vp]),
+    ("b3_advantages_workspace", _sz, [_ll, _ll]),
+    ("b3_advantages_gpu", _i, [C.POINTER(B3Rollout), _d, _d, _vp, _sz, _vp]),
+    ("b3_adamw_size", _ll, [C.POINTER(B3AdamWTensor), _i]),
+    ("b3_adamw_create", _i, [C.POINTER(_vp), C.POINTER(B3AdamWTensor), _i, B3AdamWState, B3AdamWConfig]),
+    ("b3_adamw_step_gpu", _i, [_vp, _vp, _vp, _d, _d, _vp, _vp]),
+    ("b3_adamw_steps", _ll, [_vp, _i]),
+    ("b3_adamw_set_steps", _i, [_vp, _i, _ll]),
+    ("b3_adamw_moments_gpu", _i, [_vp, _vp, _vp, _vp]),
+    ("b3_adamw_load_moments_gpu", _i, [_vp, _vp, _vp, _vp]),
+    ("b3_adamw_destroy", _i, [_vp]),
+]
+
+_lib = None
+
+
+def policy_lib():
+    """libb3policy.so, loaded once; raises if it has not been built."""
+    global _lib
+    if _lib is None:
+        if not os.path.exists(POLICY_PATH):
+            raise RuntimeError("%s is missing: run __graft_entry__.build()" % POLICY_PATH)
+        _native._torch_runtime_first()
+        lib = C.CDLL(POLICY_PATH)
+        for name, res, args in POLICY_SYMBOLS:
+            fn = getattr(lib, name)
+            fn.restype = res
+            fn.argtypes = args
+        _lib = lib
+    return _lib
+
+
+def _check(name, code):
+    if code != 0:
+        raise B3Error(name, code)
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _on(*tensors):
+    """Raise unless all are on the current device, where the work runs."""
+    device = None
+    for t in tensors:
+        if t is None:
+            continue
+        if device is None and t.is_cuda:
+            device = torch.cuda.current_device()
+        _need(t.is_cuda and t.get_device() == device, "tensors have to be on the current CUDA device")
+
+
+# ---- log probabilities ----
+
+LogProbs = collections.namedtuple("LogProbs", "log_prob entropy top_log_prob top_action")
+
+
+def _logits(x, mask):
+    """B3Logits of x [rows, actions] and a mask [rows or 1, actions]."""
+    rows, actions = x.shape
+    # the stride of a lone row says nothing
+    stride = x.stride(0) if rows > 1 else actions
+    if mask is None:
+        return B3Logits(x.data_ptr(), _TYPE[x.dtype], rows, actions, stride, None, 0)
+    mask_stride = 0 if mask.shape[0] == 1 else mask.stride(0)
+    return B3Logits(x.data_ptr(), _TYPE[x.dtype], rows, actions, stride, mask.data_ptr(), mask_stride)
+
+
+def _rows(x):
+    """x, or a copy of it, with contiguous rows that do not overlap."""
+    if x.stride(1) == 1 and (x.shape[0] == 1 or x.stride(0) >= x.shape[1]):
+        return x
+    return x.contiguous()
+
+
+class _LogProbs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, taken, mask, top):
+        rows, actions = x.shape
+        lib = policy_lib()
+        x = _rows(x)
+        kept = ctx.needs_input_grad[0]
+        log_prob = torch.empty(rows, dtype=torch.float32, device=x.device)
+        entropy = torch.empty_like(log_prob)
+        stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if kept else None
+        top_lp = top_action = None
+        if top:
+            top_lp = torch.empty((rows, top), dtype=torch.float32, device=x.device)
+            top_action = torch.empty((rows, top), dtype=torch.int64, device=x.device)
+        size = lib.b3_log_probs_workspace(rows, actions, top)
+        work = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+        _check("b3_log_probs_gpu", lib.b3_log_probs_gpu(
+            _logits(x, mask), taken.data_ptr(), log_prob.data_ptr(), entropy.data_ptr(),
+            stats.data_ptr() if kept else None, top, top_lp.data_ptr() if top else None,
+            top_action.data_ptr() if top else None,
+            work.data_ptr() if size else None, size, _stream()))
+        if kept:
+            ctx.save_for_backward(x, taken, mask, stats, entropy)
+            ctx.set_materialize_grads(False)
+        if top:
+            ctx.mark_non_differentiable(top_lp, top_action)
+        return log_prob, entropy, top_lp, top_action
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_log_prob, d_entropy, *_):
+        x, taken, mask, stats, entropy = ctx.saved_tensors
+        d = torch.empty_like(x, memory_format=torch.contiguous_format)
+        _check("b3_log_probs_backward_gpu", policy_lib().b3_log_probs_backward_gpu(
+            _logits(x, mask), taken.data_ptr(), stats.data_ptr(), entropy.data_ptr(), *_upstream(d_log_prob),
+            *_upstream(d_entropy), d.data_ptr(), x.shape[1], _stream()))
+        return d, None, None, None
+
+
+def _upstream(d):
+    """Pointer and stride of a gradient [rows] (None: zero)."""
+    return (None, 0) if d is None else (d.data_ptr(), d.stride(0))
+
+
+def log_probs(logits, taken, mask=None, top=0):
+    """Log probabilities of the actions `taken` under `logits`, as
+    LogProbs(log_prob, entropy, top_log_prob, top_action).
+
+    logits  [..., actions], float32, float16 or bfloat16
+    taken   [...] whole numbers; below 0 for padding, whose log_prob is 0
+    mask    None or bool, [..., actions] or [actions]: the allowed actions
+    top     how many of each row's best actions to return (at most 32), by
+            descending log probability, the lowest action first among equals
+
+    log_prob and entropy are float32 [...] and differentiable in the logits;
+    top_log_prob and top_action are [..., top], or None without `top`.  A row
+    that allows nothing has log_prob -inf, entropy 0 and no gradient; an
+    action past the last has log_prob NaN."""
+    _need(logits.dtype in _TYPE, "logits have to be float32, float16 or bfloat16")
+    _need(logits.dim() >= 1 and logits.shape[-1] >= 1, "logits need at least one action")
+    _need(not taken.is_floating_point() and taken.dtype != torch.bool, "taken has to be whole numbers")
+    _need(taken.shape == logits.shape[:-1], "taken has to have the shape of logits without the last axis")
+    _need(0 <= top <= min(MAX_TOP, logits.shape[-1]), "top has to be between 0 and %d, and at most the actions" % MAX_TOP)
+    _on(logits, taken, mask)
+    actions = logits.shape[-1]
+    if mask is not None:
+        _need(mask.dtype == torch.bool, "mask has to be bool")
+        _need(mask.shape == logits.shape or mask.shape == (actions,),
+              "mask has to have the shape of logits, or of one row")
+        mask = _rows(mask.reshape(-1, actions))
+    shape = taken.shape
+    if len(shape) != 1:
+        logits, taken = logits.reshape(-1, actions), taken.reshape(-1)
+    taken = taken.to(torch.int64).contiguous()
+    log_prob, entropy, top_lp, top_action = _LogProbs.apply(logits, taken, mask, top)
+    if len(shape) != 1:
+        log_prob, entropy = log_prob.reshape(shape), entropy.reshape(shape)
+        if top:
+            top_lp, top_action = top_lp.reshape(*shape, top), top_action.reshape(*shape, top)
+    return LogProbs(log_prob, entropy, top_lp, top_action)
+
+
+# ---- advantages ----
+
+def advantages(rewards, values, terminals, last_values, gamma=0.99, lam=0.95):
+    """(advantages, returns) of a rollout, both float32 and laid out like the
+    rewards: A_t = r_t + gamma V_{t+1} - V_t + gamma lam A_{t+1}, where a
+    terminal at t drops what lies after it, and R_t = A_t + V_t.
+
+    rewards      [steps, envs] float32
+    values       [steps, envs] float32, float16 or bfloat16: before each step
+    terminals    [steps, envs] float32, bool or uint8: nonzero where the step
+                 ended an episode (HoverEnvs.terminals)
+    last_values  [envs], of values' type: after the last step
+
+    Any strides; the result has no gradient."""
+    _need(rewards.dim() == 2 and rewards.dtype == torch.float32, "rewards have to be float32 [steps, envs]")
+    _need(values.shape == rewards.shape and terminals.shape == rewards.shape,
+          "values and terminals have to have the shape of rewards")
+    _need(values.dtype in _TYPE, "values have to be float32, float16 or bfloat16")
+    _need(last_values.shape == rewards.shape[1:] and last_values.dtype == values.dtype,
+          "last_values have to be [envs], of the type of values")
+    _need(terminals.dtype in (torch.float32, torch.bool, torch.uint8), "terminals have to be float32, bool or uint8")
+    _need(0 <= gamma <= 1 and 0 <= lam <= 1, "gamma and lam have to be between 0 and 1")
+    _on(rewards, values, terminals, last_values)
+    lib = policy_lib()
+    steps, envs = rewards.shape
+    # the longer stride is the outer axis: (steps, envs) unless the rewards are a transposed array
+    turned = rewards.stride(0) < rewards.stride(1)
+    out = torch.empty((2, envs, steps) if turned else (2, steps, envs), dtype=torch.float32, device=rewards.device)
+    adv, ret = (out[0].t(), out[1].t()) if turned else (out[0], out[1])
+    pair = _ll * 2
+    g = B3Rollout(steps, envs, rewards.data_ptr(), pair(*rewards.stride()), values.data_ptr(), _TYPE[values.dtype],
+                  pair(*values.stride()), last_values.data_ptr(), last_values.stride(0), terminals.data_ptr(),
+                  _F32 if terminals.dtype == torch.float32 else _U8, pair(*terminals.stride()), adv.data_ptr(),
+                  ret.data_ptr(), pair(*adv.stride()))
+    size = lib.b3_advantages_workspace(steps, envs)
+    work = torch.empty(size, dtype=torch.uint8, device=rewards.device) if size else None
+    _check("b3_advantages_gpu", lib.b3_advantages_gpu(C.byref(g), gamma, lam, work.data_ptr() if size else None, size,
+                                                      _stream()))
+    return adv, ret
+
+
+# ---- AdamW ----
+
+class AdamW:
+    """AdamW over all of `params` in one step: contiguous float32, float16 or
+    bfloat16 tensors on the current device.
+
+    state_bits     32, or 8: moments as e4m3 numbers (the first, and the root
+                   of the second) with a power of two for every 32 of them,
+                   rounded by random bits that `seed`, step and place give
+    max_grad_norm  the global norm that gradients are scaled down to, or None
+    weight_decay   a number, or one for each tensor
+    master         keep 32-bit copies of 16-bit weights and round those; without
+                   them small updates of such weights are lost
+
+    The moments lie in flat arrays, tensor i's from offsets[i] on."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32,
+                 max_grad_norm=None, master=True, seed=0):
+        self._h = _vp()
+        self.params = list(params)
+        n = len(self.params)
+        decay = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * n
+        for p in self.params:
+            _need(p.dtype in _TYPE, "parameters have to be float32, float16 or bfloat16")
+            _need(p.is_contiguous(), "parameters have to be contiguous")
+        _on(*self.params)
+        _need(len({p.data_ptr() for p in self.params if p.numel()}) == sum(p.numel() > 0 for p in self.params),
+              "a parameter is given twice")
+        _need(len(decay) == n and all(d >= 0 for d in decay), "weight_decay has to be at least 0, one for each tensor")
+        _need(0 <= betas[0] < 1 and 0 <= betas[1] < 1 and eps >= 0, "betas have to be in [0, 1), eps at least 0")
+        _need(state_bits in (8, 32), "state_bits has to be 8 or 32")
+        self.lr, self.max_grad_norm, self.state_bits = lr, max_grad_norm, state_bits
+        self.device = torch.device("cuda", torch.cuda.current_device())
+        self._lib = policy_lib()
+        table = (B3AdamWTensor * max(n, 1))(*[B3AdamWTensor(p.data_ptr(), _TYPE[p.dtype], p.numel(), d)
+                                              for p, d in zip(self.params, decay)])
+        self.size = self._lib.b3_adamw_size(table, n)
+        self.offsets, at = [], 0
+        for p in self.params:
+            self.offsets.append(at)
+            at += -(-p.numel() // SEGMENT) * SEGMENT
+        assert at == self.size
+        kind = torch.float32 if state_bits == 32 else torch.uint8
+        new = lambda count, dtype: torch.zeros(count, dtype=dtype, device=self.device)  # noqa: E731
+        self._exp_avg, self._exp_avg_sq = new(self.size, kind), new(self.size, kind)
+        scales = self.size // 32 if state_bits == 8 else 0
+        self._scale = new((2, scales), torch.uint8).fill_(1)
+        self._master = None
+        if master and any(p.dtype != torch.float32 for p in self.params):
+            self._master = new(self.size, torch.float32)
+            for p, m in zip(self.params, self._views(self._master)):
+                m.copy_(p.detach())
+        state = B3AdamWState(state_bits, self._exp_avg.data_ptr(), self._exp_avg_sq.data_ptr(),
+                             self._scale[0].data_ptr(), self._scale[1].data_ptr(),
+                             self._master.data_ptr() if self._master is not None else None)
+        self._grads, self._types = (_vp * max(n, 1))(), (_i * max(n, 1))()
+        torch.cuda.current_stream().synchronize()     # the state is ready for a step on any stream
+        _check("b3_adamw_create", self._lib.b3_adamw_create(C.byref(self._h), table, n, state,
+                                                            B3AdamWConfig(betas[0], betas[1], eps, seed)))
+
+    def _views(self, flat):
+        return [flat[at:at + p.numel()].view(p.shape) for at, p in zip(self.offsets, self.params)]
+
+    def step(self, grads=None, lr=None):
+        """One step by `grads` (one for each parameter, of its type or
+        float32, None to leave it out), or by the parameters' own `.grad`.
+        Returns the gradients' norm before the clip as a tensor, or None
+        without max_grad_norm."""
+        if grads is None:
+            grads = [p.grad for p in self.params]
+        _need(len(grads) == len(self.params), "need one gradient for each parameter")
+        _on(*grads)
+        for i, (p, g) in enumerate(zip(self.params, grads)):
+            if g is None:
+                self._grads[i] = None
+                continue
+            _need(g.shape == p.shape and g.is_contiguous(), "gradients have to be contiguous, of the parameters' shapes")
+            _need(g.dtype == p.dtype or g.dtype == torch.float32, "gradients have to be of the parameters' type or float32")
+            self._grads[i], self._types[i] = g.data_ptr(), _TYPE[g.dtype]
+        norm = torch.empty((), dtype=torch.float32, device=self.device) if self.max_grad_norm else None
+        _check("b3_adamw_step_gpu", self._lib.b3_adamw_step_gpu(
+            self._h, self._grads, self._types, self.lr if lr is None else lr, self.max_grad_norm or 0.0,
+            norm.data_ptr() if norm is not None else None, _stream()))
+        return norm
+
+    def moments(self):
+        """The flat arrays (exp_avg, exp_avg_sq): the state's own in 32 bits,
+        in 8 bits the values it stands for as new bfloat16 arrays, which hold
+        them exactly."""
+        if self.state_bits == 32:
+            return self._exp_avg, self._exp_avg_sq
+        out = torch.empty((2, self.size), dtype=torch.bfloat16, device=self.device)
+        _check("b3_adamw_moments_gpu", self._lib.b3_adamw_moments_gpu(self._h, out[0].data_ptr(), out[1].data_ptr(),
+                                                                      _stream()))
+        return out[0], out[1]
+
+    def master(self):
+        """The flat array of 32-bit copies of 16-bit weights, or None."""
+        return self._master
+
+    def steps(self, i=0):
+        """Steps that parameter i has taken."""
+        return self._lib.b3_adamw_steps(self._h, i)
+
+    def load_moments(self, exp_avg, exp_avg_sq, step, master=None):
+        """Go on from moments (lists of a tensor for each parameter) after
+        `step` steps, and from 32-bit copies of the weights if given."""
+        n = len(self.params)
+        _need(len(exp_avg) == n and len(exp_avg_sq) == n and (master is None or len(master) == n),
+              "need one tensor for each parameter")
+        _need(step >= 0, "step has to be at least 0")
+        _need(master is None or self._master is not None, "this optimizer keeps no 32-bit copies")
+        flat = (self._exp_avg, self._exp_avg_sq) if self.state_bits == 32 else \
+            torch.zeros((2, self.size), dtype=torch.float32, device=self.device)
+        lists = [(flat[0], exp_avg), (flat[1], exp_avg_sq)] + ([(self._master, master)] if master is not None else [])
+        for to, given in lists:
+            for view, x in zip(self._views(to), given):
+                _need(x.shape == view.shape, "need tensors of the parameters' shapes")
+                view.copy_(x)
+        if self.state_bits == 8:
+            _check("b3_adamw_load_moments_gpu", self._lib.b3_adamw_load_moments_gpu(
+                self._h, flat[0].data_ptr(), flat[1].data_ptr(), _stream()))
+        for i in range(n):
+            _check("b3_adamw_set_steps", self._lib.b3_adamw_set_steps(self._h, i, step))
+
+    def close(self):
+        if self._h:
+            code = self._lib.b3_adamw_destroy(self._h)
+            self._h = _vp()
+            _check("b3_adamw_destroy", code)
+
+    def __del__(self):
+        try:
+            if getattr(self, "_h", None):
+                self._lib.b3_adamw_destroy(self._h)
+                self._h = _vp()
+        except Exception:
+            pass
