@@ -5,6 +5,20 @@
  * With m = max x, z = x - m and S = sum exp(z):
  *   log p_j = z_j - log S          H = log S - (sum z exp(z)) / S
  *   dx_j = dlp ([j = taken] - p_j) - dH p_j (log p_j + H)
+ *
+ * Both directions are bound by memory: the forward reads the logits once,
+ * the backward reads them once and writes as much.  A row, or a piece of one,
+ * is held in the registers of the threads that share it, so that the maximum
+ * comes before the sums with one read and no rescaling:
+ *   up to 1,024 actions   G lanes of a wave to a row, by a rule on the
+ *                         actions alone (with_small)
+ *   up to 16,384          a workgroup to a row
+ *   more                  a workgroup to a piece of 16,384, or of 4,096 where
+ *                         the larger ones would not fill the chip; the pieces'
+ *                         (m, S, sum z exp(z)) and best alternatives are
+ *                         joined by a wave per row
+ * A lane loads W neighbouring logits at once; lanes take turns, so the order
+ * of places is (load, lane, place in the load).
  */
 #include "policy_common.h"
 
@@ -12,6 +26,10 @@ namespace b3p {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kMaxActions = 1 << 22;
+constexpr int kMaxPieces = 256;
+constexpr float kLog2e = 1.44269504f;
 
 /* A logit, -inf where its action is not allowed. */
 template <typename T>
@@ -19,107 +37,550 @@ __device__ float logit(const T* row, const unsigned char* mask, int64_t j) {
     return mask && !mask[j] ? -INFINITY : to_float(row[j]);
 }
 
-/* Whole numbers in the order of the logits: NaN above +inf, -0 as 0; never 0
- * or 2^32 - 1, so that a key of order and action is neither all zeros nor all
- * ones. */
+template <typename T>
+__device__ const T* row_of(const B3Logits& g, int64_t r) {
+    return (const T*)g.data + r * g.row_stride;
+}
+
+__device__ const unsigned char* mask_of(const B3Logits& g, int64_t r) {
+    return g.mask ? g.mask + r * g.mask_row_stride : NULL;
+}
+
+/* The logits of a thread: places from + (v G + lane) W + w below `n`; -inf in
+ * the others. */
+template <typename T, int G, int PER, int W>
+__device__ void load_logits(const T* row, const unsigned char* mask, int from, int n, int lane, float x[PER]) {
+#pragma unroll
+    for (int v = 0; v < PER / W; v++) {
+        const int j = from + (v * G + lane) * W;
+        if (j + W <= n) {
+            Pack<T, W> p = *(const Pack<T, W>*)(row + j);
+#pragma unroll
+            for (int w = 0; w < W; w++) x[v * W + w] = to_float(p.v[w]);
+            if (mask) {
+                Pack<unsigned char, W> k = *(const Pack<unsigned char, W>*)(mask + j);
+#pragma unroll
+                for (int w = 0; w < W; w++) x[v * W + w] = k.v[w] ? x[v * W + w] : -INFINITY;
+            }
+        } else {
+#pragma unroll
+            for (int w = 0; w < W; w++) x[v * W + w] = j + w < n ? logit(row, mask, j + w) : -INFINITY;
+        }
+    }
+}
+
+/* ---- reductions over the G threads that share a row ---- */
+
+template <int G, typename F>
+__device__ float reduce(float x, float* lds, F f) {
+#pragma unroll
+    for (int d = 1; d < (G < kWave ? G : kWave); d *= 2) x = f(x, __shfl_xor(x, d));
+    if (G > kWave) {
+        if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = x;
+        __syncthreads();
+        x = f(f(lds[0], lds[1]), f(lds[2], lds[3]));
+        __syncthreads();
+    }
+    return x;
+}
+
+/* m, S and D = sum z exp(z) of a row or a piece.  m is 0 where nothing is
+ * allowed, and where all that is allowed is NaN (S is then NaN). */
+struct Sums {
+    float m, s, d;
+};
+
+/* exp as 2^(z log2 e): the product is off by |z| 2^-24, and so is exp(z),
+ * relative to itself; terms with |z| > 20 do not count.  z is bounded in D
+ * alone, where 0 times -inf would be NaN. */
+template <int G, int PER>
+__device__ Sums sums_of(const float x[PER], float* lds) {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < PER; i++) m = fmaxf(m, x[i]);
+    m = reduce<G>(m, lds, [](float a, float b) { return fmaxf(a, b); });
+    m = m == -INFINITY || m != m ? 0.0f : m;
+    float s = 0, d = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        float z = x[i] - m, e = __builtin_amdgcn_exp2f(z * kLog2e);
+        s += e;
+        d = __builtin_fmaf(e, fmaxf(z, -1e4f), d);
+    }
+    auto add = [](float a, float b) { return a + b; };
+    s = reduce<G>(s, lds, add);
+    d = reduce<G>(d, lds, add);
+    return Sums{m, s, d};
+}
+
+struct Outputs {
+    const int64_t* taken;
+    float* log_prob;
+    float* entropy;
+    float* stats;
+    int top;
+    float* top_log_prob;
+    int64_t* top_action;
+};
+
+/* What one thread of a row writes. */
+template <typename T>
+__device__ void finish_row(const B3Logits& g, const Outputs& o, int64_t r, Sums s, float log_sum) {
+    const int64_t a = o.taken[r];
+    const bool empty = s.s == 0.0f;
+    float lp = 0.0f;
+    if (a >= g.actions)
+        lp = NAN;
+    else if (a >= 0)
+        lp = empty ? -INFINITY : logit(row_of<T>(g, r), mask_of(g, r), a) - s.m - log_sum;
+    o.log_prob[r] = lp;
+    o.entropy[r] = empty ? 0.0f : log_sum - s.d / s.s;
+    if (o.stats) {
+        o.stats[2 * r] = s.m;
+        o.stats[2 * r + 1] = log_sum;
+    }
+}
+
+/* ---- best alternatives ---- */
+
+/* Whole numbers in the order of the logits: NaN above +inf, -0 as 0; never 0,
+ * which stands for one that has been taken out. */
 __device__ uint32_t order_of(float x) {
     if (x != x) return 0xfffffffeu;
     uint32_t b = __float_as_uint(x + 0.0f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-template <typename V, typename F>
-__device__ V block_reduce(V v, V* lds, F f) {
-    lds[threadIdx.x] = v;
-    __syncthreads();
-    for (int half = kThreads / 2; half > 0; half /= 2) {
-        if ((int)threadIdx.x < half) lds[threadIdx.x] = f(lds[threadIdx.x], lds[threadIdx.x + half]);
-        __syncthreads();
-    }
-    v = lds[0];
-    __syncthreads();
-    return v;
+__device__ float value_of(uint32_t order) {
+    return __uint_as_float(order & 0x80000000u ? order ^ 0x80000000u : ~order);
 }
 
-template <int TYPE>
-__global__ __launch_bounds__(kThreads) void lp_rows(B3Logits g, const int64_t* taken, float* log_prob, float* entropy,
-    float* stats, int top, float* top_log_prob, int64_t* top_action) {
-    using T = typename Element<TYPE>::type;
-    __shared__ float lds[kThreads];
-    __shared__ uint64_t keys[kThreads];
+__device__ void write_top(const Outputs& o, int64_t r, int k, uint32_t order, int64_t action, Sums s, float log_sum) {
+    o.top_log_prob[r * o.top + k] = s.s == 0.0f ? -INFINITY : value_of(order) - s.m - log_sum;
+    o.top_action[r * o.top + k] = action;
+}
+
+__device__ uint32_t wave_max(uint32_t x) {
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        uint32_t y = __shfl_xor(x, d);
+        x = x > y ? x : y;
+    }
+    return x;
+}
+
+/* The `top` largest of the wave's NV loads of W orders, one after the other:
+ * lane k gets the k-th's order and place (load, lane, place in the load).
+ * Among equals the lowest place is taken: the first load that any lane has it
+ * in, the first such lane, its first place.  Every round takes one of at
+ * least `top` orders that are not 0, or finds 0 and gives it. */
+template <int NV, int W>
+__device__ void wave_top(uint32_t order[NV * W], int top, uint32_t& my_order, int& my_load, int& my_lane, int& my_place) {
+    const int lane = threadIdx.x % kWave;
+    uint32_t best[NV];
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+        best[v] = order[v * W];
+#pragma unroll
+        for (int w = 1; w < W; w++) best[v] = best[v] > order[v * W + w] ? best[v] : order[v * W + w];
+    }
+    my_order = 0;
+    my_load = my_lane = my_place = 0;
+    for (int k = 0; k < top; k++) {
+        uint32_t most = best[0];
+#pragma unroll
+        for (int v = 1; v < NV; v++) most = most > best[v] ? most : best[v];
+        most = wave_max(most);
+        bool found = false;
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            const uint64_t have = __ballot(best[v] == most);
+            if (!found && have) {
+                found = true;
+                const int who = __builtin_ctzll(have);
+                int place = W - 1;
+#pragma unroll
+                for (int w = W - 2; w >= 0; w--) place = order[v * W + w] == most ? w : place;
+                place = __builtin_amdgcn_readlane(place, who);
+                uint32_t b = 0;
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    if (w == place && lane == who) order[v * W + w] = 0;
+                    b = b > order[v * W + w] ? b : order[v * W + w];
+                }
+                best[v] = b;
+                if (lane == k) {
+                    my_order = most;
+                    my_load = v;
+                    my_lane = who;
+                    my_place = place;
+                }
+            }
+        }
+    }
+}
+
+/* The same for G < 64 lanes to a row: each round the largest key of order and
+ * place below the last. */
+template <int G, int PER, int W>
+__device__ void group_top(const float x[PER], int n, const Outputs& o, int64_t r, Sums s, float log_sum) {
+    const int lane = threadIdx.x % G;
+    uint64_t last = ~0ull;
+    for (int k = 0; k < o.top; k++) {
+        uint64_t best = 0;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int j = ((i / W) * G + lane) * W + i % W;
+            uint64_t key = (uint64_t)order_of(x[i]) << 32 | (uint32_t)~j;
+            if (j < n && key < last && key > best) best = key;
+        }
+#pragma unroll
+        for (int d = 1; d < G; d *= 2) {
+            uint64_t other = __shfl_xor(best, d);
+            best = best > other ? best : other;
+        }
+        last = best;
+        if (lane == 0) write_top(o, r, k, (uint32_t)(best >> 32), (uint32_t)~(uint32_t)best, s, log_sum);
+    }
+}
+
+/* ---- forward ---- */
+
+/* G lanes to a row: up to G PER actions. */
+template <typename T, int G, int PER, int W>
+__global__ __launch_bounds__(kThreads) void lp_small(B3Logits g, Outputs o) {
+    const int64_t r = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / G;
+    if (r >= g.rows) return;                     // all G lanes of it
+    const int lane = threadIdx.x % G, n = (int)g.actions;
+    float x[PER];
+    load_logits<T, G, PER, W>(row_of<T>(g, r), mask_of(g, r), 0, n, lane, x);
+    const Sums s = sums_of<G, PER>(x, NULL);
+    const float log_sum = logf(s.s);
+    if (lane == 0) finish_row<T>(g, o, r, s, log_sum);
+    if (!o.top) return;
+    if (G == kWave) {
+        uint32_t order[PER], my_order;
+        int v, l, w;
+#pragma unroll
+        for (int i = 0; i < PER; i++) order[i] = ((i / W) * G + lane) * W + i % W < n ? order_of(x[i]) : 0;
+        wave_top<PER / W, W>(order, o.top, my_order, v, l, w);
+        if (lane < o.top) write_top(o, r, lane, my_order, (v * G + l) * W + w, s, log_sum);
+    } else {
+        group_top<G, PER, W>(x, n, o, r, s, log_sum);
+    }
+}
+
+/* A piece's sums and alternatives, in the caller's workspace. */
+struct Pieces {
+    int count, size;                             // pieces of a row, actions of a piece
+    Sums* sums;                                  // [rows][count]
+    uint2* top;                                  // [rows][count][top]: order, action
+};
+
+/* A workgroup to a row (one piece) or to a piece of it.  TOP: whether
+ * alternatives are asked for (what they take of registers would halve the
+ * waves of a call that does not). */
+template <typename T, int PER, int W, bool TOP>
+__global__ __launch_bounds__(kThreads) void lp_piece(B3Logits g, Outputs o, Pieces p) {
+    __shared__ float lds[kWaves];
+    __shared__ uint2 found[kWaves][B3_MAX_TOP];
+    const int64_t r = blockIdx.x / (unsigned)p.count;
+    const int piece = blockIdx.x % (unsigned)p.count;
+    const int from = piece * p.size, end = from + p.size, n = end < g.actions ? end : (int)g.actions;
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    float x[PER];
+    load_logits<T, kThreads, PER, W>(row_of<T>(g, r), mask_of(g, r), from, n, threadIdx.x, x);
+    const Sums s = sums_of<kThreads, PER>(x, lds);
+    const float log_sum = logf(s.s);
+    if (threadIdx.x == 0) {
+        if (p.count == 1)
+            finish_row<T>(g, o, r, s, log_sum);
+        else
+            p.sums[r * p.count + piece] = s;
+    }
+    if (!TOP) return;
+    uint32_t order[PER], my_order;
+    int v, l, w;
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+        order[i] = from + ((i / W) * kThreads + (int)threadIdx.x) * W + i % W < n ? order_of(x[i]) : 0;
+    wave_top<PER / W, W>(order, o.top, my_order, v, l, w);
+    /* a wave of a short piece may have fewer than `top`: order 0 */
+    if (lane < o.top)
+        found[wave][lane] = make_uint2(my_order, from + (v * kThreads + wave * kWave + l) * W + w);
+    __syncthreads();
+    /* an alternative's place among the waves' is the number of larger ones */
+    for (int i = threadIdx.x; i < kWaves * o.top; i += kThreads) {
+        const uint2 mine = found[i / o.top][i % o.top];
+        if (mine.x == 0) continue;
+        int rank = i % o.top;
+        for (int u = 0; u < kWaves; u++) {
+            if (u == i / o.top) continue;
+            for (int k = 0; k < o.top; k++) {
+                const uint2 it = found[u][k];
+                rank += it.x > mine.x || (it.x == mine.x && it.y < mine.y);
+            }
+        }
+        if (rank >= o.top) continue;
+        if (p.count == 1)
+            write_top(o, r, rank, mine.x, mine.y, s, log_sum);
+        else
+            p.top[(r * p.count + piece) * o.top + rank] = mine;
+    }
+    /* a piece of fewer than `top` actions fills its list up */
+    const int have = n - from;
+    if (p.count > 1 && (int)threadIdx.x < o.top && (int)threadIdx.x >= have)
+        p.top[(r * p.count + piece) * o.top + threadIdx.x] = make_uint2(0, 0);
+}
+
+/* A wave to a row: up to 256 pieces, four to a lane. */
+template <typename T>
+__global__ __launch_bounds__(kWave) void lp_join(B3Logits g, Outputs o, Pieces p) {
+    constexpr int kHeads = kMaxPieces / kWave;
+    extern __shared__ uint2 lists[];             // [count][top]
     const int64_t r = blockIdx.x;
-    const T* row = (const T*)g.data + r * g.row_stride;
-    const unsigned char* mask = g.mask ? g.mask + r * g.mask_row_stride : NULL;
-    float most = -INFINITY;
-    for (int64_t j = threadIdx.x; j < g.actions; j += kThreads) most = fmaxf(most, logit(row, mask, j));
-    most = block_reduce(most, lds, [](float a, float b) { return fmaxf(a, b); });
-    const bool none = most == -INFINITY;
-    const float m = none ? 0.0f : most;
-    float sum = 0, dot = 0;
-    for (int64_t j = threadIdx.x; j < g.actions; j += kThreads) {
-        float z = logit(row, mask, j) - m, e = expf(z);
-        sum += e;
-        dot += e == 0.0f ? 0.0f : z * e;
+    const int lane = threadIdx.x;
+    Sums part[kHeads];
+    float m = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < kHeads; q++) {
+        const int c = q * kWave + lane;
+        part[q] = c < p.count ? p.sums[r * p.count + c] : Sums{0, 0, 0};
+        /* a piece that allows nothing has no say */
+        m = part[q].s == 0.0f ? m : fmaxf(m, part[q].m);
+    }
+    m = reduce<kWave>(m, NULL, [](float a, float b) { return fmaxf(a, b); });
+    m = m == -INFINITY ? 0.0f : m;
+    float s = 0, d = 0;
+#pragma unroll
+    for (int q = 0; q < kHeads; q++) {
+        if (part[q].s == 0.0f) continue;
+        const float z = part[q].m - m, e = __builtin_amdgcn_exp2f(z * kLog2e);
+        s += e * part[q].s;
+        d += e * (part[q].d + fmaxf(z, -1e4f) * part[q].s);
     }
     auto add = [](float a, float b) { return a + b; };
-    sum = block_reduce(sum, lds, add);
-    dot = block_reduce(dot, lds, add);
-    const float log_sum = logf(sum);
-    /* a row of NaN alone has no largest logit: its sum is NaN */
-    const bool empty = none && sum == 0.0f;
-    if (threadIdx.x == 0) {
-        int64_t a = taken[r];
-        float lp = a < 0 ? 0.0f : a >= g.actions ? NAN : empty ? -INFINITY : logit(row, mask, a) - m - log_sum;
-        log_prob[r] = lp;
-        entropy[r] = empty ? 0.0f : log_sum - dot / sum;
-        if (stats) {
-            stats[2 * r] = m;
-            stats[2 * r + 1] = log_sum;
-        }
+    const Sums all = {m, reduce<kWave>(s, NULL, add), reduce<kWave>(d, NULL, add)};
+    const float log_sum = logf(all.s);
+    if (lane == 0) finish_row<T>(g, o, r, all, log_sum);
+    if (!o.top) return;
+    /* the pieces' lists are sorted, and of equal orders the one of the lower
+     * piece has the lower action */
+    for (int i = lane; i < p.count * o.top; i += kWave) lists[i] = p.top[r * p.count * o.top + i];
+    __syncthreads();
+    uint2 head[kHeads];
+    int next[kHeads];
+#pragma unroll
+    for (int q = 0; q < kHeads; q++) {
+        const int c = q * kWave + lane;
+        head[q] = c < p.count ? lists[c * o.top] : make_uint2(0, 0);
+        next[q] = 1;
     }
-    uint64_t below = ~0ull;
-    for (int k = 0; k < top; k++) {
-        uint64_t best = 0;
-        for (int64_t j = threadIdx.x; j < g.actions; j += kThreads) {
-            uint64_t key = (uint64_t)order_of(logit(row, mask, j)) << 32 | (uint32_t)~j;
-            if (key < below && key > best) best = key;
-        }
-        best = block_reduce(best, keys, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
-        below = best;
-        if (threadIdx.x == 0) {
-            int64_t j = (uint32_t)~(uint32_t)best;
-            top_action[r * top + k] = j;
-            top_log_prob[r * top + k] = empty ? -INFINITY : logit(row, mask, j) - m - log_sum;
+    for (int k = 0; k < o.top; k++) {
+        uint32_t most = head[0].x;
+#pragma unroll
+        for (int q = 1; q < kHeads; q++) most = most > head[q].x ? most : head[q].x;
+        most = wave_max(most);
+        bool found = false;
+#pragma unroll
+        for (int q = 0; q < kHeads; q++) {
+            const uint64_t have = __ballot(head[q].x == most);
+            if (!found && have) {
+                found = true;
+                if (lane == __builtin_ctzll(have)) {
+                    write_top(o, r, k, most, head[q].y, all, log_sum);
+                    head[q] = next[q] < o.top ? lists[(q * kWave + lane) * o.top + next[q]] : make_uint2(0, 0);
+                    next[q]++;
+                }
+            }
         }
     }
 }
 
-template <int TYPE>
-__global__ __launch_bounds__(kThreads) void lp_backward(B3Logits g, const int64_t* taken, const float* stats,
-    const float* entropy, const float* d_log_prob, int64_t dl_stride, const float* d_entropy, int64_t dh_stride,
-    void* d_logits, int64_t d_row_stride) {
-    using T = typename Element<TYPE>::type;
-    const int64_t r = blockIdx.x;
-    const T* row = (const T*)g.data + r * g.row_stride;
-    const unsigned char* mask = g.mask ? g.mask + r * g.mask_row_stride : NULL;
-    T* out = (T*)d_logits + r * d_row_stride;
-    const int64_t a = taken[r];
-    const float m = stats[2 * r], log_sum = stats[2 * r + 1], h = entropy[r];
-    float dl = d_log_prob && a >= 0 ? d_log_prob[r * dl_stride] : 0.0f;
-    if (a >= g.actions) dl *= NAN;
-    const float dh = d_entropy ? d_entropy[r * dh_stride] : 0.0f;
-    const bool empty = log_sum == -INFINITY;
-    for (int64_t j = threadIdx.x; j < g.actions; j += kThreads) {
-        float x = logit(row, mask, j), lp = x - m - log_sum, p = expf(lp);
-        float d = (j == a ? dl : 0.0f) - p * (p == 0.0f ? 0.0f : dl + dh * (lp + h));
-        out[j] = (T)(empty || x == -INFINITY ? 0.0f : d);
+/* ---- backward ---- */
+
+/* What a row's gradient is made of. */
+struct Upstream {
+    const int64_t* taken;
+    const float* stats;
+    const float* entropy;
+    const float* d_log_prob;
+    int64_t d_log_prob_stride;
+    const float* d_entropy;
+    int64_t d_entropy_stride;
+    void* out;
+    int64_t row_stride;
+};
+
+struct RowGradient {
+    int64_t a;
+    float m, log_sum, h, dl, dh;
+    bool empty;
+};
+
+__device__ RowGradient row_gradient(const Upstream& u, int64_t r, int64_t actions) {
+    RowGradient q;
+    q.a = u.taken[r];
+    q.m = u.stats[2 * r];
+    q.log_sum = u.stats[2 * r + 1];
+    q.h = u.entropy[r];
+    q.dl = u.d_log_prob && q.a >= 0 ? u.d_log_prob[r * u.d_log_prob_stride] : 0.0f;
+    if (q.a >= actions) q.dl *= NAN;
+    q.dh = u.d_entropy ? u.d_entropy[r * u.d_entropy_stride] : 0.0f;
+    q.empty = q.log_sum == -INFINITY;
+    return q;
+}
+
+/* p log p is 0 where p is, also where log p is -inf. */
+__device__ float gradient_of(const RowGradient& q, float x, bool taken) {
+    const float lp = x - q.m - q.log_sum, p = __builtin_amdgcn_exp2f(lp * kLog2e);
+    const float d = (taken ? q.dl : 0.0f) - p * __builtin_fmaf(q.dh, fmaxf(lp, -1e4f) + q.h, q.dl);
+    return q.empty || x == -INFINITY ? 0.0f : d;
+}
+
+template <typename T, int G, int PER, int W>
+__device__ void backward_row(const B3Logits& g, const Upstream& u, int64_t r, int from, int lane) {
+    const RowGradient q = row_gradient(u, r, g.actions);
+    const int n = (int)g.actions;
+    float x[PER];
+    load_logits<T, G, PER, W>(row_of<T>(g, r), mask_of(g, r), from, n, lane, x);
+    T* out = (T*)u.out + r * u.row_stride;
+#pragma unroll
+    for (int v = 0; v < PER / W; v++) {
+        const int j = from + (v * G + lane) * W;
+        Pack<T, W> p;
+#pragma unroll
+        for (int w = 0; w < W; w++) p.v[w] = (T)gradient_of(q, x[v * W + w], j + w == q.a);
+        if (j + W <= n) {
+            *(Pack<T, W>*)(out + j) = p;
+        } else {
+#pragma unroll
+            for (int w = 0; w < W; w++)
+                if (j + w < n) out[j + w] = p.v[w];
+        }
     }
 }
 
+template <typename T, int G, int PER, int W>
+__global__ __launch_bounds__(kThreads) void lp_small_backward(B3Logits g, Upstream u) {
+    const int64_t r = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / G;
+    if (r < g.rows) backward_row<T, G, PER, W>(g, u, r, 0, threadIdx.x % G);
+}
+
+/* A workgroup to a piece of kThreads PER actions. */
+template <typename T, int PER, int W>
+__global__ __launch_bounds__(kThreads) void lp_piece_backward(B3Logits g, Upstream u, unsigned pieces) {
+    backward_row<T, kThreads, PER, W>(g, u, blockIdx.x / pieces, (int)(blockIdx.x % pieces) * (kThreads * PER),
+        threadIdx.x);
+}
+
+/* ---- launches ---- */
+
+/* Calls f with the shape for rows of up to 1,024 actions: the fewest lanes
+ * that hold them at four each (16 each beyond 256). */
+template <typename T, typename F>
+void with_small(int64_t actions, F f) {
+    if (actions <= 4)
+        f.template operator()<T, 1, 4, 4>();
+    else if (actions <= 16)
+        f.template operator()<T, 4, 4, 4>();
+    else if (actions <= 64)
+        f.template operator()<T, 16, 4, 4>();
+    else if (actions <= 256)
+        f.template operator()<T, 64, 4, 4>();
+    else
+        f.template operator()<T, 64, 16, 16 / sizeof(T)>();
+}
+
+constexpr int kSmall = 1024, kPiece = 16384, kShortPiece = 4096;
+constexpr int64_t kFill = 512;                   // workgroups: two to a compute unit
+
+template <typename F>
+void with_type(int type, F f) {
+    if (type == B3_F32)
+        f(float());
+    else if (type == B3_F16)
+        f((_Float16)0);
+    else
+        f((__bf16)0);
+}
+
+/* Pieces of a row: none of them in workspace where there is one. */
+Pieces pieces_of(int64_t rows, int64_t actions) {
+    Pieces p = {};
+    p.size = kPiece;
+    if (actions > kShortPiece && rows * ceil_div(actions, kPiece) < kFill && ceil_div(actions, kShortPiece) <= kMaxPieces)
+        p.size = kShortPiece;
+    p.count = actions <= kSmall ? 1 : (int)ceil_div(actions, p.size);
+    return p;
+}
+
+struct SmallForward {
+    const B3Logits& g;
+    const Outputs& o;
+    hipStream_t stream;
+    template <typename T, int G, int PER, int W>
+    void operator()() const {
+        lp_small<T, G, PER, W><<<(unsigned)ceil_div(g.rows, kThreads / G), kThreads, 0, stream>>>(g, o);
+    }
+};
+
+struct SmallBackward {
+    const B3Logits& g;
+    const Upstream& u;
+    hipStream_t stream;
+    template <typename T, int G, int PER, int W>
+    void operator()() const {
+        lp_small_backward<T, G, PER, W><<<(unsigned)ceil_div(g.rows, kThreads / G), kThreads, 0, stream>>>(g, u);
+    }
+};
+
+template <typename T, int PER, int W>
+void launch_piece(const B3Logits& g, const Outputs& o, const Pieces& p, unsigned grid, hipStream_t stream) {
+    if (o.top)
+        lp_piece<T, PER, W, true><<<grid, kThreads, 0, stream>>>(g, o, p);
+    else
+        lp_piece<T, PER, W, false><<<grid, kThreads, 0, stream>>>(g, o, p);
+}
+
+template <typename T>
+hipError_t forward(const B3Logits& g, const Outputs& o, Pieces p, hipStream_t stream) {
+    constexpr int W = 16 / sizeof(T);
+    if (g.actions <= kSmall) {
+        with_small<T>(g.actions, SmallForward{g, o, stream});
+        return hipGetLastError();
+    }
+    const unsigned grid = (unsigned)(g.rows * p.count);
+    const int64_t most = p.count == 1 ? g.actions : p.size;
+    if (most <= kThreads * 16)
+        launch_piece<T, 16, W>(g, o, p, grid, stream);
+    else if (most <= kThreads * 32)
+        launch_piece<T, 32, W>(g, o, p, grid, stream);
+    else
+        launch_piece<T, 64, W>(g, o, p, grid, stream);
+    hipError_t err = hipGetLastError();
+    if (err != hipSuccess || p.count == 1) return err;
+    lp_join<T><<<(unsigned)g.rows, kWave, (size_t)p.count * o.top * sizeof(uint2), stream>>>(g, o, p);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t backward(const B3Logits& g, const Upstream& u, hipStream_t stream) {
+    constexpr int W = 16 / sizeof(T), PER = 4 * W;
+    if (g.actions <= kSmall) {
+        with_small<T>(g.actions, SmallBackward{g, u, stream});
+    } else {
+        const int64_t pieces = ceil_div(g.actions, kThreads * PER);
+        lp_piece_backward<T, PER, W><<<(unsigned)(g.rows * pieces), kThreads, 0, stream>>>(g, u, (unsigned)pieces);
+    }
+    return hipGetLastError();
+}
+
+/* The rows' count keeps every grid below 2^31 workgroups. */
 bool valid(const B3Logits& g, const int64_t* taken) {
-    return is_float_type(g.type) && g.rows >= 0 && g.rows <= 0x7fffffff && g.actions >= 1 && g.actions <= 1 << 30
-        && g.row_stride >= g.actions && (!g.mask || g.mask_row_stride == 0 || g.mask_row_stride >= g.actions)
-        && (g.rows == 0 || (g.data && taken));
+    return is_float_type(g.type) && g.rows >= 0 && g.rows <= 0x7fffffff && g.actions >= 1 && g.actions <= kMaxActions
+        && g.rows * ceil_div(g.actions, 1024) <= 0x7fffffff && g.row_stride >= g.actions
+        && (!g.mask || g.mask_row_stride == 0 || g.mask_row_stride >= g.actions) && (g.rows == 0 || (g.data && taken));
 }
 
 }  // namespace
@@ -129,23 +590,26 @@ using namespace b3p;
 
 extern "C" {
 
-size_t b3_log_probs_workspace(int64_t, int64_t, int) { return 0; }
+size_t b3_log_probs_workspace(int64_t rows, int64_t actions, int top) {
+    if (rows <= 0 || actions <= kSmall || actions > kMaxActions || top < 0) return 0;
+    const Pieces p = pieces_of(rows, actions);
+    return p.count == 1 ? 0 : (size_t)rows * p.count * (16 + (size_t)top * sizeof(uint2));
+}
 
 hipError_t b3_log_probs_gpu(B3Logits g, const int64_t* taken, float* log_prob, float* entropy, float* stats, int top,
         float* top_log_prob, int64_t* top_action, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     if (!valid(g, taken) || top < 0 || top > B3_MAX_TOP || top > g.actions) return hipErrorInvalidValue;
-    if (workspace_bytes < b3_log_probs_workspace(g.rows, g.actions, top)) return hipErrorInvalidValue;
+    const size_t need = b3_log_probs_workspace(g.rows, g.actions, top);
+    if (workspace_bytes < need || (need && !workspace)) return hipErrorInvalidValue;
     if (g.rows == 0) return hipSuccess;
     if (!log_prob || !entropy || (top && (!top_log_prob || !top_action))) return hipErrorInvalidValue;
-    (void)workspace;
-    dim3 grid((unsigned)g.rows);
-    if (g.type == B3_F32)
-        lp_rows<B3_F32><<<grid, kThreads, 0, stream>>>(g, taken, log_prob, entropy, stats, top, top_log_prob, top_action);
-    else if (g.type == B3_F16)
-        lp_rows<B3_F16><<<grid, kThreads, 0, stream>>>(g, taken, log_prob, entropy, stats, top, top_log_prob, top_action);
-    else
-        lp_rows<B3_BF16><<<grid, kThreads, 0, stream>>>(g, taken, log_prob, entropy, stats, top, top_log_prob, top_action);
-    return hipGetLastError();
+    const Outputs o = {taken, log_prob, entropy, stats, top, top_log_prob, top_action};
+    Pieces p = pieces_of(g.rows, g.actions);
+    p.top = (uint2*)workspace;
+    p.sums = (Sums*)((char*)workspace + (size_t)g.rows * p.count * top * sizeof(uint2));
+    hipError_t err = hipSuccess;
+    with_type(g.type, [&](auto t) { err = forward<decltype(t)>(g, o, p, stream); });
+    return err;
 }
 
 hipError_t b3_log_probs_backward_gpu(B3Logits g, const int64_t* taken, const float* stats, const float* entropy,
@@ -154,17 +618,10 @@ hipError_t b3_log_probs_backward_gpu(B3Logits g, const int64_t* taken, const flo
     if (!valid(g, taken) || d_row_stride < g.actions || dl_stride < 0 || dh_stride < 0) return hipErrorInvalidValue;
     if (g.rows == 0) return hipSuccess;
     if (!stats || !entropy || !d_logits) return hipErrorInvalidValue;
-    dim3 grid((unsigned)g.rows);
-    if (g.type == B3_F32)
-        lp_backward<B3_F32><<<grid, kThreads, 0, stream>>>(g, taken, stats, entropy, d_log_prob, dl_stride, d_entropy,
-            dh_stride, d_logits, d_row_stride);
-    else if (g.type == B3_F16)
-        lp_backward<B3_F16><<<grid, kThreads, 0, stream>>>(g, taken, stats, entropy, d_log_prob, dl_stride, d_entropy,
-            dh_stride, d_logits, d_row_stride);
-    else
-        lp_backward<B3_BF16><<<grid, kThreads, 0, stream>>>(g, taken, stats, entropy, d_log_prob, dl_stride, d_entropy,
-            dh_stride, d_logits, d_row_stride);
-    return hipGetLastError();
+    const Upstream u = {taken, stats, entropy, d_log_prob, dl_stride, d_entropy, dh_stride, d_logits, d_row_stride};
+    hipError_t err = hipSuccess;
+    with_type(g.type, [&](auto t) { err = backward<decltype(t)>(g, u, stream); });
+    return err;
 }
 
 }  // extern "C"
