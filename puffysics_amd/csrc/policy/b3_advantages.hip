@@ -4,6 +4,17 @@
  *
  *   A_t = d_t + a_t A_{t+1},  d_t = r_t + gamma V_{t+1} - V_t,
  *   a_t = gamma lambda; a terminal at t drops the terms of t + 1.
+ *
+ * Each step maps the advantage after it to its own by x -> b + a x, and such
+ * maps compose, so that time can be cut.  A thread holds the E steps of a
+ * segment in registers and composes them; SEGS threads compose their
+ * segments in LDS; then each goes over its steps again from the advantage
+ * that enters its segment, and writes.  A workgroup's tile of SEGS E steps of
+ * COLS environments moves from the end of the rollout to its start.  Where
+ * environments alone would not give every compute unit a workgroup, the steps
+ * are cut into pieces: a first launch composes each piece, and the second
+ * folds the later pieces before it writes.  Everything is read once (twice
+ * where cut: from the caches) and written once.
  */
 #include "policy_common.h"
 
@@ -11,40 +22,238 @@ namespace b3p {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMaxPieces = 512;
+constexpr int64_t kFill = 256;                   // workgroups: one to a compute unit
 
-template <typename V, typename D>
-__global__ __launch_bounds__(kThreads) void adv_columns(B3Rollout g, float gamma, float decay) {
-    const int64_t n = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (n >= g.envs) return;
-    const float* rewards = g.rewards + n * g.rewards_stride[1];
-    const V* values = (const V*)g.values + n * g.values_stride[1];
-    const D* terminals = (const D*)g.terminals + n * g.terminals_stride[1];
-    float after = to_float(((const V*)g.last_values)[n * g.last_values_stride]), adv = 0;
-    for (int64_t t = g.steps - 1; t >= 0; t--) {
-        float v = to_float(values[t * g.values_stride[0]]);
-        float r = rewards[t * g.rewards_stride[0]];
-        adv = terminals[t * g.terminals_stride[0]] != 0 ? r - v : r + gamma * after - v + decay * adv;
-        g.advantages[n * g.out_stride[1] + t * g.out_stride[0]] = adv;
-        g.returns[n * g.out_stride[1] + t * g.out_stride[0]] = adv + v;
-        after = v;
+/* x -> b + a x.  a < 0 stands for a map that drops x altogether, as a
+ * terminal does: 0 times a NaN would not.  A product of rates stays over 0,
+ * since an infinity goes all the way back to the last terminal. */
+struct Map {
+    float a, b;
+};
+
+constexpr float kLeast = 1.17549435e-38f;
+
+__device__ float apply(Map f, float x) { return f.a < 0 ? f.b : f.b + f.a * x; }
+
+/* f after g: the earlier steps' f takes what the later ones' g gives. */
+__device__ Map compose(Map f, Map g) {
+    if (f.a < 0) return f;
+    return Map{g.a < 0 ? -1.0f : fmaxf(f.a * g.a, kLeast), f.b + f.a * g.b};
+}
+
+struct Job {
+    B3Rollout g;
+    float gamma, decay;
+    bool wide;                                   // steps are neighbours in every array
+    int64_t tiles;                               // of a piece
+    int64_t pieces;
+    Map* piece;                                  // [pieces][envs]
+};
+
+/* `count` (at most E) steps' values. */
+template <int E, typename T>
+__device__ void load_typed(const T* p, int64_t stride, int count, bool wide, float x[E]) {
+    if (wide && count >= E) {
+#pragma unroll
+        for (int v = 0; v < E / 4; v++) {
+            Pack<T, 4> k = *(const Pack<T, 4>*)(p + 4 * v);
+#pragma unroll
+            for (int w = 0; w < 4; w++) x[4 * v + w] = to_float(k.v[w]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; e++) x[e] = e < count ? to_float(p[e * stride]) : 0.0f;
     }
+}
+
+template <int E>
+__device__ void load_steps(const void* p, int type, int64_t at, int64_t stride, int count, bool wide, float x[E]) {
+    if (type == B3_F32)
+        load_typed<E>((const float*)p + at, stride, count, wide, x);
+    else if (type == B3_BF16)
+        load_typed<E>((const __bf16*)p + at, stride, count, wide, x);
+    else if (type == B3_F16)
+        load_typed<E>((const _Float16*)p + at, stride, count, wide, x);
+    else
+        load_typed<E>((const uint8_t*)p + at, stride, count, wide, x);
+}
+
+__device__ float load_one(const void* p, int type, int64_t at) {
+    return type == B3_F32 ? ((const float*)p)[at]
+        : type == B3_BF16 ? to_float(((const __bf16*)p)[at]) : to_float(((const _Float16*)p)[at]);
+}
+
+/* BY_ENV: neighbouring threads have neighbouring environments, else
+ * neighbouring segments.  SUM: compose the piece and write its map; else
+ * write the advantages. */
+template <bool BY_ENV, int COLS, int E, bool SUM>
+__global__ __launch_bounds__(kThreads) void adv_tiles(Job job) {
+    constexpr int SEGS = kThreads / COLS;
+    __shared__ Map lds[2][kThreads];
+    const B3Rollout& g = job.g;
+    const int tid = threadIdx.x;
+    const int col = BY_ENV ? tid % COLS : tid / SEGS, seg = BY_ENV ? tid / COLS : tid % SEGS;
+    const int64_t blocks = (g.envs + COLS - 1) / COLS;
+    const int64_t env = (int64_t)(blockIdx.x % blocks) * COLS + col, piece = blockIdx.x / blocks;
+    const bool live = env < g.envs;
+    const int64_t all_tiles = (g.steps + SEGS * E - 1) / (SEGS * E);
+    const int64_t first = piece * job.tiles;
+    int64_t tile = first + job.tiles < all_tiles ? first + job.tiles : all_tiles;
+
+    /* lds[.][segment of a column]: the maps of its segments from `seg` on,
+     * composed; the result is in lds[at] */
+    auto compose_later = [&](Map mine, int& at) {
+        lds[0][seg * COLS + col] = mine;
+        at = 0;
+        __syncthreads();
+#pragma unroll
+        for (int d = 1; d < SEGS; d *= 2) {
+            if (seg + d < SEGS) mine = compose(mine, lds[at][(seg + d) * COLS + col]);
+            at ^= 1;
+            lds[at][seg * COLS + col] = mine;
+            __syncthreads();
+        }
+    };
+
+    /* the advantage after the piece, from the maps of the later ones */
+    float carry = 0;
+    if (!SUM && job.pieces > 1) {
+        const int64_t later = job.pieces - piece - 1, each = (later + SEGS - 1) / SEGS;
+        Map f = {1, 0};
+        for (int64_t k = each - 1; k >= 0; k--) {
+            const int64_t p = piece + 1 + seg * each + k;
+            if (live && p < job.pieces) f = compose(job.piece[p * g.envs + env], f);
+        }
+        int at;
+        compose_later(f, at);
+        carry = apply(lds[at][col], 0);
+        __syncthreads();
+    }
+    Map total = {1, 0};                          // of the piece's tiles so far
+
+    while (--tile >= first) {
+        const int64_t t = (tile * SEGS + seg) * E;
+        const int64_t left = live ? g.steps - t : 0;
+        const int count = left < 0 ? 0 : left < E ? (int)left : E;
+        float r[E], v[E], end[E], after = 0;
+        load_steps<E>(g.rewards, B3_F32, env * g.rewards_stride[1] + t * g.rewards_stride[0], g.rewards_stride[0], count,
+            job.wide, r);
+        load_steps<E>(g.values, g.values_type, env * g.values_stride[1] + t * g.values_stride[0], g.values_stride[0],
+            count, job.wide, v);
+        load_steps<E>(g.terminals, g.terminals_type, env * g.terminals_stride[1] + t * g.terminals_stride[0],
+            g.terminals_stride[0], count, job.wide, end);
+        if (count)
+            after = t + count < g.steps
+                ? load_one(g.values, g.values_type, env * g.values_stride[1] + (t + count) * g.values_stride[0])
+                : load_one(g.last_values, g.values_type, env * g.last_values_stride);
+        /* r becomes d; the map of the segment */
+        Map f = {1, 0};
+#pragma unroll
+        for (int e = E - 1; e >= 0; e--) {
+            if (e < count) {
+                const bool ends = end[e] != 0;
+                r[e] = ends ? r[e] - v[e] : r[e] + job.gamma * after - v[e];
+                after = v[e];
+                f.b = ends ? r[e] : r[e] + job.decay * f.b;
+                f.a = ends ? -1.0f : f.a < 0 ? f.a : fmaxf(f.a * job.decay, kLeast);
+            }
+        }
+        int at;
+        compose_later(f, at);
+        const Map whole = lds[at][col];
+        if (SUM) {
+            total = compose(whole, total);
+        } else {
+            float x = seg + 1 < SEGS ? apply(lds[at][(seg + 1) * COLS + col], carry) : carry;
+            carry = apply(whole, carry);
+#pragma unroll
+            for (int e = E - 1; e >= 0; e--) {
+                if (e < count) {
+                    x = end[e] != 0 ? r[e] : r[e] + job.decay * x;
+                    r[e] = x;
+                    v[e] += x;
+                }
+            }
+            const int64_t o = env * g.out_stride[1] + t * g.out_stride[0];
+            if (job.wide && count >= E) {
+#pragma unroll
+                for (int k = 0; k < E / 4; k++) {
+                    *(Pack<float, 4>*)(g.advantages + o + 4 * k) = Pack<float, 4>{r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]};
+                    *(Pack<float, 4>*)(g.returns + o + 4 * k) = Pack<float, 4>{v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]};
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    if (e < count) {
+                        g.advantages[o + e * g.out_stride[0]] = r[e];
+                        g.returns[o + e * g.out_stride[0]] = v[e];
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (SUM && seg == 0 && live) job.piece[piece * g.envs + env] = total;
+}
+
+/* How a rollout is cut: lanes along environments or along steps, environments
+ * to a workgroup, pieces of the steps. */
+struct Plan {
+    bool by_env;
+    int cols, steps;                             // steps: E
+    int64_t blocks, tiles, pieces;
+};
+
+Plan plan_of(int64_t steps, int64_t envs, bool by_env) {
+    Plan p;
+    p.by_env = by_env;
+    if (by_env) {
+        p.cols = envs >= 64 * kFill ? 64 : 16;
+        p.steps = envs >= 64 * kFill ? 16 : 8;
+    } else {
+        p.cols = steps <= 64 ? 64 : steps <= 512 ? 16 : 1;
+        p.steps = 16;
+    }
+    const int64_t tile = (int64_t)(kThreads / p.cols) * p.steps, all = ceil_div(steps, tile);
+    p.blocks = ceil_div(envs, p.cols);
+    p.pieces = 1;
+    if (p.blocks < kFill) {
+        p.pieces = ceil_div(kFill * 2, p.blocks);
+        p.pieces = p.pieces < all ? p.pieces : all;
+        p.pieces = p.pieces < kMaxPieces ? p.pieces : kMaxPieces;
+    }
+    p.tiles = ceil_div(all, p.pieces);
+    p.pieces = ceil_div(all, p.tiles);
+    return p;
+}
+
+/* Lanes along the axis of neighbours; fewer environments than a workgroup
+ * takes side by side leave its lanes to the steps. */
+bool by_env(const B3Rollout& g) { return g.envs >= 16 && g.out_stride[1] <= g.out_stride[0]; }
+
+template <bool BY_ENV, int COLS, int E>
+hipError_t launch(const Job& job, const Plan& p, hipStream_t stream) {
+    const unsigned grid = (unsigned)(p.blocks * p.pieces);
+    if (p.pieces > 1) {
+        adv_tiles<BY_ENV, COLS, E, true><<<grid, kThreads, 0, stream>>>(job);
+        hipError_t err = hipGetLastError();
+        if (err != hipSuccess) return err;
+    }
+    adv_tiles<BY_ENV, COLS, E, false><<<grid, kThreads, 0, stream>>>(job);
+    return hipGetLastError();
 }
 
 bool valid(const B3Rollout& g) {
     if (g.steps < 0 || g.envs < 0 || !is_float_type(g.values_type)) return false;
     if (g.terminals_type != B3_F32 && g.terminals_type != B3_U8) return false;
     if (g.steps == 0 || g.envs == 0) return true;
-    return g.envs <= INT64_MAX / g.steps && g.rewards && g.values && g.last_values && g.terminals && g.advantages
-        && g.returns && g.envs <= (int64_t)kThreads * 0x7fffffff;
+    return g.envs <= 0x7fffffff && g.steps <= 0x7fffffff && g.rewards && g.values && g.last_values && g.terminals
+        && g.advantages && g.returns;
 }
 
-template <typename V>
-void launch(const B3Rollout& g, float gamma, float decay, hipStream_t stream) {
-    unsigned grid = (unsigned)ceil_div(g.envs, kThreads);
-    if (g.terminals_type == B3_F32)
-        adv_columns<V, float><<<grid, kThreads, 0, stream>>>(g, gamma, decay);
-    else
-        adv_columns<V, uint8_t><<<grid, kThreads, 0, stream>>>(g, gamma, decay);
+size_t workspace_of(const Plan& p, int64_t envs) {
+    return p.pieces > 1 ? (size_t)p.pieces * envs * sizeof(Map) : 0;
 }
 
 }  // namespace
@@ -54,22 +263,27 @@ using namespace b3p;
 
 extern "C" {
 
-size_t b3_advantages_workspace(int64_t, int64_t) { return 0; }
+/* For either layout. */
+size_t b3_advantages_workspace(int64_t steps, int64_t envs) {
+    if (steps <= 0 || envs <= 0) return 0;
+    const size_t a = workspace_of(plan_of(steps, envs, true), envs), b = workspace_of(plan_of(steps, envs, false), envs);
+    return a > b ? a : b;
+}
 
 hipError_t b3_advantages_gpu(const B3Rollout* g, double gamma, double lambda, void* workspace, size_t workspace_bytes,
         hipStream_t stream) {
-    if (!g || !valid(*g) || !(gamma >= 0 && gamma <= 1) || !(lambda >= 0 && lambda <= 1)
-            || workspace_bytes < b3_advantages_workspace(g->steps, g->envs))
-        return hipErrorInvalidValue;
+    if (!g || !valid(*g) || !(gamma >= 0 && gamma <= 1) || !(lambda >= 0 && lambda <= 1)) return hipErrorInvalidValue;
     if (g->steps == 0 || g->envs == 0) return hipSuccess;
-    (void)workspace;
-    if (g->values_type == B3_F32)
-        launch<float>(*g, (float)gamma, (float)(gamma * lambda), stream);
-    else if (g->values_type == B3_F16)
-        launch<_Float16>(*g, (float)gamma, (float)(gamma * lambda), stream);
-    else
-        launch<__bf16>(*g, (float)gamma, (float)(gamma * lambda), stream);
-    return hipGetLastError();
+    const Plan p = plan_of(g->steps, g->envs, by_env(*g));
+    const size_t need = workspace_of(p, g->envs);
+    if (workspace_bytes < need || (need && !workspace)) return hipErrorInvalidValue;
+    const bool wide = g->rewards_stride[0] == 1 && g->values_stride[0] == 1 && g->terminals_stride[0] == 1
+        && g->out_stride[0] == 1;
+    const Job job = {*g, (float)gamma, (float)(gamma * lambda), wide, p.tiles, p.pieces, (Map*)workspace};
+    if (p.by_env)
+        return p.cols == 64 ? launch<true, 64, 16>(job, p, stream) : launch<true, 16, 8>(job, p, stream);
+    return p.cols == 64 ? launch<false, 64, 16>(job, p, stream)
+        : p.cols == 16 ? launch<false, 16, 16>(job, p, stream) : launch<false, 1, 16>(job, p, stream);
 }
 
 }  // extern "C"
