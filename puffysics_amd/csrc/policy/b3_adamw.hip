@@ -2,26 +2,32 @@
  * b3_adamw.hip - AdamW over many tensors at once, moments in 32 or 8 bits,
  * with the clip of the gradients' norm (include/b3_policy.h).
  *
- * The tensors are cut into chunks of kChunk elements, a workgroup each; a
- * table of chunks made once says whose.  A launch takes the gradients of up
- * to kBatch tensors as kernel arguments, so a step copies nothing to the
- * device.  With a clip the norm is summed first: chunk by chunk, then all
- * chunks in one order.
+ * The tensors are cut into chunks of kChunk elements; a table of chunks made
+ * once says whose each is.  A launch takes the gradients of up to kBatch
+ * tensors as kernel arguments, so that a step copies nothing to the device.
+ * The step is one pass: a workgroup to a chunk, a thread's loads of two
+ * vectors of everything issued before the first is used.  It is bound by
+ * memory (28 bytes a weight in 32 bits).  With a clip the norm is summed
+ * first, by at most kSumBlocks workgroups a launch over their chunks in turn;
+ * few partial sums are added by the step itself, many by a launch of their
+ * own.  Sums go in one order always.
  */
 #include "policy_common.h"
 
 #include <stdlib.h>
-#include <string.h>
 
 namespace b3p {
 
 constexpr int kThreads = 256;
 constexpr int kVector = 4;                       // elements a thread loads at once
+constexpr int kUnroll = 2;                       // vectors of a thread in flight
 constexpr int kChunk = 4096;
-constexpr int kTurns = kChunk / (kThreads * kVector);
+constexpr int kTurn = kThreads * kVector * kUnroll;
+constexpr int kSumBlocks = 2048;
 constexpr int kBatch = 160;                      // tensors to a launch: 4,000 bytes of arguments
 constexpr int kGroup = 32;                       // 8-bit moments: elements to a scale
 constexpr int kSumThreads = 1024;
+constexpr int kFewPartials = kThreads;
 
 /* A tensor of the table. */
 struct Tensor {
@@ -63,8 +69,10 @@ struct B3AdamW {
     b3p::Moments moments;
     b3p::Tensor* tensors;                        // device
     int2* chunk;                                 // device: tensor, chunk of it
-    float* partial;                              // device: sums of squares of the chunks
+    int partials;                                // of a step with a clip
+    double* partial;                             // device: sums of squares
     float* scale;                                // device: the clip's factor
+    float* inverse;                              // device: see aw_inverse
     int64_t* first;                              // host: a tensor's first chunk; count + 1
     int64_t* steps;                              // host
     B3AdamWTensor* given;                        // host
@@ -81,9 +89,10 @@ inline __host__ __device__ uint32_t mix(uint32_t x) {
     return x ^ x >> 16;
 }
 
-template <typename T>
+/* FULL: no element passes the tensor's end. */
+template <bool FULL, typename T>
 __device__ void load(const T* p, int64_t i, int64_t n, float x[kVector]) {
-    if (i + kVector <= n) {
+    if (FULL || i + kVector <= n) {
         Pack<T, kVector> v = *(const Pack<T, kVector>*)(p + i);
 #pragma unroll
         for (int k = 0; k < kVector; k++) x[k] = to_float(v.v[k]);
@@ -93,9 +102,9 @@ __device__ void load(const T* p, int64_t i, int64_t n, float x[kVector]) {
     }
 }
 
-template <typename T>
+template <bool FULL, typename T>
 __device__ void store(T* p, int64_t i, int64_t n, const float x[kVector]) {
-    if (i + kVector <= n) {
+    if (FULL || i + kVector <= n) {
         Pack<T, kVector> v;
 #pragma unroll
         for (int k = 0; k < kVector; k++) v.v[k] = (T)x[k];
@@ -117,20 +126,37 @@ __device__ void unpack(uint32_t codes, uint8_t scale, float x[kVector]) {
     x[3] = __builtin_amdgcn_cvt_f32_fp8(codes, 3) * s;
 }
 
+/* The largest over 8 neighbouring lanes, by lanes swapped in pairs, pairs
+ * swapped, and the eight mirrored. */
+__device__ uint32_t max_of_8_lanes(uint32_t x) {
+    uint32_t y = __builtin_amdgcn_update_dpp(0, x, 0xb1, 0xf, 0xf, true);
+    x = x > y ? x : y;
+    y = __builtin_amdgcn_update_dpp(0, x, 0x4e, 0xf, 0xf, true);
+    x = x > y ? x : y;
+    y = __builtin_amdgcn_update_dpp(0, x, 0x141, 0xf, 0xf, true);
+    return x > y ? x : y;
+}
+static_assert(kGroup / kVector == 8, "a scale's lanes");
+
 /* The exponent byte of the least power of two with which none of the group's
  * finite values passes 448 (7/8 of 2^9). */
 __device__ uint32_t group_scale(const float x[kVector]) {
-    float most = 0;
+    uint32_t most = 0;
 #pragma unroll
     for (int k = 0; k < kVector; k++) {
-        float a = fabsf(x[k]);
-        most = a <= 3.4028235e38f ? fmaxf(most, a) : most;
+        uint32_t a = __float_as_uint(x[k]) & 0x7fffffffu;
+        a = a < 0x7f800000u ? a : 0;
+        most = most > a ? most : a;
     }
-    for (int d = 1; d < kGroup / kVector; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
-    uint32_t b = __float_as_uint(most);
-    int e = (int)(b >> 23) - 8 + ((b & 0x7fffffu) > 0x600000u);
+    most = max_of_8_lanes(most);
+    int e = (int)(most >> 23) - 8 + ((most & 0x7fffffu) > 0x600000u);
     return e < 1 ? 1 : e;
 }
+
+/* inverse[b] = 2^(127 - b) as pow() gives it, a unit in the last place low
+ * for some exponents: torch.ldexp multiplies by the same numbers, so that a
+ * torch program that rounds by the same bits gets the same moments. */
+__global__ void aw_inverse(float* inverse) { inverse[threadIdx.x] = powf(2.0f, 127.0f - (float)threadIdx.x); }
 
 /* x on the group's scale as an e4m3 number, still in 32 bits: one of its two
  * neighbours by 16 random bits, or the nearest. */
@@ -150,8 +176,7 @@ __device__ float round_code(float x, float inverse, uint32_t random) {
 }
 
 template <bool RANDOM, bool ROOT>
-__device__ uint32_t pack(const float x[kVector], uint32_t scale, const uint32_t random[kVector]) {
-    float inverse = __uint_as_float((254u - scale) << 23);
+__device__ uint32_t pack(const float x[kVector], float inverse, const uint32_t random[kVector]) {
     float y[kVector];
 #pragma unroll
     for (int k = 0; k < kVector; k++)
@@ -167,145 +192,200 @@ __device__ void store_codes(uint8_t* codes, uint8_t* scales, int64_t i, uint32_t
 
 /* ---- the step ---- */
 
-template <typename P, typename G, bool MASTER, int BITS>
-__device__ void step_chunk(const Tensor& t, int64_t from, const G* grad, const Moments& mo, const Rates& k, float clip,
-    float size, float root_scale, float keep, uint32_t key) {
-    for (int turn = 0; turn < kTurns; turn++) {
-        const int64_t i = from + (int64_t)(turn * kThreads + (int)threadIdx.x) * kVector;
+/* What a step is to a chunk. */
+struct Step {
+    const Moments& mo;
+    const Rates& rates;
+    const float* inverse;
+    float clip, size, root, keep;
+    uint32_t key;
+};
+
+/* kUnroll vectors of a thread.  The square root is the correctly rounded one,
+ * since what is kept of it is cut off by random bits; the division in the
+ * update is a reciprocal, good to two units. */
+template <typename P, typename G, bool MASTER, int BITS, bool FULL>
+__device__ __forceinline__ void step_turn(const Tensor& t, int64_t from, const G* grad, const Step& s) {
+    float g[kUnroll][kVector], w[kUnroll][kVector], m[kUnroll][kVector], v[kUnroll][kVector];
+    uint32_t cm[kUnroll], cv[kUnroll];
+    uint8_t sm[kUnroll], sv[kUnroll];
+    const int64_t n = t.numel;
+#pragma unroll
+    for (int u = 0; u < kUnroll; u++) {
+        const int64_t i = from + (u * kThreads + (int)threadIdx.x) * kVector, at = t.at + i;
         /* whole groups of 8-bit moments go on together */
-        if (i / kGroup * kGroup >= t.numel) return;
-        const int64_t at = t.at + i;
-        float g[kVector], w[kVector], m[kVector], v[kVector];
-        load(grad, i, t.numel, g);
+        if (!FULL && i / kGroup * kGroup >= n) continue;
+        load<FULL>(grad, i, n, g[u]);
         if (MASTER)
-            load(mo.master + t.at, i, t.numel, w);
+            load<FULL>(s.mo.master + t.at, i, n, w[u]);
         else
-            load((const P*)t.param, i, t.numel, w);
+            load<FULL>((const P*)t.param, i, n, w[u]);
         if (BITS == 32) {
-            load((const float*)mo.exp_avg + t.at, i, t.numel, m);
-            load((const float*)mo.exp_avg_sq + t.at, i, t.numel, v);
+            load<FULL>((const float*)s.mo.exp_avg + t.at, i, n, m[u]);
+            load<FULL>((const float*)s.mo.exp_avg_sq + t.at, i, n, v[u]);
         } else {
-            unpack(*(const uint32_t*)((const uint8_t*)mo.exp_avg + at), mo.exp_avg_scale[at / kGroup], m);
-            unpack(*(const uint32_t*)((const uint8_t*)mo.exp_avg_sq + at), mo.exp_avg_sq_scale[at / kGroup], v);
+            cm[u] = *(const uint32_t*)((const uint8_t*)s.mo.exp_avg + at);
+            cv[u] = *(const uint32_t*)((const uint8_t*)s.mo.exp_avg_sq + at);
+            sm[u] = s.mo.exp_avg_scale[at / kGroup];
+            sv[u] = s.mo.exp_avg_sq_scale[at / kGroup];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; u++) {
+        const int64_t i = from + (u * kThreads + (int)threadIdx.x) * kVector, at = t.at + i;
+        if (!FULL && i / kGroup * kGroup >= n) continue;
+        if (BITS == 8) {
+            unpack(cm[u], sm[u], m[u]);
+            unpack(cv[u], sv[u], v[u]);
         }
         float root[kVector];
 #pragma unroll
         for (int j = 0; j < kVector; j++) {
-            float gc = g[j] * clip;
-            float old = BITS == 32 ? v[j] : v[j] * v[j];
-            m[j] = m[j] * k.beta1 + gc * k.rest1;
-            v[j] = old * k.beta2 + gc * gc * k.rest2;
-            root[j] = sqrtf(v[j]);
-            w[j] = w[j] * keep - m[j] * size / (root[j] * root_scale + k.eps);
+            const float gc = g[u][j] * s.clip, old = BITS == 32 ? v[u][j] : v[u][j] * v[u][j];
+            m[u][j] = m[u][j] * s.rates.beta1 + gc * s.rates.rest1;
+            v[u][j] = old * s.rates.beta2 + gc * gc * s.rates.rest2;
+            root[j] = sqrtf(v[u][j]);
+            w[u][j] = w[u][j] * s.keep - m[u][j] * s.size * __builtin_amdgcn_rcpf(root[j] * s.root + s.rates.eps);
         }
-        store((P*)t.param, i, t.numel, w);
-        if (MASTER) store(mo.master + t.at, i, t.numel, w);
+        store<FULL>((P*)t.param, i, n, w[u]);
+        if (MASTER) store<FULL>(s.mo.master + t.at, i, n, w[u]);
         if (BITS == 32) {
-            store((float*)mo.exp_avg + t.at, i, t.numel, m);
-            store((float*)mo.exp_avg_sq + t.at, i, t.numel, v);
+            store<FULL>((float*)s.mo.exp_avg + t.at, i, n, m[u]);
+            store<FULL>((float*)s.mo.exp_avg_sq + t.at, i, n, v[u]);
         } else {
             uint32_t random[kVector];
+            const uint32_t key = s.key ^ mix((uint32_t)(at >> 32));
 #pragma unroll
-            for (int j = 0; j < kVector; j++)
-                random[j] = mix((uint32_t)(at + j) ^ key ^ mix((uint32_t)((at + j) >> 32)));
-            uint32_t sm = group_scale(m), sr = group_scale(root);
-            store_codes((uint8_t*)mo.exp_avg, mo.exp_avg_scale, at, pack<true, false>(m, sm, random), sm);
-            store_codes((uint8_t*)mo.exp_avg_sq, mo.exp_avg_sq_scale, at, pack<true, true>(root, sr, random), sr);
+            for (int j = 0; j < kVector; j++) random[j] = mix((uint32_t)(at + j) ^ key);
+            const uint32_t to_m = group_scale(m[u]), to_v = group_scale(root);
+            store_codes((uint8_t*)s.mo.exp_avg, s.mo.exp_avg_scale, at, pack<true, false>(m[u], s.inverse[to_m], random), to_m);
+            store_codes((uint8_t*)s.mo.exp_avg_sq, s.mo.exp_avg_sq_scale, at, pack<true, true>(root, s.inverse[to_v], random),
+                to_v);
         }
     }
 }
 
-template <typename P, bool MASTER, int BITS>
-__device__ void step_typed(const Tensor& t, int64_t from, const void* grad, bool float_grad, const Moments& mo,
-    const Rates& k, float clip, float size, float root_scale, float keep, uint32_t key) {
-    if (float_grad)
-        step_chunk<P, float, MASTER, BITS>(t, from, (const float*)grad, mo, k, clip, size, root_scale, keep, key);
-    else
-        step_chunk<P, P, MASTER, BITS>(t, from, (const P*)grad, mo, k, clip, size, root_scale, keep, key);
+template <typename P, typename G, bool MASTER, int BITS>
+__device__ __forceinline__ void step_chunk(const Tensor& t, int64_t from, const G* grad, const Step& s) {
+    if (from + kChunk <= t.numel) {
+        for (int64_t i = from; i < from + kChunk; i += kTurn) step_turn<P, G, MASTER, BITS, true>(t, i, grad, s);
+    } else {
+        for (int64_t i = from; i < t.numel; i += kTurn) step_turn<P, G, MASTER, BITS, false>(t, i, grad, s);
+    }
 }
+
+template <typename P, bool MASTER, int BITS>
+__device__ __forceinline__ void step_typed(const Tensor& t, int64_t from, const void* grad, bool float_grad, const Step& s) {
+    if (float_grad)
+        step_chunk<P, float, MASTER, BITS>(t, from, (const float*)grad, s);
+    else
+        step_chunk<P, P, MASTER, BITS>(t, from, (const P*)grad, s);
+}
+
+/* The clip's factor; a NaN norm stays one. */
+__device__ float clip_of(float norm, float max_norm) {
+    const float s = max_norm / (norm + 1e-6f);
+    return s > 1.0f ? 1.0f : s;
+}
+
+template <int THREADS>
+__device__ double block_sum(double x) {
+    __shared__ double lds[THREADS / kWave];
+    for (int d = kWave / 2; d > 0; d /= 2) x += __shfl_xor(x, d);
+    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = x;
+    __syncthreads();
+    x = 0;
+    for (int w = 0; w < THREADS / kWave; w++) x += lds[w];
+    return x;
+}
+
+/* Where a step's clip comes from. */
+struct Clip {
+    const float* scale;                          // NULL: none, or
+    const double* partial;                       // `partials` sums of squares (at most kFewPartials)
+    int partials;
+    float max_norm;
+    float* norm;
+};
 
 template <int BITS>
 __global__ __launch_bounds__(kThreads) void aw_step(StepArgs a, int base, int64_t first, const int2* chunk,
-    const Tensor* tensors, Moments mo, Rates k, const float* scale) {
+    const Tensor* tensors, Moments mo, Rates k, const float* inverse, Clip clip) {
+    float scale = 1.0f;
+    if (clip.partial) {
+        const float norm = (float)sqrt(block_sum<kThreads>((int)threadIdx.x < clip.partials ? clip.partial[threadIdx.x] : 0));
+        if (first + blockIdx.x == 0 && threadIdx.x == 0) *clip.norm = norm;
+        scale = clip_of(norm, clip.max_norm);
+    } else if (clip.scale) {
+        scale = *clip.scale;
+    }
     const int2 c = chunk[first + blockIdx.x];
     const int at = c.x - base;
     const void* grad = a.grad[at];
     if (!grad) return;
     const Tensor t = tensors[c.x];
     const int64_t from = (int64_t)c.y * kChunk;
-    const float clip = scale ? *scale : 1.0f, size = a.size[at], root = a.root[at], keep = a.keep[at];
-    const uint32_t key = a.key[at];
+    const Step s = {mo, k, inverse, scale, a.size[at], a.root[at], a.keep[at], a.key[at]};
     const bool fg = a.grad_type[at] == B3_F32;
     if (t.type == B3_F32)
-        step_chunk<float, float, false, BITS>(t, from, (const float*)grad, mo, k, clip, size, root, keep, key);
+        step_chunk<float, float, false, BITS>(t, from, (const float*)grad, s);
     else if (t.type == B3_BF16 && mo.master)
-        step_typed<__bf16, true, BITS>(t, from, grad, fg, mo, k, clip, size, root, keep, key);
+        step_typed<__bf16, true, BITS>(t, from, grad, fg, s);
     else if (t.type == B3_BF16)
-        step_typed<__bf16, false, BITS>(t, from, grad, fg, mo, k, clip, size, root, keep, key);
+        step_typed<__bf16, false, BITS>(t, from, grad, fg, s);
     else if (mo.master)
-        step_typed<_Float16, true, BITS>(t, from, grad, fg, mo, k, clip, size, root, keep, key);
+        step_typed<_Float16, true, BITS>(t, from, grad, fg, s);
     else
-        step_typed<_Float16, false, BITS>(t, from, grad, fg, mo, k, clip, size, root, keep, key);
+        step_typed<_Float16, false, BITS>(t, from, grad, fg, s);
 }
 
 /* ---- the norm ---- */
 
-template <typename G>
-__device__ float square_chunk(const G* grad, int64_t from, int64_t n) {
-    float sum = 0;
+/* A thread's squares of a chunk: at most 16 in 32 bits, the rest of the sum
+ * in 64. */
+template <bool FULL, typename G>
+__device__ float squares(const G* grad, int64_t from, int64_t n) {
+    float g[kChunk / (kThreads * kVector)][kVector], sum = 0;
 #pragma unroll
-    for (int turn = 0; turn < kTurns; turn++) {
-        const int64_t i = from + (int64_t)(turn * kThreads + (int)threadIdx.x) * kVector;
-        float g[kVector];
-        load(grad, i, n, g);
+    for (int u = 0; u < kChunk / (kThreads * kVector); u++)
+        load<FULL>(grad, from + (int64_t)(u * kThreads + (int)threadIdx.x) * kVector, n, g[u]);
 #pragma unroll
-        for (int j = 0; j < kVector; j++) sum += g[j] * g[j];
-    }
+    for (int u = 0; u < kChunk / (kThreads * kVector); u++)
+#pragma unroll
+        for (int j = 0; j < kVector; j++) sum += g[u][j] * g[u][j];
     return sum;
 }
 
-__global__ __launch_bounds__(kThreads) void aw_squares(StepArgs a, int base, int64_t first, const int2* chunk,
-    const Tensor* tensors, float* partial) {
-    __shared__ float lds[kThreads / kWave];
-    const int2 c = chunk[first + blockIdx.x];
-    const int at = c.x - base;
-    const void* grad = a.grad[at];
-    float sum = 0;
-    if (grad) {
-        const int64_t n = tensors[c.x].numel, from = (int64_t)c.y * kChunk;
-        const int type = a.grad_type[at];
-        if (type == B3_F32)
-            sum = square_chunk((const float*)grad, from, n);
-        else if (type == B3_BF16)
-            sum = square_chunk((const __bf16*)grad, from, n);
-        else
-            sum = square_chunk((const _Float16*)grad, from, n);
-    }
-    for (int d = kWave / 2; d > 0; d /= 2) sum += __shfl_xor(sum, d);
-    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        sum = 0;
-        for (int w = 0; w < kThreads / kWave; w++) sum += lds[w];
-        partial[first + blockIdx.x] = sum;
-    }
+template <typename G>
+__device__ float square_chunk(const void* grad, int64_t from, int64_t n) {
+    return from + kChunk <= n ? squares<true>((const G*)grad, from, n) : squares<false>((const G*)grad, from, n);
 }
 
-/* The sums of the chunks, added in 64 bits: there may be 10^5 of them. */
-__global__ __launch_bounds__(kSumThreads) void aw_norm(const float* partial, int64_t chunks, float max_norm, float* norm,
-    float* scale) {
-    __shared__ double lds[kSumThreads / kWave];
+__global__ __launch_bounds__(kThreads) void aw_squares(StepArgs a, int base, int64_t first, int64_t end,
+    const int2* chunk, const Tensor* tensors, double* partial) {
     double sum = 0;
-    for (int64_t i = threadIdx.x; i < chunks; i += kSumThreads) sum += partial[i];
-    for (int d = kWave / 2; d > 0; d /= 2) sum += __shfl_xor(sum, d);
-    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = sum;
-    __syncthreads();
+    for (int64_t i = first + blockIdx.x; i < end; i += gridDim.x) {
+        const int2 c = chunk[i];
+        const int at = c.x - base;
+        const void* grad = a.grad[at];
+        if (!grad) continue;
+        const int64_t n = tensors[c.x].numel, from = (int64_t)c.y * kChunk;
+        const int type = a.grad_type[at];
+        sum += type == B3_F32 ? square_chunk<float>(grad, from, n)
+            : type == B3_BF16 ? square_chunk<__bf16>(grad, from, n) : square_chunk<_Float16>(grad, from, n);
+    }
+    sum = block_sum<kThreads>(sum);
+    if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+}
+
+__global__ __launch_bounds__(kSumThreads) void aw_norm(const double* partial, int partials, float max_norm, float* norm,
+    float* scale) {
+    double sum = 0;
+    for (int i = threadIdx.x; i < partials; i += kSumThreads) sum += partial[i];
+    sum = block_sum<kSumThreads>(sum);
     if (threadIdx.x == 0) {
-        sum = 0;
-        for (int w = 0; w < kSumThreads / kWave; w++) sum += lds[w];
-        float n = (float)sqrt(sum), s = max_norm / (n + 1e-6f);
-        *norm = n;
-        *scale = s > 1.0f ? 1.0f : s;            // a NaN norm stays one
+        *norm = (float)sqrt(sum);
+        *scale = clip_of((float)sqrt(sum), max_norm);
     }
 }
 
@@ -318,22 +398,22 @@ __global__ __launch_bounds__(kThreads) void aw_moments(Moments mo, int64_t size,
     unpack(*(const uint32_t*)((const uint8_t*)mo.exp_avg + i), mo.exp_avg_scale[i / kGroup], m);
     unpack(*(const uint32_t*)((const uint8_t*)mo.exp_avg_sq + i), mo.exp_avg_sq_scale[i / kGroup], r);
     for (int k = 0; k < kVector; k++) r[k] *= r[k];
-    store(exp_avg, i, size, m);
-    store(exp_avg_sq, i, size, r);
+    store<true>(exp_avg, i, size, m);
+    store<true>(exp_avg_sq, i, size, r);
 }
 
-__global__ __launch_bounds__(kThreads) void aw_load(Moments mo, int64_t size, const float* exp_avg,
-    const float* exp_avg_sq) {
+__global__ __launch_bounds__(kThreads) void aw_load(Moments mo, int64_t size, const float* inverse,
+    const float* exp_avg, const float* exp_avg_sq) {
     const int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * kVector;
     if (i >= size) return;                        // a multiple of 256: groups stay whole
     float m[kVector], r[kVector];
-    load(exp_avg, i, size, m);
-    load(exp_avg_sq, i, size, r);
+    load<true>(exp_avg, i, size, m);
+    load<true>(exp_avg_sq, i, size, r);
     for (int k = 0; k < kVector; k++) r[k] = sqrtf(r[k]);
     const uint32_t none[kVector] = {0, 0, 0, 0};
     uint32_t sm = group_scale(m), sr = group_scale(r);
-    store_codes((uint8_t*)mo.exp_avg, mo.exp_avg_scale, i, pack<false, false>(m, sm, none), sm);
-    store_codes((uint8_t*)mo.exp_avg_sq, mo.exp_avg_sq_scale, i, pack<false, true>(r, sr, none), sr);
+    store_codes((uint8_t*)mo.exp_avg, mo.exp_avg_scale, i, pack<false, false>(m, inverse[sm], none), sm);
+    store_codes((uint8_t*)mo.exp_avg_sq, mo.exp_avg_sq_scale, i, pack<false, true>(r, inverse[sr], none), sr);
 }
 
 bool valid(const B3AdamWTensor* tensors, int count) {
@@ -351,6 +431,14 @@ bool valid(const B3AdamWTensor* tensors, int count) {
 }
 
 int64_t segment(int64_t numel) { return ceil_div(numel, B3_ADAMW_SEGMENT) * B3_ADAMW_SEGMENT; }
+
+/* Tensors of the launch that begins with tensor `base`. */
+int batch(const B3AdamW* o, int base) { return o->count - base < kBatch ? o->count - base : kBatch; }
+
+int sum_blocks(const B3AdamW* o, int base) {
+    const int64_t chunks = o->first[base + batch(o, base)] - o->first[base];
+    return (int)(chunks < kSumBlocks ? chunks : kSumBlocks);
+}
 
 hipError_t on_device(const B3AdamW* o) {
     int device;
@@ -375,7 +463,7 @@ int64_t b3_adamw_size(const B3AdamWTensor* tensors, int count) {
 hipError_t b3_adamw_destroy(B3AdamW* o) {
     if (!o) return hipSuccess;
     hipError_t first = hipSuccess;
-    void* bufs[4] = {o->tensors, o->chunk, o->partial, o->scale};
+    void* bufs[5] = {o->tensors, o->chunk, o->partial, o->scale, o->inverse};
     for (void* p : bufs) {
         hipError_t err = p ? hipFree(p) : hipSuccess;
         if (first == hipSuccess) first = err;
@@ -424,11 +512,17 @@ hipError_t b3_adamw_create(B3AdamW** out, const B3AdamWTensor* tensors, int coun
             for (int64_t j = 0; j < ceil_div(tensors[i].numel, kChunk); j++) chunk[c++] = make_int2(i, (int)j);
         }
         o->first[count] = c;
+        for (int base = 0; base < count; base += kBatch) o->partials += sum_blocks(o, base);
     }
     if (err == hipSuccess) err = hipMalloc((void**)&o->tensors, ((size_t)count + 1) * sizeof(Tensor));
     if (err == hipSuccess) err = hipMalloc((void**)&o->chunk, ((size_t)chunks + 1) * sizeof(int2));
-    if (err == hipSuccess) err = hipMalloc((void**)&o->partial, ((size_t)chunks + 1) * sizeof(float));
+    if (err == hipSuccess) err = hipMalloc((void**)&o->partial, ((size_t)o->partials + 1) * sizeof(double));
     if (err == hipSuccess) err = hipMalloc((void**)&o->scale, sizeof(float));
+    if (err == hipSuccess) err = hipMalloc((void**)&o->inverse, 256 * sizeof(float));
+    if (err == hipSuccess) {
+        aw_inverse<<<1, 256>>>(o->inverse);
+        err = hipGetLastError();
+    }
     if (err == hipSuccess)
         err = hipMemcpy(o->tensors, table, ((size_t)count + 1) * sizeof(Tensor), hipMemcpyHostToDevice);
     if (err == hipSuccess) err = hipMemcpy(o->chunk, chunk, ((size_t)chunks + 1) * sizeof(int2), hipMemcpyHostToDevice);
@@ -453,14 +547,17 @@ hipError_t b3_adamw_step_gpu(B3AdamW* o, const void* const* grads, const int* gr
     if (err != hipSuccess) return err;
     const B3AdamWConfig& cf = o->config;
     const Rates rates = {(float)cf.beta1, (float)cf.beta2, (float)(1 - cf.beta1), (float)(1 - cf.beta2), (float)cf.eps};
+    const bool few = o->partials > 0 && o->partials <= kFewPartials;
+    Clip clip = {};
+    if (max_norm > 0) clip = few ? Clip{NULL, o->partial, o->partials, (float)max_norm, norm} : Clip{o->scale, NULL, 0, 0, NULL};
     StepArgs a;
     for (int pass = max_norm > 0 ? 0 : 1; pass < 2; pass++) {
         int64_t t_last = -1;
         float size = 0, root = 0;
+        double* partial = o->partial;
         for (int base = 0; base < o->count; base += kBatch) {
-            const int n = o->count - base < kBatch ? o->count - base : kBatch;
-            const int64_t first = o->first[base], blocks = o->first[base + n] - first;
-            memset((void*)&a, 0, sizeof(a));
+            const int n = batch(o, base);
+            const int64_t first = o->first[base], end = o->first[base + n];
             for (int j = 0; j < n; j++) {
                 const int i = base + j;
                 a.grad[j] = grads[i];
@@ -477,19 +574,22 @@ hipError_t b3_adamw_step_gpu(B3AdamW* o, const void* const* grads, const int* gr
                 a.keep[j] = (float)(1 - lr * o->given[i].weight_decay);
                 a.key[j] = mix((uint32_t)t * 0x9e3779b9u + cf.seed);
             }
-            if (blocks == 0) continue;
-            if (pass == 0)
-                aw_squares<<<(unsigned)blocks, kThreads, 0, stream>>>(a, base, first, o->chunk, o->tensors, o->partial);
-            else if (o->bits == 32)
-                aw_step<32><<<(unsigned)blocks, kThreads, 0, stream>>>(a, base, first, o->chunk, o->tensors, o->moments,
-                    rates, max_norm > 0 ? o->scale : NULL);
-            else
-                aw_step<8><<<(unsigned)blocks, kThreads, 0, stream>>>(a, base, first, o->chunk, o->tensors, o->moments,
-                    rates, max_norm > 0 ? o->scale : NULL);
+            if (first == end) continue;
+            if (pass == 0) {
+                const int blocks = sum_blocks(o, base);
+                aw_squares<<<blocks, kThreads, 0, stream>>>(a, base, first, end, o->chunk, o->tensors, partial);
+                partial += blocks;
+            } else if (o->bits == 32) {
+                aw_step<32><<<(unsigned)(end - first), kThreads, 0, stream>>>(a, base, first, o->chunk, o->tensors,
+                    o->moments, rates, o->inverse, clip);
+            } else {
+                aw_step<8><<<(unsigned)(end - first), kThreads, 0, stream>>>(a, base, first, o->chunk, o->tensors,
+                    o->moments, rates, o->inverse, clip);
+            }
             if ((err = hipGetLastError()) != hipSuccess) return err;
         }
-        if (pass == 0) {
-            aw_norm<<<1, kSumThreads, 0, stream>>>(o->partial, o->chunks, (float)max_norm, norm, o->scale);
+        if (pass == 0 && !few) {
+            aw_norm<<<1, kSumThreads, 0, stream>>>(o->partial, o->partials, (float)max_norm, norm, o->scale);
             if ((err = hipGetLastError()) != hipSuccess) return err;
         }
     }
@@ -519,8 +619,8 @@ hipError_t b3_adamw_load_moments_gpu(B3AdamW* o, const float* exp_avg, const flo
     if (!o || o->bits != 8 || (o->size && (!exp_avg || !exp_avg_sq))) return hipErrorInvalidValue;
     hipError_t err = on_device(o);
     if (err != hipSuccess || o->size == 0) return err;
-    aw_load<<<(unsigned)ceil_div(o->size, kThreads * kVector), kThreads, 0, stream>>>(o->moments, o->size, exp_avg,
-        exp_avg_sq);
+    aw_load<<<(unsigned)ceil_div(o->size, kThreads * kVector), kThreads, 0, stream>>>(o->moments, o->size, o->inverse,
+        exp_avg, exp_avg_sq);
     return hipGetLastError();
 }
 

@@ -96,7 +96,7 @@ def _need(ok, what):
 
 
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _on(*tensors):
@@ -133,30 +133,35 @@ def _rows(x):
     return x.contiguous()
 
 
+def _forward(x, taken, mask, top, kept):
+    """(log_prob, entropy, top_log_prob, top_action, stats), the last only
+    where `kept`."""
+    rows, actions = x.shape
+    lib = policy_lib()
+    log_prob = torch.empty(rows, dtype=torch.float32, device=x.device)
+    entropy = torch.empty_like(log_prob)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if kept else None
+    top_lp = top_action = work = None
+    if top:
+        top_lp = torch.empty((rows, top), dtype=torch.float32, device=x.device)
+        top_action = torch.empty((rows, top), dtype=torch.int64, device=x.device)
+    size = lib.b3_log_probs_workspace(rows, actions, top)
+    if size:
+        work = torch.empty(size, dtype=torch.uint8, device=x.device)
+    _check("b3_log_probs_gpu", lib.b3_log_probs_gpu(
+        _logits(x, mask), taken.data_ptr(), log_prob.data_ptr(), entropy.data_ptr(), stats.data_ptr() if kept else None,
+        top, top_lp.data_ptr() if top else None, top_action.data_ptr() if top else None,
+        work.data_ptr() if size else None, size, _stream()))
+    return log_prob, entropy, top_lp, top_action, stats
+
+
 class _LogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, taken, mask, top):
-        rows, actions = x.shape
-        lib = policy_lib()
         x = _rows(x)
-        kept = ctx.needs_input_grad[0]
-        log_prob = torch.empty(rows, dtype=torch.float32, device=x.device)
-        entropy = torch.empty_like(log_prob)
-        stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if kept else None
-        top_lp = top_action = None
-        if top:
-            top_lp = torch.empty((rows, top), dtype=torch.float32, device=x.device)
-            top_action = torch.empty((rows, top), dtype=torch.int64, device=x.device)
-        size = lib.b3_log_probs_workspace(rows, actions, top)
-        work = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-        _check("b3_log_probs_gpu", lib.b3_log_probs_gpu(
-            _logits(x, mask), taken.data_ptr(), log_prob.data_ptr(), entropy.data_ptr(),
-            stats.data_ptr() if kept else None, top, top_lp.data_ptr() if top else None,
-            top_action.data_ptr() if top else None,
-            work.data_ptr() if size else None, size, _stream()))
-        if kept:
-            ctx.save_for_backward(x, taken, mask, stats, entropy)
-            ctx.set_materialize_grads(False)
+        log_prob, entropy, top_lp, top_action, stats = _forward(x, taken, mask, top, True)
+        ctx.save_for_backward(x, taken, mask, stats, entropy)
+        ctx.set_materialize_grads(False)
         if top:
             ctx.mark_non_differentiable(top_lp, top_action)
         return log_prob, entropy, top_lp, top_action
@@ -206,8 +211,12 @@ def log_probs(logits, taken, mask=None, top=0):
     shape = taken.shape
     if len(shape) != 1:
         logits, taken = logits.reshape(-1, actions), taken.reshape(-1)
-    taken = taken.to(torch.int64).contiguous()
-    log_prob, entropy, top_lp, top_action = _LogProbs.apply(logits, taken, mask, top)
+    if taken.dtype != torch.int64 or not taken.is_contiguous():
+        taken = taken.to(torch.int64).contiguous()
+    if logits.requires_grad and torch.is_grad_enabled():
+        log_prob, entropy, top_lp, top_action = _LogProbs.apply(logits, taken, mask, top)
+    else:
+        log_prob, entropy, top_lp, top_action, _ = _forward(_rows(logits), taken, mask, top, False)
     if len(shape) != 1:
         log_prob, entropy = log_prob.reshape(shape), entropy.reshape(shape)
         if top:
@@ -311,6 +320,7 @@ class AdamW:
         state = B3AdamWState(state_bits, self._exp_avg.data_ptr(), self._exp_avg_sq.data_ptr(),
                              self._scale[0].data_ptr(), self._scale[1].data_ptr(),
                              self._master.data_ptr() if self._master is not None else None)
+        self._given = [(p.shape, p.dtype) for p in self.params]
         self._grads, self._types = (_vp * max(n, 1))(), (_i * max(n, 1))()
         torch.cuda.current_stream().synchronize()     # the state is ready for a step on any stream
         _check("b3_adamw_create", self._lib.b3_adamw_create(C.byref(self._h), table, n, state,
@@ -327,14 +337,22 @@ class AdamW:
         if grads is None:
             grads = [p.grad for p in self.params]
         _need(len(grads) == len(self.params), "need one gradient for each parameter")
-        _on(*grads)
-        for i, (p, g) in enumerate(zip(self.params, grads)):
+        here, pointers, types = torch.cuda.current_device(), [], []
+        for g, (shape, dtype) in zip(grads, self._given):
             if g is None:
-                self._grads[i] = None
+                pointers.append(None)
+                types.append(0)
                 continue
-            _need(g.shape == p.shape and g.is_contiguous(), "gradients have to be contiguous, of the parameters' shapes")
-            _need(g.dtype == p.dtype or g.dtype == torch.float32, "gradients have to be of the parameters' type or float32")
-            self._grads[i], self._types[i] = g.data_ptr(), _TYPE[g.dtype]
+            if g.get_device() != here:
+                raise ValueError("gradients have to be on the current CUDA device")
+            if g.shape != shape or not g.is_contiguous():
+                raise ValueError("gradients have to be contiguous, of the parameters' shapes")
+            if g.dtype is not dtype and g.dtype is not torch.float32:
+                raise ValueError("gradients have to be of the parameters' type or float32")
+            pointers.append(g.data_ptr())
+            types.append(_TYPE[g.dtype])
+        n = len(pointers)
+        self._grads[:n], self._types[:n] = pointers, types
         norm = torch.empty((), dtype=torch.float32, device=self.device) if self.max_grad_norm else None
         _check("b3_adamw_step_gpu", self._lib.b3_adamw_step_gpu(
             self._h, self._grads, self._types, self.lr if lr is None else lr, self.max_grad_norm or 0.0,
