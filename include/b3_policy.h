@@ -48,7 +48,7 @@ typedef struct B3Logits {
     const void* data;
     int type;                    /* B3_F32, B3_F16 or B3_BF16 */
     int64_t rows;
-    int64_t actions;             /* 1 .. 2^22 */
+    int64_t actions;             /* 1 .. 2^21 */
     int64_t row_stride;
     const unsigned char* mask;
     int64_t mask_row_stride;

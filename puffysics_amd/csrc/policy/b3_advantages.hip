@@ -51,32 +51,68 @@ struct Job {
     Map* piece;                                  // [pieces][envs]
 };
 
-/* `count` (at most E) steps' values. */
+/* Unsigned numbers that lie anywhere. */
+template <typename T, int N>
+struct __attribute__((packed, aligned(1))) Bytes {
+    T v[N];
+};
+
+/* E steps' elements as they lie: in words of their own, or, where the steps
+ * are neighbours, packed.  Nothing is done with them here, so that the loads
+ * of all arrays are in flight together.  Steps from `count` (at least 1) on
+ * give the last one's. */
 template <int E, typename T>
-__device__ void load_typed(const T* p, int64_t stride, int count, bool wide, float x[E]) {
-    if (wide && count >= E) {
+__device__ __forceinline__ void load_raw(const T* p, int64_t stride, int count, bool packed, uint32_t raw[E]) {
+    if (packed) {
+        constexpr int kWords = E * (int)sizeof(T) / 4, kVec = kWords < 4 ? kWords : 4;
 #pragma unroll
-        for (int v = 0; v < E / 4; v++) {
-            Pack<T, 4> k = *(const Pack<T, 4>*)(p + 4 * v);
+        for (int k = 0; k < kWords; k += kVec) {
+            Bytes<uint32_t, kVec> b = *(const Bytes<uint32_t, kVec>*)((const char*)p + 4 * k);
 #pragma unroll
-            for (int w = 0; w < 4; w++) x[4 * v + w] = to_float(k.v[w]);
+            for (int w = 0; w < kVec; w++) raw[k + w] = b.v[w];
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < E; e++) x[e] = e < count ? to_float(p[e * stride]) : 0.0f;
+        for (int e = 0; e < E; e++) raw[e] = p[(e < count ? e : count - 1) * stride];
     }
 }
 
 template <int E>
-__device__ void load_steps(const void* p, int type, int64_t at, int64_t stride, int count, bool wide, float x[E]) {
+__device__ __forceinline__ void load_steps(const void* p, int type, int64_t at, int64_t stride, int count, bool packed,
+    uint32_t raw[E]) {
     if (type == B3_F32)
-        load_typed<E>((const float*)p + at, stride, count, wide, x);
-    else if (type == B3_BF16)
-        load_typed<E>((const __bf16*)p + at, stride, count, wide, x);
-    else if (type == B3_F16)
-        load_typed<E>((const _Float16*)p + at, stride, count, wide, x);
+        load_raw<E>((const uint32_t*)p + at, stride, count, packed, raw);
+    else if (type == B3_U8)
+        load_raw<E>((const uint8_t*)p + at, stride, count, packed, raw);
     else
-        load_typed<E>((const uint8_t*)p + at, stride, count, wide, x);
+        load_raw<E>((const uint16_t*)p + at, stride, count, packed, raw);
+}
+
+template <int E>
+__device__ __forceinline__ void floats_of(const uint32_t raw[E], int type, bool packed, float x[E]) {
+    if (type == B3_F32) {
+#pragma unroll
+        for (int e = 0; e < E; e++) x[e] = __uint_as_float(raw[e]);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const uint32_t h = packed ? raw[e / 2] >> (16 * (e % 2)) & 0xffffu : raw[e];
+        x[e] = type == B3_BF16 ? __uint_as_float(h << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+    }
+}
+
+/* Bit e: step e ends an episode. */
+template <int E>
+__device__ __forceinline__ uint32_t ends_of(const uint32_t raw[E], int type, bool packed) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const uint32_t h = type == B3_F32 ? raw[e] & 0x7fffffffu
+            : packed ? raw[e / 4] >> (8 * (e % 4)) & 0xffu : raw[e];
+        bits |= (h != 0) << e;
+    }
+    return bits;
 }
 
 __device__ float load_one(const void* p, int type, int64_t at) {
@@ -95,7 +131,11 @@ __global__ __launch_bounds__(kThreads) void adv_tiles(Job job) {
     const int tid = threadIdx.x;
     const int col = BY_ENV ? tid % COLS : tid / SEGS, seg = BY_ENV ? tid / COLS : tid % SEGS;
     const int64_t blocks = (g.envs + COLS - 1) / COLS;
-    const int64_t env = (int64_t)(blockIdx.x % blocks) * COLS + col, piece = blockIdx.x / blocks;
+    /* workgroups go to the 8 dies in turn: each die's take neighbouring
+     * blocks, whose rows share lines of its cache */
+    const unsigned die = blockIdx.x % 8, share = gridDim.x / 8, rest = gridDim.x % 8;
+    const unsigned block = die * share + (die < rest ? die : rest) + blockIdx.x / 8;
+    const int64_t env = (int64_t)(block % blocks) * COLS + col, piece = block / blocks;
     const bool live = env < g.envs;
     const int64_t all_tiles = (g.steps + SEGS * E - 1) / (SEGS * E);
     const int64_t first = piece * job.tiles;
@@ -136,27 +176,34 @@ __global__ __launch_bounds__(kThreads) void adv_tiles(Job job) {
         const int64_t t = (tile * SEGS + seg) * E;
         const int64_t left = live ? g.steps - t : 0;
         const int count = left < 0 ? 0 : left < E ? (int)left : E;
-        float r[E], v[E], end[E], after = 0;
-        load_steps<E>(g.rewards, B3_F32, env * g.rewards_stride[1] + t * g.rewards_stride[0], g.rewards_stride[0], count,
-            job.wide, r);
-        load_steps<E>(g.values, g.values_type, env * g.values_stride[1] + t * g.values_stride[0], g.values_stride[0],
-            count, job.wide, v);
-        load_steps<E>(g.terminals, g.terminals_type, env * g.terminals_stride[1] + t * g.terminals_stride[0],
-            g.terminals_stride[0], count, job.wide, end);
-        if (count)
+        float r[E], v[E], after = 0;
+        uint32_t ends = 0;
+        if (count) {
+            const bool packed = job.wide && count == E;
+            uint32_t raw_r[E], raw_v[E], raw_end[E];
+            load_steps<E>(g.rewards, B3_F32, env * g.rewards_stride[1] + t * g.rewards_stride[0], g.rewards_stride[0], count,
+                packed, raw_r);
+            load_steps<E>(g.terminals, g.terminals_type, env * g.terminals_stride[1] + t * g.terminals_stride[0],
+                g.terminals_stride[0], count, packed, raw_end);
+            load_steps<E>(g.values, g.values_type, env * g.values_stride[1] + t * g.values_stride[0], g.values_stride[0],
+                count, packed, raw_v);
             after = t + count < g.steps
                 ? load_one(g.values, g.values_type, env * g.values_stride[1] + (t + count) * g.values_stride[0])
                 : load_one(g.last_values, g.values_type, env * g.last_values_stride);
+            floats_of<E>(raw_r, B3_F32, packed, r);
+            floats_of<E>(raw_v, g.values_type, packed, v);
+            ends = ends_of<E>(raw_end, g.terminals_type, packed);
+        }
         /* r becomes d; the map of the segment */
         Map f = {1, 0};
 #pragma unroll
         for (int e = E - 1; e >= 0; e--) {
             if (e < count) {
-                const bool ends = end[e] != 0;
-                r[e] = ends ? r[e] - v[e] : r[e] + job.gamma * after - v[e];
+                const bool end = ends >> e & 1;
+                r[e] = end ? r[e] - v[e] : r[e] + job.gamma * after - v[e];
                 after = v[e];
-                f.b = ends ? r[e] : r[e] + job.decay * f.b;
-                f.a = ends ? -1.0f : f.a < 0 ? f.a : fmaxf(f.a * job.decay, kLeast);
+                f.b = end ? r[e] : r[e] + job.decay * f.b;
+                f.a = end ? -1.0f : f.a < 0 ? f.a : fmaxf(f.a * job.decay, kLeast);
             }
         }
         int at;
@@ -170,7 +217,7 @@ __global__ __launch_bounds__(kThreads) void adv_tiles(Job job) {
 #pragma unroll
             for (int e = E - 1; e >= 0; e--) {
                 if (e < count) {
-                    x = end[e] != 0 ? r[e] : r[e] + job.decay * x;
+                    x = ends >> e & 1 ? r[e] : r[e] + job.decay * x;
                     r[e] = x;
                     v[e] += x;
                 }

@@ -12,11 +12,9 @@
  * comes before the sums with one read and no rescaling:
  *   up to 1,024 actions   G lanes of a wave to a row, by a rule on the
  *                         actions alone (with_small)
- *   up to 16,384          a workgroup to a row
- *   more                  a workgroup to a piece of 16,384, or of 4,096 where
- *                         the larger ones would not fill the chip; the pieces'
- *                         (m, S, sum z exp(z)) and best alternatives are
- *                         joined by a wave per row
+ *   more                  a workgroup to a row, or to a piece of one
+ *                         (pieces_of); the pieces' (m, S, sum z exp(z)) and
+ *                         best alternatives are joined by a wave per row
  * A lane loads W neighbouring logits at once; lanes take turns, so the order
  * of places is (load, lane, place in the load).
  */
@@ -26,10 +24,10 @@ namespace b3p {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / kWave;
-constexpr int kMaxActions = 1 << 22;
+constexpr int kMaxActions = 1 << 21;
 constexpr int kMaxPieces = 256;
 constexpr float kLog2e = 1.44269504f;
+constexpr float kLn2 = 0.693147181f;
 
 /* A logit, -inf where its action is not allowed. */
 template <typename T>
@@ -47,70 +45,177 @@ __device__ const unsigned char* mask_of(const B3Logits& g, int64_t r) {
 }
 
 /* The logits of a thread: places from + (v G + lane) W + w below `n`; -inf in
- * the others. */
+ * the others.  All loads are issued before the first is used: whole vectors
+ * first, then the elements of the one vector that passes n. */
 template <typename T, int G, int PER, int W>
-__device__ void load_logits(const T* row, const unsigned char* mask, int from, int n, int lane, float x[PER]) {
+__device__ __forceinline__ void load_logits(const T* row, const unsigned char* mask, int from, int n, int lane, float x[PER]) {
+    constexpr int NV = PER / W;
+    Pack<T, W> p[NV];
+    Pack<unsigned char, W> k[NV];
+    if (n - from >= G * PER) {
 #pragma unroll
-    for (int v = 0; v < PER / W; v++) {
+        for (int v = 0; v < NV; v++) p[v] = *(const Pack<T, W>*)(row + from + (v * G + lane) * W);
+        if (mask) {
+#pragma unroll
+            for (int v = 0; v < NV; v++) k[v] = *(const Pack<unsigned char, W>*)(mask + from + (v * G + lane) * W);
+        }
+#pragma unroll
+        for (int i = 0; i < PER; i++) x[i] = to_float(p[i / W].v[i % W]);
+        if (mask) {
+#pragma unroll
+            for (int i = 0; i < PER; i++) x[i] = k[i / W].v[i % W] ? x[i] : -INFINITY;
+        }
+        return;
+    }
+    const int last = (n - from) / (G * W);       // the load in which some lane passes n
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
         const int j = from + (v * G + lane) * W;
-        if (j + W <= n) {
-            Pack<T, W> p = *(const Pack<T, W>*)(row + j);
+        if (j + W <= n) p[v] = *(const Pack<T, W>*)(row + j);
+    }
+    if (mask) {
 #pragma unroll
-            for (int w = 0; w < W; w++) x[v * W + w] = to_float(p.v[w]);
-            if (mask) {
-                Pack<unsigned char, W> k = *(const Pack<unsigned char, W>*)(mask + j);
+        for (int v = 0; v < NV; v++) {
+            const int j = from + (v * G + lane) * W;
+            if (j + W <= n) k[v] = *(const Pack<unsigned char, W>*)(mask + j);
+        }
+    }
 #pragma unroll
-                for (int w = 0; w < W; w++) x[v * W + w] = k.v[w] ? x[v * W + w] : -INFINITY;
-            }
-        } else {
+    for (int v = 0; v < NV; v++) {
+        const int j = from + (v * G + lane) * W;
+        const bool whole = j + W <= n;
 #pragma unroll
-            for (int w = 0; w < W; w++) x[v * W + w] = j + w < n ? logit(row, mask, j + w) : -INFINITY;
+        for (int w = 0; w < W; w++) {
+            x[v * W + w] = whole ? to_float(p[v].v[w]) : -INFINITY;
+            if (mask) x[v * W + w] = whole && k[v].v[w] ? x[v * W + w] : -INFINITY;
+        }
+        if (v == last && !whole) {
+#pragma unroll
+            for (int w = 0; w < W; w++)
+                if (j + w < n) x[v * W + w] = logit(row, mask, j + w);
         }
     }
 }
 
-/* ---- reductions over the G threads that share a row ---- */
+/* One instruction for two elements; of a NaN and a number the number. */
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 
+/* ---- reductions ---- */
+
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ float from_lane(float x, float old) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(__float_as_uint(old), __float_as_uint(x), CONTROL, ROWS, 0xf, false));
+}
+
+__device__ __forceinline__ float last_lane(float x) {
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), kWave - 1));
+}
+
+/* Over a wave, the result in a scalar register: within rows of 16 lanes by
+ * shifts of 1, 2, 4 and 8, then from each row's last lane to the rows after
+ * it.  A lane that would read from outside takes the neutral value. */
+__device__ __forceinline__ float wave_sum(float x) {
+    x += from_lane<0x111, 0xf>(x, 0.0f);
+    x += from_lane<0x112, 0xf>(x, 0.0f);
+    x += from_lane<0x114, 0xf>(x, 0.0f);
+    x += from_lane<0x118, 0xf>(x, 0.0f);
+    x += from_lane<0x142, 0xa>(x, 0.0f);
+    x += from_lane<0x143, 0xc>(x, 0.0f);
+    return last_lane(x);
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+    x = max3(x, x, from_lane<0x111, 0xf>(x, x));
+    x = max3(x, x, from_lane<0x112, 0xf>(x, x));
+    x = max3(x, x, from_lane<0x114, 0xf>(x, x));
+    x = max3(x, x, from_lane<0x118, 0xf>(x, x));
+    x = max3(x, x, from_lane<0x142, 0xf>(x, x));
+    x = max3(x, x, from_lane<0x143, 0xf>(x, x));
+    return last_lane(x);
+}
+
+/* Over the G < 64 lanes that share a row. */
 template <int G, typename F>
-__device__ float reduce(float x, float* lds, F f) {
+__device__ __forceinline__ float group_reduce(float x, F f) {
 #pragma unroll
-    for (int d = 1; d < (G < kWave ? G : kWave); d *= 2) x = f(x, __shfl_xor(x, d));
-    if (G > kWave) {
-        if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = x;
-        __syncthreads();
-        x = f(f(lds[0], lds[1]), f(lds[2], lds[3]));
-        __syncthreads();
-    }
+    for (int d = 1; d < G; d *= 2) x = f(x, __shfl_xor(x, d));
     return x;
 }
 
-/* m, S and D = sum z exp(z) of a row or a piece.  m is 0 where nothing is
- * allowed, and where all that is allowed is NaN (S is then NaN). */
+/* m, S and D = sum z exp(z) of a row or a part of it.  m is 0 where nothing
+ * is allowed, and where all that is allowed is NaN (S is then NaN). */
 struct Sums {
     float m, s, d;
 };
 
-/* exp as 2^(z log2 e): the product is off by |z| 2^-24, and so is exp(z),
- * relative to itself; terms with |z| > 20 do not count.  z is bounded in D
- * alone, where 0 times -inf would be NaN. */
+template <int PER>
+__device__ __forceinline__ float lane_max(const float x[PER]) {
+    float m = max3(x[0], x[1], x[2]);
+#pragma unroll
+    for (int i = 3; i < PER; i += 2) m = max3(m, x[i], x[i + 1 < PER ? i + 1 : i]);
+    return m;
+}
+
+/* The sums over G <= 64 lanes of a row, from each lane's maximum.  exp(z) is
+ * 2^t with t = x log2 e - fl(m log2 e) in one rounding, which is z log2 e
+ * but for `off`, what fl() left out; it is the same for every term and taken
+ * back from the sums.  Beyond 2^16 it could be large, and t is formed from z.
+ * A term is off by |t| 2^-24, relative to itself; those with |t| > 30 do not
+ * count.  t is bounded in D alone, where 0 times -inf would be NaN. */
 template <int G, int PER>
-__device__ Sums sums_of(const float x[PER], float* lds) {
-    float m = x[0];
-#pragma unroll
-    for (int i = 1; i < PER; i++) m = fmaxf(m, x[i]);
-    m = reduce<G>(m, lds, [](float a, float b) { return fmaxf(a, b); });
+__device__ __forceinline__ Sums sums_of(const float x[PER], float lane_most) {
+    float m = G == kWave ? wave_max(lane_most)
+        : group_reduce<G>(lane_most, [](float a, float b) { return max3(a, b, b); });
     m = m == -INFINITY || m != m ? 0.0f : m;
-    float s = 0, d = 0;
+    float s = 0, d = 0, off = 0;
+    if (fabsf(m) <= 65536.0f) {
+        const float ml = m * kLog2e;
+        off = __builtin_fmaf(m, kLog2e, -ml);
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-        float z = x[i] - m, e = __builtin_amdgcn_exp2f(z * kLog2e);
-        s += e;
-        d = __builtin_fmaf(e, fmaxf(z, -1e4f), d);
+        for (int i = 0; i < PER; i++) {
+            const float t = __builtin_fmaf(x[i], kLog2e, -ml), e = __builtin_amdgcn_exp2f(t);
+            s += e;
+            d = __builtin_fmaf(e, fmaxf(t, -1e4f), d);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const float t = (x[i] - m) * kLog2e, e = __builtin_amdgcn_exp2f(t);
+            s += e;
+            d = __builtin_fmaf(e, fmaxf(t, -1e4f), d);
+        }
     }
-    auto add = [](float a, float b) { return a + b; };
-    s = reduce<G>(s, lds, add);
-    d = reduce<G>(d, lds, add);
-    return Sums{m, s, d};
+    if (G == kWave) {
+        s = wave_sum(s);
+        d = wave_sum(d);
+    } else {
+        auto add = [](float a, float b) { return a + b; };
+        s = group_reduce<G>(s, add);
+        d = group_reduce<G>(d, add);
+    }
+    const float back = __builtin_amdgcn_exp2f(-off);
+    return Sums{m, s * back, __builtin_fmaf(-off, s, d) * (back * kLn2)};
+}
+
+/* Two parts of a row as one.  A part that allows nothing has no say in m. */
+__device__ __forceinline__ Sums join(Sums a, Sums b) {
+    const float m = a.s == 0.0f ? b.m : b.s == 0.0f ? a.m : fmaxf(a.m, b.m);
+    const float za = a.m - m, zb = b.m - m;
+    const float ea = __builtin_amdgcn_exp2f(za * kLog2e), eb = __builtin_amdgcn_exp2f(zb * kLog2e);
+    Sums r = {m, 0.0f, 0.0f};
+    if (a.s != 0.0f) {
+        r.s += ea * a.s;
+        r.d += ea * (a.d + fmaxf(za, -1e4f) * a.s);
+    }
+    if (b.s != 0.0f) {
+        r.s += eb * b.s;
+        r.d += eb * (b.d + fmaxf(zb, -1e4f) * b.s);
+    }
+    return r;
 }
 
 struct Outputs {
@@ -160,12 +265,34 @@ __device__ void write_top(const Outputs& o, int64_t r, int k, uint32_t order, in
     o.top_action[r * o.top + k] = action;
 }
 
-__device__ uint32_t wave_max(uint32_t x) {
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-        uint32_t y = __shfl_xor(x, d);
-        x = x > y ? x : y;
-    }
+/* The wave's largest, in a scalar register: rows of 16 lanes by shifts, then
+ * each row's last lane to the next row.  Lanes that would read from outside
+ * keep what they have. */
+__device__ __forceinline__ uint32_t wave_most(uint32_t x) {
+    uint32_t y;
+    y = __builtin_amdgcn_update_dpp(x, x, 0x111, 0xf, 0xf, false);
+    x = x > y ? x : y;
+    y = __builtin_amdgcn_update_dpp(x, x, 0x112, 0xf, 0xf, false);
+    x = x > y ? x : y;
+    y = __builtin_amdgcn_update_dpp(x, x, 0x114, 0xf, 0xf, false);
+    x = x > y ? x : y;
+    y = __builtin_amdgcn_update_dpp(x, x, 0x118, 0xf, 0xf, false);
+    x = x > y ? x : y;
+    y = __builtin_amdgcn_update_dpp(x, x, 0x142, 0xf, 0xf, false);
+    x = x > y ? x : y;
+    y = __builtin_amdgcn_update_dpp(x, x, 0x143, 0xf, 0xf, false);
+    x = x > y ? x : y;
+    return __builtin_amdgcn_readlane(x, kWave - 1);
+}
+
+/* Over the lanes up to and with this one. */
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
     return x;
 }
 
@@ -190,7 +317,7 @@ __device__ void wave_top(uint32_t order[NV * W], int top, uint32_t& my_order, in
         uint32_t most = best[0];
 #pragma unroll
         for (int v = 1; v < NV; v++) most = most > best[v] ? most : best[v];
-        most = wave_max(most);
+        most = wave_most(most);
         bool found = false;
 #pragma unroll
         for (int v = 0; v < NV; v++) {
@@ -254,7 +381,7 @@ __global__ __launch_bounds__(kThreads) void lp_small(B3Logits g, Outputs o) {
     const int lane = threadIdx.x % G, n = (int)g.actions;
     float x[PER];
     load_logits<T, G, PER, W>(row_of<T>(g, r), mask_of(g, r), 0, n, lane, x);
-    const Sums s = sums_of<G, PER>(x, NULL);
+    const Sums s = sums_of<G, PER>(x, lane_max<PER>(x));
     const float log_sum = logf(s.s);
     if (lane == 0) finish_row<T>(g, o, r, s, log_sum);
     if (!o.top) return;
@@ -277,20 +404,89 @@ struct Pieces {
     uint2* top;                                  // [rows][count][top]: order, action
 };
 
+/* The lane's first place of a value, or none. */
+template <int THREADS, int PER, int W>
+__device__ int first_place(const float x[PER], float value, int from, int n) {
+    int place = INT32_MAX;
+#pragma unroll
+    for (int i = PER - 1; i >= 0; i--) {
+        const int j = from + ((i / W) * THREADS + (int)threadIdx.x) * W + i % W;
+        place = x[i] == value && j < n ? j : place;
+    }
+    return place;
+}
+
+/* A bound that `top` of the wave's logits reach: those over `order`, and of
+ * equals those up to `place`.  It is taken from the lanes' maxima, so that at
+ * most `top` lanes of the wave hold any logit that reaches it: bit by bit the
+ * largest order that `top` lanes reach (a smaller one that exactly `top`
+ * reach does as well), and if more do, because they are equal, the place up
+ * to which `top` do. */
+struct Bound {
+    uint32_t order;
+    int place;
+};
+
+template <int THREADS, int PER, int W>
+__device__ __forceinline__ Bound wave_bound(const float x[PER], float lane_most, int top, int from, int n) {
+    const uint32_t mine = order_of(lane_most), high = wave_most(mine), low = ~wave_most(~mine);
+    /* the bits that all lanes share, and then one after the other */
+    int bit = high == low ? -1 : 31 - __builtin_clz(high ^ low), reach = kWave;
+    uint32_t order = bit < 0 ? high : high & ~((2u << bit) - 1);
+    for (; bit >= 0 && reach != top; bit--) {
+        const uint32_t next = order | 1u << bit;
+        const int count = __builtin_popcountll(__ballot(mine >= next));
+        if (count >= top) {
+            order = next;
+            reach = count;
+        }
+    }
+    if (reach == top) return Bound{order, INT32_MAX};
+    const int need = top - __builtin_popcountll(__ballot(mine > order));
+    const int place = mine == order ? first_place<THREADS, PER, W>(x, value_of(order), from, n) : INT32_MAX;
+    int up_to = -1;                              // the largest that fewer than `need` do not pass
+    for (int bit = 30; bit >= 0; bit--) {
+        const int next = up_to + (1 << bit);
+        if (__builtin_popcountll(__ballot(place <= next)) < need) up_to = next;
+    }
+    return Bound{order, up_to == INT32_MAX - 1 ? INT32_MAX : up_to + 1};
+}
+
 /* A workgroup to a row (one piece) or to a piece of it.  TOP: whether
- * alternatives are asked for (what they take of registers would halve the
- * waves of a call that does not). */
-template <typename T, int PER, int W, bool TOP>
-__global__ __launch_bounds__(kThreads) void lp_piece(B3Logits g, Outputs o, Pieces p) {
-    __shared__ float lds[kWaves];
-    __shared__ uint2 found[kWaves][B3_MAX_TOP];
+ * alternatives are asked for.  Each wave finds a bound that `top` of its
+ * logits reach; what reaches the highest of these is listed in LDS, a few
+ * more than `top` as a rule, and a listed one's rank is the number of larger
+ * ones in the list.  Rows with a NaN or +inf, whose sums say so, and lists
+ * that would be too long (many large logits in one lane's places) go by
+ * wave_top, all waves' in the end ranked alike. */
+template <typename T, int THREADS, int PER, int W, bool TOP>
+__global__ __launch_bounds__(THREADS) void lp_piece(B3Logits g, Outputs o, Pieces p) {
+    constexpr int kWaves = THREADS / kWave, kList = 1024;
+    static_assert(PER <= 32, "a bit for each");
+    static_assert(kList >= kWaves * B3_MAX_TOP, "the waves' alternatives");
+    __shared__ Sums part[kWaves];
+    __shared__ Bound bounds[TOP ? kWaves : 1];
+    __shared__ uint2 list[TOP ? kList : 1];
+    __shared__ int listed;
     const int64_t r = blockIdx.x / (unsigned)p.count;
     const int piece = blockIdx.x % (unsigned)p.count;
     const int from = piece * p.size, end = from + p.size, n = end < g.actions ? end : (int)g.actions;
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     float x[PER];
-    load_logits<T, kThreads, PER, W>(row_of<T>(g, r), mask_of(g, r), from, n, threadIdx.x, x);
-    const Sums s = sums_of<kThreads, PER>(x, lds);
+    load_logits<T, THREADS, PER, W>(row_of<T>(g, r), mask_of(g, r), from, n, threadIdx.x, x);
+    const float most = lane_max<PER>(x);
+    const Sums mine = sums_of<kWave, PER>(x, most);
+    if (lane == 0) part[wave] = mine;
+    if (TOP) {
+        const Bound b = wave_bound<THREADS, PER, W>(x, most, o.top, from, n);
+        if (lane == 0) bounds[wave] = b;
+        if (threadIdx.x == 0) listed = 0;
+    }
+    __syncthreads();
+    if (!TOP && wave > 0) return;
+    Sums s = part[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) s = join(s, part[w]);
     const float log_sum = logf(s.s);
     if (threadIdx.x == 0) {
         if (p.count == 1)
@@ -299,33 +495,71 @@ __global__ __launch_bounds__(kThreads) void lp_piece(B3Logits g, Outputs o, Piec
             p.sums[r * p.count + piece] = s;
     }
     if (!TOP) return;
-    uint32_t order[PER], my_order;
-    int v, l, w;
+    Bound bound = bounds[0];
 #pragma unroll
-    for (int i = 0; i < PER; i++)
-        order[i] = from + ((i / W) * kThreads + (int)threadIdx.x) * W + i % W < n ? order_of(x[i]) : 0;
-    wave_top<PER / W, W>(order, o.top, my_order, v, l, w);
-    /* a wave of a short piece may have fewer than `top`: order 0 */
-    if (lane < o.top)
-        found[wave][lane] = make_uint2(my_order, from + (v * kThreads + wave * kWave + l) * W + w);
-    __syncthreads();
-    /* an alternative's place among the waves' is the number of larger ones */
-    for (int i = threadIdx.x; i < kWaves * o.top; i += kThreads) {
-        const uint2 mine = found[i / o.top][i % o.top];
-        if (mine.x == 0) continue;
-        int rank = i % o.top;
-        for (int u = 0; u < kWaves; u++) {
-            if (u == i / o.top) continue;
-            for (int k = 0; k < o.top; k++) {
-                const uint2 it = found[u][k];
-                rank += it.x > mine.x || (it.x == mine.x && it.y < mine.y);
+    for (int w = 1; w < kWaves; w++) {
+        const Bound b = bounds[w];
+        if (b.order > bound.order || (b.order == bound.order && b.place < bound.place)) bound = b;
+    }
+    const float value = value_of(bound.order);
+    int count = kList + 1;
+    if (s.s == s.s) {
+        uint32_t reaches = 0;                    // bit i: x[i]
+        if (most >= value) {
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const int j = from + ((i / W) * THREADS + (int)threadIdx.x) * W + i % W;
+                reaches |= (uint32_t)(x[i] >= value && j < n && (x[i] > value || j <= bound.place)) << i;
             }
+        }
+        if (__ballot(reaches != 0)) {
+            /* the wave's part of the list, and the lane's of that */
+            int before = __builtin_popcount(reaches);
+            const int own = before;
+            before = wave_scan(before);
+            int at = 0;
+            if (lane == kWave - 1) at = atomicAdd(&listed, before);
+            at = __builtin_amdgcn_readlane(at, kWave - 1) + before - own;
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                if (reaches >> i & 1) {
+                    if (at < kList) list[at] = make_uint2(order_of(x[i]), from + ((i / W) * THREADS + (int)threadIdx.x) * W + i % W);
+                    at++;
+                }
+            }
+        }
+        __syncthreads();
+        count = listed;
+    }
+    if (count > kList) {
+        __syncthreads();
+        uint32_t order[PER], my_order;
+        int v, l, w;
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+            order[i] = from + ((i / W) * THREADS + (int)threadIdx.x) * W + i % W < n ? order_of(x[i]) : 0;
+        wave_top<PER / W, W>(order, o.top, my_order, v, l, w);
+        /* a wave of a short piece may have fewer than `top`: order 0 */
+        if (lane < o.top)
+            list[wave * o.top + lane] = make_uint2(my_order, from + (v * THREADS + wave * kWave + l) * W + w);
+        __syncthreads();
+        count = kWaves * o.top;
+    }
+    for (int i = threadIdx.x; i < count; i += THREADS) {
+        const uint2 it = list[i];
+        if (it.x == 0) continue;
+        const uint64_t key = (uint64_t)it.x << 32 | ~it.y;
+        int rank = 0;
+#pragma unroll 8
+        for (int k = 0; k < count; k++) {
+            const uint2 other = list[k];
+            rank += ((uint64_t)other.x << 32 | ~other.y) > key;
         }
         if (rank >= o.top) continue;
         if (p.count == 1)
-            write_top(o, r, rank, mine.x, mine.y, s, log_sum);
+            write_top(o, r, rank, it.x, it.y, s, log_sum);
         else
-            p.top[(r * p.count + piece) * o.top + rank] = mine;
+            p.top[(r * p.count + piece) * o.top + rank] = it;
     }
     /* a piece of fewer than `top` actions fills its list up */
     const int have = n - from;
@@ -333,41 +567,32 @@ __global__ __launch_bounds__(kThreads) void lp_piece(B3Logits g, Outputs o, Piec
         p.top[(r * p.count + piece) * o.top + threadIdx.x] = make_uint2(0, 0);
 }
 
-/* A wave to a row: up to 256 pieces, four to a lane. */
+/* A wave to a row: up to 256 pieces, four to a lane.  With alternatives three
+ * more waves fetch the lists. */
 template <typename T>
-__global__ __launch_bounds__(kWave) void lp_join(B3Logits g, Outputs o, Pieces p) {
+__global__ __launch_bounds__(kThreads) void lp_join(B3Logits g, Outputs o, Pieces p) {
     constexpr int kHeads = kMaxPieces / kWave;
     extern __shared__ uint2 lists[];             // [count][top]
     const int64_t r = blockIdx.x;
     const int lane = threadIdx.x;
-    Sums part[kHeads];
-    float m = -INFINITY;
+    /* the pieces' lists are sorted, and of equal orders the one of the lower
+     * piece has the lower action */
+    for (int i = threadIdx.x; i < p.count * o.top; i += blockDim.x) lists[i] = p.top[r * p.count * o.top + i];
+    __syncthreads();
+    if (threadIdx.x >= kWave) return;
+    Sums part = {0, 0, 0};
 #pragma unroll
     for (int q = 0; q < kHeads; q++) {
         const int c = q * kWave + lane;
-        part[q] = c < p.count ? p.sums[r * p.count + c] : Sums{0, 0, 0};
-        /* a piece that allows nothing has no say */
-        m = part[q].s == 0.0f ? m : fmaxf(m, part[q].m);
+        if (c < p.count) part = join(part, p.sums[r * p.count + c]);
     }
-    m = reduce<kWave>(m, NULL, [](float a, float b) { return fmaxf(a, b); });
-    m = m == -INFINITY ? 0.0f : m;
-    float s = 0, d = 0;
 #pragma unroll
-    for (int q = 0; q < kHeads; q++) {
-        if (part[q].s == 0.0f) continue;
-        const float z = part[q].m - m, e = __builtin_amdgcn_exp2f(z * kLog2e);
-        s += e * part[q].s;
-        d += e * (part[q].d + fmaxf(z, -1e4f) * part[q].s);
-    }
-    auto add = [](float a, float b) { return a + b; };
-    const Sums all = {m, reduce<kWave>(s, NULL, add), reduce<kWave>(d, NULL, add)};
+    for (int d = 1; d < kWave; d *= 2)
+        part = join(part, Sums{__shfl_xor(part.m, d), __shfl_xor(part.s, d), __shfl_xor(part.d, d)});
+    const Sums all = part;
     const float log_sum = logf(all.s);
     if (lane == 0) finish_row<T>(g, o, r, all, log_sum);
     if (!o.top) return;
-    /* the pieces' lists are sorted, and of equal orders the one of the lower
-     * piece has the lower action */
-    for (int i = lane; i < p.count * o.top; i += kWave) lists[i] = p.top[r * p.count * o.top + i];
-    __syncthreads();
     uint2 head[kHeads];
     int next[kHeads];
 #pragma unroll
@@ -380,7 +605,7 @@ __global__ __launch_bounds__(kWave) void lp_join(B3Logits g, Outputs o, Pieces p
         uint32_t most = head[0].x;
 #pragma unroll
         for (int q = 1; q < kHeads; q++) most = most > head[q].x ? most : head[q].x;
-        most = wave_max(most);
+        most = wave_most(most);
         bool found = false;
 #pragma unroll
         for (int q = 0; q < kHeads; q++) {
@@ -492,7 +717,7 @@ void with_small(int64_t actions, F f) {
         f.template operator()<T, 64, 16, 16 / sizeof(T)>();
 }
 
-constexpr int kSmall = 1024, kPiece = 16384, kShortPiece = 4096;
+constexpr int kSmall = 1024, kShortPiece = 4096, kPiece = 8192, kWide = 16384;
 constexpr int64_t kFill = 512;                   // workgroups: two to a compute unit
 
 template <typename F>
@@ -505,11 +730,18 @@ void with_type(int type, F f) {
         f((__bf16)0);
 }
 
-/* Pieces of a row: none of them in workspace where there is one. */
+/* Pieces of a row.  8,192 actions to a workgroup of 256 are the fastest where
+ * rows are many (4,096 rows of 131,072 in bf16: 177 us; 16,384 to 512 threads
+ * 181 us, to 1,024 286 us), but for rows that 512 threads hold well filled,
+ * which save the join (16,384 rows of 16,384: 85 us, not 101; of 9,000: 106
+ * us, not 83).  Where pieces of 8,192 would not give every compute unit two,
+ * 4,096. */
 Pieces pieces_of(int64_t rows, int64_t actions) {
     Pieces p = {};
     p.size = kPiece;
-    if (actions > kShortPiece && rows * ceil_div(actions, kPiece) < kFill && ceil_div(actions, kShortPiece) <= kMaxPieces)
+    if (actions > kWide * 3 / 4 && actions <= kWide && rows >= kFill)
+        p.size = kWide;
+    else if (rows * ceil_div(actions, kPiece) < kFill && ceil_div(actions, kShortPiece) <= kMaxPieces)
         p.size = kShortPiece;
     p.count = actions <= kSmall ? 1 : (int)ceil_div(actions, p.size);
     return p;
@@ -535,12 +767,12 @@ struct SmallBackward {
     }
 };
 
-template <typename T, int PER, int W>
+template <typename T, int THREADS, int PER, int W>
 void launch_piece(const B3Logits& g, const Outputs& o, const Pieces& p, unsigned grid, hipStream_t stream) {
     if (o.top)
-        lp_piece<T, PER, W, true><<<grid, kThreads, 0, stream>>>(g, o, p);
+        lp_piece<T, THREADS, PER, W, true><<<grid, THREADS, 0, stream>>>(g, o, p);
     else
-        lp_piece<T, PER, W, false><<<grid, kThreads, 0, stream>>>(g, o, p);
+        lp_piece<T, THREADS, PER, W, false><<<grid, THREADS, 0, stream>>>(g, o, p);
 }
 
 template <typename T>
@@ -552,15 +784,15 @@ hipError_t forward(const B3Logits& g, const Outputs& o, Pieces p, hipStream_t st
     }
     const unsigned grid = (unsigned)(g.rows * p.count);
     const int64_t most = p.count == 1 ? g.actions : p.size;
-    if (most <= kThreads * 16)
-        launch_piece<T, 16, W>(g, o, p, grid, stream);
-    else if (most <= kThreads * 32)
-        launch_piece<T, 32, W>(g, o, p, grid, stream);
+    if (most <= kShortPiece)
+        launch_piece<T, 256, kShortPiece / 256, W>(g, o, p, grid, stream);
+    else if (most <= kPiece)
+        launch_piece<T, 256, kPiece / 256, W>(g, o, p, grid, stream);
     else
-        launch_piece<T, 64, W>(g, o, p, grid, stream);
+        launch_piece<T, 512, kWide / 512, W>(g, o, p, grid, stream);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess || p.count == 1) return err;
-    lp_join<T><<<(unsigned)g.rows, kWave, (size_t)p.count * o.top * sizeof(uint2), stream>>>(g, o, p);
+    lp_join<T><<<(unsigned)g.rows, o.top ? kThreads : kWave, (size_t)p.count * o.top * sizeof(uint2), stream>>>(g, o, p);
     return hipGetLastError();
 }
 

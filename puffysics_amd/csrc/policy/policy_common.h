@@ -41,7 +41,6 @@ struct __attribute__((packed, aligned(sizeof(T)))) Pack {
 inline __device__ float to_float(float x) { return x; }
 inline __device__ float to_float(_Float16 x) { return (float)x; }
 inline __device__ float to_float(__bf16 x) { return (float)x; }
-inline __device__ float to_float(uint8_t x) { return x; }
 
 inline bool is_float_type(int type) { return type == B3_F32 || type == B3_F16 || type == B3_BF16; }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
