@@ -24,6 +24,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxPieces = 512;
 constexpr int64_t kFill = 256;                   // workgroups: one to a compute unit
+constexpr int kWideCols = 64, kWideSteps = 16, kSteps = 8;
 
 /* x -> b + a x.  a < 0 stands for a map that drops x altogether, as a
  * terminal does: 0 times a NaN would not.  A product of rates stays over 0,
@@ -51,79 +52,82 @@ struct Job {
     Map* piece;                                  // [pieces][envs]
 };
 
+/* Keeps the compiler from forming all steps' addresses ahead: they would take
+ * more registers than the steps. */
+template <typename T>
+__device__ __forceinline__ void in_turn(T*& p) {
+    asm("" : "+v"(p));
+}
+
 /* Unsigned numbers that lie anywhere. */
 template <typename T, int N>
 struct __attribute__((packed, aligned(1))) Bytes {
     T v[N];
 };
 
-/* E steps' elements as they lie: in words of their own, or, where the steps
- * are neighbours, packed.  Nothing is done with them here, so that the loads
- * of all arrays are in flight together.  Steps from `count` (at least 1) on
- * give the last one's. */
-template <int E, typename T>
-__device__ __forceinline__ void load_raw(const T* p, int64_t stride, int count, bool packed, uint32_t raw[E]) {
+/* E steps' elements of SIZE bytes as they lie: in words of their own, or,
+ * where the steps are neighbours, packed.  Nothing is done with them here, so
+ * that the loads of all arrays are in flight together.  Steps from `count`
+ * (at least 1) on give the last one's. */
+template <int E, int SIZE>
+__device__ __forceinline__ void load_steps(const void* base, int64_t at, int64_t stride, int count, bool packed,
+    uint32_t raw[E]) {
+    const char* p = (const char*)base + at * SIZE;
     if (packed) {
-        constexpr int kWords = E * (int)sizeof(T) / 4, kVec = kWords < 4 ? kWords : 4;
+        constexpr int kWords = E * SIZE / 4, kVec = kWords < 4 ? kWords : 4;
 #pragma unroll
         for (int k = 0; k < kWords; k += kVec) {
-            Bytes<uint32_t, kVec> b = *(const Bytes<uint32_t, kVec>*)((const char*)p + 4 * k);
+            Bytes<uint32_t, kVec> b = *(const Bytes<uint32_t, kVec>*)(p + 4 * k);
 #pragma unroll
             for (int w = 0; w < kVec; w++) raw[k + w] = b.v[w];
         }
-    } else {
-#pragma unroll
-        for (int e = 0; e < E; e++) raw[e] = p[(e < count ? e : count - 1) * stride];
-    }
-}
-
-template <int E>
-__device__ __forceinline__ void load_steps(const void* p, int type, int64_t at, int64_t stride, int count, bool packed,
-    uint32_t raw[E]) {
-    if (type == B3_F32)
-        load_raw<E>((const uint32_t*)p + at, stride, count, packed, raw);
-    else if (type == B3_U8)
-        load_raw<E>((const uint8_t*)p + at, stride, count, packed, raw);
-    else
-        load_raw<E>((const uint16_t*)p + at, stride, count, packed, raw);
-}
-
-template <int E>
-__device__ __forceinline__ void floats_of(const uint32_t raw[E], int type, bool packed, float x[E]) {
-    if (type == B3_F32) {
-#pragma unroll
-        for (int e = 0; e < E; e++) x[e] = __uint_as_float(raw[e]);
         return;
     }
+    const int64_t step = stride * SIZE;
 #pragma unroll
     for (int e = 0; e < E; e++) {
-        const uint32_t h = packed ? raw[e / 2] >> (16 * (e % 2)) & 0xffffu : raw[e];
-        x[e] = type == B3_BF16 ? __uint_as_float(h << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+        raw[e] = SIZE == 4 ? *(const uint32_t*)p : SIZE == 2 ? *(const uint16_t*)p : *(const uint8_t*)p;
+        p += e + 1 < count ? step : 0;
+        in_turn(p);
     }
+}
+
+/* A value of TYPE as it lies. */
+template <int TYPE>
+__device__ __forceinline__ float float_of(uint32_t raw) {
+    return TYPE == B3_F32 ? __uint_as_float(raw)
+        : TYPE == B3_BF16 ? __uint_as_float(raw << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)raw);
+}
+
+template <int E, int TYPE>
+__device__ __forceinline__ void floats_of(const uint32_t raw[E], bool packed, float x[E]) {
+#pragma unroll
+    for (int e = 0; e < E; e++)
+        x[e] = float_of<TYPE>(TYPE != B3_F32 && packed ? raw[e / 2] >> (16 * (e % 2)) & 0xffffu : raw[e]);
 }
 
 /* Bit e: step e ends an episode. */
-template <int E>
-__device__ __forceinline__ uint32_t ends_of(const uint32_t raw[E], int type, bool packed) {
+template <int E, int TYPE>
+__device__ __forceinline__ uint32_t ends_of(const uint32_t raw[E], bool packed) {
     uint32_t bits = 0;
 #pragma unroll
     for (int e = 0; e < E; e++) {
-        const uint32_t h = type == B3_F32 ? raw[e] & 0x7fffffffu
+        const uint32_t h = TYPE == B3_F32 ? raw[e] & 0x7fffffffu
             : packed ? raw[e / 4] >> (8 * (e % 4)) & 0xffu : raw[e];
         bits |= (h != 0) << e;
     }
     return bits;
 }
 
-__device__ float load_one(const void* p, int type, int64_t at) {
-    return type == B3_F32 ? ((const float*)p)[at]
-        : type == B3_BF16 ? to_float(((const __bf16*)p)[at]) : to_float(((const _Float16*)p)[at]);
+template <int TYPE>
+__device__ __forceinline__ float load_one(const void* p, int64_t at) {
+    return float_of<TYPE>(TYPE == B3_F32 ? ((const uint32_t*)p)[at] : ((const uint16_t*)p)[at]);
 }
 
 /* BY_ENV: neighbouring threads have neighbouring environments, else
  * neighbouring segments.  SUM: compose the piece and write its map; else
  * write the advantages. */
-template <bool BY_ENV, int COLS, int E, bool SUM>
+template <int VALUES, int ENDS, bool BY_ENV, int COLS, int E, bool SUM>
 __global__ __launch_bounds__(kThreads) void adv_tiles(Job job) {
     constexpr int SEGS = kThreads / COLS;
     __shared__ Map lds[2][kThreads];
@@ -172,6 +176,7 @@ __global__ __launch_bounds__(kThreads) void adv_tiles(Job job) {
     }
     Map total = {1, 0};                          // of the piece's tiles so far
 
+#pragma unroll 1
     while (--tile >= first) {
         const int64_t t = (tile * SEGS + seg) * E;
         const int64_t left = live ? g.steps - t : 0;
@@ -181,18 +186,18 @@ __global__ __launch_bounds__(kThreads) void adv_tiles(Job job) {
         if (count) {
             const bool packed = job.wide && count == E;
             uint32_t raw_r[E], raw_v[E], raw_end[E];
-            load_steps<E>(g.rewards, B3_F32, env * g.rewards_stride[1] + t * g.rewards_stride[0], g.rewards_stride[0], count,
+            load_steps<E, 4>(g.rewards, env * g.rewards_stride[1] + t * g.rewards_stride[0], g.rewards_stride[0], count,
                 packed, raw_r);
-            load_steps<E>(g.terminals, g.terminals_type, env * g.terminals_stride[1] + t * g.terminals_stride[0],
+            load_steps<E, ENDS == B3_F32 ? 4 : 1>(g.terminals, env * g.terminals_stride[1] + t * g.terminals_stride[0],
                 g.terminals_stride[0], count, packed, raw_end);
-            load_steps<E>(g.values, g.values_type, env * g.values_stride[1] + t * g.values_stride[0], g.values_stride[0],
-                count, packed, raw_v);
+            load_steps<E, VALUES == B3_F32 ? 4 : 2>(g.values, env * g.values_stride[1] + t * g.values_stride[0],
+                g.values_stride[0], count, packed, raw_v);
             after = t + count < g.steps
-                ? load_one(g.values, g.values_type, env * g.values_stride[1] + (t + count) * g.values_stride[0])
-                : load_one(g.last_values, g.values_type, env * g.last_values_stride);
-            floats_of<E>(raw_r, B3_F32, packed, r);
-            floats_of<E>(raw_v, g.values_type, packed, v);
-            ends = ends_of<E>(raw_end, g.terminals_type, packed);
+                ? load_one<VALUES>(g.values, env * g.values_stride[1] + (t + count) * g.values_stride[0])
+                : load_one<VALUES>(g.last_values, env * g.last_values_stride);
+            floats_of<E, B3_F32>(raw_r, packed, r);
+            floats_of<E, VALUES>(raw_v, packed, v);
+            ends = ends_of<E, ENDS>(raw_end, packed);
         }
         /* r becomes d; the map of the segment */
         Map f = {1, 0};
@@ -230,12 +235,18 @@ __global__ __launch_bounds__(kThreads) void adv_tiles(Job job) {
                     *(Pack<float, 4>*)(g.returns + o + 4 * k) = Pack<float, 4>{v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]};
                 }
             } else {
+                float* adv = g.advantages + o;
+                float* ret = g.returns + o;
 #pragma unroll
                 for (int e = 0; e < E; e++) {
                     if (e < count) {
-                        g.advantages[o + e * g.out_stride[0]] = r[e];
-                        g.returns[o + e * g.out_stride[0]] = v[e];
+                        *adv = r[e];
+                        *ret = v[e];
                     }
+                    adv += g.out_stride[0];
+                    ret += g.out_stride[0];
+                    in_turn(adv);
+                    in_turn(ret);
                 }
             }
         }
@@ -256,8 +267,8 @@ Plan plan_of(int64_t steps, int64_t envs, bool by_env) {
     Plan p;
     p.by_env = by_env;
     if (by_env) {
-        p.cols = envs >= 64 * kFill ? 64 : 16;
-        p.steps = envs >= 64 * kFill ? 16 : 8;
+        p.cols = envs >= kWideCols * kFill ? kWideCols : 16;
+        p.steps = p.cols == 16 ? kSteps : kWideSteps;
     } else {
         p.cols = steps <= 64 ? 64 : steps <= 512 ? 16 : 1;
         p.steps = 16;
@@ -279,16 +290,31 @@ Plan plan_of(int64_t steps, int64_t envs, bool by_env) {
  * takes side by side leave its lanes to the steps. */
 bool by_env(const B3Rollout& g) { return g.envs >= 16 && g.out_stride[1] <= g.out_stride[0]; }
 
-template <bool BY_ENV, int COLS, int E>
+template <int VALUES, int ENDS, bool BY_ENV, int COLS, int E>
 hipError_t launch(const Job& job, const Plan& p, hipStream_t stream) {
     const unsigned grid = (unsigned)(p.blocks * p.pieces);
     if (p.pieces > 1) {
-        adv_tiles<BY_ENV, COLS, E, true><<<grid, kThreads, 0, stream>>>(job);
+        adv_tiles<VALUES, ENDS, BY_ENV, COLS, E, true><<<grid, kThreads, 0, stream>>>(job);
         hipError_t err = hipGetLastError();
         if (err != hipSuccess) return err;
     }
-    adv_tiles<BY_ENV, COLS, E, false><<<grid, kThreads, 0, stream>>>(job);
+    adv_tiles<VALUES, ENDS, BY_ENV, COLS, E, false><<<grid, kThreads, 0, stream>>>(job);
     return hipGetLastError();
+}
+
+template <int VALUES, int ENDS>
+hipError_t launch_plan(const Job& job, const Plan& p, hipStream_t stream) {
+    if (p.by_env)
+        return p.cols == kWideCols ? launch<VALUES, ENDS, true, kWideCols, kWideSteps>(job, p, stream)
+                                   : launch<VALUES, ENDS, true, 16, kSteps>(job, p, stream);
+    return p.cols == 64 ? launch<VALUES, ENDS, false, 64, 16>(job, p, stream)
+        : p.cols == 16 ? launch<VALUES, ENDS, false, 16, 16>(job, p, stream) : launch<VALUES, ENDS, false, 1, 16>(job, p, stream);
+}
+
+template <int VALUES>
+hipError_t launch_values(const Job& job, const Plan& p, hipStream_t stream) {
+    return job.g.terminals_type == B3_F32 ? launch_plan<VALUES, B3_F32>(job, p, stream)
+                                          : launch_plan<VALUES, B3_U8>(job, p, stream);
 }
 
 bool valid(const B3Rollout& g) {
@@ -327,10 +353,8 @@ hipError_t b3_advantages_gpu(const B3Rollout* g, double gamma, double lambda, vo
     const bool wide = g->rewards_stride[0] == 1 && g->values_stride[0] == 1 && g->terminals_stride[0] == 1
         && g->out_stride[0] == 1;
     const Job job = {*g, (float)gamma, (float)(gamma * lambda), wide, p.tiles, p.pieces, (Map*)workspace};
-    if (p.by_env)
-        return p.cols == 64 ? launch<true, 64, 16>(job, p, stream) : launch<true, 16, 8>(job, p, stream);
-    return p.cols == 64 ? launch<false, 64, 16>(job, p, stream)
-        : p.cols == 16 ? launch<false, 16, 16>(job, p, stream) : launch<false, 1, 16>(job, p, stream);
+    return g->values_type == B3_F32 ? launch_values<B3_F32>(job, p, stream)
+        : g->values_type == B3_F16 ? launch_values<B3_F16>(job, p, stream) : launch_values<B3_BF16>(job, p, stream);
 }
 
 }  // extern "C"
