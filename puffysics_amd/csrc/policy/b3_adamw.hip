@@ -5,12 +5,15 @@
  * The tensors are cut into chunks of kChunk elements; a table of chunks made
  * once says whose each is.  A launch takes the gradients of up to kBatch
  * tensors as kernel arguments, so that a step copies nothing to the device.
- * The step is one pass: a workgroup to a chunk, a thread's loads of two
- * vectors of everything issued before the first is used.  It is bound by
- * memory (28 bytes a weight in 32 bits).  With a clip the norm is summed
- * first, by at most kSumBlocks workgroups a launch over their chunks in turn;
- * few partial sums are added by the step itself, many by a launch of their
- * own.  Sums go in one order always.
+ * The step is one pass: a thread's loads of a vector of everything are issued
+ * before the first is used.  It is bound by memory (28 bytes a weight in 32
+ * bits), and what it moves goes past the caches: 400 million weights take
+ * 1,872 us so (6.0 TB/s), and took 2,049 us through them.  With a clip the
+ * norm is summed first, by at most kSumBlocks workgroups a launch over their
+ * chunks in turn, through the caches, which keep gradients of a moderate size
+ * for the step (100 million in bf16: 458 us, 478 us past them); few partial
+ * sums are added by the step itself, many by a launch of their own.  Sums go
+ * in one order always.
  */
 #include "policy_common.h"
 
@@ -20,9 +23,7 @@ namespace b3p {
 
 constexpr int kThreads = 256;
 constexpr int kVector = 4;                       // elements a thread loads at once
-constexpr int kUnroll = 2;                       // vectors of a thread in flight
 constexpr int kChunk = 4096;
-constexpr int kTurn = kThreads * kVector * kUnroll;
 constexpr int kSumBlocks = 2048;
 constexpr int kBatch = 160;                      // tensors to a launch: 4,000 bytes of arguments
 constexpr int kGroup = 32;                       // 8-bit moments: elements to a scale
@@ -54,6 +55,17 @@ struct Moments {
     uint8_t* exp_avg_scale;
     uint8_t* exp_avg_sq_scale;
     float* master;
+};
+
+/* Workgroups to a chunk, and vectors of a thread in flight.  In 32 bits four
+ * workgroups of one vector a thread: 400 million weights took 2,061 us, and
+ * 2,109 us as one workgroup that goes on twice over two vectors; 30 million
+ * in bf16 155 and 171 us.  With 8-bit moments, where a vector's work is four
+ * times as long, the other way about: 200 million weights 660 and 602 us. */
+template <int BITS>
+struct Shape {
+    static constexpr int kParts = BITS == 32 ? 4 : 1, kUnroll = BITS == 32 ? 1 : 2;
+    static constexpr int kTurn = kThreads * kVector * kUnroll, kPart = kChunk / kParts;
 };
 
 struct Rates {
@@ -89,11 +101,11 @@ inline __host__ __device__ uint32_t mix(uint32_t x) {
     return x ^ x >> 16;
 }
 
-/* FULL: no element passes the tensor's end. */
-template <bool FULL, typename T>
+/* FULL: no element passes the tensor's end.  ONCE: not to be read again. */
+template <bool FULL, bool ONCE, typename T>
 __device__ void load(const T* p, int64_t i, int64_t n, float x[kVector]) {
     if (FULL || i + kVector <= n) {
-        Pack<T, kVector> v = *(const Pack<T, kVector>*)(p + i);
+        Pack<T, kVector> v = ONCE ? Stream<T, kVector>::load(p + i) : *(const Pack<T, kVector>*)(p + i);
 #pragma unroll
         for (int k = 0; k < kVector; k++) x[k] = to_float(v.v[k]);
     } else {
@@ -108,7 +120,7 @@ __device__ void store(T* p, int64_t i, int64_t n, const float x[kVector]) {
         Pack<T, kVector> v;
 #pragma unroll
         for (int k = 0; k < kVector; k++) v.v[k] = (T)x[k];
-        *(Pack<T, kVector>*)(p + i) = v;
+        Stream<T, kVector>::store(p + i, v);
     } else {
 #pragma unroll
         for (int k = 0; k < kVector; k++)
@@ -201,11 +213,12 @@ struct Step {
     uint32_t key;
 };
 
-/* kUnroll vectors of a thread.  The square root is the correctly rounded one,
+/* The vectors of a thread that are in flight together.  The square root is the correctly rounded one,
  * since what is kept of it is cut off by random bits; the division in the
  * update is a reciprocal, good to two units. */
 template <typename P, typename G, bool MASTER, int BITS, bool FULL>
 __device__ __forceinline__ void step_turn(const Tensor& t, int64_t from, const G* grad, const Step& s) {
+    constexpr int kUnroll = Shape<BITS>::kUnroll;
     float g[kUnroll][kVector], w[kUnroll][kVector], m[kUnroll][kVector], v[kUnroll][kVector];
     uint32_t cm[kUnroll], cv[kUnroll];
     uint8_t sm[kUnroll], sv[kUnroll];
@@ -215,14 +228,14 @@ __device__ __forceinline__ void step_turn(const Tensor& t, int64_t from, const G
         const int64_t i = from + (u * kThreads + (int)threadIdx.x) * kVector, at = t.at + i;
         /* whole groups of 8-bit moments go on together */
         if (!FULL && i / kGroup * kGroup >= n) continue;
-        load<FULL>(grad, i, n, g[u]);
+        load<FULL, true>(grad, i, n, g[u]);
         if (MASTER)
-            load<FULL>(s.mo.master + t.at, i, n, w[u]);
+            load<FULL, true>(s.mo.master + t.at, i, n, w[u]);
         else
-            load<FULL>((const P*)t.param, i, n, w[u]);
+            load<FULL, true>((const P*)t.param, i, n, w[u]);
         if (BITS == 32) {
-            load<FULL>((const float*)s.mo.exp_avg + t.at, i, n, m[u]);
-            load<FULL>((const float*)s.mo.exp_avg_sq + t.at, i, n, v[u]);
+            load<FULL, true>((const float*)s.mo.exp_avg + t.at, i, n, m[u]);
+            load<FULL, true>((const float*)s.mo.exp_avg_sq + t.at, i, n, v[u]);
         } else {
             cm[u] = *(const uint32_t*)((const uint8_t*)s.mo.exp_avg + at);
             cv[u] = *(const uint32_t*)((const uint8_t*)s.mo.exp_avg_sq + at);
@@ -267,10 +280,12 @@ __device__ __forceinline__ void step_turn(const Tensor& t, int64_t from, const G
 
 template <typename P, typename G, bool MASTER, int BITS>
 __device__ __forceinline__ void step_chunk(const Tensor& t, int64_t from, const G* grad, const Step& s) {
-    if (from + kChunk <= t.numel) {
-        for (int64_t i = from; i < from + kChunk; i += kTurn) step_turn<P, G, MASTER, BITS, true>(t, i, grad, s);
+    constexpr int kTurn = Shape<BITS>::kTurn;
+    const int64_t end = from + Shape<BITS>::kPart;
+    if (end <= t.numel) {
+        for (int64_t i = from; i < end; i += kTurn) step_turn<P, G, MASTER, BITS, true>(t, i, grad, s);
     } else {
-        for (int64_t i = from; i < t.numel; i += kTurn) step_turn<P, G, MASTER, BITS, false>(t, i, grad, s);
+        for (int64_t i = from; i < end && i < t.numel; i += kTurn) step_turn<P, G, MASTER, BITS, false>(t, i, grad, s);
     }
 }
 
@@ -319,12 +334,14 @@ __global__ __launch_bounds__(kThreads) void aw_step(StepArgs a, int base, int64_
     } else if (clip.scale) {
         scale = *clip.scale;
     }
-    const int2 c = chunk[first + blockIdx.x];
+    constexpr int kParts = Shape<BITS>::kParts;
+    const int2 c = chunk[first + blockIdx.x / kParts];
     const int at = c.x - base;
     const void* grad = a.grad[at];
     if (!grad) return;
     const Tensor t = tensors[c.x];
-    const int64_t from = (int64_t)c.y * kChunk;
+    const int64_t from = (int64_t)c.y * kChunk + blockIdx.x % kParts * Shape<BITS>::kPart;
+    if (from >= t.numel) return;
     const Step s = {mo, k, inverse, scale, a.size[at], a.root[at], a.keep[at], a.key[at]};
     const bool fg = a.grad_type[at] == B3_F32;
     if (t.type == B3_F32)
@@ -348,7 +365,7 @@ __device__ float squares(const G* grad, int64_t from, int64_t n) {
     float g[kChunk / (kThreads * kVector)][kVector], sum = 0;
 #pragma unroll
     for (int u = 0; u < kChunk / (kThreads * kVector); u++)
-        load<FULL>(grad, from + (int64_t)(u * kThreads + (int)threadIdx.x) * kVector, n, g[u]);
+        load<FULL, false>(grad, from + (int64_t)(u * kThreads + (int)threadIdx.x) * kVector, n, g[u]);
 #pragma unroll
     for (int u = 0; u < kChunk / (kThreads * kVector); u++)
 #pragma unroll
@@ -407,8 +424,8 @@ __global__ __launch_bounds__(kThreads) void aw_load(Moments mo, int64_t size, co
     const int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * kVector;
     if (i >= size) return;                        // a multiple of 256: groups stay whole
     float m[kVector], r[kVector];
-    load<true>(exp_avg, i, size, m);
-    load<true>(exp_avg_sq, i, size, r);
+    load<true, true>(exp_avg, i, size, m);
+    load<true, true>(exp_avg_sq, i, size, r);
     for (int k = 0; k < kVector; k++) r[k] = sqrtf(r[k]);
     const uint32_t none[kVector] = {0, 0, 0, 0};
     uint32_t sm = group_scale(m), sr = group_scale(r);
@@ -487,7 +504,7 @@ hipError_t b3_adamw_create(B3AdamW** out, const B3AdamWTensor* tensors, int coun
             || (state.bits == 8 && (!state.exp_avg_scale || !state.exp_avg_sq_scale))))
         return hipErrorInvalidValue;
     for (int i = 0; i < count; i++) chunks += ceil_div(tensors[i].numel, kChunk);
-    if (chunks > 0x7fffffff) return hipErrorInvalidValue;
+    if (chunks > 0x7fffffff / Shape<32>::kParts) return hipErrorInvalidValue;
     B3AdamW* o = (B3AdamW*)calloc(1, sizeof(B3AdamW));
     if (!o) return hipErrorOutOfMemory;
     o->count = count;
@@ -580,10 +597,10 @@ hipError_t b3_adamw_step_gpu(B3AdamW* o, const void* const* grads, const int* gr
                 aw_squares<<<blocks, kThreads, 0, stream>>>(a, base, first, end, o->chunk, o->tensors, partial);
                 partial += blocks;
             } else if (o->bits == 32) {
-                aw_step<32><<<(unsigned)(end - first), kThreads, 0, stream>>>(a, base, first, o->chunk, o->tensors,
+                aw_step<32><<<(unsigned)((end - first) * Shape<32>::kParts), kThreads, 0, stream>>>(a, base, first, o->chunk, o->tensors,
                     o->moments, rates, o->inverse, clip);
             } else {
-                aw_step<8><<<(unsigned)(end - first), kThreads, 0, stream>>>(a, base, first, o->chunk, o->tensors,
+                aw_step<8><<<(unsigned)((end - first) * Shape<8>::kParts), kThreads, 0, stream>>>(a, base, first, o->chunk, o->tensors,
                     o->moments, rates, o->inverse, clip);
             }
             if ((err = hipGetLastError()) != hipSuccess) return err;

@@ -46,15 +46,22 @@ __device__ const unsigned char* mask_of(const B3Logits& g, int64_t r) {
 
 /* The logits of a thread: places from + (v G + lane) W + w below `n`; -inf in
  * the others.  All loads are issued before the first is used: whole vectors
- * first, then the elements of the one vector that passes n. */
+ * first, then the elements of the one vector that passes n.  `once`: past the
+ * caches (see stream_logits). */
 template <typename T, int G, int PER, int W>
-__device__ __forceinline__ void load_logits(const T* row, const unsigned char* mask, int from, int n, int lane, float x[PER]) {
+__device__ __forceinline__ void load_logits(const T* row, const unsigned char* mask, int from, int n, int lane, bool once,
+    float x[PER]) {
     constexpr int NV = PER / W;
     Pack<T, W> p[NV];
     Pack<unsigned char, W> k[NV];
     if (n - from >= G * PER) {
+        if (once) {
 #pragma unroll
-        for (int v = 0; v < NV; v++) p[v] = *(const Pack<T, W>*)(row + from + (v * G + lane) * W);
+            for (int v = 0; v < NV; v++) p[v] = Stream<T, W>::load(row + from + (v * G + lane) * W);
+        } else {
+#pragma unroll
+            for (int v = 0; v < NV; v++) p[v] = *(const Pack<T, W>*)(row + from + (v * G + lane) * W);
+        }
         if (mask) {
 #pragma unroll
             for (int v = 0; v < NV; v++) k[v] = *(const Pack<unsigned char, W>*)(mask + from + (v * G + lane) * W);
@@ -380,7 +387,7 @@ __global__ __launch_bounds__(kThreads) void lp_small(B3Logits g, Outputs o) {
     if (r >= g.rows) return;                     // all G lanes of it
     const int lane = threadIdx.x % G, n = (int)g.actions;
     float x[PER];
-    load_logits<T, G, PER, W>(row_of<T>(g, r), mask_of(g, r), 0, n, lane, x);
+    load_logits<T, G, PER, W>(row_of<T>(g, r), mask_of(g, r), 0, n, lane, false, x);
     const Sums s = sums_of<G, PER>(x, lane_max<PER>(x));
     const float log_sum = logf(s.s);
     if (lane == 0) finish_row<T>(g, o, r, s, log_sum);
@@ -400,6 +407,7 @@ __global__ __launch_bounds__(kThreads) void lp_small(B3Logits g, Outputs o) {
 /* A piece's sums and alternatives, in the caller's workspace. */
 struct Pieces {
     int count, size;                             // pieces of a row, actions of a piece
+    bool once;
     Sums* sums;                                  // [rows][count]
     uint2* top;                                  // [rows][count][top]: order, action
 };
@@ -473,7 +481,7 @@ __global__ __launch_bounds__(THREADS) void lp_piece(B3Logits g, Outputs o, Piece
     const int from = piece * p.size, end = from + p.size, n = end < g.actions ? end : (int)g.actions;
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     float x[PER];
-    load_logits<T, THREADS, PER, W>(row_of<T>(g, r), mask_of(g, r), from, n, threadIdx.x, x);
+    load_logits<T, THREADS, PER, W>(row_of<T>(g, r), mask_of(g, r), from, n, threadIdx.x, p.once, x);
     const float most = lane_max<PER>(x);
     const Sums mine = sums_of<kWave, PER>(x, most);
     if (lane == 0) part[wave] = mine;
@@ -635,6 +643,7 @@ struct Upstream {
     int64_t d_entropy_stride;
     void* out;
     int64_t row_stride;
+    bool once;
 };
 
 struct RowGradient {
@@ -668,7 +677,7 @@ __device__ void backward_row(const B3Logits& g, const Upstream& u, int64_t r, in
     const RowGradient q = row_gradient(u, r, g.actions);
     const int n = (int)g.actions;
     float x[PER];
-    load_logits<T, G, PER, W>(row_of<T>(g, r), mask_of(g, r), from, n, lane, x);
+    load_logits<T, G, PER, W>(row_of<T>(g, r), mask_of(g, r), from, n, lane, u.once, x);
     T* out = (T*)u.out + r * u.row_stride;
 #pragma unroll
     for (int v = 0; v < PER / W; v++) {
@@ -677,7 +686,7 @@ __device__ void backward_row(const B3Logits& g, const Upstream& u, int64_t r, in
 #pragma unroll
         for (int w = 0; w < W; w++) p.v[w] = (T)gradient_of(q, x[v * W + w], j + w == q.a);
         if (j + W <= n) {
-            *(Pack<T, W>*)(out + j) = p;
+            Stream<T, W>::store(out + j, p);
         } else {
 #pragma unroll
             for (int w = 0; w < W; w++)
@@ -702,19 +711,21 @@ __global__ __launch_bounds__(kThreads) void lp_piece_backward(B3Logits g, Upstre
 /* ---- launches ---- */
 
 /* Calls f with the shape for rows of up to 1,024 actions: the fewest lanes
- * that hold them at four each (16 each beyond 256). */
+ * that hold them at 16 each, since what is done once a row is shared by few
+ * elements already; four in a lane where that is all. */
 template <typename T, typename F>
 void with_small(int64_t actions, F f) {
+    constexpr int W = 16 / sizeof(T);
     if (actions <= 4)
         f.template operator()<T, 1, 4, 4>();
     else if (actions <= 16)
-        f.template operator()<T, 4, 4, 4>();
+        f.template operator()<T, 1, 16, W>();
     else if (actions <= 64)
-        f.template operator()<T, 16, 4, 4>();
+        f.template operator()<T, 4, 16, W>();
     else if (actions <= 256)
-        f.template operator()<T, 64, 4, 4>();
+        f.template operator()<T, 16, 16, W>();
     else
-        f.template operator()<T, 64, 16, 16 / sizeof(T)>();
+        f.template operator()<T, 64, 16, W>();
 }
 
 constexpr int kSmall = 1024, kShortPiece = 4096, kPiece = 8192, kWide = 16384;
@@ -729,6 +740,12 @@ void with_type(int type, F f) {
     else
         f((__bf16)0);
 }
+
+/* Logits that the caches cannot hold from the forward pass to the backward go
+ * past them (4,096 rows of 131,072 in bf16: 161 and 350 us forward and
+ * backward, not 178 and 363); smaller ones do not (8,192 rows of 1,024: 11.1
+ * us for both passes, 12.4 us past the caches). */
+bool stream_logits(const B3Logits& g) { return g.rows * g.actions * (g.type == B3_F32 ? 4 : 2) > (int64_t)1 << 28; }
 
 /* Pieces of a row.  8,192 actions to a workgroup of 256 are the fastest where
  * rows are many (4,096 rows of 131,072 in bf16: 177 us; 16,384 to 512 threads
@@ -837,6 +854,7 @@ hipError_t b3_log_probs_gpu(B3Logits g, const int64_t* taken, float* log_prob, f
     if (!log_prob || !entropy || (top && (!top_log_prob || !top_action))) return hipErrorInvalidValue;
     const Outputs o = {taken, log_prob, entropy, stats, top, top_log_prob, top_action};
     Pieces p = pieces_of(g.rows, g.actions);
+    p.once = stream_logits(g);
     p.top = (uint2*)workspace;
     p.sums = (Sums*)((char*)workspace + (size_t)g.rows * p.count * top * sizeof(uint2));
     hipError_t err = hipSuccess;
@@ -850,7 +868,8 @@ hipError_t b3_log_probs_backward_gpu(B3Logits g, const int64_t* taken, const flo
     if (!valid(g, taken) || d_row_stride < g.actions || dl_stride < 0 || dh_stride < 0) return hipErrorInvalidValue;
     if (g.rows == 0) return hipSuccess;
     if (!stats || !entropy || !d_logits) return hipErrorInvalidValue;
-    const Upstream u = {taken, stats, entropy, d_log_prob, dl_stride, d_entropy, dh_stride, d_logits, d_row_stride};
+    const Upstream u = {taken, stats, entropy, d_log_prob, dl_stride, d_entropy, dh_stride, d_logits, d_row_stride,
+        stream_logits(g)};
     hipError_t err = hipSuccess;
     with_type(g.type, [&](auto t) { err = backward<decltype(t)>(g, u, stream); });
     return err;

@@ -38,6 +38,19 @@ struct __attribute__((packed, aligned(sizeof(T)))) Pack {
     T v[N];
 };
 
+/* The same for data that is used once: not kept in the caches.  N elements
+ * are 4, 8 or 16 bytes. */
+template <typename T, int N>
+struct Stream {
+    typedef uint32_t Words __attribute__((ext_vector_type(sizeof(T) * N / 4), aligned(sizeof(T))));
+    static __device__ __forceinline__ Pack<T, N> load(const T* p) {
+        return __builtin_bit_cast(Pack<T, N>, __builtin_nontemporal_load((const Words*)p));
+    }
+    static __device__ __forceinline__ void store(T* p, Pack<T, N> v) {
+        __builtin_nontemporal_store(__builtin_bit_cast(Words, v), (Words*)p);
+    }
+};
+
 inline __device__ float to_float(float x) { return x; }
 inline __device__ float to_float(_Float16 x) { return (float)x; }
 inline __device__ float to_float(__bf16 x) { return (float)x; }
