@@ -326,22 +326,21 @@ struct Clip {
 template <int BITS>
 __global__ __launch_bounds__(kThreads) void aw_step(StepArgs a, int base, int64_t first, const int2* chunk,
     const Tensor* tensors, Moments mo, Rates k, const float* inverse, Clip clip) {
-    float scale = 1.0f;
-    if (clip.partial) {
-        const float norm = (float)sqrt(block_sum<kThreads>((int)threadIdx.x < clip.partials ? clip.partial[threadIdx.x] : 0));
-        if (first + blockIdx.x == 0 && threadIdx.x == 0) *clip.norm = norm;
-        scale = clip_of(norm, clip.max_norm);
-    } else if (clip.scale) {
-        scale = *clip.scale;
-    }
     constexpr int kParts = Shape<BITS>::kParts;
+    /* fetched together: the sums of squares and whose chunk it is */
+    const double part = clip.partial && (int)threadIdx.x < clip.partials ? clip.partial[threadIdx.x] : 0;
     const int2 c = chunk[first + blockIdx.x / kParts];
+    const Tensor t = tensors[c.x];
     const int at = c.x - base;
     const void* grad = a.grad[at];
-    if (!grad) return;
-    const Tensor t = tensors[c.x];
+    float scale = clip.scale ? *clip.scale : 1.0f;
+    if (clip.partial) {
+        const float norm = (float)sqrt(block_sum<kThreads>(part));
+        if (first + blockIdx.x == 0 && threadIdx.x == 0) *clip.norm = norm;
+        scale = clip_of(norm, clip.max_norm);
+    }
     const int64_t from = (int64_t)c.y * kChunk + blockIdx.x % kParts * Shape<BITS>::kPart;
-    if (from >= t.numel) return;
+    if (!grad || from >= t.numel) return;
     const Step s = {mo, k, inverse, scale, a.size[at], a.root[at], a.keep[at], a.key[at]};
     const bool fg = a.grad_type[at] == B3_F32;
     if (t.type == B3_F32)

@@ -271,7 +271,8 @@ Plan plan_of(int64_t steps, int64_t envs, bool by_env) {
         p.steps = p.cols == 16 ? kSteps : kWideSteps;
     } else {
         p.cols = steps <= 64 ? 64 : steps <= 512 ? 16 : 1;
-        p.steps = 16;
+        /* where tiles of 4,096 steps are few, of 1,024 */
+        p.steps = p.cols == 1 && envs * ceil_div(steps, kThreads * 16) < 2 * kFill ? 4 : 16;
     }
     const int64_t tile = (int64_t)(kThreads / p.cols) * p.steps, all = ceil_div(steps, tile);
     p.blocks = ceil_div(envs, p.cols);
@@ -308,7 +309,8 @@ hipError_t launch_plan(const Job& job, const Plan& p, hipStream_t stream) {
         return p.cols == kWideCols ? launch<VALUES, ENDS, true, kWideCols, kWideSteps>(job, p, stream)
                                    : launch<VALUES, ENDS, true, 16, kSteps>(job, p, stream);
     return p.cols == 64 ? launch<VALUES, ENDS, false, 64, 16>(job, p, stream)
-        : p.cols == 16 ? launch<VALUES, ENDS, false, 16, 16>(job, p, stream) : launch<VALUES, ENDS, false, 1, 16>(job, p, stream);
+        : p.cols == 16 ? launch<VALUES, ENDS, false, 16, 16>(job, p, stream)
+        : p.steps == 16 ? launch<VALUES, ENDS, false, 1, 16>(job, p, stream) : launch<VALUES, ENDS, false, 1, 4>(job, p, stream);
 }
 
 template <int VALUES>

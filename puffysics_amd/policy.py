@@ -19,6 +19,7 @@ from .engine import B3Error
 POLICY_PATH = os.path.join(_native.HERE, "libb3policy.so")
 MAX_TOP = 32
 SEGMENT = 256
+_ONE_WAVE = 1024             # rows of up to so many actions need no workspace
 
 _F32, _F16, _BF16, _U8 = 0, 1, 2, 3
 _TYPE = {torch.float32: _F32, torch.float16: _F16, torch.bfloat16: _BF16}
@@ -101,13 +102,15 @@ def _stream():
 
 def _on(*tensors):
     """Raise unless all are on the current device, where the work runs."""
-    device = None
+    device = -1
     for t in tensors:
         if t is None:
             continue
-        if device is None and t.is_cuda:
+        at = t.get_device()                  # -1: on the host
+        if at >= 0 and device < 0:
             device = torch.cuda.current_device()
-        _need(t.is_cuda and t.get_device() == device, "tensors have to be on the current CUDA device")
+        if at != device or at < 0:
+            raise ValueError("tensors have to be on the current CUDA device")
 
 
 # ---- log probabilities ----
@@ -145,7 +148,7 @@ def _forward(x, taken, mask, top, kept):
     if top:
         top_lp = torch.empty((rows, top), dtype=torch.float32, device=x.device)
         top_action = torch.empty((rows, top), dtype=torch.int64, device=x.device)
-    size = lib.b3_log_probs_workspace(rows, actions, top)
+    size = 0 if actions <= _ONE_WAVE else lib.b3_log_probs_workspace(rows, actions, top)
     if size:
         work = torch.empty(size, dtype=torch.uint8, device=x.device)
     _check("b3_log_probs_gpu", lib.b3_log_probs_gpu(
@@ -200,9 +203,9 @@ def log_probs(logits, taken, mask=None, top=0):
     _need(logits.dim() >= 1 and logits.shape[-1] >= 1, "logits need at least one action")
     _need(not taken.is_floating_point() and taken.dtype != torch.bool, "taken has to be whole numbers")
     _need(taken.shape == logits.shape[:-1], "taken has to have the shape of logits without the last axis")
-    _need(0 <= top <= min(MAX_TOP, logits.shape[-1]), "top has to be between 0 and %d, and at most the actions" % MAX_TOP)
-    _on(logits, taken, mask)
     actions = logits.shape[-1]
+    _need(0 <= top <= MAX_TOP and top <= actions, "top has to be between 0 and 32, and at most the actions")
+    _on(logits, taken, mask)
     if mask is not None:
         _need(mask.dtype == torch.bool, "mask has to be bool")
         _need(mask.shape == logits.shape or mask.shape == (actions,),
@@ -253,11 +256,10 @@ def advantages(rewards, values, terminals, last_values, gamma=0.99, lam=0.95):
     turned = rewards.stride(0) < rewards.stride(1)
     out = torch.empty((2, envs, steps) if turned else (2, steps, envs), dtype=torch.float32, device=rewards.device)
     adv, ret = (out[0].t(), out[1].t()) if turned else (out[0], out[1])
-    pair = _ll * 2
-    g = B3Rollout(steps, envs, rewards.data_ptr(), pair(*rewards.stride()), values.data_ptr(), _TYPE[values.dtype],
-                  pair(*values.stride()), last_values.data_ptr(), last_values.stride(0), terminals.data_ptr(),
-                  _F32 if terminals.dtype == torch.float32 else _U8, pair(*terminals.stride()), adv.data_ptr(),
-                  ret.data_ptr(), pair(*adv.stride()))
+    g = B3Rollout(steps, envs, rewards.data_ptr(), rewards.stride(), values.data_ptr(), _TYPE[values.dtype],
+                  values.stride(), last_values.data_ptr(), last_values.stride(0), terminals.data_ptr(),
+                  _F32 if terminals.dtype == torch.float32 else _U8, terminals.stride(), adv.data_ptr(), ret.data_ptr(),
+                  adv.stride())
     size = lib.b3_advantages_workspace(steps, envs)
     work = torch.empty(size, dtype=torch.uint8, device=rewards.device) if size else None
     _check("b3_advantages_gpu", lib.b3_advantages_gpu(C.byref(g), gamma, lam, work.data_ptr() if size else None, size,
