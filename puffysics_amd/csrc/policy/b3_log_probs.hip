@@ -235,16 +235,21 @@ struct Outputs {
     int64_t* top_action;
 };
 
-/* What one thread of a row writes. */
+/* The taken action's logit, fetched before the sums are formed. */
 template <typename T>
-__device__ void finish_row(const B3Logits& g, const Outputs& o, int64_t r, Sums s, float log_sum) {
-    const int64_t a = o.taken[r];
+__device__ __forceinline__ float taken_logit(const B3Logits& g, int64_t r, int64_t a) {
+    return a >= 0 && a < g.actions ? logit(row_of<T>(g, r), mask_of(g, r), a) : 0.0f;
+}
+
+/* What one thread of a row writes; x is the logit of the taken action a. */
+__device__ __forceinline__ void finish_row(const B3Logits& g, const Outputs& o, int64_t r, int64_t a, float x, Sums s,
+    float log_sum) {
     const bool empty = s.s == 0.0f;
     float lp = 0.0f;
     if (a >= g.actions)
         lp = NAN;
     else if (a >= 0)
-        lp = empty ? -INFINITY : logit(row_of<T>(g, r), mask_of(g, r), a) - s.m - log_sum;
+        lp = empty ? -INFINITY : x - s.m - log_sum;
     o.log_prob[r] = lp;
     o.entropy[r] = empty ? 0.0f : log_sum - s.d / s.s;
     if (o.stats) {
@@ -386,11 +391,13 @@ __global__ __launch_bounds__(kThreads) void lp_small(B3Logits g, Outputs o) {
     const int64_t r = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / G;
     if (r >= g.rows) return;                     // all G lanes of it
     const int lane = threadIdx.x % G, n = (int)g.actions;
+    const int64_t a = o.taken[r];
     float x[PER];
     load_logits<T, G, PER, W>(row_of<T>(g, r), mask_of(g, r), 0, n, lane, false, x);
+    const float xa = taken_logit<T>(g, r, a);
     const Sums s = sums_of<G, PER>(x, lane_max<PER>(x));
     const float log_sum = logf(s.s);
-    if (lane == 0) finish_row<T>(g, o, r, s, log_sum);
+    if (lane == 0) finish_row(g, o, r, a, xa, s, log_sum);
     if (!o.top) return;
     if (G == kWave) {
         uint32_t order[PER], my_order;
@@ -424,12 +431,13 @@ __device__ int first_place(const float x[PER], float value, int from, int n) {
     return place;
 }
 
-/* A bound that `top` of the wave's logits reach: those over `order`, and of
- * equals those up to `place`.  It is taken from the lanes' maxima, so that at
- * most `top` lanes of the wave hold any logit that reaches it: bit by bit the
- * largest order that `top` lanes reach (a smaller one that exactly `top`
- * reach does as well), and if more do, because they are equal, the place up
- * to which `top` do. */
+/* A bound that at least `top` of the wave's logits reach: those over `order`,
+ * and of equals those up to `place`.  It is taken from the lanes' maxima, bit
+ * by bit the largest order that `top` lanes reach; a smaller one that few more
+ * reach will do.  Where more reach the last, because they are equal, it is
+ * the place up to which `top` do: so no more than `top` + kSlack lanes of the
+ * wave hold any logit that reaches the bound. */
+constexpr int kSlack = 8;
 struct Bound {
     uint32_t order;
     int place;
@@ -441,7 +449,7 @@ __device__ __forceinline__ Bound wave_bound(const float x[PER], float lane_most,
     /* the bits that all lanes share, and then one after the other */
     int bit = high == low ? -1 : 31 - __builtin_clz(high ^ low), reach = kWave;
     uint32_t order = bit < 0 ? high : high & ~((2u << bit) - 1);
-    for (; bit >= 0 && reach != top; bit--) {
+    for (; bit >= 0 && reach > top + kSlack; bit--) {
         const uint32_t next = order | 1u << bit;
         const int count = __builtin_popcountll(__ballot(mine >= next));
         if (count >= top) {
@@ -449,7 +457,7 @@ __device__ __forceinline__ Bound wave_bound(const float x[PER], float lane_most,
             reach = count;
         }
     }
-    if (reach == top) return Bound{order, INT32_MAX};
+    if (reach <= top + kSlack) return Bound{order, INT32_MAX};
     const int need = top - __builtin_popcountll(__ballot(mine > order));
     const int place = mine == order ? first_place<THREADS, PER, W>(x, value_of(order), from, n) : INT32_MAX;
     int up_to = -1;                              // the largest that fewer than `need` do not pass
@@ -475,13 +483,16 @@ __global__ __launch_bounds__(THREADS) void lp_piece(B3Logits g, Outputs o, Piece
     __shared__ Sums part[kWaves];
     __shared__ Bound bounds[TOP ? kWaves : 1];
     __shared__ uint2 list[TOP ? kList : 1];
+    __shared__ int places[TOP ? kList : 1];
     __shared__ int listed;
     const int64_t r = blockIdx.x / (unsigned)p.count;
     const int piece = blockIdx.x % (unsigned)p.count;
     const int from = piece * p.size, end = from + p.size, n = end < g.actions ? end : (int)g.actions;
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int64_t a = p.count == 1 ? o.taken[r] : -1;
     float x[PER];
     load_logits<T, THREADS, PER, W>(row_of<T>(g, r), mask_of(g, r), from, n, threadIdx.x, p.once, x);
+    const float xa = taken_logit<T>(g, r, a);
     const float most = lane_max<PER>(x);
     const Sums mine = sums_of<kWave, PER>(x, most);
     if (lane == 0) part[wave] = mine;
@@ -498,7 +509,7 @@ __global__ __launch_bounds__(THREADS) void lp_piece(B3Logits g, Outputs o, Piece
     const float log_sum = logf(s.s);
     if (threadIdx.x == 0) {
         if (p.count == 1)
-            finish_row<T>(g, o, r, s, log_sum);
+            finish_row(g, o, r, a, xa, s, log_sum);
         else
             p.sums[r * p.count + piece] = s;
     }
@@ -512,32 +523,36 @@ __global__ __launch_bounds__(THREADS) void lp_piece(B3Logits g, Outputs o, Piece
     const float value = value_of(bound.order);
     int count = kList + 1;
     if (s.s == s.s) {
-        uint32_t reaches = 0;                    // bit i: x[i]
+        uint32_t reaches = 0;                    // bit PER - 1 - i: x[i]
         if (most >= value) {
 #pragma unroll
-            for (int i = 0; i < PER; i++) {
-                const int j = from + ((i / W) * THREADS + (int)threadIdx.x) * W + i % W;
-                reaches |= (uint32_t)(x[i] >= value && j < n && (x[i] > value || j <= bound.place)) << i;
-            }
+            for (int i = 0; i < PER; i++) reaches = reaches << 1 | (x[i] >= value);
         }
         if (__ballot(reaches != 0)) {
             /* the wave's part of the list, and the lane's of that */
-            int before = __builtin_popcount(reaches);
-            const int own = before;
-            before = wave_scan(before);
+            const int own = __builtin_popcount(reaches), upto = wave_scan(own);
             int at = 0;
-            if (lane == kWave - 1) at = atomicAdd(&listed, before);
-            at = __builtin_amdgcn_readlane(at, kWave - 1) + before - own;
-#pragma unroll
-            for (int i = 0; i < PER; i++) {
-                if (reaches >> i & 1) {
-                    if (at < kList) list[at] = make_uint2(order_of(x[i]), from + ((i / W) * THREADS + (int)threadIdx.x) * W + i % W);
-                    at++;
-                }
+            if (lane == kWave - 1) at = atomicAdd(&listed, upto);
+            at = __builtin_amdgcn_readlane(at, kWave - 1) + upto - own;
+            for (; reaches; at++) {
+                const int i = PER - 1 - (31 - __builtin_clz(reaches));
+                reaches &= ~(0x80000000u >> __builtin_clz(reaches));
+                if (at < kList) places[at] = from + ((i / W) * THREADS + (int)threadIdx.x) * W + i % W;
             }
         }
         __syncthreads();
         count = listed;
+        if (count <= kList) {
+            /* their logits are fetched again: a thread cannot take those that
+             * it has in registers by number */
+            for (int i = threadIdx.x; i < count; i += THREADS) {
+                const int j = places[i];
+                const float xj = j < n ? logit(row_of<T>(g, r), mask_of(g, r), j) : -INFINITY;
+                const bool in = j < n && (xj > value || (xj == value && j <= bound.place));
+                list[i] = make_uint2(in ? order_of(xj) : 0, j);
+            }
+            __syncthreads();
+        }
     }
     if (count > kList) {
         __syncthreads();
@@ -585,7 +600,17 @@ __global__ __launch_bounds__(kThreads) void lp_join(B3Logits g, Outputs o, Piece
     const int lane = threadIdx.x;
     /* the pieces' lists are sorted, and of equal orders the one of the lower
      * piece has the lower action */
-    for (int i = threadIdx.x; i < p.count * o.top; i += blockDim.x) lists[i] = p.top[r * p.count * o.top + i];
+    const int entries = p.count * o.top;
+    const uint2* from = p.top + r * entries;
+    for (int i = threadIdx.x; i < entries; i += 4 * blockDim.x) {
+        uint2 it[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) it[k] = from[min(i + k * (int)blockDim.x, entries - 1)];
+#pragma unroll
+        for (int k = 0; k < 4; k++) lists[min(i + k * (int)blockDim.x, entries - 1)] = it[k];
+    }
+    const int64_t a = o.taken[r];
+    const float xa = taken_logit<T>(g, r, a);
     __syncthreads();
     if (threadIdx.x >= kWave) return;
     Sums part = {0, 0, 0};
@@ -599,7 +624,7 @@ __global__ __launch_bounds__(kThreads) void lp_join(B3Logits g, Outputs o, Piece
         part = join(part, Sums{__shfl_xor(part.m, d), __shfl_xor(part.s, d), __shfl_xor(part.d, d)});
     const Sums all = part;
     const float log_sum = logf(all.s);
-    if (lane == 0) finish_row<T>(g, o, r, all, log_sum);
+    if (lane == 0) finish_row(g, o, r, a, xa, all, log_sum);
     if (!o.top) return;
     uint2 head[kHeads];
     int next[kHeads];
