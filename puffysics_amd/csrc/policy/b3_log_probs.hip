@@ -10,7 +10,7 @@
  * the backward reads them once and writes as much.  A row, or a piece of one,
  * is held in the registers of the threads that share it, so that the maximum
  * comes before the sums with one read and no rescaling:
- *   up to 1,024 actions   G lanes of a wave to a row, by a rule on the
+ *   up to 2,048 actions   G lanes of a wave to a row, by a rule on the
  *                         actions alone (with_small)
  *   more                  a workgroup to a row, or to a piece of one
  *                         (pieces_of); the pieces' (m, S, sum z exp(z)) and
@@ -78,25 +78,33 @@ __device__ __forceinline__ void load_logits(const T* row, const unsigned char* m
 #pragma unroll
     for (int v = 0; v < NV; v++) {
         const int j = from + (v * G + lane) * W;
-        if (j + W <= n) p[v] = *(const Pack<T, W>*)(row + j);
-    }
-    if (mask) {
-#pragma unroll
-        for (int v = 0; v < NV; v++) {
-            const int j = from + (v * G + lane) * W;
-            if (j + W <= n) k[v] = *(const Pack<unsigned char, W>*)(mask + j);
+        if (v < last || (v == last && j + W <= n)) {
+            p[v] = *(const Pack<T, W>*)(row + j);
+            if (mask) k[v] = *(const Pack<unsigned char, W>*)(mask + j);
         }
     }
 #pragma unroll
     for (int v = 0; v < NV; v++) {
         const int j = from + (v * G + lane) * W;
-        const bool whole = j + W <= n;
+        if (v < last) {
 #pragma unroll
-        for (int w = 0; w < W; w++) {
-            x[v * W + w] = whole ? to_float(p[v].v[w]) : -INFINITY;
-            if (mask) x[v * W + w] = whole && k[v].v[w] ? x[v * W + w] : -INFINITY;
+            for (int w = 0; w < W; w++) x[v * W + w] = to_float(p[v].v[w]);
+            if (mask) {
+#pragma unroll
+                for (int w = 0; w < W; w++) x[v * W + w] = k[v].v[w] ? x[v * W + w] : -INFINITY;
+            }
+            continue;
         }
-        if (v == last && !whole) {
+#pragma unroll
+        for (int w = 0; w < W; w++) x[v * W + w] = -INFINITY;
+        if (v > last) continue;
+        if (j + W <= n) {
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                x[v * W + w] = to_float(p[v].v[w]);
+                if (mask) x[v * W + w] = k[v].v[w] ? x[v * W + w] : -INFINITY;
+            }
+        } else {
 #pragma unroll
             for (int w = 0; w < W; w++)
                 if (j + w < n) x[v * W + w] = logit(row, mask, j + w);
@@ -159,41 +167,58 @@ struct Sums {
     float m, s, d;
 };
 
-template <int PER>
-__device__ __forceinline__ float lane_max(const float x[PER]) {
-    float m = max3(x[0], x[1], x[2]);
+/* Loads of W in a thread's PER that have any place below n. */
+template <int G, int PER, int W>
+__device__ __forceinline__ int live_loads(int from, int n) {
+    const int loads = (n - from + G * W - 1) / (G * W);
+    return loads < PER / W ? loads : PER / W;
+}
+
+template <int PER, int W>
+__device__ __forceinline__ float lane_max(const float x[PER], int live) {
+    float m = -INFINITY;
 #pragma unroll
-    for (int i = 3; i < PER; i += 2) m = max3(m, x[i], x[i + 1 < PER ? i + 1 : i]);
+    for (int v = 0; v < PER / W; v++) {
+        if (v < live) {
+#pragma unroll
+            for (int i = v * W; i < (v + 1) * W; i += 2) m = max3(m, x[i], x[i + 1]);
+        }
+    }
     return m;
 }
 
-/* The sums over G <= 64 lanes of a row, from each lane's maximum.  exp(z) is
+/* The sums over G <= 64 lanes of a row, of its first `live` loads, from each
+ * lane's maximum.  exp(z) is
  * 2^t with t = x log2 e - fl(m log2 e) in one rounding, which is z log2 e
  * but for `off`, what fl() left out; it is the same for every term and taken
  * back from the sums.  Beyond 2^16 it could be large, and t is formed from z.
  * A term is off by |t| 2^-24, relative to itself; those with |t| > 30 do not
  * count.  t is bounded in D alone, where 0 times -inf would be NaN. */
-template <int G, int PER>
-__device__ __forceinline__ Sums sums_of(const float x[PER], float lane_most) {
+template <int G, int PER, int W>
+__device__ __forceinline__ Sums sums_of(const float x[PER], int live, float lane_most) {
     float m = G == kWave ? wave_max(lane_most)
         : group_reduce<G>(lane_most, [](float a, float b) { return max3(a, b, b); });
     m = m == -INFINITY || m != m ? 0.0f : m;
     float s = 0, d = 0, off = 0;
-    if (fabsf(m) <= 65536.0f) {
-        const float ml = m * kLog2e;
-        off = __builtin_fmaf(m, kLog2e, -ml);
+    const bool small = fabsf(m) <= 65536.0f;
+    const float ml = m * kLog2e;
+    if (small) off = __builtin_fmaf(m, kLog2e, -ml);
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const float t = __builtin_fmaf(x[i], kLog2e, -ml), e = __builtin_amdgcn_exp2f(t);
-            s += e;
-            d = __builtin_fmaf(e, fmaxf(t, -1e4f), d);
-        }
-    } else {
+    for (int v = 0; v < PER / W; v++) {
+        if (v < live && small) {
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const float t = (x[i] - m) * kLog2e, e = __builtin_amdgcn_exp2f(t);
-            s += e;
-            d = __builtin_fmaf(e, fmaxf(t, -1e4f), d);
+            for (int i = v * W; i < (v + 1) * W; i++) {
+                const float t = __builtin_fmaf(x[i], kLog2e, -ml), e = __builtin_amdgcn_exp2f(t);
+                s += e;
+                d = __builtin_fmaf(e, fmaxf(t, -1e4f), d);
+            }
+        } else if (v < live) {
+#pragma unroll
+            for (int i = v * W; i < (v + 1) * W; i++) {
+                const float t = (x[i] - m) * kLog2e, e = __builtin_amdgcn_exp2f(t);
+                s += e;
+                d = __builtin_fmaf(e, fmaxf(t, -1e4f), d);
+            }
         }
     }
     if (G == kWave) {
@@ -395,7 +420,8 @@ __global__ __launch_bounds__(kThreads) void lp_small(B3Logits g, Outputs o) {
     float x[PER];
     load_logits<T, G, PER, W>(row_of<T>(g, r), mask_of(g, r), 0, n, lane, false, x);
     const float xa = taken_logit<T>(g, r, a);
-    const Sums s = sums_of<G, PER>(x, lane_max<PER>(x));
+    const int live = live_loads<G, PER, W>(0, n);
+    const Sums s = sums_of<G, PER, W>(x, live, lane_max<PER, W>(x, live));
     const float log_sum = logf(s.s);
     if (lane == 0) finish_row(g, o, r, a, xa, s, log_sum);
     if (!o.top) return;
@@ -493,8 +519,9 @@ __global__ __launch_bounds__(THREADS) void lp_piece(B3Logits g, Outputs o, Piece
     float x[PER];
     load_logits<T, THREADS, PER, W>(row_of<T>(g, r), mask_of(g, r), from, n, threadIdx.x, p.once, x);
     const float xa = taken_logit<T>(g, r, a);
-    const float most = lane_max<PER>(x);
-    const Sums mine = sums_of<kWave, PER>(x, most);
+    const int live = live_loads<THREADS, PER, W>(from, n);
+    const float most = lane_max<PER, W>(x, live);
+    const Sums mine = sums_of<kWave, PER, W>(x, live, most);
     if (lane == 0) part[wave] = mine;
     if (TOP) {
         const Bound b = wave_bound<THREADS, PER, W>(x, most, o.top, from, n);
@@ -735,9 +762,9 @@ __global__ __launch_bounds__(kThreads) void lp_piece_backward(B3Logits g, Upstre
 
 /* ---- launches ---- */
 
-/* Calls f with the shape for rows of up to 1,024 actions: the fewest lanes
- * that hold them at 16 each, since what is done once a row is shared by few
- * elements already; four in a lane where that is all. */
+/* Calls f with the shape for rows of up to 2,048 actions: the fewest lanes
+ * that hold them at 16 each, or 32, since what is done once a row is shared by
+ * few elements already; four in a lane where that is all. */
 template <typename T, typename F>
 void with_small(int64_t actions, F f) {
     constexpr int W = 16 / sizeof(T);
@@ -749,11 +776,13 @@ void with_small(int64_t actions, F f) {
         f.template operator()<T, 4, 16, W>();
     else if (actions <= 256)
         f.template operator()<T, 16, 16, W>();
-    else
+    else if (actions <= 1024)
         f.template operator()<T, 64, 16, W>();
+    else
+        f.template operator()<T, 64, 32, W>();
 }
 
-constexpr int kSmall = 1024, kShortPiece = 4096, kPiece = 8192, kWide = 16384;
+constexpr int kSmall = 2048, kShortPiece = 4096, kPiece = 8192, kWide = 16384;
 constexpr int64_t kFill = 512;                   // workgroups: two to a compute unit
 
 template <typename F>
@@ -827,7 +856,7 @@ hipError_t forward(const B3Logits& g, const Outputs& o, Pieces p, hipStream_t st
     const unsigned grid = (unsigned)(g.rows * p.count);
     const int64_t most = p.count == 1 ? g.actions : p.size;
     if (most <= kShortPiece)
-        launch_piece<T, 256, kShortPiece / 256, W>(g, o, p, grid, stream);
+        launch_piece<T, 128, kShortPiece / 128, W>(g, o, p, grid, stream);
     else if (most <= kPiece)
         launch_piece<T, 256, kPiece / 256, W>(g, o, p, grid, stream);
     else
