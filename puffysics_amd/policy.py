@@ -281,7 +281,8 @@ class AdamW:
     master         keep 32-bit copies of 16-bit weights and round those; without
                    them small updates of such weights are lost
 
-    The moments lie in flat arrays, tensor i's from offsets[i] on."""
+    The moments lie in flat arrays, tensor i's from offsets[i] on.  Steps of
+    one optimizer follow one another: on several streams, order them."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32,
                  max_grad_norm=None, master=True, seed=0):
@@ -322,7 +323,7 @@ class AdamW:
         state = B3AdamWState(state_bits, self._exp_avg.data_ptr(), self._exp_avg_sq.data_ptr(),
                              self._scale[0].data_ptr(), self._scale[1].data_ptr(),
                              self._master.data_ptr() if self._master is not None else None)
-        self._given = [(p.shape, p.dtype) for p in self.params]
+        self._given = [(p.shape, p.dtype, p.data_ptr()) for p in self.params]
         self._grads, self._types = (_vp * max(n, 1))(), (_i * max(n, 1))()
         torch.cuda.current_stream().synchronize()     # the state is ready for a step on any stream
         _check("b3_adamw_create", self._lib.b3_adamw_create(C.byref(self._h), table, n, state,
@@ -339,12 +340,15 @@ class AdamW:
         if grads is None:
             grads = [p.grad for p in self.params]
         _need(len(grads) == len(self.params), "need one gradient for each parameter")
-        here, pointers, types = torch.cuda.current_device(), [], []
-        for g, (shape, dtype) in zip(grads, self._given):
+        here, pointers, types, stepped = torch.cuda.current_device(), [], [], []
+        for g, p, (shape, dtype, at) in zip(grads, self.params, self._given):
+            if p.data_ptr() != at:
+                raise ValueError("a parameter's memory is not where it was")
             if g is None:
                 pointers.append(None)
                 types.append(0)
                 continue
+            stepped.append(p)
             if g.get_device() != here:
                 raise ValueError("gradients have to be on the current CUDA device")
             if g.shape != shape or not g.is_contiguous():
@@ -359,6 +363,7 @@ class AdamW:
         _check("b3_adamw_step_gpu", self._lib.b3_adamw_step_gpu(
             self._h, self._grads, self._types, self.lr if lr is None else lr, self.max_grad_norm or 0.0,
             norm.data_ptr() if norm is not None else None, _stream()))
+        torch.autograd.graph.increment_version(stepped)      # as an operation in place does
         return norm
 
     def moments(self):

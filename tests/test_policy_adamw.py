@@ -386,6 +386,40 @@ def test_refusals_of_gradients():
             policy.AdamW(p, LR, **bad)
 
 
+@pytest.mark.gpu
+def test_a_step_is_an_operation_in_place():
+    """Autograd notices weights that were stepped between a forward pass and
+    its backward; a parameter whose memory went elsewhere is refused."""
+    from puffysics_amd import policy
+    w = torch.randn(5, device="cuda", requires_grad=True)
+    opt = policy.AdamW([w], LR)
+    y = (w * w).sum()
+    opt.step([torch.ones(5, device="cuda")])
+    with pytest.raises(RuntimeError):
+        y.backward()
+    w.data = torch.randn(5, device="cuda")
+    with pytest.raises(ValueError):
+        opt.step([torch.ones(5, device="cuda")])
+
+
+@pytest.mark.gpu
+def test_places_past_32_bits():
+    """The weights at the far end of more than 2^32."""
+    from puffysics_amd import policy
+    n = 2 ** 32 + 70_001
+    p = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    g = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    g[-5:] = torch.tensor([1.0, -1.0, 0.5, 2.0, -3.0])
+    g[2 ** 32] = 4.0
+    opt = policy.AdamW([p], LR, weight_decay=0.0, state_bits=8, master=False, max_grad_norm=100.0)
+    assert abs(float(opt.step([g])) - (1 + 1 + 0.25 + 4 + 9 + 16) ** 0.5) < 1e-5
+    assert torch.equal(p[-5:].float().sign(), -g[-5:].float().sign()) and float(p[2 ** 32]) < 0
+    assert int(torch.count_nonzero(p[-100_000:])) == 6 and int(torch.count_nonzero(p[:100_000])) == 0
+    m, v = opt.moments()
+    assert (m[2 ** 32:n][g[2 ** 32:] == 0] == 0).all() and abs(float(m[n - 1]) + 0.3) < 0.3 / 8
+    assert abs(float(v[2 ** 32]) - 0.016) < 0.016 / 3
+
+
 def test_refusals():
     from puffysics_amd import policy
     for p in (torch.zeros(3, dtype=torch.float64), torch.zeros(4, 6).t(), torch.zeros(4, dtype=torch.int64), torch.zeros(3)):

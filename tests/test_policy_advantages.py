@@ -106,6 +106,28 @@ def test_an_episode_keeps_its_nan(steps, envs):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("by_env", [False, True])
+def test_places_past_32_bits(by_env):
+    """More than 2^31 steps in all: the last environments have what they have
+    alone."""
+    from puffysics_amd import policy
+    steps, envs = 1024, 2 ** 21 + 3
+    shape = (envs, steps) if by_env else (steps, envs)
+    turn = (lambda x: x.t()) if by_env else (lambda x: x)
+    r, v = turn(torch.zeros(shape, device="cuda")), turn(torch.zeros(shape, dtype=torch.bfloat16, device="cuda"))
+    d = turn(torch.zeros(shape, dtype=torch.uint8, device="cuda"))
+    few = rollout(steps, 5, "bf16", 12)
+    for to, x in zip((r, v, d), few):
+        to[:, -5:].copy_(x)
+    last = torch.zeros(envs, dtype=torch.bfloat16, device="cuda")
+    last[-5:] = few[3].cuda()
+    adv, ret = policy.advantages(r, v, d, last)
+    alone = check(*few)
+    assert torch.allclose(adv[:, -5:], alone[0], rtol=1e-5, atol=1e-4) and torch.allclose(ret[:, -5:], alone[1], rtol=1e-5, atol=1e-4)
+    assert int(torch.count_nonzero(adv[:, :1000])) == 0 and int(torch.count_nonzero(adv[-1, :-5])) == 0
+
+
+@pytest.mark.gpu
 def test_nothing():
     from puffysics_amd import policy
     for steps, envs in ((0, 4), (4, 0), (0, 0)):

@@ -91,6 +91,34 @@ def test_few_and_many_rows(rows, actions):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("actions", [2 ** 20, 2 ** 20 + 1, 2 ** 21])
+def test_the_longest_rows(actions):
+    """As many pieces to a row as there may be, with as many alternatives."""
+    x, taken = inputs(2, actions, "f32", actions)
+    check(x, taken, "f32", top=32)
+
+
+@pytest.mark.gpu
+def test_rows_past_32_bits():
+    """More than 2^31 logits: the last rows are what they are alone."""
+    from puffysics_amd import policy
+    rows, actions = 17000, 131072
+    x = torch.zeros(rows, actions, dtype=torch.bfloat16, device="cuda")
+    x[-3:].copy_(inputs(3, actions, "bf16", 1)[0])
+    taken = torch.full((rows,), 7, device="cuda")
+    x.requires_grad_(True)
+    got = policy.log_probs(x, taken, top=2)
+    dl = torch.ones(rows, device="cuda")
+    d, = torch.autograd.grad((got.log_prob, got.entropy), x, (dl, dl))
+    tail = x.detach()[-3:].clone().requires_grad_(True)
+    alone = policy.log_probs(tail, taken[-3:], top=2)
+    d_alone, = torch.autograd.grad((alone.log_prob, alone.entropy), tail, (dl[-3:], dl[-3:]))
+    assert torch.allclose(got.log_prob[-3:], alone.log_prob, rtol=0, atol=SUM) and torch.equal(got.top_action[-3:], alone.top_action)
+    assert abs(float(got.log_prob[rows // 2].detach()) + np.log(actions)) < SUM
+    assert torch.allclose(d[-3:].float(), d_alone.float(), rtol=2.0 ** -7, atol=1e-9)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("type", TYPES)
 @pytest.mark.parametrize("actions,wide", [(3, 8), (21, 22), (1021, 1040), (4097, 5003), (40001, 40020)])
 def test_slices_of_wider_rows(actions, wide, type):
@@ -279,6 +307,15 @@ def test_same_results_every_time_and_on_another_stream():
             b = policy.log_probs(y, taken, top=2)
         torch.cuda.current_stream().wait_stream(s)
         assert all(torch.equal(p, q) for p, q in zip(a, b))
+        grads = []
+        for stream in (torch.cuda.current_stream(), s):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                leaf = x.clone().requires_grad_(True)
+                policy.log_probs(leaf, taken)[0].sum().backward()
+            torch.cuda.current_stream().wait_stream(stream)
+            grads.append(leaf.grad)
+        assert torch.equal(*grads)
 
 
 @pytest.mark.gpu
