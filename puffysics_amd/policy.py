@@ -7,6 +7,7 @@ stream and runs in libb3policy.so.  Arguments that do not fit raise
 ValueError before anything is launched; an error of a call raises B3Error.
 The reference leaves these to the trainer (docs/RL_LIBRARY.md).
 """
+import array
 import collections
 import ctypes as C
 import os
@@ -170,14 +171,21 @@ class _LogProbs(torch.autograd.Function):
         return log_prob, entropy, top_lp, top_action
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_log_prob, d_entropy, *_):
-        x, taken, mask, stats, entropy = ctx.saved_tensors
-        d = torch.empty_like(x, memory_format=torch.contiguous_format)
-        _check("b3_log_probs_backward_gpu", policy_lib().b3_log_probs_backward_gpu(
-            _logits(x, mask), taken.data_ptr(), stats.data_ptr(), entropy.data_ptr(), *_upstream(d_log_prob),
-            *_upstream(d_entropy), d.data_ptr(), x.shape[1], _stream()))
-        return d, None, None, None
+        # a gradient that is differentiated again says that it cannot be
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, d_log_prob, d_entropy)
+
+
+def _backward(ctx, d_log_prob, d_entropy):
+    x, taken, mask, stats, entropy = ctx.saved_tensors
+    d = torch.empty_like(x, memory_format=torch.contiguous_format)
+    _check("b3_log_probs_backward_gpu", policy_lib().b3_log_probs_backward_gpu(
+        _logits(x, mask), taken.data_ptr(), stats.data_ptr(), entropy.data_ptr(), *_upstream(d_log_prob),
+        *_upstream(d_entropy), d.data_ptr(), x.shape[1], _stream()))
+    return d, None, None, None
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 def _upstream(d):
@@ -323,8 +331,8 @@ class AdamW:
         state = B3AdamWState(state_bits, self._exp_avg.data_ptr(), self._exp_avg_sq.data_ptr(),
                              self._scale[0].data_ptr(), self._scale[1].data_ptr(),
                              self._master.data_ptr() if self._master is not None else None)
-        self._given = [(p.shape, p.dtype, p.data_ptr()) for p in self.params]
-        self._grads, self._types = (_vp * max(n, 1))(), (_i * max(n, 1))()
+        self._at, self._shapes, self._dtypes = ([f(p) for p in self.params] for f in (
+            torch.Tensor.data_ptr, lambda p: p.shape, lambda p: p.dtype))
         torch.cuda.current_stream().synchronize()     # the state is ready for a step on any stream
         _check("b3_adamw_create", self._lib.b3_adamw_create(C.byref(self._h), table, n, state,
                                                             B3AdamWConfig(betas[0], betas[1], eps, seed)))
@@ -340,28 +348,29 @@ class AdamW:
         if grads is None:
             grads = [p.grad for p in self.params]
         _need(len(grads) == len(self.params), "need one gradient for each parameter")
-        here, pointers, types, stepped = torch.cuda.current_device(), [], [], []
-        for g, p, (shape, dtype, at) in zip(grads, self.params, self._given):
-            if p.data_ptr() != at:
-                raise ValueError("a parameter's memory is not where it was")
-            if g is None:
-                pointers.append(None)
-                types.append(0)
-                continue
-            stepped.append(p)
-            if g.get_device() != here:
-                raise ValueError("gradients have to be on the current CUDA device")
-            if g.shape != shape or not g.is_contiguous():
-                raise ValueError("gradients have to be contiguous, of the parameters' shapes")
-            if g.dtype is not dtype and g.dtype is not torch.float32:
-                raise ValueError("gradients have to be of the parameters' type or float32")
-            pointers.append(g.data_ptr())
-            types.append(_TYPE[g.dtype])
-        n = len(pointers)
-        self._grads[:n], self._types[:n] = pointers, types
+        if [p.data_ptr() for p in self.params] != self._at:
+            raise ValueError("a parameter's memory is not where it was")
+        stepped, shapes, dtypes, given = self.params, self._shapes, self._dtypes, grads
+        with_grad = [i for i, g in enumerate(grads) if g is not None]
+        if len(with_grad) < len(grads):
+            stepped, shapes, dtypes, given = ([x[i] for i in with_grad] for x in (stepped, shapes, dtypes, grads))
+        if not {g.get_device() for g in given} <= {torch.cuda.current_device()}:
+            raise ValueError("gradients have to be on the current CUDA device")
+        if [g.shape for g in given] != shapes or not all([g.is_contiguous() for g in given]):
+            raise ValueError("gradients have to be contiguous, of the parameters' shapes")
+        types = [g.dtype for g in given]
+        if types != dtypes and any([t is not d and t is not torch.float32 for t, d in zip(types, dtypes)]):
+            raise ValueError("gradients have to be of the parameters' type or float32")
+        if given is grads:
+            pointers = array.array("Q", [g.data_ptr() for g in grads])
+        else:
+            pointers = array.array("Q", [0 if g is None else g.data_ptr() for g in grads])
+        kinds = None if types == dtypes else \
+            array.array("i", [_TYPE[d if g is None else g.dtype] for g, d in zip(grads, self._dtypes)])
         norm = torch.empty((), dtype=torch.float32, device=self.device) if self.max_grad_norm else None
         _check("b3_adamw_step_gpu", self._lib.b3_adamw_step_gpu(
-            self._h, self._grads, self._types, self.lr if lr is None else lr, self.max_grad_norm or 0.0,
+            self._h, pointers.buffer_info()[0], kinds.buffer_info()[0] if kinds else None,
+            self.lr if lr is None else lr, self.max_grad_norm or 0.0,
             norm.data_ptr() if norm is not None else None, _stream()))
         torch.autograd.graph.increment_version(stepped)      # as an operation in place does
         return norm

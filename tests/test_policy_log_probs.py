@@ -274,6 +274,19 @@ def test_one_of_the_outputs_alone():
 
 
 @pytest.mark.gpu
+def test_differentiated_once():
+    from puffysics_amd import policy
+    x, taken = inputs(4, 6, "f32", 2)
+    x = x.detach().requires_grad_(True)
+    lp = policy.log_probs(x, taken.cuda()).log_prob
+    d, = torch.autograd.grad(lp.sum(), x, create_graph=True)
+    plain, = torch.autograd.grad(policy.log_probs(x, taken.cuda()).log_prob.sum(), x)
+    assert torch.equal(d, plain)
+    with pytest.raises(RuntimeError):
+        d.square().sum().backward()
+
+
+@pytest.mark.gpu
 def test_shapes_and_types_of_arguments():
     from puffysics_amd import policy
     g = torch.Generator().manual_seed(0)
