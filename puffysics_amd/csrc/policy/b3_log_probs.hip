@@ -384,27 +384,48 @@ __device__ void wave_top(uint32_t order[NV * W], int top, uint32_t& my_order, in
     }
 }
 
-/* The same for G < 64 lanes to a row: each round the largest key of order and
- * place below the last. */
+/* The largest (or, of the complements, the smallest) over the G = 1, 4 or 16
+ * lanes of a row, to all of them: lanes swapped in pairs, pairs swapped,
+ * eights and sixteens mirrored. */
+template <int G>
+__device__ __forceinline__ uint32_t group_most(uint32_t x) {
+    uint32_t y;
+    if (G >= 4) {
+        y = __builtin_amdgcn_update_dpp(x, x, 0xb1, 0xf, 0xf, false);
+        x = x > y ? x : y;
+        y = __builtin_amdgcn_update_dpp(x, x, 0x4e, 0xf, 0xf, false);
+        x = x > y ? x : y;
+    }
+    if (G >= 16) {
+        y = __builtin_amdgcn_update_dpp(x, x, 0x141, 0xf, 0xf, false);
+        x = x > y ? x : y;
+        y = __builtin_amdgcn_update_dpp(x, x, 0x140, 0xf, 0xf, false);
+        x = x > y ? x : y;
+    }
+    return x;
+}
+
+/* The same for G < 64 lanes to a row: each round the largest order, its lowest
+ * place, and that one taken out. */
 template <int G, int PER, int W>
 __device__ void group_top(const float x[PER], int n, const Outputs& o, int64_t r, Sums s, float log_sum) {
+    static_assert(G == 1 || G == 4 || G == 16, "group_most");
     const int lane = threadIdx.x % G;
-    uint64_t last = ~0ull;
+    uint32_t order[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) order[i] = ((i / W) * G + lane) * W + i % W < n ? order_of(x[i]) : 0;
     for (int k = 0; k < o.top; k++) {
-        uint64_t best = 0;
+        uint32_t most = order[0];
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int j = ((i / W) * G + lane) * W + i % W;
-            uint64_t key = (uint64_t)order_of(x[i]) << 32 | (uint32_t)~j;
-            if (j < n && key < last && key > best) best = key;
-        }
+        for (int i = 1; i < PER; i++) most = most > order[i] ? most : order[i];
+        most = group_most<G>(most);
+        uint32_t not_place = 0;                  // the complement of the place: the lowest is the largest
 #pragma unroll
-        for (int d = 1; d < G; d *= 2) {
-            uint64_t other = __shfl_xor(best, d);
-            best = best > other ? best : other;
-        }
-        last = best;
-        if (lane == 0) write_top(o, r, k, (uint32_t)(best >> 32), (uint32_t)~(uint32_t)best, s, log_sum);
+        for (int i = PER - 1; i >= 0; i--) not_place = order[i] == most ? ~(uint32_t)(((i / W) * G + lane) * W + i % W) : not_place;
+        not_place = group_most<G>(not_place);
+#pragma unroll
+        for (int i = 0; i < PER; i++) order[i] = ~(uint32_t)(((i / W) * G + lane) * W + i % W) == not_place ? 0 : order[i];
+        if (lane == 0) write_top(o, r, k, most, ~not_place, s, log_sum);
     }
 }
 
@@ -425,7 +446,7 @@ __global__ __launch_bounds__(kThreads) void lp_small(B3Logits g, Outputs o) {
     const float log_sum = logf(s.s);
     if (lane == 0) finish_row(g, o, r, a, xa, s, log_sum);
     if (!o.top) return;
-    if (G == kWave) {
+    if constexpr (G == kWave) {
         uint32_t order[PER], my_order;
         int v, l, w;
 #pragma unroll
