@@ -638,14 +638,20 @@ __global__ __launch_bounds__(THREADS) void lp_piece(B3Logits g, Outputs o, Piece
         p.top[(r * p.count + piece) * o.top + threadIdx.x] = make_uint2(0, 0);
 }
 
-/* A wave to a row: up to 256 pieces, four to a lane.  With alternatives three
- * more waves fetch the lists. */
-template <typename T>
+/* A wave to a row, HEADS pieces to a lane.  With alternatives three more
+ * waves fetch the lists.  Everything is fetched before anything is used. */
+template <typename T, int HEADS>
 __global__ __launch_bounds__(kThreads) void lp_join(B3Logits g, Outputs o, Pieces p) {
-    constexpr int kHeads = kMaxPieces / kWave;
     extern __shared__ uint2 lists[];             // [count][top]
     const int64_t r = blockIdx.x;
     const int lane = threadIdx.x;
+    const int64_t a = o.taken[r];
+    Sums sums[HEADS];
+#pragma unroll
+    for (int q = 0; q < HEADS; q++) {
+        const int c = q * kWave + lane;
+        sums[q] = p.sums[r * p.count + (c < p.count ? c : 0)];
+    }
     /* the pieces' lists are sorted, and of equal orders the one of the lower
      * piece has the lower action */
     const int entries = p.count * o.top;
@@ -657,50 +663,51 @@ __global__ __launch_bounds__(kThreads) void lp_join(B3Logits g, Outputs o, Piece
 #pragma unroll
         for (int k = 0; k < 4; k++) lists[min(i + k * (int)blockDim.x, entries - 1)] = it[k];
     }
-    const int64_t a = o.taken[r];
     const float xa = taken_logit<T>(g, r, a);
     __syncthreads();
     if (threadIdx.x >= kWave) return;
     Sums part = {0, 0, 0};
 #pragma unroll
-    for (int q = 0; q < kHeads; q++) {
-        const int c = q * kWave + lane;
-        if (c < p.count) part = join(part, p.sums[r * p.count + c]);
-    }
+    for (int q = 0; q < HEADS; q++)
+        if (q * kWave + lane < p.count) part = join(part, sums[q]);
 #pragma unroll
     for (int d = 1; d < kWave; d *= 2)
         part = join(part, Sums{__shfl_xor(part.m, d), __shfl_xor(part.s, d), __shfl_xor(part.d, d)});
-    const Sums all = part;
-    const float log_sum = logf(all.s);
-    if (lane == 0) finish_row(g, o, r, a, xa, all, log_sum);
+    const float log_sum = logf(part.s);
+    if (lane == 0) finish_row(g, o, r, a, xa, part, log_sum);
     if (!o.top) return;
-    uint2 head[kHeads];
-    int next[kHeads];
+    /* the first of each list that is left, the largest of these, and so on;
+     * lane k keeps the k-th */
+    uint2 head[HEADS], mine = make_uint2(0, 0);
+    int next[HEADS];
 #pragma unroll
-    for (int q = 0; q < kHeads; q++) {
+    for (int q = 0; q < HEADS; q++) {
         const int c = q * kWave + lane;
         head[q] = c < p.count ? lists[c * o.top] : make_uint2(0, 0);
-        next[q] = 1;
+        next[q] = c * o.top + 1;
     }
     for (int k = 0; k < o.top; k++) {
         uint32_t most = head[0].x;
 #pragma unroll
-        for (int q = 1; q < kHeads; q++) most = most > head[q].x ? most : head[q].x;
+        for (int q = 1; q < HEADS; q++) most = most > head[q].x ? most : head[q].x;
         most = wave_most(most);
         bool found = false;
 #pragma unroll
-        for (int q = 0; q < kHeads; q++) {
+        for (int q = 0; q < HEADS; q++) {
             const uint64_t have = __ballot(head[q].x == most);
             if (!found && have) {
                 found = true;
-                if (lane == __builtin_ctzll(have)) {
-                    write_top(o, r, k, most, head[q].y, all, log_sum);
-                    head[q] = next[q] < o.top ? lists[(q * kWave + lane) * o.top + next[q]] : make_uint2(0, 0);
+                const int who = __builtin_ctzll(have);
+                const uint32_t action = __builtin_amdgcn_readlane(head[q].y, who);
+                mine = lane == k ? make_uint2(most, action) : mine;
+                if (lane == who) {
+                    head[q] = next[q] < (q * kWave + lane + 1) * o.top ? lists[next[q]] : make_uint2(0, 0);
                     next[q]++;
                 }
             }
         }
     }
+    if (lane < o.top) write_top(o, r, lane, mine.x, mine.y, part, log_sum);
 }
 
 /* ---- backward ---- */
@@ -884,7 +891,12 @@ hipError_t forward(const B3Logits& g, const Outputs& o, Pieces p, hipStream_t st
         launch_piece<T, 512, kWide / 512, W>(g, o, p, grid, stream);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess || p.count == 1) return err;
-    lp_join<T><<<(unsigned)g.rows, o.top ? kThreads : kWave, (size_t)p.count * o.top * sizeof(uint2), stream>>>(g, o, p);
+    const size_t lists = (size_t)p.count * o.top * sizeof(uint2);
+    const int threads = o.top ? kThreads : kWave;
+    if (p.count <= kWave)
+        lp_join<T, 1><<<(unsigned)g.rows, threads, lists, stream>>>(g, o, p);
+    else
+        lp_join<T, kMaxPieces / kWave><<<(unsigned)g.rows, threads, lists, stream>>>(g, o, p);
     return hipGetLastError();
 }
 
