@@ -433,7 +433,7 @@ __device__ void group_top(const float x[PER], int n, const Outputs& o, int64_t r
 
 /* G lanes to a row: up to G PER actions. */
 template <typename T, int G, int PER, int W>
-__global__ __launch_bounds__(kThreads) void lp_small(B3Logits g, Outputs o) {
+__global__ __launch_bounds__(kThreads, 8) void lp_small(B3Logits g, Outputs o) {
     const int64_t r = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / G;
     if (r >= g.rows) return;                     // all G lanes of it
     const int lane = threadIdx.x % G, n = (int)g.actions;
@@ -523,7 +523,7 @@ __device__ __forceinline__ Bound wave_bound(const float x[PER], float lane_most,
  * that would be too long (many large logits in one lane's places) go by
  * wave_top, all waves' in the end ranked alike. */
 template <typename T, int THREADS, int PER, int W, bool TOP>
-__global__ __launch_bounds__(THREADS) void lp_piece(B3Logits g, Outputs o, Pieces p) {
+__global__ __launch_bounds__(THREADS, TOP ? 6 : 8) void lp_piece(B3Logits g, Outputs o, Pieces p) {
     constexpr int kWaves = THREADS / kWave, kList = 1024;
     static_assert(PER <= 32, "a bit for each");
     static_assert(kList >= kWaves * B3_MAX_TOP, "the waves' alternatives");
@@ -810,7 +810,7 @@ void with_small(int64_t actions, F f) {
         f.template operator()<T, 64, 32, W>();
 }
 
-constexpr int kSmall = 2048, kShortPiece = 4096, kPiece = 8192, kWide = 16384;
+constexpr int kSmall = 2048, kShortPiece = 4096, kPiece = 8192;
 constexpr int64_t kFill = 512;                   // workgroups: two to a compute unit
 
 template <typename F>
@@ -829,19 +829,15 @@ void with_type(int type, F f) {
  * us for both passes, 12.4 us past the caches). */
 bool stream_logits(const B3Logits& g) { return g.rows * g.actions * (g.type == B3_F32 ? 4 : 2) > (int64_t)1 << 28; }
 
-/* Pieces of a row.  8,192 actions to a workgroup of 256 are the fastest where
- * rows are many (4,096 rows of 131,072 in bf16: 177 us; 16,384 to 512 threads
- * 181 us, to 1,024 286 us), but for rows that 512 threads hold well filled,
- * which save the join (16,384 rows of 16,384: 85 us, not 101; of 9,000: 106
- * us, not 83).  Where pieces of 8,192 would not give every compute unit two,
- * 4,096. */
+/* Pieces of a row.  8,192 actions to a workgroup of 256 threads, also where
+ * one of 512 could hold the row (16,384 rows of 16,384 in bf16: 86 us, not
+ * 103; of 14,000: 82 us, not 123): with fewer to a barrier, loads and sums of
+ * different workgroups overlap.  Where pieces of 8,192 would not give every
+ * compute unit two, 4,096. */
 Pieces pieces_of(int64_t rows, int64_t actions) {
     Pieces p = {};
     p.size = kPiece;
-    if (actions > kWide * 3 / 4 && actions <= kWide && rows >= kFill)
-        p.size = kWide;
-    else if (rows * ceil_div(actions, kPiece) < kFill && ceil_div(actions, kShortPiece) <= kMaxPieces)
-        p.size = kShortPiece;
+    if (rows * ceil_div(actions, kPiece) < kFill && ceil_div(actions, kShortPiece) <= kMaxPieces) p.size = kShortPiece;
     p.count = actions <= kSmall ? 1 : (int)ceil_div(actions, p.size);
     return p;
 }
@@ -885,10 +881,8 @@ hipError_t forward(const B3Logits& g, const Outputs& o, Pieces p, hipStream_t st
     const int64_t most = p.count == 1 ? g.actions : p.size;
     if (most <= kShortPiece)
         launch_piece<T, 128, kShortPiece / 128, W>(g, o, p, grid, stream);
-    else if (most <= kPiece)
-        launch_piece<T, 256, kPiece / 256, W>(g, o, p, grid, stream);
     else
-        launch_piece<T, 512, kWide / 512, W>(g, o, p, grid, stream);
+        launch_piece<T, 256, kPiece / 256, W>(g, o, p, grid, stream);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess || p.count == 1) return err;
     const size_t lists = (size_t)p.count * o.top * sizeof(uint2);
