@@ -60,8 +60,8 @@ struct Moments {
 /* Workgroups to a chunk, and vectors of a thread in flight.  In 32 bits four
  * workgroups of one vector a thread: 400 million weights took 2,061 us, and
  * 2,109 us as one workgroup that goes on twice over two vectors; 30 million
- * in bf16 155 and 171 us.  With 8-bit moments, where a vector's work is four
- * times as long, the other way about: 200 million weights 660 and 602 us. */
+ * in bf16 155 and 171 us.  With 8-bit moments, where a vector is more work for
+ * fewer bytes, the other way about: 200 million weights 660 and 602 us. */
 template <int BITS>
 struct Shape {
     static constexpr int kParts = BITS == 32 ? 4 : 1, kUnroll = BITS == 32 ? 1 : 2;
@@ -93,6 +93,7 @@ struct B3AdamW {
 namespace b3p {
 namespace {
 
+/* 32 well mixed bits of 32: two rounds of shift, xor and multiply. */
 inline __host__ __device__ uint32_t mix(uint32_t x) {
     x ^= x >> 16;
     x *= 0x7feb352du;
@@ -405,17 +406,30 @@ __global__ __launch_bounds__(kSumThreads) void aw_norm(const double* partial, in
     }
 }
 
-/* ---- 8-bit moments in and out: a thread to four elements ---- */
+/* ---- 8-bit moments in and out ---- */
+
+/* Eight of one of the moments a thread, so that neighbouring threads write 16
+ * neighbouring bytes each. */
+constexpr int kMomentsOut = 8;
+
+template <bool ROOT>
+__device__ __forceinline__ void moments_of(const uint8_t* codes, const uint8_t* scales, int64_t i, __bf16* out) {
+    const uint2 c = *(const uint2*)(codes + i);
+    const uint8_t scale = scales[i / kGroup];
+    float x[kMomentsOut];
+    unpack(c.x, scale, x);
+    unpack(c.y, scale, x + kVector);
+    Pack<__bf16, kMomentsOut> y;
+#pragma unroll
+    for (int k = 0; k < kMomentsOut; k++) y.v[k] = (__bf16)(ROOT ? x[k] * x[k] : x[k]);
+    Stream<__bf16, kMomentsOut>::store(out + i, y);
+}
 
 __global__ __launch_bounds__(kThreads) void aw_moments(Moments mo, int64_t size, __bf16* exp_avg, __bf16* exp_avg_sq) {
-    const int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * kVector;
-    if (i >= size) return;
-    float m[kVector], r[kVector];
-    unpack(*(const uint32_t*)((const uint8_t*)mo.exp_avg + i), mo.exp_avg_scale[i / kGroup], m);
-    unpack(*(const uint32_t*)((const uint8_t*)mo.exp_avg_sq + i), mo.exp_avg_sq_scale[i / kGroup], r);
-    for (int k = 0; k < kVector; k++) r[k] *= r[k];
-    store<true>(exp_avg, i, size, m);
-    store<true>(exp_avg_sq, i, size, r);
+    const int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * kMomentsOut;
+    if (i >= size) return;                        // a multiple of 256
+    moments_of<false>((const uint8_t*)mo.exp_avg, mo.exp_avg_scale, i, exp_avg);
+    moments_of<true>((const uint8_t*)mo.exp_avg_sq, mo.exp_avg_sq_scale, i, exp_avg_sq);
 }
 
 __global__ __launch_bounds__(kThreads) void aw_load(Moments mo, int64_t size, const float* inverse,
@@ -626,7 +640,7 @@ hipError_t b3_adamw_moments_gpu(const B3AdamW* o, void* exp_avg, void* exp_avg_s
     if (!o || o->bits != 8 || (o->size && (!exp_avg || !exp_avg_sq))) return hipErrorInvalidValue;
     hipError_t err = on_device(o);
     if (err != hipSuccess || o->size == 0) return err;
-    aw_moments<<<(unsigned)ceil_div(o->size, kThreads * kVector), kThreads, 0, stream>>>(o->moments, o->size,
+    aw_moments<<<(unsigned)ceil_div(o->size, kThreads * kMomentsOut), kThreads, 0, stream>>>(o->moments, o->size,
         (__bf16*)exp_avg, (__bf16*)exp_avg_sq);
     return hipGetLastError();
 }
