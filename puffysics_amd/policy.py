@@ -209,7 +209,7 @@ def log_probs(logits, taken, mask=None, top=0):
     action past the last has log_prob NaN."""
     _need(logits.dtype in _TYPE, "logits have to be float32, float16 or bfloat16")
     _need(logits.dim() >= 1 and logits.shape[-1] >= 1, "logits need at least one action")
-    _need(not taken.is_floating_point() and taken.dtype != torch.bool, "taken has to be whole numbers")
+    _need(not (taken.is_floating_point() or taken.is_complex() or taken.dtype == torch.bool), "taken has to be whole numbers")
     _need(taken.shape == logits.shape[:-1], "taken has to have the shape of logits without the last axis")
     actions = logits.shape[-1]
     _need(0 <= top <= MAX_TOP and top <= actions, "top has to be between 0 and 32, and at most the actions")
@@ -307,6 +307,7 @@ class AdamW:
         _need(len(decay) == n and all(d >= 0 for d in decay), "weight_decay has to be at least 0, one for each tensor")
         _need(0 <= betas[0] < 1 and 0 <= betas[1] < 1 and eps >= 0, "betas have to be in [0, 1), eps at least 0")
         _need(state_bits in (8, 32), "state_bits has to be 8 or 32")
+        _need(max_grad_norm is None or max_grad_norm > 0, "max_grad_norm has to be over 0, or None")
         self.lr, self.max_grad_norm, self.state_bits = lr, max_grad_norm, state_bits
         self.device = torch.device("cuda", torch.cuda.current_device())
         self._lib = policy_lib()
@@ -348,6 +349,7 @@ class AdamW:
         if grads is None:
             grads = [p.grad for p in self.params]
         _need(len(grads) == len(self.params), "need one gradient for each parameter")
+        _need(self.max_grad_norm is None or self.max_grad_norm > 0, "max_grad_norm has to be over 0, or None")
         if [p.data_ptr() for p in self.params] != self._at:
             raise ValueError("a parameter's memory is not where it was")
         stepped, shapes, dtypes, given = self.params, self._shapes, self._dtypes, grads
@@ -367,7 +369,7 @@ class AdamW:
             pointers = array.array("Q", [0 if g is None else g.data_ptr() for g in grads])
         kinds = None if types == dtypes else \
             array.array("i", [_TYPE[d if g is None else g.dtype] for g, d in zip(grads, self._dtypes)])
-        norm = torch.empty((), dtype=torch.float32, device=self.device) if self.max_grad_norm else None
+        norm = torch.empty((), dtype=torch.float32, device=self.device) if self.max_grad_norm is not None else None
         _check("b3_adamw_step_gpu", self._lib.b3_adamw_step_gpu(
             self._h, pointers.buffer_info()[0], kinds.buffer_info()[0] if kinds else None,
             self.lr if lr is None else lr, self.max_grad_norm or 0.0,
@@ -402,12 +404,13 @@ class AdamW:
               "need one tensor for each parameter")
         _need(step >= 0, "step has to be at least 0")
         _need(master is None or self._master is not None, "this optimizer keeps no 32-bit copies")
+        for given in (exp_avg, exp_avg_sq, master or []):
+            _need(all(x.shape == p.shape for x, p in zip(given, self.params)), "need tensors of the parameters' shapes")
         flat = (self._exp_avg, self._exp_avg_sq) if self.state_bits == 32 else \
             torch.zeros((2, self.size), dtype=torch.float32, device=self.device)
         lists = [(flat[0], exp_avg), (flat[1], exp_avg_sq)] + ([(self._master, master)] if master is not None else [])
         for to, given in lists:
             for view, x in zip(self._views(to), given):
-                _need(x.shape == view.shape, "need tensors of the parameters' shapes")
                 view.copy_(x)
         if self.state_bits == 8:
             _check("b3_adamw_load_moments_gpu", self._lib.b3_adamw_load_moments_gpu(

@@ -387,6 +387,34 @@ def test_refusals_of_gradients():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+def test_refused_moments_leave_the_state(bits):
+    from puffysics_amd import policy
+    p = [torch.zeros(40, device="cuda"), torch.zeros(7, device="cuda", dtype=torch.bfloat16)]
+    opt = policy.AdamW(p, LR, state_bits=bits)
+    good, bad = [torch.ones(40), torch.ones(7)], [torch.ones(40), torch.ones(8)]
+    for args in ((bad, good, 3), (good, bad, 3), (good, good, 3, bad)):
+        with pytest.raises(ValueError):
+            opt.load_moments(*args)
+    assert all(int(torch.count_nonzero(x)) == 0 for x in (*opt.moments(), opt.master())) and opt.steps() == 0
+
+
+@pytest.mark.gpu
+def test_a_clip_of_0_is_refused():
+    """Also where it is set later: it would have meant no clip at all."""
+    from puffysics_amd import policy
+    p = torch.zeros(5, device="cuda")
+    for most in (0.0, 0, -1.0, float("nan")):
+        with pytest.raises(ValueError):
+            policy.AdamW([p], LR, max_grad_norm=most)
+        opt = policy.AdamW([p], LR, max_grad_norm=1.0)
+        opt.max_grad_norm = most
+        with pytest.raises(ValueError):
+            opt.step([torch.ones(5, device="cuda")])
+        assert opt.steps() == 0 and int(torch.count_nonzero(p)) == 0
+
+
+@pytest.mark.gpu
 def test_a_step_is_an_operation_in_place():
     """Autograd notices weights that were stepped between a forward pass and
     its backward; a parameter whose memory went elsewhere is refused."""

@@ -374,6 +374,12 @@ def test_refusals():
         policy.log_probs(torch.zeros(4, 600), t, top=33)
 
 
+def test_complex_actions_are_refused():
+    from puffysics_amd import policy
+    with pytest.raises(ValueError, match="whole numbers"):
+        policy.log_probs(torch.zeros(4, 6), torch.zeros(4, dtype=torch.complex64))
+
+
 def test_refusals_of_the_c_entry():
     from puffysics_amd import policy
     lib = policy.policy_lib()
