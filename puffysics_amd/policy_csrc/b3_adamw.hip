@@ -214,9 +214,10 @@ struct Step {
     uint32_t key;
 };
 
-/* The vectors of a thread that are in flight together.  The square root is the correctly rounded one,
- * since what is kept of it is cut off by random bits; the division in the
- * update is a reciprocal, good to two units. */
+/* The vectors of a thread that are in flight together.  The square root is the
+ * correctly rounded one, since what is kept of it is cut off by random bits
+ * (the hardware's with its residuals' correction took as long, and gives 0 for
+ * denormals); the division in the update is a reciprocal, good to two units. */
 template <typename P, typename G, bool MASTER, int BITS, bool FULL>
 __device__ __forceinline__ void step_turn(const Tensor& t, int64_t from, const G* grad, const Step& s) {
     constexpr int kUnroll = Shape<BITS>::kUnroll;
@@ -425,16 +426,18 @@ __device__ __forceinline__ void moments_of(const uint8_t* codes, const uint8_t* 
     Stream<__bf16, kMomentsOut>::store(out + i, y);
 }
 
-__global__ __launch_bounds__(kThreads) void aw_moments(Moments mo, int64_t size, __bf16* exp_avg, __bf16* exp_avg_sq) {
-    const int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * kMomentsOut;
+/* Element i of the flat arrays, from `first` on, to a thread. */
+__global__ __launch_bounds__(kThreads) void aw_moments(Moments mo, int64_t first, int64_t size, __bf16* exp_avg,
+    __bf16* exp_avg_sq) {
+    const int64_t i = first + ((int64_t)blockIdx.x * kThreads + threadIdx.x) * kMomentsOut;
     if (i >= size) return;                        // a multiple of 256
     moments_of<false>((const uint8_t*)mo.exp_avg, mo.exp_avg_scale, i, exp_avg);
     moments_of<true>((const uint8_t*)mo.exp_avg_sq, mo.exp_avg_sq_scale, i, exp_avg_sq);
 }
 
-__global__ __launch_bounds__(kThreads) void aw_load(Moments mo, int64_t size, const float* inverse,
+__global__ __launch_bounds__(kThreads) void aw_load(Moments mo, int64_t first, int64_t size, const float* inverse,
     const float* exp_avg, const float* exp_avg_sq) {
-    const int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * kVector;
+    const int64_t i = first + ((int64_t)blockIdx.x * kThreads + threadIdx.x) * kVector;
     if (i >= size) return;                        // a multiple of 256: groups stay whole
     float m[kVector], r[kVector];
     load<true, true>(exp_avg, i, size, m);
@@ -468,6 +471,17 @@ int batch(const B3AdamW* o, int base) { return o->count - base < kBatch ? o->cou
 int sum_blocks(const B3AdamW* o, int base) {
     const int64_t chunks = o->first[base + batch(o, base)] - o->first[base];
     return (int)(chunks < kSumBlocks ? chunks : kSumBlocks);
+}
+
+template <int BITS>
+void launch_step(const B3AdamW* o, const StepArgs& a, int base, int64_t first, int64_t end, const Rates& rates, const Clip& clip,
+        hipStream_t stream) {
+    constexpr int64_t kMost = kMostBlocks / Shape<BITS>::kParts;
+    for (; first < end; first += kMost) {
+        const int64_t chunks = end - first < kMost ? end - first : kMost;
+        aw_step<BITS><<<(unsigned)(chunks * Shape<BITS>::kParts), kThreads, 0, stream>>>(a, base, first, o->chunk, o->tensors,
+            o->moments, rates, o->inverse, clip);
+    }
 }
 
 hipError_t on_device(const B3AdamW* o) {
@@ -517,7 +531,7 @@ hipError_t b3_adamw_create(B3AdamW** out, const B3AdamWTensor* tensors, int coun
             || (state.bits == 8 && (!state.exp_avg_scale || !state.exp_avg_sq_scale))))
         return hipErrorInvalidValue;
     for (int i = 0; i < count; i++) chunks += ceil_div(tensors[i].numel, kChunk);
-    if (chunks > 0x7fffffff / Shape<32>::kParts) return hipErrorInvalidValue;
+    if (chunks > 0x7fffffff) return hipErrorInvalidValue;
     B3AdamW* o = (B3AdamW*)calloc(1, sizeof(B3AdamW));
     if (!o) return hipErrorOutOfMemory;
     o->count = count;
@@ -610,11 +624,9 @@ hipError_t b3_adamw_step_gpu(B3AdamW* o, const void* const* grads, const int* gr
                 aw_squares<<<blocks, kThreads, 0, stream>>>(a, base, first, end, o->chunk, o->tensors, partial);
                 partial += blocks;
             } else if (o->bits == 32) {
-                aw_step<32><<<(unsigned)((end - first) * Shape<32>::kParts), kThreads, 0, stream>>>(a, base, first, o->chunk, o->tensors,
-                    o->moments, rates, o->inverse, clip);
+                launch_step<32>(o, a, base, first, end, rates, clip, stream);
             } else {
-                aw_step<8><<<(unsigned)((end - first) * Shape<8>::kParts), kThreads, 0, stream>>>(a, base, first, o->chunk, o->tensors,
-                    o->moments, rates, o->inverse, clip);
+                launch_step<8>(o, a, base, first, end, rates, clip, stream);
             }
             if ((err = hipGetLastError()) != hipSuccess) return err;
         }
@@ -640,18 +652,28 @@ hipError_t b3_adamw_moments_gpu(const B3AdamW* o, void* exp_avg, void* exp_avg_s
     if (!o || o->bits != 8 || (o->size && (!exp_avg || !exp_avg_sq))) return hipErrorInvalidValue;
     hipError_t err = on_device(o);
     if (err != hipSuccess || o->size == 0) return err;
-    aw_moments<<<(unsigned)ceil_div(o->size, kThreads * kMomentsOut), kThreads, 0, stream>>>(o->moments, o->size,
-        (__bf16*)exp_avg, (__bf16*)exp_avg_sq);
-    return hipGetLastError();
+    const int64_t most = kMostBlocks * kThreads * kMomentsOut;
+    for (int64_t first = 0; first < o->size && err == hipSuccess; first += most) {
+        const int64_t n = o->size - first < most ? o->size - first : most;
+        aw_moments<<<(unsigned)ceil_div(n, kThreads * kMomentsOut), kThreads, 0, stream>>>(o->moments, first, o->size,
+            (__bf16*)exp_avg, (__bf16*)exp_avg_sq);
+        err = hipGetLastError();
+    }
+    return err;
 }
 
 hipError_t b3_adamw_load_moments_gpu(B3AdamW* o, const float* exp_avg, const float* exp_avg_sq, hipStream_t stream) {
     if (!o || o->bits != 8 || (o->size && (!exp_avg || !exp_avg_sq))) return hipErrorInvalidValue;
     hipError_t err = on_device(o);
     if (err != hipSuccess || o->size == 0) return err;
-    aw_load<<<(unsigned)ceil_div(o->size, kThreads * kVector), kThreads, 0, stream>>>(o->moments, o->size, o->inverse,
-        exp_avg, exp_avg_sq);
-    return hipGetLastError();
+    const int64_t most = kMostBlocks * kThreads * kVector;
+    for (int64_t first = 0; first < o->size && err == hipSuccess; first += most) {
+        const int64_t n = o->size - first < most ? o->size - first : most;
+        aw_load<<<(unsigned)ceil_div(n, kThreads * kVector), kThreads, 0, stream>>>(o->moments, first, o->size, o->inverse,
+            exp_avg, exp_avg_sq);
+        err = hipGetLastError();
+    }
+    return err;
 }
 
 }  // extern "C"

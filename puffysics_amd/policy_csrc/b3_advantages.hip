@@ -365,6 +365,19 @@ size_t workspace_of(const Plan& p, int64_t envs) {
     return p.pieces > 1 ? (size_t)p.pieces * envs * sizeof(Map) : 0;
 }
 
+/* Environments from `first` on. */
+B3Rollout some_envs(B3Rollout g, int64_t first, int64_t envs) {
+    const int64_t value = g.values_type == B3_F32 ? 4 : 2, end = g.terminals_type == B3_F32 ? 4 : 1;
+    g.envs = envs;
+    g.rewards += first * g.rewards_stride[1];
+    g.values = (const char*)g.values + first * g.values_stride[1] * value;
+    g.last_values = (const char*)g.last_values + first * g.last_values_stride * value;
+    g.terminals = (const char*)g.terminals + first * g.terminals_stride[1] * end;
+    g.advantages += first * g.out_stride[1];
+    g.returns += first * g.out_stride[1];
+    return g;
+}
+
 }  // namespace
 }  // namespace b3p
 
@@ -388,9 +401,18 @@ hipError_t b3_advantages_gpu(const B3Rollout* g, double gamma, double lambda, vo
     if (workspace_bytes < need || (need && !workspace)) return hipErrorInvalidValue;
     const bool wide = g->rewards_stride[0] == 1 && g->values_stride[0] == 1 && g->terminals_stride[0] == 1
         && g->out_stride[0] == 1;
-    const Job job = {*g, (float)gamma, (float)(gamma * lambda), wide, stream_inputs(*g, p), p.tiles, p.pieces, (Map*)workspace};
-    return g->values_type == B3_F32 ? launch_values<B3_F32>(job, p, stream)
-        : g->values_type == B3_F16 ? launch_values<B3_F16>(job, p, stream) : launch_values<B3_BF16>(job, p, stream);
+    Job job = {*g, (float)gamma, (float)(gamma * lambda), wide, stream_inputs(*g, p), p.tiles, p.pieces, (Map*)workspace};
+    /* cut steps have few blocks: more than a launch's are of whole rollouts */
+    const int64_t most = kMostBlocks * p.cols;
+    hipError_t err = hipSuccess;
+    for (int64_t e = 0; e < g->envs && err == hipSuccess; e += most) {
+        Plan part = p;
+        job.g = some_envs(*g, e, g->envs - e < most ? g->envs - e : most);
+        part.blocks = ceil_div(job.g.envs, p.cols);
+        err = g->values_type == B3_F32 ? launch_values<B3_F32>(job, part, stream)
+            : g->values_type == B3_F16 ? launch_values<B3_F16>(job, part, stream) : launch_values<B3_BF16>(job, part, stream);
+    }
+    return err;
 }
 
 }  // extern "C"

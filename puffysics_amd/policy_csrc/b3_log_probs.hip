@@ -906,10 +906,21 @@ hipError_t backward(const B3Logits& g, const Upstream& u, hipStream_t stream) {
     return hipGetLastError();
 }
 
-/* The rows' count keeps every grid below 2^31 workgroups. */
+/* Rows to a launch: no kernel has more workgroups to a row than a piece of
+ * 4,096 (or less) takes. */
+int64_t rows_of_launch(int64_t actions) { return kMostBlocks / ceil_div(actions, kShortPiece); }
+
+/* Rows `first` to `first` + `rows`. */
+B3Logits some_rows(B3Logits g, int64_t first, int64_t rows) {
+    g.data = (const char*)g.data + first * g.row_stride * (g.type == B3_F32 ? 4 : 2);
+    if (g.mask) g.mask += first * g.mask_row_stride;
+    g.rows = rows;
+    return g;
+}
+
 bool valid(const B3Logits& g, const int64_t* taken) {
     return is_float_type(g.type) && g.rows >= 0 && g.rows <= 0x7fffffff && g.actions >= 1 && g.actions <= kMaxActions
-        && g.rows * ceil_div(g.actions, 1024) <= 0x7fffffff && g.row_stride >= g.actions
+        && g.row_stride >= g.actions
         && (!g.mask || g.mask_row_stride == 0 || g.mask_row_stride >= g.actions) && (g.rows == 0 || (g.data && taken));
 }
 
@@ -933,13 +944,30 @@ hipError_t b3_log_probs_gpu(B3Logits g, const int64_t* taken, float* log_prob, f
     if (workspace_bytes < need || (need && !workspace)) return hipErrorInvalidValue;
     if (g.rows == 0) return hipSuccess;
     if (!log_prob || !entropy || (top && (!top_log_prob || !top_action))) return hipErrorInvalidValue;
-    const Outputs o = {taken, log_prob, entropy, stats, top, top_log_prob, top_action};
+    Outputs o = {taken, log_prob, entropy, stats, top, top_log_prob, top_action};
     Pieces p = pieces_of(g.rows, g.actions);
     p.once = stream_logits(g);
     p.top = (uint2*)workspace;
     p.sums = (Sums*)((char*)workspace + (size_t)g.rows * p.count * top * sizeof(uint2));
+    const int64_t most = rows_of_launch(g.actions);
     hipError_t err = hipSuccess;
-    with_type(g.type, [&](auto t) { err = forward<decltype(t)>(g, o, p, stream); });
+    for (int64_t r = 0; r < g.rows && err == hipSuccess; r += most) {
+        const int64_t rows = g.rows - r < most ? g.rows - r : most;
+        const B3Logits part = some_rows(g, r, rows);
+        with_type(g.type, [&](auto t) { err = forward<decltype(t)>(part, o, p, stream); });
+        o.taken += rows;
+        o.log_prob += rows;
+        o.entropy += rows;
+        if (stats) o.stats += 2 * rows;
+        if (top) {
+            o.top_log_prob += rows * top;
+            o.top_action += rows * top;
+        }
+        if (need) {
+            p.sums += rows * p.count;
+            p.top += rows * p.count * top;
+        }
+    }
     return err;
 }
 
@@ -949,10 +977,21 @@ hipError_t b3_log_probs_backward_gpu(B3Logits g, const int64_t* taken, const flo
     if (!valid(g, taken) || d_row_stride < g.actions || dl_stride < 0 || dh_stride < 0) return hipErrorInvalidValue;
     if (g.rows == 0) return hipSuccess;
     if (!stats || !entropy || !d_logits) return hipErrorInvalidValue;
-    const Upstream u = {taken, stats, entropy, d_log_prob, dl_stride, d_entropy, dh_stride, d_logits, d_row_stride,
+    Upstream u = {taken, stats, entropy, d_log_prob, dl_stride, d_entropy, dh_stride, d_logits, d_row_stride,
         stream_logits(g)};
+    const int64_t most = rows_of_launch(g.actions);
     hipError_t err = hipSuccess;
-    with_type(g.type, [&](auto t) { err = backward<decltype(t)>(g, u, stream); });
+    for (int64_t r = 0; r < g.rows && err == hipSuccess; r += most) {
+        const int64_t rows = g.rows - r < most ? g.rows - r : most;
+        const B3Logits part = some_rows(g, r, rows);
+        with_type(g.type, [&](auto t) { err = backward<decltype(t)>(part, u, stream); });
+        u.taken += rows;
+        u.stats += 2 * rows;
+        u.entropy += rows;
+        if (d_log_prob) u.d_log_prob += rows * dl_stride;
+        if (d_entropy) u.d_entropy += rows * dh_stride;
+        u.out = (char*)u.out + rows * d_row_stride * (g.type == B3_F32 ? 4 : 2);
+    }
     return err;
 }
 

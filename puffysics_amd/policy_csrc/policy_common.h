@@ -56,6 +56,10 @@ inline __device__ float to_float(_Float16 x) { return (float)x; }
 inline __device__ float to_float(__bf16 x) { return (float)x; }
 
 inline bool is_float_type(int type) { return type == B3_F32 || type == B3_F16 || type == B3_BF16; }
+/* Workgroups of up to 256 threads that a launch may have: it takes fewer than
+ * 2^32 threads. */
+constexpr int64_t kMostBlocks = (1 << 24) - 1;
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace b3p

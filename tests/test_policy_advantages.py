@@ -128,6 +128,21 @@ def test_places_past_32_bits(by_env):
 
 
 @pytest.mark.gpu
+def test_more_environments_than_a_launch_takes():
+    """2^24 - 1 workgroups of 64 environments and some more; one step, so that
+    A = r - V, + gamma V_1 where the episode goes on, of three roundings."""
+    from puffysics_amd import policy
+    envs = (2 ** 24 - 1) * 64 + 70
+    last = (torch.arange(envs, dtype=torch.int32, device="cuda") % 251).to(torch.bfloat16)
+    ends = (torch.arange(envs, dtype=torch.int32, device="cuda") % 7 == 3).view(1, envs)
+    r, v = (torch.full((1, 1), x, device="cuda").expand(1, envs) for x in (0.5, 0.25))
+    adv, ret = policy.advantages(r, v.to(torch.bfloat16), ends, last, gamma=0.75)
+    want = torch.where(ends[0], 0.25, 0.75 * last.float() + 0.25)
+    assert float((adv[0] - want).abs().max()) <= 256 * 2.0 ** -23
+    assert float((ret[0] - adv[0] - 0.25).abs().max()) <= 256 * 2.0 ** -23
+
+
+@pytest.mark.gpu
 def test_nothing():
     from puffysics_amd import policy
     for steps, envs in ((0, 4), (4, 0), (0, 0)):

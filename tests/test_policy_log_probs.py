@@ -119,6 +119,40 @@ def test_rows_past_32_bits():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,actions", [(2 ** 24 + 3, 2), (2 ** 23 + 3, 4097)])
+def test_more_rows_than_a_launch_takes(rows, actions):
+    """What follows the rows of the first launch (2^24 - 1, or half as many of
+    two pieces) is what it is alone, in every result."""
+    from puffysics_amd import policy
+    odd = torch.tensor([0, rows // 2, rows - 77, rows - 5, rows - 4, rows - 3, rows - 2, rows - 1])
+    x = torch.zeros(rows, actions, dtype=torch.bfloat16, device="cuda")
+    x[odd] = inputs(len(odd), actions, "bf16", 1)[0]
+    taken = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    taken[odd] = torch.arange(len(odd), device="cuda") % 2
+    mask = torch.ones(actions, dtype=torch.bool, device="cuda")
+    if actions == 2:
+        mask = mask.repeat(rows, 1)
+        mask[odd[-2], 0] = False
+    x.requires_grad_(True)
+    dl, dh = torch.ones(rows, device="cuda"), torch.zeros(rows, device="cuda")
+    dl[odd], dh[odd] = torch.randn(len(odd), device="cuda"), torch.randn(len(odd), device="cuda")
+    got = policy.log_probs(x, taken, mask, top=2)
+    d, = torch.autograd.grad((got.log_prob, got.entropy), x, (dl, dh))
+    few = x.detach()[odd].requires_grad_(True)
+    alone = policy.log_probs(few, taken[odd], mask[odd] if mask.dim() == 2 else mask, top=2)
+    d_alone, = torch.autograd.grad((alone.log_prob, alone.entropy), few, (dl[odd], dh[odd]))
+    for a, b in zip(got, alone):
+        assert torch.allclose(a[odd].double(), b.double(), rtol=0, atol=SUM)
+    assert torch.allclose(d[odd].float(), d_alone.float(), rtol=2.0 ** -7, atol=1e-9)
+    other = torch.ones(rows, dtype=torch.bool, device="cuda")
+    other[odd] = False
+    assert float((got.log_prob.detach()[other] + np.log(actions)).abs().max()) < SUM
+    assert float((got.entropy.detach()[other] - np.log(actions)).abs().max()) < SUM
+    assert (got.top_action[other] == torch.arange(2, device="cuda")).all()
+    assert float((d[:, 0][other].float() - (1 - 1 / actions)).abs().max()) < 2.0 ** -8
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("type", TYPES)
 @pytest.mark.parametrize("actions,wide", [(3, 8), (21, 22), (1021, 1040), (4097, 5003), (40001, 40020)])
 def test_slices_of_wider_rows(actions, wide, type):
