@@ -129,7 +129,9 @@ typedef struct B3AdamWTensor {
  *                   moment): OCP e4m3 bytes, with the exponent byte b of a
  *                   scale 2^(b - 127) for every 32 of them
  * `master` holds the 32-bit copies that 16-bit weights are rounded from; NULL
- * keeps none, and the weights are then rounded to the nearest every step. */
+ * keeps none, and the weights are then rounded to the nearest every step.  A
+ * weight that is not what its copy rounds to (to the nearest) has been written
+ * since, and the next step goes on from the weight. */
 #define B3_ADAMW_SEGMENT 256
 typedef struct B3AdamWState {
     int bits;

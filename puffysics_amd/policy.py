@@ -287,7 +287,8 @@ class AdamW:
     max_grad_norm  the global norm that gradients are scaled down to, or None
     weight_decay   a number, or one for each tensor
     master         keep 32-bit copies of 16-bit weights and round those; without
-                   them small updates of such weights are lost
+                   them small updates of such weights are lost.  A weight that
+                   was written between two steps counts, not its copy
 
     The moments lie in flat arrays, tensor i's from offsets[i] on.  Steps of
     one optimizer follow one another: on several streams, order them."""
@@ -327,8 +328,7 @@ class AdamW:
         self._master = None
         if master and any(p.dtype != torch.float32 for p in self.params):
             self._master = new(self.size, torch.float32)
-            for p, m in zip(self.params, self._views(self._master)):
-                m.copy_(p.detach())
+            self._copy_weights()
         state = B3AdamWState(state_bits, self._exp_avg.data_ptr(), self._exp_avg_sq.data_ptr(),
                              self._scale[0].data_ptr(), self._scale[1].data_ptr(),
                              self._master.data_ptr() if self._master is not None else None)
@@ -340,6 +340,26 @@ class AdamW:
 
     def _views(self, flat):
         return [flat[at:at + p.numel()].view(p.shape) for at, p in zip(self.offsets, self.params)]
+
+    def _rounded(self):
+        """The 16-bit parameters and the views of their copies."""
+        return [(p, m) for p, m in zip(self.params, self._views(self._master)) if p.dtype != torch.float32]
+
+    @torch.inference_mode()
+    def _copy_weights(self):
+        for p, m in self._rounded():
+            m.copy_(p)
+        self._master_version = self._version()
+
+    @torch.inference_mode()
+    def _round_copies(self):
+        for p, m in self._rounded():
+            p.copy_(m)
+        self._master_version = self._version()
+
+    def _version(self):
+        """Changes where a program writes to the copies."""
+        return None if self._master.is_inference() else self._master._version
 
     def step(self, grads=None, lr=None):
         """One step by `grads` (one for each parameter, of its type or
@@ -369,6 +389,8 @@ class AdamW:
             pointers = array.array("Q", [0 if g is None else g.data_ptr() for g in grads])
         kinds = None if types == dtypes else \
             array.array("i", [_TYPE[d if g is None else g.dtype] for g, d in zip(grads, self._dtypes)])
+        if self._master is not None and self._version() != self._master_version:
+            self._round_copies()
         norm = torch.empty((), dtype=torch.float32, device=self.device) if self.max_grad_norm is not None else None
         _check("b3_adamw_step_gpu", self._lib.b3_adamw_step_gpu(
             self._h, pointers.buffer_info()[0], kinds.buffer_info()[0] if kinds else None,
@@ -389,7 +411,9 @@ class AdamW:
         return out[0], out[1]
 
     def master(self):
-        """The flat array of 32-bit copies of 16-bit weights, or None."""
+        """The flat array of 32-bit copies of 16-bit weights (the places of
+        32-bit weights hold nothing), or None.  What is written there is what
+        the next step goes on from."""
         return self._master
 
     def steps(self, i=0):
@@ -398,7 +422,8 @@ class AdamW:
 
     def load_moments(self, exp_avg, exp_avg_sq, step, master=None):
         """Go on from moments (lists of a tensor for each parameter) after
-        `step` steps, and from 32-bit copies of the weights if given."""
+        `step` steps.  Where 32-bit copies of the weights are given, 16-bit
+        weights become what these round to; else the copies are the weights."""
         n = len(self.params)
         _need(len(exp_avg) == n and len(exp_avg_sq) == n and (master is None or len(master) == n),
               "need one tensor for each parameter")
@@ -415,6 +440,10 @@ class AdamW:
         if self.state_bits == 8:
             _check("b3_adamw_load_moments_gpu", self._lib.b3_adamw_load_moments_gpu(
                 self._h, flat[0].data_ptr(), flat[1].data_ptr(), _stream()))
+        if master is not None:
+            self._round_copies()
+        elif self._master is not None:
+            self._copy_weights()
         for i in range(n):
             _check("b3_adamw_set_steps", self._lib.b3_adamw_set_steps(self._h, i, step))
 
