@@ -167,7 +167,8 @@ hipError_t b3_adamw_create(B3AdamW** out, const B3AdamWTensor* tensors, int coun
  * where max_norm is 0).  t counts a tensor's own steps, on the host: a
  * captured step replays the corrections of the step that was captured.
  * 8-bit moments are rounded to one of their two neighbours by random bits
- * that seed, t and place give; a root over 0 stays over 0.  Steps of one
+ * that seed, t and place give, and in a captured step the count of the
+ * optimizer's captured steps that have run; a root over 0 stays over 0.  Steps of one
  * optimizer must follow one another on the device. */
 hipError_t b3_adamw_step_gpu(B3AdamW* optimizer, const void* const* grads, const int* grad_types, double lr,
     double max_norm, float* norm, hipStream_t stream);

@@ -291,7 +291,9 @@ class AdamW:
                    was written between two steps counts, not its copy
 
     The moments lie in flat arrays, tensor i's from offsets[i] on.  Steps of
-    one optimizer follow one another: on several streams, order them."""
+    one optimizer follow one another: on several streams, order them.  A step
+    that is captured in a graph repeats the bias corrections of its own count
+    in every replay; 8-bit moments are rounded by other bits each time."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32,
                  max_grad_norm=None, master=True, seed=0):

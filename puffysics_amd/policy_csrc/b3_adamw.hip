@@ -85,6 +85,7 @@ struct B3AdamW {
     double* partial;                             // device: sums of squares
     float* scale;                                // device: the clip's factor
     float* inverse;                              // device: see aw_inverse
+    uint32_t* replays;                           // device: captured steps of 8-bit moments that have run
     int64_t* first;                              // host: a tensor's first chunk; count + 1
     int64_t* steps;                              // host
     B3AdamWTensor* given;                        // host
@@ -351,9 +352,14 @@ struct Clip {
     float* norm;
 };
 
+/* The key of the nth run of a captured step.  With the captured step's own a
+ * replay would round every moment as the one before it did, and moments that
+ * change by little would stay where they are. */
+__device__ uint32_t key_of_replay(uint32_t key, uint32_t n) { return n ? mix(key + n * 0x9e3779b9u) : key; }
+
 template <int BITS>
 __global__ __launch_bounds__(kThreads) void aw_step(StepArgs a, int base, int64_t first, const int2* chunk,
-    const Tensor* tensors, Moments mo, Rates k, const float* inverse, Clip clip) {
+    const Tensor* tensors, Moments mo, Rates k, const float* inverse, const uint32_t* replays, Clip clip) {
     constexpr int kParts = Shape<BITS>::kParts;
     /* fetched together: the sums of squares and whose chunk it is */
     const double part = clip.partial && (int)threadIdx.x < clip.partials ? clip.partial[threadIdx.x] : 0;
@@ -369,7 +375,8 @@ __global__ __launch_bounds__(kThreads) void aw_step(StepArgs a, int base, int64_
     }
     const int64_t from = (int64_t)c.y * kChunk + blockIdx.x % kParts * Shape<BITS>::kPart;
     if (!grad || from >= t.numel) return;
-    const Step s = {mo, k, inverse, scale, a.size[at], a.root[at], a.keep[at], a.key[at]};
+    const uint32_t key = BITS == 8 && replays ? key_of_replay(a.key[at], *replays) : a.key[at];
+    const Step s = {mo, k, inverse, scale, a.size[at], a.root[at], a.keep[at], key};
     const bool fg = a.grad_type[at] == B3_F32;
     if (t.type == B3_F32)
         step_chunk<float, float, false, BITS>(t, from, (const float*)grad, s);
@@ -382,6 +389,9 @@ __global__ __launch_bounds__(kThreads) void aw_step(StepArgs a, int base, int64_
     else
         step_typed<_Float16, false, BITS>(t, from, grad, fg, s);
 }
+
+/* After a captured step. */
+__global__ void aw_count(uint32_t* replays) { ++*replays; }
 
 /* ---- the norm ---- */
 
@@ -500,13 +510,13 @@ int sum_blocks(const B3AdamW* o, int base) {
 }
 
 template <int BITS>
-void launch_step(const B3AdamW* o, const StepArgs& a, int base, int64_t first, int64_t end, const Rates& rates, const Clip& clip,
-        hipStream_t stream) {
+void launch_step(const B3AdamW* o, const StepArgs& a, int base, int64_t first, int64_t end, const Rates& rates,
+        const uint32_t* replays, const Clip& clip, hipStream_t stream) {
     constexpr int64_t kMost = kMostBlocks / Shape<BITS>::kParts;
     for (; first < end; first += kMost) {
         const int64_t chunks = end - first < kMost ? end - first : kMost;
         aw_step<BITS><<<(unsigned)(chunks * Shape<BITS>::kParts), kThreads, 0, stream>>>(a, base, first, o->chunk, o->tensors,
-            o->moments, rates, o->inverse, clip);
+            o->moments, rates, o->inverse, replays, clip);
     }
 }
 
@@ -533,7 +543,7 @@ int64_t b3_adamw_size(const B3AdamWTensor* tensors, int count) {
 hipError_t b3_adamw_destroy(B3AdamW* o) {
     if (!o) return hipSuccess;
     hipError_t first = hipSuccess;
-    void* bufs[5] = {o->tensors, o->chunk, o->partial, o->scale, o->inverse};
+    void* bufs[6] = {o->tensors, o->chunk, o->partial, o->scale, o->inverse, o->replays};
     for (void* p : bufs) {
         hipError_t err = p ? hipFree(p) : hipSuccess;
         if (first == hipSuccess) first = err;
@@ -589,6 +599,9 @@ hipError_t b3_adamw_create(B3AdamW** out, const B3AdamWTensor* tensors, int coun
     if (err == hipSuccess) err = hipMalloc((void**)&o->partial, ((size_t)o->partials + 1) * sizeof(double));
     if (err == hipSuccess) err = hipMalloc((void**)&o->scale, sizeof(float));
     if (err == hipSuccess) err = hipMalloc((void**)&o->inverse, 256 * sizeof(float));
+    if (err == hipSuccess) err = hipMalloc((void**)&o->replays, sizeof(uint32_t));
+    const uint32_t none = 0;
+    if (err == hipSuccess) err = hipMemcpy(o->replays, &none, sizeof(none), hipMemcpyHostToDevice);
     if (err == hipSuccess) {
         aw_inverse<<<1, 256>>>(o->inverse);
         err = hipGetLastError();
@@ -615,6 +628,9 @@ hipError_t b3_adamw_step_gpu(B3AdamW* o, const void* const* grads, const int* gr
         if (grads[i] && grad_types[i] != o->given[i].type && grad_types[i] != B3_F32) return hipErrorInvalidValue;
     hipError_t err = on_device(o);
     if (err != hipSuccess) return err;
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    if (o->bits == 8 && (err = hipStreamIsCapturing(stream, &capture)) != hipSuccess) return err;
+    uint32_t* const replays = capture == hipStreamCaptureStatusNone ? NULL : o->replays;
     const B3AdamWConfig& cf = o->config;
     const Rates rates = {(float)cf.beta1, (float)cf.beta2, (float)(1 - cf.beta1), (float)(1 - cf.beta2), (float)cf.eps};
     const bool few = o->partials > 0 && o->partials <= kFewPartials;
@@ -650,9 +666,9 @@ hipError_t b3_adamw_step_gpu(B3AdamW* o, const void* const* grads, const int* gr
                 aw_squares<<<blocks, kThreads, 0, stream>>>(a, base, first, end, o->chunk, o->tensors, partial);
                 partial += blocks;
             } else if (o->bits == 32) {
-                launch_step<32>(o, a, base, first, end, rates, clip, stream);
+                launch_step<32>(o, a, base, first, end, rates, NULL, clip, stream);
             } else {
-                launch_step<8>(o, a, base, first, end, rates, clip, stream);
+                launch_step<8>(o, a, base, first, end, rates, replays, clip, stream);
             }
             if ((err = hipGetLastError()) != hipSuccess) return err;
         }
@@ -661,7 +677,11 @@ hipError_t b3_adamw_step_gpu(B3AdamW* o, const void* const* grads, const int* gr
             if ((err = hipGetLastError()) != hipSuccess) return err;
         }
     }
-    return hipSuccess;
+    if (replays) {
+        aw_count<<<1, 1, 0, stream>>>(replays);
+        err = hipGetLastError();
+    }
+    return err;
 }
 
 int64_t b3_adamw_steps(const B3AdamW* o, int tensor) {
