@@ -10,6 +10,7 @@ The reference leaves these to the trainer (docs/RL_LIBRARY.md).
 import array
 import collections
 import ctypes as C
+import operator
 import os
 
 import torch
@@ -424,12 +425,15 @@ class AdamW:
 
     def load_moments(self, exp_avg, exp_avg_sq, step, master=None):
         """Go on from moments (lists of a tensor for each parameter) after
-        `step` steps.  Where 32-bit copies of the weights are given, 16-bit
-        weights become what these round to; else the copies are the weights."""
+        `step` steps, a number or a list of one for each parameter.  Where
+        32-bit copies of the weights are given, 16-bit weights become what
+        these round to; else the copies are the weights."""
         n = len(self.params)
         _need(len(exp_avg) == n and len(exp_avg_sq) == n and (master is None or len(master) == n),
               "need one tensor for each parameter")
-        _need(step >= 0, "step has to be at least 0")
+        counts = list(step) if isinstance(step, (list, tuple)) else [step] * n
+        _need(len(counts) == n and all(hasattr(k, "__index__") and 0 <= k < 2 ** 63 for k in counts),
+              "step has to be a whole number from 0 on, or a list of one for each parameter")
         _need(master is None or self._master is not None, "this optimizer keeps no 32-bit copies")
         for given in (exp_avg, exp_avg_sq, master or []):
             _need(all(x.shape == p.shape for x, p in zip(given, self.params)), "need tensors of the parameters' shapes")
@@ -446,8 +450,8 @@ class AdamW:
             self._round_copies()
         elif self._master is not None:
             self._copy_weights()
-        for i in range(n):
-            _check("b3_adamw_set_steps", self._lib.b3_adamw_set_steps(self._h, i, step))
+        for i, k in enumerate(counts):
+            _check("b3_adamw_set_steps", self._lib.b3_adamw_set_steps(self._h, i, operator.index(k)))
 
     def close(self):
         if self._h:

@@ -215,3 +215,42 @@ def test_replays_round_by_other_bits_and_the_first_by_its_own():
     for i in range(4):
         for j in range(i):
             assert all(int((a != b).sum()) > 400 for a, b in zip(got[i], got[j]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_every_tensor_resumes_from_its_own_count(bits):
+    """Tensors that had no gradient in some steps go on with the corrections
+    and the rounding of their own counts."""
+    from puffysics_amd import policy
+    params = tensors(SIZES, torch.float32, 7)
+    opt = policy.AdamW(params, LR, BETAS, EPS, DECAY, state_bits=bits, seed=4)
+    for t in range(4):
+        opt.step([g if (i + t) % 3 or i == 0 else None for i, g in enumerate(tensors(SIZES, torch.float32, 50 + t))])
+    counts = [opt.steps(i) for i in range(len(params))]
+    assert len(set(counts)) > 1
+    twins = [p.clone() for p in params]
+    twin = policy.AdamW(twins, LR, BETAS, EPS, DECAY, state_bits=bits, seed=4)
+    m, v = opt.moments()
+    twin.load_moments(views(opt, m), views(opt, v), counts)
+    assert [twin.steps(i) for i in range(len(params))] == counts
+    for t in range(2):
+        grads = tensors(SIZES, torch.float32, 60 + t)
+        opt.step(grads)
+        twin.step(grads)
+    assert equal(params, twins) and equal(opt.moments(), twin.moments())
+    assert [opt.steps(i) for i in range(len(params))] == [k + 2 for k in counts]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("step", [-1, 2.5, [1], [1, -1], [1, 2, 3], [1, 2.0], "3", 2 ** 63])
+def test_refused_counts_leave_the_state(step):
+    from puffysics_amd import policy
+    p = [torch.zeros(40, device="cuda"), torch.zeros(7, device="cuda")]
+    opt = policy.AdamW(p, LR)
+    one = [torch.ones(40), torch.ones(7)]
+    with pytest.raises(ValueError):
+        opt.load_moments(one, one, step)
+    assert all(int(torch.count_nonzero(x)) == 0 for x in opt.moments()) and opt.steps(0) == opt.steps(1) == 0
+    opt.load_moments(one, one, (np.int64(3), 4))
+    assert opt.steps(0) == 3 and opt.steps(1) == 4
