@@ -168,7 +168,9 @@ hipError_t b3_adamw_create(B3AdamW** out, const B3AdamWTensor* tensors, int coun
  * captured step replays the corrections of the step that was captured.
  * 8-bit moments are rounded to one of their two neighbours by random bits
  * that seed, t and place give, and in a captured step the count of the
- * optimizer's captured steps that have run; a root over 0 stays over 0.  Steps of one
+ * optimizer's captured steps that have run (one that 8 bits hold as it is may
+ * fall a step of the grid, by one in 2^16 of the bits); a root over 0 stays
+ * over 0.  Steps of one
  * optimizer must follow one another on the device. */
 hipError_t b3_adamw_step_gpu(B3AdamW* optimizer, const void* const* grads, const int* grad_types, double lr,
     double max_norm, float* norm, hipStream_t stream);

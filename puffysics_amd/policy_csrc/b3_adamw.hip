@@ -179,9 +179,17 @@ __device__ uint32_t group_scale(const float x[kVector]) {
 }
 
 /* inverse[b] = 2^(127 - b) as pow() gives it, a unit in the last place low
- * for some exponents: torch.ldexp multiplies by the same numbers, so that a
- * torch program that rounds by the same bits gets the same moments. */
-__global__ void aw_inverse(float* inverse) { inverse[threadIdx.x] = powf(2.0f, 127.0f - (float)threadIdx.x); }
+ * for 41 exponents: torch.ldexp multiplies by the same numbers, so that a
+ * torch program that rounds by the same bits gets the same moments.  With the
+ * exact powers 1.3 in a million roundings go the other way, as many as a unit
+ * in the last place of the moment itself moves; a moment on the grid falls a
+ * step by one in 65,536 random bits on those scales.  Never over the exact
+ * power: a group's largest, where it is 448 on its scale, would pass the
+ * greatest number.  b goes from 1 to 247. */
+__global__ void aw_inverse(float* inverse) {
+    const uint32_t b = threadIdx.x;
+    inverse[b] = fminf(powf(2.0f, 127.0f - (float)b), __uint_as_float((b < 254 ? 254 - b : 0) << 23));
+}
 
 /* x on the group's scale as an e4m3 number, still in 32 bits: one of its two
  * neighbours by 16 random bits, or the nearest. */

@@ -254,3 +254,59 @@ def test_refused_counts_leave_the_state(step):
     assert all(int(torch.count_nonzero(x)) == 0 for x in opt.moments()) and opt.steps(0) == opt.steps(1) == 0
     opt.load_moments(one, one, (np.int64(3), 4))
     assert opt.steps(0) == 3 and opt.steps(1) == 4
+
+
+def grid_values(first, last, groups, seed):
+    """e4m3 numbers in groups of 32 on every scale 2^(b - 127) from b = first
+    to last: random ones of both signs and the largest, which pins the scale."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    codes = torch.arange(0, 127, dtype=torch.uint8).view(torch.float8_e4m3fn).float().cuda()
+    x = codes[torch.randint(0, 127, (last - first + 1, groups, 32), generator=g, device="cuda")]
+    x[..., 0] = 448.0
+    x *= torch.randint(0, 2, x.shape, generator=g, device="cuda") * 2 - 1
+    scale = (torch.arange(first, last + 1, dtype=torch.int32, device="cuda") << 23).view(torch.float32)
+    return (x * scale[:, None, None]).reshape(-1)
+
+
+def same_where_held(got, x):
+    """got, in bf16, is x wherever bf16 holds it, and for nearly all it does."""
+    held = x.bfloat16().float() == x
+    return float(held.float().mean()) > 0.95 and torch.equal(got[held].float(), x[held])
+
+
+@pytest.mark.gpu
+def test_values_on_the_grid_stay():
+    """A moment that 8 bits can hold is not rounded, on every scale: with
+    rates of 0 a step's moments are the gradient and its square.  Where the
+    factor to the grid is a unit low, one in 2^16 random bits takes it a step
+    of the grid down; 2^18 values a scale meet each four times.  A factor that
+    is high would make the largest of a group NaN.  Squares stay within 32
+    bits on the scales from 80 to 180."""
+    from puffysics_amd import policy
+    for first, last, square in ((1, 246, False), (80, 180, True)):
+        x = grid_values(first, last, 2 ** 13, first)
+        opt = policy.AdamW([torch.zeros_like(x)], 0.0, (0.0, 0.0), state_bits=8)
+        opt.step([x])
+        for got, want in zip(opt.moments(), (x, x * x) if square else (x,)):
+            held = want.bfloat16().float() == want
+            assert float(held.float().mean()) > 0.95 and torch.isfinite(got[held]).all()
+            off = held & (got.float() != want)
+            assert (off.view(last - first + 1, -1).sum(1) <= 40).all()
+            down = (want[off].abs() - got[off].float().abs()) / want[off].abs()
+            # a step of the grid is an eighth at most
+            assert (down > 0).all() and (down <= (0.235 if square and want is not x else 0.126)).all()
+
+
+@pytest.mark.gpu
+def test_values_on_the_grid_are_read_in_and_out():
+    from puffysics_amd import policy
+    for first, last in ((1, 246), (80, 180)):
+        x = grid_values(first, last, 16, first + 5)
+        opt = policy.AdamW([torch.zeros_like(x)], state_bits=8)
+        opt.load_moments([x], [x * x if first == 80 else torch.zeros_like(x)], 1)
+        m, v = opt.moments()
+        assert same_where_held(m, x)
+        if first == 80:
+            assert same_where_held(v, x * x)
+            opt.load_moments([m], [v], 1)
+            assert equal(opt.moments(), (m, v))
