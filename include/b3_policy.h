@@ -152,8 +152,9 @@ typedef struct B3AdamW B3AdamW;
 /* Elements of a flat array of the tensors' moments; -1 for bad arguments. */
 int64_t b3_adamw_size(const B3AdamWTensor* tensors, int count);
 
-/* The weights and the state stay the caller's, and stay where they are.
- * Allocates; synchronises. */
+/* The weights and the state stay the caller's, and stay where they are.  No
+ * two tensors overlap (hipErrorInvalidValue), nor do weights, state and
+ * gradients.  Allocates; synchronises. */
 hipError_t b3_adamw_create(B3AdamW** out, const B3AdamWTensor* tensors, int count, B3AdamWState state,
     B3AdamWConfig config);
 

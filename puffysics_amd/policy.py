@@ -280,7 +280,7 @@ def advantages(rewards, values, terminals, last_values, gamma=0.99, lam=0.95):
 
 class AdamW:
     """AdamW over all of `params` in one step: contiguous float32, float16 or
-    bfloat16 tensors on the current device.
+    bfloat16 tensors on the current device, no two of which overlap.
 
     state_bits     32, or 8: moments as e4m3 numbers (the first, and the root
                    of the second) with a power of two for every 32 of them,
@@ -305,9 +305,9 @@ class AdamW:
         for p in self.params:
             _need(p.dtype in _TYPE, "parameters have to be float32, float16 or bfloat16")
             _need(p.is_contiguous(), "parameters have to be contiguous")
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
+        _need(all(a[1] <= b[0] for a, b in zip(spans, spans[1:])), "a parameter is given twice, or two overlap")
         _on(*self.params)
-        _need(len({p.data_ptr() for p in self.params if p.numel()}) == sum(p.numel() > 0 for p in self.params),
-              "a parameter is given twice")
         _need(len(decay) == n and all(d >= 0 for d in decay), "weight_decay has to be at least 0, one for each tensor")
         _need(0 <= betas[0] < 1 and 0 <= betas[1] < 1 and eps >= 0, "betas have to be in [0, 1), eps at least 0")
         _need(state_bits in (8, 32), "state_bits has to be 8 or 32")

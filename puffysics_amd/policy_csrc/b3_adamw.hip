@@ -507,6 +507,26 @@ bool valid(const B3AdamWTensor* tensors, int count) {
     return true;
 }
 
+int by_address(const void* a, const void* b) {
+    const uintptr_t x = (uintptr_t)((const B3AdamWTensor*)a)->param, y = (uintptr_t)((const B3AdamWTensor*)b)->param;
+    return (x > y) - (x < y);
+}
+
+/* Whether two of the tensors that have elements overlap; `sorted` has room for
+ * all.  Weights that belong to two would be written by two workgroups. */
+bool overlap(const B3AdamWTensor* tensors, int count, B3AdamWTensor* sorted) {
+    int n = 0;
+    for (int i = 0; i < count; i++)
+        if (tensors[i].numel) sorted[n++] = tensors[i];
+    qsort(sorted, (size_t)n, sizeof(B3AdamWTensor), by_address);
+    for (int i = 1; i < n; i++) {
+        const B3AdamWTensor& before = sorted[i - 1];
+        const uintptr_t end = (uintptr_t)before.param + (uintptr_t)before.numel * (before.type == B3_F32 ? 4 : 2);
+        if (end > (uintptr_t)sorted[i].param) return true;
+    }
+    return false;
+}
+
 int64_t segment(int64_t numel) { return ceil_div(numel, B3_ADAMW_SEGMENT) * B3_ADAMW_SEGMENT; }
 
 /* Tensors of the launch that begins with tensor `base`. */
@@ -589,7 +609,8 @@ hipError_t b3_adamw_create(B3AdamW** out, const B3AdamWTensor* tensors, int coun
     o->given = (B3AdamWTensor*)calloc((size_t)count + 1, sizeof(B3AdamWTensor));
     Tensor* table = (Tensor*)calloc((size_t)count + 1, sizeof(Tensor));
     int2* chunk = (int2*)calloc((size_t)chunks + 1, sizeof(int2));
-    hipError_t err = o->first && o->steps && o->given && table && chunk ? hipGetDevice(&o->device) : hipErrorOutOfMemory;
+    hipError_t err = !(o->first && o->steps && o->given && table && chunk) ? hipErrorOutOfMemory
+        : overlap(tensors, count, o->given) ? hipErrorInvalidValue : hipGetDevice(&o->device);
     if (err == hipSuccess) {
         int64_t at = 0, c = 0;
         for (int i = 0; i < count; i++) {

@@ -310,3 +310,27 @@ def test_values_on_the_grid_are_read_in_and_out():
             assert same_where_held(v, x * x)
             opt.load_moments([m], [v], 1)
             assert equal(opt.moments(), (m, v))
+
+
+def test_overlapping_parameters_are_refused():
+    """Before anything is done with them: this runs without a GPU."""
+    from puffysics_amd import policy
+    whole = torch.zeros(100)
+    for params in ([whole[:60], whole[59:]], [whole[50:], whole[:51]], [whole, whole[99:]], [whole[10:20], whole],
+                   [whole, whole.view(torch.bfloat16)[199:]], [whole, whole[:0], whole[5:6]]):
+        with pytest.raises(ValueError, match="overlap"):
+            policy.AdamW(params, LR)
+    for params in ([whole[:60], whole[60:]], [whole, whole[:0], whole[7:7]], [whole.view(torch.float16)[:3], whole[2:]]):
+        with pytest.raises(ValueError, match="CUDA device"):          # the next check
+            policy.AdamW(params, LR)
+
+
+def test_overlapping_tensors_are_refused_by_the_c_entry():
+    from puffysics_amd import policy
+    lib, C, T = policy.policy_lib(), policy.C, policy.B3AdamWTensor
+    state, config = policy.B3AdamWState(32, 64, 64, None, None, None), policy.B3AdamWConfig(0.9, 0.999, 1e-8, 0)
+    h = C.c_void_p()
+    for tensors in ([(4096, 0, 10), (4132, 0, 3)], [(4132, 0, 3), (4096, 0, 10)], [(4096, 1, 10), (4114, 2, 1)],
+                    [(4096, 0, 100), (8192, 0, 1), (4097, 2, 1)]):
+        table = (T * len(tensors))(*[T(*t, 0.0) for t in tensors])
+        assert lib.b3_adamw_create(C.byref(h), table, len(tensors), state, config) == 1 and not h.value
