@@ -25,7 +25,8 @@ constexpr int kThreads = 256;
 constexpr int kVector = 4;                       // elements a thread loads at once
 constexpr int kChunk = 4096;
 constexpr int kSumBlocks = 2048;
-constexpr int kBatch = 160;                      // tensors to a launch: 4,000 bytes of arguments
+constexpr int kBatch = 156;                      // tensors to a launch, see StepLaunch
+constexpr size_t kMostArguments = 4096;          // bytes of a launch
 constexpr int kGroup = 32;                       // 8-bit moments: elements to a scale
 constexpr int kSumThreads = 1024;
 constexpr int kFewPartials = kThreads;
@@ -38,16 +39,19 @@ struct Tensor {
     int type;
 };
 
+/* The gradients of a launch's tensors. */
+struct Gradients {
+    const void* at[kBatch];                      // NULL: not stepped
+    uint8_t type[kBatch];
+};
+
 /* What a step says of each tensor of a launch. */
 struct StepArgs {
-    const void* grad[kBatch];                    // NULL: not stepped
     float size[kBatch];                          // lr / (1 - beta1^t)
     float root[kBatch];                          // 1 / sqrt(1 - beta2^t)
     float keep[kBatch];                          // 1 - lr weight_decay
     uint32_t key[kBatch];                        // of the 8-bit moments' rounding
-    uint8_t grad_type[kBatch];
 };
-static_assert(sizeof(StepArgs) <= 4096 - 96, "kernel arguments");
 
 struct Moments {
     void* exp_avg;
@@ -71,6 +75,43 @@ struct Shape {
 struct Rates {
     float beta1, beta2, rest1, rest2, eps;       // rest = 1 - beta, rounded once
 };
+
+/* Where a step's clip comes from. */
+struct Clip {
+    const float* scale;                          // NULL: none, or
+    const double* partial;                       // `partials` sums of squares (at most kFewPartials)
+    int partials;
+    float max_norm;
+    float* norm;
+};
+
+/* All arguments of a launch of aw_step: the chunks from `first` on, of tensors
+ * from `base` on. */
+struct StepLaunch {
+    Gradients g;
+    StepArgs a;
+    int base;
+    int64_t first;
+    const int2* chunk;
+    const Tensor* tensors;
+    Moments mo;
+    Rates rates;
+    const float* inverse;
+    const uint32_t* replays;                     // of a captured step, else NULL
+    Clip clip;
+};
+static_assert(sizeof(StepLaunch) <= kMostArguments, "kernel arguments");
+
+/* All arguments of a launch of aw_squares: the chunks from `first` to `end`. */
+struct SquaresLaunch {
+    Gradients g;
+    int base;
+    int64_t first, end;
+    const int2* chunk;
+    const Tensor* tensors;
+    double* partial;
+};
+static_assert(sizeof(SquaresLaunch) <= kMostArguments, "kernel arguments");
 
 }  // namespace b3p
 
@@ -351,48 +392,39 @@ __device__ double block_sum(double x) {
     return x;
 }
 
-/* Where a step's clip comes from. */
-struct Clip {
-    const float* scale;                          // NULL: none, or
-    const double* partial;                       // `partials` sums of squares (at most kFewPartials)
-    int partials;
-    float max_norm;
-    float* norm;
-};
-
 /* The key of the nth run of a captured step.  With the captured step's own a
  * replay would round every moment as the one before it did, and moments that
  * change by little would stay where they are. */
 __device__ uint32_t key_of_replay(uint32_t key, uint32_t n) { return n ? mix(key + n * 0x9e3779b9u) : key; }
 
 template <int BITS>
-__global__ __launch_bounds__(kThreads) void aw_step(StepArgs a, int base, int64_t first, const int2* chunk,
-    const Tensor* tensors, Moments mo, Rates k, const float* inverse, const uint32_t* replays, Clip clip) {
+__global__ __launch_bounds__(kThreads) void aw_step(StepLaunch l) {
     constexpr int kParts = Shape<BITS>::kParts;
+    const Clip& clip = l.clip;
     /* fetched together: the sums of squares and whose chunk it is */
     const double part = clip.partial && (int)threadIdx.x < clip.partials ? clip.partial[threadIdx.x] : 0;
-    const int2 c = chunk[first + blockIdx.x / kParts];
-    const Tensor t = tensors[c.x];
-    const int at = c.x - base;
-    const void* grad = a.grad[at];
+    const int2 c = l.chunk[l.first + blockIdx.x / kParts];
+    const Tensor t = l.tensors[c.x];
+    const int at = c.x - l.base;
+    const void* grad = l.g.at[at];
     float scale = clip.scale ? *clip.scale : 1.0f;
     if (clip.partial) {
         const float norm = (float)sqrt(block_sum<kThreads>(part));
-        if (first + blockIdx.x == 0 && threadIdx.x == 0) *clip.norm = norm;
+        if (l.first + blockIdx.x == 0 && threadIdx.x == 0) *clip.norm = norm;
         scale = clip_of(norm, clip.max_norm);
     }
     const int64_t from = (int64_t)c.y * kChunk + blockIdx.x % kParts * Shape<BITS>::kPart;
     if (!grad || from >= t.numel) return;
-    const uint32_t key = BITS == 8 && replays ? key_of_replay(a.key[at], *replays) : a.key[at];
-    const Step s = {mo, k, inverse, scale, a.size[at], a.root[at], a.keep[at], key};
-    const bool fg = a.grad_type[at] == B3_F32;
+    const uint32_t key = BITS == 8 && l.replays ? key_of_replay(l.a.key[at], *l.replays) : l.a.key[at];
+    const Step s = {l.mo, l.rates, l.inverse, scale, l.a.size[at], l.a.root[at], l.a.keep[at], key};
+    const bool fg = l.g.type[at] == B3_F32;
     if (t.type == B3_F32)
         step_chunk<float, float, false, BITS>(t, from, (const float*)grad, s);
-    else if (t.type == B3_BF16 && mo.master)
+    else if (t.type == B3_BF16 && l.mo.master)
         step_typed<__bf16, true, BITS>(t, from, grad, fg, s);
     else if (t.type == B3_BF16)
         step_typed<__bf16, false, BITS>(t, from, grad, fg, s);
-    else if (mo.master)
+    else if (l.mo.master)
         step_typed<_Float16, true, BITS>(t, from, grad, fg, s);
     else
         step_typed<_Float16, false, BITS>(t, from, grad, fg, s);
@@ -423,21 +455,20 @@ __device__ float square_chunk(const void* grad, int64_t from, int64_t n) {
     return from + kChunk <= n ? squares<true>((const G*)grad, from, n) : squares<false>((const G*)grad, from, n);
 }
 
-__global__ __launch_bounds__(kThreads) void aw_squares(StepArgs a, int base, int64_t first, int64_t end,
-    const int2* chunk, const Tensor* tensors, double* partial) {
+__global__ __launch_bounds__(kThreads) void aw_squares(SquaresLaunch l) {
     double sum = 0;
-    for (int64_t i = first + blockIdx.x; i < end; i += gridDim.x) {
-        const int2 c = chunk[i];
-        const int at = c.x - base;
-        const void* grad = a.grad[at];
+    for (int64_t i = l.first + blockIdx.x; i < l.end; i += gridDim.x) {
+        const int2 c = l.chunk[i];
+        const int at = c.x - l.base;
+        const void* grad = l.g.at[at];
         if (!grad) continue;
-        const int64_t n = tensors[c.x].numel, from = (int64_t)c.y * kChunk;
-        const int type = a.grad_type[at];
+        const int64_t n = l.tensors[c.x].numel, from = (int64_t)c.y * kChunk;
+        const int type = l.g.type[at];
         sum += type == B3_F32 ? square_chunk<float>(grad, from, n)
             : type == B3_BF16 ? square_chunk<__bf16>(grad, from, n) : square_chunk<_Float16>(grad, from, n);
     }
     sum = block_sum<kThreads>(sum);
-    if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+    if (threadIdx.x == 0) l.partial[blockIdx.x] = sum;
 }
 
 __global__ __launch_bounds__(kSumThreads) void aw_norm(const double* partial, int partials, float max_norm, float* norm,
@@ -537,14 +568,13 @@ int sum_blocks(const B3AdamW* o, int base) {
     return (int)(chunks < kSumBlocks ? chunks : kSumBlocks);
 }
 
+/* The chunks from l.first to `end`. */
 template <int BITS>
-void launch_step(const B3AdamW* o, const StepArgs& a, int base, int64_t first, int64_t end, const Rates& rates,
-        const uint32_t* replays, const Clip& clip, hipStream_t stream) {
+void launch_step(StepLaunch& l, int64_t end, hipStream_t stream) {
     constexpr int64_t kMost = kMostBlocks / Shape<BITS>::kParts;
-    for (; first < end; first += kMost) {
-        const int64_t chunks = end - first < kMost ? end - first : kMost;
-        aw_step<BITS><<<(unsigned)(chunks * Shape<BITS>::kParts), kThreads, 0, stream>>>(a, base, first, o->chunk, o->tensors,
-            o->moments, rates, o->inverse, replays, clip);
+    for (; l.first < end; l.first += kMost) {
+        const int64_t chunks = end - l.first < kMost ? end - l.first : kMost;
+        aw_step<BITS><<<(unsigned)(chunks * Shape<BITS>::kParts), kThreads, 0, stream>>>(l);
     }
 }
 
@@ -665,7 +695,14 @@ hipError_t b3_adamw_step_gpu(B3AdamW* o, const void* const* grads, const int* gr
     const bool few = o->partials > 0 && o->partials <= kFewPartials;
     Clip clip = {};
     if (max_norm > 0) clip = few ? Clip{NULL, o->partial, o->partials, (float)max_norm, norm} : Clip{o->scale, NULL, 0, 0, NULL};
-    StepArgs a;
+    StepLaunch l = {};
+    l.chunk = o->chunk;
+    l.tensors = o->tensors;
+    l.mo = o->moments;
+    l.rates = rates;
+    l.inverse = o->inverse;
+    l.replays = replays;
+    l.clip = clip;
     for (int pass = max_norm > 0 ? 0 : 1; pass < 2; pass++) {
         int64_t t_last = -1;
         float size = 0, root = 0;
@@ -675,8 +712,8 @@ hipError_t b3_adamw_step_gpu(B3AdamW* o, const void* const* grads, const int* gr
             const int64_t first = o->first[base], end = o->first[base + n];
             for (int j = 0; j < n; j++) {
                 const int i = base + j;
-                a.grad[j] = grads[i];
-                a.grad_type[j] = (uint8_t)(grad_types ? grad_types[i] : o->given[i].type);
+                l.g.at[j] = grads[i];
+                l.g.type[j] = (uint8_t)(grad_types ? grad_types[i] : o->given[i].type);
                 if (pass == 0 || !grads[i]) continue;
                 const int64_t t = ++o->steps[i];
                 if (t != t_last) {
@@ -684,20 +721,23 @@ hipError_t b3_adamw_step_gpu(B3AdamW* o, const void* const* grads, const int* gr
                     root = (float)(1 / sqrt(1 - pow(cf.beta2, (double)t)));
                     t_last = t;
                 }
-                a.size[j] = size;
-                a.root[j] = root;
-                a.keep[j] = (float)(1 - lr * o->given[i].weight_decay);
-                a.key[j] = mix((uint32_t)t * 0x9e3779b9u + cf.seed);
+                l.a.size[j] = size;
+                l.a.root[j] = root;
+                l.a.keep[j] = (float)(1 - lr * o->given[i].weight_decay);
+                l.a.key[j] = mix((uint32_t)t * 0x9e3779b9u + cf.seed);
             }
             if (first == end) continue;
             if (pass == 0) {
                 const int blocks = sum_blocks(o, base);
-                aw_squares<<<blocks, kThreads, 0, stream>>>(a, base, first, end, o->chunk, o->tensors, partial);
+                aw_squares<<<blocks, kThreads, 0, stream>>>({l.g, base, first, end, o->chunk, o->tensors, partial});
                 partial += blocks;
-            } else if (o->bits == 32) {
-                launch_step<32>(o, a, base, first, end, rates, NULL, clip, stream);
             } else {
-                launch_step<8>(o, a, base, first, end, rates, replays, clip, stream);
+                l.base = base;
+                l.first = first;
+                if (o->bits == 32)
+                    launch_step<32>(l, end, stream);
+                else
+                    launch_step<8>(l, end, stream);
             }
             if ((err = hipGetLastError()) != hipSuccess) return err;
         }
