@@ -15,8 +15,8 @@
  * successful no-op; the *_gpu functions enqueue on `stream` without
  * allocating or synchronising, on the current device, whose memory every
  * pointer is.  b3_adamw_create alone allocates.  Arrays need the alignment
- * of their elements and no more.  Results do not depend on the order in
- * which workgroups run.
+ * of their elements and no more (8-bit moments none), workspaces that of 8
+ * bytes.  Results do not depend on the order in which workgroups run.
  */
 #ifndef PUFFYSICS_AMD_B3_POLICY_H
 #define PUFFYSICS_AMD_B3_POLICY_H

@@ -184,6 +184,12 @@ __device__ void store(T* p, int64_t i, int64_t n, const float x[kVector]) {
 
 /* ---- 8-bit moments: four e4m3 bytes of a thread, 8 threads to a scale ---- */
 
+/* 4 N codes; bytes lie anywhere. */
+template <int N>
+__device__ Bytes<uint32_t, N> load_codes(const uint8_t* codes) {
+    return *(const Bytes<uint32_t, N>*)codes;
+}
+
 __device__ void unpack(uint32_t codes, uint8_t scale, float x[kVector]) {
     float s = __uint_as_float((uint32_t)scale << 23);
     x[0] = __builtin_amdgcn_cvt_f32_fp8(codes, 0) * s;
@@ -260,7 +266,7 @@ __device__ uint32_t pack(const float x[kVector], float inverse, const uint32_t r
 }
 
 __device__ void store_codes(uint8_t* codes, uint8_t* scales, int64_t i, uint32_t code, uint32_t scale) {
-    *(uint32_t*)(codes + i) = code;
+    *(Bytes<uint32_t, 1>*)(codes + i) = Bytes<uint32_t, 1>{{code}};
     if (i % kGroup == 0) scales[i / kGroup] = (uint8_t)scale;
 }
 
@@ -314,8 +320,8 @@ __device__ __forceinline__ void step_turn(const Tensor& t, int64_t from, const G
             load<FULL, true>((const float*)s.mo.exp_avg + t.at, i, n, m[u]);
             load<FULL, true>((const float*)s.mo.exp_avg_sq + t.at, i, n, v[u]);
         } else {
-            cm[u] = *(const uint32_t*)((const uint8_t*)s.mo.exp_avg + at);
-            cv[u] = *(const uint32_t*)((const uint8_t*)s.mo.exp_avg_sq + at);
+            cm[u] = load_codes<1>((const uint8_t*)s.mo.exp_avg + at).v[0];
+            cv[u] = load_codes<1>((const uint8_t*)s.mo.exp_avg_sq + at).v[0];
             sm[u] = s.mo.exp_avg_scale[at / kGroup];
             sv[u] = s.mo.exp_avg_sq_scale[at / kGroup];
         }
@@ -490,11 +496,11 @@ constexpr int kMomentsOut = 8;
 
 template <bool ROOT>
 __device__ __forceinline__ void moments_of(const uint8_t* codes, const uint8_t* scales, int64_t i, __bf16* out) {
-    const uint2 c = *(const uint2*)(codes + i);
+    const Bytes<uint32_t, 2> c = load_codes<2>(codes + i);
     const uint8_t scale = scales[i / kGroup];
     float x[kMomentsOut];
-    unpack(c.x, scale, x);
-    unpack(c.y, scale, x + kVector);
+    unpack(c.v[0], scale, x);
+    unpack(c.v[1], scale, x + kVector);
     Pack<__bf16, kMomentsOut> y;
 #pragma unroll
     for (int k = 0; k < kMomentsOut; k++) y.v[k] = (__bf16)(ROOT ? x[k] * x[k] : x[k]);

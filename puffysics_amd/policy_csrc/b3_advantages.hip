@@ -60,12 +60,6 @@ __device__ __forceinline__ void in_turn(T*& p) {
     asm("" : "+v"(p));
 }
 
-/* Unsigned numbers that lie anywhere. */
-template <typename T, int N>
-struct __attribute__((packed, aligned(1))) Bytes {
-    T v[N];
-};
-
 template <int SIZE, bool ONCE>
 __device__ __forceinline__ uint32_t load_raw(const char* p) {
     if (SIZE == 4) return ONCE ? __builtin_nontemporal_load((const uint32_t*)p) : *(const uint32_t*)p;
@@ -398,7 +392,7 @@ hipError_t b3_advantages_gpu(const B3Rollout* g, double gamma, double lambda, vo
     if (g->steps == 0 || g->envs == 0) return hipSuccess;
     const Plan p = plan_of(g->steps, g->envs, by_env(*g));
     const size_t need = workspace_of(p, g->envs);
-    if (workspace_bytes < need || (need && !workspace)) return hipErrorInvalidValue;
+    if (!holds(workspace, workspace_bytes, need)) return hipErrorInvalidValue;
     const bool wide = g->rewards_stride[0] == 1 && g->values_stride[0] == 1 && g->terminals_stride[0] == 1
         && g->out_stride[0] == 1;
     Job job = {*g, (float)gamma, (float)(gamma * lambda), wide, stream_inputs(*g, p), p.tiles, p.pieces, (Map*)workspace};

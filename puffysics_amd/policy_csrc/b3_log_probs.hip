@@ -941,7 +941,7 @@ hipError_t b3_log_probs_gpu(B3Logits g, const int64_t* taken, float* log_prob, f
         float* top_log_prob, int64_t* top_action, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     if (!valid(g, taken) || top < 0 || top > B3_MAX_TOP || top > g.actions) return hipErrorInvalidValue;
     const size_t need = b3_log_probs_workspace(g.rows, g.actions, top);
-    if (workspace_bytes < need || (need && !workspace)) return hipErrorInvalidValue;
+    if (!holds(workspace, workspace_bytes, need)) return hipErrorInvalidValue;
     if (g.rows == 0) return hipSuccess;
     if (!log_prob || !entropy || (top && (!top_log_prob || !top_action))) return hipErrorInvalidValue;
     Outputs o = {taken, log_prob, entropy, stats, top, top_log_prob, top_action};

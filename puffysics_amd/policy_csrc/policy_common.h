@@ -38,7 +38,13 @@ struct __attribute__((packed, aligned(sizeof(T)))) Pack {
     T v[N];
 };
 
-/* The same for data that is used once: not kept in the caches.  N elements
+/* Unsigned numbers that lie anywhere, as arrays of bytes do. */
+template <typename T, int N>
+struct __attribute__((packed, aligned(1))) Bytes {
+    T v[N];
+};
+
+/* A Pack's data where it is used once: not kept in the caches.  N elements
  * are 4, 8 or 16 bytes. */
 template <typename T, int N>
 struct Stream {
@@ -59,6 +65,11 @@ inline bool is_float_type(int type) { return type == B3_F32 || type == B3_F16 ||
 /* Workgroups of up to 256 threads that a launch may have: it takes fewer than
  * 2^32 threads. */
 constexpr int64_t kMostBlocks = (1 << 24) - 1;
+
+/* Whether a workspace has `need` bytes, aligned for what kernels keep there. */
+inline bool holds(const void* workspace, size_t bytes, size_t need) {
+    return need == 0 || (bytes >= need && workspace && (uintptr_t)workspace % 8 == 0);
+}
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 

@@ -334,3 +334,59 @@ def test_overlapping_tensors_are_refused_by_the_c_entry():
                     [(4096, 0, 100), (8192, 0, 1), (4097, 2, 1)]):
         table = (T * len(tensors))(*[T(*t, 0.0) for t in tensors])
         assert lib.b3_adamw_create(C.byref(h), table, len(tensors), state, config) == 1 and not h.value
+
+
+@pytest.mark.gpu
+def test_8_bit_moments_lie_anywhere():
+    """Codes and scales are bytes: a state at odd addresses goes the way of
+    an aligned one, in steps, out and in again."""
+    from puffysics_amd import policy
+    lib, C = policy.policy_lib(), policy.C
+    sizes = [1, 300, 4097, 20000]
+    offsets = [0, 256, 768, 768 + 4352]
+    total = 768 + 4352 + 20224
+    runs = []
+    for odd in ((0, 0, 0, 0), (1, 3, 1, 1), (2, 1, 3, 5)):
+        params = tensors(sizes, torch.float32, 8)
+        memory = [torch.zeros(n + 64, dtype=torch.uint8, device="cuda") for n in (total, total, total // 32, total // 32)]
+        at = [x[16 + o:] for x, o in zip(memory, odd)]
+        for x in at[2:]:
+            x.fill_(1)
+        table = (policy.B3AdamWTensor * 4)(*[policy.B3AdamWTensor(p.data_ptr(), 0, p.numel(), DECAY) for p in params])
+        assert lib.b3_adamw_size(table, 4) == total
+        state = policy.B3AdamWState(8, *[x.data_ptr() for x in at], None)
+        h = C.c_void_p()
+        torch.cuda.synchronize()
+        assert lib.b3_adamw_create(C.byref(h), table, 4, state, policy.B3AdamWConfig(*BETAS, EPS, 4)) == 0
+        out = torch.zeros((2, total), dtype=torch.bfloat16, device="cuda")
+        for t in range(3):
+            grads = tensors(sizes, torch.float32, 80 + t)
+            pointers = (C.c_void_p * 4)(*[g.data_ptr() for g in grads])
+            assert lib.b3_adamw_step_gpu(h, pointers, None, LR, 0.0, None, None) == 0
+            torch.cuda.synchronize()
+        for _ in range(2):
+            assert lib.b3_adamw_moments_gpu(h, out[0].data_ptr(), out[1].data_ptr(), None) == 0
+            torch.cuda.synchronize()
+            runs.append((*params, out.clone()))
+            flat = out.float()
+            assert lib.b3_adamw_load_moments_gpu(h, flat[0].data_ptr(), flat[1].data_ptr(), None) == 0
+            torch.cuda.synchronize()
+        assert all(int(torch.count_nonzero(x[:16 + o])) == 0 for x, o in zip(memory[:2], odd))
+        assert lib.b3_adamw_destroy(h) == 0
+    assert offsets[3] + 20224 == total and all(equal(r, runs[0]) for r in runs[1:])
+
+
+def test_workspaces_are_aligned():
+    """Nothing is launched: this runs without a GPU."""
+    from puffysics_amd import policy
+    lib, C = policy.policy_lib(), policy.C
+    need = lib.b3_log_probs_workspace(2, 100000, 3)
+    x = policy.B3Logits(64, 0, 2, 100000, 100000, None, 0)
+    g = policy.B3Rollout(20000, 2, 64, (2, 1), 64, 0, (2, 1), 64, 1, 64, 0, (2, 1), 64, 64, (2, 1))
+    size = lib.b3_advantages_workspace(20000, 2)
+    assert need > 0 and size > 0
+    for at in (None, 65, 68):
+        assert lib.b3_log_probs_gpu(x, 64, 64, 64, None, 3, 64, 64, at, need, None) == 1
+        assert lib.b3_advantages_gpu(C.byref(g), 0.9, 0.9, at, size, None) == 1
+    assert lib.b3_log_probs_gpu(x, 64, 64, 64, None, 3, 64, 64, 64, need - 1, None) == 1
+    assert lib.b3_advantages_gpu(C.byref(g), 0.9, 0.9, 64, 8, None) == 1      # the size is for either layout
