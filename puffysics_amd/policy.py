@@ -115,6 +115,12 @@ def _on(*tensors):
             raise ValueError("tensors have to be on the current CUDA device")
 
 
+def _as_read(x):
+    """x, or where its elements are only marked as negated, as those of a
+    conjugate's imaginary part are, a copy that holds them so."""
+    return x if x is None or not x.is_neg() else x.resolve_neg()
+
+
 # ---- log probabilities ----
 
 LogProbs = collections.namedtuple("LogProbs", "log_prob entropy top_log_prob top_action")
@@ -179,6 +185,7 @@ class _LogProbs(torch.autograd.Function):
 
 def _backward(ctx, d_log_prob, d_entropy):
     x, taken, mask, stats, entropy = ctx.saved_tensors
+    d_log_prob, d_entropy = _as_read(d_log_prob), _as_read(d_entropy)
     d = torch.empty_like(x, memory_format=torch.contiguous_format)
     _check("b3_log_probs_backward_gpu", policy_lib().b3_log_probs_backward_gpu(
         _logits(x, mask), taken.data_ptr(), stats.data_ptr(), entropy.data_ptr(), *_upstream(d_log_prob),
@@ -220,6 +227,7 @@ def log_probs(logits, taken, mask=None, top=0):
         _need(mask.shape == logits.shape or mask.shape == (actions,),
               "mask has to have the shape of logits, or of one row")
         mask = _rows(mask.reshape(-1, actions))
+    logits = _as_read(logits)
     shape = taken.shape
     if len(shape) != 1:
         logits, taken = logits.reshape(-1, actions), taken.reshape(-1)
@@ -259,6 +267,7 @@ def advantages(rewards, values, terminals, last_values, gamma=0.99, lam=0.95):
     _need(terminals.dtype in (torch.float32, torch.bool, torch.uint8), "terminals have to be float32, bool or uint8")
     _need(0 <= gamma <= 1 and 0 <= lam <= 1, "gamma and lam have to be between 0 and 1")
     _on(rewards, values, terminals, last_values)
+    rewards, values, last_values = _as_read(rewards), _as_read(values), _as_read(last_values)
     lib = policy_lib()
     steps, envs = rewards.shape
     # the longer stride is the outer axis: (steps, envs) unless the rewards are a transposed array
@@ -304,7 +313,7 @@ class AdamW:
         decay = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * n
         for p in self.params:
             _need(p.dtype in _TYPE, "parameters have to be float32, float16 or bfloat16")
-            _need(p.is_contiguous(), "parameters have to be contiguous")
+            _need(p.is_contiguous() and not p.is_neg(), "parameters have to be contiguous, and not marked as negated")
         spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
         _need(all(a[1] <= b[0] for a, b in zip(spans, spans[1:])), "a parameter is given twice, or two overlap")
         _on(*self.params)
@@ -379,6 +388,9 @@ class AdamW:
         with_grad = [i for i, g in enumerate(grads) if g is not None]
         if len(with_grad) < len(grads):
             stepped, shapes, dtypes, given = ([x[i] for i in with_grad] for x in (stepped, shapes, dtypes, grads))
+        if any([g.is_neg() for g in given]):
+            grads = [_as_read(g) for g in grads]
+            given = [g for g in grads if g is not None]
         if not {g.get_device() for g in given} <= {torch.cuda.current_device()}:
             raise ValueError("gradients have to be on the current CUDA device")
         if [g.shape for g in given] != shapes or not all([g.is_contiguous() for g in given]):
@@ -386,7 +398,7 @@ class AdamW:
         types = [g.dtype for g in given]
         if types != dtypes and any([t is not d and t is not torch.float32 for t, d in zip(types, dtypes)]):
             raise ValueError("gradients have to be of the parameters' type or float32")
-        if given is grads:
+        if len(given) == len(grads):
             pointers = array.array("Q", [g.data_ptr() for g in grads])
         else:
             pointers = array.array("Q", [0 if g is None else g.data_ptr() for g in grads])

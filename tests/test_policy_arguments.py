@@ -1,0 +1,73 @@
+"""Tensors that puffysics_amd.policy has to read as torch does, or refuse."""
+import pytest
+import torch
+
+
+def negated(x):
+    """x as the imaginary part of a conjugate: marked as negated, every other
+    number of the memory below."""
+    return torch.complex(torch.zeros_like(x), -x).conj().imag
+
+
+def test_negated_is_marked():
+    x = negated(torch.tensor([1.0, -2.0]))
+    assert x.is_neg() and x.tolist() == [1.0, -2.0] and x[:1].is_contiguous()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("actions", [1, 3, 300, 5000])
+def test_log_probs_of_negated_logits(actions):
+    """And of the gradient that comes in, of each output."""
+    from puffysics_amd import policy
+    g = torch.Generator().manual_seed(actions)
+    x = torch.randn(7, actions, generator=g).cuda()
+    taken = torch.randint(0, actions, (7,), generator=g).cuda()
+    mask = (torch.rand(7, actions, generator=g) < 0.8).cuda()
+    dl, dh = torch.randn(7, generator=g).cuda(), torch.randn(7, generator=g).cuda()
+    for m in (None, mask):
+        got, want = policy.log_probs(negated(x), taken, m, top=1), policy.log_probs(x, taken, m, top=1)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    want = torch.autograd.grad(policy.log_probs(x.requires_grad_(), taken)[:2], x, (dl, dh))[0]
+    leaf = x.detach().requires_grad_()
+    assert torch.equal(torch.autograd.grad(policy.log_probs(negated(leaf), taken)[:2], leaf, (dl, dh))[0], want)
+    for pair in ((negated(dl), dh), (dl, negated(dh)), (negated(dl), negated(dh))):
+        assert torch.equal(torch.autograd.grad(policy.log_probs(x, taken)[:2], x, pair)[0], want)
+    # as autograd itself makes one
+    z = torch.complex(torch.zeros_like(dl), policy.log_probs(x, taken).log_prob).conj() * torch.complex(dl, dh)
+    d = torch.autograd.grad(z.real.sum(), x)[0]
+    assert torch.equal(d, torch.autograd.grad(policy.log_probs(x, taken).log_prob, x, dh)[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("steps,envs", [(1, 1), (1, 5), (200, 3), (40, 70)])
+def test_advantages_of_negated_arrays(steps, envs):
+    from puffysics_amd import policy
+    g = torch.Generator().manual_seed(steps)
+    r, v, d = (torch.randn(steps, envs, generator=g).cuda() for _ in range(3))
+    d, last = (d > 1).float(), torch.randn(envs, generator=g).cuda()
+    want = policy.advantages(r, v, d, last)
+    for args in ((negated(r), v, d, last), (r, negated(v), d, last), (r, v, negated(d), last), (r, v, d, negated(last)),
+                 [negated(x) for x in (r, v, d, last)]):
+        got = policy.advantages(*args)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+def test_adamw_with_negated_gradients():
+    from puffysics_amd import policy
+    params, twins = ([torch.ones(n, device="cuda") for n in (1, 50, 1)] for _ in range(2))
+    a, b = policy.AdamW(params), policy.AdamW(twins)
+    g = torch.tensor([0.5, -0.25], device="cuda")
+    long = torch.randn(50, device="cuda")
+    for grads, marked in (([g[:1], long, g[1:]], [negated(g)[:1], long, negated(g)[1:]]),
+                          ([None, long, g[1:]], [None, torch._neg_view(-long), negated(g)[1:]])):
+        b.step(grads)
+        a.step(marked)
+        assert all(torch.equal(p, q) for p, q in zip(params, twins)) and torch.equal(a.moments()[0], b.moments()[0])
+    assert [a.steps(i) for i in range(3)] == [1, 2, 2]
+
+
+def test_negated_parameters_are_refused():
+    from puffysics_amd import policy
+    with pytest.raises(ValueError, match="negated"):
+        policy.AdamW([negated(torch.ones(1))])
