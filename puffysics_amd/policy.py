@@ -14,6 +14,7 @@ import operator
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .engine import B3Error
@@ -211,7 +212,8 @@ def log_probs(logits, taken, mask=None, top=0):
     top     how many of each row's best actions to return (at most 32), by
             descending log probability, the lowest action first among equals
 
-    log_prob and entropy are float32 [...] and differentiable in the logits;
+    log_prob and entropy are float32 [...] and differentiable in the logits
+    (backward and once; a tangent is refused);
     top_log_prob and top_action are [..., top], or None without `top`.  A row
     that allows nothing has log_prob -inf, entropy 0 and no gradient; an
     action past the last has log_prob NaN."""
@@ -219,6 +221,9 @@ def log_probs(logits, taken, mask=None, top=0):
     _need(logits.dim() >= 1 and logits.shape[-1] >= 1, "logits need at least one action")
     _need(not (taken.is_floating_point() or taken.is_complex() or taken.dtype == torch.bool), "taken has to be whole numbers")
     _need(taken.shape == logits.shape[:-1], "taken has to have the shape of logits without the last axis")
+    # a level is entered: the tensor may have a tangent
+    _need(forward_ad._current_level < 0 or forward_ad.unpack_dual(logits).tangent is None,
+          "log_probs has no forward-mode derivative")
     actions = logits.shape[-1]
     _need(0 <= top <= MAX_TOP and top <= actions, "top has to be between 0 and 32, and at most the actions")
     _on(logits, taken, mask)
@@ -257,7 +262,7 @@ def advantages(rewards, values, terminals, last_values, gamma=0.99, lam=0.95):
                  ended an episode (HoverEnvs.terminals)
     last_values  [envs], of values' type: after the last step
 
-    Any strides; the result has no gradient."""
+    Any strides; the result has no gradient and no tangent."""
     _need(rewards.dim() == 2 and rewards.dtype == torch.float32, "rewards have to be float32 [steps, envs]")
     _need(values.shape == rewards.shape and terminals.shape == rewards.shape,
           "values and terminals have to have the shape of rewards")

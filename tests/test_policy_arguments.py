@@ -71,3 +71,34 @@ def test_negated_parameters_are_refused():
     from puffysics_amd import policy
     with pytest.raises(ValueError, match="negated"):
         policy.AdamW([negated(torch.ones(1))])
+
+
+@pytest.mark.parametrize("needs", [False, True])
+def test_tangents_are_refused(needs):
+    """Nothing is launched: this runs without a GPU.  Without a tangent the
+    next check is reached, also between the levels."""
+    from puffysics_amd import policy
+    from torch.autograd import forward_ad
+    x, t = torch.randn(4, 6, requires_grad=needs), torch.zeros(4, dtype=torch.int64)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(4, 6))
+        for logits in (dual, dual * 2, dual[:, 1:3], dual.view(2, 2, 6)[0]):
+            with pytest.raises(ValueError, match="forward-mode"):
+                policy.log_probs(logits, t[:logits.shape[0]])
+        with pytest.raises(ValueError, match="CUDA device"):
+            policy.log_probs(x, t)
+    with pytest.raises(ValueError, match="CUDA device"):
+        policy.log_probs(dual, t)
+
+
+@pytest.mark.gpu
+def test_forward_mode_does_not_lose_the_tangent():
+    from puffysics_amd import policy
+    x, t = torch.randn(4, 6, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")
+    with pytest.raises(Exception):
+        torch.func.jvp(lambda y: policy.log_probs(y, t).log_prob, (x,), (torch.ones_like(x),))
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(ValueError):
+            policy.log_probs(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)), t)
+        inside = policy.log_probs(x, t).log_prob
+    assert torch.equal(inside, policy.log_probs(x, t).log_prob)
