@@ -21,6 +21,8 @@ from .engine import B3Error
 
 POLICY_PATH = os.path.join(_native.HERE, "libb3policy.so")
 MAX_TOP = 32
+MAX_ACTIONS = 1 << 21
+MAX_ROWS = (1 << 31) - 1     # and steps and environments of a rollout
 SEGMENT = 256
 _ONE_WAVE = 1024             # rows of up to so many actions need no workspace
 
@@ -225,6 +227,7 @@ def log_probs(logits, taken, mask=None, top=0):
     _need(forward_ad._current_level < 0 or forward_ad.unpack_dual(logits).tangent is None,
           "log_probs has no forward-mode derivative")
     actions = logits.shape[-1]
+    _need(actions <= MAX_ACTIONS and taken.numel() <= MAX_ROWS, "at most 2^21 actions and 2^31 - 1 rows")
     _need(0 <= top <= MAX_TOP and top <= actions, "top has to be between 0 and 32, and at most the actions")
     _on(logits, taken, mask)
     if mask is not None:
@@ -270,6 +273,7 @@ def advantages(rewards, values, terminals, last_values, gamma=0.99, lam=0.95):
     _need(last_values.shape == rewards.shape[1:] and last_values.dtype == values.dtype,
           "last_values have to be [envs], of the type of values")
     _need(terminals.dtype in (torch.float32, torch.bool, torch.uint8), "terminals have to be float32, bool or uint8")
+    _need(max(rewards.shape) <= MAX_ROWS or not rewards.numel(), "at most 2^31 - 1 steps and environments")
     _need(0 <= gamma <= 1 and 0 <= lam <= 1, "gamma and lam have to be between 0 and 1")
     _on(rewards, values, terminals, last_values)
     rewards, values, last_values = _as_read(rewards), _as_read(values), _as_read(last_values)
@@ -386,6 +390,8 @@ class AdamW:
         if grads is None:
             grads = [p.grad for p in self.params]
         _need(len(grads) == len(self.params), "need one gradient for each parameter")
+        lr = self.lr if lr is None else lr
+        _need(lr >= 0, "lr has to be at least 0")
         _need(self.max_grad_norm is None or self.max_grad_norm > 0, "max_grad_norm has to be over 0, or None")
         if [p.data_ptr() for p in self.params] != self._at:
             raise ValueError("a parameter's memory is not where it was")
@@ -414,7 +420,7 @@ class AdamW:
         norm = torch.empty((), dtype=torch.float32, device=self.device) if self.max_grad_norm is not None else None
         _check("b3_adamw_step_gpu", self._lib.b3_adamw_step_gpu(
             self._h, pointers.buffer_info()[0], kinds.buffer_info()[0] if kinds else None,
-            self.lr if lr is None else lr, self.max_grad_norm or 0.0,
+            lr, self.max_grad_norm or 0.0,
             norm.data_ptr() if norm is not None else None, _stream()))
         torch.autograd.graph.increment_version(stepped)      # as an operation in place does
         return norm

@@ -102,3 +102,34 @@ def test_forward_mode_does_not_lose_the_tangent():
             policy.log_probs(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)), t)
         inside = policy.log_probs(x, t).log_prob
     assert torch.equal(inside, policy.log_probs(x, t).log_prob)
+
+
+def test_sizes_past_the_limits_are_refused():
+    """Nothing is launched: this runs without a GPU."""
+    from puffysics_amd import policy
+    one, none = torch.zeros(1), torch.zeros(1, dtype=torch.int64)
+    for rows, actions in ((2, 2 ** 21 + 1), (2 ** 31, 3)):
+        with pytest.raises(ValueError, match="at most 2"):
+            policy.log_probs(one.expand(rows, actions), none.expand(rows))
+    for steps, envs in ((2 ** 31, 1), (1, 2 ** 31)):
+        x = one.expand(steps, envs)
+        with pytest.raises(ValueError, match="at most 2"):
+            policy.advantages(x, x, x, one.expand(envs))
+    for rows, actions in ((2, 2 ** 21), (2 ** 31 - 1, 3)):
+        with pytest.raises(ValueError, match="CUDA device"):          # the next check
+            policy.log_probs(one.expand(rows, actions), none.expand(rows))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lr", [-1e-3, float("nan")])
+def test_rates_below_0_are_refused(lr):
+    from puffysics_amd import policy
+    p, g = torch.zeros(5, device="cuda"), torch.ones(5, device="cuda")
+    opt = policy.AdamW([p], lr)
+    with pytest.raises(ValueError):
+        opt.step([g])
+    with pytest.raises(ValueError):
+        policy.AdamW([p]).step([g], lr=lr)
+    assert opt.steps() == 0 and int(torch.count_nonzero(p)) == 0
+    opt.step([g], lr=0.5)
+    assert opt.steps() == 1 and (p < 0).all()
