@@ -25,6 +25,7 @@ MAX_ACTIONS = 1 << 21
 MAX_ROWS = (1 << 31) - 1     # and steps and environments of a rollout
 SEGMENT = 256
 _ONE_WAVE = 1024             # rows of up to so many actions need no workspace
+_EMPTY = 8                   # stands for the address of a gradient without elements; NULL is no gradient
 
 _F32, _F16, _BF16, _U8 = 0, 1, 2, 3
 _TYPE = {torch.float32: _F32, torch.float16: _F16, torch.bfloat16: _BF16}
@@ -410,9 +411,9 @@ class AdamW:
         if types != dtypes and any([t is not d and t is not torch.float32 for t, d in zip(types, dtypes)]):
             raise ValueError("gradients have to be of the parameters' type or float32")
         if len(given) == len(grads):
-            pointers = array.array("Q", [g.data_ptr() for g in grads])
+            pointers = array.array("Q", [g.data_ptr() or _EMPTY for g in grads])
         else:
-            pointers = array.array("Q", [0 if g is None else g.data_ptr() for g in grads])
+            pointers = array.array("Q", [0 if g is None else g.data_ptr() or _EMPTY for g in grads])
         kinds = None if types == dtypes else \
             array.array("i", [_TYPE[d if g is None else g.dtype] for g, d in zip(grads, self._dtypes)])
         if self._master is not None and self._version() != self._master_version:

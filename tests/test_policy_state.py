@@ -390,3 +390,16 @@ def test_workspaces_are_aligned():
         assert lib.b3_advantages_gpu(C.byref(g), 0.9, 0.9, at, size, None) == 1
     assert lib.b3_log_probs_gpu(x, 64, 64, 64, None, 3, 64, 64, 64, need - 1, None) == 1
     assert lib.b3_advantages_gpu(C.byref(g), 0.9, 0.9, 64, 8, None) == 1      # the size is for either layout
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("clip", [None, 1.0])
+def test_empty_tensors_count_their_steps(clip):
+    """A gradient without elements is a gradient: steps() of the first tensor
+    is what a run is taken up from."""
+    from puffysics_amd import policy
+    params = [torch.zeros(0, device="cuda"), torch.ones(5, device="cuda"), torch.zeros((3, 0), device="cuda")]
+    opt = policy.AdamW(params, LR, max_grad_norm=clip)
+    for t in range(3):
+        opt.step([torch.ones_like(p) if t != 1 or i else None for i, p in enumerate(params)])
+    assert [opt.steps(i) for i in range(3)] == [2, 3, 3]
