@@ -1,7 +1,7 @@
 /*
- * policy_common.h - what the kernels of include/b3_policy.h share: element
- * types, loads of vectors with the alignment of their elements, and
- * reductions over a wave and a workgroup in a fixed order.
+ * policy_common.h - what the kernels of include/b3_policy.h share: loads and
+ * stores of vectors with the alignment of their elements, conversions, and the
+ * bounds of launches and workspaces.
  */
 #ifndef PUFFYSICS_AMD_POLICY_COMMON_H
 #define PUFFYSICS_AMD_POLICY_COMMON_H
@@ -15,21 +15,6 @@
 namespace b3p {
 
 constexpr int kWave = 64;
-
-template <int TYPE>
-struct Element;
-template <>
-struct Element<B3_F32> {
-    using type = float;
-};
-template <>
-struct Element<B3_F16> {
-    using type = _Float16;
-};
-template <>
-struct Element<B3_BF16> {
-    using type = __bf16;
-};
 
 /* N elements that lie anywhere their type may: the hardware takes wide
  * global loads and stores at any such address. */
