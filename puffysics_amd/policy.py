@@ -24,7 +24,7 @@ MAX_TOP = 32
 MAX_ACTIONS = 1 << 21
 MAX_ROWS = (1 << 31) - 1     # and steps and environments of a rollout
 SEGMENT = 256
-_ONE_WAVE = 1024             # rows of up to so many actions need no workspace
+_SMALL = 2048                # rows of up to so many actions need no workspace
 _EMPTY = 8                   # stands for the address of a gradient without elements; NULL is no gradient
 
 _F32, _F16, _BF16, _U8 = 0, 1, 2, 3
@@ -160,7 +160,7 @@ def _forward(x, taken, mask, top, kept):
     if top:
         top_lp = torch.empty((rows, top), dtype=torch.float32, device=x.device)
         top_action = torch.empty((rows, top), dtype=torch.int64, device=x.device)
-    size = 0 if actions <= _ONE_WAVE else lib.b3_log_probs_workspace(rows, actions, top)
+    size = 0 if actions <= _SMALL else lib.b3_log_probs_workspace(rows, actions, top)
     if size:
         work = torch.empty(size, dtype=torch.uint8, device=x.device)
     _check("b3_log_probs_gpu", lib.b3_log_probs_gpu(

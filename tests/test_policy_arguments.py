@@ -133,3 +133,16 @@ def test_rates_below_0_are_refused(lr):
     assert opt.steps() == 0 and int(torch.count_nonzero(p)) == 0
     opt.step([g], lr=0.5)
     assert opt.steps() == 1 and (p < 0).all()
+
+
+def test_rows_without_a_workspace():
+    """The sizes for which log_probs does not ask are those that need none."""
+    from puffysics_amd import policy
+    lib = policy.policy_lib()
+    for rows in (1, 16, 4096, 2 ** 20):
+        for actions in (1, policy._SMALL - 1, policy._SMALL):
+            assert lib.b3_log_probs_workspace(rows, actions, 32) == 0
+        assert lib.b3_log_probs_workspace(rows, 2 ** 18, 32) > 0
+    from b3test import ROOT
+    text = open(ROOT + "/puffysics_amd/policy_csrc/b3_log_probs.hip").read()
+    assert "kSmall = %d," % policy._SMALL in text
