@@ -135,7 +135,9 @@ struct B3AdamW {
 namespace b3p {
 namespace {
 
-/* 32 well mixed bits of 32: two rounds of shift, xor and multiply. */
+/* 32 well mixed bits of 32: two rounds of shift, xor and multiply.  The shifts
+ * and multipliers are those of a published search for the least biased (C.
+ * Wellons, "Prospecting for Hash Functions", 2018). */
 inline __host__ __device__ uint32_t mix(uint32_t x) {
     x ^= x >> 16;
     x *= 0x7feb352du;
