@@ -180,8 +180,8 @@ hipError_t b3_adamw_step_gpu(B3AdamW* optimizer, const void* const* grads, const
 int64_t b3_adamw_steps(const B3AdamW* optimizer, int tensor);
 hipError_t b3_adamw_set_steps(B3AdamW* optimizer, int tensor, int64_t steps);
 
-/* 8-bit moments as the values they stand for, in bf16 (exact but for
- * exp_avg_sq below its range): flat arrays of b3_adamw_size() elements. */
+/* 8-bit moments as the values they stand for, in bf16 (exact but for what lies
+ * below its range): flat arrays of b3_adamw_size() elements. */
 hipError_t b3_adamw_moments_gpu(const B3AdamW* optimizer, void* exp_avg, void* exp_avg_sq, hipStream_t stream);
 
 /* float moments (flat arrays) to the 8-bit state, each to the nearest. */

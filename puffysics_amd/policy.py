@@ -429,7 +429,7 @@ class AdamW:
     def moments(self):
         """The flat arrays (exp_avg, exp_avg_sq): the state's own in 32 bits,
         in 8 bits the values it stands for as new bfloat16 arrays, which hold
-        them exactly."""
+        them exactly but for what lies below their range."""
         if self.state_bits == 32:
             return self._exp_avg, self._exp_avg_sq
         out = torch.empty((2, self.size), dtype=torch.bfloat16, device=self.device)
