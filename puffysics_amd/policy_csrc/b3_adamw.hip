@@ -7,11 +7,12 @@
  * tensors as kernel arguments, so that a step copies nothing to the device.
  * The step is one pass: a thread's loads of a vector of everything are issued
  * before the first is used.  It is bound by memory (28 bytes a weight in 32
- * bits), and what it moves goes past the caches: 400 million weights take
- * 1,872 us so (6.0 TB/s), and took 2,049 us through them.  With a clip the
- * norm is summed first, by at most kSumBlocks workgroups a launch over their
- * chunks in turn, through the caches, which keep gradients of a moderate size
- * for the step (100 million in bf16: 458 us, 478 us past them); few partial
+ * bits, 30 of 16-bit weights with copies), and what it moves goes past the
+ * caches: 400 million weights in 32 bits take 1,953 us so (5.7 TB/s), and 2,098
+ * through them.  With a clip the norm is summed first, by at most kSumBlocks
+ * workgroups a launch over their chunks in turn, through the caches, which
+ * keep gradients of a moderate size for the step (100 million in bf16 with the
+ * clip: 520 us, 545 past them; 60 million in fp32: 290 to 296, 327); few partial
  * sums are added by the step itself, many by a launch of their own.  Sums go
  * in one order always.
  */
@@ -61,16 +62,12 @@ struct Moments {
     float* master;
 };
 
-/* Workgroups to a chunk, and vectors of a thread in flight.  In 32 bits four
- * workgroups of one vector a thread: 400 million weights took 2,061 us, and
- * 2,109 us as one workgroup that goes on twice over two vectors; 30 million
- * in bf16 155 and 171 us.  With 8-bit moments, where a vector is more work for
- * fewer bytes, the other way about: 200 million weights 660 and 602 us. */
-template <int BITS>
-struct Shape {
-    static constexpr int kParts = BITS == 32 ? 4 : 1, kUnroll = BITS == 32 ? 1 : 2;
-    static constexpr int kTurn = kThreads * kVector * kUnroll, kPart = kChunk / kParts;
-};
+/* Workgroups to a chunk: a thread has one vector.  400 million weights in 32
+ * bits take 1,953 us, and 2,000 with one workgroup to a chunk whose threads go
+ * on twice over two vectors; 30 million in bf16 148 and 160; 200 million with
+ * 8-bit moments 541 and 567. */
+constexpr int kParts = 4, kPart = kChunk / kParts;
+static_assert(kPart == kThreads * kVector, "a vector to a thread");
 
 struct Rates {
     float beta1, beta2, rest1, rest2, eps;       // rest = 1 - beta, rounded once
@@ -294,93 +291,73 @@ __device__ __forceinline__ float copy_or_weight(float copy, P held) {
     return __builtin_bit_cast(uint16_t, rounded) == __builtin_bit_cast(uint16_t, held) ? copy : to_float(held);
 }
 
-/* The vectors of a thread that are in flight together.  The square root is the
+/* A thread's vector of the part from `from` on.  The square root is the
  * correctly rounded one, since what is kept of it is cut off by random bits
  * (the hardware's with its residuals' correction took as long, and gives 0 for
  * denormals); the division in the update is a reciprocal, good to two units. */
 template <typename P, typename G, bool MASTER, int BITS, bool FULL>
-__device__ __forceinline__ void step_turn(const Tensor& t, int64_t from, const G* grad, const Step& s) {
-    constexpr int kUnroll = Shape<BITS>::kUnroll;
-    float g[kUnroll][kVector], w[kUnroll][kVector], m[kUnroll][kVector], v[kUnroll][kVector];
-    Pack<P, kVector> held[kUnroll];              // MASTER: the weights themselves
-    uint32_t cm[kUnroll], cv[kUnroll];
-    uint8_t sm[kUnroll], sv[kUnroll];
-    const int64_t n = t.numel;
-#pragma unroll
-    for (int u = 0; u < kUnroll; u++) {
-        const int64_t i = from + (u * kThreads + (int)threadIdx.x) * kVector, at = t.at + i;
-        /* whole groups of 8-bit moments go on together */
-        if (!FULL && i / kGroup * kGroup >= n) continue;
-        load<FULL, true>(grad, i, n, g[u]);
-        if (MASTER) {
-            load<FULL, true>(s.mo.master + t.at, i, n, w[u]);
-            held[u] = load_raw<FULL>((const P*)t.param, i, n);
-        } else {
-            load<FULL, true>((const P*)t.param, i, n, w[u]);
-        }
-        if (BITS == 32) {
-            load<FULL, true>((const float*)s.mo.exp_avg + t.at, i, n, m[u]);
-            load<FULL, true>((const float*)s.mo.exp_avg_sq + t.at, i, n, v[u]);
-        } else {
-            cm[u] = load_codes<1>((const uint8_t*)s.mo.exp_avg + at).v[0];
-            cv[u] = load_codes<1>((const uint8_t*)s.mo.exp_avg_sq + at).v[0];
-            sm[u] = s.mo.exp_avg_scale[at / kGroup];
-            sv[u] = s.mo.exp_avg_sq_scale[at / kGroup];
-        }
+__device__ __forceinline__ void step_vector(const Tensor& t, int64_t from, const G* grad, const Step& s) {
+    float g[kVector], w[kVector], m[kVector], v[kVector];
+    Pack<P, kVector> held;                       // MASTER: the weights themselves
+    const int64_t n = t.numel, i = from + (int)threadIdx.x * kVector, at = t.at + i;
+    /* whole groups of 8-bit moments go on together */
+    if (!FULL && i / kGroup * kGroup >= n) return;
+    load<FULL, true>(grad, i, n, g);
+    if (MASTER) {
+        load<FULL, true>(s.mo.master + t.at, i, n, w);
+        held = load_raw<FULL>((const P*)t.param, i, n);
+    } else {
+        load<FULL, true>((const P*)t.param, i, n, w);
     }
+    if (BITS == 32) {
+        load<FULL, true>((const float*)s.mo.exp_avg + t.at, i, n, m);
+        load<FULL, true>((const float*)s.mo.exp_avg_sq + t.at, i, n, v);
+    } else {
+        const uint32_t cm = load_codes<1>((const uint8_t*)s.mo.exp_avg + at).v[0];
+        const uint32_t cv = load_codes<1>((const uint8_t*)s.mo.exp_avg_sq + at).v[0];
+        unpack(cm, s.mo.exp_avg_scale[at / kGroup], m);
+        unpack(cv, s.mo.exp_avg_sq_scale[at / kGroup], v);
+    }
+    float root[kVector];
 #pragma unroll
-    for (int u = 0; u < kUnroll; u++) {
-        const int64_t i = from + (u * kThreads + (int)threadIdx.x) * kVector, at = t.at + i;
-        if (!FULL && i / kGroup * kGroup >= n) continue;
-        if (BITS == 8) {
-            unpack(cm[u], sm[u], m[u]);
-            unpack(cv[u], sv[u], v[u]);
-        }
-        float root[kVector];
+    for (int j = 0; j < kVector; j++) {
+        if constexpr (MASTER) w[j] = copy_or_weight(w[j], held.v[j]);
+        const float gc = g[j] * s.clip, old = BITS == 32 ? v[j] : v[j] * v[j];
+        m[j] = m[j] * s.rates.beta1 + gc * s.rates.rest1;
+        v[j] = old * s.rates.beta2 + gc * gc * s.rates.rest2;
+        root[j] = sqrtf(v[j]);
+        w[j] = w[j] * s.keep - m[j] * s.size * __builtin_amdgcn_rcpf(root[j] * s.root + s.rates.eps);
+    }
+    store<FULL>((P*)t.param, i, n, w);
+    if (MASTER) store<FULL>(s.mo.master + t.at, i, n, w);
+    if (BITS == 32) {
+        store<FULL>((float*)s.mo.exp_avg + t.at, i, n, m);
+        store<FULL>((float*)s.mo.exp_avg_sq + t.at, i, n, v);
+    } else {
+        uint32_t random[kVector];
+        const uint32_t key = s.key ^ mix((uint32_t)(at >> 32));
 #pragma unroll
-        for (int j = 0; j < kVector; j++) {
-            if constexpr (MASTER) w[u][j] = copy_or_weight(w[u][j], held[u].v[j]);
-            const float gc = g[u][j] * s.clip, old = BITS == 32 ? v[u][j] : v[u][j] * v[u][j];
-            m[u][j] = m[u][j] * s.rates.beta1 + gc * s.rates.rest1;
-            v[u][j] = old * s.rates.beta2 + gc * gc * s.rates.rest2;
-            root[j] = sqrtf(v[u][j]);
-            w[u][j] = w[u][j] * s.keep - m[u][j] * s.size * __builtin_amdgcn_rcpf(root[j] * s.root + s.rates.eps);
-        }
-        store<FULL>((P*)t.param, i, n, w[u]);
-        if (MASTER) store<FULL>(s.mo.master + t.at, i, n, w[u]);
-        if (BITS == 32) {
-            store<FULL>((float*)s.mo.exp_avg + t.at, i, n, m[u]);
-            store<FULL>((float*)s.mo.exp_avg_sq + t.at, i, n, v[u]);
-        } else {
-            uint32_t random[kVector];
-            const uint32_t key = s.key ^ mix((uint32_t)(at >> 32));
-#pragma unroll
-            for (int j = 0; j < kVector; j++) random[j] = mix((uint32_t)(at + j) ^ key);
-            const uint32_t to_m = group_scale(m[u]), to_v = group_scale(root);
-            store_codes((uint8_t*)s.mo.exp_avg, s.mo.exp_avg_scale, at, pack<true, false>(m[u], s.inverse[to_m], random), to_m);
-            store_codes((uint8_t*)s.mo.exp_avg_sq, s.mo.exp_avg_sq_scale, at, pack<true, true>(root, s.inverse[to_v], random),
-                to_v);
-        }
+        for (int j = 0; j < kVector; j++) random[j] = mix((uint32_t)(at + j) ^ key);
+        const uint32_t to_m = group_scale(m), to_v = group_scale(root);
+        store_codes((uint8_t*)s.mo.exp_avg, s.mo.exp_avg_scale, at, pack<true, false>(m, s.inverse[to_m], random), to_m);
+        store_codes((uint8_t*)s.mo.exp_avg_sq, s.mo.exp_avg_sq_scale, at, pack<true, true>(root, s.inverse[to_v], random), to_v);
     }
 }
 
 template <typename P, typename G, bool MASTER, int BITS>
-__device__ __forceinline__ void step_chunk(const Tensor& t, int64_t from, const G* grad, const Step& s) {
-    constexpr int kTurn = Shape<BITS>::kTurn;
-    const int64_t end = from + Shape<BITS>::kPart;
-    if (end <= t.numel) {
-        for (int64_t i = from; i < end; i += kTurn) step_turn<P, G, MASTER, BITS, true>(t, i, grad, s);
-    } else {
-        for (int64_t i = from; i < end && i < t.numel; i += kTurn) step_turn<P, G, MASTER, BITS, false>(t, i, grad, s);
-    }
+__device__ __forceinline__ void step_part(const Tensor& t, int64_t from, const G* grad, const Step& s) {
+    if (from + kPart <= t.numel)
+        step_vector<P, G, MASTER, BITS, true>(t, from, grad, s);
+    else
+        step_vector<P, G, MASTER, BITS, false>(t, from, grad, s);
 }
 
 template <typename P, bool MASTER, int BITS>
 __device__ __forceinline__ void step_typed(const Tensor& t, int64_t from, const void* grad, bool float_grad, const Step& s) {
     if (float_grad)
-        step_chunk<P, float, MASTER, BITS>(t, from, (const float*)grad, s);
+        step_part<P, float, MASTER, BITS>(t, from, (const float*)grad, s);
     else
-        step_chunk<P, P, MASTER, BITS>(t, from, (const P*)grad, s);
+        step_part<P, P, MASTER, BITS>(t, from, (const P*)grad, s);
 }
 
 /* The clip's factor; a NaN norm stays one. */
@@ -407,7 +384,6 @@ __device__ uint32_t key_of_replay(uint32_t key, uint32_t n) { return n ? mix(key
 
 template <int BITS>
 __global__ __launch_bounds__(kThreads) void aw_step(StepLaunch l) {
-    constexpr int kParts = Shape<BITS>::kParts;
     const Clip& clip = l.clip;
     /* fetched together: the sums of squares and whose chunk it is */
     const double part = clip.partial && (int)threadIdx.x < clip.partials ? clip.partial[threadIdx.x] : 0;
@@ -421,13 +397,13 @@ __global__ __launch_bounds__(kThreads) void aw_step(StepLaunch l) {
         if (l.first + blockIdx.x == 0 && threadIdx.x == 0) *clip.norm = norm;
         scale = clip_of(norm, clip.max_norm);
     }
-    const int64_t from = (int64_t)c.y * kChunk + blockIdx.x % kParts * Shape<BITS>::kPart;
+    const int64_t from = (int64_t)c.y * kChunk + blockIdx.x % kParts * kPart;
     if (!grad || from >= t.numel) return;
     const uint32_t key = BITS == 8 && l.replays ? key_of_replay(l.a.key[at], *l.replays) : l.a.key[at];
     const Step s = {l.mo, l.rates, l.inverse, scale, l.a.size[at], l.a.root[at], l.a.keep[at], key};
     const bool fg = l.g.type[at] == B3_F32;
     if (t.type == B3_F32)
-        step_chunk<float, float, false, BITS>(t, from, (const float*)grad, s);
+        step_part<float, float, false, BITS>(t, from, (const float*)grad, s);
     else if (t.type == B3_BF16 && l.mo.master)
         step_typed<__bf16, true, BITS>(t, from, grad, fg, s);
     else if (t.type == B3_BF16)
@@ -579,10 +555,10 @@ int sum_blocks(const B3AdamW* o, int base) {
 /* The chunks from l.first to `end`. */
 template <int BITS>
 void launch_step(StepLaunch& l, int64_t end, hipStream_t stream) {
-    constexpr int64_t kMost = kMostBlocks / Shape<BITS>::kParts;
+    constexpr int64_t kMost = kMostBlocks / kParts;
     for (; l.first < end; l.first += kMost) {
         const int64_t chunks = end - l.first < kMost ? end - l.first : kMost;
-        aw_step<BITS><<<(unsigned)(chunks * Shape<BITS>::kParts), kThreads, 0, stream>>>(l);
+        aw_step<BITS><<<(unsigned)(chunks * kParts), kThreads, 0, stream>>>(l);
     }
 }
 
