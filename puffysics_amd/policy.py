@@ -26,6 +26,9 @@ MAX_ROWS = (1 << 31) - 1     # and steps and environments of a rollout
 SEGMENT = 256
 _SMALL = 2048                # rows of up to so many actions need no workspace
 _EMPTY = 8                   # stands for the address of a gradient without elements; NULL is no gradient
+# what a step asks of every tensor, called by map: a policy may have many small ones
+_address, _is_contiguous, _is_neg, _get_device = (
+    getattr(torch._C.TensorBase, name) for name in ("data_ptr", "is_contiguous", "is_neg", "get_device"))
 
 _F32, _F16, _BF16, _U8 = 0, 1, 2, 3
 _TYPE = {torch.float32: _F32, torch.float16: _F16, torch.bfloat16: _BF16}
@@ -356,6 +359,7 @@ class AdamW:
                              self._master.data_ptr() if self._master is not None else None)
         self._at, self._shapes, self._dtypes = ([f(p) for p in self.params] for f in (
             torch.Tensor.data_ptr, lambda p: p.shape, lambda p: p.dtype))
+        self._empty = any(p.numel() == 0 for p in self.params)
         torch.cuda.current_stream().synchronize()     # the state is ready for a step on any stream
         _check("b3_adamw_create", self._lib.b3_adamw_create(C.byref(self._h), table, n, state,
                                                             B3AdamWConfig(betas[0], betas[1], eps, seed)))
@@ -394,24 +398,24 @@ class AdamW:
         lr = self.lr if lr is None else lr
         _need(lr >= 0, "lr has to be at least 0")
         _need(self.max_grad_norm is None or self.max_grad_norm > 0, "max_grad_norm has to be over 0, or None")
-        if [p.data_ptr() for p in self.params] != self._at:
+        if list(map(_address, self.params)) != self._at:
             raise ValueError("a parameter's memory is not where it was")
         stepped, shapes, dtypes, given = self.params, self._shapes, self._dtypes, grads
         with_grad = [i for i, g in enumerate(grads) if g is not None]
         if len(with_grad) < len(grads):
             stepped, shapes, dtypes, given = ([x[i] for i in with_grad] for x in (stepped, shapes, dtypes, grads))
-        if any([g.is_neg() for g in given]):
+        if any(map(_is_neg, given)):
             grads = [_as_read(g) for g in grads]
             given = [g for g in grads if g is not None]
-        if not {g.get_device() for g in given} <= {torch.cuda.current_device()}:
+        if not set(map(_get_device, given)) <= {torch.cuda.current_device()}:
             raise ValueError("gradients have to be on the current CUDA device")
-        if [g.shape for g in given] != shapes or not all([g.is_contiguous() for g in given]):
+        if [g.shape for g in given] != shapes or not all(map(_is_contiguous, given)):
             raise ValueError("gradients have to be contiguous, of the parameters' shapes")
         types = [g.dtype for g in given]
         if types != dtypes and any([t is not d and t is not torch.float32 for t, d in zip(types, dtypes)]):
             raise ValueError("gradients have to be of the parameters' type or float32")
-        if len(given) == len(grads):
-            pointers = array.array("Q", [g.data_ptr() or _EMPTY for g in grads])
+        if len(given) == len(grads) and not self._empty:
+            pointers = array.array("Q", list(map(_address, grads)))
         else:
             pointers = array.array("Q", [0 if g is None else g.data_ptr() or _EMPTY for g in grads])
         kinds = None if types == dtypes else \
