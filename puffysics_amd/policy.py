@@ -227,11 +227,12 @@ def log_probs(logits, taken, mask=None, top=0):
     _need(logits.dim() >= 1 and logits.shape[-1] >= 1, "logits need at least one action")
     _need(not (taken.is_floating_point() or taken.is_complex() or taken.dtype == torch.bool), "taken has to be whole numbers")
     _need(taken.shape == logits.shape[:-1], "taken has to have the shape of logits without the last axis")
-    # a level is entered: the tensor may have a tangent
-    _need(forward_ad._current_level < 0 or forward_ad.unpack_dual(logits).tangent is None,
-          "log_probs has no forward-mode derivative")
+    # where a level is entered the tensor may have a tangent
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(logits).tangent is not None:
+        raise ValueError("log_probs has no forward-mode derivative")
     actions = logits.shape[-1]
-    _need(actions <= MAX_ACTIONS and taken.numel() <= MAX_ROWS, "at most 2^21 actions and 2^31 - 1 rows")
+    if actions > MAX_ACTIONS or taken.numel() > MAX_ROWS:
+        raise ValueError("at most 2^21 actions and 2^31 - 1 rows")
     _need(0 <= top <= MAX_TOP and top <= actions, "top has to be between 0 and 32, and at most the actions")
     _on(logits, taken, mask)
     if mask is not None:
@@ -239,7 +240,8 @@ def log_probs(logits, taken, mask=None, top=0):
         _need(mask.shape == logits.shape or mask.shape == (actions,),
               "mask has to have the shape of logits, or of one row")
         mask = _rows(mask.reshape(-1, actions))
-    logits = _as_read(logits)
+    if logits.is_neg():
+        logits = _as_read(logits)
     shape = taken.shape
     if len(shape) != 1:
         logits, taken = logits.reshape(-1, actions), taken.reshape(-1)
@@ -277,12 +279,14 @@ def advantages(rewards, values, terminals, last_values, gamma=0.99, lam=0.95):
     _need(last_values.shape == rewards.shape[1:] and last_values.dtype == values.dtype,
           "last_values have to be [envs], of the type of values")
     _need(terminals.dtype in (torch.float32, torch.bool, torch.uint8), "terminals have to be float32, bool or uint8")
-    _need(max(rewards.shape) <= MAX_ROWS or not rewards.numel(), "at most 2^31 - 1 steps and environments")
+    steps, envs = rewards.shape
+    if (steps > MAX_ROWS or envs > MAX_ROWS) and rewards.numel():
+        raise ValueError("at most 2^31 - 1 steps and environments")
     _need(0 <= gamma <= 1 and 0 <= lam <= 1, "gamma and lam have to be between 0 and 1")
     _on(rewards, values, terminals, last_values)
-    rewards, values, last_values = _as_read(rewards), _as_read(values), _as_read(last_values)
+    if rewards.is_neg() or values.is_neg() or last_values.is_neg():
+        rewards, values, last_values = _as_read(rewards), _as_read(values), _as_read(last_values)
     lib = policy_lib()
-    steps, envs = rewards.shape
     # the longer stride is the outer axis: (steps, envs) unless the rewards are a transposed array
     turned = rewards.stride(0) < rewards.stride(1)
     out = torch.empty((2, envs, steps) if turned else (2, steps, envs), dtype=torch.float32, device=rewards.device)
