@@ -345,9 +345,11 @@ bool whole_lines(const void* p, const int64_t stride[2], int64_t size, int cols)
 }
 
 /* Inputs that the caches would not keep go past them where no line is read by
- * two workgroups: 500 steps of 65,536 environments take 119 us so, and 143 us
- * through the caches; 128 steps of 32,768 take 21 and 19 us; 500 of 65,537,
- * which share lines, 171 and 143 us. */
+ * two workgroups: 500 steps of 65,536 environments with bf16 values take 106 us
+ * so, and 125 through the caches; 128 steps of 32,768 in fp32, which the caches
+ * keep, 25 and 24.  Where lines are shared it goes either way: 500 of 65,537
+ * take 131 us past them and 145 through, 128 of 300,007 178 and 162, 2,000 of
+ * 16,387 210 and 179. */
 bool stream_inputs(const B3Rollout& g, const Plan& p) {
     const int64_t value = g.values_type == B3_F32 ? 4 : 2, end = g.terminals_type == B3_F32 ? 4 : 1;
     return p.by_env && p.pieces == 1 && g.steps * g.envs > ((int64_t)1 << 27) / (4 + value + end)

@@ -824,14 +824,14 @@ void with_type(int type, F f) {
 }
 
 /* Logits that the caches cannot hold from the forward pass to the backward go
- * past them (4,096 rows of 131,072 in bf16: 161 and 350 us forward and
- * backward, not 178 and 363); smaller ones do not (8,192 rows of 1,024: 11.1
- * us for both passes, 12.4 us past the caches). */
+ * past them (4,096 rows of 131,072 in bf16: 161 and 352 us forward and
+ * backward, not 177 and 369); smaller ones do not (8,192 rows of 1,024: 17.0
+ * us for both passes in a graph, 18.6 past the caches). */
 bool stream_logits(const B3Logits& g) { return g.rows * g.actions * (g.type == B3_F32 ? 4 : 2) > (int64_t)1 << 28; }
 
 /* Pieces of a row.  8,192 actions to a workgroup of 256 threads, also where
- * one of 512 could hold the row (16,384 rows of 16,384 in bf16: 86 us, not
- * 103; of 14,000: 82 us, not 123): with fewer to a barrier, loads and sums of
+ * one of 512 could hold the row (16,384 rows of 16,384 in bf16: 88 us, not
+ * 96; of 14,000: 88 us, not 117): with fewer to a barrier, loads and sums of
  * different workgroups overlap.  Where pieces of 8,192 would not give every
  * compute unit two, 4,096. */
 Pieces pieces_of(int64_t rows, int64_t actions) {
