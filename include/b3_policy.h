@@ -1,6 +1,6 @@
 /*
- * b3_policy.h - what a policy's update needs next to the environments' step,
- * on the device buffers that the environments fill (b3_hover.h).
+ * b3_policy.h - what a policy needs next to the environments' step, on the
+ * device buffers that the environments fill (b3_hover.h).
  *
  *   log probabilities   of the taken actions under rows of logits, with the
  *                       rows' entropies, their best alternatives, and the
@@ -8,13 +8,18 @@
  *   advantages          of a rollout's rewards, values and terminals
  *   AdamW               one step over all of a policy's tensors, moments in
  *                       32 or 8 bits, with the clip of the gradients' norm
+ *   linear attention    a memory over a rollout's steps that decays and ends
+ *                       with the episode, its gradient, and one step of it
+ *   norm                root mean square, with the residual's addition, its
+ *                       gradient, and an output in 8 bits
+ *   Muon                one step over a policy's matrices, orthogonalised
  *
  * The reference leaves these to the trainer (docs/RL_LIBRARY.md).
  * Conventions are the engine's (b3_engine.h): hipError_t returns, no abort;
  * hipErrorInvalidValue for bad arguments with nothing launched; no work is a
  * successful no-op; the *_gpu functions enqueue on `stream` without
  * allocating or synchronising, on the current device, whose memory every
- * pointer is.  b3_adamw_create alone allocates.  Arrays need the alignment
+ * pointer is.  b3_adamw_create and b3_muon_create alone allocate.  Arrays need the alignment
  * of their elements and no more (8-bit moments none), workspaces that of 8
  * bytes.  Results do not depend on the order in which workgroups run.
  */
@@ -190,6 +195,138 @@ hipError_t b3_adamw_load_moments_gpu(B3AdamW* optimizer, const float* exp_avg, c
 
 /* Waits for the device; the weights and the state are left.  NULL is a no-op. */
 hipError_t b3_adamw_destroy(B3AdamW* optimizer);
+
+/* ---- linear attention ---- */
+
+#define B3_MAX_HEAD 128
+
+/* q and k [steps, envs, heads, key], v [steps, envs, heads, value]: strides
+ * in elements from step to step, environment to environment and head to
+ * head; a head's elements are contiguous.  `decay` [heads] is in [0, 1] (NaN
+ * outside).  `starts` is NULL or [steps, envs], nonzero where a step begins
+ * an episode: what lies before is dropped (not multiplied by 0: its NaN stay
+ * there).  `state` [envs, heads, key, value], contiguous, is what the first
+ * step finds; NULL: zeros. */
+typedef struct B3Attention {
+    int64_t steps, envs, heads;
+    int key, value;              /* 1 .. B3_MAX_HEAD */
+    int type;                    /* of q, k, v, the result and gradients */
+    const void *q, *k, *v;
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+    const float* decay;
+    const void* starts;
+    int starts_type;             /* B3_F32 or B3_U8 */
+    int64_t starts_stride[2];
+    const float* state;
+    double scale;
+} B3Attention;
+
+/* Bytes of workspace of either direction (0 for many sequences or few steps). */
+size_t b3_linear_attention_workspace(const B3Attention* attention, int backward);
+
+/*   S_t = decay S_{t-1} + k_t^T v_t (without the first term where an episode
+ *   starts), out_t = scale q_t S_t
+ * out [steps, envs, heads, value], contiguous; last_state (NULL: not wanted)
+ * like `state`, which it may be: S after the last step. */
+hipError_t b3_linear_attention_gpu(const B3Attention* attention, void* out, float* last_state, void* workspace,
+    size_t workspace_bytes, hipStream_t stream);
+
+/* Gradients from those of out (strides as q's) and, unless NULL, of
+ * last_state (contiguous); d_q, d_k and d_v are contiguous, d_state is like
+ * `state`.  NULL results are not wanted. */
+hipError_t b3_linear_attention_backward_gpu(const B3Attention* attention, const void* d_out,
+    const int64_t d_out_stride[3], const float* d_last_state, void* d_q, void* d_k, void* d_v, float* d_state,
+    void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* One step of every environment (steps is 1), attention->state in place.
+ * out [envs, heads, value], contiguous. */
+hipError_t b3_linear_attention_step_gpu(const B3Attention* attention, float* state, void* out, hipStream_t stream);
+
+/* ---- norm ---- */
+
+/* Rows of `width` contiguous elements, each array's rows its stride apart (in
+ * elements, at least `width`).  h = x + residual (NULL: none), in 32 bits. */
+typedef struct B3Norm {
+    int64_t rows, width;         /* width 1 .. 2^21 */
+    int type;                    /* of x, residual and what comes of them */
+    const void* x;
+    int64_t x_stride;
+    const void* residual;
+    int64_t residual_stride;
+    const void* weight;          /* [width], NULL: ones */
+    int weight_type;             /* `type`, or B3_F32 */
+    double eps;                  /* at least 0 */
+} B3Norm;
+
+/* out = weight h / sqrt(mean of h^2 + eps); with a residual, sum = h; root
+ * [rows] = 1 / sqrt(mean of h^2 + eps).  out and sum are contiguous; sum
+ * and root may be NULL. */
+hipError_t b3_rms_norm_gpu(const B3Norm* norm, void* out, void* sum, float* root, hipStream_t stream);
+
+/* The same, out as OCP e4m3 numbers, rounded to the nearest, with the exponent
+ * byte b of a scale 2^(b - 127) for every 32 of a row: the least power with
+ * which none passes 448.  out [rows, width] and scale [rows, ceil(width / 32)]
+ * are contiguous.  What is not finite becomes NaN. */
+hipError_t b3_rms_norm_8bit_gpu(const B3Norm* norm, unsigned char* out, unsigned char* scale, void* sum,
+    hipStream_t stream);
+
+/* The values that such numbers stand for, in `type`. */
+hipError_t b3_values_of_8bit_gpu(int64_t rows, int64_t width, const unsigned char* in, const unsigned char* scale,
+    void* out, int type, hipStream_t stream);
+
+/* Gradients: d_x (also the residual's) and d_weight, of weight_type (NULL: not
+ * wanted), from those of out and sum (NULL: zero).  norm->x is h, as the sum
+ * or as x where there is no residual; norm->residual is not read. */
+size_t b3_rms_norm_backward_workspace(int64_t rows, int64_t width);
+hipError_t b3_rms_norm_backward_gpu(const B3Norm* norm, const float* root, const void* d_out, int64_t d_out_stride,
+    const void* d_sum, int64_t d_sum_stride, void* d_x, void* d_weight, void* workspace, size_t workspace_bytes,
+    hipStream_t stream);
+
+/* ---- Muon ---- */
+
+/* A matrix's weights: rows x columns contiguous elements. */
+typedef struct B3MuonMatrix {
+    void* param;
+    int type;                    /* B3_F32, B3_F16 or B3_BF16 */
+    int64_t rows, columns;
+    double weight_decay;
+} B3MuonMatrix;
+
+/* Flat arrays of b3_muon_size() elements, laid out as AdamW's: `momentum`, and
+ * `master`, the 32-bit copies of 16-bit weights (NULL keeps none), with the
+ * same meaning. */
+typedef struct B3MuonState {
+    float* momentum;
+    float* master;
+} B3MuonState;
+
+typedef struct B3MuonConfig {
+    double momentum;             /* in [0, 1) */
+    int nesterov;
+    int newton_schulz;           /* steps, 1 .. 16 */
+    double eps;                  /* over 0 */
+} B3MuonConfig;
+
+typedef struct B3Muon B3Muon;
+
+int64_t b3_muon_size(const B3MuonMatrix* matrices, int count);
+
+/* As b3_adamw_create.  Allocates what a step works in too. */
+hipError_t b3_muon_create(B3Muon** out, const B3MuonMatrix* matrices, int count, B3MuonState state,
+    B3MuonConfig config);
+
+/* One step of the matrices that have a gradient, given as b3_adamw_step_gpu's:
+ *   m = momentum m + g          u = g + momentum m with nesterov, else m
+ *   x = u / (|u| + eps), its transpose where rows > columns
+ *   newton_schulz times: a = x x^T, x = 3.4445 x + (-4.775 a + 2.0315 a a) x
+ *   w = w (1 - lr decay) - lr sqrt(max(1, rows / columns)) x
+ * with products of 32-bit numbers.  Steps of one optimizer must follow one
+ * another on the device. */
+hipError_t b3_muon_step_gpu(B3Muon* optimizer, const void* const* grads, const int* grad_types, double lr,
+    hipStream_t stream);
+
+/* Waits for the device; the weights and the state are left.  NULL is a no-op. */
+hipError_t b3_muon_destroy(B3Muon* optimizer);
 
 #ifdef __cplusplus
 }

@@ -1,6 +1,9 @@
-"""What a policy's update needs next to the environments' step
-(include/b3_policy.h): `advantages` of a rollout, `log_probs` of the taken
-actions with entropies, best alternatives and the gradient, and `AdamW`.
+"""What a policy needs next to the environments' step (include/b3_policy.h):
+`advantages` of a rollout, `log_probs` of the taken actions with entropies,
+best alternatives and the gradient, `AdamW`; for a policy with memory
+`linear_attention` over a rollout, `linear_attention_step` when it acts,
+`rms_norm` with the residual's addition, `rms_norm_8bit`, and `Muon` for its
+matrices.
 
 The arrays are torch CUDA tensors; the work is enqueued on the current torch
 stream and runs in libb3policy.so.  Arguments that do not fit raise
@@ -10,6 +13,7 @@ The reference leaves these to the trainer (docs/RL_LIBRARY.md).
 import array
 import collections
 import ctypes as C
+import math
 import operator
 import os
 
@@ -23,7 +27,11 @@ POLICY_PATH = os.path.join(_native.HERE, "libb3policy.so")
 MAX_TOP = 32
 MAX_ACTIONS = 1 << 21
 MAX_ROWS = (1 << 31) - 1     # and steps and environments of a rollout
+MAX_HEAD = 128               # dimensions of a head of linear attention
+MAX_SEQUENCES = (1 << 24) - 1
+MAX_WIDTH = 1 << 21          # of a norm's row
 SEGMENT = 256
+_GROUP = 32                  # 8-bit numbers to a scale
 _SMALL = 2048                # rows of up to so many actions need no workspace
 _EMPTY = 8                   # stands for the address of a gradient without elements; NULL is no gradient
 # what a step asks of every tensor, called by map: a policy may have many small ones
@@ -60,6 +68,30 @@ class B3AdamWConfig(C.Structure):
     _fields_ = [("beta1", _d), ("beta2", _d), ("eps", _d), ("seed", C.c_uint32)]
 
 
+class B3Attention(C.Structure):
+    _fields_ = [("steps", _ll), ("envs", _ll), ("heads", _ll), ("key", _i), ("value", _i), ("type", _i), ("q", _vp),
+                ("k", _vp), ("v", _vp), ("q_stride", _ll * 3), ("k_stride", _ll * 3), ("v_stride", _ll * 3),
+                ("decay", _vp), ("starts", _vp), ("starts_type", _i), ("starts_stride", _ll * 2), ("state", _vp),
+                ("scale", _d)]
+
+
+class B3Norm(C.Structure):
+    _fields_ = [("rows", _ll), ("width", _ll), ("type", _i), ("x", _vp), ("x_stride", _ll), ("residual", _vp),
+                ("residual_stride", _ll), ("weight", _vp), ("weight_type", _i), ("eps", _d)]
+
+
+class B3MuonMatrix(C.Structure):
+    _fields_ = [("param", _vp), ("type", _i), ("rows", _ll), ("columns", _ll), ("weight_decay", _d)]
+
+
+class B3MuonState(C.Structure):
+    _fields_ = [("momentum", _vp), ("master", _vp)]
+
+
+class B3MuonConfig(C.Structure):
+    _fields_ = [("momentum", _d), ("nesterov", _i), ("newton_schulz", _i), ("eps", _d)]
+
+
 POLICY_SYMBOLS = [
     ("b3_log_probs_workspace", _sz, [_ll, _ll, _i]),
     ("b3_log_probs_gpu", _i, [B3Logits, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _sz, _vp]),
@@ -74,6 +106,20 @@ POLICY_SYMBOLS = [
     ("b3_adamw_moments_gpu", _i, [_vp, _vp, _vp, _vp]),
     ("b3_adamw_load_moments_gpu", _i, [_vp, _vp, _vp, _vp]),
     ("b3_adamw_destroy", _i, [_vp]),
+    ("b3_linear_attention_workspace", _sz, [C.POINTER(B3Attention), _i]),
+    ("b3_linear_attention_gpu", _i, [C.POINTER(B3Attention), _vp, _vp, _vp, _sz, _vp]),
+    ("b3_linear_attention_backward_gpu", _i, [C.POINTER(B3Attention), _vp, _ll * 3, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
+                                              _vp]),
+    ("b3_linear_attention_step_gpu", _i, [C.POINTER(B3Attention), _vp, _vp, _vp]),
+    ("b3_rms_norm_gpu", _i, [C.POINTER(B3Norm), _vp, _vp, _vp, _vp]),
+    ("b3_rms_norm_8bit_gpu", _i, [C.POINTER(B3Norm), _vp, _vp, _vp, _vp]),
+    ("b3_values_of_8bit_gpu", _i, [_ll, _ll, _vp, _vp, _vp, _i, _vp]),
+    ("b3_rms_norm_backward_workspace", _sz, [_ll, _ll]),
+    ("b3_rms_norm_backward_gpu", _i, [C.POINTER(B3Norm), _vp, _vp, _ll, _vp, _ll, _vp, _vp, _vp, _sz, _vp]),
+    ("b3_muon_size", _ll, [C.POINTER(B3MuonMatrix), _i]),
+    ("b3_muon_create", _i, [C.POINTER(_vp), C.POINTER(B3MuonMatrix), _i, B3MuonState, B3MuonConfig]),
+    ("b3_muon_step_gpu", _i, [_vp, _vp, _vp, _d, _vp]),
+    ("b3_muon_destroy", _i, [_vp]),
 ]
 
 _lib = None
@@ -126,6 +172,17 @@ def _as_read(x):
     """x, or where its elements are only marked as negated, as those of a
     conjugate's imaginary part are, a copy that holds them so."""
     return x if x is None or not x.is_neg() else x.resolve_neg()
+
+
+def _no_tangent(name, *tensors):
+    # where a level is entered a tensor may have a tangent
+    if forward_ad._current_level >= 0 and any(
+            x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+        raise ValueError("%s has no forward-mode derivative" % name)
+
+
+def _needs_grad(*tensors):
+    return torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in tensors)
 
 
 # ---- log probabilities ----
@@ -302,28 +359,316 @@ def advantages(rewards, values, terminals, last_values, gamma=0.99, lam=0.95):
     return adv, ret
 
 
-# ---- AdamW ----
+# ---- linear attention ----
 
-class AdamW:
-    """AdamW over all of `params` in one step: contiguous float32, float16 or
-    bfloat16 tensors on the current device, no two of which overlap.
+LinearAttention = collections.namedtuple("LinearAttention", "out state")
 
-    state_bits     32, or 8: moments as e4m3 numbers (the first, and the root
-                   of the second) with a power of two for every 32 of them,
-                   rounded by random bits that `seed`, step and place give
-    max_grad_norm  the global norm that gradients are scaled down to, or None
-    weight_decay   a number, or one for each tensor
-    master         keep 32-bit copies of 16-bit weights and round those; without
-                   them small updates of such weights are lost.  A weight that
-                   was written between two steps counts, not its copy
 
-    The moments lie in flat arrays, tensor i's from offsets[i] on.  Steps of
-    one optimizer follow one another: on several streams, order them.  A step
-    that is captured in a graph repeats the bias corrections of its own count
-    in every replay; 8-bit moments are rounded by other bits each time."""
+def _heads(x):
+    """x, or a copy of it, with contiguous heads."""
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32,
-                 max_grad_norm=None, master=True, seed=0):
+
+def _attention(q, k, v, decay, state, starts, scale):
+    """B3Attention of q, k [steps, envs, heads, key], v [.., value]."""
+    steps, envs, heads, key = q.shape
+    return B3Attention(steps, envs, heads, key, v.shape[-1], _TYPE[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                       q.stride()[:3], k.stride()[:3], v.stride()[:3], decay.data_ptr(),
+                       None if starts is None else starts.data_ptr(),
+                       _F32 if starts is not None and starts.dtype == torch.float32 else _U8,
+                       (0, 0) if starts is None else starts.stride(), None if state is None else state.data_ptr(), scale)
+
+
+def _work(size, device):
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+
+
+def _address_of(x):
+    return None if x is None else x.data_ptr()
+
+
+def _attend(q, k, v, decay, state, starts, scale, last):
+    """(out, state after the last step or None)"""
+    lib = policy_lib()
+    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    left = torch.empty((*q.shape[1:], v.shape[-1]), dtype=torch.float32, device=v.device) if last else None
+    g = _attention(q, k, v, decay, state, starts, scale)
+    size = lib.b3_linear_attention_workspace(C.byref(g), 0)
+    work = _work(size, v.device)
+    _check("b3_linear_attention_gpu", lib.b3_linear_attention_gpu(
+        C.byref(g), out.data_ptr(), _address_of(left), _address_of(work), size, _stream()))
+    return out, left
+
+
+class _LinearAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, decay, state, starts, scale, last):
+        out, left = _attend(q, k, v, decay, state, starts, scale, last)
+        ctx.save_for_backward(q, k, v, decay, state, starts)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return out, left
+
+    @staticmethod
+    def backward(ctx, d_out, d_left):
+        # a gradient that is differentiated again says that it cannot be
+        return (_attention_backward_once if torch.is_grad_enabled() else _attention_backward)(ctx, d_out, d_left)
+
+
+def _attention_backward(ctx, d_out, d_left):
+    q, k, v, decay, state, starts = ctx.saved_tensors
+    lib = policy_lib()
+    d_out = torch.zeros_like(v) if d_out is None else _heads(_as_read(d_out))
+    d_left = None if d_left is None else _as_read(d_left).contiguous()
+    new = lambda wanted, like, dtype: torch.empty(like.shape, dtype=dtype, device=v.device) if wanted else None  # noqa: E731
+    d_q, d_k, d_v, d_state = (new(ctx.needs_input_grad[i], x, v.dtype if i < 3 else torch.float32)
+                              for i, x in ((0, q), (1, k), (2, v), (4, state)))
+    g = _attention(q, k, v, decay, state, starts, ctx.scale)
+    size = lib.b3_linear_attention_workspace(C.byref(g), 1)
+    work = _work(size, v.device)
+    _check("b3_linear_attention_backward_gpu", lib.b3_linear_attention_backward_gpu(
+        C.byref(g), d_out.data_ptr(), (_ll * 3)(*d_out.stride()[:3]), _address_of(d_left), _address_of(d_q),
+        _address_of(d_k), _address_of(d_v), _address_of(d_state), _address_of(work), size, _stream()))
+    return d_q, d_k, d_v, None, d_state, None, None, None
+
+
+_attention_backward_once = torch.autograd.function.once_differentiable(_attention_backward)
+
+
+def _check_attention(q, k, v, decay, starts, scale):
+    _need(q.dtype in _TYPE and k.dtype == q.dtype and v.dtype == q.dtype,
+          "q, k and v have to be float32, float16 or bfloat16, all of one type")
+    _need(k.shape == q.shape and v.shape[:-1] == q.shape[:-1], "q and k need one shape, v the same but for the last axis")
+    _need(1 <= q.shape[-1] <= MAX_HEAD and 1 <= v.shape[-1] <= MAX_HEAD, "a head has 1 to 128 dimensions")
+    envs, heads = q.shape[-3:-1]
+    _need(decay.dtype == torch.float32 and decay.shape == (heads,), "decay has to be float32 [heads]")
+    _need(not decay.requires_grad, "decay has no gradient")
+    _need(envs * heads <= MAX_SEQUENCES and (q.dim() == 3 or q.shape[0] <= MAX_ROWS),
+          "at most 2^24 - 1 sequences (environments times heads) and 2^31 - 1 steps")
+    _need(math.isfinite(scale), "scale has to be a finite number")
+    _need(starts is None or (starts.shape == q.shape[:-2] and starts.dtype in (torch.float32, torch.bool, torch.uint8)),
+          "starts have to be float32, bool or uint8, one for each step and environment")
+
+
+def linear_attention(q, k, v, decay, state=None, starts=None, scale=1.0, last=False):
+    """Linear attention over a rollout, a memory that decays and ends with the
+    episode, as LinearAttention(out, state):
+    S_t = decay S_{t-1} + k_t^T v_t (S_t = k_t^T v_t where an episode starts),
+    out_t = scale q_t S_t.
+
+    q, k    [steps, envs, heads, key], float32, float16 or bfloat16
+    v       [steps, envs, heads, value], of their type
+    decay   [heads] float32, in [0, 1] (others give NaN); has no gradient
+    state   None (zeros) or [envs, heads, key, value] float32: what the first
+            step finds, as an earlier call returned it
+    starts  None or [steps, envs] float32, bool or uint8: nonzero where a step
+            begins an episode (HoverEnvs.terminals before the step)
+    last    whether to return the state after the last step, else None
+
+    Any strides; key and value are at most 128.  out is laid out contiguously.
+    Differentiable in q, k, v and state (backward and once; a tangent is
+    refused).  States and sums are in 32 bits; what lies before an episode's
+    start, and later steps, have no say in a step, whatever they hold."""
+    _need(q.dim() == 4, "q has to be [steps, envs, heads, key]")
+    _check_attention(q, k, v, decay, starts, scale)
+    if state is not None:
+        _need(state.dtype == torch.float32 and state.shape == (*q.shape[1:], v.shape[-1]),
+              "state has to be float32 [envs, heads, key, value]")
+    _no_tangent("linear_attention", q, k, v, state)
+    _on(q, k, v, decay, state, starts)
+    q, k, v = (_heads(_as_read(x)) for x in (q, k, v))
+    decay = _as_read(decay).contiguous()
+    if starts is not None:
+        starts = _as_read(starts)
+    if state is not None:
+        state = _as_read(state).contiguous()
+    if _needs_grad(q, k, v, state):
+        return LinearAttention(*_LinearAttention.apply(q, k, v, decay, state, starts, float(scale), bool(last)))
+    return LinearAttention(*_attend(q, k, v, decay, state, starts, scale, last))
+
+
+def linear_attention_step(q, k, v, decay, state, starts=None, scale=1.0):
+    """One step of linear_attention for every environment; returns out
+    [envs, heads, value] and updates `state` [envs, heads, key, value], float32
+    and contiguous, in place.  q, k [envs, heads, key], v [envs, heads, value],
+    starts [envs]; no gradient."""
+    _need(q.dim() == 3, "q has to be [envs, heads, key]")
+    _check_attention(q, k, v, decay, starts, scale)
+    _need(state.dtype == torch.float32 and state.shape == (*q.shape, v.shape[-1]) and state.is_contiguous()
+          and not state.is_neg(), "state has to be float32 [envs, heads, key, value], contiguous, not marked as negated")
+    if _needs_grad(q, k, v, state):
+        raise ValueError("linear_attention_step has no gradient")
+    _no_tangent("linear_attention_step", q, k, v, state)
+    _on(q, k, v, decay, state, starts)
+    q, k, v = (_heads(_as_read(x)) for x in (q, k, v))
+    decay = _as_read(decay).contiguous()
+    if starts is not None:
+        starts = _as_read(starts)[None]
+    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    g = _attention(q[None], k[None], v[None], decay, None, starts, scale)
+    _check("b3_linear_attention_step_gpu", policy_lib().b3_linear_attention_step_gpu(
+        C.byref(g), state.data_ptr(), out.data_ptr(), _stream()))
+    _written(state)
+    return out
+
+
+def _written(x):
+    """What an operation in place does to a tensor's count of versions."""
+    if not x.is_inference():
+        torch.autograd.graph.increment_version(x)
+
+
+# ---- norm ----
+
+RmsNorm = collections.namedtuple("RmsNorm", "out sum")
+RmsNorm8 = collections.namedtuple("RmsNorm8", "out scale sum")
+
+
+def _norm(x, residual, weight, eps):
+    """B3Norm of x, residual [rows, width]."""
+    rows, width = x.shape
+    stride = lambda y: y.stride(0) if rows > 1 else width  # noqa: E731
+    return B3Norm(rows, width, _TYPE[x.dtype], x.data_ptr(), stride(x), _address_of(residual),
+                  0 if residual is None else stride(residual), _address_of(weight),
+                  0 if weight is None else _TYPE[weight.dtype], eps)
+
+
+def _normalise(x, weight, residual, eps, kept):
+    """(out, sum or None, root or None), the last only where `kept`."""
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    total = None if residual is None else torch.empty_like(out)
+    root = torch.empty(x.shape[0], dtype=torch.float32, device=x.device) if kept else None
+    g = _norm(x, residual, weight, eps)
+    _check("b3_rms_norm_gpu", policy_lib().b3_rms_norm_gpu(
+        C.byref(g), out.data_ptr(), _address_of(total), _address_of(root), _stream()))
+    return out, total, root
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        shape = x.shape
+        x, residual = _as_rows(x), _as_rows(residual)
+        out, total, root = _normalise(x, weight, residual, eps, True)
+        ctx.save_for_backward(x if residual is None else total, weight, root)
+        ctx.set_materialize_grads(False)
+        return out.view(shape), None if total is None else total.view(shape)
+
+    @staticmethod
+    def backward(ctx, d_out, d_sum):
+        return (_norm_backward_once if torch.is_grad_enabled() else _norm_backward)(ctx, d_out, d_sum)
+
+
+def _norm_backward(ctx, d_out, d_sum):
+    h, weight, root = ctx.saved_tensors
+    rows, width = h.shape
+    lib = policy_lib()
+    shape = (d_sum if d_out is None else d_out).shape
+    d_out, d_sum = _as_rows(d_out), _as_rows(d_sum)
+    stride = lambda y: 0 if y is None else y.stride(0) if rows > 1 else width  # noqa: E731
+    d_x = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    d_weight = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
+    size = lib.b3_rms_norm_backward_workspace(rows, width)
+    work = _work(size, h.device)
+    g = _norm(h, None, weight, 0.0)
+    _check("b3_rms_norm_backward_gpu", lib.b3_rms_norm_backward_gpu(
+        C.byref(g), root.data_ptr(), _address_of(d_out), stride(d_out), _address_of(d_sum), stride(d_sum), d_x.data_ptr(),
+        _address_of(d_weight), _address_of(work), size, _stream()))
+    # one tensor for both, as a sum's gradient is: views of it would become the grad of two leaves
+    d_x = d_x.view(shape)
+    return (d_x if ctx.needs_input_grad[0] else None, d_weight, d_x if ctx.needs_input_grad[2] else None, None)
+
+
+_norm_backward_once = torch.autograd.function.once_differentiable(_norm_backward)
+
+
+def _check_norm(x, weight, residual, eps):
+    _need(x.dtype in _TYPE, "x has to be float32, float16 or bfloat16")
+    _need(x.dim() >= 1 and 1 <= x.shape[-1] <= MAX_WIDTH, "x needs rows of 1 to 2^21 elements")
+    _need(x.numel() // x.shape[-1] <= MAX_ROWS, "at most 2^31 - 1 rows")
+    _need(residual is None or (residual.shape == x.shape and residual.dtype == x.dtype),
+          "residual has to have the shape and type of x")
+    _need(weight is None or (weight.shape == x.shape[-1:] and weight.dtype in (x.dtype, torch.float32)),
+          "weight has to be a row, of the type of x or float32")
+    _need(eps >= 0, "eps has to be at least 0")
+
+
+def _as_rows(x):
+    """x as contiguous rows that do not overlap, or None."""
+    return None if x is None else _rows(_as_read(x).reshape(-1, x.shape[-1]))
+
+
+def rms_norm(x, weight=None, residual=None, eps=1e-6):
+    """Rows of x, plus those of `residual`, over their root mean square, as
+    RmsNorm(out, sum): sum = x + residual (None without a residual),
+    out = weight sum / sqrt(mean of sum^2 + eps).
+
+    x         [..., width], float32, float16 or bfloat16
+    weight    None (ones) or [width], of x's type or float32
+    residual  None or like x
+
+    out is of the sum before it is rounded to x's type.  Any strides; the
+    results are contiguous.  Differentiable in x, weight and residual (backward
+    and once; a tangent is refused)."""
+    _check_norm(x, weight, residual, eps)
+    _no_tangent("rms_norm", x, weight, residual)
+    _on(x, weight, residual)
+    weight = None if weight is None else _as_read(weight).contiguous()
+    if _needs_grad(x, weight, residual):
+        return RmsNorm(*_RmsNorm.apply(x, weight, residual, float(eps)))
+    out, total, _ = _normalise(_as_rows(x), weight, _as_rows(residual), eps, False)
+    return RmsNorm(out.view(x.shape), None if total is None else total.view(x.shape))
+
+
+def rms_norm_8bit(x, weight=None, residual=None, eps=1e-6):
+    """rms_norm with out in 8 bits, as RmsNorm8(out, scale, sum): float8_e4m3fn
+    numbers [..., width], rounded to the nearest, with a power of two
+    (float8_e8m0fnu) for every 32 of a row, scale [..., ceil(width / 32)]: the
+    least with which none passes 448.  No gradient."""
+    _check_norm(x, weight, residual, eps)
+    if _needs_grad(x, weight, residual):
+        raise ValueError("rms_norm_8bit has no gradient")
+    _no_tangent("rms_norm_8bit", x, weight, residual)
+    _on(x, weight, residual)
+    shape = x.shape
+    groups = -(-shape[-1] // _GROUP)
+    x, residual = _as_rows(x), _as_rows(residual)
+    weight = None if weight is None else _as_read(weight).contiguous()
+    out = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty((x.shape[0], groups), dtype=torch.float8_e8m0fnu, device=x.device)
+    total = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    g = _norm(x, residual, weight, eps)
+    _check("b3_rms_norm_8bit_gpu", policy_lib().b3_rms_norm_8bit_gpu(
+        C.byref(g), out.data_ptr(), scale.data_ptr(), _address_of(total), _stream()))
+    return RmsNorm8(out.view(shape), scale.view(*shape[:-1], groups), None if total is None else total.view(shape))
+
+
+def values_of_8bit(x, scale, dtype=torch.bfloat16):
+    """The values, in `dtype`, that float8_e4m3fn numbers with a power of two
+    for every 32 of a row stand for (rms_norm_8bit).  bfloat16 holds them
+    exactly but for what lies below its range."""
+    _need(x.dtype == torch.float8_e4m3fn and scale.dtype == torch.float8_e8m0fnu,
+          "x has to be float8_e4m3fn, scale float8_e8m0fnu")
+    _need(x.dim() >= 1 and 1 <= x.shape[-1] <= MAX_WIDTH and x.numel() // x.shape[-1] <= MAX_ROWS,
+          "x needs rows of 1 to 2^21 elements, at most 2^31 - 1")
+    _need(scale.shape == (*x.shape[:-1], -(-x.shape[-1] // _GROUP)), "need a scale for every 32 numbers of a row")
+    _need(dtype in _TYPE, "values have to be float32, float16 or bfloat16")
+    _on(x, scale)
+    x, scale = x.contiguous(), scale.contiguous()
+    out = torch.empty(x.shape, dtype=dtype, device=x.device)
+    _check("b3_values_of_8bit_gpu", policy_lib().b3_values_of_8bit_gpu(
+        x.numel() // x.shape[-1], x.shape[-1], x.data_ptr(), scale.data_ptr(), out.data_ptr(), _TYPE[dtype], _stream()))
+    return out
+
+
+# ---- what the optimizers share ----
+
+class _Optimizer:
+    """Parameters, the layout of flat arrays (parameter i's part from
+    offsets[i] on), 32-bit copies of 16-bit weights, gradients."""
+
+    def _take(self, params, weight_decay):
+        """Sets `params`; the weight decay of each."""
         self._h = _vp()
         self.params = list(params)
         n = len(self.params)
@@ -335,38 +680,23 @@ class AdamW:
         _need(all(a[1] <= b[0] for a, b in zip(spans, spans[1:])), "a parameter is given twice, or two overlap")
         _on(*self.params)
         _need(len(decay) == n and all(d >= 0 for d in decay), "weight_decay has to be at least 0, one for each tensor")
-        _need(0 <= betas[0] < 1 and 0 <= betas[1] < 1 and eps >= 0, "betas have to be in [0, 1), eps at least 0")
-        _need(state_bits in (8, 32), "state_bits has to be 8 or 32")
-        _need(max_grad_norm is None or max_grad_norm > 0, "max_grad_norm has to be over 0, or None")
-        self.lr, self.max_grad_norm, self.state_bits = lr, max_grad_norm, state_bits
-        self.device = torch.device("cuda", torch.cuda.current_device())
-        self._lib = policy_lib()
-        table = (B3AdamWTensor * max(n, 1))(*[B3AdamWTensor(p.data_ptr(), _TYPE[p.dtype], p.numel(), d)
-                                              for p, d in zip(self.params, decay)])
-        self.size = self._lib.b3_adamw_size(table, n)
+        self._at, self._shapes, self._dtypes = ([f(p) for p in self.params] for f in (
+            torch.Tensor.data_ptr, lambda p: p.shape, lambda p: p.dtype))
+        self._empty = any(p.numel() == 0 for p in self.params)
+        return decay
+
+    def _lay_out(self):
         self.offsets, at = [], 0
         for p in self.params:
             self.offsets.append(at)
             at += -(-p.numel() // SEGMENT) * SEGMENT
         assert at == self.size
-        kind = torch.float32 if state_bits == 32 else torch.uint8
-        new = lambda count, dtype: torch.zeros(count, dtype=dtype, device=self.device)  # noqa: E731
-        self._exp_avg, self._exp_avg_sq = new(self.size, kind), new(self.size, kind)
-        scales = self.size // 32 if state_bits == 8 else 0
-        self._scale = new((2, scales), torch.uint8).fill_(1)
+
+    def _make_master(self, master):
         self._master = None
         if master and any(p.dtype != torch.float32 for p in self.params):
-            self._master = new(self.size, torch.float32)
+            self._master = torch.zeros(self.size, dtype=torch.float32, device=self.device)
             self._copy_weights()
-        state = B3AdamWState(state_bits, self._exp_avg.data_ptr(), self._exp_avg_sq.data_ptr(),
-                             self._scale[0].data_ptr(), self._scale[1].data_ptr(),
-                             self._master.data_ptr() if self._master is not None else None)
-        self._at, self._shapes, self._dtypes = ([f(p) for p in self.params] for f in (
-            torch.Tensor.data_ptr, lambda p: p.shape, lambda p: p.dtype))
-        self._empty = any(p.numel() == 0 for p in self.params)
-        torch.cuda.current_stream().synchronize()     # the state is ready for a step on any stream
-        _check("b3_adamw_create", self._lib.b3_adamw_create(C.byref(self._h), table, n, state,
-                                                            B3AdamWConfig(betas[0], betas[1], eps, seed)))
 
     def _views(self, flat):
         return [flat[at:at + p.numel()].view(p.shape) for at, p in zip(self.offsets, self.params)]
@@ -391,17 +721,20 @@ class AdamW:
         """Changes where a program writes to the copies."""
         return None if self._master.is_inference() else self._master._version
 
-    def step(self, grads=None, lr=None):
-        """One step by `grads` (one for each parameter, of its type or
-        float32, None to leave it out), or by the parameters' own `.grad`.
-        Returns the gradients' norm before the clip as a tensor, or None
-        without max_grad_norm."""
+    def _follow_copies(self):
+        """Round the copies to the weights if a program wrote to them."""
+        if self._master is not None and self._version() != self._master_version:
+            self._round_copies()
+
+    def _grads(self, grads):
         if grads is None:
             grads = [p.grad for p in self.params]
         _need(len(grads) == len(self.params), "need one gradient for each parameter")
-        lr = self.lr if lr is None else lr
-        _need(lr >= 0, "lr has to be at least 0")
-        _need(self.max_grad_norm is None or self.max_grad_norm > 0, "max_grad_norm has to be over 0, or None")
+        return grads
+
+    def _pointers(self, grads):
+        """Addresses and, where they are not the parameters', types of the
+        gradients, and the parameters that have one."""
         if list(map(_address, self.params)) != self._at:
             raise ValueError("a parameter's memory is not where it was")
         stepped, shapes, dtypes, given = self.params, self._shapes, self._dtypes, grads
@@ -424,8 +757,88 @@ class AdamW:
             pointers = array.array("Q", [0 if g is None else g.data_ptr() or _EMPTY for g in grads])
         kinds = None if types == dtypes else \
             array.array("i", [_TYPE[d if g is None else g.dtype] for g, d in zip(grads, self._dtypes)])
-        if self._master is not None and self._version() != self._master_version:
-            self._round_copies()
+        return pointers, kinds, stepped
+
+    def master(self):
+        """The flat array of 32-bit copies of 16-bit weights (the places of
+        32-bit weights hold nothing), or None.  What is written there is what
+        the next step goes on from."""
+        return self._master
+
+    def close(self):
+        if self._h:
+            code = self._destroy(self._h)
+            self._h = _vp()
+            _check(self._destroy.__name__, code)
+
+    def __del__(self):
+        try:
+            if getattr(self, "_h", None):
+                self._destroy(self._h)
+                self._h = _vp()
+        except Exception:
+            pass
+
+
+# ---- AdamW ----
+
+class AdamW(_Optimizer):
+    """AdamW over all of `params` in one step: contiguous float32, float16 or
+    bfloat16 tensors on the current device, no two of which overlap.
+
+    state_bits     32, or 8: moments as e4m3 numbers (the first, and the root
+                   of the second) with a power of two for every 32 of them,
+                   rounded by random bits that `seed`, step and place give
+    max_grad_norm  the global norm that gradients are scaled down to, or None
+    weight_decay   a number, or one for each tensor
+    master         keep 32-bit copies of 16-bit weights and round those; without
+                   them small updates of such weights are lost.  A weight that
+                   was written between two steps counts, not its copy
+
+    The moments lie in flat arrays, tensor i's from offsets[i] on.  Steps of
+    one optimizer follow one another: on several streams, order them.  A step
+    that is captured in a graph repeats the bias corrections of its own count
+    in every replay; 8-bit moments are rounded by other bits each time."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32,
+                 max_grad_norm=None, master=True, seed=0):
+        decay = self._take(params, weight_decay)
+        n = len(self.params)
+        _need(0 <= betas[0] < 1 and 0 <= betas[1] < 1 and eps >= 0, "betas have to be in [0, 1), eps at least 0")
+        _need(state_bits in (8, 32), "state_bits has to be 8 or 32")
+        _need(max_grad_norm is None or max_grad_norm > 0, "max_grad_norm has to be over 0, or None")
+        self.lr, self.max_grad_norm, self.state_bits = lr, max_grad_norm, state_bits
+        self.device = torch.device("cuda", torch.cuda.current_device())
+        self._lib = policy_lib()
+        self._destroy = self._lib.b3_adamw_destroy
+        table = (B3AdamWTensor * max(n, 1))(*[B3AdamWTensor(p.data_ptr(), _TYPE[p.dtype], p.numel(), d)
+                                              for p, d in zip(self.params, decay)])
+        self.size = self._lib.b3_adamw_size(table, n)
+        self._lay_out()
+        kind = torch.float32 if state_bits == 32 else torch.uint8
+        new = lambda count, dtype: torch.zeros(count, dtype=dtype, device=self.device)  # noqa: E731
+        self._exp_avg, self._exp_avg_sq = new(self.size, kind), new(self.size, kind)
+        scales = self.size // 32 if state_bits == 8 else 0
+        self._scale = new((2, scales), torch.uint8).fill_(1)
+        self._make_master(master)
+        state = B3AdamWState(state_bits, self._exp_avg.data_ptr(), self._exp_avg_sq.data_ptr(),
+                             self._scale[0].data_ptr(), self._scale[1].data_ptr(),
+                             self._master.data_ptr() if self._master is not None else None)
+        torch.cuda.current_stream().synchronize()     # the state is ready for a step on any stream
+        _check("b3_adamw_create", self._lib.b3_adamw_create(C.byref(self._h), table, n, state,
+                                                            B3AdamWConfig(betas[0], betas[1], eps, seed)))
+
+    def step(self, grads=None, lr=None):
+        """One step by `grads` (one for each parameter, of its type or
+        float32, None to leave it out), or by the parameters' own `.grad`.
+        Returns the gradients' norm before the clip as a tensor, or None
+        without max_grad_norm."""
+        grads = self._grads(grads)
+        lr = self.lr if lr is None else lr
+        _need(lr >= 0, "lr has to be at least 0")
+        _need(self.max_grad_norm is None or self.max_grad_norm > 0, "max_grad_norm has to be over 0, or None")
+        pointers, kinds, stepped = self._pointers(grads)
+        self._follow_copies()
         norm = torch.empty((), dtype=torch.float32, device=self.device) if self.max_grad_norm is not None else None
         _check("b3_adamw_step_gpu", self._lib.b3_adamw_step_gpu(
             self._h, pointers.buffer_info()[0], kinds.buffer_info()[0] if kinds else None,
@@ -444,12 +857,6 @@ class AdamW:
         _check("b3_adamw_moments_gpu", self._lib.b3_adamw_moments_gpu(self._h, out[0].data_ptr(), out[1].data_ptr(),
                                                                       _stream()))
         return out[0], out[1]
-
-    def master(self):
-        """The flat array of 32-bit copies of 16-bit weights (the places of
-        32-bit weights hold nothing), or None.  What is written there is what
-        the next step goes on from."""
-        return self._master
 
     def steps(self, i=0):
         """Steps that parameter i has taken."""
@@ -485,16 +892,82 @@ class AdamW:
         for i, k in enumerate(counts):
             _check("b3_adamw_set_steps", self._lib.b3_adamw_set_steps(self._h, i, operator.index(k)))
 
-    def close(self):
-        if self._h:
-            code = self._lib.b3_adamw_destroy(self._h)
-            self._h = _vp()
-            _check("b3_adamw_destroy", code)
 
-    def __del__(self):
-        try:
-            if getattr(self, "_h", None):
-                self._lib.b3_adamw_destroy(self._h)
-                self._h = _vp()
-        except Exception:
-            pass
+# ---- Muon ----
+
+class Muon(_Optimizer):
+    """Muon over matrices: the momentum of the gradients, orthogonalised by
+    Newton-Schulz steps, is what the weights move by.  `params` are contiguous
+    float32, float16 or bfloat16 matrices on the current device, no two of
+    which overlap (AdamW is for the rest).  A step is
+    m = momentum m + g, u = g + momentum m (u = m without nesterov),
+    x = u / (|u| + eps), newton_schulz times
+    x = 3.4445 x + (-4.775 a + 2.0315 a a) x with a = x x^T, and
+    w = w (1 - lr weight_decay) - lr sqrt(max(1, rows / columns)) x.
+
+    weight_decay   a number, or one for each matrix
+    master         32-bit copies of 16-bit weights, as AdamW's
+
+    Products are those of 32-bit numbers.  The momenta lie in a flat array,
+    matrix i's from offsets[i] on.  Steps of one optimizer follow one another:
+    on several streams, order them.  (K. Jordan and others, "Muon: an optimizer
+    for hidden layers in neural networks", 2024.)"""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, weight_decay=0.0, nesterov=True, newton_schulz=5, eps=1e-7,
+                 master=True):
+        decay = self._take(params, weight_decay)
+        n = len(self.params)
+        _need(all(p.dim() == 2 for p in self.params), "parameters have to be matrices")
+        _need(0 <= momentum < 1 and eps > 0, "momentum has to be in [0, 1), eps over 0")
+        _need(1 <= newton_schulz <= 16, "newton_schulz has to be between 1 and 16")
+        _need(lr >= 0, "lr has to be at least 0")
+        self.lr = lr
+        self.device = torch.device("cuda", torch.cuda.current_device())
+        self._lib = policy_lib()
+        self._destroy = self._lib.b3_muon_destroy
+        table = (B3MuonMatrix * max(n, 1))(*[B3MuonMatrix(p.data_ptr(), _TYPE[p.dtype], *p.shape, d)
+                                             for p, d in zip(self.params, decay)])
+        self.size = self._lib.b3_muon_size(table, n)
+        _need(self.size >= 0, "matrices are too large")
+        self._lay_out()
+        self._momentum = torch.zeros(self.size, dtype=torch.float32, device=self.device)
+        self._make_master(master)
+        torch.cuda.current_stream().synchronize()     # the state is ready for a step on any stream
+        _check("b3_muon_create", self._lib.b3_muon_create(
+            C.byref(self._h), table, n, B3MuonState(self._momentum.data_ptr(), _address_of(self._master)),
+            B3MuonConfig(momentum, bool(nesterov), newton_schulz, eps)))
+
+    def step(self, grads=None, lr=None):
+        """One step by `grads` (one for each matrix, of its type or float32,
+        None to leave it out), or by the matrices' own `.grad`."""
+        grads = self._grads(grads)
+        lr = self.lr if lr is None else lr
+        _need(lr >= 0, "lr has to be at least 0")
+        pointers, kinds, stepped = self._pointers(grads)
+        self._follow_copies()
+        _check("b3_muon_step_gpu", self._lib.b3_muon_step_gpu(
+            self._h, pointers.buffer_info()[0], kinds.buffer_info()[0] if kinds else None, lr, _stream()))
+        torch.autograd.graph.increment_version(stepped)      # as an operation in place does
+
+    def momentum(self):
+        """The state's flat array of momenta."""
+        return self._momentum
+
+    def load_momentum(self, momentum, master=None):
+        """Go on from a list of each matrix's momentum.  Where 32-bit copies of
+        the weights are given, 16-bit weights become what these round to; else
+        the copies are the weights."""
+        n = len(self.params)
+        _need(len(momentum) == n and (master is None or len(master) == n), "need one tensor for each parameter")
+        _need(master is None or self._master is not None, "this optimizer keeps no 32-bit copies")
+        for given in (momentum, master or []):
+            _need(all(x.shape == p.shape for x, p in zip(given, self.params)), "need tensors of the parameters' shapes")
+        with torch.no_grad():
+            for view, x in zip(self._views(self._momentum), momentum):
+                view.copy_(x)
+            for view, x in zip(self._views(self._master) if master is not None else [], master or []):
+                view.copy_(x)
+        if master is not None:
+            self._round_copies()
+        elif self._master is not None:
+            self._copy_weights()

@@ -56,7 +56,7 @@ inline bool holds(const void* workspace, size_t bytes, size_t need) {
     return need == 0 || (bytes >= need && workspace && (uintptr_t)workspace % 8 == 0);
 }
 
-inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline __host__ __device__ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace b3p
 #endif

@@ -1,0 +1,442 @@
+"""puffysics_amd.policy.linear_attention and linear_attention_step against the
+definition in 64 bits."""
+import pytest
+import torch
+
+from memorytest import STEP, attention_gradient_oracle, attention_oracle
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+#        steps, envs, heads, key, value
+SIZES = [(1, 1, 1, 1, 1), (1, 3, 2, 8, 5), (2, 1, 1, 16, 16), (15, 2, 3, 17, 33), (16, 1, 2, 32, 16), (31, 2, 1, 64, 64),
+         (32, 1, 2, 48, 80), (33, 3, 1, 80, 48), (64, 2, 2, 64, 64), (65, 1, 3, 128, 128), (127, 2, 1, 100, 7),
+         (200, 1, 2, 3, 128), (513, 1, 1, 33, 65)]
+
+
+def made(steps, envs, heads, key, value, dtype, seed, rate=0.1):
+    g = torch.Generator().manual_seed(seed)
+    q, k, v = (torch.randn(steps, envs, heads, d, generator=g).to(dtype) for d in (key, key, value))
+    decay = 1 - torch.rand(heads, generator=g) ** 4            # from 0 to nearly 1
+    starts = torch.rand(steps, envs, generator=g) < rate
+    state = torch.randn(envs, heads, key, value, generator=g)
+    return [x.cuda() for x in (q, k, v, decay, starts, state)]
+
+
+def bounds(q, k, v, decay, state, starts, scale):
+    """What the roundings of a step may add up to, relative to a step's own:
+    the same sums of absolute values.  Weights decay^n come from a logarithm
+    that is rounded: n |ln decay| decay^n is at most 2/e decay^(n / 2)."""
+    state = None if state is None else state.abs()
+    return attention_oracle(q.abs(), k.abs(), v.abs(), decay.sqrt(), state, starts, abs(scale))
+
+
+def allowed(dtype, key, steps):
+    """(factor of the sums of absolute values for out, for states): in 32 bits
+    a term goes through the sums over `key` and over the steps, here or in
+    blocks; in bfloat16 the scores are rounded once, states and what enters
+    them are kept as two numbers, to 2^-16."""
+    wide = (key + steps + 64) * 2.0 ** -24
+    return (wide, wide) if dtype != torch.bfloat16 else (2.0 ** -8 + 2.0 ** -15 + wide, 2.0 ** -15 + wide)
+
+
+def close(got, want, bound, out_type):
+    bad = (got.double() - want).abs() > bound + STEP[out_type] * want.abs() + 1e-30 + (
+        2.0 ** -25 if out_type == torch.float16 else 0)                   # half a step of the least numbers
+    assert not bad.any(), (got.double() - want)[bad].abs().max()
+    assert torch.isfinite(got).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("given", ["nothing", "starts", "state", "both"])
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_forward(size, type, given):
+    from puffysics_amd import policy
+    dtype, scale = TYPES[type], size[3] ** -0.5
+    q, k, v, decay, starts, state = made(*size, dtype, sum(size))
+    starts = starts if given in ("starts", "both") else None
+    state = state if given in ("state", "both") else None
+    got = policy.linear_attention(q, k, v, decay, state=state, starts=starts, scale=scale, last=True)
+    want, states = attention_oracle(q, k, v, decay, state, starts, scale)
+    most, most_states = bounds(q, k, v, decay, state, starts, scale)
+    a, b = allowed(dtype, size[3], size[0])
+    close(got.out, want, a * most, dtype)
+    close(got.state, states[-1], b * most_states[-1], torch.float32)
+    only = policy.linear_attention(q, k, v, decay, state=state, starts=starts, scale=scale)
+    assert only.state is None and torch.equal(only.out, got.out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("given", ["nothing", "both"])
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_gradient(size, type, given):
+    from puffysics_amd import policy
+    dtype, scale = TYPES[type], size[3] ** -0.5
+    q, k, v, decay, starts, state = made(*size, dtype, sum(size) + 1)
+    g = torch.Generator().manual_seed(5)
+    d_out = torch.randn(v.shape, generator=g).to(dtype).cuda()
+    d_last = torch.randn(state.shape, generator=g).cuda()
+    if given == "nothing":
+        starts = state = d_last = None
+    leaves = [x.requires_grad_() for x in (q, k, v, state) if x is not None]
+    got = policy.linear_attention(q, k, v, decay, state=state, starts=starts, scale=scale, last=d_last is not None)
+    outs, ups = ((got.out, got.state), (d_out, d_last)) if d_last is not None else ((got.out,), (d_out,))
+    grads = torch.autograd.grad(outs, leaves, ups)
+    with torch.no_grad():
+        want = attention_gradient_oracle(q, k, v, decay, state, starts, scale, d_out, d_last)
+        most = attention_gradient_oracle(q.abs(), k.abs(), v.abs(), decay.sqrt(), None if state is None else state.abs(),
+                                         starts, scale, d_out.abs(), None if d_last is None else d_last.abs())
+    a, b = allowed(dtype, max(size[3:]), size[0])
+    for x, y, m in zip(grads[:3], want, most):
+        close(x, y, a * m, dtype)
+    if state is not None:
+        close(grads[3], want[3], b * most[3], torch.float32)
+    # one at a time: the same
+    for i, leaf in enumerate(leaves):
+        alone = policy.linear_attention(*(x.detach() if x is not leaf else x for x in (q, k, v)), decay,
+                                        state=state if state is None or state is leaf else state.detach(), starts=starts,
+                                        scale=scale, last=d_last is not None)
+        assert torch.equal(torch.autograd.grad((alone.out, alone.state)[:len(ups)], leaf, ups)[0], grads[i])
+
+
+@pytest.mark.gpu
+def test_gradient_by_differences():
+    from puffysics_amd import policy
+    q, k, v, decay, starts, state = made(9, 2, 2, 4, 3, torch.float32, 3)
+    g = torch.Generator().manual_seed(1)
+    d_out, d_last = torch.randn(v.shape, generator=g).cuda(), torch.randn(state.shape, generator=g).cuda()
+    leaves = [x.requires_grad_() for x in (q, k, v, state)]
+    got = policy.linear_attention(q, k, v, decay, state=state, starts=starts, last=True)
+    grads = torch.autograd.grad((got.out, got.state), leaves, (d_out, d_last))
+
+    def loss(*xs):
+        out, states = attention_oracle(*xs[:3], decay, xs[3], starts)
+        return (out * d_out.double()).sum() + (states[-1] * d_last.double()).sum()
+
+    base = [x.detach().double() for x in leaves]
+    for i, (x, grad) in enumerate(zip(base, grads)):
+        for at in range(0, x.numel(), max(1, x.numel() // 7)):
+            up, down = x.clone(), x.clone()
+            up.view(-1)[at] += 1e-4
+            down.view(-1)[at] -= 1e-4
+            # the loss is of the second degree in each: the difference is exact but for 64 bits' rounding
+            d = (loss(*base[:i], up, *base[i + 1:]) - loss(*base[:i], down, *base[i + 1:])) / 2e-4
+            assert abs(float(d) - float(grad.view(-1)[at])) < 1e-4 * (1 + abs(float(d)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("size", [(1, 1, 1, 1), (3, 2, 8, 5), (5, 3, 33, 17), (2, 2, 128, 128), (70, 4, 64, 64), (9, 1, 100, 30)])
+def test_step(size, type):
+    """Step after step it is the rollout's; the state is updated in place."""
+    from puffysics_amd import policy
+    dtype, steps = TYPES[type], 5
+    q, k, v, decay, starts, state = made(steps, *size, dtype, sum(size), rate=0.4)
+    want, states = attention_oracle(q, k, v, decay, state, starts, 0.5)
+    most, most_states = bounds(q, k, v, decay, state, starts, 0.5)
+    for t in range(steps):
+        version = state._version
+        out = policy.linear_attention_step(q[t], k[t], v[t], decay, state, starts=starts[t], scale=0.5)
+        assert state._version > version
+        wide = (size[2] + steps + 8) * 2.0 ** -24
+        close(out, want[t], wide * most[t], dtype)
+        close(state, states[t], wide * most_states[t], torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bool, torch.uint8])
+def test_types_of_starts(dtype):
+    from puffysics_amd import policy
+    q, k, v, decay, starts, state = made(70, 3, 2, 16, 16, torch.float32, 2)
+    want = policy.linear_attention(q, k, v, decay, state=state, starts=starts, last=True)
+    got = policy.linear_attention(q, k, v, decay, state=state, starts=starts.to(dtype), last=True)
+    turned = policy.linear_attention(q, k, v, decay, state=state, starts=starts.t().contiguous().t().to(dtype), last=True)
+    for x in (got, turned):
+        assert torch.equal(x.out, want.out) and torch.equal(x.state, want.state)
+    a, b = state.clone(), state.clone()
+    x = policy.linear_attention_step(q[0], k[0], v[0], decay, a, starts=starts[0])
+    y = policy.linear_attention_step(q[0], k[0], v[0], decay, b, starts=starts[0].to(dtype))
+    assert torch.equal(x, y) and torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", TYPES)
+def test_strides(type):
+    """Parts of a fused projection, environments first, broadcast heads, odd
+    addresses: as contiguous copies of them."""
+    from puffysics_amd import policy
+    dtype, g = TYPES[type], torch.Generator().manual_seed(8)
+    fused = torch.randn(3, 50, 2, 3 * 24 + 1, generator=g).to(dtype).cuda()      # environments, steps, heads
+    parts = [fused[..., 24 * i + 1:24 * i + 25].transpose(0, 1) for i in range(3)]
+    one = torch.randn(50, 3, 1, 24, generator=g).to(dtype).cuda().expand(50, 3, 2, 24)
+    apart = torch.randn(50, 3, 2, 48, generator=g).to(dtype).cuda()[..., ::2]
+    decay = torch.tensor([0.9, 0.97], device="cuda")
+    d_out = torch.randn(2, 50, 3, 24, generator=g).to(dtype).cuda().permute(1, 2, 0, 3)
+    for q, k, v in (parts, [parts[0], one, one], [apart, parts[1], apart]):
+        xs = [x.detach().requires_grad_() for x in (q, k, v)]
+        ys = [x.detach().contiguous().requires_grad_() for x in (q, k, v)]
+        a, b = policy.linear_attention(*xs, decay).out, policy.linear_attention(*ys, decay).out
+        assert a.is_contiguous() and torch.equal(a, b)
+        for x, y in zip(torch.autograd.grad(a, xs, d_out), torch.autograd.grad(b, ys, d_out.contiguous())):
+            assert torch.equal(x, y)
+        for u, w in zip(xs, ys):
+            u.requires_grad_(False), w.requires_grad_(False)
+        sa, sb = torch.ones(3, 2, 24, 24, device="cuda"), torch.ones(3, 2, 24, 24, device="cuda")
+        assert torch.equal(policy.linear_attention_step(*(x[7] for x in xs), decay, sa),
+                           policy.linear_attention_step(*(x[7] for x in ys), decay, sb)) and torch.equal(sa, sb)
+
+
+@pytest.mark.gpu
+def test_gradient_of_shared_heads():
+    """Keys that all heads share get the sum of the heads' gradients."""
+    from puffysics_amd import policy
+    q, k, v, decay, starts, _ = made(40, 2, 4, 16, 8, torch.float32, 4)
+    shared = k[:, :, :1].clone().requires_grad_()
+    each = shared.detach().expand(40, 2, 4, 16).contiguous().requires_grad_()
+    up = torch.randn_like(v)
+    a, = torch.autograd.grad(policy.linear_attention(q, shared.expand(40, 2, 4, 16), v, decay, starts=starts).out, shared, up)
+    b, = torch.autograd.grad(policy.linear_attention(q, each, v, decay, starts=starts).out, each, up)
+    assert torch.allclose(a, b.sum(2, keepdim=True), rtol=1e-6, atol=1e-6)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("key,value,steps", [(16, 16, 40), (64, 64, 100), (128, 40, 70)])
+def test_what_an_episode_may_not_see(key, value, steps, type, bad):
+    """NaN and infinities at a step are seen in the rest of its episode alone;
+    back in time, in what came before it of the episode."""
+    from puffysics_amd import policy
+    q, k, v, decay, _, state = made(steps, 1, 1, key, value, TYPES[type], 6)
+    decay = torch.tensor([0.9], device="cuda")
+    starts = torch.zeros(steps, 1, device="cuda")
+    first, at, after = steps // 3, steps // 2, steps // 2 + 3
+    starts[first] = starts[after] = 1
+    d_out = torch.randn_like(v)
+    want_leaves = [x.detach().clone().requires_grad_() for x in (q, k, v)]
+    want = policy.linear_attention(*want_leaves, decay, state=state, starts=starts, last=True)
+    want_grads = torch.autograd.grad(want.out, want_leaves, d_out)
+    for i in range(3):
+        leaves = [x.detach().clone() for x in (q, k, v)]
+        leaves[i][at] = bad
+        leaves = [x.requires_grad_() for x in leaves]
+        got = policy.linear_attention(*leaves, decay, state=state, starts=starts, last=True)
+        out = got.out.detach()
+        rest = torch.tensor([t < at or t >= after for t in range(steps)])
+        assert torch.isfinite(out[rest]).all() and torch.isfinite(got.state).all()
+        close(out[rest], want.out[rest].double(), 2.0 ** -7 * want.out.abs().max(), TYPES[type])
+        assert not torch.isfinite(out[at]).all()
+        episode = torch.tensor([t < first or t >= after for t in range(steps)])
+        for x, y in zip(torch.autograd.grad(got.out, leaves, d_out), want_grads):
+            assert torch.isfinite(x[episode]).all()
+            close(x[episode], y[episode].double(), 2.0 ** -7 * y.abs().max(), TYPES[type])
+    # of the upstream gradient
+    d_bad = d_out.clone()
+    d_bad[at] = bad
+    for x in torch.autograd.grad(policy.linear_attention(*want_leaves, decay, state=state, starts=starts).out, want_leaves, d_bad):
+        assert torch.isfinite(x[episode]).all() and not torch.isfinite(x[at]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+def test_ends_of_the_decay(type):
+    """0: each step alone.  1: plain sums.  Outside: NaN."""
+    from puffysics_amd import policy
+    q, k, v, _, _, state = made(100, 1, 4, 32, 32, TYPES[type], 7)
+    decay = torch.tensor([0.0, 1.0, 1.5, -0.1], device="cuda")
+    got = policy.linear_attention(q, k, v, decay, state=state, last=True)
+    want, states = attention_oracle(q, k, v, decay, state)
+    most, most_states = bounds(q[:, :, :2], k[:, :, :2], v[:, :, :2], decay[:2], state[:, :2], None, 1.0)
+    a, b = allowed(TYPES[type], 32, 100)
+    close(got.out[:, :, :2], want[:, :, :2], a * most, TYPES[type])
+    close(got.state[:, :2], states[-1][:, :2], b * most_states[-1], torch.float32)
+    assert got.out[1:, :, 2:].isnan().all() and got.state[:, 2:].isnan().all()
+    s = state.clone()
+    assert policy.linear_attention_step(q[0], k[0], v[0], decay, s)[:, 2:].isnan().all() and s[:, 2:].isnan().all()
+    assert torch.allclose(s[:, 0], k[0, :, 0, :, None].float() * v[0, :, 0, None].float())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(0, 3, 2), (5, 0, 2), (5, 3, 0)])
+def test_nothing_to_do(shape):
+    from puffysics_amd import policy
+    steps, envs, heads = shape
+    q, k, v, decay, starts, state = made(steps, envs, heads, 16, 8, torch.float32, 1)
+    for x in (q, k, v, state):
+        x.requires_grad_()
+    got = policy.linear_attention(q, k, v, decay, state=state, starts=starts, last=True)
+    assert got.out.shape == v.shape and torch.equal(got.state, state)
+    d = torch.ones_like(got.state)
+    grads = torch.autograd.grad((got.out, got.state), (q, k, v, state), (torch.ones_like(v), d))
+    assert [g.shape for g in grads] == [x.shape for x in (q, k, v, state)] and torch.equal(grads[3], d)
+    empty = policy.linear_attention(q, k, v, decay, last=True).state
+    assert int(torch.count_nonzero(empty)) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("size", [(4000, 1, 2, 64, 64), (2500, 2, 1, 128, 96), (1500, 3, 1, 20, 33)])
+def test_long(size, type):
+    """Few sequences of many steps, which are cut into parts; starts far apart,
+    so that memories cross the cuts."""
+    from puffysics_amd import policy
+    dtype, scale = TYPES[type], 0.2
+    q, k, v, _, starts, state = made(*size, dtype, 9, rate=0.002)
+    decay = 1 - 0.5 ** torch.linspace(3, 11, size[2], device="cuda")
+    g = torch.Generator().manual_seed(2)
+    d_out = torch.randn(v.shape, generator=g).to(dtype).cuda()
+    d_last = torch.randn(state.shape, generator=g).cuda()
+    leaves = [x.requires_grad_() for x in (q, k, v, state)]
+    got = policy.linear_attention(q, k, v, decay, state=state, starts=starts, scale=scale, last=True)
+    grads = torch.autograd.grad((got.out, got.state), leaves, (d_out, d_last))
+    with torch.no_grad():
+        want, states = attention_oracle(q, k, v, decay, state, starts, scale)
+        most, most_states = bounds(q, k, v, decay, state, starts, scale)
+        want_d = attention_gradient_oracle(q, k, v, decay, state, starts, scale, d_out, d_last)
+        most_d = attention_gradient_oracle(q.abs(), k.abs(), v.abs(), decay.sqrt(), state.abs(), starts, scale, d_out.abs(),
+                                           d_last.abs())
+        a, b = allowed(dtype, max(size[3:]), size[0])
+        close(got.out, want, a * most, dtype)
+        close(got.state, states[-1], b * most_states[-1], torch.float32)
+        for x, y, m in zip(grads[:3], want_d, most_d):
+            close(x, y, a * m, dtype)
+        close(grads[3], want_d[3], b * most_d[3], torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+def test_a_rollout_in_two_halves(type):
+    """The state that a first half leaves is what the second goes on from, and
+    its gradient goes back through it; a state may be written over the one it
+    came from."""
+    from puffysics_amd import policy
+    dtype = TYPES[type]
+    q, k, v, decay, starts, state = made(90, 4, 2, 32, 32, dtype, 12)
+    whole = policy.linear_attention(q, k, v, decay, state=state, starts=starts, last=True)
+    first = policy.linear_attention(q[:41], k[:41], v[:41], decay, state=state, starts=starts[:41], last=True)
+    second = policy.linear_attention(q[41:], k[41:], v[41:], decay, state=first.state, starts=starts[41:], last=True)
+    most, most_states = bounds(q, k, v, decay, state, starts, 1.0)
+    a, b = allowed(dtype, 32, 90)
+    close(torch.cat([first.out, second.out]), whole.out.double(), 2 * a * most, dtype)
+    close(second.state, whole.state.double(), 2 * b * most_states[-1], torch.float32)
+    d_out = torch.randn_like(v)
+    xs, ys = ([x.detach().clone().requires_grad_() for x in (q, k, v, state)] for _ in range(2))
+    one = torch.autograd.grad(policy.linear_attention(*xs[:3], decay, state=xs[3], starts=starts).out, xs, d_out)
+    h = policy.linear_attention(*(y[:41] for y in ys[:3]), decay, state=ys[3], starts=starts[:41], last=True)
+    out = policy.linear_attention(*(y[41:] for y in ys[:3]), decay, state=h.state, starts=starts[41:]).out
+    two = torch.autograd.grad((h.out, out), ys, (d_out[:41], d_out[41:]))
+    with torch.no_grad():
+        most = attention_gradient_oracle(q.abs(), k.abs(), v.abs(), decay.sqrt(), state.abs(), starts, 1.0, d_out.abs())
+    for x, y, m, t in zip(one, two, most, (dtype, dtype, dtype, torch.float32)):
+        close(x, y.double(), 2 * a * m, t)
+
+
+@pytest.mark.gpu
+def test_streams_and_replays():
+    """On another stream than its tensors', and captured: every replay is the
+    eager result of what the buffers hold then, with other work between."""
+    from puffysics_amd import policy
+    q, k, v, decay, starts, state = made(70, 8, 2, 32, 32, torch.bfloat16, 14)
+    long = [torch.randn(3000, 1, 1, 64, device="cuda") for _ in range(3)]
+    one = torch.tensor([0.99], device="cuda")
+    side = torch.cuda.Stream()
+    want = policy.linear_attention(q, k, v, decay, state=state, starts=starts, last=True)
+    want_long = policy.linear_attention(*long, one, last=True)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        got = policy.linear_attention(q, k, v, decay, state=state, starts=starts, last=True)
+    side.synchronize()
+    assert torch.equal(got.out, want.out) and torch.equal(got.state, want.state)
+    memory = state.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a = policy.linear_attention(q, k, v, decay, state=memory, starts=starts, last=True)
+        b = policy.linear_attention(*long, one, last=True)
+        c = policy.linear_attention_step(q[0], k[0], v[0], decay, memory, starts=starts[0])
+    twin = state.clone()
+    for i in range(3):
+        v.add_(0.25)
+        long[1].mul_(0.5)
+        graph.replay()
+        eager = policy.linear_attention(q, k, v, decay, state=twin, starts=starts, last=True)
+        eager_long = policy.linear_attention(*long, one, last=True)
+        step = policy.linear_attention_step(q[0], k[0], v[0], decay, twin, starts=starts[0])
+        torch.cuda.synchronize()
+        assert torch.equal(a.out, eager.out) and torch.equal(a.state, eager.state)
+        assert torch.equal(b.out, eager_long.out) and torch.equal(b.state, eager_long.state)
+        assert torch.equal(c, step) and torch.equal(memory, twin)
+        torch.cuda.synchronize()
+    assert torch.equal(want_long.out[:1], policy.linear_attention(*(x[:1] for x in long), one).out) or i == 2
+
+
+@pytest.mark.gpu
+def test_gradients_add_up_and_are_differentiable_once():
+    from puffysics_amd import policy
+    q, k, v, decay, starts, _ = made(20, 2, 2, 8, 8, torch.float32, 15)
+    x = q.requires_grad_()
+    out = policy.linear_attention(x, k, v, decay, starts=starts).out
+    g, = torch.autograd.grad(out.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), x)
+    # q, k and v the same leaf
+    leaf = torch.randn(20, 2, 2, 8, device="cuda", requires_grad=True)
+    parts = [leaf.detach().clone().requires_grad_() for _ in range(3)]
+    up = torch.randn(20, 2, 2, 8, device="cuda")
+    total, = torch.autograd.grad(policy.linear_attention(leaf, leaf, leaf, decay).out, leaf, up)
+    each = torch.autograd.grad(policy.linear_attention(*parts, decay).out, parts, up)
+    assert torch.allclose(total, sum(each), rtol=1e-5, atol=1e-5)
+
+
+def test_refusals():
+    """Nothing is launched: this runs without a GPU."""
+    from puffysics_amd import policy
+    z = lambda *s, **kw: torch.zeros(*s, **kw)  # noqa: E731
+    q, v, d, s = z(5, 3, 2, 8), z(5, 3, 2, 4), z(2), z(3, 2, 8, 4)
+    ok = dict(q=q, k=q, v=v, decay=d)
+    for what, change in (
+            ("of one type", dict(k=q.half())), ("float32, float16", dict(q=q.double(), k=q.double(), v=v.double())),
+            ("one shape", dict(k=z(5, 3, 2, 9))), ("one shape", dict(v=z(5, 3, 1, 4))), ("steps, envs", dict(q=q[0])),
+            ("1 to 128", dict(q=z(5, 3, 2, 129), k=z(5, 3, 2, 129))), ("1 to 128", dict(v=z(5, 3, 2, 0))),
+            ("1 to 128", dict(v=z(5, 3, 2, 129))), ("decay", dict(decay=z(3))), ("decay", dict(decay=d.double())),
+            ("no gradient", dict(decay=z(2, requires_grad=True))), ("state", dict(state=s.half())),
+            ("state", dict(state=s[:2])), ("starts", dict(starts=z(5, 2))), ("starts", dict(starts=z(5, 3).double())),
+            ("finite", dict(scale=float("nan"))), ("finite", dict(scale=float("inf"))),
+            ("2\\^24", dict(q=z(1).expand(1, 2 ** 23, 2, 8), k=z(1).expand(1, 2 ** 23, 2, 8), v=z(1).expand(1, 2 ** 23, 2, 4))),
+            ("2\\^31", dict(q=z(1).expand(2 ** 31, 1, 2, 8), k=z(1).expand(2 ** 31, 1, 2, 8), v=z(1).expand(2 ** 31, 1, 2, 4))),
+            ("CUDA device", {})):
+        with pytest.raises(ValueError, match=what):
+            policy.linear_attention(**{**ok, **change})
+    step = dict(q=q[0], k=q[0], v=v[0], decay=d, state=s)
+    for what, change in (
+            ("q has to be", dict(q=q)), ("state", dict(state=s.half())), ("state", dict(state=z(3, 2, 4, 8).transpose(2, 3))),
+            ("starts", dict(starts=z(2))), ("no gradient", dict(state=s.clone().requires_grad_())),
+            ("no gradient", dict(q=q[0].clone().requires_grad_())), ("CUDA device", {})):
+        with pytest.raises(ValueError, match=what):
+            policy.linear_attention_step(**{**step, **change})
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        for name in ("q", "k", "v"):
+            with pytest.raises(ValueError, match="forward-mode"):
+                policy.linear_attention(**{**ok, name: forward_ad.make_dual(ok[name], torch.ones_like(ok[name]))})
+
+
+def test_c_refusals():
+    """Of the C entries; no call reaches a launch."""
+    import ctypes as C
+    from puffysics_amd import policy
+    lib = policy.policy_lib()
+    one = (C.c_char * 64)()
+    at = C.addressof(one)
+
+    def call(**change):
+        g = policy.B3Attention(1, 1, 1, 8, 8, 0, at, at, at, (8, 8, 8), (8, 8, 8), (8, 8, 8), at, None, 0, (0, 0), None, 1.0)
+        for name, value in change.items():
+            setattr(g, name, value)
+        return lib.b3_linear_attention_gpu(C.byref(g), None if change.get("steps") != 0 else None, None, None, 0, None)
+
+    for change in (dict(key=0), dict(key=129), dict(value=0), dict(value=129), dict(type=3), dict(steps=-1), dict(envs=-1),
+                   dict(heads=-1), dict(q=None), dict(decay=None), dict(envs=1 << 24), dict(steps=1 << 31), dict(),
+                   dict(starts=at, starts_type=2), dict(scale=float("nan"))):
+        assert call(**change) == 1, change
+    assert call(envs=0) == 0 and call(heads=0) == 0 and call(steps=0) == 0
+    assert lib.b3_linear_attention_gpu(None, None, None, None, 0, None) == 1
