@@ -275,8 +275,8 @@ hipError_t b3_values_of_8bit_gpu(int64_t rows, int64_t width, const unsigned cha
     void* out, int type, hipStream_t stream);
 
 /* Gradients: d_x (also the residual's) and d_weight, of weight_type (NULL: not
- * wanted), from those of out and sum (NULL: zero).  norm->x is h, as the sum
- * or as x where there is no residual; norm->residual is not read. */
+ * wanted), from those of out and sum (NULL: zero).  `norm` is the forward
+ * pass's; where the sum is in 32 bits, x may be it, without a residual. */
 size_t b3_rms_norm_backward_workspace(int64_t rows, int64_t width);
 hipError_t b3_rms_norm_backward_gpu(const B3Norm* norm, const float* root, const void* d_out, int64_t d_out_stride,
     const void* d_sum, int64_t d_sum_stride, void* d_x, void* d_weight, void* workspace, size_t workspace_bytes,

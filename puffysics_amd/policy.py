@@ -550,7 +550,9 @@ class _RmsNorm(torch.autograd.Function):
         shape = x.shape
         x, residual = _as_rows(x), _as_rows(residual)
         out, total, root = _normalise(x, weight, residual, eps, True)
-        ctx.save_for_backward(x if residual is None else total, weight, root)
+        # in 32 bits the sum is what was normalised; in 16 it has been rounded
+        x, residual = (total, None) if residual is not None and x.dtype == torch.float32 else (x, residual)
+        ctx.save_for_backward(x, residual, weight, root)
         ctx.set_materialize_grads(False)
         return out.view(shape), None if total is None else total.view(shape)
 
@@ -560,17 +562,17 @@ class _RmsNorm(torch.autograd.Function):
 
 
 def _norm_backward(ctx, d_out, d_sum):
-    h, weight, root = ctx.saved_tensors
-    rows, width = h.shape
+    x, residual, weight, root = ctx.saved_tensors
+    rows, width = x.shape
     lib = policy_lib()
     shape = (d_sum if d_out is None else d_out).shape
     d_out, d_sum = _as_rows(d_out), _as_rows(d_sum)
     stride = lambda y: 0 if y is None else y.stride(0) if rows > 1 else width  # noqa: E731
-    d_x = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    d_x = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     d_weight = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
     size = lib.b3_rms_norm_backward_workspace(rows, width)
-    work = _work(size, h.device)
-    g = _norm(h, None, weight, 0.0)
+    work = _work(size, x.device)
+    g = _norm(x, residual, weight, 0.0)
     _check("b3_rms_norm_backward_gpu", lib.b3_rms_norm_backward_gpu(
         C.byref(g), root.data_ptr(), _address_of(d_out), stride(d_out), _address_of(d_sum), stride(d_sum), d_x.data_ptr(),
         _address_of(d_weight), _address_of(work), size, _stream()))

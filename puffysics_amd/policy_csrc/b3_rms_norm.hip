@@ -261,7 +261,7 @@ __global__ __launch_bounds__(kThreads) void rn_backward(Job j) {
 #pragma unroll
         for (int v = 0; v < NV; v++) {
             const int64_t c = (v * G + lane) * kVec;
-            load8((const T*)j.g.x + r * j.g.x_stride + c, j.g.width - c, u[v]);
+            load_h<T>(j.g, r, c, u[v]);
             load_d_out<T>(j, r, c, g[v]);
         }
 #pragma unroll
@@ -308,7 +308,7 @@ __global__ __launch_bounds__(kThreads) void rn_dot(Job j) {
         float dot = 0;
         for (int64_t c = threadIdx.x * kVec; c < j.g.width; c += kThreads * kVec) {
             float h[kVec], d[kVec], w[kVec], part = 0;
-            load8((const T*)j.g.x + r * j.g.x_stride + c, j.g.width - c, h);
+            load_h<T>(j.g, r, c, h);
             load_d_out<T>(j, r, c, d);
             load_weight<T>(j.g, c, w);
 #pragma unroll
@@ -330,7 +330,7 @@ __global__ __launch_bounds__(kThreads) void rn_backward_long(Job j) {
     for (int64_t r = blockIdx.y; r < j.g.rows; r += gridDim.y) {
         float u[kVec], g[kVec];
         const float s = j.root[r];
-        load8((const T*)j.g.x + r * j.g.x_stride + c, j.g.width - c, u);
+        load_h<T>(j.g, r, c, u);
         load_d_out<T>(j, r, c, g);
 #pragma unroll
         for (int k = 0; k < kVec; k++) {
