@@ -10,7 +10,12 @@
  * episode starts there) the gradients are dq_t = scale do_t S_t^T,
  * dk_t = v_t G_t^T and dv_t = k_t G_t: each a sum of the same form over the
  * earlier or the later steps, with the arrays in other places.  One kernel
- * does all four.
+ * does all four: a wave takes a sequence (an environment's head) and a part of
+ * v's columns, holds the state in the accumulators of the matrix units, and
+ * goes over chunks of 32 steps (16 in 32 bits), within which the steps are
+ * products of matrices.  No wave waits for another.  Where sequences are few
+ * their steps are cut into pieces: a first launch finds what state each leaves,
+ * a second adds up, and the third goes over all pieces at once.
  */
 #include "policy_common.h"
 
@@ -18,34 +23,41 @@ namespace b3p {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kRoles = 3;                        // of a launch
+constexpr int64_t kWaves = 2048;                 // that a launch of few sequences is cut into
+constexpr int64_t kPieceChunks = 8;              // of a piece at the least
 
 /* out_p = `reach` q_p (decay^p E + sums over p' <= p of the episode of
  * `update` decay^(p - p') k_p'^T v_p'), and the state that is left,
  * decay^steps E + sums of `update` decay^(steps - p') k_p'^T v_p'.  Places p
- * follow the steps, or go from the last one back. */
+ * follow the steps, or go from the last one back.  Forwards E is a step
+ * earlier (decayed before place 0), and the state is left a step earlier (not
+ * decayed after the last place). */
 struct Mix {
     const void *q, *k, *v;
     void* out;
     int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];   // place, environment, head
     int key, value;
     float reach, update;
-    const char* starts;                          // of place 0 (which has none where `back`), or NULL
+    bool forward;
+    const char* starts;                          // of place 0 (which has none on the way back), or NULL
     int64_t starts_stride[2];                    // in bytes
     const float* enter;                          // E, NULL: zeros
     float* leave;                                // NULL: not wanted
-    int64_t state_row, state_col;                // of both, in elements
-    bool enter_early;                            // E is a step earlier: decayed before place 0
-    bool leave_early;                            // the state is left a step earlier: not decayed after the last place
+    int64_t state_row, state_col;                // of both and of the pieces', in elements
     const char* leave_starts;                    // [environments], dropped where nonzero; or NULL
     int64_t leave_starts_stride;
+    float* pieces;                               // [pieces - 1][sequences][key value]: what each leaves
+    float* carry;                                // [pieces - 1][sequences]: decay over it, < 0 where it drops what enters
 };
 
-constexpr int kRoles = 3;
 struct Job {
     Mix mix[kRoles];
     int64_t steps, envs, heads;
     const float* decay;
     int starts_type;
+    int roles, parts;                            // parts: of v's columns
+    int64_t places, pieces;                      // places: of a piece
 };
 
 __device__ __forceinline__ bool started(const char* p, int type) {
@@ -58,53 +70,501 @@ __device__ __forceinline__ float decay_of(const float* decay, int64_t head) {
     return d >= 0.0f && d <= 1.0f ? d : NAN;
 }
 
-/* A workgroup to a sequence, place after place: thread t holds column t % 128
- * of one half of the state's rows. */
+/* ---- a wave's work on a sequence ---- */
+
+typedef float F4 __attribute__((ext_vector_type(4)));
+typedef short S4 __attribute__((ext_vector_type(4)));
+typedef short S8 __attribute__((ext_vector_type(8)));
+typedef __bf16 B4 __attribute__((ext_vector_type(4)));
+typedef __bf16 B8 __attribute__((ext_vector_type(8)));
+typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+
+/* What the arithmetic goes by.  Lane (g, c) = (lane / 16, lane % 16) holds of
+ * 16 x 16 operands the four elements 4 g .. 4 g + 3 along the axis that is
+ * summed, of row or column c: a quad.  A product's tile lies the same way, so
+ * that it is an operand of the next without a move between lanes. */
 template <typename T>
-__global__ __launch_bounds__(kThreads) void la_places(Job j) {
-    constexpr int kRows = B3_MAX_HEAD / 2;
-    __shared__ float q[B3_MAX_HEAD], k[B3_MAX_HEAD], v[B3_MAX_HEAD], half[B3_MAX_HEAD];
+struct Math {                                    // 32-bit products: of float, and of halves, whose scores could overflow
+    typedef float Lds;
+    typedef F4 Quad;
+    static constexpr int kPlaces = 16;           // of a chunk
+};
+template <>
+struct Math<__bf16> {
+    typedef __bf16 Lds;
+    typedef S4 Quad;
+    static constexpr int kPlaces = 32;
+};
+
+__device__ __forceinline__ S4 round4(F4 x) { return __builtin_bit_cast(S4, __builtin_convertvector(x, B4)); }
+/* What rounding left out, rounded. */
+__device__ __forceinline__ S4 rest4(F4 x, S4 rounded) {
+    return round4(x - __builtin_convertvector(__builtin_bit_cast(B4, rounded), F4));
+}
+
+/* d += a b over two blocks of 16. */
+__device__ __forceinline__ F4 multiply(S4 a0, S4 a1, S4 b0, S4 b1, F4 d) {
+    const S8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+    const S8 b = __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(B8, a), __builtin_bit_cast(B8, b), d, 0, 0, 0);
+}
+
+/* Over one block. */
+__device__ __forceinline__ F4 multiply(F4 a, F4 b, F4 d) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) d = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], d, 0, 0, 0);
+    return d;
+}
+
+/* Keeps a wave's writes to LDS before the reads of its other lanes; the
+ * hardware does them in order. */
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+/* decay^n, 1 for n = 0. */
+__device__ __forceinline__ float power(float log2_decay, int n) {
+    return n == 0 ? 1.0f : __builtin_amdgcn_exp2f((float)n * log2_decay);
+}
+
+/* An array's part of a chunk: COLS columns of kPlaces rows, in vectors of 16
+ * bytes, in registers until the chunk before is done and then in LDS, whose
+ * rows are 16 bytes longer so that 16 rows' neighbouring columns lie in other
+ * banks. */
+template <typename T, int COLS>
+struct Tile {
+    typedef typename Math<T>::Lds Lds;
+    static constexpr int kVec = 16 / sizeof(T), kRow = COLS + 16 / sizeof(Lds), kPlaces = Math<T>::kPlaces;
+    static constexpr int kPerRow = COLS / kVec, kAll = kPerRow * kPlaces, kLoads = (kAll + kWave - 1) / kWave;
+    static constexpr int kBytes = kPlaces * kRow * sizeof(Lds);
+    U4 raw[kLoads];
+
+    static __device__ __forceinline__ bool mine(int l) { return kAll % kWave == 0 || l * kWave + (int)threadIdx.x % kWave < kAll; }
+    static __device__ __forceinline__ int row(int l) { return (l * kWave + (int)threadIdx.x % kWave) / kPerRow; }
+    static __device__ __forceinline__ int col(int l) { return (l * kWave + (int)threadIdx.x % kWave) % kPerRow * kVec; }
+
+    /* Columns from p on, of which there are `cols`; zeros beyond and in rows from `places` on. */
+    __device__ __forceinline__ void load(const T* p, int64_t stride, int places, int cols) {
+#pragma unroll
+        for (int l = 0; l < kLoads; l++) {
+            raw[l] = U4{0, 0, 0, 0};
+            if (!mine(l) || row(l) >= places) continue;
+            const T* at = p + row(l) * stride + col(l);
+            const int left = cols - col(l);
+            if (left >= kVec) {
+                raw[l] = __builtin_bit_cast(U4, *(const Pack<T, kVec>*)at);
+            } else {
+                Pack<T, kVec> some = {};
+                for (int i = 0; i < kVec; i++)
+                    if (i < left) some.v[i] = at[i];
+                raw[l] = __builtin_bit_cast(U4, some);
+            }
+        }
+    }
+
+    /* Whether any element of the lane's is NaN or infinite. */
+    __device__ __forceinline__ bool bad() const {
+        typedef unsigned short H2 __attribute__((ext_vector_type(2)));
+        uint32_t most = 0;
+#pragma unroll
+        for (int l = 0; l < kLoads; l++)
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                if (sizeof(T) == 4) {
+                    const uint32_t x = raw[l][w] & 0x7fffffffu;
+                    most = x > most ? x : most;
+                } else {
+                    const H2 x = __builtin_bit_cast(H2, raw[l][w] & 0x7fff7fffu);
+                    most = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(x, __builtin_bit_cast(H2, most)));
+                }
+            }
+        if (sizeof(T) == 4) return most >= 0x7f800000u;
+        const uint32_t least = sizeof(Lds) == 2 ? 0x7f80u : 0x7c00u;
+        return (most & 0xffffu) >= least || most >> 16 >= least;
+    }
+
+    __device__ __forceinline__ void put(Lds* lds, int r, int c, U4 x) const {
+        if (sizeof(T) == sizeof(Lds)) {
+            *(U4*)(lds + r * kRow + c) = x;
+        } else {
+            const Pack<_Float16, 8> h = __builtin_bit_cast(Pack<_Float16, 8>, x);
+            F4 a, b;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                a[i] = (float)h.v[i];
+                b[i] = (float)h.v[i + 4];
+            }
+            *(F4*)(lds + r * kRow + c) = a;
+            *(F4*)(lds + r * kRow + c + 4) = b;
+        }
+    }
+
+    __device__ __forceinline__ void store(Lds* lds) const {
+#pragma unroll
+        for (int l = 0; l < kLoads; l++)
+            if (mine(l)) put(lds, row(l), col(l), raw[l]);
+    }
+};
+
+/* The quad of row c of 16 from `row` on, columns from `col` on. */
+template <int ROW>
+__device__ __forceinline__ S4 along(const __bf16* lds, int row, int col) {
+    const int lane = threadIdx.x % kWave;
+    return *(const S4*)(lds + (row + lane % 16) * ROW + col + lane / 16 * 4);
+}
+template <int ROW>
+__device__ __forceinline__ F4 along(const float* lds, int row, int col) {
+    const int lane = threadIdx.x % kWave;
+    return *(const F4*)(lds + (row + lane % 16) * ROW + col + lane / 16 * 4);
+}
+
+/* The quad of a column, rows from `row` on.  The column of c is first(c / 4) +
+ * c % 4 with first(n) = col + STEP n.  In 16 bits the hardware turns the four
+ * elements of 16 lanes: lane 4 a + b fetches those of row a, columns first(b)
+ * on, and lane c gets the column of c. */
+template <int ROW, int STEP>
+__device__ __forceinline__ S4 across(const __bf16* lds, int row, int col) {
+    const int lane = threadIdx.x % kWave, g = lane / 16, a = lane % 16 / 4, b = lane % 4;
+    const __bf16* p = lds + (row + 4 * g + a) * ROW + col + STEP * b;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) S4*)(p));
+}
+template <int ROW, int STEP>
+__device__ __forceinline__ F4 across(const float* lds, int row, int col) {
+    const int lane = threadIdx.x % kWave, g = lane / 16, c = lane % 16;
+    const float* p = lds + (row + 4 * g) * ROW + col + STEP * (c / 4) + c % 4;
+    return F4{p[0], p[ROW], p[2 * ROW], p[3 * ROW]};
+}
+
+/* Where a unit's work lies. */
+struct Unit {
+    int64_t env, head, piece;
+    int role, first;                             // first: column of v
+};
+
+/* One wave goes over the places of a piece of a sequence, a chunk at a time,
+ * KD the columns of q and k and VD those of its part of v, both filled up with
+ * zeros; STATE: without out, to learn what state the piece leaves.  With i and
+ * j places of the chunk, E the state that enters it and P the scores q_i k_j
+ * decay^(i - j) of an episode, j <= i:
+ *   out = P v + decay^i q E,  E' = decay^places E + (decay^(places - j) k)^T v */
+template <typename T, int KD, int VD, bool STATE>
+struct Walk {
+    typedef typename Math<T>::Lds Lds;
+    typedef typename Math<T>::Quad Quad;
+    static constexpr bool kHalf = sizeof(Lds) == 2;
+    static constexpr int kPlaces = Math<T>::kPlaces, R = kPlaces / 16, KB = KD / 16, VB = VD / 16;
+    typedef Tile<T, KD> KeyTile;
+    typedef Tile<T, VD> ValueTile;
+    static constexpr int kKeyRow = KeyTile::kRow, kValueRow = ValueTile::kRow;
+    static constexpr int kBytes = (STATE ? 1 : 2) * KeyTile::kBytes + ValueTile::kBytes;
+    /* in 16 bits two tiles' columns are dealt out so that a lane has eight neighbours of them */
+    static constexpr int kStep = kHalf ? 8 : 4;
+    static __device__ __forceinline__ int value_col(int vb) { return kHalf ? vb / 2 * 32 + vb % 2 * 4 : vb * 16; }
+
+    static __device__ __forceinline__ Quad with(F4 x) {
+        if constexpr (kHalf) return round4(x);
+        else return x;
+    }
+
+    static __device__ __forceinline__ void run(const Job& j, const Mix& m, const Unit& u, int64_t from, int64_t places, const float* enter,
+        bool early, float* leave, float* carry, char* shared) {
+        const int lane = threadIdx.x % kWave, g = lane / 16, c = lane % 16;
+        Lds* lk = (Lds*)shared;
+        Lds* lv = (Lds*)(shared + KeyTile::kBytes);
+        Lds* lq = (Lds*)(shared + KeyTile::kBytes + ValueTile::kBytes);
+        const float l2 = log2f(decay_of(j.decay, u.head));
+        const T* q = (const T*)m.q + from * m.q_stride[0] + u.env * m.q_stride[1] + u.head * m.q_stride[2];
+        const T* k = (const T*)m.k + from * m.k_stride[0] + u.env * m.k_stride[1] + u.head * m.k_stride[2];
+        const T* v = (const T*)m.v + from * m.v_stride[0] + u.env * m.v_stride[1] + u.head * m.v_stride[2] + u.first;
+        T* out = (T*)m.out + from * m.out_stride[0] + u.env * m.out_stride[1] + u.head * m.out_stride[2] + u.first;
+        const int value = m.value - u.first < VD ? m.value - u.first : VD;
+
+        /* E, lane (g, c) of tile [kb][vb] rows 16 kb + 4 g + r and the column of c */
+        F4 state[KB][VB];
+        const float first = early ? power(l2, 1) : 1.0f;
+#pragma unroll
+        for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+            for (int vb = 0; vb < VB; vb++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int row = kb * 16 + 4 * g + r, col = value_col(vb) + kStep * (c / 4) + c % 4;
+                    const bool in = enter && row < m.key && col < value;
+                    state[kb][vb][r] = in ? first * enter[row * m.state_row + (u.first + col) * m.state_col] : 0.0f;
+                }
+
+        /* weights of scores (of the tiles i = j and i = j + 16), of the state for place i, and of places for the state */
+        const float gain = m.reach * m.update;
+        F4 near[R];
+        float reach[R];
+#pragma unroll
+        for (int t = 0; t < R; t++) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int n = 16 * t + c - 4 * g - r;
+                near[t][r] = n >= 0 ? gain * power(l2, n) : 0.0f;
+            }
+            reach[t] = m.reach * power(l2, 16 * t + c);
+        }
+        F4 keep[R];
+        float pass = 0;
+        int weighted = -1;                       // places and the step less that keep and pass are for
+
+        KeyTile tq, tk;
+        ValueTile tv;
+        uint32_t flag = 0;
+        bool dropped = false;
+        auto fetch = [&](int64_t p, int most) {
+            const int n = places - p < most ? (int)(places - p) : most;
+            tk.load(k + p * m.k_stride[0], m.k_stride[0], n, m.key);
+            tv.load(v + p * m.v_stride[0], m.v_stride[0], n, value);
+            if (!STATE) tq.load(q + p * m.q_stride[0], m.q_stride[0], n, m.key);
+            flag = 0;
+            if (m.starts && lane < n && (from + p + lane || m.forward))
+                flag = started(m.starts + (from + p + lane) * m.starts_stride[0] + u.env * m.starts_stride[1], j.starts_type);
+        };
+        if (places > 0) fetch(0, kPlaces);
+        int n;
+#pragma unroll 1
+        for (int64_t p = 0; p < places; p += n) {
+            n = places - p < kPlaces ? (int)(places - p) : kPlaces;
+            /* A product with a weight of 0 would carry what is not finite in v to other places: such
+             * a place is a chunk by itself. */
+            if (__ballot(tv.bad()) && n > 1) {
+                n = 1;
+                fetch(p, 1);
+            }
+            const uint32_t starts = (uint32_t)__ballot(flag != 0);
+            wave_fence();
+            tk.store(lk);
+            tv.store(lv);
+            if (!STATE) tq.store(lq);
+            wave_fence();
+            const bool end = p + n >= places;
+            if (!end) fetch(p + n, kPlaces);
+            const int less = end && m.forward && from + places == j.steps ? 1 : 0;
+            if (weighted != 2 * n + less) {
+                weighted = 2 * n + less;
+#pragma unroll
+                for (int t = 0; t < R; t++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int at = 16 * t + 4 * g + r;
+                        keep[t][r] = at < n ? m.update * power(l2, n - at - less) : 0.0f;
+                    }
+                pass = power(l2, n - less);
+            }
+            Quad vq[R][VB];
+#pragma unroll
+            for (int t = 0; t < R; t++)
+#pragma unroll
+                for (int vb = 0; vb < VB; vb++) vq[t][vb] = across<kValueRow, kStep>(lv, 16 * t, value_col(vb));
+
+            if (!STATE) {
+                F4 o[R][VB];
+                Quad qq[R][KB];
+#pragma unroll
+                for (int t = 0; t < R; t++)
+#pragma unroll
+                    for (int kb = 0; kb < KB; kb++) qq[t][kb] = along<kKeyRow>(lq, 16 * t, 16 * kb);
+#pragma unroll
+                for (int t = 0; t < R; t++)
+#pragma unroll
+                    for (int vb = 0; vb < VB; vb++) o[t][vb] = F4{0, 0, 0, 0};
+                /* q E: in 16 bits E as two numbers */
+#pragma unroll
+                for (int vb = 0; vb < VB; vb++) {
+                    if constexpr (kHalf) {
+#pragma unroll
+                        for (int kb = 0; kb < KB; kb += 2) {
+                            const S4 h0 = round4(state[kb][vb]), h1 = round4(state[kb + 1][vb]);
+                            const S4 l0 = rest4(state[kb][vb], h0), l1 = rest4(state[kb + 1][vb], h1);
+#pragma unroll
+                            for (int t = 0; t < R; t++) {
+                                o[t][vb] = multiply(h0, h1, qq[t][kb], qq[t][kb + 1], o[t][vb]);
+                                o[t][vb] = multiply(l0, l1, qq[t][kb], qq[t][kb + 1], o[t][vb]);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                            for (int t = 0; t < R; t++) o[t][vb] = multiply(state[kb][vb], qq[t][kb], o[t][vb]);
+                    }
+                }
+                /* of place i = 16 t + c the last start at or before it */
+                int since[R];
+#pragma unroll
+                for (int t = 0; t < R; t++) {
+                    const uint32_t before = starts & (uint32_t)((2ull << (16 * t + c)) - 1);
+                    since[t] = before ? 31 - __builtin_clz(before) : -1;
+#pragma unroll
+                    for (int vb = 0; vb < VB; vb++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) o[t][vb][r] = since[t] < 0 ? o[t][vb][r] * reach[t] : 0.0f;
+                }
+                /* scores, rows j and columns i; they are what P v sums over as they lie */
+                Quad score[R][R];
+#pragma unroll
+                for (int s = 0; s < R; s++) {
+                    Quad kq[KB];
+#pragma unroll
+                    for (int kb = 0; kb < KB; kb++) kq[kb] = along<kKeyRow>(lk, 16 * s, 16 * kb);
+#pragma unroll
+                    for (int t = s; t < R; t++) {
+                        F4 x = {0, 0, 0, 0};
+                        if constexpr (kHalf) {
+#pragma unroll
+                            for (int kb = 0; kb < KB; kb += 2) x = multiply(kq[kb], kq[kb + 1], qq[t][kb], qq[t][kb + 1], x);
+                        } else {
+#pragma unroll
+                            for (int kb = 0; kb < KB; kb++) x = multiply(kq[kb], qq[t][kb], x);
+                        }
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const int at = 16 * s + 4 * g + r;
+                            x[r] = at >= since[t] && at <= 16 * t + c ? x[r] * near[t - s][r] : 0.0f;
+                        }
+                        score[t][s] = with(x);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < R; t++)
+#pragma unroll
+                    for (int vb = 0; vb < VB; vb++) {
+                        if constexpr (kHalf)
+                            o[t][vb] = multiply(vq[0][vb], vq[1][vb], score[t][0], t ? score[1][1] : S4{0, 0, 0, 0}, o[t][vb]);
+                        else
+                            o[t][vb] = multiply(vq[0][vb], score[0][0], o[t][vb]);
+                    }
+                /* lane (g, c): of place 16 t + c the columns 4 g + r of each tile */
+#pragma unroll
+                for (int t = 0; t < R; t++) {
+                    const int at = 16 * t + c;
+                    if (at >= n || !m.out) continue;
+                    T* to = out + (p + at) * m.out_stride[0];
+                    constexpr int kTiles = kHalf ? 2 : 1, kWide = 4 * kTiles;
+#pragma unroll
+                    for (int vb = 0; vb < VB; vb += kTiles) {
+                        const int col = value_col(vb) + kWide * g;
+                        Pack<T, kWide> y;
+#pragma unroll
+                        for (int i = 0; i < kWide; i++) y.v[i] = (T)o[t][vb + i / 4][i % 4];
+                        if (col + kWide <= value) {
+                            *(Pack<T, kWide>*)(to + col) = y;
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < kWide; i++)
+                                if (col + i < value) to[col + i] = y.v[i];
+                        }
+                    }
+                }
+            }
+            /* what is kept of the state, and of the places from the last start on */
+            const bool drop = starts != 0;
+            dropped |= drop;
+            const int last = drop ? 31 - __builtin_clz(starts) : -1;
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++) {
+                F4 kw[R];
+#pragma unroll
+                for (int t = 0; t < R; t++) {
+                    const Quad x = across<kKeyRow, 4>(lk, 16 * t, 16 * kb);
+                    if constexpr (kHalf) kw[t] = __builtin_convertvector(__builtin_bit_cast(B4, x), F4);
+                    else kw[t] = x;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) kw[t][r] = 16 * t + 4 * g + r >= last ? kw[t][r] * keep[t][r] : 0.0f;
+                }
+#pragma unroll
+                for (int vb = 0; vb < VB; vb++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) state[kb][vb][r] = drop ? 0.0f : state[kb][vb][r] * pass;
+                if constexpr (kHalf) {
+                    const S4 h0 = round4(kw[0]), h1 = round4(kw[1]), l0 = rest4(kw[0], h0), l1 = rest4(kw[1], h1);
+#pragma unroll
+                    for (int vb = 0; vb < VB; vb++) {
+                        state[kb][vb] = multiply(h0, h1, vq[0][vb], vq[1][vb], state[kb][vb]);
+                        state[kb][vb] = multiply(l0, l1, vq[0][vb], vq[1][vb], state[kb][vb]);
+                    }
+                } else {
+#pragma unroll
+                    for (int vb = 0; vb < VB; vb++) state[kb][vb] = multiply(kw[0], vq[0][vb], state[kb][vb]);
+                }
+            }
+        }
+        if (carry && lane == 0 && u.first == 0)
+            *carry = dropped ? -1.0f : __builtin_amdgcn_exp2f(places ? (float)places * l2 : 0.0f);
+        if (!leave) return;
+        const bool gone = !STATE && m.leave_starts && started(m.leave_starts + u.env * m.leave_starts_stride, j.starts_type);
+#pragma unroll
+        for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+            for (int vb = 0; vb < VB; vb++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int row = kb * 16 + 4 * g + r, col = value_col(vb) + kStep * (c / 4) + c % 4;
+                    if (row < m.key && col < value)
+                        leave[row * m.state_row + (u.first + col) * m.state_col] = gone ? 0.0f : state[kb][vb][r];
+                }
+    }
+};
+
+/* Waves of a workgroup: neighbours share what they read (the parts and roles
+ * of a sequence) or lie side by side in memory (heads).  Workgroups go to the
+ * 8 dies in turn: each die's take neighbouring ones. */
+template <typename T, int KD, int VD, bool STATE>
+__global__ __launch_bounds__(kThreads, KD * VD <= 64 * 64 ? 2 : 1) void la_walk(Job j) {
+    extern __shared__ __attribute__((aligned(16))) char shared[];
+    typedef Walk<T, KD, VD, STATE> W;
+    const unsigned die = blockIdx.x % 8, share = gridDim.x / 8, rest = gridDim.x % 8;
+    const unsigned block = die * share + (die < rest ? die : rest) + blockIdx.x / 8;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    int64_t id = (int64_t)block * (blockDim.x / kWave) + wave;
+    const int64_t pieces = STATE ? j.pieces - 1 : j.pieces;
+    if (id >= j.envs * j.heads * pieces * j.roles * j.parts) return;
+    Unit u;
+    u.first = (int)(id % j.parts) * VD;
+    id /= j.parts;
+    u.role = (int)(id % j.roles);
+    id /= j.roles;
+    u.head = id % j.heads;
+    id /= j.heads;
+    u.env = id % j.envs;
+    u.piece = id / j.envs;
+    const Mix& m = j.mix[u.role];
+    if (u.first >= m.value) return;
+    if (!m.forward) u.piece = pieces - 1 - u.piece;
+    const int64_t sequences = j.envs * j.heads, sequence = u.env * j.heads + u.head, size = (int64_t)m.key * m.value;
+    const int64_t from = u.piece * j.places, left = j.steps - from, places = left < j.places ? left : j.places;
+    const float* enter = m.enter ? m.enter + sequence * size : NULL;
+    float* leave = m.leave ? m.leave + sequence * size : NULL;
+    float* carry = NULL;
+    if (STATE) {
+        if (u.piece) enter = NULL;
+        leave = m.pieces + (u.piece * sequences + sequence) * size;
+        carry = m.carry + u.piece * sequences + sequence;
+    } else {
+        if (u.piece) enter = m.pieces + ((u.piece - 1) * sequences + sequence) * size;
+        if (u.piece + 1 < pieces) leave = NULL;
+    }
+    W::run(j, m, u, from, places, enter, m.forward && u.piece == 0 && j.steps, leave, carry, shared + wave * W::kBytes);
+}
+
+/* What enters each piece, over what the pieces left by themselves. */
+__global__ __launch_bounds__(kThreads) void la_join(Job j) {
     const Mix& m = j.mix[blockIdx.y];
-    const int64_t env = blockIdx.x / j.heads, head = blockIdx.x % j.heads;
-    const int col = threadIdx.x % B3_MAX_HEAD, top = threadIdx.x / B3_MAX_HEAD * kRows;
-    const float decay = decay_of(j.decay, head);
-    const int64_t state = (env * j.heads + head) * m.key * m.value;
-    float s[kRows];
-#pragma unroll
-    for (int r = 0; r < kRows; r++) {
-        const bool in = top + r < m.key && col < m.value;
-        s[r] = in && m.enter ? m.enter[state + (top + r) * m.state_row + col * m.state_col] : 0.0f;
-        if (m.enter_early) s[r] *= decay;
+    const int64_t sequences = j.envs * j.heads, size = (int64_t)m.key * m.value, all = sequences * size;
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i >= all) return;
+    float x = m.pieces[i];
+#pragma unroll 8
+    for (int64_t p = 1; p < j.pieces - 1; p++) {
+        const float f = m.carry[p * sequences + i / size], own = m.pieces[p * all + i];
+        x = f < 0 ? own : f * x + own;
+        m.pieces[p * all + i] = x;
     }
-    for (int64_t p = 0; p < j.steps; p++) {
-        const bool start = m.starts && (p || m.enter_early)
-            && started(m.starts + p * m.starts_stride[0] + env * m.starts_stride[1], j.starts_type);
-        __syncthreads();
-        if ((int)threadIdx.x < B3_MAX_HEAD) {
-            const int c = threadIdx.x;
-            q[c] = c < m.key ? to_float(((const T*)m.q)[p * m.q_stride[0] + env * m.q_stride[1] + head * m.q_stride[2] + c]) : 0;
-            k[c] = c < m.key ? m.update * to_float(((const T*)m.k)[p * m.k_stride[0] + env * m.k_stride[1] + head * m.k_stride[2] + c]) : 0;
-            v[c] = c < m.value ? to_float(((const T*)m.v)[p * m.v_stride[0] + env * m.v_stride[1] + head * m.v_stride[2] + c]) : 0;
-        }
-        __syncthreads();
-        float o = 0;
-#pragma unroll
-        for (int r = 0; r < kRows; r++) {
-            s[r] = (start ? 0.0f : s[r]) + k[top + r] * v[col];
-            o += q[top + r] * s[r];
-            if (p + 1 < j.steps || !m.leave_early) s[r] *= decay;
-        }
-        if (top) half[col] = o;
-        __syncthreads();
-        if (!top && col < m.value && m.out)
-            ((T*)m.out)[p * m.out_stride[0] + env * m.out_stride[1] + head * m.out_stride[2] + col] = (T)(m.reach * (o + half[col]));
-    }
-    if (!m.leave) return;
-    const bool drop = m.leave_starts && started(m.leave_starts + env * m.leave_starts_stride, j.starts_type);
-#pragma unroll
-    for (int r = 0; r < kRows; r++)
-        if (top + r < m.key && col < m.value)
-            m.leave[state + (top + r) * m.state_row + col * m.state_col] = drop ? 0.0f : s[r];
 }
 
 /* ---- one step ---- */
@@ -116,29 +576,69 @@ struct StepJob {
     void* out;
 };
 
-template <typename T>
+/* A wave to a sequence: L lanes with four neighbouring columns each to a row
+ * of the state, 64 / L rows at once.  The state, read and written, is all but
+ * all that there is to move. */
+template <typename T, int L>
 __global__ __launch_bounds__(kThreads) void la_step(StepJob j) {
-    constexpr int kRows = B3_MAX_HEAD / 2;
-    __shared__ float half[B3_MAX_HEAD];
+    constexpr int kRows = kWave / L, kAhead = 8;
     const B3Attention& g = j.g;
-    const int64_t env = blockIdx.x / g.heads, head = blockIdx.x % g.heads;
-    const int col = threadIdx.x % B3_MAX_HEAD, top = threadIdx.x / B3_MAX_HEAD * kRows;
+    const int64_t id = (int64_t)blockIdx.x * (kThreads / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    if (id >= g.envs * g.heads) return;
+    const int64_t env = id / g.heads, head = id % g.heads;
+    const int lane = threadIdx.x % kWave, col = lane % L * 4, row = lane / L, left = g.value - col;
     const float decay = decay_of(g.decay, head);
     const bool start = g.starts
         && started((const char*)g.starts + env * g.starts_stride[1] * (g.starts_type == B3_F32 ? 4 : 1), g.starts_type);
-    float* s = j.state + (env * g.heads + head) * g.key * g.value + col;
+    float* s = j.state + id * g.key * g.value + col;
     const T* q = (const T*)g.q + env * g.q_stride[1] + head * g.q_stride[2];
     const T* k = (const T*)g.k + env * g.k_stride[1] + head * g.k_stride[2];
-    const float v = col < g.value ? to_float(((const T*)g.v)[env * g.v_stride[1] + head * g.v_stride[2] + col]) : 0.0f;
-    float o = 0;
-    for (int r = top; r < top + kRows && r < g.key && col < g.value; r++) {
-        const float x = (start ? 0.0f : decay * s[r * g.value]) + to_float(k[r]) * v;
-        s[r * g.value] = x;
-        o += to_float(q[r]) * x;
+    const T* pv = (const T*)g.v + env * g.v_stride[1] + head * g.v_stride[2] + col;
+    float v[4], o[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = i < left ? to_float(pv[i]) : 0.0f;
+    for (int r0 = 0; r0 < g.key; r0 += kRows * kAhead) {
+        Pack<float, 4> x[kAhead];
+        float kr[kAhead], qr[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; a++) {
+            const int r = r0 + a * kRows + row;
+            const bool in = r < g.key;
+            x[a] = Pack<float, 4>{0, 0, 0, 0};
+            if (in && !start && left >= 4) {
+                x[a] = *(const Pack<float, 4>*)(s + (int64_t)r * g.value);
+            } else if (in && !start) {
+                for (int i = 0; i < 3; i++)
+                    if (i < left) x[a].v[i] = s[(int64_t)r * g.value + i];
+            }
+            kr[a] = in ? to_float(k[r]) : 0.0f;
+            qr[a] = in ? to_float(q[r]) : 0.0f;
+        }
+#pragma unroll
+        for (int a = 0; a < kAhead; a++) {
+            const int r = r0 + a * kRows + row;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                x[a].v[i] = (start ? 0.0f : decay * x[a].v[i]) + kr[a] * v[i];
+                if (r < g.key) o[i] += qr[a] * x[a].v[i];
+            }
+            if (r < g.key && left >= 4) {
+                *(Pack<float, 4>*)(s + (int64_t)r * g.value) = x[a];
+            } else if (r < g.key) {
+                for (int i = 0; i < 3; i++)
+                    if (i < left) s[(int64_t)r * g.value + i] = x[a].v[i];
+            }
+        }
     }
-    if (top) half[col] = o;
-    __syncthreads();
-    if (!top && col < g.value) ((T*)j.out)[(env * g.heads + head) * g.value + col] = (T)(j.scale * (o + half[col]));
+#pragma unroll
+    for (int d = L; d < kWave; d *= 2)
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] += __shfl_xor(o[i], d);
+    if (row) return;
+    T* out = (T*)j.out + id * g.value + col;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (i < left) out[i] = (T)(j.scale * o[i]);
 }
 
 /* ---- launches ---- */
@@ -194,11 +694,11 @@ Mix forwards(const B3Attention& g) {
     const int64_t size = g.starts_type == B3_F32 ? 4 : 1;
     m.reach = (float)g.scale;
     m.update = 1;
+    m.forward = true;
     m.starts = (const char*)g.starts;
     m.starts_stride[0] = g.starts_stride[0] * size;
     m.starts_stride[1] = g.starts_stride[1] * size;
     m.enter = g.state;
-    m.enter_early = m.leave_early = g.steps > 0;
     return m;
 }
 
@@ -207,6 +707,7 @@ Mix backwards(const B3Attention& g, const float* d_last) {
     Mix m = forwards(g);
     m.reach = 1;
     m.update = (float)g.scale;
+    m.forward = false;
     if (m.starts && g.steps) {
         m.leave_starts = m.starts;
         m.leave_starts_stride = m.starts_stride[1];
@@ -214,19 +715,98 @@ Mix backwards(const B3Attention& g, const float* d_last) {
         m.starts_stride[0] = -m.starts_stride[0];
     }
     m.enter = d_last;
-    m.enter_early = m.leave_early = false;
     return m;
 }
 
-template <typename T>
-hipError_t launch(const Job& j, int roles, hipStream_t stream) {
-    la_places<T><<<dim3((unsigned)(j.envs * j.heads), roles), kThreads, 0, stream>>>(j);
+int columns_of(int dims) { return dims <= 32 ? 32 : dims <= 64 ? 64 : 128; }
+int part_of(int value) { return value <= 32 ? 32 : 64; }
+int places_of(int type) { return type == B3_BF16 ? 32 : 16; }
+
+/* How the work is cut: into parts of v's columns and, where that leaves
+ * compute units idle, into pieces of the steps. */
+struct Plan {
+    int key, value, parts;                       // columns of tiles
+    int64_t places, pieces;
+};
+
+Plan plan_of(const B3Attention& g, bool backward) {
+    Plan p;
+    const int most = g.key > g.value ? g.key : g.value;
+    p.key = columns_of(backward ? most : g.key);
+    p.value = part_of(backward ? most : g.value);
+    p.parts = (int)ceil_div(backward ? most : g.value, p.value);
+    const int64_t units = g.envs * g.heads * p.parts * (backward ? kRoles : 1);
+    const int64_t chunk = places_of(g.type), most_pieces = g.steps / (chunk * kPieceChunks);
+    p.pieces = units >= kWaves / 2 ? 1 : ceil_div(kWaves, units);
+    p.pieces = p.pieces < most_pieces ? p.pieces : most_pieces;
+    p.pieces = p.pieces > 1 ? p.pieces : 1;
+    p.places = ceil_div(ceil_div(g.steps, p.pieces), chunk) * chunk;
+    p.places = p.places > 0 ? p.places : chunk;
+    p.pieces = g.steps > 0 ? ceil_div(g.steps, p.places) : 1;
+    return p;
+}
+
+/* Floats of a way's pieces. */
+int64_t pieces_size(const B3Attention& g, const Plan& p) {
+    return (p.pieces - 1) * g.envs * g.heads * ((int64_t)g.key * g.value + 1);
+}
+
+size_t workspace_of(const B3Attention& g, const Plan& p, bool backward) {
+    return (size_t)(pieces_size(g, p) * (backward ? 2 : 1)) * sizeof(float);
+}
+
+void place_pieces(Mix& m, const B3Attention& g, const Plan& p, void* workspace, int way) {
+    m.pieces = (float*)workspace + way * pieces_size(g, p);
+    m.carry = m.pieces + (p.pieces - 1) * g.envs * g.heads * g.key * g.value;
+}
+
+template <typename T, int KD, int VD, bool STATE>
+hipError_t launch(const Job& j, hipStream_t stream) {
+    typedef Walk<T, KD, VD, STATE> W;
+    constexpr int kLds = 64 << 10, kMost = kLds / W::kBytes, kWavesHere = kMost >= 4 ? 4 : kMost >= 2 ? 2 : 1;
+    static_assert(kMost >= 1, "a wave's tiles");
+    const int64_t units = j.envs * j.heads * (STATE ? j.pieces - 1 : j.pieces) * j.roles * j.parts;
+    la_walk<T, KD, VD, STATE><<<(unsigned)ceil_div(units, kWavesHere), kWavesHere * kWave, kWavesHere * W::kBytes, stream>>>(j);
     return hipGetLastError();
 }
 
-hipError_t launch(const Job& j, int roles, int type, hipStream_t stream) {
-    return type == B3_F32 ? launch<float>(j, roles, stream) : type == B3_F16 ? launch<_Float16>(j, roles, stream)
-                                                                            : launch<__bf16>(j, roles, stream);
+template <typename T, bool STATE>
+hipError_t launch_columns(const Job& j, const Plan& p, hipStream_t stream) {
+    if (p.value == 32)
+        return p.key == 32 ? launch<T, 32, 32, STATE>(j, stream) : p.key == 64 ? launch<T, 64, 32, STATE>(j, stream)
+                                                                            : launch<T, 128, 32, STATE>(j, stream);
+    return p.key == 32 ? launch<T, 32, 64, STATE>(j, stream) : p.key == 64 ? launch<T, 64, 64, STATE>(j, stream)
+                                                                           : launch<T, 128, 64, STATE>(j, stream);
+}
+
+/* `ways`: what of the job's mixes learns the pieces' states, one for each. */
+template <typename T>
+hipError_t launch_typed(const Job& j, const Job& ways, const Plan& p, hipStream_t stream) {
+    if (j.pieces > 1) {
+        hipError_t err = launch_columns<T, true>(ways, p, stream);
+        if (err != hipSuccess) return err;
+        const int64_t all = j.envs * j.heads * j.mix[0].key * j.mix[0].value;
+        if (j.pieces > 2) la_join<<<dim3((unsigned)ceil_div(all, kThreads), ways.roles), kThreads, 0, stream>>>(ways);
+        if ((err = hipGetLastError()) != hipSuccess) return err;
+    }
+    return launch_columns<T, false>(j, p, stream);
+}
+
+hipError_t launch_job(Job& j, Job& ways, const Plan& p, int type, hipStream_t stream) {
+    j.parts = ways.parts = p.parts;
+    j.places = ways.places = p.places;
+    j.pieces = ways.pieces = p.pieces;
+    return type == B3_F32 ? launch_typed<float>(j, ways, p, stream)
+        : type == B3_F16 ? launch_typed<_Float16>(j, ways, p, stream) : launch_typed<__bf16>(j, ways, p, stream);
+}
+
+template <typename T>
+hipError_t launch_step(const StepJob& j, hipStream_t stream) {
+    const unsigned blocks = (unsigned)ceil_div(j.g.envs * j.g.heads, kThreads / kWave);
+    if (j.g.value <= 32) la_step<T, 8><<<blocks, kThreads, 0, stream>>>(j);
+    else if (j.g.value <= 64) la_step<T, 16><<<blocks, kThreads, 0, stream>>>(j);
+    else la_step<T, 32><<<blocks, kThreads, 0, stream>>>(j);
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -236,13 +816,17 @@ using namespace b3p;
 
 extern "C" {
 
-size_t b3_linear_attention_workspace(const B3Attention* g, int backward) { return 0; }
+size_t b3_linear_attention_workspace(const B3Attention* g, int backward) {
+    if (!valid(g) || g->envs == 0 || g->heads == 0) return 0;
+    return workspace_of(*g, plan_of(*g, backward != 0), backward != 0);
+}
 
 hipError_t b3_linear_attention_gpu(const B3Attention* g, void* out, float* last_state, void* workspace,
         size_t workspace_bytes, hipStream_t stream) {
     if (!valid(g)) return hipErrorInvalidValue;
     if (g->envs == 0 || g->heads == 0 || (g->steps == 0 && !last_state)) return hipSuccess;
-    if (g->steps && !out) return hipErrorInvalidValue;
+    const Plan p = plan_of(*g, false);
+    if ((g->steps && !out) || !holds(workspace, workspace_bytes, workspace_of(*g, p, false))) return hipErrorInvalidValue;
     Job j = job_of(*g);
     Mix m = forwards(*g);
     m.q = g->q;
@@ -258,8 +842,11 @@ hipError_t b3_linear_attention_gpu(const B3Attention* g, void* out, float* last_
     m.leave = last_state;
     m.state_row = g->value;
     m.state_col = 1;
+    place_pieces(m, *g, p, workspace, 0);
     j.mix[0] = m;
-    return launch(j, 1, g->type, stream);
+    j.roles = 1;
+    Job ways = j;
+    return launch_job(j, ways, p, g->type, stream);
 }
 
 hipError_t b3_linear_attention_backward_gpu(const B3Attention* g, const void* d_out, const int64_t d_out_stride[3],
@@ -267,7 +854,9 @@ hipError_t b3_linear_attention_backward_gpu(const B3Attention* g, const void* d_
         size_t workspace_bytes, hipStream_t stream) {
     if (!valid(g)) return hipErrorInvalidValue;
     if (g->envs == 0 || g->heads == 0) return hipSuccess;
-    if (g->steps && (!d_out || !d_out_stride)) return hipErrorInvalidValue;
+    const Plan p = plan_of(*g, true);
+    if ((g->steps && (!d_out || !d_out_stride)) || !holds(workspace, workspace_bytes, workspace_of(*g, p, true)))
+        return hipErrorInvalidValue;
     Job j = job_of(*g);
     Mix a = forwards(*g);                        // d_q: S^T, of d_out, v and k
     a.q = d_out;
@@ -313,11 +902,16 @@ hipError_t b3_linear_attention_backward_gpu(const B3Attention* g, const void* d_
         backwards_arrays(b, *g);
         backwards_arrays(c, *g);
     }
-    int roles = 0;
-    if (d_q && g->steps) j.mix[roles++] = a;
-    if (d_k && g->steps) j.mix[roles++] = b;
-    if (d_v || d_state) j.mix[roles++] = c;
-    return roles ? launch(j, roles, g->type, stream) : hipSuccess;
+    place_pieces(a, *g, p, workspace, 0);
+    place_pieces(b, *g, p, workspace, 1);
+    place_pieces(c, *g, p, workspace, 1);
+    Job ways = j;
+    if (d_q && g->steps) j.mix[j.roles++] = ways.mix[ways.roles++] = a;
+    if (d_k && g->steps) j.mix[j.roles++] = b;
+    if (d_v || d_state) j.mix[j.roles++] = c;
+    if (!j.roles) return hipSuccess;
+    if (!j.mix[j.roles - 1].forward) ways.mix[ways.roles++] = c;      // for d_k and d_v alike
+    return launch_job(j, ways, p, g->type, stream);
 }
 
 hipError_t b3_linear_attention_step_gpu(const B3Attention* g, float* state, void* out, hipStream_t stream) {
@@ -325,11 +919,8 @@ hipError_t b3_linear_attention_step_gpu(const B3Attention* g, float* state, void
     if (g->envs == 0 || g->heads == 0) return hipSuccess;
     if (!state || !out) return hipErrorInvalidValue;
     const StepJob j = {*g, (float)g->scale, state, out};
-    const unsigned blocks = (unsigned)(g->envs * g->heads);
-    if (g->type == B3_F32) la_step<float><<<blocks, kThreads, 0, stream>>>(j);
-    else if (g->type == B3_F16) la_step<_Float16><<<blocks, kThreads, 0, stream>>>(j);
-    else la_step<__bf16><<<blocks, kThreads, 0, stream>>>(j);
-    return hipGetLastError();
+    return g->type == B3_F32 ? launch_step<float>(j, stream) : g->type == B3_F16 ? launch_step<_Float16>(j, stream)
+                                                                                : launch_step<__bf16>(j, stream);
 }
 
 }  // extern "C"
