@@ -2,10 +2,24 @@
  * b3_muon.hip - Muon's step over a policy's matrices (include/b3_policy.h).
  *
  *   m = momentum m + g, u = g + momentum m, x = u / (|u| + eps)
- *   x = a x + (b y + c y y) x, y = x x^T, some times; then w moves by x
+ *   y = x x^T, z = a + b y + c y y, x = z x, some times; then w moves by x
  *
- * A matrix is worked on with its shorter side first, so that y is as small as
- * it can be.
+ * x is a matrix with its shorter side first, so that y and z are as small as
+ * they can be; they are symmetric, and half of their tiles are computed.
+ *
+ * Products of 32-bit numbers come of three on the 16-bit matrix units: a
+ * number is kept as a half and the half of what is left, 22 bits in all, and
+ * h h' + h l' + l h' leaves out 2^-22 of a term (S. Markidis and others,
+ * "NVIDIA Tensor Core Programmability, Performance & Precision", 2018, has the
+ * idea).  The range of halves is enough, since x, y and z are bounded: their
+ * singular values stay under 1.21, 1.47 and 3.45, whatever the gradient, and
+ * kScale brings their elements to where 2^-24, the least half, is 2^-37.
+ * Accumulators are in 32 bits.
+ *
+ * A launch computes one product of all matrices, a workgroup to a tile of 128
+ * x 128.  Matrices lie in blocks of 32 columns, halves and what is left side by
+ * side, 128 bytes to a row's block; both sides are filled up with zeros to
+ * whole tiles.
  */
 #include "policy_common.h"
 
@@ -14,9 +28,58 @@
 namespace b3p {
 
 constexpr int kThreads = 256;
-constexpr int kTile = 32;
-constexpr int kSumBlocks = 256;
+constexpr int kBatch = 200;                      // matrices to a launch that takes gradients
+constexpr size_t kMostArguments = 4096;          // bytes of a launch
+constexpr int kTile = 128, kStep = 32;           // of a product: rows and columns, and what is summed at once
+constexpr int kCut = 64;                         // tile of the first x
+constexpr int kMostParts = 256;                  // workgroups that a matrix' gradient is gone over by
+constexpr int64_t kPart = 4096;                  // its elements at the least
 constexpr double kA = 3.4445, kB = -4.7750, kC = 2.0315;
+constexpr float kScale = 8192.0f;
+
+/* A matrix of the table.  x, next, y and z are in elements of `work`, of 4
+ * bytes (both halves). */
+struct Matrix {
+    void* param;
+    int64_t rows, columns, at;                   // at: in the flat arrays
+    int64_t m, n;                                // x's sides, filled up
+    int64_t x, next, y, z;
+    int64_t part;                                // elements of a workgroup's part of the gradient
+    int64_t partial;                             // its first sum
+    double decay, factor;                        // of the rate, by shape
+    int type, parts;
+};
+
+struct Place {
+    int matrix, i, j;
+};
+
+/* The gradients of matrices from `base` on. */
+struct Gradients {
+    const void* at[kBatch];                      // NULL: not stepped
+    uint8_t type[kBatch];
+    int base;
+};
+
+struct Common {
+    const Matrix* matrices;
+    const Place* places;
+    float* momentum;
+    float* master;
+    char* work;
+    double* partial;
+    int* live;                                   // [matrices]: has a gradient
+    float keep;                                  // momentum
+    int nesterov;
+    double eps, lr;
+    int64_t first;                               // place of the launch's first workgroup
+};
+
+struct GradientLaunch {
+    Gradients g;
+    Common c;
+};
+static_assert(sizeof(GradientLaunch) <= kMostArguments, "kernel arguments");
 
 }  // namespace b3p
 
@@ -25,89 +88,289 @@ struct B3Muon {
     B3MuonConfig config;
     B3MuonState state;
     B3MuonMatrix* given;                         // host
-    int64_t* at;                                 // host: of each in the flat arrays
-    float* work;                                 // device: x and its next, y and its polynomial
+    b3p::Matrix* matrices;                       // device
+    b3p::Place* places;                          // device: of parts, cuts, symmetric and whole tiles in turn
+    int64_t* first_part;                         // host: by matrix; count + 1
+    int64_t* first_cut;                          // host
+    int64_t cuts, halves, tiles;                 // where those places begin, after the parts
+    int64_t end;
+    char* work;                                  // device
     double* partial;                             // device
-    int64_t most, side;                          // elements of the largest matrix, of its y
+    int* live;                                   // device
 };
 
 namespace b3p {
 namespace {
 
-template <typename T>
-__device__ __forceinline__ float element(const void* p, int64_t i) { return to_float(((const T*)p)[i]); }
+typedef _Float16 H8 __attribute__((ext_vector_type(8)));
+typedef _Float16 H4 __attribute__((ext_vector_type(4)));
+typedef short S4 __attribute__((ext_vector_type(4)));
+typedef float F4 __attribute__((ext_vector_type(4)));
+typedef uint32_t U4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float element(const void* p, int type, int64_t i) {
-    return type == B3_F32 ? element<float>(p, i) : type == B3_F16 ? element<_Float16>(p, i) : element<__bf16>(p, i);
+    return type == B3_F32 ? ((const float*)p)[i] : type == B3_F16 ? to_float(((const _Float16*)p)[i])
+                                                                  : to_float(((const __bf16*)p)[i]);
 }
 
-__global__ __launch_bounds__(kThreads) void mu_momentum(const void* grad, int type, float* momentum, int64_t rows,
-    int64_t columns, float keep, int nesterov, float* x, double* partial) {
-    __shared__ double lds[kThreads];
-    const bool turned = rows > columns;
+/* Of workgroups in turn to the 8 dies: each die's take neighbouring places. */
+__device__ __forceinline__ unsigned by_die() {
+    const unsigned die = blockIdx.x % 8, share = gridDim.x / 8, rest = gridDim.x % 8;
+    return die * share + (die < rest ? die : rest) + blockIdx.x / 8;
+}
+
+__device__ double block_sum(double x) {
+    __shared__ double lds[kThreads / kWave];
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) x += __shfl_xor(x, d);
+    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = x;
+    __syncthreads();
+    x = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / kWave; w++) x += lds[w];
+    return x;
+}
+
+__device__ __forceinline__ float direction(float g, float m, const Common& c) { return c.nesterov ? g + c.keep * m : m; }
+
+/* The momentum, and a part's sum of squares of u. */
+__global__ __launch_bounds__(kThreads) void mu_momentum(GradientLaunch l) {
+    const Place p = l.c.places[l.c.first + blockIdx.x];
+    const Matrix& t = l.c.matrices[p.matrix];
+    const void* grad = l.g.at[p.matrix - l.g.base];
+    const int type = l.g.type[p.matrix - l.g.base];
+    if (p.i == 0 && threadIdx.x == 0) l.c.live[p.matrix] = grad != NULL;
+    if (!grad) return;
+    float* momentum = l.c.momentum + t.at;
+    const int64_t from = p.i * t.part, all = t.rows * t.columns, end = from + t.part < all ? from + t.part : all;
     double sum = 0;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < rows * columns; i += (int64_t)gridDim.x * kThreads) {
-        const float g = element(grad, type, i), m = keep * momentum[i] + g, u = nesterov ? g + keep * m : m;
+#pragma unroll 4
+    for (int64_t i = from + threadIdx.x; i < end; i += kThreads) {
+        const float g = element(grad, type, i), m = l.c.keep * momentum[i] + g, u = direction(g, m, l.c);
         momentum[i] = m;
-        x[turned ? i % columns * rows + i / columns : i] = u;
         sum += (double)u * u;
     }
-    lds[threadIdx.x] = sum;
-    __syncthreads();
-    if (threadIdx.x) return;
-    for (int i = 1; i < kThreads; i++) sum += lds[i];
-    partial[blockIdx.x] = sum;
+    sum = block_sum(sum);
+    if (threadIdx.x == 0) l.c.partial[t.partial + p.i] = sum;
 }
 
-__global__ __launch_bounds__(kThreads) void mu_scale(float* x, int64_t n, const double* partial, int partials, float eps) {
-    double sum = 0;
-    for (int i = 0; i < partials; i++) sum += partial[i];
-    const float size = (float)sqrt(sum) + eps;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) x[i] /= size;
+/* Where halves of row r, columns from 32 b on, lie: 32 of them, then what is
+ * left of those. */
+__device__ __forceinline__ _Float16* block_of(char* work, int64_t base, int64_t columns, int64_t r, int64_t b) {
+    return (_Float16*)(work + base * 4 + (r * columns + b * kStep) * 4);
 }
 
-/* out[m][n] = p add + q left[m][k] right, where right is [k][n], or [n][k] with TURNED. */
-template <bool TURNED>
-__global__ __launch_bounds__(kThreads) void mu_product(const float* left, const float* right, const float* add, float* out,
-    int64_t m, int64_t n, int64_t k, float p, float q) {
-    __shared__ float a[kTile][kTile + 1], b[kTile][kTile + 1];
-    const int col = threadIdx.x % kTile, row = threadIdx.x / kTile;
-    constexpr int kRows = kThreads / kTile;
-    const int64_t j0 = (int64_t)blockIdx.x * kTile, i0 = (int64_t)blockIdx.y * kTile;
-    float sum[kTile / kRows] = {};
-    for (int64_t k0 = 0; k0 < k; k0 += kTile) {
-        for (int r = row; r < kTile; r += kRows) {
-            a[r][col] = i0 + r < m && k0 + col < k ? left[(i0 + r) * k + k0 + col] : 0.0f;
-            if (TURNED)
-                b[col][r] = j0 + r < n && k0 + col < k ? right[(j0 + r) * k + k0 + col] : 0.0f;
-            else
-                b[r][col] = k0 + r < k && j0 + col < n ? right[(k0 + r) * n + j0 + col] : 0.0f;
+/* The first x, a square of it: u over its norm. */
+__global__ __launch_bounds__(kThreads) void mu_split(GradientLaunch l) {
+    __shared__ float tile[kCut][kCut + 1];
+    const Place p = l.c.places[l.c.first + blockIdx.x];
+    const Matrix& t = l.c.matrices[p.matrix];
+    const void* grad = l.g.at[p.matrix - l.g.base];
+    const int type = l.g.type[p.matrix - l.g.base];
+    if (!grad) return;
+    const double size = sqrt(block_sum((int)threadIdx.x < t.parts ? l.c.partial[t.partial + threadIdx.x] : 0.0));
+    const double scale = kScale / (size + l.c.eps);
+    const bool turned = t.rows > t.columns;
+    const int64_t r0 = (int64_t)(turned ? p.j : p.i) * kCut, c0 = (int64_t)(turned ? p.i : p.j) * kCut;
+    const float* momentum = l.c.momentum + t.at;
+    const int col = threadIdx.x % kCut, row = threadIdx.x / kCut;
+#pragma unroll 4
+    for (int r = row; r < kCut; r += kThreads / kCut) {
+        float u = 0;
+        if (r0 + r < t.rows && c0 + col < t.columns) {
+            const int64_t i = (r0 + r) * t.columns + c0 + col;
+            u = (float)(scale * direction(element(grad, type, i), momentum[i], l.c));
         }
-        __syncthreads();
-        for (int i = 0; i < kTile; i++)
-#pragma unroll
-            for (int r = 0; r < kTile / kRows; r++) sum[r] = __builtin_fmaf(a[row + r * kRows][i], b[i][col], sum[r]);
-        __syncthreads();
+        tile[turned ? col : r][turned ? r : col] = u;
     }
-    for (int r = 0; r < kTile / kRows; r++) {
-        const int64_t i = i0 + row + r * kRows, j = j0 + col;
-        if (i < m && j < n) out[i * n + j] = q * sum[r] + (add ? p * add[i * n + j] : 0.0f);
+    __syncthreads();
+    /* a row's block of 32 to four threads of eight */
+    for (int k = threadIdx.x; k < kCut * kCut / 8; k += kThreads) {
+        const int r = k / (kCut / 8), b = k % (kCut / 8) / 4, o = k % 4 * 8;
+        H8 h, rest;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float x = tile[r][b * kStep + o + e];
+            h[e] = (_Float16)x;
+            rest[e] = (_Float16)(x - (float)h[e]);
+        }
+        _Float16* to = block_of(l.c.work, t.x, t.n, (int64_t)p.i * kCut + r, (int64_t)p.j * (kCut / kStep) + b) + o;
+        *(H8*)to = h;
+        *(H8*)(to + kStep) = rest;
     }
 }
+
+enum Product { GRAM, POLYNOMIAL, NEXT, LAST };
+
+/* What a launch of mu_product does: y = x x^T, z = a + b y + c y y, or x = z x
+ * (LAST: and the weights move by it). */
+struct ProductLaunch {
+    Common c;
+    bool swapped;                                // x is in `next`
+};
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void mu_update(T* param, float* master, const float* x, int64_t rows,
-    int64_t columns, float keep, float rate) {
-    const bool turned = rows > columns;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < rows * columns; i += (int64_t)gridDim.x * kThreads) {
-        const T old = param[i];
-        float w = to_float(old);
-        if (master && to_float((T)master[i]) == w) w = master[i];
-        w = w * keep - rate * x[turned ? i % columns * rows + i / columns : i];
-        if (master) master[i] = w;
-        param[i] = (T)w;
-    }
+__device__ __forceinline__ void move(const Common& c, const Matrix& t, int64_t i, float x, float keep, float rate) {
+    T* param = (T*)t.param + i;
+    const T old = *param;
+    float w = to_float(old);
+    float* copy = c.master && sizeof(T) == 2 ? c.master + t.at + i : NULL;
+    if (copy && to_float((T)*copy) == w) w = *copy;
+    w = w * keep - rate * x;
+    if (copy) *copy = w;
+    *param = (T)w;
 }
+
+/* Four waves, each with 64 x 64 of the tile.  A step of 32 of what is summed
+ * is fetched into registers while the one before is worked on, and goes to
+ * the other half of LDS. */
+template <Product KIND>
+__global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
+    constexpr bool kAcross = KIND == NEXT || KIND == LAST;      // the right side's rows are what is summed over
+    constexpr int kRow = kStep * 4 + 16, kAcrossRow = kTile * 4 + 32;      // bytes of a row in LDS, in different banks
+    constexpr int kSide = kTile * kRow, kLoads = kTile * kStep * 4 / 16 / kThreads;
+    static_assert(kStep * kAcrossRow <= kSide, "either side");
+    extern __shared__ __attribute__((aligned(16))) char shared[];
+    const Place p = l.c.places[l.c.first + by_die()];
+    const Matrix& t = l.c.matrices[p.matrix];
+    if (!l.c.live[p.matrix]) return;
+    const int64_t x = l.swapped ? t.next : t.x;
+    const int64_t left = KIND == GRAM ? x : KIND == POLYNOMIAL ? t.y : t.z, right = KIND == POLYNOMIAL ? t.y : x;
+    const int64_t sum = KIND == GRAM ? t.n : t.m;               // a row of the left side
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, g = lane / 16, c = lane % 16;
+    const int wi = wave / 2 * 64, wj = wave % 2 * 64;
+    const char* from_left = l.c.work + left * 4 + ((int64_t)p.i * kTile + tid / 8) * sum * 4 + tid % 8 * 16;
+    const char* from_right = l.c.work + right * 4
+        + (kAcross ? (int64_t)(tid / 32) * t.n * 4 + (int64_t)p.j * kTile * 4 + tid % 32 * 16
+                   : ((int64_t)p.j * kTile + tid / 8) * sum * 4 + tid % 8 * 16);
+    U4 a[kLoads], b[kLoads];
+    auto fetch = [&](int64_t k) {
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+            a[i] = *(const U4*)(from_left + i * 32 * sum * 4 + k * 4);
+            b[i] = kAcross ? *(const U4*)(from_right + (k + i * 8) * t.n * 4) : *(const U4*)(from_right + i * 32 * sum * 4 + k * 4);
+        }
+    };
+    auto put = [&](char* to) {
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+            *(U4*)(to + (tid / 8 + i * 32) * kRow + tid % 8 * 16) = a[i];
+            if (kAcross) *(U4*)(to + kSide + (tid / 32 + i * 8) * kAcrossRow + tid % 32 * 16) = b[i];
+            else *(U4*)(to + kSide + (tid / 8 + i * 32) * kRow + tid % 8 * 16) = b[i];
+        }
+    };
+    /* eight of what is summed to a lane: from 8 g on, or (across) from 4 g and from 16 + 4 g on */
+    auto row_of = [&](const char* at) {
+        if (!kAcross) return *(const H8*)(at + g * 16);
+        const H4 u = *(const H4*)(at + g * 8), v = *(const H4*)(at + g * 8 + 32);
+        return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    /* the hardware turns four elements of 16 lanes: lane 4 r + k fetches those of row r from 4 k on */
+    auto column_of = [&](const char* at) {
+        typedef __attribute__((address_space(3))) S4* Lds;
+        const char* q = at + (4 * g + c / 4) * kAcrossRow + c % 4 * 8;
+        const S4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)q);
+        const S4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(q + 16 * kAcrossRow));
+        return __builtin_bit_cast(H8, __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    F4 d[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) d[i][j] = F4{0, 0, 0, 0};
+    fetch(0);
+    put(shared);
+    __syncthreads();
+    int half = 0;
+#pragma unroll 1
+    for (int64_t k = 0; k < sum; k += kStep) {
+        const bool more = k + kStep < sum;
+        if (more) fetch(k + kStep);
+        const char* at = shared + half * 2 * kSide;
+        H8 lh[4], ll[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            lh[i] = row_of(at + (wi + 16 * i + c) * kRow);
+            ll[i] = row_of(at + (wi + 16 * i + c) * kRow + kStep * 2);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            H8 rh, rl;
+            if (kAcross) {
+                const char* q = at + kSide + (wj + 16 * j) / kStep * kStep * 4 + 16 * j % kStep * 2;
+                rh = column_of(q);
+                rl = column_of(q + kStep * 2);
+            } else {
+                rh = row_of(at + kSide + (wj + 16 * j + c) * kRow);
+                rl = row_of(at + kSide + (wj + 16 * j + c) * kRow + kStep * 2);
+            }
+            /* rows of the tile along the right side's: a lane has four neighbouring columns of one row of out */
+#pragma unroll
+            for (int i = 0; i < 4; i++) d[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rl, lh[i], d[i][j], 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; i++) d[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rh, ll[i], d[i][j], 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; i++) d[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rh, lh[i], d[i][j], 0, 0, 0);
+        }
+        half ^= 1;
+        if (more) put(shared + half * 2 * kSide);
+        __syncthreads();
+    }
+    const bool turned = t.rows > t.columns;
+    const float keep = (float)(1 - l.c.lr * t.decay), rate = (float)(l.c.lr * t.factor);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int64_t row = (int64_t)p.i * kTile + wi + 16 * i + c, col = (int64_t)p.j * kTile + wj + 16 * j + 4 * g;
+            F4 y;
+#pragma unroll
+            for (int r = 0; r < 4; r++) y[r] = d[i][j][r] * (1.0f / kScale);
+            if (KIND == LAST) {
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int64_t pr = turned ? col + r : row, pc = turned ? row : col + r;
+                    if (pr >= t.rows || pc >= t.columns) continue;
+                    const float v = y[r] * (1.0f / kScale);
+                    if (t.type == B3_F32) move<float>(l.c, t, pr * t.columns + pc, v, keep, rate);
+                    else if (t.type == B3_F16) move<_Float16>(l.c, t, pr * t.columns + pc, v, keep, rate);
+                    else move<__bf16>(l.c, t, pr * t.columns + pc, v, keep, rate);
+                }
+                continue;
+            }
+            const int64_t out = KIND == GRAM ? t.y : KIND == POLYNOMIAL ? t.z : l.swapped ? t.x : t.next;
+            const int64_t columns = KIND == NEXT ? t.n : t.m;
+            const int64_t block = col / kStep, o = col % kStep;
+            if (KIND == POLYNOMIAL) {
+                const _Float16* own = block_of(l.c.work, t.y, columns, row, block) + o;
+                const H4 h = *(const H4*)own, rest = *(const H4*)(own + kStep);
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    y[r] = __builtin_fmaf((float)kC, y[r], (float)kB * ((float)h[r] + (float)rest[r]));
+                    if (row == col + r) y[r] += (float)kA * kScale;
+                }
+            }
+            H4 h, rest;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                h[r] = (_Float16)y[r];
+                rest[r] = (_Float16)(y[r] - (float)h[r]);
+            }
+            _Float16* to = block_of(l.c.work, out, columns, row, block) + o;
+            *(H4*)to = h;
+            *(H4*)(to + kStep) = rest;
+            if (KIND != NEXT && p.i != p.j) {
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    _Float16* other = block_of(l.c.work, out, columns, col + r, row / kStep) + row % kStep;
+                    other[0] = h[r];
+                    other[kStep] = rest[r];
+                }
+            }
+        }
+}
+
+/* ---- launches ---- */
 
 bool valid(const B3MuonMatrix* matrices, int count) {
     if (count < 0 || (count && !matrices)) return false;
@@ -145,6 +408,34 @@ bool overlap(const B3MuonMatrix* matrices, int count, B3MuonMatrix* sorted) {
 
 int64_t segment(int64_t numel) { return ceil_div(numel, B3_ADAMW_SEGMENT) * B3_ADAMW_SEGMENT; }
 
+
+int batch(const B3Muon* o, int base) { return o->count - base < kBatch ? o->count - base : kBatch; }
+
+int64_t filled(int64_t n) { return ceil_div(n, kTile) * kTile; }
+
+/* Launches over places from `first` to `end`, which may be more than one takes. */
+template <typename F>
+hipError_t over(int64_t first, int64_t end, F launch) {
+    for (int64_t at = first; at < end; at += kMostBlocks)
+        launch(at, (unsigned)(end - at < kMostBlocks ? end - at : kMostBlocks));
+    return hipGetLastError();
+}
+
+template <Product KIND>
+hipError_t launch_product(ProductLaunch l, int64_t first, int64_t end, hipStream_t stream) {
+    constexpr int kLds = 4 * kTile * (kStep * 4 + 16);
+    return over(first, end, [&](int64_t at, unsigned blocks) {
+        l.c.first = at;
+        mu_product<KIND><<<blocks, kThreads, kLds, stream>>>(l);
+    });
+}
+
+template <Product KIND>
+hipError_t allow_lds() {
+    return hipFuncSetAttribute((const void*)mu_product<KIND>, hipFuncAttributeMaxDynamicSharedMemorySize,
+        4 * kTile * (kStep * 4 + 16));
+}
+
 }  // namespace
 }  // namespace b3p
 
@@ -162,13 +453,14 @@ int64_t b3_muon_size(const B3MuonMatrix* matrices, int count) {
 hipError_t b3_muon_destroy(B3Muon* o) {
     if (!o) return hipSuccess;
     hipError_t first = hipSuccess;
-    void* bufs[2] = {o->work, o->partial};
+    void* bufs[5] = {o->matrices, o->places, o->work, o->partial, o->live};
     for (void* p : bufs) {
         hipError_t err = p ? hipFree(p) : hipSuccess;
         if (first == hipSuccess) first = err;
     }
     free(o->given);
-    free(o->at);
+    free(o->first_part);
+    free(o->first_cut);
     free(o);
     return first;
 }
@@ -186,22 +478,82 @@ hipError_t b3_muon_create(B3Muon** out, const B3MuonMatrix* matrices, int count,
     o->config = config;
     o->state = state;
     o->given = (B3MuonMatrix*)calloc((size_t)count + 1, sizeof(B3MuonMatrix));
-    o->at = (int64_t*)calloc((size_t)count + 1, sizeof(int64_t));
-    hipError_t err = !(o->given && o->at) ? hipErrorOutOfMemory
+    o->first_part = (int64_t*)calloc((size_t)count + 1, sizeof(int64_t));
+    o->first_cut = (int64_t*)calloc((size_t)count + 1, sizeof(int64_t));
+    Matrix* table = (Matrix*)calloc((size_t)count + 1, sizeof(Matrix));
+    Place* places = NULL;
+    int64_t work = 0, partials = 0;
+    hipError_t err = !(o->given && o->first_part && o->first_cut && table) ? hipErrorOutOfMemory
         : overlap(matrices, count, o->given) ? hipErrorInvalidValue : hipGetDevice(&o->device);
     if (err == hipSuccess) {
-        int64_t at = 0;
+        int64_t at = 0, parts = 0, cuts = 0, halves = 0, tiles = 0;
         for (int i = 0; i < count; i++) {
-            const B3MuonMatrix& t = o->given[i] = matrices[i];
-            const int64_t m = t.rows < t.columns ? t.rows : t.columns;
-            o->at[i] = at;
-            at += segment(t.rows * t.columns);
-            if (t.rows * t.columns > o->most) o->most = t.rows * t.columns;
-            if (m * m > o->side) o->side = m * m;
+            const B3MuonMatrix& g = o->given[i] = matrices[i];
+            Matrix& t = table[i];
+            const int64_t numel = g.rows * g.columns, m = g.rows < g.columns ? g.rows : g.columns;
+            t.param = g.param;
+            t.rows = g.rows;
+            t.columns = g.columns;
+            t.at = at;
+            at += segment(numel);
+            t.type = g.type;
+            t.decay = g.weight_decay;
+            t.factor = g.rows > g.columns && g.columns ? sqrt((double)g.rows / (double)g.columns) : 1.0;
+            o->first_part[i] = parts;
+            o->first_cut[i] = cuts;
+            if (!numel) continue;
+            t.m = filled(m);
+            t.n = filled(numel / m);
+            t.x = work;
+            t.next = t.x + t.m * t.n;
+            t.y = t.next + t.m * t.n;
+            t.z = t.y + t.m * t.m;
+            work = t.z + t.m * t.m;
+            t.part = ceil_div(numel, kMostParts);
+            t.part = t.part < kPart ? kPart : t.part;
+            t.parts = (int)ceil_div(numel, t.part);
+            t.partial = partials;
+            partials += t.parts;
+            const int64_t mt = t.m / kTile, nt = t.n / kTile, per = kTile / kCut;
+            parts += t.parts;
+            cuts += mt * nt * per * per;
+            halves += mt * (mt + 1) / 2;
+            tiles += mt * nt;
         }
-        err = hipMalloc((void**)&o->work, (size_t)(2 * (o->most + o->side) + 1) * sizeof(float));
+        o->first_part[count] = parts;
+        o->first_cut[count] = cuts;
+        o->cuts = parts;
+        o->halves = o->cuts + cuts;
+        o->tiles = o->halves + halves;
+        o->end = o->tiles + tiles;
+        places = (Place*)malloc((size_t)(o->end + 1) * sizeof(Place));
+        if (!places) err = hipErrorOutOfMemory;
+        Place* to = places;
+        for (int i = 0; i < count && places; i++)
+            for (int k = 0; k < table[i].parts; k++) *to++ = Place{i, k, 0};
+        for (int i = 0; i < count && places; i++)
+            for (int64_t r = 0; r < table[i].m / kCut; r++)
+                for (int64_t c = 0; c < table[i].n / kCut; c++) *to++ = Place{i, (int)r, (int)c};
+        for (int i = 0; i < count && places; i++)
+            for (int64_t r = 0; r < table[i].m / kTile; r++)
+                for (int64_t c = 0; c <= r; c++) *to++ = Place{i, (int)r, (int)c};
+        for (int i = 0; i < count && places; i++)
+            for (int64_t r = 0; r < table[i].m / kTile; r++)
+                for (int64_t c = 0; c < table[i].n / kTile; c++) *to++ = Place{i, (int)r, (int)c};
     }
-    if (err == hipSuccess) err = hipMalloc((void**)&o->partial, kSumBlocks * sizeof(double));
+    if (err == hipSuccess) err = hipMalloc((void**)&o->matrices, ((size_t)count + 1) * sizeof(Matrix));
+    if (err == hipSuccess) err = hipMalloc((void**)&o->places, (size_t)(o->end + 1) * sizeof(Place));
+    if (err == hipSuccess) err = hipMalloc((void**)&o->work, (size_t)(work + 1) * 4);
+    if (err == hipSuccess) err = hipMalloc((void**)&o->partial, (size_t)(partials + 1) * sizeof(double));
+    if (err == hipSuccess) err = hipMalloc((void**)&o->live, ((size_t)count + 1) * sizeof(int));
+    if (err == hipSuccess) err = hipMemcpy(o->matrices, table, ((size_t)count + 1) * sizeof(Matrix), hipMemcpyHostToDevice);
+    if (err == hipSuccess) err = hipMemcpy(o->places, places, (size_t)o->end * sizeof(Place), hipMemcpyHostToDevice);
+    if (err == hipSuccess) err = allow_lds<GRAM>();
+    if (err == hipSuccess) err = allow_lds<POLYNOMIAL>();
+    if (err == hipSuccess) err = allow_lds<NEXT>();
+    if (err == hipSuccess) err = allow_lds<LAST>();
+    free(table);
+    free(places);
     if (err != hipSuccess) {
         (void)b3_muon_destroy(o);
         return err;
@@ -217,36 +569,46 @@ hipError_t b3_muon_step_gpu(B3Muon* o, const void* const* grads, const int* grad
     int device;
     hipError_t err = hipGetDevice(&device);
     if (err != hipSuccess || device != o->device) return err != hipSuccess ? err : hipErrorInvalidDevice;
-    for (int i = 0; i < o->count; i++) {
-        const B3MuonMatrix& t = o->given[i];
-        const int64_t numel = t.rows * t.columns, m = t.rows < t.columns ? t.rows : t.columns, n = numel ? numel / m : 0;
-        if (!grads[i] || !numel) continue;
-        float *x = o->work, *next = x + o->most, *y = next + o->most, *poly = y + o->side;
-        const int blocks = (int)(ceil_div(numel, kThreads) < kSumBlocks ? ceil_div(numel, kThreads) : kSumBlocks);
-        mu_momentum<<<blocks, kThreads, 0, stream>>>(grads[i], grad_types ? grad_types[i] : t.type,
-            o->state.momentum + o->at[i], t.rows, t.columns, (float)o->config.momentum, o->config.nesterov, x, o->partial);
-        mu_scale<<<blocks, kThreads, 0, stream>>>(x, numel, o->partial, blocks, (float)o->config.eps);
-        const unsigned gm = (unsigned)ceil_div(m, kTile), gn = (unsigned)ceil_div(n, kTile);
-        for (int s = 0; s < o->config.newton_schulz; s++) {
-            mu_product<true><<<dim3(gm, gm), kThreads, 0, stream>>>(x, x, NULL, y, m, m, n, 0, 1);
-            mu_product<false><<<dim3(gm, gm), kThreads, 0, stream>>>(y, y, y, poly, m, m, m, (float)kB, (float)kC);
-            mu_product<false><<<dim3(gn, gm), kThreads, 0, stream>>>(poly, x, x, next, m, n, m, (float)kA, 1);
-            float* swap = x;
-            x = next;
-            next = swap;
+    GradientLaunch l = {};
+    l.c.matrices = o->matrices;
+    l.c.places = o->places;
+    l.c.momentum = o->state.momentum;
+    l.c.master = o->state.master;
+    l.c.work = o->work;
+    l.c.partial = o->partial;
+    l.c.live = o->live;
+    l.c.keep = (float)o->config.momentum;
+    l.c.nesterov = o->config.nesterov;
+    l.c.eps = o->config.eps;
+    l.c.lr = lr;
+    for (int base = 0; base < o->count; base += kBatch) {
+        const int n = batch(o, base);
+        l.g.base = base;
+        for (int j = 0; j < n; j++) {
+            l.g.at[j] = grads[base + j];
+            l.g.type[j] = (uint8_t)(grad_types ? grad_types[base + j] : o->given[base + j].type);
         }
-        const float keep = (float)(1 - lr * t.weight_decay);
-        const float rate = (float)(lr * sqrt(t.rows > t.columns ? (double)t.rows / (double)t.columns : 1.0));
-        float* master = o->state.master ? o->state.master + o->at[i] : NULL;
-        if (t.type == B3_F32)
-            mu_update<float><<<blocks, kThreads, 0, stream>>>((float*)t.param, NULL, x, t.rows, t.columns, keep, rate);
-        else if (t.type == B3_F16)
-            mu_update<_Float16><<<blocks, kThreads, 0, stream>>>((_Float16*)t.param, master, x, t.rows, t.columns, keep, rate);
-        else
-            mu_update<__bf16><<<blocks, kThreads, 0, stream>>>((__bf16*)t.param, master, x, t.rows, t.columns, keep, rate);
-        if ((err = hipGetLastError()) != hipSuccess) return err;
+        err = over(o->first_part[base], o->first_part[base + n], [&](int64_t at, unsigned blocks) {
+            l.c.first = at;
+            mu_momentum<<<blocks, kThreads, 0, stream>>>(l);
+        });
+        if (err != hipSuccess) return err;
+        err = over(o->cuts + o->first_cut[base], o->cuts + o->first_cut[base + n], [&](int64_t at, unsigned blocks) {
+            l.c.first = at;
+            mu_split<<<blocks, kThreads, 0, stream>>>(l);
+        });
+        if (err != hipSuccess) return err;
     }
-    return hipSuccess;
+    ProductLaunch p = {l.c, false};
+    for (int s = 0; s < o->config.newton_schulz && err == hipSuccess; s++) {
+        err = launch_product<GRAM>(p, o->halves, o->tiles, stream);
+        if (err == hipSuccess) err = launch_product<POLYNOMIAL>(p, o->halves, o->tiles, stream);
+        if (err == hipSuccess)
+            err = s + 1 < o->config.newton_schulz ? launch_product<NEXT>(p, o->tiles, o->end, stream)
+                                                  : launch_product<LAST>(p, o->tiles, o->end, stream);
+        p.swapped = !p.swapped;
+    }
+    return err;
 }
 
 }  // extern "C"
