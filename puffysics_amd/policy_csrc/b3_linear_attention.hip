@@ -137,31 +137,52 @@ template <typename T, int COLS>
 struct Tile {
     typedef typename Math<T>::Lds Lds;
     static constexpr int kVec = 16 / sizeof(T), kRow = COLS + 16 / sizeof(Lds), kPlaces = Math<T>::kPlaces;
-    static constexpr int kPerRow = COLS / kVec, kAll = kPerRow * kPlaces, kLoads = (kAll + kWave - 1) / kWave;
+    static constexpr int kPerRow = COLS / kVec, kRows = kWave / kPerRow, kLoads = kPlaces / kRows;
     static constexpr int kBytes = kPlaces * kRow * sizeof(Lds);
+    static_assert(kWave % kPerRow == 0 && kPlaces % kRows == 0, "whole loads");
     U4 raw[kLoads];
 
-    static __device__ __forceinline__ bool mine(int l) { return kAll % kWave == 0 || l * kWave + (int)threadIdx.x % kWave < kAll; }
-    static __device__ __forceinline__ int row(int l) { return (l * kWave + (int)threadIdx.x % kWave) / kPerRow; }
-    static __device__ __forceinline__ int col(int l) { return (l * kWave + (int)threadIdx.x % kWave) % kPerRow * kVec; }
+    /* Vector l of a lane is of row(l), from col() on. */
+    static __device__ __forceinline__ int row(int l) { return l * kRows + (int)threadIdx.x % kWave / kPerRow; }
+    static __device__ __forceinline__ int col() { return (int)threadIdx.x % kPerRow * kVec; }
 
-    /* Columns from p on, of which there are `cols`; zeros beyond and in rows from `places` on. */
+    /* Columns from p on, of which there are `cols`; zeros beyond and in rows from
+     * `places` (at least 1) on.  What lies beyond is not fetched, but no branch of
+     * a lane's is taken for it, so that all loads are in flight together. */
     __device__ __forceinline__ void load(const T* p, int64_t stride, int places, int cols) {
+        const bool in = col() < cols;
+        if (cols % kVec == 0 && places == kPlaces) {
+            const T* at = p + row(0) * stride + (in ? col() : 0);
 #pragma unroll
-        for (int l = 0; l < kLoads; l++) {
-            raw[l] = U4{0, 0, 0, 0};
-            if (!mine(l) || row(l) >= places) continue;
-            const T* at = p + row(l) * stride + col(l);
-            const int left = cols - col(l);
-            if (left >= kVec) {
-                raw[l] = __builtin_bit_cast(U4, *(const Pack<T, kVec>*)at);
-            } else {
-                Pack<T, kVec> some = {};
+            for (int l = 0; l < kLoads; l++) raw[l] = __builtin_bit_cast(U4, *(const Pack<T, kVec>*)(at + l * (kRows * stride)));
+            if (cols < COLS) {
+#pragma unroll
+                for (int l = 0; l < kLoads; l++)
+                    if (!in) raw[l] = U4{0, 0, 0, 0};
+            }
+        } else {
+#pragma unroll
+            for (int l = 0; l < kLoads; l++) {
+                const T* at = p + (row(l) < places ? row(l) : places - 1) * stride;
+                Pack<T, kVec> x;
+                if (cols % kVec == 0) {
+                    x = *(const Pack<T, kVec>*)(at + (in ? col() : 0));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kVec; i++) x.v[i] = at[col() + i < cols ? col() + i : 0];
+                }
+#pragma unroll
                 for (int i = 0; i < kVec; i++)
-                    if (i < left) some.v[i] = at[i];
-                raw[l] = __builtin_bit_cast(U4, some);
+                    if (row(l) >= places || col() + i >= cols) x.v[i] = (T)0.0f;
+                raw[l] = __builtin_bit_cast(U4, x);
             }
         }
+    }
+
+    __device__ __forceinline__ void first_row_alone() {
+#pragma unroll
+        for (int l = 0; l < kLoads; l++)
+            if (row(l)) raw[l] = U4{0, 0, 0, 0};
     }
 
     /* Whether any element of the lane's is NaN or infinite. */
@@ -204,7 +225,7 @@ struct Tile {
     __device__ __forceinline__ void store(Lds* lds) const {
 #pragma unroll
         for (int l = 0; l < kLoads; l++)
-            if (mine(l)) put(lds, row(l), col(l), raw[l]);
+            put(lds, row(l), col(), raw[l]);
     }
 };
 
@@ -281,20 +302,6 @@ struct Walk {
         T* out = (T*)m.out + from * m.out_stride[0] + u.env * m.out_stride[1] + u.head * m.out_stride[2] + u.first;
         const int value = m.value - u.first < VD ? m.value - u.first : VD;
 
-        /* E, lane (g, c) of tile [kb][vb] rows 16 kb + 4 g + r and the column of c */
-        F4 state[KB][VB];
-        const float first = early ? power(l2, 1) : 1.0f;
-#pragma unroll
-        for (int kb = 0; kb < KB; kb++)
-#pragma unroll
-            for (int vb = 0; vb < VB; vb++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int row = kb * 16 + 4 * g + r, col = value_col(vb) + kStep * (c / 4) + c % 4;
-                    const bool in = enter && row < m.key && col < value;
-                    state[kb][vb][r] = in ? first * enter[row * m.state_row + (u.first + col) * m.state_col] : 0.0f;
-                }
-
         /* weights of scores (of the tiles i = j and i = j + 16), of the state for place i, and of places for the state */
         const float gain = m.reach * m.update;
         F4 near[R];
@@ -312,38 +319,91 @@ struct Walk {
         float pass = 0;
         int weighted = -1;                       // places and the step less that keep and pass are for
 
-        KeyTile tq, tk;
+        KeyTile tk, tq;
         ValueTile tv;
         uint32_t flag = 0;
         bool dropped = false;
-        auto fetch = [&](int64_t p, int most) {
-            const int n = places - p < most ? (int)(places - p) : most;
+        auto fetch = [&](int64_t p) {
+            const int n = places - p < kPlaces ? (int)(places - p) : kPlaces;
             tk.load(k + p * m.k_stride[0], m.k_stride[0], n, m.key);
             tv.load(v + p * m.v_stride[0], m.v_stride[0], n, value);
             if (!STATE) tq.load(q + p * m.q_stride[0], m.q_stride[0], n, m.key);
-            flag = 0;
-            if (m.starts && lane < n && (from + p + lane || m.forward))
-                flag = started(m.starts + (from + p + lane) * m.starts_stride[0] + u.env * m.starts_stride[1], j.starts_type);
+            if (m.starts) {
+                /* the first place on the way back has none: a later one's is fetched, and dropped */
+                const int at = lane < n ? lane : n - 1, none = from + p == 0 && !m.forward ? 1 : 0;
+                if (n > none)
+                    flag = started(m.starts + (from + p + (at > none ? at : none)) * m.starts_stride[0] + u.env * m.starts_stride[1],
+                        j.starts_type) && lane < n && lane >= none;
+                else
+                    flag = 0;
+            }
         };
-        if (places > 0) fetch(0, kPlaces);
+        if (places > 0) fetch(0);
+        /* E, lane (g, c) of tile [kb][vb] rows 16 kb + 4 g + r and the column of c */
+        F4 state[KB][VB];
+        const float first = early ? power(l2, 1) : 1.0f;
+        const int state_row = (int)m.state_row, state_col = (int)m.state_col;
+        if (enter) {
+            const float* at[VB];
+#pragma unroll
+            for (int vb = 0; vb < VB; vb++) {
+                const int col = value_col(vb) + kStep * (c / 4) + c % 4;
+                at[vb] = enter + (u.first + (col < value ? col : 0)) * state_col;
+            }
+            if (state_row == 1 && m.key % 4 == 0) {
+#pragma unroll
+                for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                    for (int vb = 0; vb < VB; vb++) {
+                        const int row = kb * 16 + 4 * g;
+                        state[kb][vb] = __builtin_bit_cast(F4, *(const Pack<float, 4>*)(at[vb] + (row < m.key ? row : 0)));
+                    }
+            } else {
+#pragma unroll
+                for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int row = kb * 16 + 4 * g + r, offset = (row < m.key ? row : 0) * state_row;
+#pragma unroll
+                        for (int vb = 0; vb < VB; vb++) state[kb][vb][r] = at[vb][offset];
+                    }
+            }
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                for (int vb = 0; vb < VB; vb++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int row = kb * 16 + 4 * g + r, col = value_col(vb) + kStep * (c / 4) + c % 4;
+                        state[kb][vb][r] = row < m.key && col < value ? first * state[kb][vb][r] : 0.0f;
+                    }
+        } else {
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                for (int vb = 0; vb < VB; vb++) state[kb][vb] = F4{0, 0, 0, 0};
+        }
+
         int n;
 #pragma unroll 1
         for (int64_t p = 0; p < places; p += n) {
             n = places - p < kPlaces ? (int)(places - p) : kPlaces;
             /* A product with a weight of 0 would carry what is not finite in v to other places: such
              * a place is a chunk by itself. */
-            if (__ballot(tv.bad()) && n > 1) {
+            if (n > 1 && __ballot(tv.bad())) {
                 n = 1;
-                fetch(p, 1);
+                tk.first_row_alone();
+                tv.first_row_alone();
+                if (!STATE) tq.first_row_alone();
             }
-            const uint32_t starts = (uint32_t)__ballot(flag != 0);
+            const uint32_t starts = (uint32_t)__ballot(flag != 0 && lane < n);
             wave_fence();
             tk.store(lk);
             tv.store(lv);
             if (!STATE) tq.store(lq);
             wave_fence();
             const bool end = p + n >= places;
-            if (!end) fetch(p + n, kPlaces);
+            if (!end) fetch(p + n);
             const int less = end && m.forward && from + places == j.steps ? 1 : 0;
             if (weighted != 2 * n + less) {
                 weighted = 2 * n + less;
