@@ -323,6 +323,7 @@ struct Walk {
         ValueTile tv;
         uint32_t flag = 0;
         bool dropped = false;
+        float scale = 1.0f;                      // of the state
         auto fetch = [&](int64_t p) {
             const int n = places - p < kPlaces ? (int)(places - p) : kPlaces;
             tk.load(k + p * m.k_stride[0], m.k_stride[0], n, m.key);
@@ -388,9 +389,9 @@ struct Walk {
 #pragma unroll 1
         for (int64_t p = 0; p < places; p += n) {
             n = places - p < kPlaces ? (int)(places - p) : kPlaces;
-            /* A product with a weight of 0 would carry what is not finite in v to other places: such
-             * a place is a chunk by itself. */
-            if (n > 1 && __ballot(tv.bad())) {
+            /* A product with a weight of 0 would carry what is not finite in k or v to other places:
+             * such a place is a chunk by itself. */
+            if (n > 1 && __ballot(tk.bad() || tv.bad())) {
                 n = 1;
                 tk.first_row_alone();
                 tv.first_row_alone();
@@ -442,10 +443,9 @@ struct Walk {
                             const S4 h0 = round4(state[kb][vb]), h1 = round4(state[kb + 1][vb]);
                             const S4 l0 = rest4(state[kb][vb], h0), l1 = rest4(state[kb + 1][vb], h1);
 #pragma unroll
-                            for (int t = 0; t < R; t++) {
-                                o[t][vb] = multiply(h0, h1, qq[t][kb], qq[t][kb + 1], o[t][vb]);
-                                o[t][vb] = multiply(l0, l1, qq[t][kb], qq[t][kb + 1], o[t][vb]);
-                            }
+                            for (int t = 0; t < R; t++) o[t][vb] = multiply(l0, l1, qq[t][kb], qq[t][kb + 1], o[t][vb]);
+#pragma unroll
+                            for (int t = 0; t < R; t++) o[t][vb] = multiply(h0, h1, qq[t][kb], qq[t][kb + 1], o[t][vb]);
                         }
                     } else {
 #pragma unroll
@@ -460,10 +460,16 @@ struct Walk {
                 for (int t = 0; t < R; t++) {
                     const uint32_t before = starts & (uint32_t)((2ull << (16 * t + c)) - 1);
                     since[t] = before ? 31 - __builtin_clz(before) : -1;
+                    const float f = reach[t] * scale;
 #pragma unroll
-                    for (int vb = 0; vb < VB; vb++)
+                    for (int vb = 0; vb < VB; vb++) o[t][vb] *= f;
+                }
+                if (starts) {
 #pragma unroll
-                        for (int r = 0; r < 4; r++) o[t][vb][r] = since[t] < 0 ? o[t][vb][r] * reach[t] : 0.0f;
+                    for (int t = 0; t < R; t++)
+#pragma unroll
+                        for (int vb = 0; vb < VB; vb++)
+                            if (since[t] >= 0) o[t][vb] = F4{0, 0, 0, 0};
                 }
                 /* scores, rows j and columns i; they are what P v sums over as they lie */
                 Quad score[R][R];
@@ -522,35 +528,59 @@ struct Walk {
                     }
                 }
             }
-            /* what is kept of the state, and of the places from the last start on */
-            const bool drop = starts != 0;
-            dropped |= drop;
-            const int last = drop ? 31 - __builtin_clz(starts) : -1;
+            /* What is kept of the state, and of the places from the last start on.  The state is
+             * held as E / scale, so that no chunk has to go over it: its decay goes into scale and,
+             * before that becomes small, into the state. */
+            const int last = starts ? 31 - __builtin_clz(starts) : -1;
+            if (starts) {
+                dropped = true;
+                scale = 1.0f;
 #pragma unroll
-            for (int kb = 0; kb < KB; kb++) {
-                F4 kw[R];
+                for (int kb = 0; kb < KB; kb++)
 #pragma unroll
-                for (int t = 0; t < R; t++) {
-                    const Quad x = across<kKeyRow, 4>(lk, 16 * t, 16 * kb);
-                    if constexpr (kHalf) kw[t] = __builtin_convertvector(__builtin_bit_cast(B4, x), F4);
-                    else kw[t] = x;
+                    for (int vb = 0; vb < VB; vb++) state[kb][vb] = F4{0, 0, 0, 0};
+            } else if (scale * pass > 0x1p-20f) {
+                scale *= pass;
+            } else {
+                const float f = scale * pass;
+                scale = 1.0f;
 #pragma unroll
-                    for (int r = 0; r < 4; r++) kw[t][r] = 16 * t + 4 * g + r >= last ? kw[t][r] * keep[t][r] : 0.0f;
-                }
+                for (int kb = 0; kb < KB; kb++)
 #pragma unroll
-                for (int vb = 0; vb < VB; vb++)
+                    for (int vb = 0; vb < VB; vb++) state[kb][vb] *= f;
+            }
+            const float over = 1.0f / scale;
+            F4 weight[R];
 #pragma unroll
-                    for (int r = 0; r < 4; r++) state[kb][vb][r] = drop ? 0.0f : state[kb][vb][r] * pass;
-                if constexpr (kHalf) {
-                    const S4 h0 = round4(kw[0]), h1 = round4(kw[1]), l0 = rest4(kw[0], h0), l1 = rest4(kw[1], h1);
+            for (int t = 0; t < R; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) weight[t][r] = 16 * t + 4 * g + r >= last ? keep[t][r] * over : 0.0f;
+            if constexpr (kHalf) {
+                S4 h[R][VB], rest[R][VB];        // weighted v as two numbers
+#pragma unroll
+                for (int t = 0; t < R; t++)
 #pragma unroll
                     for (int vb = 0; vb < VB; vb++) {
-                        state[kb][vb] = multiply(h0, h1, vq[0][vb], vq[1][vb], state[kb][vb]);
-                        state[kb][vb] = multiply(l0, l1, vq[0][vb], vq[1][vb], state[kb][vb]);
+                        const F4 x = weight[t] * __builtin_convertvector(__builtin_bit_cast(B4, vq[t][vb]), F4);
+                        h[t][vb] = round4(x);
+                        rest[t][vb] = rest4(x, h[t][vb]);
                     }
-                } else {
 #pragma unroll
-                    for (int vb = 0; vb < VB; vb++) state[kb][vb] = multiply(kw[0], vq[0][vb], state[kb][vb]);
+                for (int kb = 0; kb < KB; kb++) {
+                    const S4 k0 = across<kKeyRow, 4>(lk, 0, 16 * kb), k1 = across<kKeyRow, 4>(lk, 16, 16 * kb);
+#pragma unroll
+                    for (int vb = 0; vb < VB; vb++) state[kb][vb] = multiply(k0, k1, rest[0][vb], rest[1][vb], state[kb][vb]);
+#pragma unroll
+                    for (int vb = 0; vb < VB; vb++) state[kb][vb] = multiply(k0, k1, h[0][vb], h[1][vb], state[kb][vb]);
+                }
+            } else {
+#pragma unroll
+                for (int vb = 0; vb < VB; vb++) vq[0][vb] *= weight[0];
+#pragma unroll
+                for (int kb = 0; kb < KB; kb++) {
+                    const F4 x = across<kKeyRow, 4>(lk, 0, 16 * kb);
+#pragma unroll
+                    for (int vb = 0; vb < VB; vb++) state[kb][vb] = multiply(x, vq[0][vb], state[kb][vb]);
                 }
             }
         }
@@ -566,7 +596,7 @@ struct Walk {
                 for (int r = 0; r < 4; r++) {
                     const int row = kb * 16 + 4 * g + r, col = value_col(vb) + kStep * (c / 4) + c % 4;
                     if (row < m.key && col < value)
-                        leave[row * m.state_row + (u.first + col) * m.state_col] = gone ? 0.0f : state[kb][vb][r];
+                        leave[row * m.state_row + (u.first + col) * m.state_col] = gone ? 0.0f : scale * state[kb][vb][r];
                 }
     }
 };
@@ -575,7 +605,7 @@ struct Walk {
  * of a sequence) or lie side by side in memory (heads).  Workgroups go to the
  * 8 dies in turn: each die's take neighbouring ones. */
 template <typename T, int KD, int VD, bool STATE>
-__global__ __launch_bounds__(kThreads, KD * VD <= 64 * 64 ? 2 : 1) void la_walk(Job j) {
+__global__ __launch_bounds__(kThreads, 2) void la_walk(Job j) {
     extern __shared__ __attribute__((aligned(16))) char shared[];
     typedef Walk<T, KD, VD, STATE> W;
     const unsigned die = blockIdx.x % 8, share = gridDim.x / 8, rest = gridDim.x % 8;
@@ -779,7 +809,9 @@ Mix backwards(const B3Attention& g, const float* d_last) {
 }
 
 int columns_of(int dims) { return dims <= 32 ? 32 : dims <= 64 ? 64 : 128; }
-int part_of(int value) { return value <= 32 ? 32 : 64; }
+/* The state is at most 64 of a lane's registers, so that two waves fit a SIMD: one reads two histories of
+ * 65,536 steps and 8 heads of 128 in 783 us with 128, two in 380 with 64. */
+int part_of(int key, int value) { return value <= 32 || key > 64 ? 32 : 64; }
 int places_of(int type) { return type == B3_BF16 ? 32 : 16; }
 
 /* How the work is cut: into parts of v's columns and, where that leaves
@@ -793,7 +825,7 @@ Plan plan_of(const B3Attention& g, bool backward) {
     Plan p;
     const int most = g.key > g.value ? g.key : g.value;
     p.key = columns_of(backward ? most : g.key);
-    p.value = part_of(backward ? most : g.value);
+    p.value = part_of(backward ? most : g.key, backward ? most : g.value);
     p.parts = (int)ceil_div(backward ? most : g.value, p.value);
     const int64_t units = g.envs * g.heads * p.parts * (backward ? kRoles : 1);
     const int64_t chunk = places_of(g.type), most_pieces = g.steps / (chunk * kPieceChunks);
@@ -832,11 +864,9 @@ hipError_t launch(const Job& j, hipStream_t stream) {
 
 template <typename T, bool STATE>
 hipError_t launch_columns(const Job& j, const Plan& p, hipStream_t stream) {
-    if (p.value == 32)
-        return p.key == 32 ? launch<T, 32, 32, STATE>(j, stream) : p.key == 64 ? launch<T, 64, 32, STATE>(j, stream)
-                                                                            : launch<T, 128, 32, STATE>(j, stream);
-    return p.key == 32 ? launch<T, 32, 64, STATE>(j, stream) : p.key == 64 ? launch<T, 64, 64, STATE>(j, stream)
-                                                                           : launch<T, 128, 64, STATE>(j, stream);
+    if (p.key == 128) return launch<T, 128, 32, STATE>(j, stream);
+    if (p.value == 32) return p.key == 32 ? launch<T, 32, 32, STATE>(j, stream) : launch<T, 64, 32, STATE>(j, stream);
+    return p.key == 32 ? launch<T, 32, 64, STATE>(j, stream) : launch<T, 64, 64, STATE>(j, stream);
 }
 
 /* `ways`: what of the job's mixes learns the pieces' states, one for each. */
