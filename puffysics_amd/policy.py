@@ -16,6 +16,7 @@ import ctypes as C
 import math
 import operator
 import os
+import struct
 
 import torch
 from torch.autograd import forward_ad
@@ -80,6 +81,12 @@ class B3Norm(C.Structure):
                 ("residual_stride", _ll), ("weight", _vp), ("weight_type", _i), ("eps", _d)]
 
 
+# the same, packed: a structure of many fields takes 5 us to fill, as long as a small kernel runs
+_ATTENTION = struct.Struct("@3q3i4x3P9q2Pi4x2qPd")
+_NORM = struct.Struct("@2qi4xPqPqPi4xd")
+assert _ATTENTION.size == C.sizeof(B3Attention) and _NORM.size == C.sizeof(B3Norm)
+
+
 class B3MuonMatrix(C.Structure):
     _fields_ = [("param", _vp), ("type", _i), ("rows", _ll), ("columns", _ll), ("weight_decay", _d)]
 
@@ -106,16 +113,16 @@ POLICY_SYMBOLS = [
     ("b3_adamw_moments_gpu", _i, [_vp, _vp, _vp, _vp]),
     ("b3_adamw_load_moments_gpu", _i, [_vp, _vp, _vp, _vp]),
     ("b3_adamw_destroy", _i, [_vp]),
-    ("b3_linear_attention_workspace", _sz, [C.POINTER(B3Attention), _i]),
-    ("b3_linear_attention_gpu", _i, [C.POINTER(B3Attention), _vp, _vp, _vp, _sz, _vp]),
-    ("b3_linear_attention_backward_gpu", _i, [C.POINTER(B3Attention), _vp, _ll * 3, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
+    ("b3_linear_attention_workspace", _sz, [_vp, _i]),
+    ("b3_linear_attention_gpu", _i, [_vp, _vp, _vp, _vp, _sz, _vp]),
+    ("b3_linear_attention_backward_gpu", _i, [_vp, _vp, _ll * 3, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
                                               _vp]),
-    ("b3_linear_attention_step_gpu", _i, [C.POINTER(B3Attention), _vp, _vp, _vp]),
-    ("b3_rms_norm_gpu", _i, [C.POINTER(B3Norm), _vp, _vp, _vp, _vp]),
-    ("b3_rms_norm_8bit_gpu", _i, [C.POINTER(B3Norm), _vp, _vp, _vp, _vp]),
+    ("b3_linear_attention_step_gpu", _i, [_vp, _vp, _vp, _vp]),
+    ("b3_rms_norm_gpu", _i, [_vp, _vp, _vp, _vp, _vp]),
+    ("b3_rms_norm_8bit_gpu", _i, [_vp, _vp, _vp, _vp, _vp]),
     ("b3_values_of_8bit_gpu", _i, [_ll, _ll, _vp, _vp, _vp, _i, _vp]),
     ("b3_rms_norm_backward_workspace", _sz, [_ll, _ll]),
-    ("b3_rms_norm_backward_gpu", _i, [C.POINTER(B3Norm), _vp, _vp, _ll, _vp, _ll, _vp, _vp, _vp, _sz, _vp]),
+    ("b3_rms_norm_backward_gpu", _i, [_vp, _vp, _vp, _ll, _vp, _ll, _vp, _vp, _vp, _sz, _vp]),
     ("b3_muon_size", _ll, [C.POINTER(B3MuonMatrix), _i]),
     ("b3_muon_create", _i, [C.POINTER(_vp), C.POINTER(B3MuonMatrix), _i, B3MuonState, B3MuonConfig]),
     ("b3_muon_step_gpu", _i, [_vp, _vp, _vp, _d, _vp]),
@@ -365,18 +372,24 @@ LinearAttention = collections.namedtuple("LinearAttention", "out state")
 
 
 def _heads(x):
-    """x, or a copy of it, with contiguous heads."""
+    """x as it is read, or a copy of it with contiguous heads."""
+    if x.is_neg():
+        x = x.resolve_neg()
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
-def _attention(q, k, v, decay, state, starts, scale):
-    """B3Attention of q, k [steps, envs, heads, key], v [.., value]."""
-    steps, envs, heads, key = q.shape
-    return B3Attention(steps, envs, heads, key, v.shape[-1], _TYPE[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                       q.stride()[:3], k.stride()[:3], v.stride()[:3], decay.data_ptr(),
-                       None if starts is None else starts.data_ptr(),
-                       _F32 if starts is not None and starts.dtype == torch.float32 else _U8,
-                       (0, 0) if starts is None else starts.stride(), None if state is None else state.data_ptr(), scale)
+def _attention(steps, q, k, v, decay, state, starts, scale):
+    """B3Attention, packed, of q, k [steps, envs, heads, key], v [.., value], or of
+    one step's without the first axis."""
+    envs, heads, key = q.shape[-3:]
+    first = () if q.dim() == 4 else (0,)
+    # the heads' elements are contiguous: strides to them are 1 and left out
+    strides = (*first, *q.stride()[:-1], *first, *k.stride()[:-1], *first, *v.stride()[:-1])
+    at, kind, by = (0, _U8, (0, 0)) if starts is None else (
+        starts.data_ptr(), _F32 if starts.dtype == torch.float32 else _U8, (*first, *starts.stride()))
+    return _ATTENTION.pack(steps, envs, heads, key, v.shape[-1], _TYPE[q.dtype], q.data_ptr(), k.data_ptr(),
+                           v.data_ptr(), *strides, decay.data_ptr(), at, kind, *by,
+                           0 if state is None else state.data_ptr(), scale)
 
 
 def _work(size, device):
@@ -390,13 +403,13 @@ def _address_of(x):
 def _attend(q, k, v, decay, state, starts, scale, last):
     """(out, state after the last step or None)"""
     lib = policy_lib()
-    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    out = torch.empty_like(v, memory_format=torch.contiguous_format)
     left = torch.empty((*q.shape[1:], v.shape[-1]), dtype=torch.float32, device=v.device) if last else None
-    g = _attention(q, k, v, decay, state, starts, scale)
-    size = lib.b3_linear_attention_workspace(C.byref(g), 0)
+    g = _attention(q.shape[0], q, k, v, decay, state, starts, scale)
+    size = lib.b3_linear_attention_workspace(g, 0)
     work = _work(size, v.device)
     _check("b3_linear_attention_gpu", lib.b3_linear_attention_gpu(
-        C.byref(g), out.data_ptr(), _address_of(left), _address_of(work), size, _stream()))
+        g, out.data_ptr(), _address_of(left), _address_of(work), size, _stream()))
     return out, left
 
 
@@ -418,16 +431,16 @@ class _LinearAttention(torch.autograd.Function):
 def _attention_backward(ctx, d_out, d_left):
     q, k, v, decay, state, starts = ctx.saved_tensors
     lib = policy_lib()
-    d_out = torch.zeros_like(v) if d_out is None else _heads(_as_read(d_out))
+    d_out = torch.zeros_like(v) if d_out is None else _heads(d_out)
     d_left = None if d_left is None else _as_read(d_left).contiguous()
     new = lambda wanted, like, dtype: torch.empty(like.shape, dtype=dtype, device=v.device) if wanted else None  # noqa: E731
     d_q, d_k, d_v, d_state = (new(ctx.needs_input_grad[i], x, v.dtype if i < 3 else torch.float32)
                               for i, x in ((0, q), (1, k), (2, v), (4, state)))
-    g = _attention(q, k, v, decay, state, starts, ctx.scale)
-    size = lib.b3_linear_attention_workspace(C.byref(g), 1)
+    g = _attention(q.shape[0], q, k, v, decay, state, starts, ctx.scale)
+    size = lib.b3_linear_attention_workspace(g, 1)
     work = _work(size, v.device)
     _check("b3_linear_attention_backward_gpu", lib.b3_linear_attention_backward_gpu(
-        C.byref(g), d_out.data_ptr(), (_ll * 3)(*d_out.stride()[:3]), _address_of(d_left), _address_of(d_q),
+        g, d_out.data_ptr(), (_ll * 3)(*d_out.stride()[:3]), _address_of(d_left), _address_of(d_q),
         _address_of(d_k), _address_of(d_v), _address_of(d_state), _address_of(work), size, _stream()))
     return d_q, d_k, d_v, None, d_state, None, None, None
 
@@ -436,18 +449,19 @@ _attention_backward_once = torch.autograd.function.once_differentiable(_attentio
 
 
 def _check_attention(q, k, v, decay, starts, scale):
-    _need(q.dtype in _TYPE and k.dtype == q.dtype and v.dtype == q.dtype,
+    shape, dtype, last = q.shape, q.dtype, v.shape[-1]
+    _need(dtype in _TYPE and k.dtype is dtype and v.dtype is dtype,
           "q, k and v have to be float32, float16 or bfloat16, all of one type")
-    _need(k.shape == q.shape and v.shape[:-1] == q.shape[:-1], "q and k need one shape, v the same but for the last axis")
-    _need(1 <= q.shape[-1] <= MAX_HEAD and 1 <= v.shape[-1] <= MAX_HEAD, "a head has 1 to 128 dimensions")
-    envs, heads = q.shape[-3:-1]
-    _need(decay.dtype == torch.float32 and decay.shape == (heads,), "decay has to be float32 [heads]")
+    _need(k.shape == shape and v.shape == (*shape[:-1], last), "q and k need one shape, v the same but for the last axis")
+    _need(1 <= shape[-1] <= MAX_HEAD and 1 <= last <= MAX_HEAD, "a head has 1 to 128 dimensions")
+    _need(decay.dtype == torch.float32 and decay.dim() == 1 and decay.shape[0] == shape[-2], "decay has to be float32 [heads]")
     _need(not decay.requires_grad, "decay has no gradient")
-    _need(envs * heads <= MAX_SEQUENCES and (q.dim() == 3 or q.shape[0] <= MAX_ROWS),
-          "at most 2^24 - 1 sequences (environments times heads) and 2^31 - 1 steps")
+    if shape[-3] * shape[-2] > MAX_SEQUENCES or (len(shape) == 4 and shape[0] > MAX_ROWS):
+        raise ValueError("at most 2^24 - 1 sequences (environments times heads) and 2^31 - 1 steps")
+    if starts is not None:
+        _need(starts.shape == shape[:-2] and starts.dtype in (torch.float32, torch.bool, torch.uint8),
+              "starts have to be float32, bool or uint8, one for each step and environment")
     _need(math.isfinite(scale), "scale has to be a finite number")
-    _need(starts is None or (starts.shape == q.shape[:-2] and starts.dtype in (torch.float32, torch.bool, torch.uint8)),
-          "starts have to be float32, bool or uint8, one for each step and environment")
 
 
 def linear_attention(q, k, v, decay, state=None, starts=None, scale=1.0, last=False):
@@ -476,10 +490,7 @@ def linear_attention(q, k, v, decay, state=None, starts=None, scale=1.0, last=Fa
               "state has to be float32 [envs, heads, key, value]")
     _no_tangent("linear_attention", q, k, v, state)
     _on(q, k, v, decay, state, starts)
-    q, k, v = (_heads(_as_read(x)) for x in (q, k, v))
-    decay = _as_read(decay).contiguous()
-    if starts is not None:
-        starts = _as_read(starts)
+    q, k, v, decay, starts = _heads(q), _heads(k), _heads(v), _as_read(decay).contiguous(), _as_read(starts)
     if state is not None:
         state = _as_read(state).contiguous()
     if _needs_grad(q, k, v, state):
@@ -500,14 +511,10 @@ def linear_attention_step(q, k, v, decay, state, starts=None, scale=1.0):
         raise ValueError("linear_attention_step has no gradient")
     _no_tangent("linear_attention_step", q, k, v, state)
     _on(q, k, v, decay, state, starts)
-    q, k, v = (_heads(_as_read(x)) for x in (q, k, v))
-    decay = _as_read(decay).contiguous()
-    if starts is not None:
-        starts = _as_read(starts)[None]
-    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-    g = _attention(q[None], k[None], v[None], decay, None, starts, scale)
+    q, k, v, decay, starts = _heads(q), _heads(k), _heads(v), _as_read(decay).contiguous(), _as_read(starts)
+    out = torch.empty_like(v, memory_format=torch.contiguous_format)
     _check("b3_linear_attention_step_gpu", policy_lib().b3_linear_attention_step_gpu(
-        C.byref(g), state.data_ptr(), out.data_ptr(), _stream()))
+        _attention(1, q, k, v, decay, None, starts, scale), state.data_ptr(), out.data_ptr(), _stream()))
     _written(state)
     return out
 
@@ -525,22 +532,22 @@ RmsNorm8 = collections.namedtuple("RmsNorm8", "out scale sum")
 
 
 def _norm(x, residual, weight, eps):
-    """B3Norm of x, residual [rows, width]."""
+    """B3Norm, packed, of x, residual [rows, width]."""
     rows, width = x.shape
-    stride = lambda y: y.stride(0) if rows > 1 else width  # noqa: E731
-    return B3Norm(rows, width, _TYPE[x.dtype], x.data_ptr(), stride(x), _address_of(residual),
-                  0 if residual is None else stride(residual), _address_of(weight),
-                  0 if weight is None else _TYPE[weight.dtype], eps)
+    # the stride of a lone row says nothing
+    return _NORM.pack(rows, width, _TYPE[x.dtype], x.data_ptr(), x.stride(0) if rows > 1 else width,
+                      0 if residual is None else residual.data_ptr(),
+                      0 if residual is None else residual.stride(0) if rows > 1 else width,
+                      0 if weight is None else weight.data_ptr(), 0 if weight is None else _TYPE[weight.dtype], eps)
 
 
 def _normalise(x, weight, residual, eps, kept):
     """(out, sum or None, root or None), the last only where `kept`."""
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
     total = None if residual is None else torch.empty_like(out)
     root = torch.empty(x.shape[0], dtype=torch.float32, device=x.device) if kept else None
-    g = _norm(x, residual, weight, eps)
     _check("b3_rms_norm_gpu", policy_lib().b3_rms_norm_gpu(
-        C.byref(g), out.data_ptr(), _address_of(total), _address_of(root), _stream()))
+        _norm(x, residual, weight, eps), out.data_ptr(), _address_of(total), _address_of(root), _stream()))
     return out, total, root
 
 
@@ -572,9 +579,8 @@ def _norm_backward(ctx, d_out, d_sum):
     d_weight = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
     size = lib.b3_rms_norm_backward_workspace(rows, width)
     work = _work(size, x.device)
-    g = _norm(x, residual, weight, 0.0)
     _check("b3_rms_norm_backward_gpu", lib.b3_rms_norm_backward_gpu(
-        C.byref(g), root.data_ptr(), _address_of(d_out), stride(d_out), _address_of(d_sum), stride(d_sum), d_x.data_ptr(),
+        _norm(x, residual, weight, 0.0), root.data_ptr(), _address_of(d_out), stride(d_out), _address_of(d_sum), stride(d_sum), d_x.data_ptr(),
         _address_of(d_weight), _address_of(work), size, _stream()))
     # one tensor for both, as a sum's gradient is: views of it would become the grad of two leaves
     d_x = d_x.view(shape)
@@ -585,19 +591,25 @@ _norm_backward_once = torch.autograd.function.once_differentiable(_norm_backward
 
 
 def _check_norm(x, weight, residual, eps):
-    _need(x.dtype in _TYPE, "x has to be float32, float16 or bfloat16")
-    _need(x.dim() >= 1 and 1 <= x.shape[-1] <= MAX_WIDTH, "x needs rows of 1 to 2^21 elements")
-    _need(x.numel() // x.shape[-1] <= MAX_ROWS, "at most 2^31 - 1 rows")
-    _need(residual is None or (residual.shape == x.shape and residual.dtype == x.dtype),
+    shape, dtype = x.shape, x.dtype
+    _need(dtype in _TYPE, "x has to be float32, float16 or bfloat16")
+    _need(len(shape) >= 1 and 1 <= shape[-1] <= MAX_WIDTH, "x needs rows of 1 to 2^21 elements")
+    if x.numel() > MAX_ROWS * shape[-1]:
+        raise ValueError("at most 2^31 - 1 rows")
+    _need(residual is None or (residual.shape == shape and residual.dtype is dtype),
           "residual has to have the shape and type of x")
-    _need(weight is None or (weight.shape == x.shape[-1:] and weight.dtype in (x.dtype, torch.float32)),
+    _need(weight is None or (weight.shape == shape[-1:] and weight.dtype in (dtype, torch.float32)),
           "weight has to be a row, of the type of x or float32")
     _need(eps >= 0, "eps has to be at least 0")
 
 
 def _as_rows(x):
     """x as contiguous rows that do not overlap, or None."""
-    return None if x is None else _rows(_as_read(x).reshape(-1, x.shape[-1]))
+    if x is None:
+        return None
+    if x.is_neg():
+        x = x.resolve_neg()
+    return _rows(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
 
 
 def rms_norm(x, weight=None, residual=None, eps=1e-6):
@@ -619,6 +631,8 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6):
     if _needs_grad(x, weight, residual):
         return RmsNorm(*_RmsNorm.apply(x, weight, residual, float(eps)))
     out, total, _ = _normalise(_as_rows(x), weight, _as_rows(residual), eps, False)
+    if x.dim() == 2:
+        return RmsNorm(out, total)
     return RmsNorm(out.view(x.shape), None if total is None else total.view(x.shape))
 
 
@@ -639,9 +653,8 @@ def rms_norm_8bit(x, weight=None, residual=None, eps=1e-6):
     out = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
     scale = torch.empty((x.shape[0], groups), dtype=torch.float8_e8m0fnu, device=x.device)
     total = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    g = _norm(x, residual, weight, eps)
     _check("b3_rms_norm_8bit_gpu", policy_lib().b3_rms_norm_8bit_gpu(
-        C.byref(g), out.data_ptr(), scale.data_ptr(), _address_of(total), _stream()))
+        _norm(x, residual, weight, eps), out.data_ptr(), scale.data_ptr(), _address_of(total), _stream()))
     return RmsNorm8(out.view(shape), scale.view(*shape[:-1], groups), None if total is None else total.view(shape))
 
 

@@ -16,10 +16,18 @@
  * kScale brings their elements to where 2^-24, the least half, is 2^-37.
  * Accumulators are in 32 bits.
  *
+ * Where x is longer than wide, its steps are taken on the short side: with y
+ * and z as above y becomes z y z, p = .. z z z collects the steps, and x becomes
+ * p x once.  That is 3 m m n + (4 steps - 3) m^3 multiplications rather than
+ * steps (3 m m n + m^3), half tiles taken for half.  The rounding of y, some
+ * 2^-22 of its norm, grows by at most 3.4445^2 a step where y is all but 0, so
+ * that y is formed anew from x after kGroup steps.
+ *
  * A launch computes one product of all matrices, a workgroup to a tile of 128
  * x 128.  Matrices lie in blocks of 32 columns, halves and what is left side by
  * side, 128 bytes to a row's block; both sides are filled up with zeros to
- * whole tiles.
+ * whole tiles.  Matrices of at most 64 x 256 take all of their step in one
+ * workgroup's LDS.
  */
 #include "policy_common.h"
 
@@ -35,7 +43,9 @@ constexpr int kCut = 64;                         // tile of the first x
 constexpr int kMostParts = 256;                  // workgroups that a matrix' gradient is gone over by
 constexpr int64_t kPart = 4096;                  // its elements at the least
 constexpr double kA = 3.4445, kB = -4.7750, kC = 2.0315;
-constexpr float kScale = 8192.0f;
+constexpr float kScale = 8192.0f, kCollected = 16.0f;      // of x, y and z, and of p, whose singular values reach 3.4445^5
+constexpr int kGroup = 5;
+constexpr int kSmallSide = 64, kSmallLength = 256, kSmallThreads = 512;
 
 /* A matrix of the table.  x, next, y and z are in elements of `work`, of 4
  * bytes (both halves). */
@@ -44,10 +54,12 @@ struct Matrix {
     int64_t rows, columns, at;                   // at: in the flat arrays
     int64_t m, n;                                // x's sides, filled up
     int64_t x, next, y, z;
+    int64_t between, collected[2];               // of long ones: z y, and p by turns
     int64_t part;                                // elements of a workgroup's part of the gradient
     int64_t partial;                             // its first sum
     double decay, factor;                        // of the rate, by shape
     int type, parts;
+    bool is_long;
 };
 
 struct Place {
@@ -89,11 +101,13 @@ struct B3Muon {
     B3MuonState state;
     B3MuonMatrix* given;                         // host
     b3p::Matrix* matrices;                       // device
-    b3p::Place* places;                          // device: of parts, cuts, symmetric and whole tiles in turn
+    b3p::Place* places;                          // device: of parts, cuts, half of the tiles, tiles, small ones in turn
     int64_t* first_part;                         // host: by matrix; count + 1
     int64_t* first_cut;                          // host
     int64_t cuts, halves, tiles;                 // where those places begin, after the parts
-    int64_t end;
+    int64_t long_halves, long_tiles, end;        // those of long matrices come last
+    int64_t smalls;
+    int64_t* first_small;                        // host: by matrix, of the small ones; count + 1
     char* work;                                  // device
     double* partial;                             // device
     int* live;                                   // device
@@ -200,14 +214,21 @@ __global__ __launch_bounds__(kThreads) void mu_split(GradientLaunch l) {
     }
 }
 
-enum Product { GRAM, POLYNOMIAL, NEXT, LAST };
+enum Product { GRAM, POLYNOMIAL, MIDDLE, NEXT, LAST };
 
-/* What a launch of mu_product does: y = x x^T, z = a + b y + c y y, or x = z x
- * (LAST: and the weights move by it). */
+/* What a launch of mu_product does: y = x x^T (of long matrices within a
+ * group z y z, from z y), z = a + b y + c y y, z y and z p of long matrices, or
+ * x = z x, p x (LAST: and the weights move by it). */
 struct ProductLaunch {
     Common c;
-    bool swapped;                                // x is in `next`
+    bool swapped, swapped_long;                  // x is in `next`
+    int step;                                    // of a group
+    int middle;                                  // 0: z y, 1: z p; of the launch's first row of workgroups
 };
+
+/* Where z of a long matrix' step is (the first one is p), and p after a step. */
+__device__ __forceinline__ int64_t step_of(const Matrix& t, int step) { return step ? t.z : t.collected[0]; }
+__device__ __forceinline__ int64_t collected_of(const Matrix& t, int step) { return t.collected[step % 2]; }
 
 template <typename T>
 __device__ __forceinline__ void move(const Common& c, const Matrix& t, int64_t i, float x, float keep, float rate) {
@@ -234,9 +255,31 @@ __global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
     const Place p = l.c.places[l.c.first + by_die()];
     const Matrix& t = l.c.matrices[p.matrix];
     if (!l.c.live[p.matrix]) return;
-    const int64_t x = l.swapped ? t.next : t.x;
-    const int64_t left = KIND == GRAM ? x : KIND == POLYNOMIAL ? t.y : t.z, right = KIND == POLYNOMIAL ? t.y : x;
-    const int64_t sum = KIND == GRAM ? t.n : t.m;               // a row of the left side
+    const bool swapped = t.is_long ? l.swapped_long : l.swapped;
+    const int64_t x = swapped ? t.next : t.x, z = t.is_long ? step_of(t, l.step) : t.z;
+    int64_t left, right, out, sum = t.m;                        // sum: a row of the left side
+    float scale = 1.0f / kScale;                                // of the product
+    if (KIND == GRAM) {
+        const bool go_on = t.is_long && l.step;
+        left = go_on ? t.between : x;
+        right = go_on ? step_of(t, l.step - 1) : x;
+        sum = go_on ? t.m : t.n;
+        out = t.y;
+    } else if (KIND == POLYNOMIAL) {
+        left = right = t.y;
+        out = z;
+    } else if (KIND == MIDDLE) {
+        const bool collect = l.middle + blockIdx.y == 1;
+        left = z;
+        right = collect ? collected_of(t, l.step - 1) : t.y;
+        out = collect ? collected_of(t, l.step) : t.between;
+        if (collect && l.step == 1) scale *= kCollected / kScale;        // p was the first z
+    } else {
+        left = t.is_long ? collected_of(t, l.step) : z;
+        right = x;
+        out = swapped ? t.x : t.next;
+        if (t.is_long && l.step) scale = 1.0f / kCollected;
+    }
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, g = lane / 16, c = lane % 16;
     const int wi = wave / 2 * 64, wj = wave % 2 * 64;
     const char* from_left = l.c.work + left * 4 + ((int64_t)p.i * kTile + tid / 8) * sum * 4 + tid % 8 * 16;
@@ -325,7 +368,7 @@ __global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
             const int64_t row = (int64_t)p.i * kTile + wi + 16 * i + c, col = (int64_t)p.j * kTile + wj + 16 * j + 4 * g;
             F4 y;
 #pragma unroll
-            for (int r = 0; r < 4; r++) y[r] = d[i][j][r] * (1.0f / kScale);
+            for (int r = 0; r < 4; r++) y[r] = d[i][j][r] * scale;
             if (KIND == LAST) {
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
@@ -338,7 +381,6 @@ __global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
                 }
                 continue;
             }
-            const int64_t out = KIND == GRAM ? t.y : KIND == POLYNOMIAL ? t.z : l.swapped ? t.x : t.next;
             const int64_t columns = KIND == NEXT ? t.n : t.m;
             const int64_t block = col / kStep, o = col % kStep;
             if (KIND == POLYNOMIAL) {
@@ -368,6 +410,114 @@ __global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
                 }
             }
         }
+}
+
+/* ---- small matrices ---- */
+
+/* The quad of the sum's elements k .. k + 3 of row c, and of column c. */
+__device__ __forceinline__ F4 small_row(const float* lds, int row, int stride, int k) {
+    const int lane = threadIdx.x % kWave;
+    return *(const F4*)(lds + (row + lane % 16) * stride + k + lane / 16 * 4);
+}
+__device__ __forceinline__ F4 small_column(const float* lds, int col, int stride, int k) {
+    const int lane = threadIdx.x % kWave;
+    const float* p = lds + (k + lane / 16 * 4) * stride + col + lane % 16;
+    return F4{p[0], p[stride], p[2 * stride], p[3 * stride]};
+}
+
+__device__ __forceinline__ F4 multiply(F4 a, F4 b, F4 d) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) d = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], d, 0, 0, 0);
+    return d;
+}
+
+/* A matrix' whole step, in 32 bits: tiles of 16 x 16 of y and z to a wave each,
+ * and 16 columns of x, which become their next in place. */
+__global__ __launch_bounds__(kSmallThreads) void mu_small(GradientLaunch l, int steps) {
+    extern __shared__ __attribute__((aligned(16))) char shared[];
+    __shared__ double sums[kSmallThreads / kWave];
+    const int matrix = l.c.places[l.c.first + blockIdx.x].matrix;
+    const Matrix& t = l.c.matrices[matrix];
+    const void* grad = l.g.at[matrix - l.g.base];
+    const int type = l.g.type[matrix - l.g.base];
+    if (!grad) return;
+    const bool turned = t.rows > t.columns;
+    const int rows = (int)t.rows, columns = (int)t.columns, m = turned ? columns : rows, n = turned ? rows : columns;
+    const int mb = (m + 15) / 16, nb = (n + 15) / 16, stride = nb * 16 + 4, side = mb * 16 + 4;
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, g = lane / 16, c = lane % 16;
+    constexpr int kWaves = kSmallThreads / kWave;
+    float* x = (float*)shared;
+    float* y = x + mb * 16 * stride;
+    float* z = y + mb * 16 * side;
+    for (int i = tid; i < mb * 16 * stride; i += kSmallThreads) x[i] = 0.0f;
+    __syncthreads();
+    float* momentum = l.c.momentum + t.at;
+    double sum = 0;
+    for (int i = tid; i < rows * columns; i += kSmallThreads) {
+        const float gr = element(grad, type, i), mo = l.c.keep * momentum[i] + gr, u = direction(gr, mo, l.c);
+        const int r = i / columns, k = i % columns;
+        momentum[i] = mo;
+        x[turned ? k * stride + r : r * stride + k] = u;
+        sum += (double)u * u;
+    }
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) sum += __shfl_xor(sum, d);
+    if (lane == 0) sums[wave] = sum;
+    __syncthreads();
+    sum = 0;
+    for (int w = 0; w < kWaves; w++) sum += sums[w];
+    const double scale = 1.0 / (sqrt(sum) + l.c.eps);
+    for (int i = tid; i < mb * 16 * stride; i += kSmallThreads) x[i] = (float)(scale * x[i]);
+    __syncthreads();
+    for (int s = 0; s < steps; s++) {
+        for (int k = wave; k < mb * mb; k += kWaves) {
+            const int i = k / mb * 16, j = k % mb * 16;
+            F4 d = {0, 0, 0, 0};
+            for (int at = 0; at < nb * 16; at += 16) d = multiply(small_row(x, j, stride, at), small_row(x, i, stride, at), d);
+            *(F4*)(y + (i + c) * side + j + 4 * g) = d;          // symmetric: rows or columns
+        }
+        __syncthreads();
+        for (int k = wave; k < mb * mb; k += kWaves) {
+            const int i = k / mb * 16, j = k % mb * 16;
+            F4 d = {0, 0, 0, 0};
+            for (int at = 0; at < mb * 16; at += 16) d = multiply(small_row(y, j, side, at), small_row(y, i, side, at), d);
+            const F4 own = *(const F4*)(y + (i + c) * side + j + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                d[r] = __builtin_fmaf((float)kC, d[r], (float)kB * own[r]);
+                if (i + c == j + 4 * g + r) d[r] += (float)kA;
+            }
+            *(F4*)(z + (i + c) * side + j + 4 * g) = d;
+        }
+        __syncthreads();
+        for (int j = wave; j < nb; j += kWaves) {
+            F4 d[kSmallSide / 16] = {};
+            for (int at = 0; at < mb * 16; at += 16) {
+                const F4 b = small_column(x, j * 16, stride, at);
+#pragma unroll
+                for (int i = 0; i < kSmallSide / 16; i++)
+                    if (i < mb) d[i] = multiply(b, small_row(z, i * 16, side, at), d[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < kSmallSide / 16; i++)
+                if (i < mb) *(F4*)(x + (i * 16 + c) * stride + j * 16 + 4 * g) = d[i];
+        }
+        __syncthreads();
+    }
+    const float keep = (float)(1 - l.c.lr * t.decay), rate = (float)(l.c.lr * t.factor);
+    for (int i = tid; i < rows * columns; i += kSmallThreads) {
+        const int r = i / columns, k = i % columns;
+        const float v = x[turned ? k * stride + r : r * stride + k];
+        if (t.type == B3_F32) move<float>(l.c, t, i, v, keep, rate);
+        else if (t.type == B3_F16) move<_Float16>(l.c, t, i, v, keep, rate);
+        else move<__bf16>(l.c, t, i, v, keep, rate);
+    }
+}
+
+/* Bytes of LDS for sides of at most m and n. */
+constexpr int small_lds(int m, int n) {
+    const int mb = (m + 15) / 16 * 16, nb = (n + 15) / 16 * 16;
+    return (mb * (nb + 4) + 2 * mb * (mb + 4)) * 4;
 }
 
 /* ---- launches ---- */
@@ -422,12 +572,17 @@ hipError_t over(int64_t first, int64_t end, F launch) {
 }
 
 template <Product KIND>
-hipError_t launch_product(ProductLaunch l, int64_t first, int64_t end, hipStream_t stream) {
+hipError_t launch_product(ProductLaunch l, int64_t first, int64_t end, hipStream_t stream, unsigned both = 1) {
     constexpr int kLds = 4 * kTile * (kStep * 4 + 16);
     return over(first, end, [&](int64_t at, unsigned blocks) {
         l.c.first = at;
-        mu_product<KIND><<<blocks, kThreads, kLds, stream>>>(l);
+        mu_product<KIND><<<dim3(blocks, both), kThreads, kLds, stream>>>(l);
     });
+}
+
+bool is_small(int64_t rows, int64_t columns) {
+    const int64_t m = rows < columns ? rows : columns, n = rows < columns ? columns : rows;
+    return m <= kSmallSide && n <= kSmallLength;
 }
 
 template <Product KIND>
@@ -461,6 +616,7 @@ hipError_t b3_muon_destroy(B3Muon* o) {
     free(o->given);
     free(o->first_part);
     free(o->first_cut);
+    free(o->first_small);
     free(o);
     return first;
 }
@@ -480,13 +636,14 @@ hipError_t b3_muon_create(B3Muon** out, const B3MuonMatrix* matrices, int count,
     o->given = (B3MuonMatrix*)calloc((size_t)count + 1, sizeof(B3MuonMatrix));
     o->first_part = (int64_t*)calloc((size_t)count + 1, sizeof(int64_t));
     o->first_cut = (int64_t*)calloc((size_t)count + 1, sizeof(int64_t));
+    o->first_small = (int64_t*)calloc((size_t)count + 1, sizeof(int64_t));
     Matrix* table = (Matrix*)calloc((size_t)count + 1, sizeof(Matrix));
     Place* places = NULL;
     int64_t work = 0, partials = 0;
-    hipError_t err = !(o->given && o->first_part && o->first_cut && table) ? hipErrorOutOfMemory
+    hipError_t err = !(o->given && o->first_part && o->first_cut && o->first_small && table) ? hipErrorOutOfMemory
         : overlap(matrices, count, o->given) ? hipErrorInvalidValue : hipGetDevice(&o->device);
     if (err == hipSuccess) {
-        int64_t at = 0, parts = 0, cuts = 0, halves = 0, tiles = 0;
+        int64_t at = 0, parts = 0, cuts = 0, small = 0, halves[2] = {0, 0}, tiles[2] = {0, 0};
         for (int i = 0; i < count; i++) {
             const B3MuonMatrix& g = o->given[i] = matrices[i];
             Matrix& t = table[i];
@@ -501,14 +658,23 @@ hipError_t b3_muon_create(B3Muon** out, const B3MuonMatrix* matrices, int count,
             t.factor = g.rows > g.columns && g.columns ? sqrt((double)g.rows / (double)g.columns) : 1.0;
             o->first_part[i] = parts;
             o->first_cut[i] = cuts;
+            o->first_small[i] = small;
             if (!numel) continue;
+            if (is_small(g.rows, g.columns)) {
+                small++;
+                continue;
+            }
             t.m = filled(m);
             t.n = filled(numel / m);
+            t.is_long = t.n > t.m;
+            int64_t* const squares[5] = {&t.y, &t.z, &t.between, &t.collected[0], &t.collected[1]};
             t.x = work;
             t.next = t.x + t.m * t.n;
-            t.y = t.next + t.m * t.n;
-            t.z = t.y + t.m * t.m;
-            work = t.z + t.m * t.m;
+            work = t.next + t.m * t.n;
+            for (int k = 0; k < (t.is_long ? 5 : 2); k++) {
+                *squares[k] = work;
+                work += t.m * t.m;
+            }
             t.part = ceil_div(numel, kMostParts);
             t.part = t.part < kPart ? kPart : t.part;
             t.parts = (int)ceil_div(numel, t.part);
@@ -517,16 +683,19 @@ hipError_t b3_muon_create(B3Muon** out, const B3MuonMatrix* matrices, int count,
             const int64_t mt = t.m / kTile, nt = t.n / kTile, per = kTile / kCut;
             parts += t.parts;
             cuts += mt * nt * per * per;
-            halves += mt * (mt + 1) / 2;
-            tiles += mt * nt;
+            halves[t.is_long] += mt * (mt + 1) / 2;
+            tiles[t.is_long] += mt * nt;
         }
         o->first_part[count] = parts;
         o->first_cut[count] = cuts;
+        o->first_small[count] = small;
         o->cuts = parts;
         o->halves = o->cuts + cuts;
-        o->tiles = o->halves + halves;
-        o->end = o->tiles + tiles;
-        places = (Place*)malloc((size_t)(o->end + 1) * sizeof(Place));
+        o->long_halves = o->halves + halves[0];
+        o->tiles = o->long_halves + halves[1];
+        o->long_tiles = o->tiles + tiles[0];
+        o->end = o->long_tiles + tiles[1];
+        places = (Place*)malloc((size_t)(o->end + small + 1) * sizeof(Place));
         if (!places) err = hipErrorOutOfMemory;
         Place* to = places;
         for (int i = 0; i < count && places; i++)
@@ -534,24 +703,29 @@ hipError_t b3_muon_create(B3Muon** out, const B3MuonMatrix* matrices, int count,
         for (int i = 0; i < count && places; i++)
             for (int64_t r = 0; r < table[i].m / kCut; r++)
                 for (int64_t c = 0; c < table[i].n / kCut; c++) *to++ = Place{i, (int)r, (int)c};
+        for (int k = 0; k < 4 && places; k++)            // half of the tiles, then all, and of both long matrices last
+            for (int i = 0; i < count; i++)
+                for (int64_t r = 0; r < table[i].m / kTile && table[i].is_long == k % 2; r++)
+                    for (int64_t c = 0; c < (k < 2 ? r + 1 : table[i].n / kTile); c++) *to++ = Place{i, (int)r, (int)c};
         for (int i = 0; i < count && places; i++)
-            for (int64_t r = 0; r < table[i].m / kTile; r++)
-                for (int64_t c = 0; c <= r; c++) *to++ = Place{i, (int)r, (int)c};
-        for (int i = 0; i < count && places; i++)
-            for (int64_t r = 0; r < table[i].m / kTile; r++)
-                for (int64_t c = 0; c < table[i].n / kTile; c++) *to++ = Place{i, (int)r, (int)c};
+            if (o->first_small[i + 1] > o->first_small[i]) *to++ = Place{i, 0, 0};
+        o->smalls = small;
     }
     if (err == hipSuccess) err = hipMalloc((void**)&o->matrices, ((size_t)count + 1) * sizeof(Matrix));
-    if (err == hipSuccess) err = hipMalloc((void**)&o->places, (size_t)(o->end + 1) * sizeof(Place));
+    if (err == hipSuccess) err = hipMalloc((void**)&o->places, (size_t)(o->end + o->smalls + 1) * sizeof(Place));
     if (err == hipSuccess) err = hipMalloc((void**)&o->work, (size_t)(work + 1) * 4);
     if (err == hipSuccess) err = hipMalloc((void**)&o->partial, (size_t)(partials + 1) * sizeof(double));
     if (err == hipSuccess) err = hipMalloc((void**)&o->live, ((size_t)count + 1) * sizeof(int));
     if (err == hipSuccess) err = hipMemcpy(o->matrices, table, ((size_t)count + 1) * sizeof(Matrix), hipMemcpyHostToDevice);
-    if (err == hipSuccess) err = hipMemcpy(o->places, places, (size_t)o->end * sizeof(Place), hipMemcpyHostToDevice);
+    if (err == hipSuccess) err = hipMemcpy(o->places, places, (size_t)(o->end + o->smalls) * sizeof(Place), hipMemcpyHostToDevice);
     if (err == hipSuccess) err = allow_lds<GRAM>();
     if (err == hipSuccess) err = allow_lds<POLYNOMIAL>();
+    if (err == hipSuccess) err = allow_lds<MIDDLE>();
     if (err == hipSuccess) err = allow_lds<NEXT>();
     if (err == hipSuccess) err = allow_lds<LAST>();
+    if (err == hipSuccess)
+        err = hipFuncSetAttribute((const void*)mu_small, hipFuncAttributeMaxDynamicSharedMemorySize,
+            small_lds(kSmallSide, kSmallLength));
     free(table);
     free(places);
     if (err != hipSuccess) {
@@ -593,20 +767,32 @@ hipError_t b3_muon_step_gpu(B3Muon* o, const void* const* grads, const int* grad
             mu_momentum<<<blocks, kThreads, 0, stream>>>(l);
         });
         if (err != hipSuccess) return err;
+        err = over(o->end + o->first_small[base], o->end + o->first_small[base + n], [&](int64_t at, unsigned blocks) {
+            l.c.first = at;
+            mu_small<<<blocks, kSmallThreads, small_lds(kSmallSide, kSmallLength), stream>>>(l, o->config.newton_schulz);
+        });
+        if (err != hipSuccess) return err;
         err = over(o->cuts + o->first_cut[base], o->cuts + o->first_cut[base + n], [&](int64_t at, unsigned blocks) {
             l.c.first = at;
             mu_split<<<blocks, kThreads, 0, stream>>>(l);
         });
         if (err != hipSuccess) return err;
     }
-    ProductLaunch p = {l.c, false};
-    for (int s = 0; s < o->config.newton_schulz && err == hipSuccess; s++) {
+    const int steps = o->config.newton_schulz;
+    ProductLaunch p = {l.c, false, false, 0, 0};
+    for (int s = 0; s < steps && o->halves < o->end && err == hipSuccess; s++) {
+        const bool last = s + 1 == steps, joined = last || p.step + 1 == kGroup;     // long x becomes its next
         err = launch_product<GRAM>(p, o->halves, o->tiles, stream);
         if (err == hipSuccess) err = launch_product<POLYNOMIAL>(p, o->halves, o->tiles, stream);
+        p.middle = joined ? 1 : 0;
+        const unsigned both = (joined ? 0 : 1) + (p.step ? 1 : 0);
+        if (err == hipSuccess && both) err = launch_product<MIDDLE>(p, o->long_halves, o->tiles, stream, both);
         if (err == hipSuccess)
-            err = s + 1 < o->config.newton_schulz ? launch_product<NEXT>(p, o->tiles, o->end, stream)
-                                                  : launch_product<LAST>(p, o->tiles, o->end, stream);
+            err = last ? launch_product<LAST>(p, o->tiles, o->end, stream)
+                       : launch_product<NEXT>(p, o->tiles, joined ? o->end : o->long_tiles, stream);
         p.swapped = !p.swapped;
+        p.swapped_long ^= joined;
+        p.step = joined ? 0 : p.step + 1;
     }
     return err;
 }
