@@ -46,6 +46,7 @@ constexpr double kA = 3.4445, kB = -4.7750, kC = 2.0315;
 constexpr float kScale = 8192.0f, kCollected = 16.0f;      // of x, y and z, and of p, whose singular values reach 3.4445^5
 constexpr int kGroup = 5;
 constexpr int kSmallSide = 64, kSmallLength = 256, kSmallThreads = 512;
+constexpr int kSmallTiles = kSmallSide / 16 * kSmallLength / 16 / (kSmallThreads / kWave);      // of a wave
 
 /* A matrix of the table.  x, next, y and z are in elements of `work`, of 4
  * bytes (both halves). */
@@ -147,6 +148,66 @@ __device__ double block_sum(double x) {
 
 __device__ __forceinline__ float direction(float g, float m, const Common& c) { return c.nesterov ? g + c.keep * m : m; }
 
+/* Four neighbours of an array of `all`, zeros past its end. */
+template <typename T>
+__device__ __forceinline__ F4 load4(const T* p, int64_t i, int64_t all) {
+    F4 x;
+    if (i + 4 <= all) {
+        const Pack<T, 4> v = *(const Pack<T, 4>*)(p + i);
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = to_float(v.v[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = i + k < all ? to_float(p[i + k]) : 0.0f;
+    }
+    return x;
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int64_t i, int64_t all, F4 x) {
+    if (i + 4 <= all) {
+        Pack<T, 4> v;
+#pragma unroll
+        for (int k = 0; k < 4; k++) v.v[k] = (T)x[k];
+        *(Pack<T, 4>*)(p + i) = v;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (i + k < all) p[i + k] = (T)x[k];
+    }
+}
+
+/* The momentum of elements from .. end - 1, a thread's sum of squares of u. */
+template <typename T>
+__device__ __forceinline__ double momentum_part(const T* grad, float* momentum, int64_t from, int64_t end, const Common& c) {
+    constexpr int kAhead = 4;
+    double sum = 0;
+    for (int64_t i0 = from + threadIdx.x * 4; i0 < end; i0 += kThreads * 4 * kAhead) {
+        F4 g[kAhead], m[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            const int64_t i = i0 + k * kThreads * 4;
+            g[k] = m[k] = F4{0, 0, 0, 0};
+            if (i < end) {
+                g[k] = load4(grad, i, end);
+                m[k] = load4(momentum, i, end);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            const int64_t i = i0 + k * kThreads * 4;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                m[k][e] = c.keep * m[k][e] + g[k][e];
+                const float u = direction(g[k][e], m[k][e], c);
+                sum += (double)u * u;
+            }
+            if (i < end) store4(momentum, i, end, m[k]);
+        }
+    }
+    return sum;
+}
+
 /* The momentum, and a part's sum of squares of u. */
 __global__ __launch_bounds__(kThreads) void mu_momentum(GradientLaunch l) {
     const Place p = l.c.places[l.c.first + blockIdx.x];
@@ -157,13 +218,9 @@ __global__ __launch_bounds__(kThreads) void mu_momentum(GradientLaunch l) {
     if (!grad) return;
     float* momentum = l.c.momentum + t.at;
     const int64_t from = p.i * t.part, all = t.rows * t.columns, end = from + t.part < all ? from + t.part : all;
-    double sum = 0;
-#pragma unroll 4
-    for (int64_t i = from + threadIdx.x; i < end; i += kThreads) {
-        const float g = element(grad, type, i), m = l.c.keep * momentum[i] + g, u = direction(g, m, l.c);
-        momentum[i] = m;
-        sum += (double)u * u;
-    }
+    double sum = type == B3_F32 ? momentum_part((const float*)grad, momentum, from, end, l.c)
+        : type == B3_F16 ? momentum_part((const _Float16*)grad, momentum, from, end, l.c)
+                         : momentum_part((const __bf16*)grad, momentum, from, end, l.c);
     sum = block_sum(sum);
     if (threadIdx.x == 0) l.c.partial[t.partial + p.i] = sum;
 }
@@ -172,6 +229,32 @@ __global__ __launch_bounds__(kThreads) void mu_momentum(GradientLaunch l) {
  * left of those. */
 __device__ __forceinline__ _Float16* block_of(char* work, int64_t base, int64_t columns, int64_t r, int64_t b) {
     return (_Float16*)(work + base * 4 + (r * columns + b * kStep) * 4);
+}
+
+/* A square of u, scaled, turned as x lies. */
+template <typename T>
+__device__ __forceinline__ void first_square(float (*tile)[kCut + 1], const T* grad, const float* momentum, const Matrix& t,
+    int64_t r0, int64_t c0, bool turned, double scale, const Common& c) {
+    constexpr int kAcross = kCut / 4, kDown = kThreads / kAcross, kLoads = kCut / kDown;
+    const int col = threadIdx.x % kAcross * 4, row = threadIdx.x / kAcross;
+    F4 g[kLoads], m[kLoads];
+#pragma unroll
+    for (int k = 0; k < kLoads; k++) {
+        const int64_t r = r0 + row + k * kDown, at = r * t.columns;
+        g[k] = m[k] = F4{0, 0, 0, 0};
+        if (r < t.rows && c0 + col < t.columns) {
+            g[k] = load4(grad + at, c0 + col, t.columns);
+            m[k] = load4(momentum + at, c0 + col, t.columns);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kLoads; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float u = (float)(scale * direction(g[k][e], m[k][e], c));
+            if (turned) tile[col + e][row + k * kDown] = u;
+            else tile[row + k * kDown][col + e] = u;
+        }
 }
 
 /* The first x, a square of it: u over its norm. */
@@ -187,16 +270,9 @@ __global__ __launch_bounds__(kThreads) void mu_split(GradientLaunch l) {
     const bool turned = t.rows > t.columns;
     const int64_t r0 = (int64_t)(turned ? p.j : p.i) * kCut, c0 = (int64_t)(turned ? p.i : p.j) * kCut;
     const float* momentum = l.c.momentum + t.at;
-    const int col = threadIdx.x % kCut, row = threadIdx.x / kCut;
-#pragma unroll 4
-    for (int r = row; r < kCut; r += kThreads / kCut) {
-        float u = 0;
-        if (r0 + r < t.rows && c0 + col < t.columns) {
-            const int64_t i = (r0 + r) * t.columns + c0 + col;
-            u = (float)(scale * direction(element(grad, type, i), momentum[i], l.c));
-        }
-        tile[turned ? col : r][turned ? r : col] = u;
-    }
+    if (type == B3_F32) first_square(tile, (const float*)grad, momentum, t, r0, c0, turned, scale, l.c);
+    else if (type == B3_F16) first_square(tile, (const _Float16*)grad, momentum, t, r0, c0, turned, scale, l.c);
+    else first_square(tile, (const __bf16*)grad, momentum, t, r0, c0, turned, scale, l.c);
     __syncthreads();
     /* a row's block of 32 to four threads of eight */
     for (int k = threadIdx.x; k < kCut * kCut / 8; k += kThreads) {
@@ -230,16 +306,55 @@ struct ProductLaunch {
 __device__ __forceinline__ int64_t step_of(const Matrix& t, int step) { return step ? t.z : t.collected[0]; }
 __device__ __forceinline__ int64_t collected_of(const Matrix& t, int step) { return t.collected[step % 2]; }
 
+/* A weight after the step.  A copy that the weight is not rounded from has been
+ * overtaken by what was written to the weight. */
+template <typename T>
+__device__ __forceinline__ float moved(T old, float copy, bool copied, float x, float keep, float rate) {
+    float w = to_float(old);
+    if (copied && to_float((T)copy) == w) w = copy;
+    return w * keep - rate * x;
+}
+
 template <typename T>
 __device__ __forceinline__ void move(const Common& c, const Matrix& t, int64_t i, float x, float keep, float rate) {
     T* param = (T*)t.param + i;
-    const T old = *param;
-    float w = to_float(old);
     float* copy = c.master && sizeof(T) == 2 ? c.master + t.at + i : NULL;
-    if (copy && to_float((T)*copy) == w) w = *copy;
-    w = w * keep - rate * x;
+    const float w = moved(*param, copy ? *copy : 0.0f, copy != NULL, x, keep, rate);
     if (copy) *copy = w;
     *param = (T)w;
+}
+
+/* The weights from row r0 and column c0 on, by a tile of x that lies as they do. */
+constexpr int kMoveRow = kTile + 4;
+template <typename T>
+__device__ __forceinline__ void move_tile(const Common& c, const Matrix& t, const float* tile, int64_t r0, int64_t c0) {
+    constexpr int kAcross = kTile / 4, kDown = kThreads / kAcross, kAhead = 4;
+    const float keep = (float)(1 - c.lr * t.decay), rate = (float)(c.lr * t.factor);
+    const int col = threadIdx.x % kAcross * 4, row = threadIdx.x / kAcross;
+    const bool copied = c.master && sizeof(T) == 2;
+    if (c0 + col >= t.columns) return;
+    for (int k0 = 0; k0 < kTile && r0 + k0 < t.rows; k0 += kDown * kAhead) {
+        F4 w[kAhead], copy[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            const int64_t r = r0 + k0 + k * kDown + row, at = r * t.columns;
+            w[k] = copy[k] = F4{0, 0, 0, 0};
+            if (r < t.rows) {
+                w[k] = load4((const T*)t.param + at, c0 + col, t.columns);
+                if (copied) copy[k] = load4(c.master + t.at + at, c0 + col, t.columns);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            const int64_t r = r0 + k0 + k * kDown + row, at = r * t.columns;
+            if (r >= t.rows) continue;
+            const F4 x = *(const F4*)(tile + (k0 + k * kDown + row) * kMoveRow + col);
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[k][e] = moved((T)w[k][e], copy[k][e], copied, x[e], keep, rate);
+            if (copied) store4(c.master + t.at + at, c0 + col, t.columns, w[k]);
+            store4((T*)t.param + at, c0 + col, t.columns, w[k]);
+        }
+    }
 }
 
 /* Four waves, each with 64 x 64 of the tile.  A step of 32 of what is summed
@@ -359,8 +474,30 @@ __global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
         if (more) put(shared + half * 2 * kSide);
         __syncthreads();
     }
-    const bool turned = t.rows > t.columns;
-    const float keep = (float)(1 - l.c.lr * t.decay), rate = (float)(l.c.lr * t.factor);
+    if (KIND == LAST) {
+        /* to LDS as the weights lie, so that a row's neighbours are moved together */
+        const bool turned = t.rows > t.columns;
+        float* tile = (float*)shared;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int row = wi + 16 * i + c, col = wj + 16 * j + 4 * g;
+                F4 y;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    y[r] = d[i][j][r] * scale * (1.0f / kScale);
+                    if (turned) tile[(col + r) * kMoveRow + row] = y[r];
+                }
+                if (!turned) *(F4*)(tile + row * kMoveRow + col) = y;
+            }
+        __syncthreads();
+        const int64_t r0 = (int64_t)(turned ? p.j : p.i) * kTile, c0 = (int64_t)(turned ? p.i : p.j) * kTile;
+        if (t.type == B3_F32) move_tile<float>(l.c, t, tile, r0, c0);
+        else if (t.type == B3_F16) move_tile<_Float16>(l.c, t, tile, r0, c0);
+        else move_tile<__bf16>(l.c, t, tile, r0, c0);
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -369,18 +506,6 @@ __global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
             F4 y;
 #pragma unroll
             for (int r = 0; r < 4; r++) y[r] = d[i][j][r] * scale;
-            if (KIND == LAST) {
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int64_t pr = turned ? col + r : row, pc = turned ? row : col + r;
-                    if (pr >= t.rows || pc >= t.columns) continue;
-                    const float v = y[r] * (1.0f / kScale);
-                    if (t.type == B3_F32) move<float>(l.c, t, pr * t.columns + pc, v, keep, rate);
-                    else if (t.type == B3_F16) move<_Float16>(l.c, t, pr * t.columns + pc, v, keep, rate);
-                    else move<__bf16>(l.c, t, pr * t.columns + pc, v, keep, rate);
-                }
-                continue;
-            }
             const int64_t columns = KIND == NEXT ? t.n : t.m;
             const int64_t block = col / kStep, o = col % kStep;
             if (KIND == POLYNOMIAL) {
@@ -432,7 +557,7 @@ __device__ __forceinline__ F4 multiply(F4 a, F4 b, F4 d) {
 }
 
 /* A matrix' whole step, in 32 bits: tiles of 16 x 16 of y and z to a wave each,
- * and 16 columns of x, which become their next in place. */
+ * and of x up to kSmallTiles. */
 __global__ __launch_bounds__(kSmallThreads) void mu_small(GradientLaunch l, int steps) {
     extern __shared__ __attribute__((aligned(16))) char shared[];
     __shared__ double sums[kSmallThreads / kWave];
@@ -490,17 +615,21 @@ __global__ __launch_bounds__(kSmallThreads) void mu_small(GradientLaunch l, int 
             *(F4*)(z + (i + c) * side + j + 4 * g) = d;
         }
         __syncthreads();
-        for (int j = wave; j < nb; j += kWaves) {
-            F4 d[kSmallSide / 16] = {};
-            for (int at = 0; at < mb * 16; at += 16) {
-                const F4 b = small_column(x, j * 16, stride, at);
+        F4 next[kSmallTiles];
 #pragma unroll
-                for (int i = 0; i < kSmallSide / 16; i++)
-                    if (i < mb) d[i] = multiply(b, small_row(z, i * 16, side, at), d[i]);
-            }
+        for (int k = 0; k < kSmallTiles; k++) {
+            const int tile = wave + k * kWaves, i = tile / nb * 16, j = tile % nb * 16;
+            next[k] = F4{0, 0, 0, 0};
+            if (tile >= mb * nb) break;
+            for (int at = 0; at < mb * 16; at += 16)
+                next[k] = multiply(small_column(x, j, stride, at), small_row(z, i, side, at), next[k]);
+        }
+        __syncthreads();
 #pragma unroll
-            for (int i = 0; i < kSmallSide / 16; i++)
-                if (i < mb) *(F4*)(x + (i * 16 + c) * stride + j * 16 + 4 * g) = d[i];
+        for (int k = 0; k < kSmallTiles; k++) {
+            const int tile = wave + k * kWaves, i = tile / nb * 16, j = tile % nb * 16;
+            if (tile >= mb * nb) break;
+            *(F4*)(x + (i + c) * stride + j + 4 * g) = next[k];
         }
         __syncthreads();
     }
