@@ -159,7 +159,7 @@ def _need(ok, what):
 
 
 def _stream():
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _on(*tensors):
@@ -433,8 +433,7 @@ def _attention_backward(ctx, d_out, d_left):
     lib = policy_lib()
     d_out = torch.zeros_like(v) if d_out is None else _heads(d_out)
     d_left = None if d_left is None else _as_read(d_left).contiguous()
-    new = lambda wanted, like, dtype: torch.empty(like.shape, dtype=dtype, device=v.device) if wanted else None  # noqa: E731
-    d_q, d_k, d_v, d_state = (new(ctx.needs_input_grad[i], x, v.dtype if i < 3 else torch.float32)
+    d_q, d_k, d_v, d_state = (torch.empty_like(x, memory_format=torch.contiguous_format) if ctx.needs_input_grad[i] else None
                               for i, x in ((0, q), (1, k), (2, v), (4, state)))
     g = _attention(q.shape[0], q, k, v, decay, state, starts, ctx.scale)
     size = lib.b3_linear_attention_workspace(g, 1)
@@ -575,7 +574,7 @@ def _norm_backward(ctx, d_out, d_sum):
     shape = (d_sum if d_out is None else d_out).shape
     d_out, d_sum = _as_rows(d_out), _as_rows(d_sum)
     stride = lambda y: 0 if y is None else y.stride(0) if rows > 1 else width  # noqa: E731
-    d_x = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    d_x = torch.empty_like(x, memory_format=torch.contiguous_format)
     d_weight = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
     size = lib.b3_rms_norm_backward_workspace(rows, width)
     work = _work(size, x.device)

@@ -77,6 +77,7 @@ typedef short S4 __attribute__((ext_vector_type(4)));
 typedef short S8 __attribute__((ext_vector_type(8)));
 typedef __bf16 B4 __attribute__((ext_vector_type(4)));
 typedef __bf16 B8 __attribute__((ext_vector_type(8)));
+typedef _Float16 H8 __attribute__((ext_vector_type(8)));
 typedef uint32_t U4 __attribute__((ext_vector_type(4)));
 
 /* What the arithmetic goes by.  Lane (g, c) = (lane / 16, lane % 16) holds of
@@ -161,19 +162,22 @@ struct Tile {
                     if (!in) raw[l] = U4{0, 0, 0, 0};
             }
         } else {
+            /* (values of their own, so that nothing of this is formed ahead of the loop and held) */
+            int first = col();
+            asm volatile("" : "+s"(stride), "+v"(first));
 #pragma unroll
             for (int l = 0; l < kLoads; l++) {
                 const T* at = p + (row(l) < places ? row(l) : places - 1) * stride;
                 Pack<T, kVec> x;
                 if (cols % kVec == 0) {
-                    x = *(const Pack<T, kVec>*)(at + (in ? col() : 0));
+                    x = *(const Pack<T, kVec>*)(at + (first < cols ? first : 0));
                 } else {
 #pragma unroll
-                    for (int i = 0; i < kVec; i++) x.v[i] = at[col() + i < cols ? col() + i : 0];
+                    for (int i = 0; i < kVec; i++) x.v[i] = at[first + i < cols ? first + i : 0];
                 }
 #pragma unroll
                 for (int i = 0; i < kVec; i++)
-                    if (row(l) >= places || col() + i >= cols) x.v[i] = (T)0.0f;
+                    if (row(l) >= places || first + i >= cols) x.v[i] = (T)0.0f;
                 raw[l] = __builtin_bit_cast(U4, x);
             }
         }
@@ -185,25 +189,20 @@ struct Tile {
             if (row(l)) raw[l] = U4{0, 0, 0, 0};
     }
 
-    /* Whether any element of the lane's is NaN or infinite. */
-    __device__ __forceinline__ bool bad() const {
-        typedef unsigned short H2 __attribute__((ext_vector_type(2)));
-        uint32_t most = 0;
+    /* Adds to sums in turn what is NaN in some lane if any element of the chunk is
+     * NaN or infinite, else 0: the elements' products with 0, which the matrix
+     * units form as they lie. */
+    __device__ __forceinline__ void times_0(F4 sum[4]) const {
 #pragma unroll
-        for (int l = 0; l < kLoads; l++)
-#pragma unroll
-            for (int w = 0; w < 4; w++) {
-                if (sizeof(T) == 4) {
-                    const uint32_t x = raw[l][w] & 0x7fffffffu;
-                    most = x > most ? x : most;
-                } else {
-                    const H2 x = __builtin_bit_cast(H2, raw[l][w] & 0x7fff7fffu);
-                    most = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(x, __builtin_bit_cast(H2, most)));
-                }
+        for (int l = 0; l < kLoads; l++) {
+            if constexpr (__is_same(T, __bf16)) {
+                sum[l % 4] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(B8, raw[l]), B8{}, sum[l % 4], 0, 0, 0);
+            } else if constexpr (__is_same(T, _Float16)) {
+                sum[l % 4] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(H8, raw[l]), H8{}, sum[l % 4], 0, 0, 0);
+            } else {
+                sum[l % 4] = __builtin_elementwise_fma(__builtin_bit_cast(F4, raw[l]), F4{0, 0, 0, 0}, sum[l % 4]);
             }
-        if (sizeof(T) == 4) return most >= 0x7f800000u;
-        const uint32_t least = sizeof(Lds) == 2 ? 0x7f80u : 0x7c00u;
-        return (most & 0xffffu) >= least || most >> 16 >= least;
+        }
     }
 
     __device__ __forceinline__ void put(Lds* lds, int r, int c, U4 x) const {
@@ -282,6 +281,8 @@ struct Walk {
     static constexpr int kBytes = (STATE ? 1 : 2) * KeyTile::kBytes + ValueTile::kBytes;
     /* in 16 bits two tiles' columns are dealt out so that a lane has eight neighbours of them */
     static constexpr int kStep = kHalf ? 8 : 4;
+    /* where registers do not hold all of the next chunk beside the operands of out, its q is fetched after out */
+    static constexpr bool kLate = kHalf && KD == 128;
     static __device__ __forceinline__ int value_col(int vb) { return kHalf ? vb / 2 * 32 + vb % 2 * 4 : vb * 16; }
 
     static __device__ __forceinline__ Quad with(F4 x) {
@@ -324,11 +325,12 @@ struct Walk {
         uint32_t flag = 0;
         bool dropped = false;
         float scale = 1.0f;                      // of the state
+        bool any = enter != NULL;                // state
         auto fetch = [&](int64_t p) {
             const int n = places - p < kPlaces ? (int)(places - p) : kPlaces;
             tk.load(k + p * m.k_stride[0], m.k_stride[0], n, m.key);
             tv.load(v + p * m.v_stride[0], m.v_stride[0], n, value);
-            if (!STATE) tq.load(q + p * m.q_stride[0], m.q_stride[0], n, m.key);
+            if (!STATE && !kLate) tq.load(q + p * m.q_stride[0], m.q_stride[0], n, m.key);
             if (m.starts) {
                 /* the first place on the way back has none: a later one's is fetched, and dropped */
                 const int at = lane < n ? lane : n - 1, none = from + p == 0 && !m.forward ? 1 : 0;
@@ -339,7 +341,14 @@ struct Walk {
                     flag = 0;
             }
         };
-        if (places > 0) fetch(0);
+        auto fetch_late = [&](int64_t p) {
+            const int n = places - p < kPlaces ? (int)(places - p) : kPlaces;
+            if (!STATE && kLate) tq.load(q + p * m.q_stride[0], m.q_stride[0], n, m.key);
+        };
+        if (places > 0) {
+            fetch(0);
+            fetch_late(0);
+        }
         /* E, lane (g, c) of tile [kb][vb] rows 16 kb + 4 g + r and the column of c */
         F4 state[KB][VB];
         const float first = early ? power(l2, 1) : 1.0f;
@@ -351,6 +360,7 @@ struct Walk {
                 const int col = value_col(vb) + kStep * (c / 4) + c % 4;
                 at[vb] = enter + (u.first + (col < value ? col : 0)) * state_col;
             }
+            /* (a transposed state's four rows are neighbours) */
             if (state_row == 1 && m.key % 4 == 0) {
 #pragma unroll
                 for (int kb = 0; kb < KB; kb++)
@@ -369,15 +379,18 @@ struct Walk {
                         for (int vb = 0; vb < VB; vb++) state[kb][vb][r] = at[vb][offset];
                     }
             }
+            scale = first;
+            if (m.key < KD || value < VD) {
 #pragma unroll
-            for (int kb = 0; kb < KB; kb++)
+                for (int kb = 0; kb < KB; kb++)
 #pragma unroll
-                for (int vb = 0; vb < VB; vb++)
+                    for (int vb = 0; vb < VB; vb++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const int row = kb * 16 + 4 * g + r, col = value_col(vb) + kStep * (c / 4) + c % 4;
-                        state[kb][vb][r] = row < m.key && col < value ? first * state[kb][vb][r] : 0.0f;
-                    }
+                        for (int r = 0; r < 4; r++) {
+                            const int row = kb * 16 + 4 * g + r, col = value_col(vb) + kStep * (c / 4) + c % 4;
+                            if (row >= m.key || col >= value) state[kb][vb][r] = 0.0f;
+                        }
+            }
         } else {
 #pragma unroll
             for (int kb = 0; kb < KB; kb++)
@@ -391,7 +404,11 @@ struct Walk {
             n = places - p < kPlaces ? (int)(places - p) : kPlaces;
             /* A product with a weight of 0 would carry what is not finite in k or v to other places:
              * such a place is a chunk by itself. */
-            if (n > 1 && __ballot(tk.bad() || tv.bad())) {
+            F4 zero[4] = {};
+            tk.times_0(zero);
+            tv.times_0(zero);
+            zero[0] = zero[0] + zero[1] + (zero[2] + zero[3]);
+            if (n > 1 && __ballot(zero[0][0] + zero[0][1] + (zero[0][2] + zero[0][3]) != 0.0f)) {
                 n = 1;
                 tk.first_row_alone();
                 tv.first_row_alone();
@@ -405,18 +422,6 @@ struct Walk {
             wave_fence();
             const bool end = p + n >= places;
             if (!end) fetch(p + n);
-            const int less = end && m.forward && from + places == j.steps ? 1 : 0;
-            if (weighted != 2 * n + less) {
-                weighted = 2 * n + less;
-#pragma unroll
-                for (int t = 0; t < R; t++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const int at = 16 * t + 4 * g + r;
-                        keep[t][r] = at < n ? m.update * power(l2, n - at - less) : 0.0f;
-                    }
-                pass = power(l2, n - less);
-            }
             Quad vq[R][VB];
 #pragma unroll
             for (int t = 0; t < R; t++)
@@ -424,52 +429,17 @@ struct Walk {
                 for (int vb = 0; vb < VB; vb++) vq[t][vb] = across<kValueRow, kStep>(lv, 16 * t, value_col(vb));
 
             if (!STATE) {
-                F4 o[R][VB];
                 Quad qq[R][KB];
 #pragma unroll
                 for (int t = 0; t < R; t++)
 #pragma unroll
                     for (int kb = 0; kb < KB; kb++) qq[t][kb] = along<kKeyRow>(lq, 16 * t, 16 * kb);
-#pragma unroll
-                for (int t = 0; t < R; t++)
-#pragma unroll
-                    for (int vb = 0; vb < VB; vb++) o[t][vb] = F4{0, 0, 0, 0};
-                /* q E: in 16 bits E as two numbers */
-#pragma unroll
-                for (int vb = 0; vb < VB; vb++) {
-                    if constexpr (kHalf) {
-#pragma unroll
-                        for (int kb = 0; kb < KB; kb += 2) {
-                            const S4 h0 = round4(state[kb][vb]), h1 = round4(state[kb + 1][vb]);
-                            const S4 l0 = rest4(state[kb][vb], h0), l1 = rest4(state[kb + 1][vb], h1);
-#pragma unroll
-                            for (int t = 0; t < R; t++) o[t][vb] = multiply(l0, l1, qq[t][kb], qq[t][kb + 1], o[t][vb]);
-#pragma unroll
-                            for (int t = 0; t < R; t++) o[t][vb] = multiply(h0, h1, qq[t][kb], qq[t][kb + 1], o[t][vb]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int kb = 0; kb < KB; kb++)
-#pragma unroll
-                            for (int t = 0; t < R; t++) o[t][vb] = multiply(state[kb][vb], qq[t][kb], o[t][vb]);
-                    }
-                }
                 /* of place i = 16 t + c the last start at or before it */
                 int since[R];
 #pragma unroll
                 for (int t = 0; t < R; t++) {
                     const uint32_t before = starts & (uint32_t)((2ull << (16 * t + c)) - 1);
                     since[t] = before ? 31 - __builtin_clz(before) : -1;
-                    const float f = reach[t] * scale;
-#pragma unroll
-                    for (int vb = 0; vb < VB; vb++) o[t][vb] *= f;
-                }
-                if (starts) {
-#pragma unroll
-                    for (int t = 0; t < R; t++)
-#pragma unroll
-                        for (int vb = 0; vb < VB; vb++)
-                            if (since[t] >= 0) o[t][vb] = F4{0, 0, 0, 0};
                 }
                 /* scores, rows j and columns i; they are what P v sums over as they lie */
                 Quad score[R][R];
@@ -488,36 +458,78 @@ struct Walk {
 #pragma unroll
                             for (int kb = 0; kb < KB; kb++) x = multiply(kq[kb], qq[t][kb], x);
                         }
+                        x *= near[t - s];
+                        if (t == s) {
 #pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            const int at = 16 * s + 4 * g + r;
-                            x[r] = at >= since[t] && at <= 16 * t + c ? x[r] * near[t - s][r] : 0.0f;
+                            for (int r = 0; r < 4; r++)
+                                if (4 * g + r > c) x[r] = 0.0f;
+                        }
+                        if (starts) {
+#pragma unroll
+                            for (int r = 0; r < 4; r++)
+                                if (16 * s + 4 * g + r < since[t]) x[r] = 0.0f;
                         }
                         score[t][s] = with(x);
                     }
                 }
+                /* kTiles tiles of columns at a time, which a lane writes together */
+                constexpr int kTiles = kHalf ? 2 : 1, kWide = 4 * kTiles;
 #pragma unroll
-                for (int t = 0; t < R; t++)
+                for (int v0 = 0; v0 < VB; v0 += kTiles) {
+                    F4 o[R][kTiles];
 #pragma unroll
-                    for (int vb = 0; vb < VB; vb++) {
-                        if constexpr (kHalf)
-                            o[t][vb] = multiply(vq[0][vb], vq[1][vb], score[t][0], t ? score[1][1] : S4{0, 0, 0, 0}, o[t][vb]);
-                        else
-                            o[t][vb] = multiply(vq[0][vb], score[0][0], o[t][vb]);
+                    for (int t = 0; t < R; t++)
+#pragma unroll
+                        for (int i = 0; i < kTiles; i++) o[t][i] = F4{0, 0, 0, 0};
+                    if (any) {
+                        /* q E: in 16 bits E as two numbers */
+#pragma unroll
+                        for (int i = 0; i < kTiles; i++) {
+                            const int vb = v0 + i;
+                            if constexpr (kHalf) {
+#pragma unroll
+                                for (int kb = 0; kb < KB; kb += 2) {
+                                    const S4 h0 = round4(state[kb][vb]), h1 = round4(state[kb + 1][vb]);
+                                    const S4 l0 = rest4(state[kb][vb], h0), l1 = rest4(state[kb + 1][vb], h1);
+#pragma unroll
+                                    for (int t = 0; t < R; t++) o[t][i] = multiply(l0, l1, qq[t][kb], qq[t][kb + 1], o[t][i]);
+#pragma unroll
+                                    for (int t = 0; t < R; t++) o[t][i] = multiply(h0, h1, qq[t][kb], qq[t][kb + 1], o[t][i]);
+                                }
+                            } else {
+#pragma unroll
+                                for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                                    for (int t = 0; t < R; t++) o[t][i] = multiply(state[kb][vb], qq[t][kb], o[t][i]);
+                            }
+                        }
+#pragma unroll
+                        for (int t = 0; t < R; t++)
+#pragma unroll
+                            for (int i = 0; i < kTiles; i++) {
+                                o[t][i] *= reach[t] * scale;
+                                if (starts && since[t] >= 0) o[t][i] = F4{0, 0, 0, 0};
+                            }
                     }
-                /* lane (g, c): of place 16 t + c the columns 4 g + r of each tile */
 #pragma unroll
-                for (int t = 0; t < R; t++) {
-                    const int at = 16 * t + c;
-                    if (at >= n || !m.out) continue;
-                    T* to = out + (p + at) * m.out_stride[0];
-                    constexpr int kTiles = kHalf ? 2 : 1, kWide = 4 * kTiles;
+                    for (int t = 0; t < R; t++)
 #pragma unroll
-                    for (int vb = 0; vb < VB; vb += kTiles) {
-                        const int col = value_col(vb) + kWide * g;
+                        for (int i = 0; i < kTiles; i++) {
+                            if constexpr (kHalf)
+                                o[t][i] = multiply(vq[0][v0 + i], vq[1][v0 + i], score[t][0], t ? score[1][1] : S4{0, 0, 0, 0}, o[t][i]);
+                            else
+                                o[t][i] = multiply(vq[0][v0 + i], score[0][0], o[t][i]);
+                        }
+                    /* lane (g, c): of place 16 t + c the columns 4 g + r of each tile */
+                    const int col = value_col(v0) + kWide * g;
+#pragma unroll
+                    for (int t = 0; t < R; t++) {
+                        const int at = 16 * t + c;
+                        if (at >= n || !m.out) continue;
+                        T* to = out + (p + at) * m.out_stride[0];
                         Pack<T, kWide> y;
 #pragma unroll
-                        for (int i = 0; i < kWide; i++) y.v[i] = (T)o[t][vb + i / 4][i % 4];
+                        for (int i = 0; i < kWide; i++) y.v[i] = (T)o[t][i / 4][i % 4];
                         if (col + kWide <= value) {
                             *(Pack<T, kWide>*)(to + col) = y;
                         } else {
@@ -528,6 +540,21 @@ struct Walk {
                     }
                 }
             }
+            if (end && !leave) break;
+            if (!end) fetch_late(p + n);
+            const int less = end && m.forward && from + places == j.steps ? 1 : 0;
+            if (weighted != 2 * n + less) {
+                weighted = 2 * n + less;
+#pragma unroll
+                for (int t = 0; t < R; t++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int at = 16 * t + 4 * g + r;
+                        keep[t][r] = at < n ? m.update * power(l2, n - at - less) : 0.0f;
+                    }
+                pass = power(l2, n - less);
+            }
+            any = true;
             /* What is kept of the state, and of the places from the last start on.  The state is
              * held as E / scale, so that no chunk has to go over it: its decay goes into scale and,
              * before that becomes small, into the state. */

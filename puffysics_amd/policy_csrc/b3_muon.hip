@@ -234,7 +234,7 @@ __device__ __forceinline__ _Float16* block_of(char* work, int64_t base, int64_t 
 /* A square of u, scaled, turned as x lies. */
 template <typename T>
 __device__ __forceinline__ void first_square(float (*tile)[kCut + 1], const T* grad, const float* momentum, const Matrix& t,
-    int64_t r0, int64_t c0, bool turned, double scale, const Common& c) {
+    int64_t r0, int64_t c0, bool turned, const Common& c) {
     constexpr int kAcross = kCut / 4, kDown = kThreads / kAcross, kLoads = kCut / kDown;
     const int col = threadIdx.x % kAcross * 4, row = threadIdx.x / kAcross;
     F4 g[kLoads], m[kLoads];
@@ -247,6 +247,9 @@ __device__ __forceinline__ void first_square(float (*tile)[kCut + 1], const T* g
             m[k] = load4(momentum + at, c0 + col, t.columns);
         }
     }
+    /* what is fetched meanwhile waits for the norm */
+    const double size = sqrt(block_sum((int)threadIdx.x < t.parts ? c.partial[t.partial + threadIdx.x] : 0.0));
+    const double scale = kScale / (size + c.eps);
 #pragma unroll
     for (int k = 0; k < kLoads; k++)
 #pragma unroll
@@ -265,14 +268,12 @@ __global__ __launch_bounds__(kThreads) void mu_split(GradientLaunch l) {
     const void* grad = l.g.at[p.matrix - l.g.base];
     const int type = l.g.type[p.matrix - l.g.base];
     if (!grad) return;
-    const double size = sqrt(block_sum((int)threadIdx.x < t.parts ? l.c.partial[t.partial + threadIdx.x] : 0.0));
-    const double scale = kScale / (size + l.c.eps);
     const bool turned = t.rows > t.columns;
     const int64_t r0 = (int64_t)(turned ? p.j : p.i) * kCut, c0 = (int64_t)(turned ? p.i : p.j) * kCut;
     const float* momentum = l.c.momentum + t.at;
-    if (type == B3_F32) first_square(tile, (const float*)grad, momentum, t, r0, c0, turned, scale, l.c);
-    else if (type == B3_F16) first_square(tile, (const _Float16*)grad, momentum, t, r0, c0, turned, scale, l.c);
-    else first_square(tile, (const __bf16*)grad, momentum, t, r0, c0, turned, scale, l.c);
+    if (type == B3_F32) first_square(tile, (const float*)grad, momentum, t, r0, c0, turned, l.c);
+    else if (type == B3_F16) first_square(tile, (const _Float16*)grad, momentum, t, r0, c0, turned, l.c);
+    else first_square(tile, (const __bf16*)grad, momentum, t, r0, c0, turned, l.c);
     __syncthreads();
     /* a row's block of 32 to four threads of eight */
     for (int k = threadIdx.x; k < kCut * kCut / 8; k += kThreads) {
@@ -598,6 +599,7 @@ __global__ __launch_bounds__(kSmallThreads) void mu_small(GradientLaunch l, int 
         for (int k = wave; k < mb * mb; k += kWaves) {
             const int i = k / mb * 16, j = k % mb * 16;
             F4 d = {0, 0, 0, 0};
+#pragma unroll 4
             for (int at = 0; at < nb * 16; at += 16) d = multiply(small_row(x, j, stride, at), small_row(x, i, stride, at), d);
             *(F4*)(y + (i + c) * side + j + 4 * g) = d;          // symmetric: rows or columns
         }
@@ -605,6 +607,7 @@ __global__ __launch_bounds__(kSmallThreads) void mu_small(GradientLaunch l, int 
         for (int k = wave; k < mb * mb; k += kWaves) {
             const int i = k / mb * 16, j = k % mb * 16;
             F4 d = {0, 0, 0, 0};
+#pragma unroll 4
             for (int at = 0; at < mb * 16; at += 16) d = multiply(small_row(y, j, side, at), small_row(y, i, side, at), d);
             const F4 own = *(const F4*)(y + (i + c) * side + j + 4 * g);
 #pragma unroll
@@ -621,6 +624,7 @@ __global__ __launch_bounds__(kSmallThreads) void mu_small(GradientLaunch l, int 
             const int tile = wave + k * kWaves, i = tile / nb * 16, j = tile % nb * 16;
             next[k] = F4{0, 0, 0, 0};
             if (tile >= mb * nb) break;
+#pragma unroll 4
             for (int at = 0; at < mb * 16; at += 16)
                 next[k] = multiply(small_column(x, j, stride, at), small_row(z, i, side, at), next[k]);
         }
