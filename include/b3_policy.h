@@ -227,7 +227,7 @@ size_t b3_linear_attention_workspace(const B3Attention* attention, int backward)
 /*   S_t = decay S_{t-1} + k_t^T v_t (without the first term where an episode
  *   starts), out_t = scale q_t S_t
  * out [steps, envs, heads, value], contiguous; last_state (NULL: not wanted)
- * like `state`, which it may be: S after the last step. */
+ * like `state`, and apart from it: S after the last step. */
 hipError_t b3_linear_attention_gpu(const B3Attention* attention, void* out, float* last_state, void* workspace,
     size_t workspace_bytes, hipStream_t stream);
 

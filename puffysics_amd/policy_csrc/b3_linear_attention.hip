@@ -133,18 +133,18 @@ __device__ __forceinline__ float power(float log2_decay, int n) {
 /* An array's part of a chunk: COLS columns of kPlaces rows, in vectors of 16
  * bytes, in registers until the chunk before is done and then in LDS, whose
  * rows are 16 bytes longer so that 16 rows' neighbouring columns lie in other
- * banks. */
-template <typename T, int COLS>
+ * banks.  W waves share it, and each moves every W-th of its vectors. */
+template <typename T, int COLS, int W>
 struct Tile {
     typedef typename Math<T>::Lds Lds;
     static constexpr int kVec = 16 / sizeof(T), kRow = COLS + 16 / sizeof(Lds), kPlaces = Math<T>::kPlaces;
-    static constexpr int kPerRow = COLS / kVec, kRows = kWave / kPerRow, kLoads = kPlaces / kRows;
+    static constexpr int kPerRow = COLS / kVec, kRows = kWave / kPerRow, kLoads = kPlaces / (kRows * W);
     static constexpr int kBytes = kPlaces * kRow * sizeof(Lds);
-    static_assert(kWave % kPerRow == 0 && kPlaces % kRows == 0, "whole loads");
+    static_assert(kWave % kPerRow == 0 && kPlaces % (kRows * W) == 0, "whole loads");
     U4 raw[kLoads];
 
     /* Vector l of a lane is of row(l), from col() on. */
-    static __device__ __forceinline__ int row(int l) { return l * kRows + (int)threadIdx.x % kWave / kPerRow; }
+    static __device__ __forceinline__ int row(int l) { return l * (kRows * W) + (int)threadIdx.x % (kWave * W) / kPerRow; }
     static __device__ __forceinline__ int col() { return (int)threadIdx.x % kPerRow * kVec; }
 
     /* Columns from p on, of which there are `cols`; zeros beyond and in rows from
@@ -155,7 +155,7 @@ struct Tile {
         if (cols % kVec == 0 && places == kPlaces) {
             const T* at = p + row(0) * stride + (in ? col() : 0);
 #pragma unroll
-            for (int l = 0; l < kLoads; l++) raw[l] = __builtin_bit_cast(U4, *(const Pack<T, kVec>*)(at + l * (kRows * stride)));
+            for (int l = 0; l < kLoads; l++) raw[l] = __builtin_bit_cast(U4, *(const Pack<T, kVec>*)(at + l * (kRows * W * stride)));
             if (cols < COLS) {
 #pragma unroll
                 for (int l = 0; l < kLoads; l++)
@@ -181,6 +181,11 @@ struct Tile {
                 raw[l] = __builtin_bit_cast(U4, x);
             }
         }
+    }
+
+    __device__ __forceinline__ void none() {
+#pragma unroll
+        for (int l = 0; l < kLoads; l++) raw[l] = U4{0, 0, 0, 0};
     }
 
     __device__ __forceinline__ void first_row_alone() {
@@ -263,26 +268,25 @@ struct Unit {
     int role, first;                             // first: column of v
 };
 
-/* One wave goes over the places of a piece of a sequence, a chunk at a time,
- * KD the columns of q and k and VD those of its part of v, both filled up with
- * zeros; STATE: without out, to learn what state the piece leaves.  With i and
- * j places of the chunk, E the state that enters it and P the scores q_i k_j
+/* A wave goes over the places of a piece of a sequence, a chunk at a time, KD
+ * the columns of q and k and VD those of its part of v, both filled up with
+ * zeros; STATE: without out, to learn what state the piece leaves.  W waves, a
+ * workgroup where W > 1, have parts of one sequence and share q and k.  With i
+ * and j places of the chunk, E the state that enters it and P the scores q_i k_j
  * decay^(i - j) of an episode, j <= i:
  *   out = P v + decay^i q E,  E' = decay^places E + (decay^(places - j) k)^T v */
-template <typename T, int KD, int VD, bool STATE>
+template <typename T, int KD, int VD, int W, bool STATE>
 struct Walk {
     typedef typename Math<T>::Lds Lds;
     typedef typename Math<T>::Quad Quad;
     static constexpr bool kHalf = sizeof(Lds) == 2;
     static constexpr int kPlaces = Math<T>::kPlaces, R = kPlaces / 16, KB = KD / 16, VB = VD / 16;
-    typedef Tile<T, KD> KeyTile;
-    typedef Tile<T, VD> ValueTile;
+    typedef Tile<T, KD, W> KeyTile;
+    typedef Tile<T, VD, 1> ValueTile;
     static constexpr int kKeyRow = KeyTile::kRow, kValueRow = ValueTile::kRow;
-    static constexpr int kBytes = (STATE ? 1 : 2) * KeyTile::kBytes + ValueTile::kBytes;
+    static constexpr int kBytes = (STATE ? 1 : 2) * KeyTile::kBytes + W * ValueTile::kBytes + (W > 1 ? 16 : 0);
     /* in 16 bits two tiles' columns are dealt out so that a lane has eight neighbours of them */
     static constexpr int kStep = kHalf ? 8 : 4;
-    /* where registers do not hold all of the next chunk beside the operands of out, its q is fetched after out */
-    static constexpr bool kLate = kHalf && KD == 128;
     static __device__ __forceinline__ int value_col(int vb) { return kHalf ? vb / 2 * 32 + vb % 2 * 4 : vb * 16; }
 
     static __device__ __forceinline__ Quad with(F4 x) {
@@ -290,18 +294,26 @@ struct Walk {
         else return x;
     }
 
+    static __device__ __forceinline__ void fence() {
+        if (W == 1) wave_fence();
+        else __syncthreads();
+    }
+
     static __device__ __forceinline__ void run(const Job& j, const Mix& m, const Unit& u, int64_t from, int64_t places, const float* enter,
         bool early, float* leave, float* carry, char* shared) {
         const int lane = threadIdx.x % kWave, g = lane / 16, c = lane % 16;
+        const int wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
         Lds* lk = (Lds*)shared;
-        Lds* lv = (Lds*)(shared + KeyTile::kBytes);
-        Lds* lq = (Lds*)(shared + KeyTile::kBytes + ValueTile::kBytes);
+        Lds* lv = (Lds*)(shared + KeyTile::kBytes + wave * ValueTile::kBytes);
+        Lds* lq = (Lds*)(shared + KeyTile::kBytes + W * ValueTile::kBytes);
+        int* bad = (int*)(shared + kBytes - 16);                    // of each wave
         const float l2 = log2f(decay_of(j.decay, u.head));
         const T* q = (const T*)m.q + from * m.q_stride[0] + u.env * m.q_stride[1] + u.head * m.q_stride[2];
         const T* k = (const T*)m.k + from * m.k_stride[0] + u.env * m.k_stride[1] + u.head * m.k_stride[2];
         const T* v = (const T*)m.v + from * m.v_stride[0] + u.env * m.v_stride[1] + u.head * m.v_stride[2] + u.first;
         T* out = (T*)m.out + from * m.out_stride[0] + u.env * m.out_stride[1] + u.head * m.out_stride[2] + u.first;
         const int value = m.value - u.first < VD ? m.value - u.first : VD;
+        const bool active = W == 1 || value > 0;                    // else it has q and k to move alone
 
         /* weights of scores (of the tiles i = j and i = j + 16), of the state for place i, and of places for the state */
         const float gain = m.reach * m.update;
@@ -329,8 +341,8 @@ struct Walk {
         auto fetch = [&](int64_t p) {
             const int n = places - p < kPlaces ? (int)(places - p) : kPlaces;
             tk.load(k + p * m.k_stride[0], m.k_stride[0], n, m.key);
-            tv.load(v + p * m.v_stride[0], m.v_stride[0], n, value);
-            if (!STATE && !kLate) tq.load(q + p * m.q_stride[0], m.q_stride[0], n, m.key);
+            if (active) tv.load(v + p * m.v_stride[0], m.v_stride[0], n, value);
+            if (!STATE) tq.load(q + p * m.q_stride[0], m.q_stride[0], n, m.key);
             if (m.starts) {
                 /* the first place on the way back has none: a later one's is fetched, and dropped */
                 const int at = lane < n ? lane : n - 1, none = from + p == 0 && !m.forward ? 1 : 0;
@@ -341,19 +353,13 @@ struct Walk {
                     flag = 0;
             }
         };
-        auto fetch_late = [&](int64_t p) {
-            const int n = places - p < kPlaces ? (int)(places - p) : kPlaces;
-            if (!STATE && kLate) tq.load(q + p * m.q_stride[0], m.q_stride[0], n, m.key);
-        };
-        if (places > 0) {
-            fetch(0);
-            fetch_late(0);
-        }
+        if (W > 1) tv.none();
+        if (places > 0) fetch(0);
         /* E, lane (g, c) of tile [kb][vb] rows 16 kb + 4 g + r and the column of c */
         F4 state[KB][VB];
         const float first = early ? power(l2, 1) : 1.0f;
         const int state_row = (int)m.state_row, state_col = (int)m.state_col;
-        if (enter) {
+        if (enter && active) {
             const float* at[VB];
 #pragma unroll
             for (int vb = 0; vb < VB; vb++) {
@@ -408,20 +414,39 @@ struct Walk {
             tk.times_0(zero);
             tv.times_0(zero);
             zero[0] = zero[0] + zero[1] + (zero[2] + zero[3]);
-            if (n > 1 && __ballot(zero[0][0] + zero[0][1] + (zero[0][2] + zero[0][3]) != 0.0f)) {
+            const bool found = __ballot(zero[0][0] + zero[0][1] + (zero[0][2] + zero[0][3]) != 0.0f) != 0;
+            auto alone = [&]() {
                 n = 1;
                 tk.first_row_alone();
                 tv.first_row_alone();
                 if (!STATE) tq.first_row_alone();
+            };
+            auto stage = [&]() {
+                fence();
+                tk.store(lk);
+                tv.store(lv);
+                if (!STATE) tq.store(lq);
+                if (W > 1 && lane == 0) bad[wave] = found;
+                fence();
+            };
+            if (W == 1 && found && n > 1) alone();
+            stage();
+            if (W > 1 && n > 1) {
+                int any_found = 0;
+#pragma unroll
+                for (int w = 0; w < W; w++) any_found |= bad[w];
+                if (any_found) {
+                    alone();
+                    stage();
+                }
             }
             const uint32_t starts = (uint32_t)__ballot(flag != 0 && lane < n);
-            wave_fence();
-            tk.store(lk);
-            tv.store(lv);
-            if (!STATE) tq.store(lq);
-            wave_fence();
             const bool end = p + n >= places;
             if (!end) fetch(p + n);
+            if (!active) {
+                if (end) break;
+                continue;
+            }
             Quad vq[R][VB];
 #pragma unroll
             for (int t = 0; t < R; t++)
@@ -541,7 +566,6 @@ struct Walk {
                 }
             }
             if (end && !leave) break;
-            if (!end) fetch_late(p + n);
             const int less = end && m.forward && from + places == j.steps ? 1 : 0;
             if (weighted != 2 * n + less) {
                 weighted = 2 * n + less;
@@ -613,7 +637,7 @@ struct Walk {
         }
         if (carry && lane == 0 && u.first == 0)
             *carry = dropped ? -1.0f : __builtin_amdgcn_exp2f(places ? (float)places * l2 : 0.0f);
-        if (!leave) return;
+        if (!leave || !active) return;
         const bool gone = !STATE && m.leave_starts && started(m.leave_starts + u.env * m.leave_starts_stride, j.starts_type);
 #pragma unroll
         for (int kb = 0; kb < KB; kb++)
@@ -628,22 +652,22 @@ struct Walk {
     }
 };
 
-/* Waves of a workgroup: neighbours share what they read (the parts and roles
- * of a sequence) or lie side by side in memory (heads).  Workgroups go to the
- * 8 dies in turn: each die's take neighbouring ones. */
-template <typename T, int KD, int VD, bool STATE>
+/* Waves of a workgroup: the parts of a sequence where they share, else
+ * neighbours in memory (roles of a sequence, heads).  Workgroups go to the 8
+ * dies in turn: each die's take neighbouring ones. */
+template <typename T, int KD, int VD, int W, bool STATE>
 __global__ __launch_bounds__(kThreads, 2) void la_walk(Job j) {
     extern __shared__ __attribute__((aligned(16))) char shared[];
-    typedef Walk<T, KD, VD, STATE> W;
+    typedef Walk<T, KD, VD, W, STATE> Walker;
     const unsigned die = blockIdx.x % 8, share = gridDim.x / 8, rest = gridDim.x % 8;
     const unsigned block = die * share + (die < rest ? die : rest) + blockIdx.x / 8;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    int64_t id = (int64_t)block * (blockDim.x / kWave) + wave;
+    int64_t id = W > 1 ? (int64_t)block : (int64_t)block * (blockDim.x / kWave) + wave;
     const int64_t pieces = STATE ? j.pieces - 1 : j.pieces;
-    if (id >= j.envs * j.heads * pieces * j.roles * j.parts) return;
+    if (W == 1 && id >= j.envs * j.heads * pieces * j.roles * j.parts) return;
     Unit u;
-    u.first = (int)(id % j.parts) * VD;
-    id /= j.parts;
+    u.first = (W > 1 ? wave : (int)(id % j.parts)) * VD;
+    id /= W > 1 ? 1 : j.parts;
     u.role = (int)(id % j.roles);
     id /= j.roles;
     u.head = id % j.heads;
@@ -651,7 +675,7 @@ __global__ __launch_bounds__(kThreads, 2) void la_walk(Job j) {
     u.env = id % j.envs;
     u.piece = id / j.envs;
     const Mix& m = j.mix[u.role];
-    if (u.first >= m.value) return;
+    if (W == 1 && u.first >= m.value) return;
     if (!m.forward) u.piece = pieces - 1 - u.piece;
     const int64_t sequences = j.envs * j.heads, sequence = u.env * j.heads + u.head, size = (int64_t)m.key * m.value;
     const int64_t from = u.piece * j.places, left = j.steps - from, places = left < j.places ? left : j.places;
@@ -666,7 +690,8 @@ __global__ __launch_bounds__(kThreads, 2) void la_walk(Job j) {
         if (u.piece) enter = m.pieces + ((u.piece - 1) * sequences + sequence) * size;
         if (u.piece + 1 < pieces) leave = NULL;
     }
-    W::run(j, m, u, from, places, enter, m.forward && u.piece == 0 && j.steps, leave, carry, shared + wave * W::kBytes);
+    Walker::run(j, m, u, from, places, enter, m.forward && u.piece == 0 && j.steps, leave, carry,
+        shared + (W > 1 ? 0 : wave * Walker::kBytes));
 }
 
 /* What enters each piece, over what the pieces left by themselves. */
@@ -879,21 +904,23 @@ void place_pieces(Mix& m, const B3Attention& g, const Plan& p, void* workspace, 
     m.carry = m.pieces + (p.pieces - 1) * g.envs * g.heads * g.key * g.value;
 }
 
-template <typename T, int KD, int VD, bool STATE>
+template <typename T, int KD, int VD, int W, bool STATE>
 hipError_t launch(const Job& j, hipStream_t stream) {
-    typedef Walk<T, KD, VD, STATE> W;
-    constexpr int kLds = 64 << 10, kMost = kLds / W::kBytes, kWavesHere = kMost >= 4 ? 4 : kMost >= 2 ? 2 : 1;
-    static_assert(kMost >= 1, "a wave's tiles");
-    const int64_t units = j.envs * j.heads * (STATE ? j.pieces - 1 : j.pieces) * j.roles * j.parts;
-    la_walk<T, KD, VD, STATE><<<(unsigned)ceil_div(units, kWavesHere), kWavesHere * kWave, kWavesHere * W::kBytes, stream>>>(j);
+    typedef Walk<T, KD, VD, W, STATE> Walker;
+    constexpr int kLds = 64 << 10, kMost = kLds / Walker::kBytes, kGroups = W > 1 ? 1 : kMost >= 4 ? 4 : kMost >= 2 ? 2 : 1;
+    static_assert(kMost >= 1, "a workgroup's tiles");
+    const int64_t units = j.envs * j.heads * (STATE ? j.pieces - 1 : j.pieces) * j.roles * (W > 1 ? 1 : j.parts);
+    la_walk<T, KD, VD, W, STATE><<<(unsigned)ceil_div(units, kGroups), kGroups * W * kWave, kGroups * Walker::kBytes, stream>>>(j);
     return hipGetLastError();
 }
 
 template <typename T, bool STATE>
 hipError_t launch_columns(const Job& j, const Plan& p, hipStream_t stream) {
-    if (p.key == 128) return launch<T, 128, 32, STATE>(j, stream);
-    if (p.value == 32) return p.key == 32 ? launch<T, 32, 32, STATE>(j, stream) : launch<T, 64, 32, STATE>(j, stream);
-    return p.key == 32 ? launch<T, 32, 64, STATE>(j, stream) : launch<T, 64, 64, STATE>(j, stream);
+    if (p.key == 128)
+        return p.parts > 2 ? launch<T, 128, 32, 4, STATE>(j, stream) : p.parts > 1 ? launch<T, 128, 32, 2, STATE>(j, stream)
+                                                                                   : launch<T, 128, 32, 1, STATE>(j, stream);
+    if (p.value == 32) return p.key == 32 ? launch<T, 32, 32, 1, STATE>(j, stream) : launch<T, 64, 32, 1, STATE>(j, stream);
+    return p.key == 32 ? launch<T, 32, 64, 1, STATE>(j, stream) : launch<T, 64, 64, 1, STATE>(j, stream);
 }
 
 /* `ways`: what of the job's mixes learns the pieces' states, one for each. */

@@ -307,8 +307,7 @@ def test_long(size, type):
 @pytest.mark.parametrize("type", ["f32", "bf16"])
 def test_a_rollout_in_two_halves(type):
     """The state that a first half leaves is what the second goes on from, and
-    its gradient goes back through it; a state may be written over the one it
-    came from."""
+    its gradient goes back through it."""
     from puffysics_amd import policy
     dtype = TYPES[type]
     q, k, v, decay, starts, state = made(90, 4, 2, 32, 32, dtype, 12)
