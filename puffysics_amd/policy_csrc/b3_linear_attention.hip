@@ -98,10 +98,9 @@ struct Math<__bf16> {
 };
 
 __device__ __forceinline__ S4 round4(F4 x) { return __builtin_bit_cast(S4, __builtin_convertvector(x, B4)); }
-/* What rounding left out, rounded. */
-__device__ __forceinline__ S4 rest4(F4 x, S4 rounded) {
-    return round4(x - __builtin_convertvector(__builtin_bit_cast(B4, rounded), F4));
-}
+/* What rounding left out, and that rounded. */
+__device__ __forceinline__ F4 left4(F4 x, S4 rounded) { return x - __builtin_convertvector(__builtin_bit_cast(B4, rounded), F4); }
+__device__ __forceinline__ S4 rest4(F4 x, S4 rounded) { return round4(left4(x, rounded)); }
 
 /* d += a b over two blocks of 16. */
 __device__ __forceinline__ F4 multiply(S4 a0, S4 a1, S4 b0, S4 b1, F4 d) {
@@ -607,22 +606,49 @@ struct Walk {
 #pragma unroll
                 for (int r = 0; r < 4; r++) weight[t][r] = 16 * t + 4 * g + r >= last ? keep[t][r] * over : 0.0f;
             if constexpr (kHalf) {
-                S4 h[R][VB], rest[R][VB];        // weighted v as two numbers
+                /* weighted v as three numbers, since the state is one of 32 bits */
+                auto split = [&](int vb, S4 h[R], S4 rest[R], S4 third[R]) {
 #pragma unroll
-                for (int t = 0; t < R; t++)
+                    for (int t = 0; t < R; t++) {
+                        const F4 x = weight[t] * __builtin_convertvector(__builtin_bit_cast(B4, vq[t][vb]), F4);
+                        h[t] = round4(x);
+                        const F4 y = left4(x, h[t]);
+                        rest[t] = round4(y);
+                        third[t] = rest4(y, rest[t]);
+                    }
+                };
+                /* either of k's and v's operands are held while the others pass, those of the fewer columns */
+                if constexpr (KB <= VB) {
+                    S4 kq[KB][R];
+#pragma unroll
+                    for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                        for (int t = 0; t < R; t++) kq[kb][t] = across<kKeyRow, 4>(lk, 16 * t, 16 * kb);
 #pragma unroll
                     for (int vb = 0; vb < VB; vb++) {
-                        const F4 x = weight[t] * __builtin_convertvector(__builtin_bit_cast(B4, vq[t][vb]), F4);
-                        h[t][vb] = round4(x);
-                        rest[t][vb] = rest4(x, h[t][vb]);
+                        S4 h[R], rest[R], third[R];
+                        split(vb, h, rest, third);
+#pragma unroll
+                        for (int kb = 0; kb < KB; kb++) state[kb][vb] = multiply(kq[kb][0], kq[kb][1], third[0], third[1], state[kb][vb]);
+#pragma unroll
+                        for (int kb = 0; kb < KB; kb++) state[kb][vb] = multiply(kq[kb][0], kq[kb][1], rest[0], rest[1], state[kb][vb]);
+#pragma unroll
+                        for (int kb = 0; kb < KB; kb++) state[kb][vb] = multiply(kq[kb][0], kq[kb][1], h[0], h[1], state[kb][vb]);
                     }
+                } else {
+                    S4 h[VB][R], rest[VB][R], third[VB][R];
 #pragma unroll
-                for (int kb = 0; kb < KB; kb++) {
-                    const S4 k0 = across<kKeyRow, 4>(lk, 0, 16 * kb), k1 = across<kKeyRow, 4>(lk, 16, 16 * kb);
+                    for (int vb = 0; vb < VB; vb++) split(vb, h[vb], rest[vb], third[vb]);
 #pragma unroll
-                    for (int vb = 0; vb < VB; vb++) state[kb][vb] = multiply(k0, k1, rest[0][vb], rest[1][vb], state[kb][vb]);
+                    for (int kb = 0; kb < KB; kb++) {
+                        const S4 k0 = across<kKeyRow, 4>(lk, 0, 16 * kb), k1 = across<kKeyRow, 4>(lk, 16, 16 * kb);
 #pragma unroll
-                    for (int vb = 0; vb < VB; vb++) state[kb][vb] = multiply(k0, k1, h[0][vb], h[1][vb], state[kb][vb]);
+                        for (int vb = 0; vb < VB; vb++) state[kb][vb] = multiply(k0, k1, third[vb][0], third[vb][1], state[kb][vb]);
+#pragma unroll
+                        for (int vb = 0; vb < VB; vb++) state[kb][vb] = multiply(k0, k1, rest[vb][0], rest[vb][1], state[kb][vb]);
+#pragma unroll
+                        for (int vb = 0; vb < VB; vb++) state[kb][vb] = multiply(k0, k1, h[vb][0], h[vb][1], state[kb][vb]);
+                    }
                 }
             } else {
 #pragma unroll

@@ -32,10 +32,10 @@ def bounds(q, k, v, decay, state, starts, scale):
 def allowed(dtype, key, steps):
     """(factor of the sums of absolute values for out, for states): in 32 bits
     a term goes through the sums over `key` and over the steps, here or in
-    blocks; in bfloat16 the scores are rounded once, states and what enters
-    them are kept as two numbers, to 2^-16."""
+    blocks; in bfloat16 the scores are rounded once, and the state that they
+    are multiplied with is two numbers, to 2^-16."""
     wide = (key + steps + 64) * 2.0 ** -24
-    return (wide, wide) if dtype != torch.bfloat16 else (2.0 ** -8 + 2.0 ** -15 + wide, 2.0 ** -15 + wide)
+    return (wide, wide) if dtype != torch.bfloat16 else (2.0 ** -8 + 2.0 ** -16 + wide, wide)
 
 
 def close(got, want, bound, out_type):
