@@ -41,6 +41,11 @@ constexpr size_t kMostArguments = 4096;          // bytes of a launch
 constexpr int kTile = 128, kStep = 32;           // of a product: rows and columns, and what is summed at once
 constexpr int kCut = 64;                         // tile of the first x
 constexpr int kMostParts = 256;                  // workgroups that a matrix' gradient is gone over by
+/* Where row r of a side that is read across lies in LDS: the 32 bytes that 16
+ * lanes fetch of each of four rows, and those of the rows 8 on, are in
+ * different banks. */
+constexpr int across_row(int r) { return r * (kTile * 4 + 32) + r / 8 * 128; }
+constexpr int kSideLds = across_row(kStep), kProductLds = 4 * kSideLds;      // bytes: two of either side
 constexpr int64_t kPart = 4096;                  // its elements at the least
 constexpr double kA = 3.4445, kB = -4.7750, kC = 2.0315;
 constexpr float kScale = 8192.0f, kCollected = 16.0f;      // of x, y and z, and of p, whose singular values reach 3.4445^5
@@ -327,6 +332,7 @@ __device__ __forceinline__ void move(const Common& c, const Matrix& t, int64_t i
 
 /* The weights from row r0 and column c0 on, by a tile of x that lies as they do. */
 constexpr int kMoveRow = kTile + 4;
+static_assert(kTile * kMoveRow * 4 <= kProductLds, "a tile of x");
 template <typename T>
 __device__ __forceinline__ void move_tile(const Common& c, const Matrix& t, const float* tile, int64_t r0, int64_t c0) {
     constexpr int kAcross = kTile / 4, kDown = kThreads / kAcross, kAhead = 4;
@@ -358,15 +364,19 @@ __device__ __forceinline__ void move_tile(const Common& c, const Matrix& t, cons
     }
 }
 
+/* Where the 16 bytes k of a row of 128 bytes lie: two rows to all banks, turned
+ * so that 16 rows' same bytes, and neighbouring ones, lie in different banks. */
+__device__ __forceinline__ int in_row(int row, int k) { return row / 2 * 256 + (row % 2 * 8 + (k ^ row / 2 % 8)) * 16; }
+
 /* Four waves, each with 64 x 64 of the tile.  A step of 32 of what is summed
  * is fetched into registers while the one before is worked on, and goes to
  * the other half of LDS. */
 template <Product KIND>
 __global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
     constexpr bool kAcross = KIND == NEXT || KIND == LAST;      // the right side's rows are what is summed over
-    constexpr int kRow = kStep * 4 + 16, kAcrossRow = kTile * 4 + 32;      // bytes of a row in LDS, in different banks
-    constexpr int kSide = kTile * kRow, kLoads = kTile * kStep * 4 / 16 / kThreads;
-    static_assert(kStep * kAcrossRow <= kSide, "either side");
+    constexpr int kRow = kStep * 4;                             // bytes of a row in LDS
+    constexpr int kSide = kSideLds, kLoads = kTile * kStep * 4 / 16 / kThreads;
+    static_assert(kTile * kRow <= kSide, "either side");
     extern __shared__ __attribute__((aligned(16))) char shared[];
     const Place p = l.c.places[l.c.first + by_die()];
     const Matrix& t = l.c.matrices[p.matrix];
@@ -413,23 +423,19 @@ __global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
     auto put = [&](char* to) {
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {
-            *(U4*)(to + (tid / 8 + i * 32) * kRow + tid % 8 * 16) = a[i];
-            if (kAcross) *(U4*)(to + kSide + (tid / 32 + i * 8) * kAcrossRow + tid % 32 * 16) = b[i];
-            else *(U4*)(to + kSide + (tid / 8 + i * 32) * kRow + tid % 8 * 16) = b[i];
+            *(U4*)(to + in_row(tid / 8 + i * 32, tid % 8)) = a[i];
+            if (kAcross) *(U4*)(to + kSide + across_row(tid / 32 + i * 8) + tid % 32 * 16) = b[i];
+            else *(U4*)(to + kSide + in_row(tid / 8 + i * 32, tid % 8)) = b[i];
         }
     };
-    /* eight of what is summed to a lane: from 8 g on, or (across) from 4 g and from 16 + 4 g on */
-    auto row_of = [&](const char* at) {
-        if (!kAcross) return *(const H8*)(at + g * 16);
-        const H4 u = *(const H4*)(at + g * 8), v = *(const H4*)(at + g * 8 + 32);
-        return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
-    };
+    /* eight of what is summed to a lane, from 8 g on; `rest` is 4 for those of what is left */
+    auto row_of = [&](const char* at, int row, int rest) { return *(const H8*)(at + in_row(row, rest + g)); };
     /* the hardware turns four elements of 16 lanes: lane 4 r + k fetches those of row r from 4 k on */
     auto column_of = [&](const char* at) {
         typedef __attribute__((address_space(3))) S4* Lds;
-        const char* q = at + (4 * g + c / 4) * kAcrossRow + c % 4 * 8;
+        const char* q = at + across_row(8 * g + c / 4) + c % 4 * 8;
         const S4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)q);
-        const S4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(q + 16 * kAcrossRow));
+        const S4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(q + across_row(4)));
         return __builtin_bit_cast(H8, __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7));
     };
     F4 d[4][4];
@@ -449,8 +455,8 @@ __global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
         H8 lh[4], ll[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            lh[i] = row_of(at + (wi + 16 * i + c) * kRow);
-            ll[i] = row_of(at + (wi + 16 * i + c) * kRow + kStep * 2);
+            lh[i] = row_of(at, wi + 16 * i + c, 0);
+            ll[i] = row_of(at, wi + 16 * i + c, 4);
         }
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -460,8 +466,8 @@ __global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
                 rh = column_of(q);
                 rl = column_of(q + kStep * 2);
             } else {
-                rh = row_of(at + kSide + (wj + 16 * j + c) * kRow);
-                rl = row_of(at + kSide + (wj + 16 * j + c) * kRow + kStep * 2);
+                rh = row_of(at + kSide, wj + 16 * j + c, 0);
+                rl = row_of(at + kSide, wj + 16 * j + c, 4);
             }
             /* rows of the tile along the right side's: a lane has four neighbouring columns of one row of out */
 #pragma unroll
@@ -706,10 +712,9 @@ hipError_t over(int64_t first, int64_t end, F launch) {
 
 template <Product KIND>
 hipError_t launch_product(ProductLaunch l, int64_t first, int64_t end, hipStream_t stream, unsigned both = 1) {
-    constexpr int kLds = 4 * kTile * (kStep * 4 + 16);
     return over(first, end, [&](int64_t at, unsigned blocks) {
         l.c.first = at;
-        mu_product<KIND><<<dim3(blocks, both), kThreads, kLds, stream>>>(l);
+        mu_product<KIND><<<dim3(blocks, both), kThreads, kProductLds, stream>>>(l);
     });
 }
 
@@ -721,7 +726,7 @@ bool is_small(int64_t rows, int64_t columns) {
 template <Product KIND>
 hipError_t allow_lds() {
     return hipFuncSetAttribute((const void*)mu_product<KIND>, hipFuncAttributeMaxDynamicSharedMemorySize,
-        4 * kTile * (kStep * 4 + 16));
+        kProductLds);
 }
 
 }  // namespace
