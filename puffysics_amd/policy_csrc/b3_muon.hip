@@ -364,6 +364,28 @@ __device__ __forceinline__ void move_tile(const Common& c, const Matrix& t, cons
     }
 }
 
+/* Writes a tile's rows from r0 and blocks of columns from b0 on, a row's line of
+ * 128 bytes by four threads. */
+__device__ __forceinline__ void store_tile(char* work, int64_t base, int64_t columns, int64_t r0, int64_t b0,
+    const uint32_t* tile) {
+#pragma unroll 4
+    for (int k = threadIdx.x; k < kTile * kTile / 8; k += kThreads) {
+        const int row = k / (kTile / 8), o = k % (kTile / 8) * 8;
+        const U4 a = *(const U4*)(tile + row * kMoveRow + o), b = *(const U4*)(tile + row * kMoveRow + o + 4);
+        U4 h, rest;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            h[e] = (a[2 * e] & 0xffffu) | a[2 * e + 1] << 16;
+            h[e + 2] = (b[2 * e] & 0xffffu) | b[2 * e + 1] << 16;
+            rest[e] = a[2 * e] >> 16 | (a[2 * e + 1] & 0xffff0000u);
+            rest[e + 2] = b[2 * e] >> 16 | (b[2 * e + 1] & 0xffff0000u);
+        }
+        _Float16* to = block_of(work, base, columns, r0 + row, b0 + o / kStep) + o % kStep;
+        *(U4*)to = h;
+        *(U4*)(to + kStep) = rest;
+    }
+}
+
 /* Where the 16 bytes k of a row of 128 bytes lie: two rows to all banks, turned
  * so that 16 rows' same bytes, and neighbouring ones, lie in different banks. */
 __device__ __forceinline__ int in_row(int row, int k) { return row / 2 * 256 + (row % 2 * 8 + (k ^ row / 2 % 8)) * 16; }
@@ -505,43 +527,47 @@ __global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
         else move_tile<__bf16>(l.c, t, tile, r0, c0);
         return;
     }
+    const int64_t columns = KIND == NEXT ? t.n : t.m;
+    uint32_t* tile = (uint32_t*)shared;          // halves, and what is left of them in the high bits
+    U4 both[4][4];
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const int64_t row = (int64_t)p.i * kTile + wi + 16 * i + c, col = (int64_t)p.j * kTile + wj + 16 * j + 4 * g;
+            const int row = wi + 16 * i + c, col = wj + 16 * j + 4 * g;
             F4 y;
 #pragma unroll
             for (int r = 0; r < 4; r++) y[r] = d[i][j][r] * scale;
-            const int64_t columns = KIND == NEXT ? t.n : t.m;
-            const int64_t block = col / kStep, o = col % kStep;
             if (KIND == POLYNOMIAL) {
-                const _Float16* own = block_of(l.c.work, t.y, columns, row, block) + o;
+                const int64_t at = (int64_t)p.j * kTile + col;
+                const _Float16* own = block_of(l.c.work, t.y, columns, (int64_t)p.i * kTile + row, at / kStep) + at % kStep;
                 const H4 h = *(const H4*)own, rest = *(const H4*)(own + kStep);
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     y[r] = __builtin_fmaf((float)kC, y[r], (float)kB * ((float)h[r] + (float)rest[r]));
-                    if (row == col + r) y[r] += (float)kA * kScale;
+                    if (p.i == p.j && row == col + r) y[r] += (float)kA * kScale;
                 }
             }
-            H4 h, rest;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                h[r] = (_Float16)y[r];
-                rest[r] = (_Float16)(y[r] - (float)h[r]);
+                const _Float16 h = (_Float16)y[r], rest = (_Float16)(y[r] - (float)h);
+                both[i][j][r] = (uint32_t)__builtin_bit_cast(uint16_t, rest) << 16 | __builtin_bit_cast(uint16_t, h);
             }
-            _Float16* to = block_of(l.c.work, out, columns, row, block) + o;
-            *(H4*)to = h;
-            *(H4*)(to + kStep) = rest;
-            if (KIND != NEXT && p.i != p.j) {
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    _Float16* other = block_of(l.c.work, out, columns, col + r, row / kStep) + row % kStep;
-                    other[0] = h[r];
-                    other[kStep] = rest[r];
-                }
-            }
+            *(U4*)(tile + row * kMoveRow + col) = both[i][j];
         }
+    __syncthreads();
+    store_tile(l.c.work, out, columns, (int64_t)p.i * kTile, (int64_t)p.j * (kTile / kStep), tile);
+    if (KIND == NEXT || p.i == p.j) return;
+    /* and the tile across from it */
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) tile[(wj + 16 * j + 4 * g + r) * kMoveRow + wi + 16 * i + c] = both[i][j][r];
+    __syncthreads();
+    store_tile(l.c.work, out, columns, (int64_t)p.j * kTile, (int64_t)p.i * (kTile / kStep), tile);
 }
 
 /* ---- small matrices ---- */
