@@ -391,8 +391,8 @@ __device__ __forceinline__ void store_tile(char* work, int64_t base, int64_t col
 __device__ __forceinline__ int in_row(int row, int k) { return row / 2 * 256 + (row % 2 * 8 + (k ^ row / 2 % 8)) * 16; }
 
 /* Four waves, each with 64 x 64 of the tile.  A step of 32 of what is summed
- * is fetched into registers while the one before is worked on, and goes to
- * the other half of LDS. */
+ * is fetched into registers while the two before are worked on, since one takes
+ * less time than memory does, and goes to the other half of LDS. */
 template <Product KIND>
 __global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
     constexpr bool kAcross = KIND == NEXT || KIND == LAST;      // the right side's rows are what is summed over
@@ -434,20 +434,22 @@ __global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
     const char* from_right = l.c.work + right * 4
         + (kAcross ? (int64_t)(tid / 32) * t.n * 4 + (int64_t)p.j * kTile * 4 + tid % 32 * 16
                    : ((int64_t)p.j * kTile + tid / 8) * sum * 4 + tid % 8 * 16);
-    U4 a[kLoads], b[kLoads];
-    auto fetch = [&](int64_t k) {
+    struct Fetched {
+        U4 a[kLoads], b[kLoads];
+    } even, odd;                                 // steps to come
+    auto fetch = [&](Fetched& f, int64_t k) {
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {
-            a[i] = *(const U4*)(from_left + i * 32 * sum * 4 + k * 4);
-            b[i] = kAcross ? *(const U4*)(from_right + (k + i * 8) * t.n * 4) : *(const U4*)(from_right + i * 32 * sum * 4 + k * 4);
+            f.a[i] = *(const U4*)(from_left + i * 32 * sum * 4 + k * 4);
+            f.b[i] = kAcross ? *(const U4*)(from_right + (k + i * 8) * t.n * 4) : *(const U4*)(from_right + i * 32 * sum * 4 + k * 4);
         }
     };
-    auto put = [&](char* to) {
+    auto put = [&](const Fetched& f, char* to) {
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {
-            *(U4*)(to + in_row(tid / 8 + i * 32, tid % 8)) = a[i];
-            if (kAcross) *(U4*)(to + kSide + across_row(tid / 32 + i * 8) + tid % 32 * 16) = b[i];
-            else *(U4*)(to + kSide + in_row(tid / 8 + i * 32, tid % 8)) = b[i];
+            *(U4*)(to + in_row(tid / 8 + i * 32, tid % 8)) = f.a[i];
+            if (kAcross) *(U4*)(to + kSide + across_row(tid / 32 + i * 8) + tid % 32 * 16) = f.b[i];
+            else *(U4*)(to + kSide + in_row(tid / 8 + i * 32, tid % 8)) = f.b[i];
         }
     };
     /* eight of what is summed to a lane, from 8 g on; `rest` is 4 for those of what is left */
@@ -465,15 +467,7 @@ __global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
     for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++) d[i][j] = F4{0, 0, 0, 0};
-    fetch(0);
-    put(shared);
-    __syncthreads();
-    int half = 0;
-#pragma unroll 1
-    for (int64_t k = 0; k < sum; k += kStep) {
-        const bool more = k + kStep < sum;
-        if (more) fetch(k + kStep);
-        const char* at = shared + half * 2 * kSide;
+    auto work = [&](const char* at) {
         H8 lh[4], ll[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -499,8 +493,22 @@ __global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
 #pragma unroll
             for (int i = 0; i < 4; i++) d[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rh, lh[i], d[i][j], 0, 0, 0);
         }
-        half ^= 1;
-        if (more) put(shared + half * 2 * kSide);
+    };
+    fetch(even, 0);
+    fetch(odd, kStep);
+    put(even, shared);
+    __syncthreads();
+    /* (sums are of whole tiles: an even number of steps) */
+#pragma unroll 1
+    for (int64_t k = 0; k < sum; k += 2 * kStep) {
+        const bool more = k + 2 * kStep < sum;
+        if (more) fetch(even, k + 2 * kStep);
+        work(shared);
+        put(odd, shared + 2 * kSide);
+        __syncthreads();
+        if (more) fetch(odd, k + 3 * kStep);
+        work(shared + 2 * kSide);
+        if (more) put(even, shared);
         __syncthreads();
     }
     if (KIND == LAST) {
