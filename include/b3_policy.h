@@ -199,6 +199,7 @@ hipError_t b3_adamw_destroy(B3AdamW* optimizer);
 /* ---- linear attention ---- */
 
 #define B3_MAX_HEAD 128
+#define B3_MAX_SEQUENCES (1 << 22)
 
 /* q and k [steps, envs, heads, key], v [steps, envs, heads, value]: strides
  * in elements from step to step, environment to environment and head to
@@ -208,7 +209,7 @@ hipError_t b3_adamw_destroy(B3AdamW* optimizer);
  * there).  `state` [envs, heads, key, value], contiguous, is what the first
  * step finds; NULL: zeros. */
 typedef struct B3Attention {
-    int64_t steps, envs, heads;
+    int64_t steps, envs, heads;  /* envs * heads at most B3_MAX_SEQUENCES */
     int key, value;              /* 1 .. B3_MAX_HEAD */
     int type;                    /* of q, k, v, the result and gradients */
     const void *q, *k, *v;

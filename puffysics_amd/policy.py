@@ -29,7 +29,7 @@ MAX_TOP = 32
 MAX_ACTIONS = 1 << 21
 MAX_ROWS = (1 << 31) - 1     # and steps and environments of a rollout
 MAX_HEAD = 128               # dimensions of a head of linear attention
-MAX_SEQUENCES = (1 << 24) - 1
+MAX_SEQUENCES = 1 << 22      # environments times heads
 MAX_WIDTH = 1 << 21          # of a norm's row
 SEGMENT = 256
 _GROUP = 32                  # 8-bit numbers to a scale
@@ -456,7 +456,7 @@ def _check_attention(q, k, v, decay, starts, scale):
     _need(decay.dtype == torch.float32 and decay.dim() == 1 and decay.shape[0] == shape[-2], "decay has to be float32 [heads]")
     _need(not decay.requires_grad, "decay has no gradient")
     if shape[-3] * shape[-2] > MAX_SEQUENCES or (len(shape) == 4 and shape[0] > MAX_ROWS):
-        raise ValueError("at most 2^24 - 1 sequences (environments times heads) and 2^31 - 1 steps")
+        raise ValueError("at most 2^22 sequences (environments times heads) and 2^31 - 1 steps")
     if starts is not None:
         _need(starts.shape == shape[:-2] and starts.dtype in (torch.float32, torch.bool, torch.uint8),
               "starts have to be float32, bool or uint8, one for each step and environment")

@@ -24,6 +24,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kRoles = 3;                        // of a launch
+static_assert((int64_t)B3_MAX_SEQUENCES * kRoles * kThreads < (int64_t)1 << 32, "threads of a launch");
 constexpr int64_t kWaves = 2048;                 // that a launch of few sequences is cut into
 constexpr int64_t kPieceChunks = 4;              // of a piece at the least
 
@@ -817,7 +818,7 @@ bool valid(const B3Attention* g) {
         return false;
     if (g->starts && g->starts_type != B3_F32 && g->starts_type != B3_U8) return false;
     if (g->envs == 0 || g->heads == 0) return true;
-    if (g->envs > 0x7fffffff || g->heads > 0x7fffffff || g->steps > 0x7fffffff || g->envs * g->heads > kMostBlocks) return false;
+    if (g->envs > 0x7fffffff || g->heads > 0x7fffffff || g->steps > 0x7fffffff || g->envs * g->heads > B3_MAX_SEQUENCES) return false;
     return g->steps == 0 || (g->q && g->k && g->v && g->decay);
 }
 

@@ -22,6 +22,7 @@ constexpr int kVec = 8;
 constexpr int kMostInRegisters = kThreads * kVec * 8;
 constexpr int64_t kMaxWidth = 1 << 21;
 constexpr int64_t kForwardBlocks = 2048, kBackwardBlocks = 1024;
+constexpr int64_t kMostSums = 1 << 25;           // of long rows: floats of the workgroups' sums
 constexpr int kGroup = 32;                       // 8 bits: elements to a scale
 constexpr int kSumColumns = 64, kSumSlices = 16;
 
@@ -419,7 +420,9 @@ int lanes_of(int64_t width) {
 
 int64_t blocks_of(int64_t rows, int64_t width, bool backward) {
     const int lanes = lanes_of(width);
-    const int64_t need = ceil_div(rows, lanes ? kThreads / lanes : 1), most = backward ? kBackwardBlocks : kForwardBlocks;
+    int64_t most = backward ? kBackwardBlocks : kForwardBlocks;
+    if (backward && !lanes && most > kMostSums / width) most = kMostSums / width;
+    const int64_t need = ceil_div(rows, lanes ? kThreads / lanes : 1);
     return need < most ? need : most;
 }
 
@@ -438,7 +441,7 @@ void launch_typed(const Job& j, hipStream_t stream) {
     else if (v <= 2048) launch_row<T, 256, 8, PASS>(j, blocks, stream);
     else if (PASS != BACKWARD) rn_forward_long<T, PASS == FORWARD_8BIT><<<blocks, kThreads, 0, stream>>>(j);
     else {
-        rn_dot<T><<<blocks, kThreads, 0, stream>>>(j);
+        rn_dot<T><<<(unsigned)blocks_of(j.g.rows, width, false), kThreads, 0, stream>>>(j);
         rn_backward_long<T><<<dim3((unsigned)ceil_div(v, kThreads), blocks), kThreads, 0, stream>>>(j);
     }
 }

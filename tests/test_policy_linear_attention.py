@@ -386,6 +386,60 @@ def test_gradients_add_up_and_are_differentiable_once():
     assert torch.allclose(total, sum(each), rtol=1e-5, atol=1e-5)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("size", [(5, 2, 2, 64, 64), (40, 1, 2, 128, 128), (2000, 1, 1, 32, 32)])
+def test_a_dropped_state_is_not_seen(size, type):
+    """NaN in a state that an episode's start drops, forwards and back."""
+    from puffysics_amd import policy
+    q, k, v, decay, starts, state = made(*size, TYPES[type], 21, rate=0.0)
+    starts[0] = True
+    nan = torch.full_like(state, float("nan"))
+    leaves = [x.requires_grad_() for x in (q, k, v, nan)]
+    got = policy.linear_attention(q, k, v, decay, state=nan, starts=starts, last=True)
+    want = policy.linear_attention(q.detach(), k.detach(), v.detach(), decay, starts=starts, last=True)
+    assert torch.equal(got.state, want.state) and torch.equal(got.out, want.out)
+    grads = torch.autograd.grad(got.out, leaves, torch.ones_like(v))
+    assert all(torch.isfinite(g).all() for g in grads) and int(torch.count_nonzero(grads[3])) == 0
+    s = nan.detach().clone()
+    out = policy.linear_attention_step(q[0].detach(), k[0].detach(), v[0].detach(), decay, s, starts=starts[0])
+    assert torch.isfinite(out).all() and torch.isfinite(s).all()
+
+
+@pytest.mark.gpu
+def test_negated_arrays():
+    """Tensors that are only marked as negated are read as what they are."""
+    from puffysics_amd import policy
+    from test_policy_arguments import negated
+    q, k, v, decay, starts, state = made(20, 2, 2, 8, 8, torch.float32, 22)
+    d = torch.randn_like(v)
+    want = policy.linear_attention(q, k, v, decay, state=state, last=True)
+    got = policy.linear_attention(negated(q), negated(k), negated(v), negated(decay), state=negated(state), last=True)
+    assert torch.equal(got.out, want.out) and torch.equal(got.state, want.state)
+    x = q.clone().requires_grad_()
+    a, = torch.autograd.grad(policy.linear_attention(x, k, v, decay).out, x, d)
+    b, = torch.autograd.grad(policy.linear_attention(x, k, v, decay).out, x, negated(d))
+    assert torch.equal(a, b)
+    s, t = state.clone(), state.clone()
+    assert torch.equal(policy.linear_attention_step(q[0], k[0], v[0], decay, s),
+                       policy.linear_attention_step(negated(q[0]), negated(k[0]), negated(v[0]), decay, t)) and torch.equal(s, t)
+
+
+@pytest.mark.gpu
+def test_many_sequences():
+    """The most there may be, of one step."""
+    from puffysics_amd import policy
+    envs, heads = 2 ** 20, 4
+    q = torch.randn(1, envs, heads, 3, device="cuda")
+    x = q.clone().requires_grad_()
+    decay = torch.ones(heads, device="cuda")
+    out = policy.linear_attention(x, x, x, decay).out
+    want = (q * q).sum(-1, keepdim=True) * q
+    assert torch.allclose(out, want, rtol=1e-5, atol=1e-5)
+    d, = torch.autograd.grad(out, x, torch.ones_like(out))
+    assert torch.allclose(d, (q * q).sum(-1, keepdim=True) + 2 * q * q.sum(-1, keepdim=True), rtol=1e-4, atol=1e-4)
+
+
 def test_refusals():
     """Nothing is launched: this runs without a GPU."""
     from puffysics_amd import policy
@@ -400,7 +454,8 @@ def test_refusals():
             ("no gradient", dict(decay=z(2, requires_grad=True))), ("state", dict(state=s.half())),
             ("state", dict(state=s[:2])), ("starts", dict(starts=z(5, 2))), ("starts", dict(starts=z(5, 3).double())),
             ("finite", dict(scale=float("nan"))), ("finite", dict(scale=float("inf"))),
-            ("2\\^24", dict(q=z(1).expand(1, 2 ** 23, 2, 8), k=z(1).expand(1, 2 ** 23, 2, 8), v=z(1).expand(1, 2 ** 23, 2, 4))),
+            ("2\\^22", dict(q=z(1).expand(1, 2 ** 21 + 1, 2, 8), k=z(1).expand(1, 2 ** 21 + 1, 2, 8),
+                             v=z(1).expand(1, 2 ** 21 + 1, 2, 4))),
             ("2\\^31", dict(q=z(1).expand(2 ** 31, 1, 2, 8), k=z(1).expand(2 ** 31, 1, 2, 8), v=z(1).expand(2 ** 31, 1, 2, 4))),
             ("CUDA device", {})):
         with pytest.raises(ValueError, match=what):
@@ -434,7 +489,7 @@ def test_c_refusals():
         return lib.b3_linear_attention_gpu(C.byref(g), None if change.get("steps") != 0 else None, None, None, 0, None)
 
     for change in (dict(key=0), dict(key=129), dict(value=0), dict(value=129), dict(type=3), dict(steps=-1), dict(envs=-1),
-                   dict(heads=-1), dict(q=None), dict(decay=None), dict(envs=1 << 24), dict(steps=1 << 31), dict(),
+                   dict(heads=-1), dict(q=None), dict(decay=None), dict(envs=(1 << 22) + 1), dict(steps=1 << 31), dict(),
                    dict(starts=at, starts_type=2), dict(scale=float("nan"))):
         assert call(**change) == 1, change
     assert call(envs=0) == 0 and call(heads=0) == 0 and call(steps=0) == 0

@@ -262,6 +262,37 @@ def test_streams_and_replays():
 
 
 @pytest.mark.gpu
+def test_negated_arrays():
+    """Tensors that are only marked as negated are read as what they are."""
+    from puffysics_amd import policy
+    from test_policy_arguments import negated
+    x, r, w, dy, dh = made(6, 50, torch.float32, 4)
+    want, got = policy.rms_norm(x, w, residual=r), policy.rms_norm(negated(x), negated(w), residual=negated(r))
+    assert torch.equal(got.out, want.out) and torch.equal(got.sum, want.sum)
+    a, b = policy.rms_norm_8bit(x, w, residual=r), policy.rms_norm_8bit(negated(x), negated(w), residual=negated(r))
+    assert torch.equal(a.out.view(torch.uint8), b.out.view(torch.uint8)) and torch.equal(a.sum, b.sum)
+    leaf = x.clone().requires_grad_()
+    c, = torch.autograd.grad(policy.rms_norm(leaf, w).out, leaf, dy)
+    d, = torch.autograd.grad(policy.rms_norm(leaf, w).out, leaf, negated(dy))
+    assert torch.equal(c, d)
+
+
+@pytest.mark.gpu
+def test_the_longest_rows():
+    """Of 2^21 elements, whose weights' gradient is summed by few workgroups."""
+    from puffysics_amd import policy
+    x = torch.randn(20, 2 ** 21, device="cuda").requires_grad_()
+    w = torch.ones(2 ** 21, device="cuda").requires_grad_()
+    out = policy.rms_norm(x, w).out
+    y, _, s = norm_oracle(x.detach(), None, None, 1e-6)
+    # a lane of 256 adds 1,024 vectors of 8 one after the other
+    assert (out - y).abs().max() < 1040 * 2.0 ** -24 * float(y.abs().max())
+    dx, dw = torch.autograd.grad(out, (x, w), out.detach())
+    assert (dw - y.square().sum(0)).abs().max() < 1100 * 2.0 ** -23 * float(y.square().sum(0).max())
+    assert torch.isfinite(dx).all()
+
+
+@pytest.mark.gpu
 def test_places_past_32_bits():
     """The last rows of an array of more than 2^32 bytes, and of 2^31 elements."""
     from puffysics_amd import policy
