@@ -6,8 +6,9 @@
  *   dh = d_h + s (w dy - h s mean(w dy h s)), dw = sum over rows of dy h s
  *
  * Everything is read once and written once, so that memory bounds it.  G lanes
- * share a row and hold it in registers, NV vectors of 8 neighbouring elements
- * each: 4 to 64 lanes of a wave, or a workgroup's 256 beyond 2,048 elements.
+ * share a row and hold it in registers, one or two vectors of 8 neighbouring
+ * elements each: 4 to 64 lanes of a wave, or a workgroup's 256 beyond 1,024
+ * elements and 1,024 beyond 4,096.
  * Rows of more than 16,384 are gone over twice.  A lane keeps its columns from
  * row to row: of the weights' gradient each workgroup writes the sums over its
  * rows, in one order always, and a second launch adds these.
@@ -19,7 +20,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kVec = 8;
-constexpr int kMostInRegisters = kThreads * kVec * 8;
+constexpr int kWide = 1024;                      // lanes to the longest rows that registers hold
+constexpr int kMostInRegisters = kWide * kVec * 2;
 constexpr int64_t kMaxWidth = 1 << 21;
 constexpr int64_t kForwardBlocks = 2048, kBackwardBlocks = 1024;
 constexpr int64_t kMostSums = 1 << 25;           // of long rows: floats of the workgroups' sums
@@ -41,16 +43,30 @@ struct Job {
     float* dot;                                  // [rows], of long rows
 };
 
-/* Eight elements of a row, zeros past its end; left is what lies from p on. */
+/* Eight elements of a row of `width` from column c on, zeros past its end.  Of
+ * the last ones, fewer than eight, the eight that end the row are fetched and
+ * moved down: by the same steps in all rows. */
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, int64_t left, float x[kVec]) {
-    if (left >= kVec) {
-        const Pack<T, kVec> v = *(const Pack<T, kVec>*)p;
+__device__ __forceinline__ void load8(const T* row, int64_t c, int64_t width, float x[kVec]) {
+    const int64_t left = width - c;
+    const int past = (int)(-width & (kVec - 1));
+    if (left <= 0) {
+#pragma unroll
+        for (int k = 0; k < kVec; k++) x[k] = 0.0f;
+    } else if (left >= kVec || width >= kVec) {
+        const Pack<T, kVec> v = *(const Pack<T, kVec>*)(row + (left >= kVec ? c : width - kVec));
 #pragma unroll
         for (int k = 0; k < kVec; k++) x[k] = to_float(v.v[k]);
+        if (past && left < kVec) {
+#pragma unroll
+            for (int s = kVec / 2; s; s /= 2) {
+#pragma unroll
+                for (int k = 0; k < kVec; k++) x[k] = past & s ? (k + s < kVec ? x[k + s] : 0.0f) : x[k];
+            }
+        }
     } else {
 #pragma unroll
-        for (int k = 0; k < kVec; k++) x[k] = k < left ? to_float(p[k]) : 0.0f;
+        for (int k = 0; k < kVec; k++) x[k] = k < left ? to_float(row[c + k]) : 0.0f;
     }
 }
 
@@ -74,9 +90,9 @@ __device__ __forceinline__ void load_weight(const B3Norm& g, int64_t c, float w[
 #pragma unroll
         for (int k = 0; k < kVec; k++) w[k] = 1.0f;
     } else if (g.weight_type == B3_F32) {
-        load8((const float*)g.weight + c, g.width - c, w);
+        load8((const float*)g.weight, c, g.width, w);
     } else {
-        load8((const T*)g.weight + c, g.width - c, w);
+        load8((const T*)g.weight, c, g.width, w);
     }
 }
 
@@ -99,10 +115,10 @@ __device__ __forceinline__ float row_sum(float x, float* lds) {
 /* h of eight elements. */
 template <typename T>
 __device__ __forceinline__ void load_h(const B3Norm& g, int64_t r, int64_t c, float h[kVec]) {
-    load8((const T*)g.x + r * g.x_stride + c, g.width - c, h);
+    load8((const T*)g.x + r * g.x_stride, c, g.width, h);
     if (g.residual) {
         float d[kVec];
-        load8((const T*)g.residual + r * g.residual_stride + c, g.width - c, d);
+        load8((const T*)g.residual + r * g.residual_stride, c, g.width, d);
 #pragma unroll
         for (int k = 0; k < kVec; k++) h[k] += d[k];
     }
@@ -167,15 +183,18 @@ __device__ __forceinline__ float root_of(const Job& j, float squares) {
     return rsqrtf(squares / (float)j.g.width + j.eps);
 }
 
+/* Threads of a workgroup whose rows have G lanes. */
+constexpr int threads_of(int g) { return g > kThreads ? g : kThreads; }
+
 template <typename T, int G, int NV, bool BITS8>
-__global__ __launch_bounds__(kThreads) void rn_forward(Job j) {
-    __shared__ float lds[kThreads / kWave];
+__global__ __launch_bounds__(threads_of(G)) void rn_forward(Job j) {
+    constexpr int kGroups = threads_of(G) / G;
+    __shared__ float lds[threads_of(G) / kWave];
     const int lane = threadIdx.x % G;
     float w[NV][kVec];
 #pragma unroll
     for (int v = 0; v < NV; v++) load_weight<T>(j.g, (v * G + lane) * kVec, w[v]);
-    for (int64_t r = (int64_t)blockIdx.x * (kThreads / G) + threadIdx.x / G; r < j.g.rows;
-            r += (int64_t)gridDim.x * (kThreads / G)) {
+    for (int64_t r = (int64_t)blockIdx.x * kGroups + threadIdx.x / G; r < j.g.rows; r += (int64_t)gridDim.x * kGroups) {
         float h[NV][kVec], squares = 0;
 #pragma unroll
         for (int v = 0; v < NV; v++) load_h<T>(j.g, r, (v * G + lane) * kVec, h[v]);
@@ -226,7 +245,7 @@ __device__ __forceinline__ void write_d(const Job& j, int64_t r, int64_t c, cons
     for (int k = 0; k < kVec; k++) d[k] = s * (g[k] - u[k] * mean);
     if (j.d_sum) {
         float up[kVec];
-        load8((const T*)j.d_sum + r * j.d_sum_stride + c, j.g.width - c, up);
+        load8((const T*)j.d_sum + r * j.d_sum_stride, c, j.g.width, up);
 #pragma unroll
         for (int k = 0; k < kVec; k++) d[k] += up[k];
     }
@@ -236,7 +255,7 @@ __device__ __forceinline__ void write_d(const Job& j, int64_t r, int64_t c, cons
 template <typename T>
 __device__ __forceinline__ void load_d_out(const Job& j, int64_t r, int64_t c, float d[kVec]) {
     if (j.d_out) {
-        load8((const T*)j.d_out + r * j.d_out_stride + c, j.g.width - c, d);
+        load8((const T*)j.d_out + r * j.d_out_stride, c, j.g.width, d);
     } else {
 #pragma unroll
         for (int k = 0; k < kVec; k++) d[k] = 0;
@@ -244,9 +263,9 @@ __device__ __forceinline__ void load_d_out(const Job& j, int64_t r, int64_t c, f
 }
 
 template <typename T, int G, int NV>
-__global__ __launch_bounds__(kThreads) void rn_backward(Job j) {
-    constexpr int kGroups = kThreads / G;
-    __shared__ float lds[kThreads / kWave];
+__global__ __launch_bounds__(threads_of(G)) void rn_backward(Job j) {
+    constexpr int kGroups = threads_of(G) / G;
+    __shared__ float lds[threads_of(G) / kWave];
     __shared__ float sums[kGroups > 1 ? kThreads * kVec * NV : 1];
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
     float w[NV][kVec], dw[NV][kVec];
@@ -407,22 +426,22 @@ enum Pass { FORWARD, FORWARD_8BIT, BACKWARD };
 template <typename T, int G, int NV, Pass PASS>
 void launch_row(const Job& j, unsigned blocks, hipStream_t stream) {
     if (PASS == BACKWARD)
-        rn_backward<T, G, NV><<<blocks, kThreads, 0, stream>>>(j);
+        rn_backward<T, G, NV><<<blocks, threads_of(G), 0, stream>>>(j);
     else
-        rn_forward<T, G, NV, PASS == FORWARD_8BIT><<<blocks, kThreads, 0, stream>>>(j);
+        rn_forward<T, G, NV, PASS == FORWARD_8BIT><<<blocks, threads_of(G), 0, stream>>>(j);
 }
 
 /* Lanes to a row; 0 where registers do not hold it. */
 int lanes_of(int64_t width) {
     const int64_t v = ceil_div(width, kVec);
-    return v <= 4 ? 4 : v <= 16 ? 16 : v <= 32 ? 32 : v <= 256 ? 64 : width <= kMostInRegisters ? kThreads : 0;
+    return v <= 4 ? 4 : v <= 16 ? 16 : v <= 32 ? 32 : v <= 128 ? 64 : v <= 512 ? kThreads : width <= kMostInRegisters ? kWide : 0;
 }
 
 int64_t blocks_of(int64_t rows, int64_t width, bool backward) {
     const int lanes = lanes_of(width);
     int64_t most = backward ? kBackwardBlocks : kForwardBlocks;
     if (backward && !lanes && most > kMostSums / width) most = kMostSums / width;
-    const int64_t need = ceil_div(rows, lanes ? kThreads / lanes : 1);
+    const int64_t need = ceil_div(rows, lanes && lanes < kThreads ? kThreads / lanes : 1);
     return need < most ? need : most;
 }
 
@@ -435,10 +454,10 @@ void launch_typed(const Job& j, hipStream_t stream) {
     else if (v <= 32) launch_row<T, 32, 1, PASS>(j, blocks, stream);
     else if (v <= 64) launch_row<T, 64, 1, PASS>(j, blocks, stream);
     else if (v <= 128) launch_row<T, 64, 2, PASS>(j, blocks, stream);
-    else if (v <= 256) launch_row<T, 64, 4, PASS>(j, blocks, stream);
-    else if (v <= 512) launch_row<T, 256, 2, PASS>(j, blocks, stream);
-    else if (v <= 1024) launch_row<T, 256, 4, PASS>(j, blocks, stream);
-    else if (v <= 2048) launch_row<T, 256, 8, PASS>(j, blocks, stream);
+    else if (v <= 256) launch_row<T, kThreads, 1, PASS>(j, blocks, stream);
+    else if (v <= 512) launch_row<T, kThreads, 2, PASS>(j, blocks, stream);
+    else if (v <= 1024) launch_row<T, kWide, 1, PASS>(j, blocks, stream);
+    else if (v <= 2048) launch_row<T, kWide, 2, PASS>(j, blocks, stream);
     else if (PASS != BACKWARD) rn_forward_long<T, PASS == FORWARD_8BIT><<<blocks, kThreads, 0, stream>>>(j);
     else {
         rn_dot<T><<<(unsigned)blocks_of(j.g.rows, width, false), kThreads, 0, stream>>>(j);
