@@ -8,7 +8,7 @@
  * Everything is read once and written once, so that memory bounds it.  G lanes
  * share a row and hold it in registers, one or two vectors of 8 neighbouring
  * elements each: 4 to 64 lanes of a wave, or a workgroup's 256 beyond 1,024
- * elements and 1,024 beyond 4,096.
+ * elements, 512 beyond 2,048 and 1,024 beyond 4,096.
  * Rows of more than 16,384 are gone over twice.  A lane keeps its columns from
  * row to row: of the weights' gradient each workgroup writes the sums over its
  * rows, in one order always, and a second launch adds these.
@@ -434,7 +434,7 @@ void launch_row(const Job& j, unsigned blocks, hipStream_t stream) {
 /* Lanes to a row; 0 where registers do not hold it. */
 int lanes_of(int64_t width) {
     const int64_t v = ceil_div(width, kVec);
-    return v <= 4 ? 4 : v <= 16 ? 16 : v <= 32 ? 32 : v <= 128 ? 64 : v <= 512 ? kThreads : width <= kMostInRegisters ? kWide : 0;
+    return v <= 4 ? 4 : v <= 16 ? 16 : v <= 32 ? 32 : v <= 128 ? 64 : v <= 256 ? kThreads : v <= 512 ? 2 * kThreads : width <= kMostInRegisters ? kWide : 0;
 }
 
 int64_t blocks_of(int64_t rows, int64_t width, bool backward) {
@@ -455,7 +455,7 @@ void launch_typed(const Job& j, hipStream_t stream) {
     else if (v <= 64) launch_row<T, 64, 1, PASS>(j, blocks, stream);
     else if (v <= 128) launch_row<T, 64, 2, PASS>(j, blocks, stream);
     else if (v <= 256) launch_row<T, kThreads, 1, PASS>(j, blocks, stream);
-    else if (v <= 512) launch_row<T, kThreads, 2, PASS>(j, blocks, stream);
+    else if (v <= 512) launch_row<T, 2 * kThreads, 1, PASS>(j, blocks, stream);
     else if (v <= 1024) launch_row<T, kWide, 1, PASS>(j, blocks, stream);
     else if (v <= 2048) launch_row<T, kWide, 2, PASS>(j, blocks, stream);
     else if (PASS != BACKWARD) rn_forward_long<T, PASS == FORWARD_8BIT><<<blocks, kThreads, 0, stream>>>(j);
