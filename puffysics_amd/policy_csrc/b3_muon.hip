@@ -39,6 +39,7 @@ constexpr int kThreads = 256;
 constexpr int kBatch = 200;                      // matrices to a launch that takes gradients
 constexpr size_t kMostArguments = 4096;          // bytes of a launch
 constexpr int kTile = 128, kStep = 32;           // of a product: rows and columns, and what is summed at once
+constexpr int kSquare = 8;                       // tiles
 constexpr int kCut = 64;                         // tile of the first x
 constexpr int kMostParts = 256;                  // workgroups that a matrix' gradient is gone over by
 /* Where row r of a side that is read across lies in LDS: the 32 bytes that 16
@@ -732,6 +733,18 @@ bool overlap(const B3MuonMatrix* matrices, int count, B3MuonMatrix* sorted) {
 int64_t segment(int64_t numel) { return ceil_div(numel, B3_ADAMW_SEGMENT) * B3_ADAMW_SEGMENT; }
 
 
+/* Tiles of a matrix (`half`: on and under the diagonal), in squares of kSquare by
+ * kSquare: those that a die works on at the same time share their sides in its
+ * cache. */
+Place* place_tiles(Place* to, int matrix, int64_t rows, int64_t columns, bool half) {
+    for (int64_t r0 = 0; r0 < rows; r0 += kSquare)
+        for (int64_t c0 = 0; c0 < (half ? r0 + 1 : columns); c0 += kSquare)
+            for (int64_t r = r0; r < rows && r < r0 + kSquare; r++)
+                for (int64_t c = c0; c < c0 + kSquare && c < (half ? r + 1 : columns); c++)
+                    *to++ = Place{matrix, (int)r, (int)c};
+    return to;
+}
+
 int batch(const B3Muon* o, int base) { return o->count - base < kBatch ? o->count - base : kBatch; }
 
 int64_t filled(int64_t n) { return ceil_div(n, kTile) * kTile; }
@@ -877,8 +890,7 @@ hipError_t b3_muon_create(B3Muon** out, const B3MuonMatrix* matrices, int count,
                 for (int64_t c = 0; c < table[i].n / kCut; c++) *to++ = Place{i, (int)r, (int)c};
         for (int k = 0; k < 4 && places; k++)            // half of the tiles, then all, and of both long matrices last
             for (int i = 0; i < count; i++)
-                for (int64_t r = 0; r < table[i].m / kTile && table[i].is_long == k % 2; r++)
-                    for (int64_t c = 0; c < (k < 2 ? r + 1 : table[i].n / kTile); c++) *to++ = Place{i, (int)r, (int)c};
+                if (table[i].is_long == k % 2) to = place_tiles(to, i, table[i].m / kTile, table[i].n / kTile, k < 2);
         for (int i = 0; i < count && places; i++)
             if (o->first_small[i + 1] > o->first_small[i]) *to++ = Place{i, 0, 0};
         o->smalls = small;
