@@ -560,6 +560,8 @@ class _RmsNorm(torch.autograd.Function):
         x, residual = (total, None) if residual is not None and x.dtype == torch.float32 else (x, residual)
         ctx.save_for_backward(x, residual, weight, root)
         ctx.set_materialize_grads(False)
+        if len(shape) == 2:
+            return out, total
         return out.view(shape), None if total is None else total.view(shape)
 
     @staticmethod
@@ -573,16 +575,18 @@ def _norm_backward(ctx, d_out, d_sum):
     lib = policy_lib()
     shape = (d_sum if d_out is None else d_out).shape
     d_out, d_sum = _as_rows(d_out), _as_rows(d_sum)
-    stride = lambda y: 0 if y is None else y.stride(0) if rows > 1 else width  # noqa: E731
+    # the stride of a lone row says nothing
+    out_stride, sum_stride = (0 if d is None else d.stride(0) if rows > 1 else width for d in (d_out, d_sum))
     d_x = torch.empty_like(x, memory_format=torch.contiguous_format)
     d_weight = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
     size = lib.b3_rms_norm_backward_workspace(rows, width)
     work = _work(size, x.device)
     _check("b3_rms_norm_backward_gpu", lib.b3_rms_norm_backward_gpu(
-        _norm(x, residual, weight, 0.0), root.data_ptr(), _address_of(d_out), stride(d_out), _address_of(d_sum), stride(d_sum), d_x.data_ptr(),
+        _norm(x, residual, weight, 0.0), root.data_ptr(), _address_of(d_out), out_stride, _address_of(d_sum), sum_stride, d_x.data_ptr(),
         _address_of(d_weight), _address_of(work), size, _stream()))
     # one tensor for both, as a sum's gradient is: views of it would become the grad of two leaves
-    d_x = d_x.view(shape)
+    if len(shape) != 2:
+        d_x = d_x.view(shape)
     return (d_x if ctx.needs_input_grad[0] else None, d_weight, d_x if ctx.needs_input_grad[2] else None, None)
 
 

@@ -24,6 +24,7 @@ constexpr int kWide = 1024;                      // lanes to the longest rows th
 constexpr int kMostInRegisters = kWide * kVec * 2;
 constexpr int64_t kMaxWidth = 1 << 21;
 constexpr int64_t kForwardBlocks = 2048, kBackwardBlocks = 1024;
+constexpr int64_t kAlone = 4;                    // turns of one workgroup over its rows
 constexpr int64_t kMostSums = 1 << 25;           // of long rows: floats of the workgroups' sums
 constexpr int kGroup = 32;                       // 8 bits: elements to a scale
 constexpr int kSumColumns = 64, kSumSlices = 16;
@@ -39,7 +40,8 @@ struct Job {
     int64_t d_out_stride;
     const void* d_sum;
     int64_t d_sum_stride;
-    float* partial;                              // [workgroups][width]
+    float* partial;                              // [workgroups][width], or NULL
+    void* d_weight;                              // of one workgroup, or NULL
     float* dot;                                  // [rows], of long rows
 };
 
@@ -262,6 +264,15 @@ __device__ __forceinline__ void load_d_out(const Job& j, int64_t r, int64_t c, f
     }
 }
 
+__device__ __forceinline__ void store_weight(void* out, int type, int64_t c, float x) {
+    if (type == B3_F32)
+        ((float*)out)[c] = x;
+    else if (type == B3_F16)
+        ((_Float16*)out)[c] = (_Float16)x;
+    else
+        ((__bf16*)out)[c] = (__bf16)x;
+}
+
 template <typename T, int G, int NV>
 __global__ __launch_bounds__(threads_of(G)) void rn_backward(Job j) {
     constexpr int kGroups = threads_of(G) / G;
@@ -297,7 +308,7 @@ __global__ __launch_bounds__(threads_of(G)) void rn_backward(Job j) {
 #pragma unroll
         for (int v = 0; v < NV; v++) write_d<T>(j, r, (v * G + lane) * kVec, u[v], g[v], s, mean);
     }
-    if (!j.partial) return;
+    if (!j.partial && !j.d_weight) return;
     float* to = j.partial + (int64_t)blockIdx.x * j.g.width;
     if (kGroups > 1) {
 #pragma unroll
@@ -309,13 +320,16 @@ __global__ __launch_bounds__(threads_of(G)) void rn_backward(Job j) {
             float x = 0;
 #pragma unroll
             for (int i = 0; i < kGroups; i++) x += sums[i * G * NV * kVec + c];
-            to[c] = x;
+            if (j.d_weight) store_weight(j.d_weight, j.g.weight_type, c, x);
+            else to[c] = x;
         }
     } else {
 #pragma unroll
         for (int v = 0; v < NV; v++) {
-            const int64_t c = (v * G + lane) * kVec;
-            store8(to + c, j.g.width - c, dw[v]);
+            const int64_t c = (v * G + lane) * kVec, left = j.g.width - c;
+            if (!j.d_weight) store8(to + c, left, dw[v]);
+            else if (j.g.weight_type == B3_F32) store8((float*)j.d_weight + c, left, dw[v]);
+            else store8((T*)j.d_weight + c, left, dw[v]);
         }
     }
 }
@@ -380,12 +394,7 @@ __global__ __launch_bounds__(kSumColumns * kSumSlices) void rn_weight(const floa
     x = 0;
 #pragma unroll
     for (int i = 0; i < kSumSlices; i++) x += lds[i][col];
-    if (type == B3_F32)
-        ((float*)out)[c] = x;
-    else if (type == B3_F16)
-        ((_Float16*)out)[c] = (_Float16)x;
-    else
-        ((__bf16*)out)[c] = (__bf16)x;
+    store_weight(out, type, c, x);
 }
 
 /* Eight values of a row to a thread. */
@@ -442,6 +451,8 @@ int64_t blocks_of(int64_t rows, int64_t width, bool backward) {
     int64_t most = backward ? kBackwardBlocks : kForwardBlocks;
     if (backward && !lanes && most > kMostSums / width) most = kMostSums / width;
     const int64_t need = ceil_div(rows, lanes && lanes < kThreads ? kThreads / lanes : 1);
+    /* few rows are one workgroup's, which has the weights' gradient without a second launch */
+    if (backward && lanes && need <= kAlone) return 1;
     return need < most ? need : most;
 }
 
@@ -530,7 +541,7 @@ hipError_t b3_values_of_8bit_gpu(int64_t rows, int64_t width, const unsigned cha
 
 size_t b3_rms_norm_backward_workspace(int64_t rows, int64_t width) {
     if (rows <= 0 || width <= 0) return 0;
-    const int64_t sums = blocks_of(rows, width, true) * width;
+    const int64_t blocks = blocks_of(rows, width, true), sums = blocks == 1 && lanes_of(width) ? 0 : blocks * width;
     return (size_t)(sums + (lanes_of(width) ? 0 : rows)) * sizeof(float);
 }
 
@@ -552,10 +563,12 @@ hipError_t b3_rms_norm_backward_gpu(const B3Norm* norm, const float* root, const
     j.d_sum = d_sum;
     j.d_sum_stride = d_sum_stride;
     const int64_t blocks = norm->rows ? blocks_of(norm->rows, norm->width, true) : 0;
-    j.partial = d_weight ? (float*)workspace : NULL;
+    const bool alone = blocks == 1 && lanes_of(norm->width);
+    j.partial = d_weight && !alone ? (float*)workspace : NULL;
+    j.d_weight = alone ? d_weight : NULL;
     j.dot = (float*)workspace + blocks * norm->width;
     hipError_t err = norm->rows ? launch<BACKWARD>(j, stream) : hipSuccess;
-    if (err != hipSuccess || !d_weight) return err;
+    if (err != hipSuccess || !d_weight || alone) return err;
     rn_weight<<<(unsigned)ceil_div(norm->width, kSumColumns), kSumColumns * kSumSlices, 0, stream>>>((float*)workspace,
         (int)blocks, norm->width, d_weight, norm->weight_type);
     return hipGetLastError();
