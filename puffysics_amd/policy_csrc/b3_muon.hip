@@ -154,11 +154,12 @@ __device__ double block_sum(double x) {
 
 __device__ __forceinline__ float direction(float g, float m, const Common& c) { return c.nesterov ? g + c.keep * m : m; }
 
-/* Four neighbours of an array of `all`, zeros past its end. */
-template <typename T>
+/* Four neighbours of an array of `all`, zeros past its end.  WHOLE: all there;
+ * without a branch many are in flight together. */
+template <bool WHOLE, typename T>
 __device__ __forceinline__ F4 load4(const T* p, int64_t i, int64_t all) {
     F4 x;
-    if (i + 4 <= all) {
+    if (WHOLE || i + 4 <= all) {
         const Pack<T, 4> v = *(const Pack<T, 4>*)(p + i);
 #pragma unroll
         for (int k = 0; k < 4; k++) x[k] = to_float(v.v[k]);
@@ -169,9 +170,9 @@ __device__ __forceinline__ F4 load4(const T* p, int64_t i, int64_t all) {
     return x;
 }
 
-template <typename T>
+template <bool WHOLE, typename T>
 __device__ __forceinline__ void store4(T* p, int64_t i, int64_t all, F4 x) {
-    if (i + 4 <= all) {
+    if (WHOLE || i + 4 <= all) {
         Pack<T, 4> v;
 #pragma unroll
         for (int k = 0; k < 4; k++) v.v[k] = (T)x[k];
@@ -183,34 +184,43 @@ __device__ __forceinline__ void store4(T* p, int64_t i, int64_t all, F4 x) {
     }
 }
 
-/* The momentum of elements from .. end - 1, a thread's sum of squares of u. */
-template <typename T>
-__device__ __forceinline__ double momentum_part(const T* grad, float* momentum, int64_t from, int64_t end, const Common& c) {
-    constexpr int kAhead = 4;
+constexpr int kMomentumAhead = 4;
+
+/* The momentum of a thread's elements from i0 on, the sum of squares of u. */
+template <bool WHOLE, typename T>
+__device__ __forceinline__ double momentum_step(const T* grad, float* momentum, int64_t i0, int64_t end, const Common& c) {
+    F4 g[kMomentumAhead], m[kMomentumAhead];
     double sum = 0;
-    for (int64_t i0 = from + threadIdx.x * 4; i0 < end; i0 += kThreads * 4 * kAhead) {
-        F4 g[kAhead], m[kAhead];
 #pragma unroll
-        for (int k = 0; k < kAhead; k++) {
-            const int64_t i = i0 + k * kThreads * 4;
-            g[k] = m[k] = F4{0, 0, 0, 0};
-            if (i < end) {
-                g[k] = load4(grad, i, end);
-                m[k] = load4(momentum, i, end);
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < kAhead; k++) {
-            const int64_t i = i0 + k * kThreads * 4;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                m[k][e] = c.keep * m[k][e] + g[k][e];
-                const float u = direction(g[k][e], m[k][e], c);
-                sum += (double)u * u;
-            }
-            if (i < end) store4(momentum, i, end, m[k]);
+    for (int k = 0; k < kMomentumAhead; k++) {
+        const int64_t i = i0 + k * kThreads * 4;
+        g[k] = m[k] = F4{0, 0, 0, 0};
+        if (WHOLE || i < end) {
+            g[k] = load4<WHOLE>(grad, i, end);
+            m[k] = load4<WHOLE>(momentum, i, end);
         }
     }
+#pragma unroll
+    for (int k = 0; k < kMomentumAhead; k++) {
+        const int64_t i = i0 + k * kThreads * 4;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            m[k][e] = c.keep * m[k][e] + g[k][e];
+            const float u = direction(g[k][e], m[k][e], c);
+            sum += (double)u * u;
+        }
+        if (WHOLE || i < end) store4<WHOLE>(momentum, i, end, m[k]);
+    }
+    return sum;
+}
+
+/* Of elements from .. end - 1. */
+template <typename T>
+__device__ __forceinline__ double momentum_part(const T* grad, float* momentum, int64_t from, int64_t end, const Common& c) {
+    constexpr int kTurn = kThreads * 4 * kMomentumAhead;
+    double sum = 0;
+    for (; from + kTurn <= end; from += kTurn) sum += momentum_step<true>(grad, momentum, from + threadIdx.x * 4, end, c);
+    if (from < end) sum += momentum_step<false>(grad, momentum, from + threadIdx.x * 4, end, c);
     return sum;
 }
 
@@ -238,7 +248,7 @@ __device__ __forceinline__ _Float16* block_of(char* work, int64_t base, int64_t 
 }
 
 /* A square of u, scaled, turned as x lies. */
-template <typename T>
+template <bool WHOLE, typename T>
 __device__ __forceinline__ void first_square(float (*tile)[kCut + 1], const T* grad, const float* momentum, const Matrix& t,
     int64_t r0, int64_t c0, bool turned, const Common& c) {
     constexpr int kAcross = kCut / 4, kDown = kThreads / kAcross, kLoads = kCut / kDown;
@@ -248,9 +258,9 @@ __device__ __forceinline__ void first_square(float (*tile)[kCut + 1], const T* g
     for (int k = 0; k < kLoads; k++) {
         const int64_t r = r0 + row + k * kDown, at = r * t.columns;
         g[k] = m[k] = F4{0, 0, 0, 0};
-        if (r < t.rows && c0 + col < t.columns) {
-            g[k] = load4(grad + at, c0 + col, t.columns);
-            m[k] = load4(momentum + at, c0 + col, t.columns);
+        if (WHOLE || (r < t.rows && c0 + col < t.columns)) {
+            g[k] = load4<WHOLE>(grad + at, c0 + col, t.columns);
+            m[k] = load4<WHOLE>(momentum + at, c0 + col, t.columns);
         }
     }
     /* what is fetched meanwhile waits for the norm */
@@ -277,9 +287,13 @@ __global__ __launch_bounds__(kThreads) void mu_split(GradientLaunch l) {
     const bool turned = t.rows > t.columns;
     const int64_t r0 = (int64_t)(turned ? p.j : p.i) * kCut, c0 = (int64_t)(turned ? p.i : p.j) * kCut;
     const float* momentum = l.c.momentum + t.at;
-    if (type == B3_F32) first_square(tile, (const float*)grad, momentum, t, r0, c0, turned, l.c);
-    else if (type == B3_F16) first_square(tile, (const _Float16*)grad, momentum, t, r0, c0, turned, l.c);
-    else first_square(tile, (const __bf16*)grad, momentum, t, r0, c0, turned, l.c);
+    auto fill = [&](const auto* g) {
+        if (r0 + kCut <= t.rows && c0 + kCut <= t.columns) first_square<true>(tile, g, momentum, t, r0, c0, turned, l.c);
+        else first_square<false>(tile, g, momentum, t, r0, c0, turned, l.c);
+    };
+    if (type == B3_F32) fill((const float*)grad);
+    else if (type == B3_F16) fill((const _Float16*)grad);
+    else fill((const __bf16*)grad);
     __syncthreads();
     /* a row's block of 32 to four threads of eight */
     for (int k = threadIdx.x; k < kCut * kCut / 8; k += kThreads) {
@@ -331,37 +345,38 @@ __device__ __forceinline__ void move(const Common& c, const Matrix& t, int64_t i
     *param = (T)w;
 }
 
-/* The weights from row r0 and column c0 on, by a tile of x that lies as they do. */
 constexpr int kMoveRow = kTile + 4;
 static_assert(kTile * kMoveRow * 4 <= kProductLds, "a tile of x");
-template <typename T>
-__device__ __forceinline__ void move_tile(const Common& c, const Matrix& t, const float* tile, int64_t r0, int64_t c0) {
-    constexpr int kAcross = kTile / 4, kDown = kThreads / kAcross, kAhead = 4;
+
+/* The weights from row r0 and column c0 on, by a tile of x that lies as they
+ * do, which `put` writes to LDS: what is fetched is on its way before. */
+template <bool WHOLE, typename T, typename F>
+__device__ __forceinline__ void move_tile(const Common& c, const Matrix& t, const float* tile, int64_t r0, int64_t c0, F put) {
+    constexpr int kAcross = kTile / 4, kDown = kThreads / kAcross, kLoads = kTile / kDown;
     const float keep = (float)(1 - c.lr * t.decay), rate = (float)(c.lr * t.factor);
     const int col = threadIdx.x % kAcross * 4, row = threadIdx.x / kAcross;
-    const bool copied = c.master && sizeof(T) == 2;
-    if (c0 + col >= t.columns) return;
-    for (int k0 = 0; k0 < kTile && r0 + k0 < t.rows; k0 += kDown * kAhead) {
-        F4 w[kAhead], copy[kAhead];
+    const bool copied = c.master && sizeof(T) == 2, in = c0 + col < t.columns;
+    F4 w[kLoads], copy[kLoads];
 #pragma unroll
-        for (int k = 0; k < kAhead; k++) {
-            const int64_t r = r0 + k0 + k * kDown + row, at = r * t.columns;
-            w[k] = copy[k] = F4{0, 0, 0, 0};
-            if (r < t.rows) {
-                w[k] = load4((const T*)t.param + at, c0 + col, t.columns);
-                if (copied) copy[k] = load4(c.master + t.at + at, c0 + col, t.columns);
-            }
+    for (int k = 0; k < kLoads; k++) {
+        const int64_t r = r0 + k * kDown + row, at = r * t.columns;
+        w[k] = copy[k] = F4{0, 0, 0, 0};
+        if (WHOLE || (in && r < t.rows)) {
+            w[k] = load4<WHOLE>((const T*)t.param + at, c0 + col, t.columns);
+            if (copied) copy[k] = load4<WHOLE>(c.master + t.at + at, c0 + col, t.columns);
         }
+    }
+    put();
+    __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kAhead; k++) {
-            const int64_t r = r0 + k0 + k * kDown + row, at = r * t.columns;
-            if (r >= t.rows) continue;
-            const F4 x = *(const F4*)(tile + (k0 + k * kDown + row) * kMoveRow + col);
+    for (int k = 0; k < kLoads; k++) {
+        const int64_t r = r0 + k * kDown + row, at = r * t.columns;
+        if (!WHOLE && (!in || r >= t.rows)) continue;
+        const F4 x = *(const F4*)(tile + (k * kDown + row) * kMoveRow + col);
 #pragma unroll
-            for (int e = 0; e < 4; e++) w[k][e] = moved((T)w[k][e], copy[k][e], copied, x[e], keep, rate);
-            if (copied) store4(c.master + t.at + at, c0 + col, t.columns, w[k]);
-            store4((T*)t.param + at, c0 + col, t.columns, w[k]);
-        }
+        for (int e = 0; e < 4; e++) w[k][e] = moved((T)w[k][e], copy[k][e], copied, x[e], keep, rate);
+        if (copied) store4<WHOLE>(c.master + t.at + at, c0 + col, t.columns, w[k]);
+        store4<WHOLE>((T*)t.param + at, c0 + col, t.columns, w[k]);
     }
 }
 
@@ -516,24 +531,30 @@ __global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
         /* to LDS as the weights lie, so that a row's neighbours are moved together */
         const bool turned = t.rows > t.columns;
         float* tile = (float*)shared;
+        auto put_tile = [&]() {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+            for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int row = wi + 16 * i + c, col = wj + 16 * j + 4 * g;
-                F4 y;
+                for (int j = 0; j < 4; j++) {
+                    const int row = wi + 16 * i + c, col = wj + 16 * j + 4 * g;
+                    F4 y;
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    y[r] = d[i][j][r] * scale * (1.0f / kScale);
-                    if (turned) tile[(col + r) * kMoveRow + row] = y[r];
+                    for (int r = 0; r < 4; r++) {
+                        y[r] = d[i][j][r] * scale * (1.0f / kScale);
+                        if (turned) tile[(col + r) * kMoveRow + row] = y[r];
+                    }
+                    if (!turned) *(F4*)(tile + row * kMoveRow + col) = y;
                 }
-                if (!turned) *(F4*)(tile + row * kMoveRow + col) = y;
-            }
-        __syncthreads();
+        };
         const int64_t r0 = (int64_t)(turned ? p.j : p.i) * kTile, c0 = (int64_t)(turned ? p.i : p.j) * kTile;
-        if (t.type == B3_F32) move_tile<float>(l.c, t, tile, r0, c0);
-        else if (t.type == B3_F16) move_tile<_Float16>(l.c, t, tile, r0, c0);
-        else move_tile<__bf16>(l.c, t, tile, r0, c0);
+        const bool whole = r0 + kTile <= t.rows && c0 + kTile <= t.columns;
+        auto move_all = [&](auto none) {
+            if (whole) move_tile<true, decltype(none)>(l.c, t, tile, r0, c0, put_tile);
+            else move_tile<false, decltype(none)>(l.c, t, tile, r0, c0, put_tile);
+        };
+        if (t.type == B3_F32) move_all(0.0f);
+        else if (t.type == B3_F16) move_all((_Float16)0.0f);
+        else move_all((__bf16)0.0f);
         return;
     }
     const int64_t columns = KIND == NEXT ? t.n : t.m;
