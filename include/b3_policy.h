@@ -203,8 +203,8 @@ hipError_t b3_adamw_destroy(B3AdamW* optimizer);
 
 /* q and k [steps, envs, heads, key], v [steps, envs, heads, value]: strides
  * in elements from step to step, environment to environment and head to
- * head; a head's elements are contiguous.  `decay` [heads] is in [0, 1] (NaN
- * outside).  `starts` is NULL or [steps, envs], nonzero where a step begins
+ * head; a head's elements are contiguous.  `decay` [heads] is in [0, 1] (a state
+ * becomes NaN by others).  `starts` is NULL or [steps, envs], nonzero where a step begins
  * an episode: what lies before is dropped (not multiplied by 0: its NaN stay
  * there).  `state` [envs, heads, key, value], contiguous, is what the first
  * step finds; NULL: zeros. */
@@ -246,7 +246,8 @@ hipError_t b3_linear_attention_step_gpu(const B3Attention* attention, float* sta
 /* ---- norm ---- */
 
 /* Rows of `width` contiguous elements, each array's rows its stride apart (in
- * elements, at least `width`).  h = x + residual (NULL: none), in 32 bits. */
+ * elements, at least `width`).  h = x + residual (NULL: none), in 32 bits, and
+ * so are the squares: those of elements past 2^63 overflow. */
 typedef struct B3Norm {
     int64_t rows, width;         /* width 1 .. 2^21 */
     int type;                    /* of x, residual and what comes of them */

@@ -13,7 +13,6 @@ The reference leaves these to the trainer (docs/RL_LIBRARY.md).
 import array
 import collections
 import ctypes as C
-import math
 import operator
 import os
 import struct
@@ -33,6 +32,7 @@ MAX_SEQUENCES = 1 << 22      # environments times heads
 MAX_WIDTH = 1 << 21          # of a norm's row
 SEGMENT = 256
 _GROUP = 32                  # 8-bit numbers to a scale
+_MOST = torch.finfo(torch.float32).max
 _SMALL = 2048                # rows of up to so many actions need no workspace
 _EMPTY = 8                   # stands for the address of a gradient without elements; NULL is no gradient
 # what a step asks of every tensor, called by map: a policy may have many small ones
@@ -429,6 +429,8 @@ class _LinearAttention(torch.autograd.Function):
 
 
 def _attention_backward(ctx, d_out, d_left):
+    if d_out is None and d_left is None:     # of what takes part in nothing that has a gradient
+        return (None,) * 8
     q, k, v, decay, state, starts = ctx.saved_tensors
     lib = policy_lib()
     d_out = torch.zeros_like(v) if d_out is None else _heads(d_out)
@@ -448,7 +450,9 @@ _attention_backward_once = torch.autograd.function.once_differentiable(_attentio
 
 
 def _check_attention(q, k, v, decay, starts, scale):
-    shape, dtype, last = q.shape, q.dtype, v.shape[-1]
+    shape, dtype = q.shape, q.dtype
+    _need(v.dim() == len(shape), "q and k need one shape, v the same but for the last axis")
+    last = v.shape[-1]
     _need(dtype in _TYPE and k.dtype is dtype and v.dtype is dtype,
           "q, k and v have to be float32, float16 or bfloat16, all of one type")
     _need(k.shape == shape and v.shape == (*shape[:-1], last), "q and k need one shape, v the same but for the last axis")
@@ -460,7 +464,7 @@ def _check_attention(q, k, v, decay, starts, scale):
     if starts is not None:
         _need(starts.shape == shape[:-2] and starts.dtype in (torch.float32, torch.bool, torch.uint8),
               "starts have to be float32, bool or uint8, one for each step and environment")
-    _need(math.isfinite(scale), "scale has to be a finite number")
+    _need(abs(scale) <= _MOST, "scale has to be a finite number of 32 bits")
 
 
 def linear_attention(q, k, v, decay, state=None, starts=None, scale=1.0, last=False):
@@ -471,7 +475,7 @@ def linear_attention(q, k, v, decay, state=None, starts=None, scale=1.0, last=Fa
 
     q, k    [steps, envs, heads, key], float32, float16 or bfloat16
     v       [steps, envs, heads, value], of their type
-    decay   [heads] float32, in [0, 1] (others give NaN); has no gradient
+    decay   [heads] float32, in [0, 1] (by others a state becomes NaN); has no gradient
     state   None (zeros) or [envs, heads, key, value] float32: what the first
             step finds, as an earlier call returned it
     starts  None or [steps, envs] float32, bool or uint8: nonzero where a step
@@ -570,6 +574,8 @@ class _RmsNorm(torch.autograd.Function):
 
 
 def _norm_backward(ctx, d_out, d_sum):
+    if d_out is None and d_sum is None:      # of what takes part in nothing that has a gradient
+        return (None,) * 4
     x, residual, weight, root = ctx.saved_tensors
     rows, width = x.shape
     lib = policy_lib()

@@ -113,3 +113,38 @@ def test_update_captured():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), i
         assert all(torch.equal(a, b) for a, b in zip(weights, twins)), i
+
+
+class _Dropped(torch.autograd.Function):
+    """x, which gets no gradient."""
+
+    @staticmethod
+    def forward(ctx, x):
+        return x.clone()
+
+    @staticmethod
+    def backward(ctx, d):
+        return None
+
+
+@pytest.mark.gpu
+def test_results_that_get_no_gradient():
+    """The backward pass runs, and is given none."""
+    from puffysics_amd import policy
+    x, w = (torch.ones(*s, device="cuda", requires_grad=True) for s in ((4, 3, 2, 8), (8,)))
+    _Dropped.apply(policy.rms_norm(x, w, residual=x).out).sum().backward()
+    assert x.grad is None and w.grad is None
+    _Dropped.apply(policy.linear_attention(x, x, x, torch.ones(2, device="cuda"), last=True).out).sum().backward()
+    assert x.grad is None
+
+
+def test_refusals_of_axes_and_scales():
+    """Nothing is launched: this runs without a GPU."""
+    from puffysics_amd import policy
+    q, decay = torch.zeros(5, 3, 2, 8), torch.zeros(2)
+    for v in (torch.zeros(()), torch.zeros(8), torch.zeros(1, 5, 3, 2, 8)):
+        with pytest.raises(ValueError, match="one shape"):
+            policy.linear_attention(q, q, v, decay)
+    for scale in (1e39, -1e39):                  # infinite in 32 bits
+        with pytest.raises(ValueError, match="finite"):
+            policy.linear_attention(q, q, q, decay, scale=scale)
