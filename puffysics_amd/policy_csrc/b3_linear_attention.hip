@@ -274,8 +274,12 @@ struct Unit {
  * workgroup where W > 1, have parts of one sequence and share q and k.  With i
  * and j places of the chunk, E the state that enters it and P the scores q_i k_j
  * decay^(i - j) of an episode, j <= i:
- *   out = P v + decay^i q E,  E' = decay^places E + (decay^(places - j) k)^T v */
-template <typename T, int KD, int VD, int W, bool STATE>
+ *   out = P v + decay^i q E,  E' = decay^places E + (decay^(places - j) k)^T v
+ * PART: tiles of 16 columns that are all filled up are left out of products,
+ * which in 32 bits are most of the time: the backward pass of 333 steps of 57 x
+ * 3 with heads of 48 and 80 takes 120 us so, 150 without.  Where no tile is,
+ * asking costs 2 to 5 % (heads of 64 and of 128). */
+template <typename T, int KD, int VD, int W, bool STATE, bool PART>
 struct Walk {
     typedef typename Math<T>::Lds Lds;
     typedef typename Math<T>::Quad Quad;
@@ -481,7 +485,10 @@ struct Walk {
                             for (int kb = 0; kb < KB; kb += 2) x = multiply(kq[kb], kq[kb + 1], qq[t][kb], qq[t][kb + 1], x);
                         } else {
 #pragma unroll
-                            for (int kb = 0; kb < KB; kb++) x = multiply(kq[kb], qq[t][kb], x);
+                            for (int kb = 0; kb < KB; kb++) {
+                                if (PART && 16 * kb >= m.key) break;
+                                x = multiply(kq[kb], qq[t][kb], x);
+                            }
                         }
                         x *= near[t - s];
                         if (t == s) {
@@ -501,6 +508,7 @@ struct Walk {
                 constexpr int kTiles = kHalf ? 2 : 1, kWide = 4 * kTiles;
 #pragma unroll
                 for (int v0 = 0; v0 < VB; v0 += kTiles) {
+                    if (PART && 16 * v0 >= value) break;
                     F4 o[R][kTiles];
 #pragma unroll
                     for (int t = 0; t < R; t++)
@@ -523,9 +531,11 @@ struct Walk {
                                 }
                             } else {
 #pragma unroll
-                                for (int kb = 0; kb < KB; kb++)
+                                for (int kb = 0; kb < KB; kb++) {
+                                    if (PART && 16 * kb >= m.key) break;
 #pragma unroll
                                     for (int t = 0; t < R; t++) o[t][i] = multiply(state[kb][vb], qq[t][kb], o[t][i]);
+                                }
                             }
                         }
 #pragma unroll
@@ -656,9 +666,13 @@ struct Walk {
                 for (int vb = 0; vb < VB; vb++) vq[0][vb] *= weight[0];
 #pragma unroll
                 for (int kb = 0; kb < KB; kb++) {
+                    if (PART && 16 * kb >= m.key) break;
                     const F4 x = across<kKeyRow, 4>(lk, 0, 16 * kb);
 #pragma unroll
-                    for (int vb = 0; vb < VB; vb++) state[kb][vb] = multiply(x, vq[0][vb], state[kb][vb]);
+                    for (int vb = 0; vb < VB; vb++) {
+                        if (PART && 16 * vb >= value) break;
+                        state[kb][vb] = multiply(x, vq[0][vb], state[kb][vb]);
+                    }
                 }
             }
         }
@@ -682,10 +696,10 @@ struct Walk {
 /* Waves of a workgroup: the parts of a sequence where they share, else
  * neighbours in memory (roles of a sequence, heads).  Workgroups go to the 8
  * dies in turn: each die's take neighbouring ones. */
-template <typename T, int KD, int VD, int W, bool STATE>
+template <typename T, int KD, int VD, int W, bool STATE, bool PART>
 __global__ __launch_bounds__(kThreads, 2) void la_walk(Job j) {
     extern __shared__ __attribute__((aligned(16))) char shared[];
-    typedef Walk<T, KD, VD, W, STATE> Walker;
+    typedef Walk<T, KD, VD, W, STATE, PART> Walker;
     const unsigned die = blockIdx.x % 8, share = gridDim.x / 8, rest = gridDim.x % 8;
     const unsigned block = die * share + (die < rest ? die : rest) + blockIdx.x / 8;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -931,14 +945,25 @@ void place_pieces(Mix& m, const B3Attention& g, const Plan& p, void* workspace, 
     m.carry = m.pieces + (p.pieces - 1) * g.envs * g.heads * g.key * g.value;
 }
 
-template <typename T, int KD, int VD, int W, bool STATE>
-hipError_t launch(const Job& j, hipStream_t stream) {
-    typedef Walk<T, KD, VD, W, STATE> Walker;
+template <typename T, int KD, int VD, int W, bool STATE, bool PART>
+hipError_t launch_walk(const Job& j, hipStream_t stream) {
+    typedef Walk<T, KD, VD, W, STATE, PART> Walker;
     constexpr int kLds = 64 << 10, kMost = kLds / Walker::kBytes, kGroups = W > 1 ? 1 : kMost >= 4 ? 4 : kMost >= 2 ? 2 : 1;
     static_assert(kMost >= 1, "a workgroup's tiles");
     const int64_t units = j.envs * j.heads * (STATE ? j.pieces - 1 : j.pieces) * j.roles * (W > 1 ? 1 : j.parts);
-    la_walk<T, KD, VD, W, STATE><<<(unsigned)ceil_div(units, kGroups), kGroups * W * kWave, kGroups * Walker::kBytes, stream>>>(j);
+    la_walk<T, KD, VD, W, STATE, PART><<<(unsigned)ceil_div(units, kGroups), kGroups * W * kWave, kGroups * Walker::kBytes, stream>>>(j);
     return hipGetLastError();
+}
+
+template <typename T, int KD, int VD, int W, bool STATE>
+hipError_t launch(const Job& j, hipStream_t stream) {
+    if constexpr (!__is_same(T, __bf16)) {
+        for (int i = 0; i < j.roles; i++) {
+            const Mix& m = j.mix[i];
+            if (ceil_div(m.key, 16) * 16 < KD || ceil_div(m.value, 16) * 16 % VD) return launch_walk<T, KD, VD, W, STATE, true>(j, stream);
+        }
+    }
+    return launch_walk<T, KD, VD, W, STATE, false>(j, stream);
 }
 
 template <typename T, bool STATE>
@@ -946,7 +971,8 @@ hipError_t launch_columns(const Job& j, const Plan& p, hipStream_t stream) {
     if (p.key == 128) {
         /* In 16 bits parts share what they fetch: two histories of 65,536 steps and 8 heads of 128 take 370 us
          * so, 435 each for itself.  In 32 the products take most of the time, and waves had better not wait for
-         * each other: the backward pass of 333 steps of 57 x 3 with heads of 48 and 80 takes 154 us, 240 shared. */
+         * each other: the backward pass of 333 steps of 57 x 3 with heads of 48 and 80 took 154 us, 240 shared, with
+         * all tiles. */
         if constexpr (__is_same(T, __bf16)) {
             if (p.parts > 2) return launch<T, 128, 32, 4, STATE>(j, stream);
             if (p.parts > 1) return launch<T, 128, 32, 2, STATE>(j, stream);
