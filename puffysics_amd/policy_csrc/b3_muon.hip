@@ -320,7 +320,9 @@ struct ProductLaunch {
     Common c;
     bool swapped, swapped_long;                  // x is in `next`
     int step;                                    // of a group
-    int middle;                                  // 0: z y, 1: z p; of the launch's first row of workgroups
+    int middle;                                  // 0: z y, 1: z p; the first that the launch forms
+    int64_t middles;                             // workgroups that form one of them
+    int64_t before;                              // workgroups of the launches before
 };
 
 /* Where z of a long matrix' step is (the first one is p), and p after a step. */
@@ -410,13 +412,12 @@ __device__ __forceinline__ int in_row(int row, int k) { return row / 2 * 256 + (
  * is fetched into registers while the two before are worked on, since one takes
  * less time than memory does, and goes to the other half of LDS. */
 template <Product KIND>
-__global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
+__device__ __forceinline__ void product(const ProductLaunch& l, const Place& p, bool collect) {
     constexpr bool kAcross = KIND == NEXT || KIND == LAST;      // the right side's rows are what is summed over
     constexpr int kRow = kStep * 4;                             // bytes of a row in LDS
     constexpr int kSide = kSideLds, kLoads = kTile * kStep * 4 / 16 / kThreads;
     static_assert(kTile * kRow <= kSide, "either side");
     extern __shared__ __attribute__((aligned(16))) char shared[];
-    const Place p = l.c.places[l.c.first + by_die()];
     const Matrix& t = l.c.matrices[p.matrix];
     if (!l.c.live[p.matrix]) return;
     const bool swapped = t.is_long ? l.swapped_long : l.swapped;
@@ -433,7 +434,6 @@ __global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
         left = right = t.y;
         out = z;
     } else if (KIND == MIDDLE) {
-        const bool collect = l.middle + blockIdx.y == 1;
         left = z;
         right = collect ? collected_of(t, l.step - 1) : t.y;
         out = collect ? collected_of(t, l.step) : t.between;
@@ -598,6 +598,20 @@ __global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
             for (int r = 0; r < 4; r++) tile[(wj + 16 * j + 4 * g + r) * kMoveRow + wi + 16 * i + c] = both[i][j][r];
     __syncthreads();
     store_tile(l.c.work, out, columns, (int64_t)p.j * kTile, (int64_t)p.i * (kTile / kStep), tile);
+}
+
+template <Product KIND>
+__global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
+    product<KIND>(l, l.c.places[l.c.first + l.before + by_die()], false);
+}
+
+/* z y and z p of long matrices, as the launch has them, and z x of others, whose
+ * places follow: neither needs the other, and together they fill the device
+ * better. */
+__global__ __launch_bounds__(kThreads, 2) void mu_products(ProductLaunch l, int formed) {
+    const int64_t i = l.before + by_die(), middles = l.middles * formed;
+    if (i < middles) product<MIDDLE>(l, l.c.places[l.c.first + i % l.middles], l.middle + i / l.middles == 1);
+    else product<NEXT>(l, l.c.places[l.c.first + l.middles + i - middles], false);
 }
 
 /* ---- small matrices ---- */
@@ -779,10 +793,21 @@ hipError_t over(int64_t first, int64_t end, F launch) {
 }
 
 template <Product KIND>
-hipError_t launch_product(ProductLaunch l, int64_t first, int64_t end, hipStream_t stream, unsigned both = 1) {
-    return over(first, end, [&](int64_t at, unsigned blocks) {
-        l.c.first = at;
-        mu_product<KIND><<<dim3(blocks, both), kThreads, kProductLds, stream>>>(l);
+hipError_t launch_product(ProductLaunch l, int64_t first, int64_t end, hipStream_t stream) {
+    l.c.first = first;
+    return over(0, end - first, [&](int64_t at, unsigned blocks) {
+        l.before = at;
+        mu_product<KIND><<<blocks, kThreads, kProductLds, stream>>>(l);
+    });
+}
+
+/* `formed` of z y and z p for the places from first to middle, then z x to end. */
+hipError_t launch_products(ProductLaunch l, int64_t first, int64_t middle, int64_t end, int formed, hipStream_t stream) {
+    l.c.first = first;
+    l.middles = middle - first;
+    return over(0, l.middles * formed + end - middle, [&](int64_t at, unsigned blocks) {
+        l.before = at;
+        mu_products<<<blocks, kThreads, kProductLds, stream>>>(l, formed);
     });
 }
 
@@ -791,10 +816,8 @@ bool is_small(int64_t rows, int64_t columns) {
     return m <= kSmallSide && n <= kSmallLength;
 }
 
-template <Product KIND>
-hipError_t allow_lds() {
-    return hipFuncSetAttribute((const void*)mu_product<KIND>, hipFuncAttributeMaxDynamicSharedMemorySize,
-        kProductLds);
+hipError_t allow_lds(const void* kernel) {
+    return hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kProductLds);
 }
 
 }  // namespace
@@ -923,11 +946,11 @@ hipError_t b3_muon_create(B3Muon** out, const B3MuonMatrix* matrices, int count,
     if (err == hipSuccess) err = hipMalloc((void**)&o->live, ((size_t)count + 1) * sizeof(int));
     if (err == hipSuccess) err = hipMemcpy(o->matrices, table, ((size_t)count + 1) * sizeof(Matrix), hipMemcpyHostToDevice);
     if (err == hipSuccess) err = hipMemcpy(o->places, places, (size_t)(o->end + o->smalls) * sizeof(Place), hipMemcpyHostToDevice);
-    if (err == hipSuccess) err = allow_lds<GRAM>();
-    if (err == hipSuccess) err = allow_lds<POLYNOMIAL>();
-    if (err == hipSuccess) err = allow_lds<MIDDLE>();
-    if (err == hipSuccess) err = allow_lds<NEXT>();
-    if (err == hipSuccess) err = allow_lds<LAST>();
+    if (err == hipSuccess) err = allow_lds((const void*)mu_product<GRAM>);
+    if (err == hipSuccess) err = allow_lds((const void*)mu_product<POLYNOMIAL>);
+    if (err == hipSuccess) err = allow_lds((const void*)mu_products);
+    if (err == hipSuccess) err = allow_lds((const void*)mu_product<NEXT>);
+    if (err == hipSuccess) err = allow_lds((const void*)mu_product<LAST>);
     if (err == hipSuccess)
         err = hipFuncSetAttribute((const void*)mu_small, hipFuncAttributeMaxDynamicSharedMemorySize,
             small_lds(kSmallSide, kSmallLength));
@@ -984,17 +1007,16 @@ hipError_t b3_muon_step_gpu(B3Muon* o, const void* const* grads, const int* grad
         if (err != hipSuccess) return err;
     }
     const int steps = o->config.newton_schulz;
-    ProductLaunch p = {l.c, false, false, 0, 0};
+    ProductLaunch p = {l.c, false, false, 0, 0, 0, 0};
     for (int s = 0; s < steps && o->halves < o->end && err == hipSuccess; s++) {
         const bool last = s + 1 == steps, joined = last || p.step + 1 == kGroup;     // long x becomes its next
         err = launch_product<GRAM>(p, o->halves, o->tiles, stream);
         if (err == hipSuccess) err = launch_product<POLYNOMIAL>(p, o->halves, o->tiles, stream);
         p.middle = joined ? 1 : 0;
-        const unsigned both = (joined ? 0 : 1) + (p.step ? 1 : 0);
-        if (err == hipSuccess && both) err = launch_product<MIDDLE>(p, o->long_halves, o->tiles, stream, both);
-        if (err == hipSuccess)
-            err = last ? launch_product<LAST>(p, o->tiles, o->end, stream)
-                       : launch_product<NEXT>(p, o->tiles, joined ? o->end : o->long_tiles, stream);
+        const int formed = (joined ? 0 : 1) + (p.step ? 1 : 0);
+        if (err == hipSuccess) err = launch_products(p, o->long_halves, o->tiles, last ? o->tiles : o->long_tiles, formed, stream);
+        if (err == hipSuccess && last) err = launch_product<LAST>(p, o->tiles, o->end, stream);
+        else if (err == hipSuccess && joined) err = launch_product<NEXT>(p, o->long_tiles, o->end, stream);
         p.swapped = !p.swapped;
         p.swapped_long ^= joined;
         p.step = joined ? 0 : p.step + 1;
