@@ -16,15 +16,15 @@
  * kScale brings their elements to where 2^-24, the least half, is 2^-37.
  * Accumulators are in 32 bits.
  *
- * Where x is longer than wide, its steps are taken on the short side: with y
+ * Where x is longer than wide by some tiles, its steps are taken on the short side: with y
  * and z as above y becomes z y z, p = .. z z z collects the steps, and x becomes
  * p x once.  That is 3 m m n + (4 steps - 3) m^3 multiplications rather than
  * steps (3 m m n + m^3), half tiles taken for half.  The rounding of y, some
  * 2^-22 of its norm, grows by at most 3.4445^2 a step where y is all but 0, so
  * that y is formed anew from x after kGroup steps.
  *
- * A launch computes one product of all matrices, a workgroup to a tile of 128
- * x 128.  Matrices lie in blocks of 32 columns, halves and what is left side by
+ * A launch computes a product of all matrices, or those that need not wait for
+ * each other, a workgroup to a tile of 128 x 128.  Matrices lie in blocks of 32 columns, halves and what is left side by
  * side, 128 bytes to a row's block; both sides are filled up with zeros to
  * whole tiles.  Matrices of at most 64 x 256 take all of their step in one
  * workgroup's LDS.
@@ -51,6 +51,12 @@ constexpr int64_t kPart = 4096;                  // its elements at the least
 constexpr double kA = 3.4445, kB = -4.7750, kC = 2.0315;
 constexpr float kScale = 8192.0f, kCollected = 16.0f;      // of x, y and z, and of p, whose singular values reach 3.4445^5
 constexpr int kGroup = 5;
+/* x that is so much longer than wide takes its steps on the short side, for a
+ * launch more in each.  So or not, us a step: 16 matrices of 128 x 256 156 and
+ * 150, of 256 x 512 266 and 246, of 512 x 640 418 and 407, of 128 x 512 167 and
+ * 188, of 512 x 1,024 445 and 480, of 512 x 2,048 533 and 769; 4 of 2,048 x 4,096
+ * 3,116 and 4,024. */
+constexpr int64_t kLonger = 3 * kTile;
 constexpr int kSmallSide = 64, kSmallLength = 256, kSmallThreads = 512;
 constexpr int kSmallTiles = kSmallSide / 16 * kSmallLength / 16 / (kSmallThreads / kWave);      // of a wave
 
@@ -224,7 +230,8 @@ __device__ __forceinline__ double momentum_part(const T* grad, float* momentum, 
     return sum;
 }
 
-/* The momentum, and a part's sum of squares of u. */
+/* The momentum, and a part's sum of squares of u.  Memory bounds it: 12 matrices
+ * of 2,048 and 8,192 in fp32 209 us, 5.8 TB/s. */
 __global__ __launch_bounds__(kThreads) void mu_momentum(GradientLaunch l) {
     const Place p = l.c.places[l.c.first + blockIdx.x];
     const Matrix& t = l.c.matrices[p.matrix];
@@ -276,7 +283,8 @@ __device__ __forceinline__ void first_square(float (*tile)[kCut + 1], const T* g
         }
 }
 
-/* The first x, a square of it: u over its norm. */
+/* The first x, a square of it: u over its norm.  The same matrices 262 us, 4.6
+ * TB/s. */
 __global__ __launch_bounds__(kThreads) void mu_split(GradientLaunch l) {
     __shared__ float tile[kCut][kCut + 1];
     const Place p = l.c.places[l.c.first + blockIdx.x];
@@ -410,7 +418,12 @@ __device__ __forceinline__ int in_row(int row, int k) { return row / 2 * 256 + (
 
 /* Four waves, each with 64 x 64 of the tile.  A step of 32 of what is summed
  * is fetched into registers while the two before are worked on, since one takes
- * less time than memory does, and goes to the other half of LDS. */
+ * less time than memory does, and goes to the other half of LDS.  z of 12
+ * matrices of 2,048 and 8,192 takes 360 us, 913 TFLOP/s of 16-bit products (a
+ * large library product reaches 1,111), z of 50 matrices of 512 wide 39 us, 620
+ * TFLOP/s: of 16 steps the beginnings and ends of tiles take the most, and what
+ * a launch reads and writes (131 MB, 3.3 TB/s).  The last product, with the
+ * weights, takes 1,248 and 150 us (3.4 TB/s). */
 template <Product KIND>
 __device__ __forceinline__ void product(const ProductLaunch& l, const Place& p, bool collect) {
     constexpr bool kAcross = KIND == NEXT || KIND == LAST;      // the right side's rows are what is summed over
@@ -607,7 +620,8 @@ __global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
 
 /* z y and z p of long matrices, as the launch has them, and z x of others, whose
  * places follow: neither needs the other, and together they fill the device
- * better. */
+ * better.  Of 50 matrices of 512 wide 324 + 512 tiles take 61 us, 33 + 35 in two
+ * launches, of 12 of 2,048 and 8,192 1,088 + 2,048 tiles 656, 257 + 408. */
 __global__ __launch_bounds__(kThreads, 2) void mu_products(ProductLaunch l, int formed) {
     const int64_t i = l.before + by_die(), middles = l.middles * formed;
     if (i < middles) product<MIDDLE>(l, l.c.places[l.c.first + i % l.middles], l.middle + i / l.middles == 1);
@@ -634,7 +648,9 @@ __device__ __forceinline__ F4 multiply(F4 a, F4 b, F4 d) {
 }
 
 /* A matrix' whole step, in 32 bits: tiles of 16 x 16 of y and z to a wave each,
- * and of x up to kSmallTiles. */
+ * and of x up to kSmallTiles.  15 products that wait for each other bound it:
+ * four of up to 64 x 64 32 us; 64 of 64 x 256 84 us and 512 of them 280, in
+ * launches of products 194 and 451. */
 __global__ __launch_bounds__(kSmallThreads) void mu_small(GradientLaunch l, int steps) {
     extern __shared__ __attribute__((aligned(16))) char shared[];
     __shared__ double sums[kSmallThreads / kWave];
@@ -895,7 +911,7 @@ hipError_t b3_muon_create(B3Muon** out, const B3MuonMatrix* matrices, int count,
             }
             t.m = filled(m);
             t.n = filled(numel / m);
-            t.is_long = t.n > t.m;
+            t.is_long = t.n >= t.m + kLonger;
             int64_t* const squares[5] = {&t.y, &t.z, &t.between, &t.collected[0], &t.collected[1]};
             t.x = work;
             t.next = t.x + t.m * t.n;
