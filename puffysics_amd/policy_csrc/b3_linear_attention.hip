@@ -25,8 +25,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kRoles = 3;                        // of a launch
 static_assert((int64_t)B3_MAX_SEQUENCES * kRoles * kThreads < (int64_t)1 << 32, "threads of a launch");
-constexpr int64_t kWaves = 2048;                 // that a launch of few sequences is cut into
-constexpr int64_t kPieceChunks = 4;              // of a piece at the least
+constexpr int64_t kAlone = 1024, kFull = 2048;   // waves with a SIMD to themselves, and two to each
 
 /* out_p = `reach` q_p (decay^p E + sums over p' <= p of the episode of
  * `update` decay^(p - p') k_p'^T v_p'), and the state that is left,
@@ -278,7 +277,13 @@ struct Unit {
  * PART: tiles of 16 columns that are all filled up are left out of products,
  * which in 32 bits are most of the time: the backward pass of 333 steps of 57 x
  * 3 with heads of 48 and 80 takes 120 us so, 150 without.  Where no tile is,
- * asking costs 2 to 5 % (heads of 64 and of 128). */
+ * asking costs 2 to 5 % (heads of 64 and of 128).
+ * 64 steps of 4,096 environments with 4 heads of 64 in bf16 take 185 us forward
+ * (4.4 TB/s, vector units 33 % busy, matrix units 9) and 395 back (3.1 TB/s, 41
+ * and 12), two histories of 65,536 steps and 8 heads of 128 151 us for the
+ * pieces' states and 358 for all (3.1 TB/s, 52 and 27): what bounds it is that
+ * the registers hold but two waves of a SIMD, which wait for each other's
+ * instructions more than for memory. */
 template <typename T, int KD, int VD, int W, bool STATE, bool PART>
 struct Walk {
     typedef typename Math<T>::Lds Lds;
@@ -735,18 +740,31 @@ __global__ __launch_bounds__(kThreads, 2) void la_walk(Job j) {
         shared + (W > 1 ? 0 : wave * Walker::kBytes));
 }
 
-/* What enters each piece, over what the pieces left by themselves. */
+/* What enters each piece, over what the pieces left by themselves; kAhead of
+ * them are on their way at a time.  Of few sequences that is what it takes, else
+ * memory: 31 pieces of 16 states of 128 x 128 15 us, 4.1 TB/s. */
 __global__ __launch_bounds__(kThreads) void la_join(Job j) {
+    constexpr int kAhead = 8;
     const Mix& m = j.mix[blockIdx.y];
     const int64_t sequences = j.envs * j.heads, size = (int64_t)m.key * m.value, all = sequences * size;
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x, end = j.pieces - 1;
     if (i >= all) return;
+    const float* carry = m.carry + i / size;
     float x = m.pieces[i];
-#pragma unroll 8
-    for (int64_t p = 1; p < j.pieces - 1; p++) {
-        const float f = m.carry[p * sequences + i / size], own = m.pieces[p * all + i];
-        x = f < 0 ? own : f * x + own;
-        m.pieces[p * all + i] = x;
+    for (int64_t p = 1; p < end; p += kAhead) {
+        float f[kAhead], own[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; a++) {
+            if (p + a >= end) break;
+            f[a] = carry[(p + a) * sequences];
+            own[a] = m.pieces[(p + a) * all + i];
+        }
+#pragma unroll
+        for (int a = 0; a < kAhead; a++) {
+            if (p + a >= end) break;
+            x = f[a] < 0 ? own[a] : f[a] * x + own[a];
+            m.pieces[(p + a) * all + i] = x;
+        }
     }
 }
 
@@ -761,7 +779,7 @@ struct StepJob {
 
 /* A wave to a sequence: L lanes with four neighbouring columns each to a row
  * of the state, 64 / L rows at once.  The state, read and written, is all but
- * all that there is to move. */
+ * all that there is to move: 16,384 states of 64 x 64 102 us, 5.3 TB/s. */
 template <typename T, int L>
 __global__ __launch_bounds__(kThreads) void la_step(StepJob j) {
     constexpr int kRows = kWave / L, kAhead = 8;
@@ -914,6 +932,31 @@ struct Plan {
     int64_t places, pieces;
 };
 
+/* Chunks' times that a launch's waves take for one each: 1.45 where two share a
+ * SIMD, and of more waves something between what a last round takes by its
+ * share and whole. */
+double rounds(int64_t waves) {
+    if (waves <= kAlone) return 1;
+    if (waves <= kFull) return 1.45;
+    return 1.45 * ((double)waves / kFull + (double)ceil_div(waves, kFull)) / 2;
+}
+
+/* What a pass takes in pieces, in us: a chunk 3.5 (1.8 of narrow heads), 0.6 of
+ * it for a state alone; the two launches more 8, and 0.25 for a piece; the states, which are written,
+ * added up and read, 4.5 MB a us.  Measured, us in 1, 2, 4, 8 and 16 pieces,
+ * this took in brackets: bf16, heads of 64, 1,024 steps of 256 sequences 108,
+ * 91, [62], 66, 91; 256 steps of them [29], 32, 33, 41, -; 4,096 of 64 sequences
+ * 414, 320, 171, 97, [66], in 32 pieces 70; back, 12 pieces 139, 128 in 8, [119]
+ * in 16; of 256 sequences of 1,024 steps [108], 119, 119, 141, 196. */
+double time_of(const B3Attention& g, const Plan& p, int64_t units, int64_t pieces, bool backward) {
+    const double chunks = (double)ceil_div(ceil_div(g.steps, pieces), places_of(g.type)), chunk = p.key == 32 ? 1.8 : 3.5;
+    const double walk = chunks * chunk * rounds(units * pieces);
+    if (pieces == 1) return walk;
+    const int ways = backward ? 2 : 1;
+    const int64_t states = g.envs * g.heads * (pieces - 1) * ways;
+    return walk + chunks * chunk * 0.6 * rounds(states * p.parts) + 8 + 0.25 * (double)pieces + (double)states * (double)(g.key * g.value) * 16 / 4.5e6;
+}
+
 Plan plan_of(const B3Attention& g, bool backward) {
     Plan p;
     const int most = g.key > g.value ? g.key : g.value;
@@ -921,10 +964,19 @@ Plan plan_of(const B3Attention& g, bool backward) {
     p.value = part_of(backward ? most : g.key, backward ? most : g.value);
     p.parts = (int)ceil_div(backward ? most : g.value, p.value);
     const int64_t units = g.envs * g.heads * p.parts * (backward ? kRoles : 1);
-    const int64_t chunk = places_of(g.type), most_pieces = g.steps / (chunk * kPieceChunks);
-    p.pieces = units >= kWaves / 2 ? 1 : ceil_div(kWaves, units);
-    p.pieces = p.pieces < most_pieces ? p.pieces : most_pieces;
-    p.pieces = p.pieces > 1 ? p.pieces : 1;
+    const int64_t chunk = places_of(g.type), chunks = ceil_div(g.steps, chunk);
+    double least = 0;
+    p.pieces = 1;
+    auto look = [&](int64_t pieces) {
+        const double time = time_of(g, p, units, pieces, backward);
+        if (pieces > 1 && time >= least) return;
+        p.pieces = pieces;
+        least = time;
+    };
+    look(1);
+    for (int64_t n = 2; n <= chunks && units * n <= 2 * kFull; n *= 2) look(n);
+    for (int64_t waves : {kAlone, kFull})
+        if (waves / units > 1 && waves / units <= chunks) look(waves / units);
     p.places = ceil_div(ceil_div(g.steps, p.pieces), chunk) * chunk;
     p.places = p.places > 0 ? p.places : chunk;
     p.pieces = g.steps > 0 ? ceil_div(g.steps, p.places) : 1;
@@ -948,8 +1000,10 @@ void place_pieces(Mix& m, const B3Attention& g, const Plan& p, void* workspace, 
 template <typename T, int KD, int VD, int W, bool STATE, bool PART>
 hipError_t launch_walk(const Job& j, hipStream_t stream) {
     typedef Walk<T, KD, VD, W, STATE, PART> Walker;
-    constexpr int kLds = 64 << 10, kMost = kLds / Walker::kBytes, kGroups = W > 1 ? 1 : kMost >= 4 ? 4 : kMost >= 2 ? 2 : 1;
+    constexpr int kLds = 64 << 10, kMost = kLds / Walker::kBytes, kGroups = W > 1 ? 1 : kMost >= 4 ? 4 : 1;
     static_assert(kMost >= 1, "a workgroup's tiles");
+    /* (workgroups of two would leave SIMDs empty: 32-bit heads of 128, two histories of 2,048 steps, take 84 us so, 67
+     * one wave each; 1,000 environments of 512 steps 1,690 and 1,807) */
     const int64_t units = j.envs * j.heads * (STATE ? j.pieces - 1 : j.pieces) * j.roles * (W > 1 ? 1 : j.parts);
     la_walk<T, KD, VD, W, STATE, PART><<<(unsigned)ceil_div(units, kGroups), kGroups * W * kWave, kGroups * Walker::kBytes, stream>>>(j);
     return hipGetLastError();
