@@ -24,10 +24,10 @@
  * that y is formed anew from x after kGroup steps.
  *
  * A launch computes a product of all matrices, or those that need not wait for
- * each other, a workgroup to a tile of 128 x 128.  Matrices lie in blocks of 32 columns, halves and what is left side by
- * side, 128 bytes to a row's block; both sides are filled up with zeros to
- * whole tiles.  Matrices of at most 64 x 256 take all of their step in one
- * workgroup's LDS.
+ * each other, a workgroup to a tile of 128 x 128.  Matrices lie in blocks of 32
+ * columns, halves and what is left side by side, 128 bytes to a row's block;
+ * both sides are filled up with zeros to whole tiles.  Matrices of at most 64 x
+ * 256 take all of their step in one workgroup's LDS.
  */
 #include "policy_common.h"
 

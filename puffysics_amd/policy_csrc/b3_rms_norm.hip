@@ -6,9 +6,9 @@
  *   dh = d_h + s (w dy - h s mean(w dy h s)), dw = sum over rows of dy h s
  *
  * Everything is read once and written once, so that memory bounds it.  G lanes
- * share a row and hold it in registers, one or two vectors of 8 neighbouring
+ * share a row and hold it in registers, one to four vectors of 8 neighbouring
  * elements each: 4 to 64 lanes of a wave, or a workgroup's 256 beyond 1,024
- * elements, 512 beyond 2,048 and 1,024 beyond 8,192.
+ * elements, 512 beyond 2,048 and, back, 1,024 beyond 8,192.
  * Rows of more than 16,384 are gone over twice.  A lane keeps its columns from
  * row to row: of the weights' gradient each workgroup writes the sums over its
  * rows, in one order always, and a second launch adds these.
@@ -439,7 +439,7 @@ enum Pass { FORWARD, FORWARD_8BIT, BACKWARD };
 
 template <typename T, int G, int NV, Pass PASS>
 void launch_row(const Job& j, unsigned blocks, hipStream_t stream) {
-    if (PASS == BACKWARD)
+    if constexpr (PASS == BACKWARD)
         rn_backward<T, G, NV><<<blocks, threads_of(G), 0, stream>>>(j);
     else
         rn_forward<T, G, NV, PASS == FORWARD_8BIT><<<blocks, threads_of(G), 0, stream>>>(j);
@@ -479,7 +479,12 @@ void launch_typed(const Job& j, hipStream_t stream) {
     else if (v <= 256) launch_row<T, kThreads, 1, PASS>(j, blocks, stream);
     else if (v <= 512) launch_row<T, 2 * kThreads, 1, PASS>(j, blocks, stream);
     else if (v <= 1024) launch_row<T, 2 * kThreads, 2, PASS>(j, blocks, stream);
-    else if (v <= 2048) launch_row<T, kWide, 2, PASS>(j, blocks, stream);
+    else if (v <= 2048) {
+        /* 8,192 rows of 12,000 in bf16: 88 us forward and 230 back with four vectors to each of 512 lanes, 101 and 163
+         * with two to 1,024 */
+        if constexpr (PASS == BACKWARD) launch_row<T, kWide, 2, PASS>(j, blocks, stream);
+        else launch_row<T, 2 * kThreads, 4, PASS>(j, blocks, stream);
+    }
     else if (PASS != BACKWARD) rn_forward_long<T, PASS == FORWARD_8BIT><<<blocks, kThreads, 0, stream>>>(j);
     else {
         rn_dot<T><<<(unsigned)blocks_of(j.g.rows, width, false), kThreads, 0, stream>>>(j);
