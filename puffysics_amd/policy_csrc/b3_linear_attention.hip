@@ -146,51 +146,75 @@ struct Tile {
     static __device__ __forceinline__ int row(int l) { return l * (kRows * W) + (int)threadIdx.x % (kWave * W) / kPerRow; }
     static __device__ __forceinline__ int col() { return (int)threadIdx.x % kPerRow * kVec; }
 
-    /* Columns from p on, of which there are `cols`; zeros beyond and in rows from
-     * `places` (at least 1) on.  What lies beyond is not fetched, but no branch of
-     * a lane's is taken for it, so that all loads are in flight together. */
+    /* Columns from p on, of which there are `cols`, and `places` rows (at least 1).
+     * What lies beyond is not fetched, but no branch of a lane's is taken for it, so
+     * that all loads are in flight together: a lane that has fewer columns left than
+     * a vector, or none, fetches the row's last ones, rows beyond are the last one
+     * again.  fit_columns() is for when they have come: sooner it would wait for them. */
     __device__ __forceinline__ void load(const T* p, int64_t stride, int places, int cols) {
-        const bool in = col() < cols;
-        if (cols % kVec == 0 && places == kPlaces) {
-            const T* at = p + row(0) * stride + (in ? col() : 0);
+        int first = col() + kVec <= cols ? col() : cols - kVec;
+        if (cols >= kVec && places == kPlaces) {
+            const T* at = p + row(0) * stride + first;
 #pragma unroll
             for (int l = 0; l < kLoads; l++) raw[l] = __builtin_bit_cast(U4, *(const Pack<T, kVec>*)(at + l * (kRows * W * stride)));
-            if (cols < COLS) {
-#pragma unroll
-                for (int l = 0; l < kLoads; l++)
-                    if (!in) raw[l] = U4{0, 0, 0, 0};
-            }
         } else {
             /* (values of their own, so that nothing of this is formed ahead of the loop and held) */
-            int first = col();
             asm volatile("" : "+s"(stride), "+v"(first));
 #pragma unroll
             for (int l = 0; l < kLoads; l++) {
                 const T* at = p + (row(l) < places ? row(l) : places - 1) * stride;
                 Pack<T, kVec> x;
-                if (cols % kVec == 0) {
-                    x = *(const Pack<T, kVec>*)(at + (first < cols ? first : 0));
+                if (cols >= kVec) {
+                    x = *(const Pack<T, kVec>*)(at + first);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < kVec; i++) x.v[i] = at[first + i < cols ? first + i : 0];
+                    for (int i = 0; i < kVec; i++) x.v[i] = at[i < cols ? i : 0];
                 }
-#pragma unroll
-                for (int i = 0; i < kVec; i++)
-                    if (row(l) >= places || first + i >= cols) x.v[i] = (T)0.0f;
                 raw[l] = __builtin_bit_cast(U4, x);
             }
+            rows_beyond(places);                 // (nothing follows such a chunk)
         }
+    }
+
+    /* Zeros for columns beyond; the last ones moved to where they belong. */
+    __device__ __forceinline__ void fit_columns(int cols) {
+        if (cols < COLS) {
+            const int left = cols - col();       // of a lane
+            if (cols % kVec) {
+                const bool some = left > 0 && left < kVec;
+                const int by = cols >= kVec ? (kVec - cols % kVec) * (int)sizeof(T) : 0;
+#pragma unroll
+                for (int l = 0; l < kLoads; l++) {
+                    U4 x = raw[l];
+                    if (by & 8) x = U4{x[2], x[3], 0, 0};
+                    if (by & 4) x = U4{x[1], x[2], x[3], 0};
+                    if (by & 2) x = U4{x[0] >> 16 | x[1] << 16, x[1] >> 16 | x[2] << 16, x[2] >> 16 | x[3] << 16, x[3] >> 16};
+                    if (cols < kVec) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int n = cols * (int)sizeof(T) - 4 * i;      // bytes
+                            x[i] = n >= 4 ? x[i] : n == 2 ? x[i] & 0xffffu : 0;
+                        }
+                    }
+                    if (some) raw[l] = x;
+                }
+            }
+#pragma unroll
+            for (int l = 0; l < kLoads; l++)
+                if (left <= 0) raw[l] = U4{0, 0, 0, 0};
+        }
+    }
+
+    /* Zeros from row `places` on. */
+    __device__ __forceinline__ void rows_beyond(int places) {
+#pragma unroll
+        for (int l = 0; l < kLoads; l++)
+            if (row(l) >= places) raw[l] = U4{0, 0, 0, 0};
     }
 
     __device__ __forceinline__ void none() {
 #pragma unroll
         for (int l = 0; l < kLoads; l++) raw[l] = U4{0, 0, 0, 0};
-    }
-
-    __device__ __forceinline__ void first_row_alone() {
-#pragma unroll
-        for (int l = 0; l < kLoads; l++)
-            if (row(l)) raw[l] = U4{0, 0, 0, 0};
     }
 
     /* Adds to sums in turn what is NaN in some lane if any element of the chunk is
@@ -274,10 +298,10 @@ struct Unit {
  * and j places of the chunk, E the state that enters it and P the scores q_i k_j
  * decay^(i - j) of an episode, j <= i:
  *   out = P v + decay^i q E,  E' = decay^places E + (decay^(places - j) k)^T v
- * PART: tiles of 16 columns that are all filled up are left out of products,
- * which in 32 bits are most of the time: the backward pass of 333 steps of 57 x
- * 3 with heads of 48 and 80 takes 120 us so, 150 without.  Where no tile is,
- * asking costs 2 to 5 % (heads of 64 and of 128).
+ * PART: some columns are filled up.  Tiles of 16 that all are, are left out of
+ * products, which in 32 bits are most of the time: the backward pass of 333
+ * steps of 57 x 3 with heads of 48 and 80 takes 122 us so, 150 without.  Where
+ * none are, asking costs 2 to 10 % (heads of 64 and of 128).
  * 64 steps of 4,096 environments with 4 heads of 64 in bf16 take 185 us forward
  * (4.4 TB/s, vector units 33 % busy, matrix units 9) and 395 back (3.1 TB/s, 41
  * and 12), two histories of 65,536 steps and 8 heads of 128 151 us for the
@@ -420,15 +444,20 @@ struct Walk {
             /* A product with a weight of 0 would carry what is not finite in k or v to other places:
              * such a place is a chunk by itself. */
             F4 zero[4] = {};
+            if (PART) {
+                tk.fit_columns(m.key);
+                if (active) tv.fit_columns(value);
+                if (!STATE) tq.fit_columns(m.key);
+            }
             tk.times_0(zero);
             tv.times_0(zero);
             zero[0] = zero[0] + zero[1] + (zero[2] + zero[3]);
             const bool found = __ballot(zero[0][0] + zero[0][1] + (zero[0][2] + zero[0][3]) != 0.0f) != 0;
             auto alone = [&]() {
                 n = 1;
-                tk.first_row_alone();
-                tv.first_row_alone();
-                if (!STATE) tq.first_row_alone();
+                tk.rows_beyond(1);
+                tv.rows_beyond(1);
+                if (!STATE) tq.rows_beyond(1);
             };
             auto stage = [&]() {
                 fence();
@@ -1011,12 +1040,8 @@ hipError_t launch_walk(const Job& j, hipStream_t stream) {
 
 template <typename T, int KD, int VD, int W, bool STATE>
 hipError_t launch(const Job& j, hipStream_t stream) {
-    if constexpr (!__is_same(T, __bf16)) {
-        for (int i = 0; i < j.roles; i++) {
-            const Mix& m = j.mix[i];
-            if (ceil_div(m.key, 16) * 16 < KD || ceil_div(m.value, 16) * 16 % VD) return launch_walk<T, KD, VD, W, STATE, true>(j, stream);
-        }
-    }
+    for (int i = 0; i < j.roles; i++)
+        if (j.mix[i].key < KD || j.mix[i].value % VD) return launch_walk<T, KD, VD, W, STATE, true>(j, stream);
     return launch_walk<T, KD, VD, W, STATE, false>(j, stream);
 }
 
