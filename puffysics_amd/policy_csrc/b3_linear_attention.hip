@@ -300,7 +300,7 @@ struct Unit {
  *   out = P v + decay^i q E,  E' = decay^places E + (decay^(places - j) k)^T v
  * PART: some columns are filled up.  Tiles of 16 that all are, are left out of
  * products, which in 32 bits are most of the time: the backward pass of 333
- * steps of 57 x 3 with heads of 48 and 80 takes 122 us so, 150 without.  Where
+ * steps of 57 x 3 with heads of 48 and 80 takes 118 us so, 150 without.  Where
  * none are, asking costs 2 to 10 % (heads of 64 and of 128).
  * 64 steps of 4,096 environments with 4 heads of 64 in bf16 take 185 us forward
  * (4.4 TB/s, vector units 33 % busy, matrix units 9) and 395 back (3.1 TB/s, 41
@@ -771,7 +771,7 @@ __global__ __launch_bounds__(kThreads, 2) void la_walk(Job j) {
 
 /* What enters each piece, over what the pieces left by themselves; kAhead of
  * them are on their way at a time.  Of few sequences that is what it takes, else
- * memory: 31 pieces of 16 states of 128 x 128 15 us, 4.1 TB/s. */
+ * memory: 31 pieces of 16 states of 128 x 128 12 us, 5.2 TB/s. */
 __global__ __launch_bounds__(kThreads) void la_join(Job j) {
     constexpr int kAhead = 8;
     const Mix& m = j.mix[blockIdx.y];
