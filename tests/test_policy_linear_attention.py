@@ -494,3 +494,21 @@ def test_c_refusals():
         assert call(**change) == 1, change
     assert call(envs=0) == 0 and call(heads=0) == 0 and call(steps=0) == 0
     assert lib.b3_linear_attention_gpu(None, None, None, None, 0, None) == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", TYPES)
+def test_columns_that_do_not_fill_vectors(type):
+    """Every number of columns left over, of narrow and of wide heads; the
+    last head's rows end the arrays."""
+    from puffysics_amd import policy
+    dtype = TYPES[type]
+    for key in (*range(1, 18), 35, 39, 46, 62, 97, 109, 127):
+        size = (40, 1, 2, key, 128 - key)
+        q, k, v, decay, starts, state = made(*size, dtype, key)
+        got = policy.linear_attention(q, k, v, decay, state=state, starts=starts, scale=0.1, last=True)
+        want, states = attention_oracle(q, k, v, decay, state, starts, 0.1)
+        most, most_states = bounds(q, k, v, decay, state, starts, 0.1)
+        a, b = allowed(dtype, key, size[0])
+        close(got.out, want, a * most, dtype)
+        close(got.state, states[-1], b * most_states[-1], torch.float32)
