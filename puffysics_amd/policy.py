@@ -758,7 +758,8 @@ class _Optimizer:
 
     def _pointers(self, grads):
         """Addresses and, where they are not the parameters', types of the
-        gradients, and the parameters that have one."""
+        gradients, the parameters that have one, and the gradients that the
+        addresses are of, which a step holds until its call has returned."""
         if list(map(_address, self.params)) != self._at:
             raise ValueError("a parameter's memory is not where it was")
         stepped, shapes, dtypes, given = self.params, self._shapes, self._dtypes, grads
@@ -781,7 +782,7 @@ class _Optimizer:
             pointers = array.array("Q", [0 if g is None else g.data_ptr() or _EMPTY for g in grads])
         kinds = None if types == dtypes else \
             array.array("i", [_TYPE[d if g is None else g.dtype] for g, d in zip(grads, self._dtypes)])
-        return pointers, kinds, stepped
+        return pointers, kinds, stepped, grads
 
     def master(self):
         """The flat array of 32-bit copies of 16-bit weights (the places of
@@ -861,7 +862,7 @@ class AdamW(_Optimizer):
         lr = self.lr if lr is None else lr
         _need(lr >= 0, "lr has to be at least 0")
         _need(self.max_grad_norm is None or self.max_grad_norm > 0, "max_grad_norm has to be over 0, or None")
-        pointers, kinds, stepped = self._pointers(grads)
+        pointers, kinds, stepped, grads = self._pointers(grads)
         self._follow_copies()
         norm = torch.empty((), dtype=torch.float32, device=self.device) if self.max_grad_norm is not None else None
         _check("b3_adamw_step_gpu", self._lib.b3_adamw_step_gpu(
@@ -967,7 +968,7 @@ class Muon(_Optimizer):
         grads = self._grads(grads)
         lr = self.lr if lr is None else lr
         _need(lr >= 0, "lr has to be at least 0")
-        pointers, kinds, stepped = self._pointers(grads)
+        pointers, kinds, stepped, grads = self._pointers(grads)
         self._follow_copies()
         _check("b3_muon_step_gpu", self._lib.b3_muon_step_gpu(
             self._h, pointers.buffer_info()[0], kinds.buffer_info()[0] if kinds else None, lr, _stream()))

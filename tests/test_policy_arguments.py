@@ -146,3 +146,65 @@ def test_rows_without_a_workspace():
     from b3test import ROOT
     text = open(ROOT + "/puffysics_amd/policy_csrc/b3_log_probs.hip").read()
     assert "kSmall = %d," % policy._SMALL in text
+
+
+@pytest.mark.parametrize("optimizer,entry", [("AdamW", "b3_adamw_step_gpu"), ("Muon", "b3_muon_step_gpu")])
+def test_negated_gradients_are_held_until_the_launch(monkeypatch, optimizer, entry):
+    """The copies that a step reads live until its call has returned.  Nothing
+    is launched: the library is a stand-in, on host tensors."""
+    import ctypes
+    import types
+    import weakref
+    from puffysics_amd import policy
+    made, alive = [], []
+
+    def as_read(x):
+        y = x if x is None else x.resolve_neg()
+        if y is not x:
+            made.append(weakref.ref(y))
+        return y
+
+    def launch(handle, pointers, *rest):
+        alive.extend(r() is not None for r in made)
+        at = (ctypes.c_uint64 * 3).from_address(pointers)
+        assert [list((ctypes.c_float * 4).from_address(at[i])) for i in (0, 2)] == [[1, -2, 3, -4], [5, 6, 7, 8]]
+        assert at[1] == 0
+        return 0
+
+    monkeypatch.setattr(policy, "_as_read", as_read)
+    monkeypatch.setattr(policy, "_stream", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)            # the host's, as _get_device says
+    opt = object.__new__(getattr(policy, optimizer))
+    opt.params = [torch.zeros(2, 2) for _ in range(3)]
+    opt._at, opt._shapes, opt._dtypes = ([f(p) for p in opt.params] for f in (
+        torch.Tensor.data_ptr, lambda p: p.shape, lambda p: p.dtype))
+    opt._empty, opt._master, opt._h, opt.lr, opt.max_grad_norm, opt.device = False, None, None, 0.1, 1.0, "cpu"
+    opt._lib = types.SimpleNamespace(**{entry: launch})
+    opt.step([torch._neg_view(torch.tensor([[-1.0, 2], [-3, 4]])), None, torch.tensor([[5.0, 6], [7, 8]])])
+    assert alive == [True]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count", [1, 2, 50, 128, 1000])
+def test_adamw_clips_by_negated_gradients(count):
+    """The norm that a clip needs gets no memory of what the step reads."""
+    from puffysics_amd import policy
+    params, twins = ([torch.ones(count, device="cuda") for _ in range(3)] for _ in range(2))
+    a, b = policy.AdamW(params, max_grad_norm=0.1), policy.AdamW(twins, max_grad_norm=0.1)
+    for t in range(4):
+        g = [torch.randn(count, device="cuda") for _ in range(3)]
+        assert torch.equal(a.step([torch._neg_view(-x) for x in g]), b.step(g))
+        assert all(torch.equal(p, q) for p, q in zip(params, twins)) and torch.equal(a.moments()[1], b.moments()[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 1), (7, 9), (64, 64), (130, 150)])
+def test_muon_with_negated_gradients(shape):
+    from puffysics_amd import policy
+    params, twins = ([torch.ones(shape, device="cuda") for _ in range(2)] for _ in range(2))
+    a, b = policy.Muon(params), policy.Muon(twins)
+    for t in range(3):
+        g = [torch.randn(shape, device="cuda") for _ in range(2)]
+        a.step([torch._neg_view(-x) for x in g])
+        b.step(g)
+        assert all(torch.equal(p, q) for p, q in zip(params, twins)) and torch.equal(a.momentum(), b.momentum())
