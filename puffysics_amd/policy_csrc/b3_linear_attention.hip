@@ -26,6 +26,7 @@ constexpr int kThreads = 256;
 constexpr int kRoles = 3;                        // of a launch
 static_assert((int64_t)B3_MAX_SEQUENCES * kRoles * kThreads < (int64_t)1 << 32, "threads of a launch");
 constexpr int64_t kAlone = 1024, kFull = 2048;   // waves with a SIMD to themselves, and two to each
+constexpr float kHold = 256.0f;                  // a state is held as between itself and 1 / kHold of it
 
 /* out_p = `reach` q_p (decay^p E + sums over p' <= p of the episode of
  * `update` decay^(p - p') k_p'^T v_p'), and the state that is left,
@@ -369,7 +370,7 @@ struct Walk {
         ValueTile tv;
         uint32_t flag = 0;
         bool dropped = false;
-        float scale = 1.0f;                      // of the state
+        float scale = kHold;                     // of the state
         bool any = enter != NULL;                // state
         auto fetch = [&](int64_t p) {
             const int n = places - p < kPlaces ? (int)(places - p) : kPlaces;
@@ -625,20 +626,21 @@ struct Walk {
             any = true;
             /* What is kept of the state, and of the places from the last start on.  The state is
              * held as E / scale, so that no chunk has to go over it: its decay goes into scale and,
-             * before that becomes small, into the state. */
+             * before that is under 1, into the state.  So what is held is never larger than E, nor
+             * than k v what is added to it: nothing overflows that E does not. */
             const int last = starts ? 31 - __builtin_clz(starts) : -1;
             if (starts) {
                 dropped = true;
-                scale = 1.0f;
+                scale = kHold;
 #pragma unroll
                 for (int kb = 0; kb < KB; kb++)
 #pragma unroll
                     for (int vb = 0; vb < VB; vb++) state[kb][vb] = F4{0, 0, 0, 0};
-            } else if (scale * pass > 0x1p-20f) {
+            } else if (scale * pass >= 1.0f) {
                 scale *= pass;
             } else {
-                const float f = scale * pass;
-                scale = 1.0f;
+                const float f = scale * pass * (1.0f / kHold);
+                scale = kHold;
 #pragma unroll
                 for (int kb = 0; kb < KB; kb++)
 #pragma unroll

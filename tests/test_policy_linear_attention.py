@@ -512,3 +512,54 @@ def test_columns_that_do_not_fill_vectors(type):
         a, b = allowed(dtype, key, size[0])
         close(got.out, want, a * most, dtype)
         close(got.state, states[-1], b * most_states[-1], torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type,size", [("f32", 2e34), ("f32", 3e38), ("f32", 1e-28), ("bf16", 1e37), ("bf16", 3e38),
+                                       ("bf16", 1e-28), ("f16", 6e4)])
+@pytest.mark.parametrize("key,value", [(1, 1), (64, 64), (128, 128), (17, 100)])
+@pytest.mark.parametrize("decay", [0.9, 0.999, 1.0])
+def test_sizes_of_numbers(type, size, key, value, decay):
+    """States that 32 bits hold are right however large or small they are: of
+    few sequences, in pieces, and of many, and step by step; the gradient of
+    the state that was entered with alike."""
+    from puffysics_amd import policy
+    dtype, decay = TYPES[type], torch.tensor([decay], device="cuda")
+    g = torch.Generator().manual_seed(key)
+    steps = 300
+    some = lambda d, size: ((torch.rand(steps, 1, 1, d, generator=g) + 0.5) * size).to(dtype).cuda()  # noqa: E731
+    # one step of the size among small ones, or all of a small size
+    at = slice(100, 101) if size > 1 else slice(0, steps)
+    big = (torch.rand(steps, 1, 1, value, generator=g) * 0.5 + 0.5).mul(size).to(dtype).cuda()
+    q, k, v = some(key, 1e-6 / key if size > 1e5 else 1e-3 if size > 1 else 1.0), some(key, 0.1), some(value, 1e-3)
+    v[at] = big[at]
+
+    def near(got, want, bound):
+        assert ((got.double() - want).abs() <= bound + STEP[got.dtype] * want.abs() + (2.0 ** -25 if type == "f16" else 0)).all()
+
+    want, states = attention_oracle(q, k, v, decay)
+    a, b = allowed(dtype, key, steps)
+    most, most_states = bounds(q, k, v, decay, None, None, 1.0)
+    for envs in (1, 3000):
+        got = policy.linear_attention(*(x.expand(steps, envs, 1, x.shape[-1]) for x in (q, k, v)), decay, last=True)
+        for e in (0, envs - 1):
+            near(got.out[:, e:e + 1], want, a * most)
+            near(got.state[e:e + 1], states[-1], b * most_states[-1])
+    s = torch.zeros(1, 1, key, value, device="cuda")
+    for t in range(steps):
+        policy.linear_attention_step(q[t], k[t], v[t], decay, s)
+    near(s, states[-1], b * most_states[-1])
+    # G grows by what comes in, as the state by v
+    d_out, q, v = v, some(key, 0.1), some(value, 1e-3)
+    for envs in (1, 3000):
+        leaves = [x.expand(steps, envs, 1, x.shape[-1]).detach().requires_grad_() for x in (q, k, v)]
+        leaves.append(torch.zeros(envs, 1, key, value, device="cuda", requires_grad=True))
+        out = policy.linear_attention(*leaves[:3], decay, state=leaves[3]).out
+        _, d_k, _, d_state = torch.autograd.grad(out, leaves, d_out.expand(steps, envs, 1, value))
+        want = attention_gradient_oracle(q, k, v, decay, s, None, 1.0, d_out)
+        most = attention_gradient_oracle(q, k, v, decay.sqrt(), s, None, 1.0, d_out)
+        a, b = allowed(dtype, value, steps)
+        for e in (0, envs - 1):
+            near(d_state[e:e + 1], want[3], b * most[3])
+            if type != "f16":
+                near(d_k[:, e:e + 1], want[1], a * most[1])
