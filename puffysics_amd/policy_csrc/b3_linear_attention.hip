@@ -363,14 +363,15 @@ struct Walk {
             reach[t] = m.reach * power(l2, 16 * t + c);
         }
         F4 keep[R];
-        float pass = 0;
-        int weighted = -1;                       // places and the step less that keep and pass are for
+        int weighted = -1;                       // places and the step less that keep is for
 
         KeyTile tk, tq;
         ValueTile tv;
         uint32_t flag = 0;
         bool dropped = false;
-        float scale = kHold;                     // of the state
+        /* of the state: top decay^held, from its one rounding to 32 bits (a chunk's power times itself would add up) */
+        float scale, top = kHold;
+        int held = 0;
         bool any = enter != NULL;                // state
         auto fetch = [&](int64_t p) {
             const int n = places - p < kPlaces ? (int)(places - p) : kPlaces;
@@ -391,7 +392,6 @@ struct Walk {
         if (places > 0) fetch(0);
         /* E, lane (g, c) of tile [kb][vb] rows 16 kb + 4 g + r and the column of c */
         F4 state[KB][VB];
-        const float first = early ? power(l2, 1) : 1.0f;
         const int state_row = (int)m.state_row, state_col = (int)m.state_col;
         if (enter && active) {
             const float* at[VB];
@@ -419,7 +419,8 @@ struct Walk {
                         for (int vb = 0; vb < VB; vb++) state[kb][vb][r] = at[vb][offset];
                     }
             }
-            scale = first;
+            top = 1.0f;
+            held = early ? 1 : 0;
             if (m.key < KD || value < VD) {
 #pragma unroll
                 for (int kb = 0; kb < KB; kb++)
@@ -438,6 +439,7 @@ struct Walk {
                 for (int vb = 0; vb < VB; vb++) state[kb][vb] = F4{0, 0, 0, 0};
         }
 
+        scale = top * power(l2, held);
         int n;
 #pragma unroll 1
         for (int64_t p = 0; p < places; p += n) {
@@ -621,7 +623,6 @@ struct Walk {
                         const int at = 16 * t + 4 * g + r;
                         keep[t][r] = at < n ? m.update * power(l2, n - at - less) : 0.0f;
                     }
-                pass = power(l2, n - less);
             }
             any = true;
             /* What is kept of the state, and of the places from the last start on.  The state is
@@ -629,18 +630,22 @@ struct Walk {
              * before that is under 1, into the state.  So what is held is never larger than E, nor
              * than k v what is added to it: nothing overflows that E does not. */
             const int last = starts ? 31 - __builtin_clz(starts) : -1;
+            held += n - less;
+            const float next = top * power(l2, held);
             if (starts) {
                 dropped = true;
-                scale = kHold;
+                scale = top = kHold;
+                held = 0;
 #pragma unroll
                 for (int kb = 0; kb < KB; kb++)
 #pragma unroll
                     for (int vb = 0; vb < VB; vb++) state[kb][vb] = F4{0, 0, 0, 0};
-            } else if (scale * pass >= 1.0f) {
-                scale *= pass;
+            } else if (next >= 1.0f) {
+                scale = next;
             } else {
-                const float f = scale * pass * (1.0f / kHold);
-                scale = kHold;
+                const float f = next * (1.0f / kHold);
+                scale = top = kHold;
+                held = 0;
 #pragma unroll
                 for (int kb = 0; kb < KB; kb++)
 #pragma unroll

@@ -1,5 +1,7 @@
 """puffysics_amd.policy.linear_attention and linear_attention_step against the
 definition in 64 bits."""
+import math
+
 import pytest
 import torch
 
@@ -563,3 +565,28 @@ def test_sizes_of_numbers(type, size, key, value, decay):
             near(d_state[e:e + 1], want[3], b * most[3])
             if type != "f16":
                 near(d_k[:, e:e + 1], want[1], a * most[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("decay,steps", [(1 - 2.0 ** -14, 16384), (1 - 2.0 ** -14, 1000), (1 - 2.0 ** -10, 30000),
+                                         (0.97, 2000), (0.5, 100)])
+def test_what_is_left_after_many_steps(decay, steps, type):
+    """Of a state alone: decay^steps, forwards and back.  Its logarithm, to
+    2^-23 of it, and the product with the steps are off by 1.5 2^-23 of the
+    bits that the state falls by; a power and its product by 2^-22 each time
+    that the state is gone over, which is once for 8 bits, or where pieces
+    meet."""
+    from puffysics_amd import policy
+    decay = torch.tensor([decay], device="cuda")
+    want = float(decay.double() ** steps)
+    bits = -math.log2(want)
+    for envs, pieces in ((3000, 0), (1, 64)):
+        x = torch.zeros(1, 1, 1, 1, dtype=TYPES[type], device="cuda").expand(steps, envs, 1, 1)
+        q, k, v = (x.detach().requires_grad_() for _ in range(3))
+        state = torch.full((envs, 1, 1, 1), 3.0, device="cuda", requires_grad=True)
+        got = policy.linear_attention(q, k, v, decay, state=state, last=True)
+        d_state, = torch.autograd.grad(got.state, state, torch.full_like(state, 5.0))
+        most = math.log(2) * bits * 1.5 * 2.0 ** -23 + (bits / 8 + 3 + pieces) * 2.0 ** -22
+        assert float((got.state.detach().double() / (3 * want) - 1).abs().max()) <= most
+        assert float((d_state.double() / (5 * want) - 1).abs().max()) <= most
