@@ -228,7 +228,10 @@ size_t b3_linear_attention_workspace(const B3Attention* attention, int backward)
 /*   S_t = decay S_{t-1} + k_t^T v_t (without the first term where an episode
  *   starts), out_t = scale q_t S_t
  * out [steps, envs, heads, value], contiguous; last_state (NULL: not wanted)
- * like `state`, and apart from it: S after the last step. */
+ * like `state`, and apart from it: S after the last step.  States and sums are
+ * in 32 bits; with bfloat16 the products q_t k_s of steps of a chunk, and the
+ * state, are read to 16 bits where they give out.  Such products overflow past
+ * 2^127, also where v is small; what an infinity comes to may be NaN. */
 hipError_t b3_linear_attention_gpu(const B3Attention* attention, void* out, float* last_state, void* workspace,
     size_t workspace_bytes, hipStream_t stream);
 

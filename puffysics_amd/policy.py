@@ -484,8 +484,12 @@ def linear_attention(q, k, v, decay, state=None, starts=None, scale=1.0, last=Fa
 
     Any strides; key and value are at most 128.  out is laid out contiguously.
     Differentiable in q, k, v and state (backward and once; a tangent is
-    refused).  States and sums are in 32 bits; what lies before an episode's
-    start, and later steps, have no say in a step, whatever they hold."""
+    refused).  States and sums are in 32 bits; in bfloat16 the products q k and
+    the state are read to 16 bits where they give out.  Products q k of steps
+    near to each other are formed, in 32 bits: past 2^127 they overflow, also
+    where v is small; what an infinity comes to may be NaN.  What lies before an
+    episode's start, and later steps, have no say in a step, whatever they
+    hold."""
     _need(q.dim() == 4, "q has to be [steps, envs, heads, key]")
     _check_attention(q, k, v, decay, starts, scale)
     if state is not None:

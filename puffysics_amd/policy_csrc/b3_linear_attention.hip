@@ -507,8 +507,8 @@ struct Walk {
                     const uint32_t before = starts & (uint32_t)((2ull << (16 * t + c)) - 1);
                     since[t] = before ? 31 - __builtin_clz(before) : -1;
                 }
-                /* scores, rows j and columns i; they are what P v sums over as they lie */
-                Quad score[R][R];
+                /* scores, rows j and columns i; they are what P v sums over as they lie, in 16 bits as two numbers */
+                Quad score[R][R], rest[R][R];
 #pragma unroll
                 for (int s = 0; s < R; s++) {
                     Quad kq[KB];
@@ -539,6 +539,7 @@ struct Walk {
                                 if (16 * s + 4 * g + r < since[t]) x[r] = 0.0f;
                         }
                         score[t][s] = with(x);
+                        if constexpr (kHalf) rest[t][s] = rest4(x, score[t][s]);
                     }
                 }
                 /* kTiles tiles of columns at a time, which a lane writes together */
@@ -587,10 +588,12 @@ struct Walk {
                     for (int t = 0; t < R; t++)
 #pragma unroll
                         for (int i = 0; i < kTiles; i++) {
-                            if constexpr (kHalf)
+                            if constexpr (kHalf) {
+                                o[t][i] = multiply(vq[0][v0 + i], vq[1][v0 + i], rest[t][0], t ? rest[1][1] : S4{0, 0, 0, 0}, o[t][i]);
                                 o[t][i] = multiply(vq[0][v0 + i], vq[1][v0 + i], score[t][0], t ? score[1][1] : S4{0, 0, 0, 0}, o[t][i]);
-                            else
+                            } else {
                                 o[t][i] = multiply(vq[0][v0 + i], score[0][0], o[t][i]);
+                            }
                         }
                     /* lane (g, c): of place 16 t + c the columns 4 g + r of each tile */
                     const int col = value_col(v0) + kWide * g;

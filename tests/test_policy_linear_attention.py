@@ -590,3 +590,32 @@ def test_what_is_left_after_many_steps(decay, steps, type):
         most = math.log(2) * bits * 1.5 * 2.0 ** -23 + (bits / 8 + 3 + pieces) * 2.0 ** -22
         assert float((got.state.detach().double() / (3 * want) - 1).abs().max()) <= most
         assert float((d_state.double() / (5 * want) - 1).abs().max()) <= most
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("given", ["nothing", "both"])
+@pytest.mark.parametrize("size", [*SIZES, (4000, 1, 2, 64, 64), (64, 300, 2, 64, 64)], ids=lambda s: "x".join(map(str, s)))
+def test_sums_of_bfloat16(size, given):
+    """Rounded once, at the end: scores and the state that bfloat16 numbers are
+    multiplied with are two such numbers, to 2^-16 of them each (2^-18 where
+    they lie evenly: the half step of a second number of 8 bits)."""
+    from puffysics_amd import policy
+    dtype, scale = torch.bfloat16, size[3] ** -0.5
+    q, k, v, decay, starts, state = made(*size, dtype, sum(size))
+    d_out = torch.randn(v.shape, generator=torch.Generator().manual_seed(5)).to(dtype).cuda()
+    starts, state = (starts, state) if given == "both" else (None, None)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    got = policy.linear_attention(q, k, v, decay, state=state, starts=starts, scale=scale).out
+    grads = torch.autograd.grad(got, leaves, d_out)
+    with torch.no_grad():
+        want, _ = attention_oracle(q, k, v, decay, state, starts, scale)
+        most, _ = bounds(q, k, v, decay, state, starts, scale)
+        wants = attention_gradient_oracle(q, k, v, decay, state, starts, scale, d_out)
+        mosts = attention_gradient_oracle(q.abs(), k.abs(), v.abs(), decay.sqrt(), None if state is None else state.abs(),
+                                          starts, scale, d_out.abs())
+        a = 2.0 ** -16 + (max(size[3:]) + size[0] + 64) * 2.0 ** -24
+        for x, y, m in zip((got, *grads), (want, *wants), (most, *mosts)):
+            close(x, y, a * m, dtype)
+            # together: next to what the last rounding leaves, little
+            far, least = (x.double() - y).norm(), (y.to(dtype).double() - y).norm()
+            assert float(far) <= 1.01 * float(least) + 2.0 ** -16 * float(m.norm())
