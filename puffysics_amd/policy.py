@@ -495,7 +495,7 @@ def linear_attention(q, k, v, decay, state=None, starts=None, scale=1.0, last=Fa
     if state is not None:
         _need(state.dtype == torch.float32 and state.shape == (*q.shape[1:], v.shape[-1]),
               "state has to be float32 [envs, heads, key, value]")
-    _no_tangent("linear_attention", q, k, v, state)
+    _no_tangent("linear_attention", q, k, v, decay, state)
     _on(q, k, v, decay, state, starts)
     q, k, v, decay, starts = _heads(q), _heads(k), _heads(v), _as_read(decay).contiguous(), _as_read(starts)
     if state is not None:
@@ -516,7 +516,7 @@ def linear_attention_step(q, k, v, decay, state, starts=None, scale=1.0):
           and not state.is_neg(), "state has to be float32 [envs, heads, key, value], contiguous, not marked as negated")
     if _needs_grad(q, k, v, state):
         raise ValueError("linear_attention_step has no gradient")
-    _no_tangent("linear_attention_step", q, k, v, state)
+    _no_tangent("linear_attention_step", q, k, v, decay, state)
     _on(q, k, v, decay, state, starts)
     q, k, v, decay, starts = _heads(q), _heads(k), _heads(v), _as_read(decay).contiguous(), _as_read(starts)
     out = torch.empty_like(v, memory_format=torch.contiguous_format)

@@ -619,3 +619,22 @@ def test_sums_of_bfloat16(size, given):
             # together: next to what the last rounding leaves, little
             far, least = (x.double() - y).norm(), (y.to(dtype).double() - y).norm()
             assert float(far) <= 1.01 * float(least) + 2.0 ** -16 * float(m.norm())
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "decay", "state"])
+def test_tangents_are_refused(name):
+    """Of every argument that a derivative could go through, the rollout's and
+    the step's; without one the next check is reached.  Nothing is launched:
+    this runs without a GPU."""
+    from torch.autograd import forward_ad
+
+    from puffysics_amd import policy
+    z = torch.zeros
+    rollout = dict(q=z(5, 3, 2, 8), k=z(5, 3, 2, 8), v=z(5, 3, 2, 4), decay=z(2), state=z(3, 2, 8, 4))
+    step = {n: x[0] if n in "qkv" else x for n, x in rollout.items()}
+    with forward_ad.dual_level():
+        for call, args in ((policy.linear_attention, rollout), (policy.linear_attention_step, step)):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call(**{**args, name: forward_ad.make_dual(args[name], torch.ones_like(args[name]))})
+            with pytest.raises(ValueError, match="CUDA device"):
+                call(**args)
