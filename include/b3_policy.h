@@ -203,11 +203,11 @@ hipError_t b3_adamw_destroy(B3AdamW* optimizer);
 
 /* q and k [steps, envs, heads, key], v [steps, envs, heads, value]: strides
  * in elements from step to step, environment to environment and head to
- * head; a head's elements are contiguous.  `decay` [heads] is in [0, 1] (a state
- * becomes NaN by others).  `starts` is NULL or [steps, envs], nonzero where a step begins
- * an episode: what lies before is dropped (not multiplied by 0: its NaN stay
- * there).  `state` [envs, heads, key, value], contiguous, is what the first
- * step finds; NULL: zeros. */
+ * head; a head's elements are contiguous.  q, k and v may be NULL for no steps.
+ * `decay` [heads] is in [0, 1] (a state becomes NaN by others).  `starts` is NULL
+ * or [steps, envs], nonzero where a step begins an episode: what lies before is
+ * dropped (not multiplied by 0: its NaN stay there).  `state` [envs, heads, key,
+ * value], contiguous, is what the first step finds; NULL: zeros. */
 typedef struct B3Attention {
     int64_t steps, envs, heads;  /* envs * heads at most B3_MAX_SEQUENCES */
     int key, value;              /* 1 .. B3_MAX_HEAD */

@@ -1119,7 +1119,7 @@ hipError_t b3_linear_attention_gpu(const B3Attention* g, void* out, float* last_
     if (!valid(g)) return hipErrorInvalidValue;
     if (g->envs == 0 || g->heads == 0 || (g->steps == 0 && !last_state)) return hipSuccess;
     const Plan p = plan_of(*g, false);
-    if ((g->steps && !out) || !holds(workspace, workspace_bytes, workspace_of(*g, p, false))) return hipErrorInvalidValue;
+    if (!g->decay || (g->steps && !out) || !holds(workspace, workspace_bytes, workspace_of(*g, p, false))) return hipErrorInvalidValue;
     Job j = job_of(*g);
     Mix m = forwards(*g);
     m.q = g->q;
@@ -1146,9 +1146,9 @@ hipError_t b3_linear_attention_backward_gpu(const B3Attention* g, const void* d_
         const float* d_last_state, void* d_q, void* d_k, void* d_v, float* d_state, void* workspace,
         size_t workspace_bytes, hipStream_t stream) {
     if (!valid(g)) return hipErrorInvalidValue;
-    if (g->envs == 0 || g->heads == 0) return hipSuccess;
+    if (g->envs == 0 || g->heads == 0 || (g->steps == 0 && !d_state)) return hipSuccess;
     const Plan p = plan_of(*g, true);
-    if ((g->steps && (!d_out || !d_out_stride)) || !holds(workspace, workspace_bytes, workspace_of(*g, p, true)))
+    if (!g->decay || (g->steps && (!d_out || !d_out_stride)) || !holds(workspace, workspace_bytes, workspace_of(*g, p, true)))
         return hipErrorInvalidValue;
     Job j = job_of(*g);
     Mix a = forwards(*g);                        // d_q: S^T, of d_out, v and k

@@ -638,3 +638,25 @@ def test_tangents_are_refused(name):
                 call(**{**args, name: forward_ad.make_dual(args[name], torch.ones_like(args[name]))})
             with pytest.raises(ValueError, match="CUDA device"):
                 call(**args)
+
+
+def test_c_no_decay():
+    """Where a launch reads the decay it has to be there, also for no steps; a
+    call without work is none.  No call reaches a launch."""
+    import ctypes as C
+    from puffysics_amd import policy
+    lib = policy.policy_lib()
+    one = (C.c_char * 64)()
+    at = C.addressof(one)
+    g = policy.B3Attention(0, 1, 1, 8, 8, 0, None, None, None, (8, 8, 8), (8, 8, 8), (8, 8, 8), None, None, 0, (0, 0), None, 1.0)
+    by = (C.c_int64 * 3)(8, 8, 8)
+
+    def backward(d_v, d_state):
+        return lib.b3_linear_attention_backward_gpu(C.byref(g), None, by, None, None, None, d_v, d_state, None, 0, None)
+
+    assert lib.b3_linear_attention_gpu(C.byref(g), None, at, None, 0, None) == 1
+    assert lib.b3_linear_attention_gpu(C.byref(g), None, None, None, 0, None) == 0
+    assert backward(None, at) == 1 and backward(at, at) == 1
+    assert backward(None, None) == 0 and backward(at, None) == 0
+    g.steps, g.q, g.k, g.v = 1, at, at, at
+    assert lib.b3_linear_attention_step_gpu(C.byref(g), at, at, None) == 1
