@@ -548,9 +548,15 @@ def _norm(x, residual, weight, eps):
                       0 if weight is None else weight.data_ptr(), 0 if weight is None else _TYPE[weight.dtype], eps)
 
 
-def _normalise(x, weight, residual, eps, kept):
-    """(out, sum or None, root or None), the last only where `kept`."""
-    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+def _result(x, shape):
+    """A tensor of `shape` for what comes of rows x."""
+    return torch.empty_like(x, memory_format=torch.contiguous_format) if len(shape) == 2 else x.new_empty(shape)
+
+
+def _normalise(x, weight, residual, eps, kept, shape):
+    """(out, sum or None, root or None) of rows x, the first two of `shape`, the
+    last only where `kept`."""
+    out = _result(x, shape)
     total = None if residual is None else torch.empty_like(out)
     root = torch.empty(x.shape[0], dtype=torch.float32, device=x.device) if kept else None
     _check("b3_rms_norm_gpu", policy_lib().b3_rms_norm_gpu(
@@ -561,16 +567,15 @@ def _normalise(x, weight, residual, eps, kept):
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
+        # (made with their axes: of views that are made here a program could write to none in place)
         shape = x.shape
         x, residual = _as_rows(x), _as_rows(residual)
-        out, total, root = _normalise(x, weight, residual, eps, True)
+        out, total, root = _normalise(x, weight, residual, eps, True, shape)
         # in 32 bits the sum is what was normalised; in 16 it has been rounded
         x, residual = (total, None) if residual is not None and x.dtype == torch.float32 else (x, residual)
         ctx.save_for_backward(x, residual, weight, root)
         ctx.set_materialize_grads(False)
-        if len(shape) == 2:
-            return out, total
-        return out.view(shape), None if total is None else total.view(shape)
+        return out, total
 
     @staticmethod
     def backward(ctx, d_out, d_sum):
@@ -581,22 +586,21 @@ def _norm_backward(ctx, d_out, d_sum):
     if d_out is None and d_sum is None:      # of what takes part in nothing that has a gradient
         return (None,) * 4
     x, residual, weight, root = ctx.saved_tensors
+    x = x if x.dim() == 2 else x.view(-1, x.shape[-1])
     rows, width = x.shape
     lib = policy_lib()
     shape = (d_sum if d_out is None else d_out).shape
     d_out, d_sum = _as_rows(d_out), _as_rows(d_sum)
     # the stride of a lone row says nothing
     out_stride, sum_stride = (0 if d is None else d.stride(0) if rows > 1 else width for d in (d_out, d_sum))
-    d_x = torch.empty_like(x, memory_format=torch.contiguous_format)
+    # one tensor for both x and the residual, as a sum's gradient is: views of it would become the grad of two leaves
+    d_x = _result(x, shape)
     d_weight = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
     size = lib.b3_rms_norm_backward_workspace(rows, width)
     work = _work(size, x.device)
     _check("b3_rms_norm_backward_gpu", lib.b3_rms_norm_backward_gpu(
         _norm(x, residual, weight, 0.0), root.data_ptr(), _address_of(d_out), out_stride, _address_of(d_sum), sum_stride, d_x.data_ptr(),
         _address_of(d_weight), _address_of(work), size, _stream()))
-    # one tensor for both, as a sum's gradient is: views of it would become the grad of two leaves
-    if len(shape) != 2:
-        d_x = d_x.view(shape)
     return (d_x if ctx.needs_input_grad[0] else None, d_weight, d_x if ctx.needs_input_grad[2] else None, None)
 
 
@@ -643,10 +647,7 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6):
     weight = None if weight is None else _as_read(weight).contiguous()
     if _needs_grad(x, weight, residual):
         return RmsNorm(*_RmsNorm.apply(x, weight, residual, float(eps)))
-    out, total, _ = _normalise(_as_rows(x), weight, _as_rows(residual), eps, False)
-    if x.dim() == 2:
-        return RmsNorm(out, total)
-    return RmsNorm(out.view(x.shape), None if total is None else total.view(x.shape))
+    return RmsNorm(*_normalise(_as_rows(x), weight, _as_rows(residual), eps, False, x.shape)[:2])
 
 
 def rms_norm_8bit(x, weight=None, residual=None, eps=1e-6):

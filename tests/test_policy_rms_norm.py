@@ -327,3 +327,40 @@ def test_refusals():
     from torch.autograd import forward_ad
     with forward_ad.dual_level(), pytest.raises(ValueError, match="forward-mode"):
         policy.rms_norm(forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(30, 32), (6, 5, 32), (2, 3, 5, 32), (32,)], ids=str)
+def test_results_written_in_place(shape):
+    """A program may go on in place from either result, whatever its axes."""
+    from puffysics_amd import policy
+    x, r = (torch.randn(shape, device="cuda").bfloat16().requires_grad_() for _ in range(2))
+    w = torch.randn(32, device="cuda", requires_grad=True)
+    up = torch.randn(shape, device="cuda").bfloat16()
+    got = policy.rms_norm(x, w, residual=r)
+    want = torch.autograd.grad((got.out * 2, got.sum + up), (x, r, w), (up, up))
+    got = policy.rms_norm(x, w, residual=r)
+    got.out.mul_(2)
+    got.sum.add_(up)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad((got.out, got.sum), (x, r, w), (up, up)), want))
+    out = policy.rms_norm(x, w).out
+    out.relu_()
+    want = torch.autograd.grad(torch.relu(policy.rms_norm(x, w).out), x, up)[0]
+    assert torch.equal(torch.autograd.grad(out, x, up)[0], want)
+    with torch.no_grad():
+        policy.rms_norm(x, w, residual=r).sum.add_(up)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(30, 32), (6, 5, 32)], ids=str)
+def test_gradients_of_two_leaves_are_two(shape):
+    """x and the residual get gradients of their own, which a program may
+    write to one by one."""
+    from puffysics_amd import policy
+    x, r = (torch.randn(shape, device="cuda").requires_grad_() for _ in range(2))
+    got = policy.rms_norm(x, residual=r)
+    (got.out.sum() + got.sum.square().sum()).backward()
+    assert torch.equal(x.grad, r.grad) and x.grad.shape == shape
+    before = r.grad.clone()
+    x.grad.zero_()
+    assert torch.equal(r.grad, before)
