@@ -246,3 +246,96 @@ def test_refusals_of_a_step():
         opt.load_momentum([good[0]])
     assert all(torch.equal(a, b) for a, b in zip(params, before)) and int(torch.count_nonzero(opt.momentum())) == 0
     policy.Muon([]).step([])
+
+
+def in_32_bits(u, steps=5, eps=1e-7):
+    """Muon's steps with torch's 32-bit products."""
+    x = u.float()
+    turned = x.shape[0] > x.shape[1]
+    x = x.t() if turned else x
+    x = x / (x.square().sum().sqrt() + eps)
+    for _ in range(steps):
+        y = x @ x.t()
+        x = 3.4445 * x + (-4.7750 * y + 2.0315 * (y @ y)) @ x
+    return x.t() if turned else x
+
+
+def far(x, want):
+    return float((x.double() - want).norm())
+
+
+def near_32_bits(u, want, steps=5):
+    """What x may be off by, in the norm of all elements.  A number is kept to
+    2^-22, a quarter as exactly as in 32 bits, of both sides of a product, and
+    matrices that take their steps on the short side have twice as many
+    products: 16 times what the steps in 32 bits are off by; or, where that
+    happens to be little, as of few or simple numbers, a step of each number's
+    for all that is formed in five steps, three products and z."""
+    return 16 * far(in_32_bits(u, steps), want) + 4 * max(steps, 5) * 2.0 ** -22 * float(want.norm())
+
+
+WIDE = [(1100, 1100), (1100, 1600), (1600, 1100), (130, 1500), (600, 1030), (256, 1024)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", SHAPES + WIDE, ids=lambda s: "%dx%d" % s)
+@pytest.mark.parametrize("kind", ["even", "low rank", "spike", "graded", "strong and weak"])
+def test_as_exact_as_32_bits(shape, kind):
+    """Next to the same steps with torch's 32-bit products, by the norm of the
+    difference; sides of more than a square of tiles among them."""
+    from puffysics_amd import policy
+    g = torch.Generator().manual_seed(sum(shape))
+    u = torch.randn(*shape, generator=g, dtype=torch.float64)
+    two = torch.randn(shape[0], 2, generator=g, dtype=torch.float64) @ torch.randn(2, shape[1], generator=g, dtype=torch.float64)
+    if kind == "low rank":
+        u = two
+    elif kind == "strong and weak":
+        u = two + 1e-4 * u
+    elif kind == "spike":
+        u = u * 1e-3
+        u[0, 0] = 100.0
+    elif kind == "graded":
+        u = u * torch.logspace(0, -6, shape[0], dtype=torch.float64)[:, None]
+    u = u.float().cuda()
+    param = torch.zeros(shape, device="cuda")
+    policy.Muon([param], math.sqrt(min(1.0, shape[1] / shape[0])), momentum=0.0).step([u])
+    want = -orthogonalised_oracle(u)
+    assert far(param, want) <= near_32_bits(-u, want), (far(param, want), near_32_bits(-u, want), float(want.norm()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 5, 6, 7, 11, 16])
+@pytest.mark.parametrize("shape", [(60, 90), (130, 200), (250, 1000), (700, 129)])
+def test_as_exact_after_any_steps(shape, steps):
+    from puffysics_amd import policy
+    g = torch.Generator().manual_seed(steps)
+    u = (torch.randn(shape[0], 3, generator=g) @ torch.randn(3, shape[1], generator=g)).cuda()
+    param = torch.zeros(shape, device="cuda")
+    policy.Muon([param], math.sqrt(min(1.0, shape[1] / shape[0])), momentum=0.0, newton_schulz=steps).step([u])
+    want = -orthogonalised_oracle(u, steps)
+    assert far(param, want) <= near_32_bits(-u, want, steps)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+def test_weights_move_as_exactly(type):
+    """Three steps with momentum over matrices of many shapes at once."""
+    from puffysics_amd import policy
+    dtype, shapes = TYPES[type], SHAPES + WIDE
+    params = tensors(shapes, dtype, 1, 0.1)
+    opt = policy.Muon(params, LR, MU, weight_decay=DECAY)
+    w, m = [p.double() for p in params], [torch.zeros_like(p, dtype=torch.float64) for p in params]
+    off = [0.0] * len(params)
+    for t in range(3):
+        grads = tensors(shapes, dtype, 20 + t)
+        opt.step(grads)
+        for i, g in enumerate(grads):
+            m[i] = MU * m[i] + g.double()
+            u = g.double() + MU * m[i]
+            x = orthogonalised_oracle(u)
+            rate = LR * math.sqrt(max(1.0, g.shape[0] / g.shape[1]))
+            w[i] = w[i] * (1 - LR * DECAY) - rate * x
+            # u is of 32 bits too: half a step, which the steps carry on as that of in_32_bits
+            off[i] += rate * near_32_bits(u, x) + 2.0 ** -22 * float(w[i].norm())
+            got = params[i] if dtype == torch.float32 else views(opt, opt.master())[i]
+            assert far(got, w[i]) <= off[i], (g.shape, t)
