@@ -325,8 +325,9 @@ hipError_t b3_muon_create(B3Muon** out, const B3MuonMatrix* matrices, int count,
  *   x = u / (|u| + eps), its transpose where rows > columns
  *   newton_schulz times: a = x x^T, x = 3.4445 x + (-4.775 a + 2.0315 a a) x
  *   w = w (1 - lr decay) - lr sqrt(max(1, rows / columns)) x
- * with products of 32-bit numbers.  Steps of one optimizer must follow one
- * another on the device. */
+ * Numbers of a product are kept to 22 bits (to 32 where a matrix is at most 64 x
+ * 256), its sums are in 32.  Steps of one optimizer must follow one another on
+ * the device. */
 hipError_t b3_muon_step_gpu(B3Muon* optimizer, const void* const* grads, const int* grad_types, double lr,
     hipStream_t stream);
 

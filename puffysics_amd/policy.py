@@ -938,8 +938,9 @@ class Muon(_Optimizer):
     weight_decay   a number, or one for each matrix
     master         32-bit copies of 16-bit weights, as AdamW's
 
-    Products are those of 32-bit numbers.  The momenta lie in a flat array,
-    matrix i's from offsets[i] on.  Steps of one optimizer follow one another:
+    Numbers of a product are kept to 22 bits (to 32 where a matrix is at most 64 x
+    256), its sums are in 32.  The momenta lie in a flat array, matrix i's from
+    offsets[i] on.  Steps of one optimizer follow one another:
     on several streams, order them.  (K. Jordan and others, "Muon: an optimizer
     for hidden layers in neural networks", 2024.)"""
 

@@ -5,7 +5,8 @@
  *   y = x x^T, z = a + b y + c y y, x = z x, some times; then w moves by x
  *
  * x is a matrix with its shorter side first, so that y and z are as small as
- * they can be; they are symmetric, and half of their tiles are computed.
+ * they can be; they are symmetric, and half of their tiles are computed, but for
+ * small matrices, of which all are.
  *
  * Products of 32-bit numbers come of three on the 16-bit matrix units: a
  * number is kept as a half and the half of what is left, 22 bits in all, and
