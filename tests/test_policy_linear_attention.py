@@ -660,3 +660,71 @@ def test_c_no_decay():
     assert backward(None, None) == 0 and backward(at, None) == 0
     g.steps, g.q, g.k, g.v = 1, at, at, at
     assert lib.b3_linear_attention_step_gpu(C.byref(g), at, at, None) == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("key,value", [(128, 128), (100, 96), (70, 40), (128, 70), (64, 128)])
+@pytest.mark.parametrize("steps,at", [(100, 45), (100, 32), (70, 69), (3000, 1500)])
+def test_a_bad_column(steps, at, key, value, type, bad):
+    """What is not finite in one column of v is in that column of out and of the
+    state alone, from its step to the end of its episode: also where waves that
+    share q and k have other columns, whichever of them finds it."""
+    from puffysics_amd import policy
+    q, k, v, _, _, state = made(steps, 2, 1, key, value, TYPES[type], 31)
+    decay = torch.tensor([0.95], device="cuda")
+    starts = torch.zeros(steps, 2, device="cuda")
+    after = min(at + 5, steps - 1)
+    starts[after, 0] = 1 if after > at else 0
+    want = policy.linear_attention(q, k, v, decay, state=state, starts=starts, last=True)
+    for col in (0, value // 2, value - 1):
+        u = v.clone()
+        u[at, :, 0, col] = bad
+        got = policy.linear_attention(q, k, u, decay, state=state, starts=starts, last=True)
+        seen = torch.zeros(v.shape, dtype=torch.bool, device="cuda")
+        seen[at:, 1, 0, col] = True
+        seen[at:after if after > at else steps, 0, 0, col] = True
+        assert not torch.isfinite(got.out[seen]).any() and torch.isfinite(got.out[~seen]).all()
+        clean = torch.where(seen, 0.0, got.out.float())
+        close(clean.to(v.dtype), torch.where(seen, 0.0, want.out.float()).double(), 2.0 ** -7 * want.out.float().abs().max(), v.dtype)
+        gone = torch.zeros(state.shape, dtype=torch.bool, device="cuda")
+        gone[1, 0, :, col] = True
+        gone[0, 0, :, col] = after == at
+        assert not torch.isfinite(got.state[gone]).any() and torch.isfinite(got.state[~gone]).all()
+        assert torch.allclose(got.state[~gone], want.state[~gone], rtol=1e-4, atol=1e-4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("size", [(70, 8, 2, 32, 32), (3000, 1, 1, 64, 64), (200, 2, 1, 128, 128)])
+def test_gradient_replays(size, type):
+    """A captured update, forwards and back, and a step of acting: every replay
+    is the eager result of what the buffers hold then, the first one's too, with
+    other work between."""
+    from puffysics_amd import policy
+    q, k, v, decay, starts, state = made(*size, TYPES[type], 14, rate=0.01)
+    d = torch.randn_like(v)
+    memory, twin = state.clone(), state.clone()
+
+    def once(memory, *xs):
+        leaves = [x.detach().requires_grad_() for x in xs]
+        got = policy.linear_attention(*leaves[:3], decay, state=leaves[3], starts=starts, last=True)
+        grads = torch.autograd.grad((got.out, got.state), leaves, (d, torch.ones_like(got.state)))
+        step = policy.linear_attention_step(*(x[0] for x in xs[:3]), decay, memory, starts=starts[0])
+        return [x.detach() for x in (got.out, got.state, *grads, step)]
+
+    once(state.clone(), q, k, v, state)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = once(memory, q, k, v, state)
+    for i in range(4):
+        graph.replay()
+        want = once(twin, *(x.clone() for x in (q, k, v, state)))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(memory, twin), i
+        q.mul_(0.5)
+        v.add_(0.25)
+        starts[i + 1] = ~starts[i + 1]
+        torch.cuda.synchronize()
