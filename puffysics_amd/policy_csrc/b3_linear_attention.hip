@@ -300,15 +300,17 @@ struct Unit {
  * decay^(i - j) of an episode, j <= i:
  *   out = P v + decay^i q E,  E' = decay^places E + (decay^(places - j) k)^T v
  * PART: some columns are filled up.  Tiles of 16 that all are, are left out of
- * products, which in 32 bits are most of the time: the backward pass of 333
- * steps of 57 x 3 with heads of 48 and 80 takes 118 us so, 150 without.  Where
- * none are, asking costs 2 to 10 % (heads of 64 and of 128).
- * 64 steps of 4,096 environments with 4 heads of 64 in bf16 take 185 us forward
- * (4.4 TB/s, vector units 33 % busy, matrix units 9) and 395 back (3.1 TB/s, 41
- * and 12), two histories of 65,536 steps and 8 heads of 128 151 us for the
- * pieces' states and 358 for all (3.1 TB/s, 52 and 27): what bounds it is that
+ * products, which in 32 bits are most of the time: 333 steps of 57 x 3 with heads
+ * of 48 and 80 take 56 us forward and 98 back so, 70 and 140 without.  Where none
+ * are, asking costs 2 to 7 % (fp32 and fp16 heads of 64 and of 128).
+ * 64 steps of 4,096 environments with 4 heads of 64 in bf16 take 186 us forward
+ * (4.3 TB/s, vector units 35 % busy, matrix units 10) and 402 back (3.0 TB/s, 43
+ * and 13), two histories of 65,536 steps and 8 heads of 128 152 us for the
+ * pieces' states and 367 for all (3.0 TB/s, 56 and 29): what bounds it is that
  * the registers hold but two waves of a SIMD, which wait for each other's
- * instructions more than for memory. */
+ * instructions more than for memory.  The same 64 steps, call after call, with the
+ * last state, no episodes and none to enter with: bf16 222 and 310, fp16 262 and
+ * 546, fp32 306 and 597, whose products bound them. */
 template <typename T, int KD, int VD, int W, bool STATE, bool PART>
 struct Walk {
     typedef typename Math<T>::Lds Lds;
@@ -959,8 +961,8 @@ Mix backwards(const B3Attention& g, const float* d_last) {
 }
 
 int columns_of(int dims) { return dims <= 32 ? 32 : dims <= 64 ? 64 : 128; }
-/* The state is at most 64 of a lane's registers, so that two waves fit a SIMD: one reads two histories of
- * 65,536 steps and 8 heads of 128 in 783 us with 128, two in 380 with 64. */
+/* The state is at most 64 of a lane's registers, so that two waves fit a SIMD: two histories of 65,536 steps
+ * and 8 heads of 128 are read in 491 us (and 1,230 back), 1,475 (4,310) with 128. */
 int part_of(int key, int value) { return value <= 32 || key > 64 ? 32 : 64; }
 int places_of(int type) { return type == B3_BF16 ? 32 : 16; }
 
@@ -986,7 +988,13 @@ double rounds(int64_t waves) {
  * this took in brackets: bf16, heads of 64, 1,024 steps of 256 sequences 108,
  * 91, [62], 66, 91; 256 steps of them [29], 32, 33, 41, -; 4,096 of 64 sequences
  * 414, 320, 171, 97, [66], in 32 pieces 70; back, 12 pieces 139, 128 in 8, [119]
- * in 16; of 256 sequences of 1,024 steps [108], 119, 119, 141, 196. */
+ * in 16; of 256 sequences of 1,024 steps [108], 119, 119, 141, 196.  It holds for
+ * other types and heads as well: of 26 such rows of all types, with heads of
+ * 32, 64 and 128, what it took was within 6 % of the best, but for bf16 heads of
+ * 32 back (256 sequences of 1,024 steps [66], 69, 58, 64, 77).  fp32, heads of 64,
+ * 1,024 steps of 256 sequences 243, 192, [120], 119, 143; fp16 249, 195, [119], 112,
+ * 128; bf16, heads of 128, whose parts wait for each other, [113], 123, 164, 204,
+ * 302, of 64 sequences of 4,096 413, 314, 182, [143], 164. */
 double time_of(const B3Attention& g, const Plan& p, int64_t units, int64_t pieces, bool backward) {
     const double chunks = (double)ceil_div(ceil_div(g.steps, pieces), places_of(g.type)), chunk = p.key == 32 ? 1.8 : 3.5;
     const double walk = chunks * chunk * rounds(units * pieces);
@@ -1041,8 +1049,8 @@ hipError_t launch_walk(const Job& j, hipStream_t stream) {
     typedef Walk<T, KD, VD, W, STATE, PART> Walker;
     constexpr int kLds = 64 << 10, kMost = kLds / Walker::kBytes, kGroups = W > 1 ? 1 : kMost >= 4 ? 4 : 1;
     static_assert(kMost >= 1, "a workgroup's tiles");
-    /* (workgroups of two would leave SIMDs empty: 32-bit heads of 128, two histories of 2,048 steps, take 84 us so, 67
-     * one wave each; 1,000 environments of 512 steps 1,690 and 1,807) */
+    /* (workgroups of two would leave SIMDs empty: 32-bit heads of 128, two histories of 2,048 steps, take 88 us so, 72
+     * one wave each; 1,000 environments of 512 steps 3,355 and 3,340) */
     const int64_t units = j.envs * j.heads * (STATE ? j.pieces - 1 : j.pieces) * j.roles * (W > 1 ? 1 : j.parts);
     la_walk<T, KD, VD, W, STATE, PART><<<(unsigned)ceil_div(units, kGroups), kGroups * W * kWave, kGroups * Walker::kBytes, stream>>>(j);
     return hipGetLastError();
@@ -1058,10 +1066,10 @@ hipError_t launch(const Job& j, hipStream_t stream) {
 template <typename T, bool STATE>
 hipError_t launch_columns(const Job& j, const Plan& p, hipStream_t stream) {
     if (p.key == 128) {
-        /* In 16 bits parts share what they fetch: two histories of 65,536 steps and 8 heads of 128 take 370 us
-         * so, 435 each for itself.  In 32 the products take most of the time, and waves had better not wait for
-         * each other: the backward pass of 333 steps of 57 x 3 with heads of 48 and 80 took 154 us, 240 shared, with
-         * all tiles. */
+        /* In 16 bits parts share what they fetch: two histories of 65,536 steps and 8 heads of 128 take 491 us (1,230
+         * back) so, 600 (1,550) each for itself.  In 32 the products take most of the time, and waves had better not
+         * wait for each other: the backward pass of 333 steps of 57 x 3 with heads of 48 and 80 takes 98 us, 148 shared
+         * (2,048 of two histories with 8 heads of 128, whose parts are all alike, 155 and 150). */
         if constexpr (__is_same(T, __bf16)) {
             if (p.parts > 2) return launch<T, 128, 32, 4, STATE>(j, stream);
             if (p.parts > 1) return launch<T, 128, 32, 2, STATE>(j, stream);
