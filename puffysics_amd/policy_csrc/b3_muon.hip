@@ -22,11 +22,14 @@
  * p x after kGroup of them.  That is 3 m m n + (4 kGroup - 3) m^3 multiplications
  * rather than kGroup (3 m m n + m^3), half tiles taken for half.  y is then formed
  * anew from x, because its rounding, some 2^-22 of its norm, grows by up to
- * 3.4445^2 a step where y is all but 0: after 3 steps x is as exact as by products
- * of 32 bits, after 5 it was off by 1e-3 of its norm for gradients of two strong
- * directions over others of a tenth, 512 x 1,024, where it is by 3e-6 (by 1e-2 and
- * 5e-5 for those two alone).  The 16 matrices of 2,048 x 512 and 512 x 2,048 of a
- * network's step pay for it with 116 of 1,022 us.
+ * 3.4445^2 a step where y is all but 0: after 3 steps x is about as exact as by
+ * products of 32 bits, after 5 it was off by 1e-3 of its norm for gradients of two
+ * strong directions over others of a tenth, 512 x 1,024, where it is by 3e-6 (by
+ * 1e-2 and 5e-5 for those two alone).  The 16 matrices of 2,048 x 512 and 512 x
+ * 2,048 of a network's step pay for it with 116 of 1,022 us.  The rounding of many
+ * rows is spread over as many directions; of few rows it is not, and x of one
+ * tile's rows takes all its steps as above: 5 x 510 of that kind is off by 1.3e-6
+ * so and was by 5e-5.
  *
  * A launch computes a product of all matrices, or those that need not wait for
  * each other, a workgroup to a tile of 128 x 128.  Matrices lie in blocks of 32
@@ -56,13 +59,12 @@ constexpr int64_t kPart = 4096;                  // its elements at the least
 constexpr double kA = 3.4445, kB = -4.7750, kC = 2.0315;
 constexpr float kScale = 8192.0f, kCollected = 1024.0f;    // of x, y and z, and of p, whose singular values reach 3.4445^kGroup
 constexpr int kGroup = 3;
-/* x that is twice as long as wide, and so much longer, takes its steps on the
- * short side, for launches more.  So or not, us a step: 16 matrices of 256 x 512
- * 268 and 246, of 256 x 640 276 and 264, of 512 x 768 439 and 425, of 512 x 896 450
- * and 446, of 512 x 1,024 465 and 473, of 512 x 2,048 610 and 762, of 128 x 384 172
- * and 167, of 128 x 512 179 and 186; 4 of 1,024 x 1,408 665 and 653, of 1,024 x
- * 2,048 704 and 752, of 2,048 x 2,560 2,836 and 2,794, of 2,048 x 4,096 3,320 and
- * 3,958. */
+/* x of more than a tile's rows that is twice as long as wide, and so much longer,
+ * takes its steps on the short side, for launches more.  So or not, us a step: 16
+ * matrices of 256 x 512 268 and 246, of 256 x 640 276 and 264, of 512 x 768 439
+ * and 425, of 512 x 896 450 and 446, of 512 x 1,024 465 and 473, of 512 x 2,048 610
+ * and 762; 4 of 1,024 x 1,408 665 and 653, of 1,024 x 2,048 704 and 752, of 2,048 x
+ * 2,560 2,836 and 2,794, of 2,048 x 4,096 3,320 and 3,958. */
 constexpr int64_t kLonger = 3 * kTile;
 constexpr int kSmallSide = 64, kSmallLength = 256, kSmallThreads = 512;
 constexpr int kSmallTiles = kSmallSide / 16 * kSmallLength / 16 / (kSmallThreads / kWave);      // of a wave
@@ -918,7 +920,7 @@ hipError_t b3_muon_create(B3Muon** out, const B3MuonMatrix* matrices, int count,
             }
             t.m = filled(m);
             t.n = filled(numel / m);
-            t.is_long = t.n >= 2 * t.m && t.n >= t.m + kLonger;
+            t.is_long = t.m > kTile && t.n >= 2 * t.m && t.n >= t.m + kLonger;
             int64_t* const squares[5] = {&t.y, &t.z, &t.between, &t.collected[0], &t.collected[1]};
             t.x = work;
             t.next = t.x + t.m * t.n;

@@ -339,3 +339,23 @@ def test_weights_move_as_exactly(type):
             off[i] += rate * near_32_bits(u, x) + 2.0 ** -22 * float(w[i].norm())
             got = params[i] if dtype == torch.float32 else views(opt, opt.master())[i]
             assert far(got, w[i]) <= off[i], (g.shape, t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("steps", [3, 5, 6, 8])
+@pytest.mark.parametrize("shape", [(5, 510), (510, 5), (17, 1000), (60, 510), (100, 1000), (128, 700), (200, 1000), (513, 2048)])
+@pytest.mark.parametrize("kind", ["all rows", "five rows"])
+def test_as_exact_of_weak_directions(shape, kind, steps):
+    """Two strong directions over others of a tenth, in all rows or in a few."""
+    from puffysics_amd import policy
+    g = torch.Generator().manual_seed(shape[0] + steps)
+    some = lambda r: torch.randn(r, 2, generator=g) @ torch.randn(2, shape[1], generator=g) + 0.1 * torch.randn(r, shape[1], generator=g)  # noqa: E731
+    u = some(shape[0])
+    if kind == "five rows":
+        u = 1e-2 * torch.randn(shape, generator=g)
+        u[:5] = some(min(5, shape[0]))
+    u = u.cuda()
+    param = torch.zeros(shape, device="cuda")
+    policy.Muon([param], math.sqrt(min(1.0, shape[1] / shape[0])), momentum=0.0, newton_schulz=steps).step([u])
+    want = -orthogonalised_oracle(u, steps)
+    assert far(param, want) <= near_32_bits(-u, want, steps)
