@@ -303,10 +303,10 @@ struct Unit {
  * products, which in 32 bits are most of the time: 333 steps of 57 x 3 with heads
  * of 48 and 80 take 56 us forward and 98 back so, 70 and 140 without.  Where none
  * are, asking costs 2 to 7 % (fp32 and fp16 heads of 64 and of 128).
- * 64 steps of 4,096 environments with 4 heads of 64 in bf16 take 186 us forward
+ * 64 steps of 4,096 environments with 4 heads of 64 in bf16 take 190 us forward
  * (4.3 TB/s, vector units 35 % busy, matrix units 10) and 402 back (3.0 TB/s, 43
  * and 13), two histories of 65,536 steps and 8 heads of 128 152 us for the
- * pieces' states and 367 for all (3.0 TB/s, 56 and 29): what bounds it is that
+ * pieces' states and 361 for all (3.1 TB/s, 56 and 29): what bounds it is that
  * the registers hold but two waves of a SIMD, which wait for each other's
  * instructions more than for memory.  The same 64 steps, call after call, with the
  * last state, no episodes and none to enter with: bf16 222 and 310, fp16 262 and

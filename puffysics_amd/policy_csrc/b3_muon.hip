@@ -240,7 +240,7 @@ __device__ __forceinline__ double momentum_part(const T* grad, float* momentum, 
 }
 
 /* The momentum, and a part's sum of squares of u.  Memory bounds it: 12 matrices
- * of 2,048 and 8,192 in fp32 211 us, 5.7 TB/s. */
+ * of 2,048 and 8,192 in fp32 210 us, 5.8 TB/s. */
 __global__ __launch_bounds__(kThreads) void mu_momentum(GradientLaunch l) {
     const Place p = l.c.places[l.c.first + blockIdx.x];
     const Matrix& t = l.c.matrices[p.matrix];
@@ -428,11 +428,11 @@ __device__ __forceinline__ int in_row(int row, int k) { return row / 2 * 256 + (
 /* Four waves, each with 64 x 64 of the tile.  A step of 32 of what is summed
  * is fetched into registers while the two before are worked on, since one takes
  * less time than memory does, and goes to the other half of LDS.  z of 12
- * matrices of 2,048 and 8,192 takes 355 us, 926 TFLOP/s of 16-bit products (a
- * large library product reaches 1,111), z of 50 matrices of 512 wide 38 us, 630
+ * matrices of 2,048 and 8,192 takes 356 us, 923 TFLOP/s of 16-bit products (a
+ * large library product reaches 1,111), z of 50 matrices of 512 wide 39 us, 620
  * TFLOP/s: of 16 steps the beginnings and ends of tiles take the most, and what
- * a launch reads and writes (131 MB, 3.4 TB/s).  The last product, with the
- * weights, takes 1,240 and 151 us (3.3 TB/s). */
+ * a launch reads and writes (130 MB, 3.3 TB/s).  The last product, with the
+ * weights, takes 1,233 and 151 us (3.3 TB/s). */
 template <Product KIND>
 __device__ __forceinline__ void product(const ProductLaunch& l, const Place& p, bool collect) {
     constexpr bool kAcross = KIND == NEXT || KIND == LAST;      // the right side's rows are what is summed over
@@ -629,8 +629,8 @@ __global__ __launch_bounds__(kThreads, 2) void mu_product(ProductLaunch l) {
 
 /* z y and z p of long matrices, as the launch has them, and z x of others, whose
  * places follow: neither needs the other, and together they fill the device
- * better.  Of 50 matrices of 512 wide 324 + 512 tiles take 61 us, 33 + 35 in two
- * launches, of 12 of 2,048 and 8,192 1,088 + 2,048 tiles 641, 257 + 408. */
+ * better.  Of 50 matrices of 512 wide 320 + 520 tiles take 61 us, 33 + 35 in two
+ * launches, of 12 of 2,048 and 8,192 1,088 + 2,048 tiles 634, 257 + 408. */
 __global__ __launch_bounds__(kThreads, 2) void mu_products(ProductLaunch l, int formed) {
     const int64_t i = l.before + by_die(), middles = l.middles * formed;
     if (i < middles) product<MIDDLE>(l, l.c.places[l.c.first + i % l.middles], l.middle + i / l.middles == 1);
